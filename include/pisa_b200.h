@@ -338,6 +338,115 @@ PISA_API int pisa_rotary(const void *x, int64_t x_sb, int64_t x_st, int64_t x_sh
                          int64_t position_offset, const float *frequency, int dtype, int64_t B, int64_t T,
                          int64_t H, int64_t D, pisa_stream_t stream);
 
+/* ---- full attention (layers beside the sparse ones; no counterpart in the reference's CUDA path) ---- */
+
+/*
+ * Norm of every query and key head and the split-half position rotation in
+ * one pass.  With u = x / sqrt(mean(x^2) + eps) over a head's D elements,
+ * y = u * weight and the angle a_i = position * frequency_i (one fp32
+ * product): out_i = y_i cos a_i - y_{i+D/2} sin a_i,
+ * out_{i+D/2} = y_i sin a_i + y_{i+D/2} cos a_i.  Held in fp32, rounded once.
+ * q: [B,T,Hq,D], k: [B,T,H,D] (element strides); weights: D elements each of
+ * `weight_dtype` (PISA_F32 or `dtype`); frequency: D/2 fp32; positions as
+ * pisa_rotary.  q_out [B,T,Hq,D] and k_out [B,T,H,D] are contiguous.
+ * Constraints: D % 8 == 0, D <= 256.
+ */
+PISA_API int pisa_qk_norm_rotary(const void *q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void *k, int64_t k_sb,
+                                 int64_t k_st, int64_t k_sh, const void *q_weight, const void *k_weight,
+                                 int weight_dtype, const float *frequency, const int64_t *positions,
+                                 int64_t positions_sb, int64_t position_offset, int dtype, int64_t B, int64_t T,
+                                 int64_t Hq, int64_t H, int64_t D, float eps, void *q_out, void *k_out,
+                                 pisa_stream_t stream);
+
+/*
+ * Backward of pisa_qk_norm_rotary: dq [B,T,Hq,D] and dk [B,T,H,D] (contiguous)
+ * from dq_out and dk_out (contiguous, shapes of q_out and k_out), and the
+ * weights' gradients (D elements each, `weight_dtype`), summed over all rows
+ * in a fixed order.  workspace: pisa_qk_norm_rotary_bwd_workspace_bytes(...).
+ */
+PISA_API int pisa_qk_norm_rotary_bwd(const void *q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void *k,
+                                     int64_t k_sb, int64_t k_st, int64_t k_sh, const void *dq_out,
+                                     const void *dk_out, const void *q_weight, const void *k_weight,
+                                     int weight_dtype, const float *frequency, const int64_t *positions,
+                                     int64_t positions_sb, int64_t position_offset, int dtype, int64_t B, int64_t T,
+                                     int64_t Hq, int64_t H, int64_t D, float eps, void *dq, void *dk,
+                                     void *dq_weight, void *dk_weight, void *workspace, int64_t workspace_bytes,
+                                     pisa_stream_t stream);
+
+PISA_API int64_t pisa_qk_norm_rotary_bwd_workspace_bytes(int64_t B, int64_t T, int64_t D);
+
+/*
+ * Attention of every query over the keys of its sequence, forward.
+ * q: [B,Tq,Hq,D], k: [B,N,H,D], v: [B,N,H,Dv] (element strides), Hq = G*H.
+ * Without cumulative lengths (both NULL) every batch row is one sequence
+ * whose query i sits at position query_offset + i; a causal query sees keys up
+ * to its position (0 <= query_offset <= N - Tq).  With them (B = 1) sequence s
+ * holds queries cu_seqlens_q[s] .. cu_seqlens_q[s+1] and keys cu_seqlens_k[s]
+ * .. cu_seqlens_k[s+1] (`sequences` + 1 device integers of cu_bytes 4 or 8,
+ * nondecreasing from 0; read on the device, so the call does not wait for
+ * them) and its queries are its last positions: causal query i sees keys
+ * 0 .. k_len - q_len + i.  Sequences may be empty; rows past the last
+ * sequence are rows without keys.  Entries outside that contract give
+ * undefined results but no access outside the tensors.
+ * out: [B,Tq,Hq,Dv] contiguous; lse: [B,Tq,Hq] fp32 natural log-sum-exp of
+ *   the scaled logits, or NULL.  A query without a visible key gets 0 / -inf.
+ * scale > 0.  D, Dv multiples of 8, at most 256.
+ * workspace: NULL, or pisa_full_attn_fwd_workspace_bytes(...) bytes whose
+ *   first 4 receive the device status word; rows of a tile whose wait expired
+ *   are NaN in either case.
+ */
+PISA_API int pisa_full_attn_fwd(const void *q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void *k, int64_t k_sb,
+                                int64_t k_st, int64_t k_sh, const void *v, int64_t v_sb, int64_t v_st, int64_t v_sh,
+                                const void *cu_seqlens_q, const void *cu_seqlens_k, int cu_bytes, int64_t sequences,
+                                int64_t query_offset, int dtype, int64_t B, int64_t Tq, int64_t Hq, int64_t H,
+                                int64_t D, int64_t Dv, int64_t N, float scale, int causal, void *out, float *lse,
+                                void *workspace, int64_t workspace_bytes, pisa_stream_t stream);
+
+/* sequences: 0 without cumulative lengths. */
+PISA_API int64_t pisa_full_attn_fwd_workspace_bytes(int64_t B, int64_t Tq, int64_t Hq, int64_t H, int64_t D, int64_t Dv,
+                                                    int64_t N, int64_t sequences, int dtype);
+
+/*
+ * Backward of pisa_full_attn_fwd: dq [B,Tq,Hq,D], dk [B,N,H,D], dv [B,N,H,Dv]
+ * in dtype, contiguous, every element written (rows outside all sequences:
+ * zero).  out, dout: contiguous [B,Tq,Hq,Dv]; lse as written by the forward.
+ * Sums run in a fixed order: equal inputs give equal bits.
+ * workspace: pisa_full_attn_bwd_workspace_bytes(...) bytes, status word first.
+ */
+PISA_API int pisa_full_attn_bwd(const void *q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void *k, int64_t k_sb,
+                                int64_t k_st, int64_t k_sh, const void *v, int64_t v_sb, int64_t v_st, int64_t v_sh,
+                                const void *out, const void *dout, const float *lse, const void *cu_seqlens_q,
+                                const void *cu_seqlens_k, int cu_bytes, int64_t sequences, int64_t query_offset,
+                                int dtype, int64_t B, int64_t Tq, int64_t Hq, int64_t H, int64_t D, int64_t Dv,
+                                int64_t N, float scale, int causal, void *dq, void *dk, void *dv, void *workspace,
+                                int64_t workspace_bytes, pisa_stream_t stream);
+
+PISA_API int64_t pisa_full_attn_bwd_workspace_bytes(int64_t B, int64_t Tq, int64_t Hq, int64_t H, int64_t D, int64_t Dv,
+                                                    int64_t N, int64_t sequences, int dtype);
+
+/*
+ * Decode attention of a step's Tq newest tokens of B sequences over a prefix
+ * that all of them share and each one's own cache, one softmax over both.
+ * q: [B,Tq,Hq,D]; k, v: own caches [B,capacity,H,D|Dv] (element strides) of
+ * which the first lengths[b] keys are valid, this step's Tq included (device
+ * integers of length_bytes 4 or 8, clamped to [0, capacity]); prefix_k,
+ * prefix_v: [prefix,H,D|Dv] (element strides), or NULL with prefix 0.  Token t
+ * sees the whole prefix and own keys 0 .. lengths[b] - Tq + t.
+ * out: [B,Tq,Hq,Dv] contiguous; lse: [B,Tq,Hq] fp32 or NULL; without a
+ * visible key 0 / -inf.  scale > 0; D, Dv multiples of 8, at most 256.
+ * workspace: pisa_prefix_attn_workspace_bytes(...) bytes.
+ */
+PISA_API int pisa_prefix_attn(const void *q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void *k, int64_t k_sb,
+                              int64_t k_st, int64_t k_sh, const void *v, int64_t v_sb, int64_t v_st, int64_t v_sh,
+                              const void *lengths, int length_bytes, const void *prefix_k, int64_t pk_st,
+                              int64_t pk_sh, const void *prefix_v, int64_t pv_st, int64_t pv_sh, int dtype, int64_t B,
+                              int64_t Tq, int64_t Hq, int64_t H, int64_t D, int64_t Dv, int64_t capacity,
+                              int64_t prefix, float scale, void *out, float *lse, void *workspace,
+                              int64_t workspace_bytes, pisa_stream_t stream);
+
+PISA_API int64_t pisa_prefix_attn_workspace_bytes(int64_t B, int64_t Tq, int64_t Hq, int64_t H, int64_t D, int64_t Dv,
+                                                  int64_t capacity, int64_t prefix, int dtype);
+
 /* ---- device status (no counterpart in the reference, whose Triton kernels never wait) ----
  * Every kernel that waits on another part of the GPU waits a bounded number
  * of tries.  A wait that expires records PISA_ERR_TIMEOUT in the 4-byte

@@ -11,7 +11,9 @@ TensorCache).  All computation runs in the hand-written CUDA library
 
 from .attention import sparse_attention, sparse_attn_fn
 from .cache import PyramidCache, TensorCache
+from .dense import full_attention, prefix_attention
 from ._lib import set_status_checks
+from .norm_rotary import qk_norm_rotary
 from .selection import (bsa_fn, build_pyramid, decode_select_attend, grouped_leaf_scores, mean_pool,
                         routing_geometry, select_blocks, top_k_pyramid_fn)
 
@@ -21,4 +23,5 @@ __all__ = [
     "select_blocks", "top_k_pyramid_fn", "sparse_attention", "sparse_attn_fn", "mean_pool",
     "mean_pooling_fn", "build_pyramid", "routing_geometry", "PyramidCache", "TensorCache",
     "grouped_leaf_scores", "set_status_checks", "decode_select_attend", "bsa_fn",
+    "full_attention", "prefix_attention", "qk_norm_rotary",
 ]

@@ -59,6 +59,20 @@ SIGNATURES = {
                              _L, _I, _L, _P, _P, _L, _P]),
     "pisa_bsa_workspace_bytes": (_L, [_L, _L, _L, _L, _I, _L, _I]),
     "pisa_rotary": (_I, [_P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _P, _I, _L, _L, _L, _L, _P]),
+    "pisa_qk_norm_rotary": (_I, [_P, _L, _L, _L, _P, _L, _L, _L, _P, _P, _I, _P, _P, _L, _L, _I, _L, _L, _L, _L, _L,
+                                 _F, _P, _P, _P]),
+    "pisa_qk_norm_rotary_bwd": (_I, [_P, _L, _L, _L, _P, _L, _L, _L, _P, _P, _P, _P, _I, _P, _P, _L, _L, _I, _L, _L,
+                                     _L, _L, _L, _F, _P, _P, _P, _P, _P, _L, _P]),
+    "pisa_qk_norm_rotary_bwd_workspace_bytes": (_L, [_L, _L, _L]),
+    "pisa_full_attn_fwd": (_I, [_P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _P, _P, _I, _L, _L, _I, _L, _L, _L,
+                                _L, _L, _L, _L, _F, _I, _P, _P, _P, _L, _P]),
+    "pisa_full_attn_fwd_workspace_bytes": (_L, [_L, _L, _L, _L, _L, _L, _L, _L, _I]),
+    "pisa_full_attn_bwd": (_I, [_P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _P, _P, _P, _P, _P, _I, _L, _L, _I,
+                                _L, _L, _L, _L, _L, _L, _L, _F, _I, _P, _P, _P, _P, _L, _P]),
+    "pisa_full_attn_bwd_workspace_bytes": (_L, [_L, _L, _L, _L, _L, _L, _L, _L, _I]),
+    "pisa_prefix_attn": (_I, [_P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _P, _I, _P, _L, _L, _P, _L, _L, _I, _L,
+                              _L, _L, _L, _L, _L, _L, _L, _F, _P, _P, _P, _L, _P]),
+    "pisa_prefix_attn_workspace_bytes": (_L, [_L, _L, _L, _L, _L, _L, _L, _L, _I]),
     "pisa_workspace_status": (_I, [_P, _P]),
     "pisa_wait_selftest": (_I, [_I, _L, _P, _L, _P]),
     "pisa_ex2_selftest": (_I, [_P, _P, _P, _L, _P]),

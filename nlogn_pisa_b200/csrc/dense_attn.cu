@@ -1,0 +1,431 @@
+// Attention of every query over all keys of its sequence (causal or not), and
+// its gradient, on the FMA pipes: fp32 tensors, and 16-bit heads wider than
+// 128, which the tensor-core kernels do not hold.
+//
+// With s_ij = scale q_i . k_j over the keys that query i sees,
+//   l_i = sum_j exp(s_ij - m_i),  out_i = sum_j exp(s_ij - m_i) v_j / l_i,
+//   lse_i = m_i + ln l_i   (no visible key: out_i = 0, lse_i = -inf).
+// Backward, with P = exp(s - lse), delta_i = dout_i . out_i and
+// dS = scale P (dout v - delta):
+//   dq = dS k,   dk = dS^T q,   dv = P^T dout   (dk, dv summed over the G
+// query heads of a KV head).  Forward and dq walk the key tiles of a query
+// tile, dk / dv walk the query tiles of a key tile: no atomics, so results do
+// not vary from run to run.
+//
+// Bound by FP32 FMAs.  Tiles of R*16 x R*16 scores, a thread computes R x R
+// of them from shared memory rows padded by 16 bytes (the 8 rows that a
+// quarter of a warp reads then fall in different banks) and R rows x DP/16
+// columns of each output.  Rows outside the sequence are staged as zeros and
+// products with hidden keys are skipped, not multiplied by zero, so
+// infinities and NaN in hidden places reach nothing.
+#include "dense_attn.cuh"
+
+namespace pisa {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+// rows x DP tile of `src` (row stride `stride` elements) into fp32 shared
+// memory, zero past `valid` rows and past D columns
+template <typename T, int DP, int LD>
+__device__ __forceinline__ void stage(float* dst, const T* src, int64_t stride, int rows, int valid, int D) {
+  constexpr int VN = Vec<T>::N, SEG = DP / VN;
+  for (int i = threadIdx.x; i < rows * SEG; i += kThreads) {
+    const int r = i / SEG, c = (i - r * SEG) * VN;
+    float v[VN];
+#pragma unroll
+    for (int e = 0; e < VN; ++e) v[e] = 0.f;
+    if (r < valid && c < D) load_vec<T>(src + r * stride + c, v);
+#pragma unroll
+    for (int e = 0; e < VN; e += 4)
+      *reinterpret_cast<float4*>(dst + r * LD + c + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+  }
+}
+
+// acc[i][j] += a row (ty*R + i) . b row (tx + 16 j)
+template <int R, int DP, int LD>
+__device__ __forceinline__ void rows_dot(const float* a, const float* b, int ty, int tx, float (&acc)[R][R]) {
+#pragma unroll 4
+  for (int d = 0; d < DP; d += 4) {
+    float4 x[R], y[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) x[i] = *reinterpret_cast<const float4*>(a + (ty * R + i) * LD + d);
+#pragma unroll
+    for (int j = 0; j < R; ++j) y[j] = *reinterpret_cast<const float4*>(b + (tx + 16 * j) * LD + d);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        acc[i][j] = fmaf(x[i].x, y[j].x, acc[i][j]);
+        acc[i][j] = fmaf(x[i].y, y[j].y, acc[i][j]);
+        acc[i][j] = fmaf(x[i].z, y[j].z, acc[i][j]);
+        acc[i][j] = fmaf(x[i].w, y[j].w, acc[i][j]);
+      }
+    }
+  }
+}
+
+// acc[i][c] += sum_j w[ty*R + i][j] x[j][columns of tx]; a weight outside
+// [lo[i], hi[i]] is skipped when `partial`.  Columns of tx: 4 from tx*4 + 64 c.
+template <int R, int DP, int LD, int LP>
+__device__ __forceinline__ void rows_sum(const float* w, const float* x, int count, int ty, int tx, bool partial,
+                                         const int (&lo)[R], const int (&hi)[R], float (&acc)[R][DP / 16]) {
+  for (int j = 0; j < count; ++j) {
+    float p[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) p[i] = w[(ty * R + i) * LP + j];
+#pragma unroll
+    for (int c = 0; c < DP / 64; ++c) {
+      const float4 y = *reinterpret_cast<const float4*>(x + j * LD + tx * 4 + 64 * c);
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        if (partial && (j < lo[i] || j > hi[i])) continue;
+        acc[i][4 * c + 0] = fmaf(p[i], y.x, acc[i][4 * c + 0]);
+        acc[i][4 * c + 1] = fmaf(p[i], y.y, acc[i][4 * c + 1]);
+        acc[i][4 * c + 2] = fmaf(p[i], y.z, acc[i][4 * c + 2]);
+        acc[i][4 * c + 3] = fmaf(p[i], y.w, acc[i][4 * c + 3]);
+      }
+    }
+  }
+}
+
+template <int DP> struct Tile {
+  static constexpr int R = DP <= 128 ? 4 : 2;   // 256 dims: tiles of 32 keep four of them in shared memory
+  static constexpr int BT = R * 16, LD = DP + 4, LP = BT + 1;
+};
+
+template <typename T, int R, int DP>
+__device__ __forceinline__ void store_rows(T* dst, int64_t stride, int valid, int D, int ty, int tx,
+                                           const float (&acc)[R][DP / 16], const float (&mul)[R]) {
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int r = ty * R + i;
+    if (r >= valid) continue;
+#pragma unroll
+    for (int c = 0; c < DP / 64; ++c) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = tx * 4 + 64 * c + e;
+        if (d < D) dst[r * stride + d] = from_f32<T>(acc[i][4 * c + e] * mul[i]);
+      }
+    }
+  }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) dense_fwd_kernel(const __grid_constant__ DenseAttnArgs a) {
+  using S = Tile<DP>;
+  constexpr int R = S::R, BT = S::BT, LD = S::LD, LP = S::LP;
+  extern __shared__ __align__(16) float smem[];
+  float* qs = smem;
+  float* ks = qs + BT * LD;
+  float* vs = ks + BT * LD;
+  float* ps = vs + BT * LD;
+  // later query tiles, which see more keys, first
+  const int index = int(gridDim.x) - 1 - int(blockIdx.x);
+  const int slot = index / a.Hq, hq = index - slot * a.Hq, h = hq / a.G;
+  const SeqTile t = seq_tile(a, slot, BT, false);
+  const int q0 = t.tile * BT;
+  if (q0 >= t.q_len) return;
+  const int valid = min(BT, t.q_len - q0);
+  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  const T* qp = static_cast<const T*>(a.q) + t.b * a.q_sb + int64_t(t.q_begin + q0) * a.q_st + hq * a.q_sh;
+  const T* kp = static_cast<const T*>(a.k) + t.b * a.k_sb + int64_t(t.k_begin) * a.k_st + h * a.k_sh;
+  const T* vp = static_cast<const T*>(a.v) + t.b * a.v_sb + int64_t(t.k_begin) * a.v_st + h * a.v_sh;
+  stage<T, DP, LD>(qs, qp, a.q_st, BT, valid, a.D);
+  const float sl = a.scale * kLog2e;
+  float acc[R][DP / 16], m[R], l[R];
+  int last[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+    last[i] = last_visible(a, t, q0 + ty * R + i);
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) acc[i][c] = 0.f;
+  }
+  const int end = last_visible(a, t, q0 + valid - 1) + 1, full = last_visible(a, t, q0) + 1;
+  for (int j0 = 0; j0 < end; j0 += BT) {
+    __syncthreads();
+    const int nk = min(BT, t.k_len - j0);
+    stage<T, DP, LD>(ks, kp + int64_t(j0) * a.k_st, a.k_st, BT, nk, a.D);
+    stage<T, DP, LD>(vs, vp + int64_t(j0) * a.v_st, a.v_st, BT, nk, a.Dv);
+    __syncthreads();
+    float s[R][R] = {};
+    rows_dot<R, DP, LD>(qs, ks, ty, tx, s);
+    float corr[R];
+    int lo[R], hi[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      float top = m[i];
+      lo[i] = 0;
+      hi[i] = last[i] - j0;
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        s[i][j] = tx + 16 * j <= hi[i] ? s[i][j] * sl : -INFINITY;
+        top = fmaxf(top, s[i][j]);
+      }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
+      const float base = top == -INFINITY ? 0.f : top;
+      corr[i] = exp2f(m[i] - base);
+      m[i] = top;
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        const float p = exp2f(s[i][j] - base);
+        ps[(ty * R + i) * LP + tx + 16 * j] = p;
+        sum += p;
+      }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+      l[i] = l[i] * corr[i] + sum;
+#pragma unroll
+      for (int c = 0; c < DP / 16; ++c) acc[i][c] *= corr[i];
+    }
+    __syncwarp();   // the rows of ps that a warp reads are its own
+    rows_sum<R, DP, LD, LP>(ps, vs, min(nk, end - j0), ty, tx, j0 + BT > full, lo, hi, acc);
+  }
+  float inv[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    inv[i] = l[i] == 0.f ? 0.f : 1.f / l[i];
+    const int r = ty * R + i;
+    if (a.lse && tx == 0 && r < valid)
+      a.lse[(int64_t(t.b) * a.T + t.q_begin + q0 + r) * a.Hq + hq] =
+          l[i] == 0.f ? -INFINITY : (m[i] + log2f(l[i])) * kLn2;
+  }
+  T* op = static_cast<T*>(a.out) + ((int64_t(t.b) * a.T + t.q_begin + q0) * a.Hq + hq) * a.Dv;
+  store_rows<T, R, DP>(op, int64_t(a.Hq) * a.Dv, valid, a.Dv, ty, tx, acc, inv);
+}
+
+// delta = dout . out per row, one warp per row
+template <typename T>
+__global__ void __launch_bounds__(128) dense_delta_kernel(const T* __restrict__ dout, const T* __restrict__ out,
+                                                          float* __restrict__ delta, int64_t rows, int Dv) {
+  constexpr int VN = Vec<T>::N;
+  const int64_t r = blockIdx.x * int64_t(4) + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (r >= rows) return;
+  float acc = 0.f;
+  for (int d = lane * VN; d < Dv; d += 32 * VN) {
+    float x[VN], y[VN];
+    load_vec<T>(dout + r * Dv + d, x);
+    load_vec<T>(out + r * Dv + d, y);
+#pragma unroll
+    for (int e = 0; e < VN; ++e) acc = fmaf(x[e], y[e], acc);
+  }
+  acc = warp_sum(acc);
+  if (lane == 0) delta[r] = acc;
+}
+
+// Base-2 lse of a row for the recomputed weights; a row without weight (lse
+// -inf) gets +inf, which makes them all zero.
+__device__ __forceinline__ float lse_base2(float lse) { return lse == -INFINITY ? INFINITY : lse * kLog2e; }
+
+// P and dS of one score element: base-2 logit minus base-2 lse
+__device__ __forceinline__ float2 prob_grad(float s, float dp, float sl, float lse2, float delta, float scale,
+                                            bool visible) {
+  const float p = visible ? exp2f(fmaf(s, sl, -lse2)) : 0.f;
+  return make_float2(p, visible ? scale * p * (dp - delta) : 0.f);
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) dense_dq_kernel(const __grid_constant__ DenseAttnArgs a) {
+  using S = Tile<DP>;
+  constexpr int R = S::R, BT = S::BT, LD = S::LD, LP = S::LP;
+  extern __shared__ __align__(16) float smem[];
+  float* qs = smem;
+  float* os = qs + BT * LD;
+  float* ks = os + BT * LD;
+  float* vs = ks + BT * LD;
+  float* ds = vs + BT * LD;
+  const int index = int(gridDim.x) - 1 - int(blockIdx.x);
+  const int slot = index / a.Hq, hq = index - slot * a.Hq, h = hq / a.G;
+  const SeqTile t = seq_tile(a, slot, BT, false);
+  const int q0 = t.tile * BT;
+  if (q0 >= t.q_len) return;
+  const int valid = min(BT, t.q_len - q0);
+  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  const int64_t row0 = (int64_t(t.b) * a.T + t.q_begin + q0) * a.Hq + hq;
+  const T* kp = static_cast<const T*>(a.k) + t.b * a.k_sb + int64_t(t.k_begin) * a.k_st + h * a.k_sh;
+  const T* vp = static_cast<const T*>(a.v) + t.b * a.v_sb + int64_t(t.k_begin) * a.v_st + h * a.v_sh;
+  stage<T, DP, LD>(qs, static_cast<const T*>(a.q) + t.b * a.q_sb + int64_t(t.q_begin + q0) * a.q_st + hq * a.q_sh,
+                   a.q_st, BT, valid, a.D);
+  stage<T, DP, LD>(os, static_cast<const T*>(a.dout) + row0 * a.Dv, int64_t(a.Hq) * a.Dv, BT, valid, a.Dv);
+  const float sl = a.scale * kLog2e;
+  float acc[R][DP / 16], lse2[R], delta[R];
+  int last[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int r = ty * R + i;
+    last[i] = r < valid ? last_visible(a, t, q0 + r) : -1;
+    lse2[i] = r < valid ? lse_base2(a.lse_in[row0 + int64_t(r) * a.Hq]) : 0.f;
+    delta[i] = r < valid ? a.delta[row0 + int64_t(r) * a.Hq] : 0.f;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) acc[i][c] = 0.f;
+  }
+  const int end = last_visible(a, t, q0 + valid - 1) + 1, full = last_visible(a, t, q0) + 1;
+  for (int j0 = 0; j0 < end; j0 += BT) {
+    __syncthreads();
+    const int nk = min(BT, t.k_len - j0);
+    stage<T, DP, LD>(ks, kp + int64_t(j0) * a.k_st, a.k_st, BT, nk, a.D);
+    stage<T, DP, LD>(vs, vp + int64_t(j0) * a.v_st, a.v_st, BT, nk, a.Dv);
+    __syncthreads();
+    float s[R][R] = {}, dp[R][R] = {};
+    rows_dot<R, DP, LD>(qs, ks, ty, tx, s);
+    rows_dot<R, DP, LD>(os, vs, ty, tx, dp);
+    int lo[R], hi[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      lo[i] = 0;
+      hi[i] = last[i] - j0;
+#pragma unroll
+      for (int j = 0; j < R; ++j)
+        ds[(ty * R + i) * LP + tx + 16 * j] =
+            prob_grad(s[i][j], dp[i][j], sl, lse2[i], delta[i], a.scale, tx + 16 * j <= hi[i]).y;
+    }
+    __syncwarp();
+    rows_sum<R, DP, LD, LP>(ds, ks, min(nk, end - j0), ty, tx, j0 + BT > full || valid < BT, lo, hi, acc);
+  }
+  float one[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) one[i] = 1.f;
+  store_rows<T, R, DP>(static_cast<T*>(a.dq) + row0 * a.D, int64_t(a.Hq) * a.D, valid, a.D, ty, tx, acc, one);
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) dense_dkv_kernel(const __grid_constant__ DenseAttnArgs a) {
+  using S = Tile<DP>;
+  constexpr int R = S::R, BT = S::BT, LD = S::LD, LP = S::LP;
+  extern __shared__ __align__(16) float smem[];
+  float* ks = smem;
+  float* vs = ks + BT * LD;
+  float* qs = vs + BT * LD;
+  float* os = qs + BT * LD;
+  float* ps = os + BT * LD;      // P^T: key rows, query columns
+  float* ds = ps + BT * LP;      // dS^T
+  __shared__ float lse_s[64], delta_s[64];
+  const int slot = int(blockIdx.x) / a.H, h = int(blockIdx.x) - slot * a.H;   // early keys, seen by most queries, first
+  const SeqTile t = seq_tile(a, slot, BT, true);
+  const int j0 = t.tile * BT;
+  if (j0 >= t.k_len) return;
+  const int valid = min(BT, t.k_len - j0);
+  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  stage<T, DP, LD>(ks, static_cast<const T*>(a.k) + t.b * a.k_sb + int64_t(t.k_begin + j0) * a.k_st + h * a.k_sh,
+                   a.k_st, BT, valid, a.D);
+  stage<T, DP, LD>(vs, static_cast<const T*>(a.v) + t.b * a.v_sb + int64_t(t.k_begin + j0) * a.v_st + h * a.v_sh,
+                   a.v_st, BT, valid, a.Dv);
+  const float sl = a.scale * kLog2e;
+  float dk[R][DP / 16], dv[R][DP / 16];
+  int first[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int r = ty * R + i;
+    first[i] = r < valid ? first_seeing(a, t, j0 + r) : t.q_len;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) dk[i][c] = dv[i][c] = 0.f;
+  }
+  const int begin = first_seeing(a, t, j0) / BT * BT, full = first_seeing(a, t, j0 + valid - 1);
+  for (int g = 0; g < a.G; ++g) {
+    const int hq = h * a.G + g;
+    for (int q0 = begin; q0 < t.q_len; q0 += BT) {
+      const int nq = min(BT, t.q_len - q0);
+      const int64_t row0 = (int64_t(t.b) * a.T + t.q_begin + q0) * a.Hq + hq;
+      __syncthreads();
+      stage<T, DP, LD>(qs, static_cast<const T*>(a.q) + t.b * a.q_sb + int64_t(t.q_begin + q0) * a.q_st + hq * a.q_sh,
+                       a.q_st, BT, nq, a.D);
+      stage<T, DP, LD>(os, static_cast<const T*>(a.dout) + row0 * a.Dv, int64_t(a.Hq) * a.Dv, BT, nq, a.Dv);
+      if (threadIdx.x < BT) {
+        const bool real = int(threadIdx.x) < nq;
+        lse_s[threadIdx.x] = real ? lse_base2(a.lse_in[row0 + int64_t(threadIdx.x) * a.Hq]) : 0.f;
+        delta_s[threadIdx.x] = real ? a.delta[row0 + int64_t(threadIdx.x) * a.Hq] : 0.f;
+      }
+      __syncthreads();
+      float s[R][R] = {}, dp[R][R] = {};
+      rows_dot<R, DP, LD>(ks, qs, ty, tx, s);
+      rows_dot<R, DP, LD>(vs, os, ty, tx, dp);
+      int lo[R], hi[R];
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        lo[i] = first[i] - q0;
+        hi[i] = nq - 1;
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+          const int c = tx + 16 * j;
+          const float2 pg = prob_grad(s[i][j], dp[i][j], sl, lse_s[c], delta_s[c], a.scale, c >= lo[i] && c <= hi[i]);
+          ps[(ty * R + i) * LP + c] = pg.x;
+          ds[(ty * R + i) * LP + c] = pg.y;
+        }
+      }
+      __syncwarp();
+      const bool partial = q0 < full || valid < BT;
+      rows_sum<R, DP, LD, LP>(ps, os, nq, ty, tx, partial, lo, hi, dv);
+      rows_sum<R, DP, LD, LP>(ds, qs, nq, ty, tx, partial, lo, hi, dk);
+    }
+  }
+  float one[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) one[i] = 1.f;
+  const int64_t row0 = (int64_t(t.b) * a.N + t.k_begin + j0) * a.H + h;
+  store_rows<T, R, DP>(static_cast<T*>(a.dk) + row0 * a.D, int64_t(a.H) * a.D, valid, a.D, ty, tx, dk, one);
+  store_rows<T, R, DP>(static_cast<T*>(a.dv) + row0 * a.Dv, int64_t(a.H) * a.Dv, valid, a.Dv, ty, tx, dv, one);
+}
+
+template <typename K>
+int launch(K kernel, int64_t blocks, size_t smem, const DenseAttnArgs& a, cudaStream_t s) {
+  if (blocks >= (int64_t(1) << 31)) return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+  if (e != cudaSuccess) return fail_cuda(e, "dense attention smem attribute");
+  kernel<<<unsigned(blocks), kThreads, smem, s>>>(a);
+  PISA_CHECK_LAUNCH();
+  return PISA_OK;
+}
+
+template <typename T, int DP>
+int fwd_t(const DenseAttnArgs& a, cudaStream_t s) {
+  using L = Tile<DP>;
+  const int64_t slots = seq_slots(a.cu_q, a.B, a.T, a.sequences, L::BT);
+  return launch(dense_fwd_kernel<T, DP>, slots * a.Hq, sizeof(float) * L::BT * (3 * L::LD + L::LP), a, s);
+}
+
+template <typename T, int DP>
+int bwd_t(const DenseAttnArgs& a, cudaStream_t s) {
+  using L = Tile<DP>;
+  const int64_t rows = int64_t(a.B) * a.T * a.Hq;
+  if ((rows + 3) / 4 >= (int64_t(1) << 31)) return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
+  dense_delta_kernel<T><<<unsigned((rows + 3) / 4), 128, 0, s>>>(static_cast<const T*>(a.dout),
+                                                                 static_cast<const T*>(a.o), a.delta, rows, a.Dv);
+  PISA_CHECK_LAUNCH();
+  int rc = launch(dense_dq_kernel<T, DP>, seq_slots(a.cu_q, a.B, a.T, a.sequences, L::BT) * a.Hq,
+                  sizeof(float) * L::BT * (4 * L::LD + L::LP), a, s);
+  if (rc) return rc;
+  return launch(dense_dkv_kernel<T, DP>, seq_slots(a.cu_q, a.B, a.N, a.sequences, L::BT) * a.H,
+                sizeof(float) * L::BT * (4 * L::LD + 2 * L::LP), a, s);
+}
+
+template <typename T>
+int by_dim(const DenseAttnArgs& a, bool bwd, cudaStream_t s) {
+  const int d = a.D > a.Dv ? a.D : a.Dv;
+  if (d <= 64) return bwd ? bwd_t<T, 64>(a, s) : fwd_t<T, 64>(a, s);
+  if (d <= 128) return bwd ? bwd_t<T, 128>(a, s) : fwd_t<T, 128>(a, s);
+  return bwd ? bwd_t<T, 256>(a, s) : fwd_t<T, 256>(a, s);
+}
+
+int by_type(const DenseAttnArgs& a, int dtype, bool bwd, cudaStream_t s) {
+  if (dtype == PISA_F32) return by_dim<float>(a, bwd, s);
+  if (dtype == PISA_BF16) return by_dim<__nv_bfloat16>(a, bwd, s);
+  return by_dim<__half>(a, bwd, s);
+}
+
+}  // namespace
+
+int dense_attn_fwd_simt(const DenseAttnArgs& a, int dtype, cudaStream_t stream) {
+  return by_type(a, dtype, false, stream);
+}
+int dense_attn_bwd_simt(const DenseAttnArgs& a, int dtype, cudaStream_t stream) {
+  return by_type(a, dtype, true, stream);
+}
+
+}  // namespace pisa

@@ -1,0 +1,133 @@
+// Shared declarations of the dense (full) attention kernels: the operands,
+// and the mapping from a grid slot to a tile of one sequence.
+#pragma once
+
+#include "internal.h"
+
+namespace pisa {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+struct DenseAttnArgs {
+  const void* q;
+  int64_t q_sb, q_st, q_sh;
+  const void* k;
+  int64_t k_sb, k_st, k_sh;
+  const void* v;
+  int64_t v_sb, v_st, v_sh;
+  // packed sequences (B = 1): cumulative lengths of the queries and of the
+  // keys, `sequences` + 1 entries of cu_bytes each; null: every batch row is
+  // one sequence whose first query sits at position query_offset
+  const void* cu_q;
+  const void* cu_k;
+  int cu_bytes, sequences;
+  int64_t query_offset;
+  int B, T, N, Hq, H, G, D, Dv;
+  float scale;
+  int causal;
+  void* out;        // [B, T, Hq, Dv]
+  float* lse;       // [B, T, Hq] or null
+  int* status;      // device status word or null
+  // backward
+  const void* o;    // the forward's output, contiguous
+  const void* dout; // contiguous
+  const float* lse_in;
+  float* delta;     // [B, T, Hq] row dot products of dout and out
+  void* dq;
+  void* dk;
+  void* dv;
+};
+
+// Tile `tile` of one sequence.  Queries q_begin .. q_begin + q_len and keys
+// k_begin .. k_begin + k_len of batch row b; query i sits at position
+// shift + i, key j at position j.
+struct SeqTile {
+  int b, tile, q_begin, q_len, k_begin, k_len;
+  int64_t shift;
+};
+
+__device__ __forceinline__ int cu_at(const void* cu, int bytes, int i, int most) {
+  const int64_t v = bytes == 4 ? int64_t(static_cast<const int32_t*>(cu)[i]) : static_cast<const int64_t*>(cu)[i];
+  return int(v < 0 ? 0 : v > most ? most : v);
+}
+
+// First row of sequence s; s == sequences stands for the rows after the last
+// sequence, which no key (or no query) meets.
+__device__ __forceinline__ int seq_begin(const DenseAttnArgs& a, const void* cu, int most, int s) {
+  return s == 0 ? 0 : cu_at(cu, a.cu_bytes, s, most);
+}
+__device__ __forceinline__ int seq_end(const DenseAttnArgs& a, const void* cu, int most, int s, int begin) {
+  return s >= a.sequences ? most : max(begin, cu_at(cu, a.cu_bytes, s + 1, most));
+}
+
+// Packed sequences need no table of tiles: sequence s owns the slots from
+// floor(begin_s / rows) + s, of which there are at least ceil(len_s / rows)
+// before the next sequence's, so a binary search over the cumulative lengths
+// finds a slot's sequence.  Entries that are not in order leave rows without
+// a slot but never lead outside the tensors (every value is clamped, and the
+// search keeps base(lo) <= slot).
+__host__ __device__ __forceinline__ int64_t seq_slots(bool packed, int64_t batch, int64_t total, int64_t sequences,
+                                                      int64_t rows) {
+  return packed ? total / rows + sequences + 1 : batch * ((total + rows - 1) / rows);
+}
+
+__device__ __forceinline__ SeqTile seq_tile(const DenseAttnArgs& a, int slot, int rows, bool by_keys) {
+  SeqTile t;
+  const int total = by_keys ? a.N : a.T;
+  if (a.cu_q == nullptr) {
+    t.tile = slot / a.B;   // equal tiles of all batch rows side by side
+    t.b = slot - t.tile * a.B;
+    t.q_begin = t.k_begin = 0;
+    t.q_len = a.T;
+    t.k_len = a.N;
+    t.shift = a.query_offset;
+    return t;
+  }
+  const void* cu = by_keys ? a.cu_k : a.cu_q;
+  int lo = 0, hi = a.sequences;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (seq_begin(a, cu, total, mid) / rows + mid <= slot) lo = mid;
+    else hi = mid - 1;
+  }
+  t.b = 0;
+  t.q_begin = seq_begin(a, a.cu_q, a.T, lo);
+  t.k_begin = seq_begin(a, a.cu_k, a.N, lo);
+  t.q_len = seq_end(a, a.cu_q, a.T, lo, t.q_begin) - t.q_begin;
+  t.k_len = seq_end(a, a.cu_k, a.N, lo, t.k_begin) - t.k_begin;
+  t.tile = slot - ((by_keys ? t.k_begin : t.q_begin) / rows + lo);
+  if (lo >= a.sequences) {
+    if (by_keys) t.q_len = 0;
+    else t.k_len = 0;
+  }
+  t.shift = int64_t(t.k_len) - t.q_len;
+  return t;
+}
+
+// Keys that query i of the tile's sequence sees: 0 .. last (-1: none).
+__device__ __forceinline__ int last_visible(const DenseAttnArgs& a, const SeqTile& t, int i) {
+  const int64_t last = a.causal ? min64(t.shift + i, int64_t(t.k_len) - 1) : int64_t(t.k_len) - 1;
+  return last < -1 ? -1 : int(last);
+}
+
+// First query of the sequence that sees key j (q_len: none).
+__device__ __forceinline__ int first_seeing(const DenseAttnArgs& a, const SeqTile& t, int j) {
+  if (!a.causal) return 0;
+  const int64_t first = int64_t(j) - t.shift;
+  return int(first < 0 ? 0 : first > t.q_len ? t.q_len : first);
+}
+
+// make_tensor_map with a box of `rows` tokens of one head; strides of
+// dimensions of one element, which may hold anything, are replaced.
+inline int dense_tensor_map(CUtensorMap* map, const void* base, int dtype, int64_t B, int64_t T, int64_t H, int64_t D,
+                            int64_t sb, int64_t st, int64_t sh, uint32_t rows) {
+  if (H == 1) sh = D;
+  if (T == 1) st = H * sh;
+  return make_tensor_map(map, base, dtype, B, T, H, D, sb, st, sh, 1, rows);
+}
+
+int dense_attn_fwd_simt(const DenseAttnArgs& a, int dtype, cudaStream_t stream);
+int dense_attn_bwd_simt(const DenseAttnArgs& a, int dtype, cudaStream_t stream);
+
+}  // namespace pisa

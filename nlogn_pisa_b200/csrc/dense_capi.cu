@@ -1,0 +1,210 @@
+// C entry points of dense attention (whole prompts, and decode over a shared
+// prefix): argument checks, workspace layout and the choice of kernel.
+#include <algorithm>
+#include <cmath>
+
+#include "dense_attn.cuh"
+#include "prefix_attn.cuh"
+
+namespace pisa {
+
+namespace {
+
+int64_t round256(int64_t x) { return (x + 255) / 256 * 256; }
+
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0)
+    return 148;
+  return n;
+}
+
+bool rows16(const void* p, int dtype, int64_t sb, int64_t st, int64_t sh) {
+  const int64_t v = dtype == PISA_F32 ? 4 : 8;
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && sb % v == 0 && st % v == 0 && sh % v == 0;
+}
+
+int check_common(int dtype, int64_t Hq, int64_t H, int64_t D, int64_t Dv, float scale) {
+  if (dtype < PISA_F32 || dtype > PISA_F16) return fail(PISA_ERR_UNSUPPORTED, "the kernels support FP16, BF16 and FP32");
+  if (Hq <= 0 || H <= 0 || D <= 0 || Dv <= 0) return fail(PISA_ERR_INVALID, "nonempty tensors are required");
+  if (Hq % H) return fail(PISA_ERR_INVALID, "a whole number of query heads per KV head is required");
+  if (D % 8 || Dv % 8 || D > 256 || Dv > 256)
+    return fail(PISA_ERR_UNSUPPORTED, "head_dim must be a multiple of 8 and at most 256");
+  if (!(scale > 0.f) || std::isinf(scale)) return fail(PISA_ERR_INVALID, "scale must be positive and finite");
+  return PISA_OK;
+}
+
+int check_dense(const DenseAttnArgs& a, int dtype, int64_t B, int64_t Tq, int64_t Hq, int64_t H, int64_t D, int64_t Dv,
+                int64_t N, int64_t sequences) {
+  if (int rc = check_common(dtype, Hq, H, D, Dv, a.scale)) return rc;
+  if (B <= 0 || Tq <= 0 || N <= 0) return fail(PISA_ERR_INVALID, "nonempty tensors are required");
+  constexpr int64_t most = (int64_t(1) << 31) - 1;
+  if (Tq > most - 4096 || N > most - 4096 || B > most || Hq > 65535 || sequences > most / 2 || B * Tq * Hq > most * 4)
+    return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
+  if (!a.q || !a.k || !a.v) return fail(PISA_ERR_INVALID, "q, k and v are required");
+  if (!rows16(a.q, dtype, a.q_sb, a.q_st, a.q_sh) || !rows16(a.k, dtype, a.k_sb, a.k_st, a.k_sh) ||
+      !rows16(a.v, dtype, a.v_sb, a.v_st, a.v_sh))
+    return fail(PISA_ERR_UNSUPPORTED, "q, k and v rows must be 16-byte aligned");
+  if (a.cu_q || a.cu_k) {
+    if (!a.cu_q || !a.cu_k || sequences < 1) return fail(PISA_ERR_INVALID, "cumulative lengths of queries and keys are required");
+    if (a.cu_bytes != 4 && a.cu_bytes != 8) return fail(PISA_ERR_INVALID, "cumulative lengths must be int32 or int64");
+    if (B != 1) return fail(PISA_ERR_INVALID, "packed inputs require batch size one");
+  } else if (a.causal && (a.query_offset < 0 || a.query_offset + Tq > N)) {
+    return fail(PISA_ERR_INVALID, "queries must refer to positions within their key sequence");
+  }
+  return PISA_OK;
+}
+
+struct PrefixPlan {
+  int64_t prefix_splits, own_splits, ml_off, o_off, total;
+};
+
+// Splits of the keys: enough CTAs for two per SM, but at least 256 keys each.
+PrefixPlan plan_prefix(int64_t B, int64_t T, int64_t Hq, int64_t H, int64_t Dv, int64_t cap, int64_t P) {
+  PrefixPlan p{};
+  const int64_t want = 2 * sm_count(), G = Hq / H;
+  auto splits = [&](int64_t keys, int64_t rows, int64_t groups) {
+    const int64_t items = groups * ((rows + 63) / 64);
+    return std::max<int64_t>(1, std::min((want + items - 1) / items, (keys + 255) / 256));
+  };
+  p.own_splits = splits(cap, T * G, B * H);
+  p.prefix_splits = P > 0 ? splits(P, B * T * G, H) : 0;
+  const int64_t slots = p.own_splits + p.prefix_splits, rows = B * T * Hq;
+  p.ml_off = 256;
+  p.o_off = p.ml_off + (slots > 1 ? round256(rows * slots * 8) : 0);
+  p.total = p.o_off + (slots > 1 ? rows * slots * Dv * 4 : 0);
+  return p;
+}
+
+}  // namespace
+
+}  // namespace pisa
+
+using namespace pisa;
+
+extern "C" {
+
+int64_t pisa_full_attn_fwd_workspace_bytes(int64_t B, int64_t Tq, int64_t Hq, int64_t H, int64_t D, int64_t Dv,
+                                           int64_t N, int64_t sequences, int dtype) {
+  if (B <= 0 || Tq <= 0 || Hq <= 0 || H <= 0 || D <= 0 || Dv <= 0 || N <= 0 || sequences < 0 || dtype < PISA_F32 ||
+      dtype > PISA_F16)
+    return -1;
+  return 256;
+}
+
+int pisa_full_attn_fwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb,
+                       int64_t k_st, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_st, int64_t v_sh,
+                       const void* cu_seqlens_q, const void* cu_seqlens_k, int cu_bytes, int64_t sequences,
+                       int64_t query_offset, int dtype, int64_t B, int64_t Tq, int64_t Hq, int64_t H, int64_t D,
+                       int64_t Dv, int64_t N, float scale, int causal, void* out, float* lse, void* workspace,
+                       int64_t workspace_bytes, pisa_stream_t stream) {
+  DenseAttnArgs a{};
+  a.q = q; a.q_sb = q_sb; a.q_st = q_st; a.q_sh = q_sh;
+  a.k = k; a.k_sb = k_sb; a.k_st = k_st; a.k_sh = k_sh;
+  a.v = v; a.v_sb = v_sb; a.v_st = v_st; a.v_sh = v_sh;
+  a.cu_q = cu_seqlens_q; a.cu_k = cu_seqlens_k; a.cu_bytes = cu_bytes;
+  a.query_offset = query_offset; a.scale = scale; a.causal = causal ? 1 : 0;
+  if (int rc = check_dense(a, dtype, B, Tq, Hq, H, D, Dv, N, sequences)) return rc;
+  if (!out) return fail(PISA_ERR_INVALID, "out is required");
+  a.sequences = int(sequences);
+  a.B = int(B); a.T = int(Tq); a.N = int(N); a.Hq = int(Hq); a.H = int(H); a.G = int(Hq / H);
+  a.D = int(D); a.Dv = int(Dv);
+  a.out = out; a.lse = lse;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (workspace) {
+    if (workspace_bytes < 256) return fail(PISA_ERR_INVALID, "workspace too small");
+    cudaError_t e = cudaMemsetAsync(workspace, 0, 256, s);
+    if (e != cudaSuccess) return fail_cuda(e, "status clear");
+    a.status = static_cast<int*>(workspace);
+  }
+  return dense_attn_fwd_simt(a, dtype, s);
+}
+
+int64_t pisa_full_attn_bwd_workspace_bytes(int64_t B, int64_t Tq, int64_t Hq, int64_t H, int64_t D, int64_t Dv,
+                                           int64_t N, int64_t sequences, int dtype) {
+  if (B <= 0 || Tq <= 0 || Hq <= 0 || H <= 0 || D <= 0 || Dv <= 0 || N <= 0 || sequences < 0 || dtype < PISA_F32 ||
+      dtype > PISA_F16)
+    return -1;
+  return 256 + B * Tq * Hq * 4;
+}
+
+int pisa_full_attn_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb,
+                       int64_t k_st, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_st, int64_t v_sh,
+                       const void* out, const void* dout, const float* lse, const void* cu_seqlens_q,
+                       const void* cu_seqlens_k, int cu_bytes, int64_t sequences, int64_t query_offset, int dtype,
+                       int64_t B, int64_t Tq, int64_t Hq, int64_t H, int64_t D, int64_t Dv, int64_t N, float scale,
+                       int causal, void* dq, void* dk, void* dv, void* workspace, int64_t workspace_bytes,
+                       pisa_stream_t stream) {
+  DenseAttnArgs a{};
+  a.q = q; a.q_sb = q_sb; a.q_st = q_st; a.q_sh = q_sh;
+  a.k = k; a.k_sb = k_sb; a.k_st = k_st; a.k_sh = k_sh;
+  a.v = v; a.v_sb = v_sb; a.v_st = v_st; a.v_sh = v_sh;
+  a.cu_q = cu_seqlens_q; a.cu_k = cu_seqlens_k; a.cu_bytes = cu_bytes;
+  a.query_offset = query_offset; a.scale = scale; a.causal = causal ? 1 : 0;
+  if (int rc = check_dense(a, dtype, B, Tq, Hq, H, D, Dv, N, sequences)) return rc;
+  if (!out || !dout || !lse || !dq || !dk || !dv) return fail(PISA_ERR_INVALID, "out, dout, lse and the gradients are required");
+  if (!rows16(out, dtype, 0, 0, 0) || !rows16(dout, dtype, 0, 0, 0))
+    return fail(PISA_ERR_UNSUPPORTED, "out and dout must be 16-byte aligned");
+  a.sequences = int(sequences);
+  a.B = int(B); a.T = int(Tq); a.N = int(N); a.Hq = int(Hq); a.H = int(H); a.G = int(Hq / H);
+  a.D = int(D); a.Dv = int(Dv);
+  a.o = out; a.dout = dout; a.lse_in = lse; a.dq = dq; a.dk = dk; a.dv = dv;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (!workspace ||
+      workspace_bytes < pisa_full_attn_bwd_workspace_bytes(B, Tq, Hq, H, D, Dv, N, cu_seqlens_q ? sequences : 0, dtype))
+    return fail(PISA_ERR_INVALID, "workspace too small");
+  cudaError_t e = cudaMemsetAsync(workspace, 0, 256, s);
+  if (e != cudaSuccess) return fail_cuda(e, "status clear");
+  a.status = static_cast<int*>(workspace);
+  a.delta = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
+  return dense_attn_bwd_simt(a, dtype, s);
+}
+
+int64_t pisa_prefix_attn_workspace_bytes(int64_t B, int64_t Tq, int64_t Hq, int64_t H, int64_t D, int64_t Dv,
+                                         int64_t capacity, int64_t prefix, int dtype) {
+  if (B <= 0 || Tq <= 0 || Hq <= 0 || H <= 0 || Hq % H || D <= 0 || Dv <= 0 || capacity <= 0 || prefix < 0 ||
+      dtype < PISA_F32 || dtype > PISA_F16)
+    return -1;
+  return plan_prefix(B, Tq, Hq, H, Dv, capacity, prefix).total;
+}
+
+int pisa_prefix_attn(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb, int64_t k_st,
+                     int64_t k_sh, const void* v, int64_t v_sb, int64_t v_st, int64_t v_sh, const void* lengths,
+                     int length_bytes, const void* prefix_k, int64_t pk_st, int64_t pk_sh, const void* prefix_v,
+                     int64_t pv_st, int64_t pv_sh, int dtype, int64_t B, int64_t Tq, int64_t Hq, int64_t H, int64_t D,
+                     int64_t Dv, int64_t capacity, int64_t prefix, float scale, void* out, float* lse, void* workspace,
+                     int64_t workspace_bytes, pisa_stream_t stream) {
+  if (int rc = check_common(dtype, Hq, H, D, Dv, scale)) return rc;
+  if (B <= 0 || Tq <= 0 || capacity <= 0 || prefix < 0) return fail(PISA_ERR_INVALID, "nonempty tensors are required");
+  if (!q || !k || !v || !lengths || !out) return fail(PISA_ERR_INVALID, "q, k, v, lengths and out are required");
+  if (prefix > 0 && (!prefix_k || !prefix_v)) return fail(PISA_ERR_INVALID, "prefix keys and values are required");
+  if (length_bytes != 4 && length_bytes != 8) return fail(PISA_ERR_INVALID, "lengths must be int32 or int64");
+  constexpr int64_t most = (int64_t(1) << 31) - 4097;
+  if (capacity > most || prefix > most || B * H > 65535 || B * Tq * (Hq / H) > 65535 * 16 || B * Tq * Hq > most)
+    return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
+  if (!rows16(q, dtype, q_sb, q_st, q_sh) || !rows16(k, dtype, k_sb, k_st, k_sh) || !rows16(v, dtype, v_sb, v_st, v_sh) ||
+      (prefix > 0 && (!rows16(prefix_k, dtype, 0, pk_st, pk_sh) || !rows16(prefix_v, dtype, 0, pv_st, pv_sh))))
+    return fail(PISA_ERR_UNSUPPORTED, "q, k and v rows must be 16-byte aligned");
+  const PrefixPlan plan = plan_prefix(B, Tq, Hq, H, Dv, capacity, prefix);
+  if (!workspace || workspace_bytes < plan.total) return fail(PISA_ERR_INVALID, "workspace too small");
+  char* ws = static_cast<char*>(workspace);
+  PrefixArgs a{};
+  a.q = q; a.q_sb = q_sb; a.q_st = q_st; a.q_sh = q_sh;
+  a.k = k; a.k_sb = k_sb; a.k_st = k_st; a.k_sh = k_sh;
+  a.v = v; a.v_sb = v_sb; a.v_st = v_st; a.v_sh = v_sh;
+  a.lengths = lengths; a.len_bytes = length_bytes;
+  a.pk = prefix_k; a.pk_st = pk_st; a.pk_sh = pk_sh;
+  a.pv = prefix_v; a.pv_st = pv_st; a.pv_sh = pv_sh;
+  a.B = int(B); a.T = int(Tq); a.Hq = int(Hq); a.H = int(H); a.G = int(Hq / H); a.D = int(D); a.Dv = int(Dv);
+  a.cap = int(capacity); a.P = int(prefix);
+  a.scale = scale; a.out = out; a.lse = lse;
+  a.prefix_splits = int(plan.prefix_splits); a.own_splits = int(plan.own_splits);
+  a.part_ml = reinterpret_cast<float2*>(ws + plan.ml_off);
+  a.part_o = reinterpret_cast<float*>(ws + plan.o_off);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (int rc = prefix_attn_simt(a, dtype, s)) return rc;
+  return a.prefix_splits + a.own_splits > 1 ? prefix_combine(a, dtype, s) : PISA_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,50 @@
+// Shared declarations of the decode attention over a shared prefix and each
+// sequence's own cache.
+#pragma once
+
+#include "dense_attn.cuh"
+
+namespace pisa {
+
+struct PrefixArgs {
+  const void* q;                 // [B, T, Hq, D]
+  int64_t q_sb, q_st, q_sh;
+  const void* k;                 // own caches [B, cap, H, D]
+  int64_t k_sb, k_st, k_sh;
+  const void* v;
+  int64_t v_sb, v_st, v_sh;
+  const void* lengths;           // [B] valid own keys, this step's T included
+  int len_bytes;
+  const void* pk;                // prefix [P, H, D]
+  int64_t pk_st, pk_sh;
+  const void* pv;
+  int64_t pv_st, pv_sh;
+  int B, T, Hq, H, G, D, Dv, cap, P;
+  float scale;
+  void* out;                     // [B, T, Hq, Dv]
+  float* lse;                    // [B, T, Hq] or null
+  // partial results of every (query row, slot): prefix splits first, then own
+  // splits; with one slot in all the kernels write `out` directly
+  int prefix_splits, own_splits;
+  float* part_o;                 // [rows][slots][Dv], sum_j 2^(s_j - m) v_j
+  float2* part_ml;               // [rows][slots], (m, l) with base-2 logits
+  int* status;
+};
+
+__device__ __forceinline__ int own_length(const PrefixArgs& a, int b) {
+  const int64_t n = a.len_bytes == 4 ? int64_t(static_cast<const int32_t*>(a.lengths)[b])
+                                     : static_cast<const int64_t*>(a.lengths)[b];
+  return int(n < 0 ? 0 : n > a.cap ? a.cap : n);
+}
+
+// Keys of split `i` of `n`: [begin, end), whole multiples of `unit` keys.
+__device__ __forceinline__ void split_range(int keys, int i, int n, int unit, int& begin, int& end) {
+  const int units = (keys + unit - 1) / unit, per = (units + n - 1) / n;
+  begin = min(keys, i * per * unit);
+  end = min(keys, (i + 1) * per * unit);
+}
+
+int prefix_attn_simt(const PrefixArgs& a, int dtype, cudaStream_t stream);
+int prefix_combine(const PrefixArgs& a, int dtype, cudaStream_t stream);
+
+}  // namespace pisa
