@@ -127,6 +127,10 @@ inline int dense_tensor_map(CUtensorMap* map, const void* base, int dtype, int64
   return make_tensor_map(map, base, dtype, B, T, H, D, sb, st, sh, 1, rows);
 }
 
+// 16-bit tensors of at most 128 dims: tensor-core kernels
+bool dense_attn_tc_eligible(const DenseAttnArgs& a, int dtype);
+int dense_attn_fwd_tc(const DenseAttnArgs& a, int dtype, cudaStream_t stream);
+
 int dense_attn_fwd_simt(const DenseAttnArgs& a, int dtype, cudaStream_t stream);
 int dense_attn_bwd_simt(const DenseAttnArgs& a, int dtype, cudaStream_t stream);
 

@@ -1,0 +1,435 @@
+// Dense attention forward on the tensor cores: 16-bit tensors, heads of at
+// most 128 dims (formulas in dense_attn.cu).
+//
+// One CTA holds two tiles of 128 consecutive queries of one head and walks
+// the keys of their sequence in tiles of 128:
+//   MMA 1  S = Q K^T   (M = 128 queries, N = 128 keys)  -> TMEM
+//   softmax in registers, a thread per query row (no shuffles); P rounded to
+//          the input type overwrites S in TMEM
+//   MMA 2  O += P V    (A = P from TMEM, B = V with keys along K) -> TMEM
+// The two query tiles take turns: while four warps turn tile 0's scores into
+// weights, the tensor core works for tile 1.  Warps 0-3 and 4-7 are the two
+// tiles' softmax warps, warp 8 issues the MMAs, warp 9 the TMA loads (a ring
+// of key and value tiles).  TMEM: S/P of both tiles and O of both fill 512
+// columns at 128 dims.
+//
+// The running maximum only moves when a row's new maximum passes the one in
+// use by 2^8: weights up to 256 are as exact in 16-bit floating point as
+// weights up to 1, and O in TMEM is rescaled a few times per row instead of
+// once per key tile.  P is rounded to the input type because the second MMA
+// takes its operands so; sums of weights are taken before that rounding, in
+// fp32.
+//
+// Hidden keys of a tile weigh zero, but zero times an infinite or NaN value
+// is NaN.  A row whose output holds NaN although its weights do not is
+// therefore summed again over its visible keys alone (row_again); rows past
+// the sequence's end need nothing (they are not stored).
+#include <type_traits>
+
+#include "dense_attn.cuh"
+#include "tc.cuh"
+
+namespace pisa {
+
+namespace {
+
+constexpr int kRows = 128;                  // queries of a tile, keys of a tile
+constexpr int kMmaWarp = 8, kLoadWarp = 9;
+constexpr int kThreads = 320;
+constexpr float kRescale = 8.f;             // base-2 growth of a row maximum that moves it
+
+struct FwdTcArgs {
+  CUtensorMap tm_q, tm_k, tm_v;             // boxes of 64 dims x 128 rows of one head
+  DenseAttnArgs d;
+  int bf16;
+};
+
+template <int DP> struct FwdTile {
+  static constexpr int CH = DP / 64;                    // 64-dim chunks
+  static constexpr int BYTES = kRows * DP * 2;          // one operand tile
+  static constexpr int STAGES = DP == 128 ? 4 : 6;      // 64 dims: also keeps a second CTA off the SM's TMEM
+  static constexpr int SMEM = (2 + STAGES) * BYTES + 1024;
+};
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+  } else {
+    __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
+}
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+      :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+         "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+         "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+         "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t x0, uint32_t x1, uint32_t x2, uint32_t x3) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" :: "r"(addr), "r"(x0), "r"(x1), "r"(x2), "r"(x3) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// Largest of 64 values by four chains of three-input maxima.
+__device__ __forceinline__ float max_of(const float (&v)[64]) {
+  float m[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m[i] = v[i];
+#pragma unroll
+  for (int i = 4; i < 60; i += 8) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) m[c] = tc::max3f(m[c], v[i + 2 * c], v[i + 2 * c + 1]);
+  }
+  return fmaxf(tc::max3f(m[0], v[60], v[61]), fmaxf(tc::max3f(m[1], v[62], v[63]), fmaxf(m[2], m[3])));
+}
+
+// Output row of query `i` summed over its visible keys alone, by one warp,
+// with the row's maximum m and weight sum l (base 2): acc[e] of column
+// lane + 32 e.  Stops once every column is NaN.
+template <typename T, int DP>
+__device__ __noinline__ void row_again(const DenseAttnArgs& a, const SeqTile& t, int hq, int i, float m, float l,
+                                       float (&acc)[DP / 32]) {
+  const int lane = threadIdx.x & 31, h = hq / a.G;
+  const T* qp = static_cast<const T*>(a.q) + t.b * a.q_sb + int64_t(t.q_begin + i) * a.q_st + hq * a.q_sh;
+  const T* kp = static_cast<const T*>(a.k) + t.b * a.k_sb + int64_t(t.k_begin) * a.k_st + h * a.k_sh;
+  const T* vp = static_cast<const T*>(a.v) + t.b * a.v_sb + int64_t(t.k_begin) * a.v_st + h * a.v_sh;
+  const float sl = a.scale * kLog2e;
+  float q[DP / 32];
+#pragma unroll
+  for (int e = 0; e < DP / 32; ++e) {
+    q[e] = lane + 32 * e < a.D ? to_f32<T>(qp[lane + 32 * e]) : 0.f;
+    acc[e] = 0.f;
+  }
+  const int last = last_visible(a, t, i);
+  for (int j = 0; j <= last; ++j) {
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < DP / 32; ++e)
+      if (lane + 32 * e < a.D) s = fmaf(q[e], to_f32<T>(kp[j * a.k_st + lane + 32 * e]), s);
+    const float p = exp2f(fmaf(warp_sum(s), sl, -m));
+    bool all = true;
+#pragma unroll
+    for (int e = 0; e < DP / 32; ++e) {
+      if (lane + 32 * e < a.Dv) {
+        acc[e] = fmaf(p, to_f32<T>(vp[j * a.v_st + lane + 32 * e]), acc[e]);
+        all = all && isnan(acc[e]);
+      }
+    }
+    if (__all_sync(kFull, all)) break;
+  }
+  const float inv = 1.f / l;
+#pragma unroll
+  for (int e = 0; e < DP / 32; ++e) acc[e] *= inv;
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_constant__ FwdTcArgs args) {
+  using L = FwdTile<DP>;
+  const DenseAttnArgs& a = args.d;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t base = (tc::smem_u32(smem_raw) + 1023) & ~1023u;
+  const uint32_t q_addr = base, kv_addr = base + 2 * L::BYTES;
+  __shared__ uint64_t q_full[2], kv_full[L::STAGES], kv_empty[L::STAGES], s_full[2], p_full[2], o_done[2], drained;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int s_fail;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // the last query tiles, which see the most keys, first; heads of a tile side by side
+  const int index = int(gridDim.x) - 1 - int(blockIdx.x);
+  const int slot = index / a.Hq, hq = index - slot * a.Hq;
+  const SeqTile t = seq_tile(a, slot, 2 * kRows, false);
+  const int q0 = t.tile * 2 * kRows;
+  if (q0 >= t.q_len) return;
+  // key tiles that each query tile visits
+  int tiles[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int first = q0 + i * kRows, rows = min(kRows, t.q_len - first);
+    tiles[i] = rows > 0 ? (last_visible(a, t, first + rows - 1) + kRows) / kRows : 0;
+  }
+  const int most = max(tiles[0], tiles[1]);
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&q_full[i], 1);
+      tc::mbar_init(&s_full[i], 1);
+      tc::mbar_init(&p_full[i], 4);
+      tc::mbar_init(&o_done[i], 1);
+    }
+    for (int i = 0; i < L::STAGES; ++i) {
+      tc::mbar_init(&kv_full[i], 1);
+      tc::mbar_init(&kv_empty[i], 1);
+    }
+    tc::mbar_init(&drained, 1);
+    s_fail = 0;
+    tc::fence_barrier_init();
+  }
+  if (warp == kMmaWarp) tc::tmem_alloc(&tmem_slot, 512);
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  // TMEM columns: S/P of the two tiles, then their O
+  const uint32_t tS[2] = {tmem, tmem + 128}, tO[2] = {tmem + 256, tmem + 256 + DP};
+
+  if (warp == kLoadWarp) {
+    if (lane == 0) {
+      const int h = hq / a.G;
+      for (int i = 0; i < 2; ++i) {
+        if (!tiles[i]) continue;
+        tc::mbar_arrive_expect_tx(&q_full[i], L::BYTES);
+        for (int c = 0; c < L::CH; ++c)
+          tc::tma_load_4d(q_addr + i * L::BYTES + c * kRows * 128, &args.tm_q, c * 64, hq, t.q_begin + q0 + i * kRows, t.b,
+                          &q_full[i]);
+      }
+      for (int n = 0; n < 2 * most; ++n) {   // K0 V0 K1 V1 ...
+        const int st = n % L::STAGES;
+        if (!tc::mbar_wait(&kv_empty[st], ((n / L::STAGES) & 1) ^ 1)) {
+          s_fail = 1;
+          // the copies in flight land before the CTA ends
+          for (int x = max(0, n - L::STAGES); x < n; ++x) tc::mbar_wait(&kv_full[x % L::STAGES], (x / L::STAGES) & 1);
+          break;
+        }
+        tc::mbar_arrive_expect_tx(&kv_full[st], L::BYTES);
+        const CUtensorMap* map = n & 1 ? &args.tm_v : &args.tm_k;
+        for (int c = 0; c < L::CH; ++c)
+          tc::tma_load_4d(kv_addr + st * L::BYTES + c * kRows * 128, map, c * 64, h, t.k_begin + (n >> 1) * kRows, t.b,
+                          &kv_full[st]);
+      }
+    }
+    __syncwarp();
+  } else if (warp == kMmaWarp) {
+    if (lane == 0) {
+      const uint32_t id_s = tc::idesc_f16(kRows, kRows, args.bf16), id_o = tc::idesc_f16(kRows, DP, args.bf16, 1);
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, int phase) {
+        if (ok && !tc::mbar_wait(bar, phase & 1)) { s_fail = 1; ok = false; }
+      };
+      for (int j = 0; j <= most && ok; ++j) {
+        const int nk = 2 * j, nv = 2 * j - 1;   // ring positions of K_j and V_{j-1}
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (j >= 1 && j <= tiles[i]) {        // O += P V of key tile j - 1
+            wait(&kv_full[nv % L::STAGES], nv / L::STAGES);
+            wait(&p_full[i], j - 1);
+            if (!ok) break;
+            tc::fence_after_sync();
+            const uint32_t v = kv_addr + (nv % L::STAGES) * L::BYTES;
+#pragma unroll
+            for (int s = 0; s < kRows / 16; ++s)
+              tc::mma_f16_ts(tO[i], tS[i] + s * 8, tc::desc_make(v + s * 16 * 128, kRows * 128, 1024, 2), id_o,
+                             j > 1 || s > 0);
+            if (j == tiles[i]) tc::mma_commit(&o_done[i]);
+          }
+          if (j < tiles[i]) {                   // S = Q K^T of key tile j
+            if (j == 0) wait(&q_full[i], 0);
+            wait(&kv_full[nk % L::STAGES], nk / L::STAGES);
+            if (!ok) break;
+            tc::fence_after_sync();
+            const uint32_t k = kv_addr + (nk % L::STAGES) * L::BYTES, q = q_addr + i * L::BYTES;
+#pragma unroll
+            for (int s = 0; s < DP / 16; ++s) {
+              const uint32_t off = (s >> 2) * kRows * 128 + (s & 3) * 32;
+              tc::mma_f16(tS[i], tc::desc_sw128(q + off), tc::desc_sw128(k + off), id_s, s > 0);
+            }
+            tc::mma_commit(&s_full[i]);
+          }
+        }
+        if (!ok) break;
+        // a stage that no later tile takes is not handed back: nothing may arrive after the CTA's end
+        if (j >= 1 && nv + L::STAGES < 2 * most) tc::mma_commit(&kv_empty[nv % L::STAGES]);
+        if (j < most && nk + L::STAGES < 2 * most) tc::mma_commit(&kv_empty[nk % L::STAGES]);
+      }
+      if (!ok) {
+        tc::mma_commit(&drained);
+        tc::mbar_wait(&drained, 0);
+      }
+    }
+    __syncwarp();
+  } else {
+    const int i = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    const int qi = q0 + i * kRows + row;             // query of this thread
+    const uint32_t lane_base = uint32_t(quarter * 32) << 16;
+    const uint32_t ts = tS[i] + lane_base, to = tO[i] + lane_base;
+    const bool real = qi < t.q_len;
+    const int last = real ? last_visible(a, t, qi) : -1;
+    const float sl = a.scale * kLog2e;
+    float m = -INFINITY, l = 0.f;                    // base-2 logits
+    bool ok = true;
+    const int full = (last_visible(a, t, q0 + i * kRows) + 1) / kRows;   // key tiles that every row sees whole
+    for (int j = 0; j < tiles[i]; ++j) {
+      if (!tc::mbar_wait(&s_full[i], j & 1)) { s_fail = 1; ok = false; break; }
+      tc::fence_after_sync();
+      uint32_t s0[64], s1[64];
+      tc::tmem_ld64_nowait(ts, s0);
+      tc::tmem_ld64_nowait(ts + 64, s1);
+      tc::tmem_wait_ld2(s0, s1);
+      float x0[64], x1[64];
+#pragma unroll
+      for (int c = 0; c < 64; ++c) {
+        x0[c] = __uint_as_float(s0[c]);
+        x1[c] = __uint_as_float(s1[c]);
+      }
+      if (j >= full) {
+        const int lim = last - j * kRows;
+#pragma unroll
+        for (int c = 0; c < 64; ++c) {
+          if (c > lim) x0[c] = -INFINITY;
+          if (c + 64 > lim) x1[c] = -INFINITY;
+        }
+      }
+      const float top = fmaxf(max_of(x0), max_of(x1)) * sl;
+      if (j == 0) {
+        m = top;
+      } else if (__any_sync(kFull, top > m + kRescale)) {
+        const float to_m = fmaxf(m, top);
+        const float alpha = to_m == -INFINITY ? 1.f : tc::ex2f(m - to_m);
+        m = to_m;
+        l *= alpha;
+#pragma unroll
+        for (int c = 0; c < DP; c += 16) {
+          float o[16];
+          uint32_t r[16];
+          tc::tmem_ld16(to + c, o);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(o[e] * alpha);
+          tc::tmem_st16(to + c, r);
+        }
+      }
+      const float ref = m == -INFINITY ? 0.f : m;
+      const float2 k2 = make_float2(sl, sl), c2 = make_float2(-ref, -ref);
+      uint32_t w[32];
+      float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < 64; c += 2) {
+        float2 p = tc::fma2(make_float2(x0[c], x0[c + 1]), k2, c2);
+        p = make_float2(tc::ex2f(p.x), tc::ex2f(p.y));
+        sum0 = tc::add2(sum0, p);
+        w[c / 2] = pack2<T>(p.x, p.y);
+      }
+      tmem_st32(ts, w);
+#pragma unroll
+      for (int c = 0; c < 64; c += 2) {
+        float2 p = tc::fma2(make_float2(x1[c], x1[c + 1]), k2, c2);
+        p = make_float2(tc::ex2f(p.x), tc::ex2f(p.y));
+        sum1 = tc::add2(sum1, p);
+        w[c / 2] = pack2<T>(p.x, p.y);
+      }
+      tmem_st32(ts + 32, w);
+      l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
+      tmem_wait_st();
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&p_full[i]);
+    }
+    // O / l through this warp's rows of the query tile's shared memory (its
+    // last reader was the tile's last S, complete before o_done): whole rows
+    // to global memory
+    const bool any = tiles[i] > 0;
+    if (any && ok && !tc::mbar_wait(&o_done[i], 0)) { s_fail = 1; ok = false; }
+    tc::fence_after_sync();
+    const float inv = !ok ? NAN : l == 0.f ? 0.f : 1.f / l;
+    constexpr int SEG = DP / 8;                      // 16-byte segments of a row
+    const uint32_t stage = q_addr + i * L::BYTES + quarter * 32 * DP * 2;
+    bool wild = false;
+#pragma unroll
+    for (int c = 0; c < DP; c += 32) {
+      float o[32];
+      if (any && ok) {
+        tc::tmem_ld32(to + c, o);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        wild = wild || isnan(o[e]);
+        o[e] = l == 0.f && ok ? 0.f : o[e] * inv;
+      }
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const int seg = c / 8 + s;
+        st_shared16(stage + (lane * SEG + (seg ^ (lane & 7))) * 16, pack2<T>(o[8 * s], o[8 * s + 1]),
+                    pack2<T>(o[8 * s + 2], o[8 * s + 3]), pack2<T>(o[8 * s + 4], o[8 * s + 5]),
+                    pack2<T>(o[8 * s + 6], o[8 * s + 7]));
+      }
+    }
+    __syncwarp();
+    uint32_t again = __ballot_sync(kFull, ok && real && wild && l != 0.f && !isnan(l));
+    while (again) {
+      const int r = __ffs(again) - 1;
+      again &= again - 1;
+      float acc[DP / 32];
+      row_again<T, DP>(a, t, hq, q0 + i * kRows + quarter * 32 + r, __shfl_sync(kFull, m, r), __shfl_sync(kFull, l, r), acc);
+#pragma unroll
+      for (int e = 0; e < DP / 32; ++e) {
+        const int d = lane + 32 * e;
+        const T v = from_f32<T>(acc[e]);
+        asm volatile("st.shared.b16 [%0], %1;"
+                     :: "r"(stage + (r * SEG + ((d >> 3) ^ (r & 7))) * 16 + (d & 7) * 2),
+                        "h"(*reinterpret_cast<const uint16_t*>(&v)) : "memory");
+      }
+      __syncwarp();
+    }
+    const int64_t row0 = int64_t(t.b) * a.T + t.q_begin + q0 + i * kRows + quarter * 32;
+    const int rows = min(32, t.q_len - (q0 + i * kRows + quarter * 32));
+    T* out = static_cast<T*>(a.out);
+    for (int f = lane; f < rows * SEG; f += 32) {
+      const int r = f / SEG, seg = f % SEG;
+      const uint4 v = ld_shared16(stage + (r * SEG + (seg ^ (r & 7))) * 16);
+      if (seg * 8 < a.Dv) *reinterpret_cast<uint4*>(out + ((row0 + r) * a.Hq + hq) * a.Dv + seg * 8) = v;
+    }
+    if (a.lse && real)
+      a.lse[(row0 + lane) * a.Hq + hq] = !ok ? NAN : l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  if (tid == 0 && s_fail && a.status) atomicExch(a.status, PISA_ERR_TIMEOUT);
+  if (warp == kMmaWarp) tc::tmem_free(tmem, 512);
+}
+
+template <typename T, int DP>
+int fwd_t(const FwdTcArgs& a, cudaStream_t s) {
+  using L = FwdTile<DP>;
+  const int64_t blocks = seq_slots(a.d.cu_q, a.d.B, a.d.T, a.d.sequences, 2 * kRows) * a.d.Hq;
+  if (blocks >= (int64_t(1) << 31)) return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
+  cudaError_t e = cudaFuncSetAttribute(dense_fwd_tc_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+  if (e != cudaSuccess) return fail_cuda(e, "dense attention smem attribute");
+  dense_fwd_tc_kernel<T, DP><<<unsigned(blocks), kThreads, L::SMEM, s>>>(a);
+  PISA_CHECK_LAUNCH();
+  return PISA_OK;
+}
+
+}  // namespace
+
+bool dense_attn_tc_eligible(const DenseAttnArgs& a, int dtype) {
+  return dtype != PISA_F32 && a.D <= 128 && a.Dv <= 128;
+}
+
+int dense_attn_fwd_tc(const DenseAttnArgs& d, int dtype, cudaStream_t stream) {
+  FwdTcArgs a{};
+  a.d = d;
+  a.bf16 = dtype == PISA_BF16;
+  int rc = dense_tensor_map(&a.tm_q, d.q, dtype, d.B, d.T, d.Hq, d.D, d.q_sb, d.q_st, d.q_sh, kRows);
+  if (rc == PISA_OK) rc = dense_tensor_map(&a.tm_k, d.k, dtype, d.B, d.N, d.H, d.D, d.k_sb, d.k_st, d.k_sh, kRows);
+  if (rc == PISA_OK) rc = dense_tensor_map(&a.tm_v, d.v, dtype, d.B, d.N, d.H, d.Dv, d.v_sb, d.v_st, d.v_sh, kRows);
+  if (rc) return rc;
+  const bool narrow = d.D <= 64 && d.Dv <= 64;
+  if (dtype == PISA_BF16) return narrow ? fwd_t<__nv_bfloat16, 64>(a, stream) : fwd_t<__nv_bfloat16, 128>(a, stream);
+  return narrow ? fwd_t<__half, 64>(a, stream) : fwd_t<__half, 128>(a, stream);
+}
+
+}  // namespace pisa

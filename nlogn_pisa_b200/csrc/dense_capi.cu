@@ -118,7 +118,7 @@ int pisa_full_attn_fwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, 
     if (e != cudaSuccess) return fail_cuda(e, "status clear");
     a.status = static_cast<int*>(workspace);
   }
-  return dense_attn_fwd_simt(a, dtype, s);
+  return dense_attn_tc_eligible(a, dtype) ? dense_attn_fwd_tc(a, dtype, s) : dense_attn_fwd_simt(a, dtype, s);
 }
 
 int64_t pisa_full_attn_bwd_workspace_bytes(int64_t B, int64_t Tq, int64_t Hq, int64_t H, int64_t D, int64_t Dv,
