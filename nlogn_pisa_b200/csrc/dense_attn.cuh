@@ -33,7 +33,7 @@ struct DenseAttnArgs {
   const void* o;    // the forward's output, contiguous
   const void* dout; // contiguous
   const float* lse_in;
-  float* delta;     // [B, T, Hq] row dot products of dout and out
+  float* delta;     // workspace: [B, T, Hq] row dot products of dout and out (FMA form), row statistics (tensor-core form)
   void* dq;
   void* dk;
   void* dv;
@@ -43,7 +43,7 @@ struct DenseAttnArgs {
 // k_begin .. k_begin + k_len of batch row b; query i sits at position
 // shift + i, key j at position j.
 struct SeqTile {
-  int b, tile, q_begin, q_len, k_begin, k_len;
+  int b, seq, tile, q_begin, q_len, k_begin, k_len;
   int64_t shift;
 };
 
@@ -78,6 +78,7 @@ __device__ __forceinline__ SeqTile seq_tile(const DenseAttnArgs& a, int slot, in
   if (a.cu_q == nullptr) {
     t.tile = slot / a.B;   // equal tiles of all batch rows side by side
     t.b = slot - t.tile * a.B;
+    t.seq = t.b;
     t.q_begin = t.k_begin = 0;
     t.q_len = a.T;
     t.k_len = a.N;
@@ -92,6 +93,7 @@ __device__ __forceinline__ SeqTile seq_tile(const DenseAttnArgs& a, int slot, in
     else hi = mid - 1;
   }
   t.b = 0;
+  t.seq = lo;
   t.q_begin = seq_begin(a, a.cu_q, a.T, lo);
   t.k_begin = seq_begin(a, a.cu_k, a.N, lo);
   t.q_len = seq_end(a, a.cu_q, a.T, lo, t.q_begin) - t.q_begin;
@@ -103,6 +105,11 @@ __device__ __forceinline__ SeqTile seq_tile(const DenseAttnArgs& a, int slot, in
   }
   t.shift = int64_t(t.k_len) - t.q_len;
   return t;
+}
+
+// Slot of query tile `tile` (of `rows` queries) of t's sequence: the inverse of seq_tile.
+__device__ __forceinline__ int query_slot(const DenseAttnArgs& a, const SeqTile& t, int tile, int rows) {
+  return a.cu_q == nullptr ? tile * a.B + t.b : t.q_begin / rows + t.seq + tile;
 }
 
 // Keys that query i of the tile's sequence sees: 0 .. last (-1: none).
@@ -130,6 +137,9 @@ inline int dense_tensor_map(CUtensorMap* map, const void* base, int dtype, int64
 // 16-bit tensors of at most 128 dims: tensor-core kernels
 bool dense_attn_tc_eligible(const DenseAttnArgs& a, int dtype);
 int dense_attn_fwd_tc(const DenseAttnArgs& a, int dtype, cudaStream_t stream);
+// a.delta: dense_bwd_stat_floats(...) floats
+int64_t dense_bwd_stat_floats(bool packed, int64_t B, int64_t T, int64_t Hq, int64_t sequences);
+int dense_attn_bwd_tc(const DenseAttnArgs& a, int dtype, cudaStream_t stream);
 
 int dense_attn_fwd_simt(const DenseAttnArgs& a, int dtype, cudaStream_t stream);
 int dense_attn_bwd_simt(const DenseAttnArgs& a, int dtype, cudaStream_t stream);

@@ -1,0 +1,568 @@
+// Dense attention backward on the tensor cores: 16-bit tensors, heads of at
+// most 128 dims (formulas in dense_attn.cu).  Three launches:
+//
+// 1. Row statistics: -lse and -scale * delta of every query (delta = dout .
+//    out), base 2, in tiles of 128 queries of one sequence and head.  Rows past
+//    a sequence's end and rows without keys get lse = +inf, so their weights
+//    are zero below.
+// 2. dK, dV: one CTA per 128 keys of a KV head, over the query tiles that see
+//    them, for each of the G query heads:
+//      MMA  S^T  = K Q^T       (M = 128 keys, N = 128 queries)  -> TMEM
+//      MMA  dP^T = V dO^T                                       -> TMEM
+//      P^T = 2^(S^T - lse), dS^T = P^T (dP^T - delta) scale, a thread per key
+//      row and 64 queries; both return to TMEM as 16-bit operands
+//      MMA  dV += P^T dO,  dK += dS^T Q   (A from TMEM, B with queries along K)
+// 3. dQ: one CTA per 128 queries of a query head, over their key tiles:
+//      S = Q K^T, dP = dO V^T, dS as above, dQ += dS K.
+//
+// Recomputing S and dP in launch 3 costs two more products than one kernel
+// that adds dQ tiles into memory, but every sum stays in TMEM: no atomics, no
+// fp32 copy of dQ, and results do not vary from run to run.  P and dS are
+// rounded to the input type because the MMAs take their operands so.
+//
+// Rows of the last, ragged tile of a sequence belong to other sequences: the
+// products that sum over them take only the 16-row steps that hold real rows,
+// and a warp zeroes the rest of the last step in shared memory first (a weight
+// of zero would not silence an infinite or NaN value).
+#include "dense_tc.cuh"
+
+namespace pisa {
+
+namespace {
+
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kTrimWarp = 10;
+constexpr int kThreads = 352;
+
+struct BwdTcArgs {
+  CUtensorMap tm_q, tm_k, tm_v, tm_do;   // boxes of 64 dims x 128 rows of one head
+  DenseAttnArgs d;
+  float* stats;                          // [Hq][q_slots][2][128]
+  int64_t q_slots;
+  int bf16;
+};
+
+template <int DP> struct BwdTile {
+  static constexpr int BYTES = kRows * DP * 2;
+  // ring of operand tiles (Q dO Q dO ... or K V K V ...): 64 dims leave room
+  // for three pairs, which also keeps a second CTA off the SM's TMEM
+  static constexpr int RING = DP == 128 ? 4 : 6;
+  static constexpr int SMEM = (2 + RING) * BYTES + RING / 2 * 1024 + 1024;
+};
+
+__device__ __forceinline__ float* stat_tile(const BwdTcArgs& a, int hq, int64_t slot) {
+  return a.stats + (hq * a.q_slots + slot) * 2 * kRows;
+}
+
+// Launch 1: 16 queries x all heads per CTA, half a warp per row.
+template <typename T>
+__global__ void __launch_bounds__(256) dense_stats_kernel(const __grid_constant__ BwdTcArgs args) {
+  const DenseAttnArgs& a = args.d;
+  const int slot = blockIdx.x;
+  const SeqTile t = seq_tile(a, slot, kRows, false);
+  const int q0 = t.tile * kRows;
+  if (q0 >= t.q_len) return;
+  const int half = threadIdx.x >> 4, lane = threadIdx.x & 15;
+  const T* out = static_cast<const T*>(a.o);
+  const T* dout = static_cast<const T*>(a.dout);
+  for (int x = half; x < 16 * a.Hq; x += 16) {
+    const int r = blockIdx.y * 16 + x / a.Hq, hq = x % a.Hq;
+    const bool real = q0 + r < t.q_len;
+    float dot = 0.f, lse = -INFINITY;
+    if (real) {
+      const int64_t row = (int64_t(t.b) * a.T + t.q_begin + q0 + r) * a.Hq + hq;
+      lse = a.lse_in[row];
+      for (int d = lane * 8; d < a.Dv; d += 128) {
+        float u[8], v[8];
+        load_vec<T>(out + row * a.Dv + d, u);
+        load_vec<T>(dout + row * a.Dv + d, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dot = fmaf(u[e], v[e], dot);
+      }
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) dot += __shfl_xor_sync(kFull, dot, o);
+    if (lane == 0) {
+      float* st = stat_tile(args, hq, slot);
+      st[r] = lse == -INFINITY ? -INFINITY : -lse * kLog2e;
+      st[kRows + r] = -dot * a.scale;
+    }
+  }
+}
+
+// One operand tile of a head: DP/64 boxes on `bar`, issued by one thread.
+template <int DP>
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, int head, int row, int b, uint64_t* bar) {
+#pragma unroll
+  for (int c = 0; c < DP / 64; ++c) tc::tma_load_4d(dst + c * kRows * 128, map, c * 64, head, row, b, bar);
+}
+
+// D (+)= A B^T over DP dims, both operands K-major in shared memory.
+template <int DP>
+__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) {
+    const uint32_t off = (s >> 2) * kRows * 128 + (s & 3) * 32;
+    tc::mma_f16(d, tc::desc_sw128(a + off), tc::desc_sw128(b + off), idesc, s > 0);
+  }
+}
+
+// D (+)= A B over the first `steps` * 16 rows of B; A in TMEM as two halves of
+// 64 columns each (32 registers of pairs, 64 columns apart), B MN-major.
+__device__ __forceinline__ void mma_cols(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int steps, bool accumulate) {
+#pragma unroll
+  for (int s = 0; s < kRows / 16; ++s)
+    if (s < steps)
+      tc::mma_f16_ts(d, a + (s >> 2) * 64 + (s & 3) * 8, tc::desc_make(b + s * 16 * 128, kRows * 128, 1024, 2), idesc,
+                     accumulate || s > 0);
+}
+
+struct Wait {
+  int* fail;
+  bool ok = true;
+  __device__ __forceinline__ bool operator()(uint64_t* bar, int phase) {
+    if (ok && !tc::mbar_wait(bar, phase & 1)) { *fail = 1; ok = false; }
+    return ok;
+  }
+};
+
+// Launch 2.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_constant__ BwdTcArgs args) {
+  using L = BwdTile<DP>;
+  const DenseAttnArgs& a = args.d;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t base = (tc::smem_u32(smem_raw) + 1023) & ~1023u;
+  const uint32_t k_addr = base, v_addr = base + L::BYTES, ring = base + 2 * L::BYTES;
+  const uint32_t stat_addr = ring + L::RING * L::BYTES;
+  const float* stat_smem = reinterpret_cast<const float*>(smem_raw + (stat_addr - tc::smem_u32(smem_raw)));
+  __shared__ uint64_t kv_full, full[L::RING], raw[L::RING], empty[L::RING], s_full, p_full, dp_full, ds_full, done;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int s_fail;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int slot = int(blockIdx.x) / a.H, h = int(blockIdx.x) - slot * a.H;   // early keys, seen by most queries, first
+  const SeqTile t = seq_tile(a, slot, kRows, true);
+  const int j0 = t.tile * kRows;
+  if (j0 >= t.k_len) return;
+  const int first_tile = first_seeing(a, t, j0) / kRows, end_tile = (t.q_len + kRows - 1) / kRows;
+  const int per_head = first_seeing(a, t, j0) < t.q_len ? end_tile - first_tile : 0;
+  const int total = per_head * a.G;
+  const int tail = t.q_len - (end_tile - 1) * kRows;   // real rows of the last query tile
+  if (tid == 0) {
+    tc::mbar_init(&kv_full, 1);
+    for (int i = 0; i < L::RING; ++i) {
+      tc::mbar_init(&full[i], 1);
+      tc::mbar_init(&raw[i], 1);
+      tc::mbar_init(&empty[i], 1);
+    }
+    tc::mbar_init(&s_full, 1);
+    tc::mbar_init(&p_full, 8);
+    tc::mbar_init(&dp_full, 1);
+    tc::mbar_init(&ds_full, 8);
+    tc::mbar_init(&done, 1);
+    s_fail = 0;
+    tc::fence_barrier_init();
+  }
+  if (warp == kMmaWarp) tc::tmem_alloc(&tmem_slot, 512);
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  const uint32_t tS = tmem, tP = tmem + 128, tV = tmem + 256, tK = tmem + 256 + DP;
+  Wait wait{&s_fail};
+  // tile n: query head h*G + n / per_head, query tile first_tile + n % per_head;
+  // ring position 2n holds its Q (and statistics), 2n + 1 its dO
+  // after an expired wait: the copies in flight land before the CTA ends
+  auto drain = [&](int issued) {
+    for (int pos = max(0, issued - L::RING); pos < issued; ++pos) tc::mbar_wait(&full[pos % L::RING], (pos / L::RING) & 1);
+  };
+  auto ragged = [&](int n) { return tail < kRows && (n + 1) % per_head == 0; };
+
+  if (warp == kLoadWarp) {
+    if (lane == 0 && total > 0) {
+      tc::mbar_arrive_expect_tx(&kv_full, 2 * L::BYTES);
+      load_tile<DP>(k_addr, &args.tm_k, h, t.k_begin + j0, t.b, &kv_full);
+      load_tile<DP>(v_addr, &args.tm_v, h, t.k_begin + j0, t.b, &kv_full);
+      int g = 0, qt = first_tile, issued = 0;
+      for (int n = 0; n < total; ++n) {
+        const bool rag = ragged(n);
+        const int row = t.q_begin + qt * kRows, hq = h * a.G + g;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int pos = 2 * n + x, st = pos % L::RING;
+          if (!wait(&empty[st], (pos / L::RING) + 1)) break;
+          uint64_t* bar = rag ? &raw[st] : &full[st];
+          tc::mbar_arrive_expect_tx(bar, L::BYTES + (x == 0 ? 1024 : 0));
+          load_tile<DP>(ring + st * L::BYTES, x == 0 ? &args.tm_q : &args.tm_do, hq, row, t.b, bar);
+          issued = pos + 1;
+          if (x == 0) bulk_load(stat_addr + (st / 2) * 1024, stat_tile(args, hq, query_slot(a, t, qt, kRows)), 1024, bar);
+        }
+        if (!wait.ok) break;
+        if (++qt == end_tile) { qt = first_tile; ++g; }
+      }
+      if (!wait.ok) drain(issued);
+    }
+    __syncwarp();
+  } else if (warp == kTrimWarp) {
+    if (tail < kRows && total > 0) {
+      uint32_t uses = 0;   // parity of the ragged tiles that each ring slot has held
+      for (int n = per_head - 1; n < total && wait.ok; n += per_head) {
+        for (int pos = 2 * n; pos < 2 * n + 2; ++pos) {
+          const int st = pos % L::RING;
+          if (!wait(&raw[st], uses >> st)) break;
+          uses ^= 1u << st;
+          zero_rows<DP>(ring + st * L::BYTES, tail, (tail + 15) & ~15, lane);
+          tc::fence_async_smem();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&full[st]);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == kMmaWarp) {
+    if (lane == 0 && total > 0) {
+      const uint32_t id_s = tc::idesc_f16(kRows, kRows, args.bf16), id_o = tc::idesc_f16(kRows, DP, args.bf16, 1);
+      auto tile = [&](int pos) { return ring + (pos % L::RING) * L::BYTES; };
+      auto scores = [&](int n) {
+        if (!wait(&full[(2 * n) % L::RING], (2 * n) / L::RING)) return;
+        tc::fence_after_sync();
+        mma_rows<DP>(tS, k_addr, tile(2 * n), id_s);
+        tc::mma_commit(&s_full);
+      };
+      auto grads = [&](int n) {
+        if (!wait(&full[(2 * n + 1) % L::RING], (2 * n + 1) / L::RING)) return;
+        tc::fence_after_sync();
+        mma_rows<DP>(tP, v_addr, tile(2 * n + 1), id_s);
+        tc::mma_commit(&dp_full);
+      };
+      wait(&kv_full, 0);
+      if (wait.ok) scores(0);
+      if (wait.ok) grads(0);
+      for (int n = 0; n < total && wait.ok; ++n) {
+        const int steps = ragged(n) ? (tail + 15) / 16 : kRows / 16;
+        if (!wait(&p_full, n)) break;
+        tc::fence_after_sync();
+        mma_cols(tV, tS, tile(2 * n + 1), id_o, steps, n > 0);
+        // a slot that no later tile takes is not handed back: nothing may arrive after the CTA's end
+        if (2 * n + 1 + L::RING < 2 * total) tc::mma_commit(&empty[(2 * n + 1) % L::RING]);
+        if (n + 1 < total) scores(n + 1);
+        if (!wait(&ds_full, n)) break;
+        tc::fence_after_sync();
+        mma_cols(tK, tP, tile(2 * n), id_o, steps, n > 0);
+        if (2 * n + L::RING < 2 * total) tc::mma_commit(&empty[(2 * n) % L::RING]);
+        if (n + 1 < total) grads(n + 1);
+      }
+      tc::mma_commit(&done);
+      if (!wait.ok) tc::mbar_wait(&done, 0);
+    }
+    __syncwarp();
+  } else {
+    const int side = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;   // key row, queries 64*side ..
+    const uint32_t lanes = uint32_t(quarter * 32) << 16;
+    const uint32_t ts = tS + lanes + side * 64, tp = tP + lanes + side * 64;
+    const float2 sl2 = make_float2(a.scale * kLog2e, a.scale * kLog2e), sc2 = make_float2(a.scale, a.scale);
+    const int first = first_seeing(a, t, j0 + row), whole = first_seeing(a, t, j0 + kRows - 1);
+    int qt = first_tile;
+    for (int n = 0; n < total; ++n) {
+      const int st = (2 * n) % L::RING;
+      if (!wait(&full[st], (2 * n) / L::RING) || !wait(&s_full, n)) break;
+      tc::fence_after_sync();
+      const float4* nlse = reinterpret_cast<const float4*>(stat_smem + (st / 2) * 256 + side * 64);
+      const float4* ndel = nlse + kRows / 4;
+      float p[64];
+      uint32_t w[32];
+      tc::tmem_ld64(ts, p);
+#pragma unroll
+      for (int c = 0; c < 64; c += 4) {
+        const float4 x = nlse[c / 4];
+        const float2 u = tc::fma2(make_float2(p[c], p[c + 1]), sl2, make_float2(x.x, x.y));
+        const float2 v = tc::fma2(make_float2(p[c + 2], p[c + 3]), sl2, make_float2(x.z, x.w));
+        p[c] = tc::ex2f(u.x);
+        p[c + 1] = tc::ex2f(u.y);
+        p[c + 2] = tc::ex2f(v.x);
+        p[c + 3] = tc::ex2f(v.y);
+      }
+      if (qt * kRows < whole || ragged(n)) {
+        // queries before column `low` do not see the key, those from `high` on are not the sequence's
+        const int low = first - qt * kRows - side * 64, high = t.q_len - qt * kRows - side * 64;
+#pragma unroll
+        for (int c = 0; c < 64; ++c)
+          if (c < low || c >= high) p[c] = 0.f;
+      }
+#pragma unroll
+      for (int c = 0; c < 64; c += 2) w[c / 2] = pack2<T>(p[c], p[c + 1]);
+      tmem_st32(ts, w);
+      tmem_wait_st();
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&p_full);
+      if (!wait(&dp_full, n)) break;
+      tc::fence_after_sync();
+      float dp[64];
+      tc::tmem_ld64(tp, dp);
+#pragma unroll
+      for (int c = 0; c < 64; c += 4) {
+        const float4 x = ndel[c / 4];
+        const float2 u = mul2(tc::fma2(make_float2(dp[c], dp[c + 1]), sc2, make_float2(x.x, x.y)), make_float2(p[c], p[c + 1]));
+        const float2 v =
+            mul2(tc::fma2(make_float2(dp[c + 2], dp[c + 3]), sc2, make_float2(x.z, x.w)), make_float2(p[c + 2], p[c + 3]));
+        dp[c] = u.x;
+        dp[c + 1] = u.y;
+        dp[c + 2] = v.x;
+        dp[c + 3] = v.y;
+      }
+      // without weight no gradient, whatever dP holds there
+#pragma unroll
+      for (int c = 0; c < 64; c += 2) w[c / 2] = pack2<T>(p[c] == 0.f ? 0.f : dp[c], p[c + 1] == 0.f ? 0.f : dp[c + 1]);
+      tmem_st32(tp, w);
+      tmem_wait_st();
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&ds_full);
+      if (++qt == end_tile) qt = first_tile;
+    }
+    if (total > 0) wait(&done, 0);
+    tc::fence_after_sync();
+    // warps of side 0 store dV, of side 1 dK, staged in the V and K tiles
+    const int rows = min(32, t.k_len - (j0 + quarter * 32));
+    const int64_t at = (int64_t(t.b) * a.N + t.k_begin + j0 + quarter * 32) * a.H + h;
+    const float mul = wait.ok ? 1.f : NAN;
+    if (side == 0)
+      store_lanes<T, DP>(tV + lanes, total == 0, mul, v_addr + quarter * 32 * DP * 2, static_cast<T*>(a.dv) + at * a.Dv,
+                         int64_t(a.H) * a.Dv, rows, a.Dv, lane);
+    else
+      store_lanes<T, DP>(tK + lanes, total == 0, mul, k_addr + quarter * 32 * DP * 2, static_cast<T*>(a.dk) + at * a.D,
+                         int64_t(a.H) * a.D, rows, a.D, lane);
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  if (tid == 0 && s_fail && a.status) atomicExch(a.status, PISA_ERR_TIMEOUT);
+  if (warp == kMmaWarp) tc::tmem_free(tmem, 512);
+}
+
+// Launch 3.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_constant__ BwdTcArgs args) {
+  using L = BwdTile<DP>;
+  const DenseAttnArgs& a = args.d;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t base = (tc::smem_u32(smem_raw) + 1023) & ~1023u;
+  const uint32_t q_addr = base, o_addr = base + L::BYTES, ring = base + 2 * L::BYTES;
+  __shared__ uint64_t q_full, full[L::RING], raw, empty[L::RING], s_full[2], dp_full, dp_free, ds_full, done;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int s_fail;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int index = int(gridDim.x) - 1 - int(blockIdx.x);   // late queries, which see the most keys, first
+  const int slot = index / a.Hq, hq = index - slot * a.Hq, h = hq / a.G;
+  const SeqTile t = seq_tile(a, slot, kRows, false);
+  const int q0 = t.tile * kRows;
+  if (q0 >= t.q_len) return;
+  const int valid = min(kRows, t.q_len - q0);
+  const int keys = last_visible(a, t, q0 + valid - 1) + 1, total = (keys + kRows - 1) / kRows;
+  const int tail = min(kRows, t.k_len - (total - 1) * kRows);   // real rows of the last key tile
+  if (tid == 0) {
+    tc::mbar_init(&q_full, 1);
+    for (int i = 0; i < L::RING; ++i) {
+      tc::mbar_init(&full[i], 1);
+      tc::mbar_init(&empty[i], 1);
+    }
+    tc::mbar_init(&raw, 1);
+    tc::mbar_init(&s_full[0], 1);
+    tc::mbar_init(&s_full[1], 1);
+    tc::mbar_init(&dp_full, 1);
+    tc::mbar_init(&dp_free, 8);
+    tc::mbar_init(&ds_full, 8);
+    tc::mbar_init(&done, 1);
+    s_fail = 0;
+    tc::fence_barrier_init();
+  }
+  if (warp == kMmaWarp) tc::tmem_alloc(&tmem_slot, 512);
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  const uint32_t tS[2] = {tmem, tmem + 128}, tP = tmem + 256, tQ = tmem + 384;   // dS overwrites its S
+  Wait wait{&s_fail};
+
+  if (warp == kLoadWarp) {
+    if (lane == 0 && total > 0) {
+      tc::mbar_arrive_expect_tx(&q_full, 2 * L::BYTES);
+      load_tile<DP>(q_addr, &args.tm_q, hq, t.q_begin + q0, t.b, &q_full);
+      load_tile<DP>(o_addr, &args.tm_do, hq, t.q_begin + q0, t.b, &q_full);
+      int issued = 0;
+      for (int pos = 0; pos < 2 * total; ++pos) {   // K0 V0 K1 V1 ...
+        const int st = pos % L::RING;
+        if (!wait(&empty[st], (pos / L::RING) + 1)) break;
+        // keys of a ragged last tile pass through the trimming warp
+        uint64_t* bar = pos == 2 * total - 2 && tail < kRows ? &raw : &full[st];
+        tc::mbar_arrive_expect_tx(bar, L::BYTES);
+        load_tile<DP>(ring + st * L::BYTES, pos & 1 ? &args.tm_v : &args.tm_k, h, t.k_begin + (pos >> 1) * kRows, t.b, bar);
+        issued = pos + 1;
+      }
+      if (!wait.ok)   // the copies in flight land before the CTA ends
+        for (int pos = max(0, issued - L::RING); pos < issued; ++pos)
+          tc::mbar_wait(&full[pos % L::RING], (pos / L::RING) & 1);
+    }
+    __syncwarp();
+  } else if (warp == kTrimWarp) {
+    if (total > 0 && tail < kRows) {
+      const int st = (2 * total - 2) % L::RING;
+      if (wait(&raw, 0)) {
+        zero_rows<DP>(ring + st * L::BYTES, tail, (tail + 15) & ~15, lane);
+        tc::fence_async_smem();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&full[st]);
+      }
+    }
+    __syncwarp();
+  } else if (warp == kMmaWarp) {
+    if (lane == 0 && total > 0) {
+      const uint32_t id_s = tc::idesc_f16(kRows, kRows, args.bf16), id_o = tc::idesc_f16(kRows, DP, args.bf16, 1);
+      auto tile = [&](int pos) { return ring + (pos % L::RING) * L::BYTES; };
+      auto scores = [&](int n) {
+        if (!wait(&full[(2 * n) % L::RING], (2 * n) / L::RING)) return;
+        tc::fence_after_sync();
+        mma_rows<DP>(n & 1 ? tS[1] : tS[0], q_addr, tile(2 * n), id_s);
+        tc::mma_commit(&s_full[n & 1]);
+      };
+      auto grads = [&](int n) {
+        if (!wait(&full[(2 * n + 1) % L::RING], (2 * n + 1) / L::RING)) return;
+        tc::fence_after_sync();
+        mma_rows<DP>(tP, o_addr, tile(2 * n + 1), id_s);
+        tc::mma_commit(&dp_full);
+        if (2 * n + 1 + L::RING < 2 * total) tc::mma_commit(&empty[(2 * n + 1) % L::RING]);
+      };
+      wait(&q_full, 0);
+      if (wait.ok) scores(0);
+      if (wait.ok) grads(0);
+      for (int n = 0; n < total && wait.ok; ++n) {
+        if (n + 1 < total) {
+          scores(n + 1);                      // its buffer held dS(n - 1), whose product was issued before
+          if (!wait(&dp_free, n)) break;      // dP(n) is in registers
+          tc::fence_after_sync();
+          grads(n + 1);
+        }
+        if (!wait(&ds_full, n)) break;
+        tc::fence_after_sync();
+        const int steps = n + 1 == total ? (tail + 15) / 16 : kRows / 16;
+        mma_cols(tQ, n & 1 ? tS[1] : tS[0], tile(2 * n), id_o, steps, n > 0);
+        // a slot that no later tile takes is not handed back: nothing may arrive after the CTA's end
+        if (2 * n + L::RING < 2 * total) tc::mma_commit(&empty[(2 * n) % L::RING]);
+      }
+      tc::mma_commit(&done);
+      if (!wait.ok) tc::mbar_wait(&done, 0);
+    }
+    __syncwarp();
+  } else {
+    const int side = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;   // query row, keys 64*side ..
+    const uint32_t lanes = uint32_t(quarter * 32) << 16;
+    const float2 sl2 = make_float2(a.scale * kLog2e, a.scale * kLog2e), sc2 = make_float2(a.scale, a.scale);
+    float nlse = -INFINITY, ndel = 0.f;
+    int last = -1;
+    if (row < valid) {
+      const float* st = stat_tile(args, hq, slot);
+      nlse = st[row];
+      ndel = st[kRows + row];
+      last = last_visible(a, t, q0 + row);
+    }
+    const float2 nlse2 = make_float2(nlse, nlse), ndel2 = make_float2(ndel, ndel);
+    const int whole = (last_visible(a, t, q0) + 1) / kRows;   // key tiles that every row sees whole
+    for (int n = 0; n < total; ++n) {
+      const uint32_t ts = (n & 1 ? tS[1] : tS[0]) + lanes + side * 64;
+      if (!wait(&s_full[n & 1], n >> 1)) break;
+      tc::fence_after_sync();
+      float p[64], dp[64];
+      tc::tmem_ld64(ts, p);
+#pragma unroll
+      for (int c = 0; c < 64; c += 2) {
+        const float2 u = tc::fma2(make_float2(p[c], p[c + 1]), sl2, nlse2);
+        p[c] = tc::ex2f(u.x);
+        p[c + 1] = tc::ex2f(u.y);
+      }
+      if (!wait(&dp_full, n)) break;
+      tc::fence_after_sync();
+      tc::tmem_ld64(tP + lanes + side * 64, dp);
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&dp_free);
+      uint32_t w[32];
+      const int lim = last - n * kRows - side * 64;
+#pragma unroll
+      for (int c = 0; c < 64; c += 2) {
+        const float2 u = mul2(tc::fma2(make_float2(dp[c], dp[c + 1]), sc2, ndel2), make_float2(p[c], p[c + 1]));
+        dp[c] = u.x;
+        dp[c + 1] = u.y;
+      }
+      if (n >= whole) {
+#pragma unroll
+        for (int c = 0; c < 64; ++c)
+          if (c > lim) dp[c] = 0.f;
+      }
+#pragma unroll
+      for (int c = 0; c < 64; c += 2) w[c / 2] = pack2<T>(dp[c], dp[c + 1]);
+      tmem_st32(ts, w);
+      tmem_wait_st();
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&ds_full);
+    }
+    if (total > 0) wait(&done, 0);
+    tc::fence_after_sync();
+    // each side stores half of the columns, staged in the Q tile (its last reader is done)
+    const int rows = min(32, valid - quarter * 32);
+    const int64_t at = (int64_t(t.b) * a.T + t.q_begin + q0 + quarter * 32) * a.Hq + hq;
+    store_lanes<T, DP / 2>(tQ + lanes + side * (DP / 2), total == 0, wait.ok ? 1.f : NAN, q_addr + warp * 32 * DP,
+                           static_cast<T*>(a.dq) + at * a.D + side * (DP / 2), int64_t(a.Hq) * a.D, rows,
+                           a.D - side * (DP / 2), lane);
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  if (tid == 0 && s_fail && a.status) atomicExch(a.status, PISA_ERR_TIMEOUT);
+  if (warp == kMmaWarp) tc::tmem_free(tmem, 512);
+}
+
+template <typename K>
+int launch(K kernel, int64_t blocks, int smem, const BwdTcArgs& a, cudaStream_t s) {
+  if (blocks >= (int64_t(1) << 31)) return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return fail_cuda(e, "dense attention smem attribute");
+  kernel<<<unsigned(blocks), kThreads, smem, s>>>(a);
+  PISA_CHECK_LAUNCH();
+  return PISA_OK;
+}
+
+template <typename T, int DP>
+int bwd_t(const BwdTcArgs& a, cudaStream_t s) {
+  const DenseAttnArgs& d = a.d;
+  dense_stats_kernel<T><<<dim3(unsigned(a.q_slots), kRows / 16), 256, 0, s>>>(a);
+  PISA_CHECK_LAUNCH();
+  int rc = launch(dense_dkv_tc_kernel<T, DP>, seq_slots(d.cu_q, d.B, d.N, d.sequences, kRows) * d.H, BwdTile<DP>::SMEM, a, s);
+  return rc ? rc : launch(dense_dq_tc_kernel<T, DP>, a.q_slots * d.Hq, BwdTile<DP>::SMEM, a, s);
+}
+
+}  // namespace
+
+int64_t dense_bwd_stat_floats(bool packed, int64_t B, int64_t T, int64_t Hq, int64_t sequences) {
+  return seq_slots(packed, B, T, sequences, kRows) * Hq * 2 * kRows;
+}
+
+int dense_attn_bwd_tc(const DenseAttnArgs& d, int dtype, cudaStream_t stream) {
+  BwdTcArgs a{};
+  a.d = d;
+  a.bf16 = dtype == PISA_BF16;
+  a.stats = d.delta;
+  a.q_slots = seq_slots(d.cu_q, d.B, d.T, d.sequences, kRows);
+  if (a.q_slots >= (int64_t(1) << 31)) return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
+  int rc = dense_tensor_map(&a.tm_q, d.q, dtype, d.B, d.T, d.Hq, d.D, d.q_sb, d.q_st, d.q_sh, kRows);
+  if (rc == PISA_OK) rc = dense_tensor_map(&a.tm_k, d.k, dtype, d.B, d.N, d.H, d.D, d.k_sb, d.k_st, d.k_sh, kRows);
+  if (rc == PISA_OK) rc = dense_tensor_map(&a.tm_v, d.v, dtype, d.B, d.N, d.H, d.Dv, d.v_sb, d.v_st, d.v_sh, kRows);
+  const int64_t st = int64_t(d.Hq) * d.Dv;
+  if (rc == PISA_OK) rc = dense_tensor_map(&a.tm_do, d.dout, dtype, d.B, d.T, d.Hq, d.Dv, d.T * st, st, d.Dv, kRows);
+  if (rc) return rc;
+  const bool narrow = d.D <= 64 && d.Dv <= 64;
+  if (dtype == PISA_BF16) return narrow ? bwd_t<__nv_bfloat16, 64>(a, stream) : bwd_t<__nv_bfloat16, 128>(a, stream);
+  return narrow ? bwd_t<__half, 64>(a, stream) : bwd_t<__half, 128>(a, stream);
+}
+
+}  // namespace pisa

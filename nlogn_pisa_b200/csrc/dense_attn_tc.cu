@@ -24,16 +24,12 @@
 // is NaN.  A row whose output holds NaN although its weights do not is
 // therefore summed again over its visible keys alone (row_again); rows past
 // the sequence's end need nothing (they are not stored).
-#include <type_traits>
-
-#include "dense_attn.cuh"
-#include "tc.cuh"
+#include "dense_tc.cuh"
 
 namespace pisa {
 
 namespace {
 
-constexpr int kRows = 128;                  // queries of a tile, keys of a tile
 constexpr int kMmaWarp = 8, kLoadWarp = 9;
 constexpr int kThreads = 320;
 constexpr float kRescale = 8.f;             // base-2 growth of a row maximum that moves it
@@ -50,39 +46,6 @@ template <int DP> struct FwdTile {
   static constexpr int STAGES = DP == 128 ? 4 : 6;      // 64 dims: also keeps a second CTA off the SM's TMEM
   static constexpr int SMEM = (2 + STAGES) * BYTES + 1024;
 };
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<uint32_t*>(&v);
-  } else {
-    __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<uint32_t*>(&v);
-  }
-}
-
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
-      :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-         "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
-         "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
-         "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
-}
-__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-__device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t x0, uint32_t x1, uint32_t x2, uint32_t x3) {
-  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" :: "r"(addr), "r"(x0), "r"(x1), "r"(x2), "r"(x3) : "memory");
-}
-__device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-  return v;
-}
 
 // Largest of 64 values by four chains of three-input maxima.
 __device__ __forceinline__ float max_of(const float (&v)[64]) {

@@ -126,7 +126,8 @@ int64_t pisa_full_attn_bwd_workspace_bytes(int64_t B, int64_t Tq, int64_t Hq, in
   if (B <= 0 || Tq <= 0 || Hq <= 0 || H <= 0 || D <= 0 || Dv <= 0 || N <= 0 || sequences < 0 || dtype < PISA_F32 ||
       dtype > PISA_F16)
     return -1;
-  return 256 + B * Tq * Hq * 4;
+  if (dtype == PISA_F32 || D > 128 || Dv > 128) return 256 + B * Tq * Hq * 4;
+  return 256 + 4 * dense_bwd_stat_floats(sequences > 0, B, Tq, Hq, sequences);
 }
 
 int pisa_full_attn_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb,
@@ -151,6 +152,7 @@ int pisa_full_attn_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, 
   a.D = int(D); a.Dv = int(Dv);
   a.o = out; a.dout = dout; a.lse_in = lse; a.dq = dq; a.dk = dk; a.dv = dv;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return fail(PISA_ERR_INVALID, "workspace must be 16-byte aligned");
   if (!workspace ||
       workspace_bytes < pisa_full_attn_bwd_workspace_bytes(B, Tq, Hq, H, D, Dv, N, cu_seqlens_q ? sequences : 0, dtype))
     return fail(PISA_ERR_INVALID, "workspace too small");
@@ -158,7 +160,7 @@ int pisa_full_attn_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, 
   if (e != cudaSuccess) return fail_cuda(e, "status clear");
   a.status = static_cast<int*>(workspace);
   a.delta = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
-  return dense_attn_bwd_simt(a, dtype, s);
+  return dense_attn_tc_eligible(a, dtype) ? dense_attn_bwd_tc(a, dtype, s) : dense_attn_bwd_simt(a, dtype, s);
 }
 
 int64_t pisa_prefix_attn_workspace_bytes(int64_t B, int64_t Tq, int64_t Hq, int64_t H, int64_t D, int64_t Dv,
@@ -187,6 +189,7 @@ int pisa_prefix_attn(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, co
       (prefix > 0 && (!rows16(prefix_k, dtype, 0, pk_st, pk_sh) || !rows16(prefix_v, dtype, 0, pv_st, pv_sh))))
     return fail(PISA_ERR_UNSUPPORTED, "q, k and v rows must be 16-byte aligned");
   const PrefixPlan plan = plan_prefix(B, Tq, Hq, H, Dv, capacity, prefix);
+  if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return fail(PISA_ERR_INVALID, "workspace must be 16-byte aligned");
   if (!workspace || workspace_bytes < plan.total) return fail(PISA_ERR_INVALID, "workspace too small");
   char* ws = static_cast<char*>(workspace);
   PrefixArgs a{};
