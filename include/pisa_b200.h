@@ -390,6 +390,8 @@ PISA_API int64_t pisa_qk_norm_rotary_bwd_workspace_bytes(int64_t B, int64_t T, i
  * undefined results but no access outside the tensors.
  * out: [B,Tq,Hq,Dv] contiguous; lse: [B,Tq,Hq] fp32 natural log-sum-exp of
  *   the scaled logits, or NULL.  A query without a visible key gets 0 / -inf.
+ * out_low: contiguous like out, or NULL: receives what rounding `out` to a
+ *   16-bit dtype lost, itself rounded, for the backward (fp32: not used).
  * scale > 0.  D, Dv multiples of 8, at most 256.
  * workspace: NULL, or pisa_full_attn_fwd_workspace_bytes(...) bytes whose
  *   first 4 receive the device status word; rows of a tile whose wait expired
@@ -399,8 +401,8 @@ PISA_API int pisa_full_attn_fwd(const void *q, int64_t q_sb, int64_t q_st, int64
                                 int64_t k_st, int64_t k_sh, const void *v, int64_t v_sb, int64_t v_st, int64_t v_sh,
                                 const void *cu_seqlens_q, const void *cu_seqlens_k, int cu_bytes, int64_t sequences,
                                 int64_t query_offset, int dtype, int64_t B, int64_t Tq, int64_t Hq, int64_t H,
-                                int64_t D, int64_t Dv, int64_t N, float scale, int causal, void *out, float *lse,
-                                void *workspace, int64_t workspace_bytes, pisa_stream_t stream);
+                                int64_t D, int64_t Dv, int64_t N, float scale, int causal, void *out, void *out_low,
+                                float *lse, void *workspace, int64_t workspace_bytes, pisa_stream_t stream);
 
 /* sequences: 0 without cumulative lengths. */
 PISA_API int64_t pisa_full_attn_fwd_workspace_bytes(int64_t B, int64_t Tq, int64_t Hq, int64_t H, int64_t D, int64_t Dv,
@@ -409,14 +411,16 @@ PISA_API int64_t pisa_full_attn_fwd_workspace_bytes(int64_t B, int64_t Tq, int64
 /*
  * Backward of pisa_full_attn_fwd: dq [B,Tq,Hq,D], dk [B,N,H,D], dv [B,N,H,Dv]
  * in dtype, contiguous, every element written (rows outside all sequences:
- * zero).  out, dout: contiguous [B,Tq,Hq,Dv]; lse as written by the forward.
+ * zero).  out, dout: contiguous [B,Tq,Hq,Dv]; lse as written by the forward,
+ * and out_low too, or NULL (the row products dout . out then carry the
+ * rounding of `out` into dq and dk).
  * Sums run in a fixed order: equal inputs give equal bits.
  * workspace: pisa_full_attn_bwd_workspace_bytes(...) bytes, status word first.
  */
 PISA_API int pisa_full_attn_bwd(const void *q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void *k, int64_t k_sb,
                                 int64_t k_st, int64_t k_sh, const void *v, int64_t v_sb, int64_t v_st, int64_t v_sh,
-                                const void *out, const void *dout, const float *lse, const void *cu_seqlens_q,
-                                const void *cu_seqlens_k, int cu_bytes, int64_t sequences, int64_t query_offset,
+                                const void *out, const void *out_low, const void *dout, const float *lse,
+                                const void *cu_seqlens_q, const void *cu_seqlens_k, int cu_bytes, int64_t sequences, int64_t query_offset,
                                 int dtype, int64_t B, int64_t Tq, int64_t Hq, int64_t H, int64_t D, int64_t Dv,
                                 int64_t N, float scale, int causal, void *dq, void *dk, void *dv, void *workspace,
                                 int64_t workspace_bytes, pisa_stream_t stream);

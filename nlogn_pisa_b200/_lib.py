@@ -65,9 +65,9 @@ SIGNATURES = {
                                      _L, _L, _L, _F, _P, _P, _P, _P, _P, _L, _P]),
     "pisa_qk_norm_rotary_bwd_workspace_bytes": (_L, [_L, _L, _L]),
     "pisa_full_attn_fwd": (_I, [_P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _P, _P, _I, _L, _L, _I, _L, _L, _L,
-                                _L, _L, _L, _L, _F, _I, _P, _P, _P, _L, _P]),
+                                _L, _L, _L, _L, _F, _I, _P, _P, _P, _P, _L, _P]),
     "pisa_full_attn_fwd_workspace_bytes": (_L, [_L, _L, _L, _L, _L, _L, _L, _L, _I]),
-    "pisa_full_attn_bwd": (_I, [_P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _P, _P, _P, _P, _P, _I, _L, _L, _I,
+    "pisa_full_attn_bwd": (_I, [_P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _P, _P, _P, _P, _P, _P, _I, _L, _L, _I,
                                 _L, _L, _L, _L, _L, _L, _L, _F, _I, _P, _P, _P, _P, _L, _P]),
     "pisa_full_attn_bwd_workspace_bytes": (_L, [_L, _L, _L, _L, _L, _L, _L, _L, _I]),
     "pisa_prefix_attn": (_I, [_P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _P, _I, _P, _L, _L, _P, _L, _L, _I, _L,

@@ -198,12 +198,26 @@ __global__ void __launch_bounds__(kThreads) dense_fwd_kernel(const __grid_consta
   }
   T* op = static_cast<T*>(a.out) + ((int64_t(t.b) * a.T + t.q_begin + q0) * a.Hq + hq) * a.Dv;
   store_rows<T, R, DP>(op, int64_t(a.Hq) * a.Dv, valid, a.Dv, ty, tx, acc, inv);
+  if (a.out_low) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+#pragma unroll
+      for (int c = 0; c < DP / 16; ++c) {
+        const float v = acc[i][c] * inv[i];
+        acc[i][c] = v - to_f32<T>(from_f32<T>(v));
+      }
+      inv[i] = 1.f;
+    }
+    T* lp = static_cast<T*>(a.out_low) + ((int64_t(t.b) * a.T + t.q_begin + q0) * a.Hq + hq) * a.Dv;
+    store_rows<T, R, DP>(lp, int64_t(a.Hq) * a.Dv, valid, a.Dv, ty, tx, acc, inv);
+  }
 }
 
-// delta = dout . out per row, one warp per row
+// delta = dout . (out + out_low) per row, one warp per row
 template <typename T>
 __global__ void __launch_bounds__(128) dense_delta_kernel(const T* __restrict__ dout, const T* __restrict__ out,
-                                                          float* __restrict__ delta, int64_t rows, int Dv) {
+                                                          const T* __restrict__ low, float* __restrict__ delta,
+                                                          int64_t rows, int Dv) {
   constexpr int VN = Vec<T>::N;
   const int64_t r = blockIdx.x * int64_t(4) + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
@@ -215,6 +229,11 @@ __global__ void __launch_bounds__(128) dense_delta_kernel(const T* __restrict__ 
     load_vec<T>(out + r * Dv + d, y);
 #pragma unroll
     for (int e = 0; e < VN; ++e) acc = fmaf(x[e], y[e], acc);
+    if (low) {
+      load_vec<T>(low + r * Dv + d, y);
+#pragma unroll
+      for (int e = 0; e < VN; ++e) acc = fmaf(x[e], y[e], acc);
+    }
   }
   acc = warp_sum(acc);
   if (lane == 0) delta[r] = acc;
@@ -396,7 +415,8 @@ int bwd_t(const DenseAttnArgs& a, cudaStream_t s) {
   const int64_t rows = int64_t(a.B) * a.T * a.Hq;
   if ((rows + 3) / 4 >= (int64_t(1) << 31)) return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
   dense_delta_kernel<T><<<unsigned((rows + 3) / 4), 128, 0, s>>>(static_cast<const T*>(a.dout),
-                                                                 static_cast<const T*>(a.o), a.delta, rows, a.Dv);
+                                                                 static_cast<const T*>(a.o), static_cast<const T*>(a.o_low),
+                                                                 a.delta, rows, a.Dv);
   PISA_CHECK_LAUNCH();
   int rc = launch(dense_dq_kernel<T, DP>, seq_slots(a.cu_q, a.B, a.T, a.sequences, L::BT) * a.Hq,
                   sizeof(float) * L::BT * (4 * L::LD + L::LP), a, s);

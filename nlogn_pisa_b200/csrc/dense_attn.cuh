@@ -27,10 +27,12 @@ struct DenseAttnArgs {
   float scale;
   int causal;
   void* out;        // [B, T, Hq, Dv]
+  void* out_low;    // same shape: the part of the output that rounding dropped, or null
   float* lse;       // [B, T, Hq] or null
   int* status;      // device status word or null
   // backward
   const void* o;    // the forward's output, contiguous
+  const void* o_low;  // its dropped part, or null
   const void* dout; // contiguous
   const float* lse_in;
   float* delta;     // workspace: [B, T, Hq] row dot products of dout and out (FMA form), row statistics (tensor-core form)

@@ -2,7 +2,8 @@
 // most 128 dims (formulas in dense_attn.cu).  Three launches:
 //
 // 1. Row statistics: -lse and -scale * delta of every query (delta = dout .
-//    out), base 2, in tiles of 128 queries of one sequence and head.  Rows past
+//    out, with the part of out that its rounding dropped: it would add half
+//    again to the rounding errors of dQ and dK), base 2, in tiles of 128 queries of one sequence and head.  Rows past
 //    a sequence's end and rows without keys get lse = +inf, so their weights
 //    are zero below.
 // 2. dK, dV: one CTA per 128 keys of a KV head, over the query tiles that see
@@ -77,6 +78,11 @@ __global__ void __launch_bounds__(256) dense_stats_kernel(const __grid_constant_
         load_vec<T>(dout + row * a.Dv + d, v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) dot = fmaf(u[e], v[e], dot);
+        if (a.o_low) {
+          load_vec<T>(static_cast<const T*>(a.o_low) + row * a.Dv + d, u);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) dot = fmaf(u[e], v[e], dot);
+        }
       }
     }
 #pragma unroll

@@ -306,53 +306,60 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
     const float inv = !ok ? NAN : l == 0.f ? 0.f : 1.f / l;
     constexpr int SEG = DP / 8;                      // 16-byte segments of a row
     const uint32_t stage = q_addr + i * L::BYTES + quarter * 32 * DP * 2;
-    bool wild = false;
-#pragma unroll
-    for (int c = 0; c < DP; c += 32) {
-      float o[32];
-      if (any && ok) {
-        tc::tmem_ld32(to + c, o);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = 0.f;
-      }
-#pragma unroll
-      for (int e = 0; e < 32; ++e) {
-        wild = wild || isnan(o[e]);
-        o[e] = l == 0.f && ok ? 0.f : o[e] * inv;
-      }
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const int seg = c / 8 + s;
-        st_shared16(stage + (lane * SEG + (seg ^ (lane & 7))) * 16, pack2<T>(o[8 * s], o[8 * s + 1]),
-                    pack2<T>(o[8 * s + 2], o[8 * s + 3]), pack2<T>(o[8 * s + 4], o[8 * s + 5]),
-                    pack2<T>(o[8 * s + 6], o[8 * s + 7]));
-      }
-    }
-    __syncwarp();
-    uint32_t again = __ballot_sync(kFull, ok && real && wild && l != 0.f && !isnan(l));
-    while (again) {
-      const int r = __ffs(again) - 1;
-      again &= again - 1;
-      float acc[DP / 32];
-      row_again<T, DP>(a, t, hq, q0 + i * kRows + quarter * 32 + r, __shfl_sync(kFull, m, r), __shfl_sync(kFull, l, r), acc);
-#pragma unroll
-      for (int e = 0; e < DP / 32; ++e) {
-        const int d = lane + 32 * e;
-        const T v = from_f32<T>(acc[e]);
-        asm volatile("st.shared.b16 [%0], %1;"
-                     :: "r"(stage + (r * SEG + ((d >> 3) ^ (r & 7))) * 16 + (d & 7) * 2),
-                        "h"(*reinterpret_cast<const uint16_t*>(&v)) : "memory");
-      }
-      __syncwarp();
-    }
     const int64_t row0 = int64_t(t.b) * a.T + t.q_begin + q0 + i * kRows + quarter * 32;
     const int rows = min(32, t.q_len - (q0 + i * kRows + quarter * 32));
-    T* out = static_cast<T*>(a.out);
-    for (int f = lane; f < rows * SEG; f += 32) {
-      const int r = f / SEG, seg = f % SEG;
-      const uint4 v = ld_shared16(stage + (r * SEG + (seg ^ (r & 7))) * 16);
-      if (seg * 8 < a.Dv) *reinterpret_cast<uint4*>(out + ((row0 + r) * a.Hq + hq) * a.Dv + seg * 8) = v;
+    // pass 0 stores the rounded output, pass 1 what the rounding dropped
+    for (int pass = 0; pass < (a.out_low ? 2 : 1); ++pass) {
+      bool wild = false;
+#pragma unroll
+      for (int c = 0; c < DP; c += 32) {
+        float o[32];
+        if (any && ok) {
+          tc::tmem_ld32(to + c, o);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          wild = wild || isnan(o[e]);
+          o[e] = l == 0.f && ok ? 0.f : o[e] * inv;
+          if (pass) o[e] -= to_f32<T>(from_f32<T>(o[e]));
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const int seg = c / 8 + s;
+          st_shared16(stage + (lane * SEG + (seg ^ (lane & 7))) * 16, pack2<T>(o[8 * s], o[8 * s + 1]),
+                      pack2<T>(o[8 * s + 2], o[8 * s + 3]), pack2<T>(o[8 * s + 4], o[8 * s + 5]),
+                      pack2<T>(o[8 * s + 6], o[8 * s + 7]));
+        }
+      }
+      __syncwarp();
+      uint32_t again = __ballot_sync(kFull, ok && real && wild && l != 0.f && !isnan(l));
+      while (again) {
+        const int r = __ffs(again) - 1;
+        again &= again - 1;
+        float acc[DP / 32];
+        row_again<T, DP>(a, t, hq, q0 + i * kRows + quarter * 32 + r, __shfl_sync(kFull, m, r), __shfl_sync(kFull, l, r),
+                         acc);
+#pragma unroll
+        for (int e = 0; e < DP / 32; ++e) {
+          const int d = lane + 32 * e;
+          T v = from_f32<T>(acc[e]);
+          if (pass) v = from_f32<T>(acc[e] - to_f32<T>(v));
+          asm volatile("st.shared.b16 [%0], %1;"
+                       :: "r"(stage + (r * SEG + ((d >> 3) ^ (r & 7))) * 16 + (d & 7) * 2),
+                          "h"(*reinterpret_cast<const uint16_t*>(&v)) : "memory");
+        }
+        __syncwarp();
+      }
+      T* out = static_cast<T*>(pass ? a.out_low : a.out);
+      for (int f = lane; f < rows * SEG; f += 32) {
+        const int r = f / SEG, seg = f % SEG;
+        const uint4 v = ld_shared16(stage + (r * SEG + (seg ^ (r & 7))) * 16);
+        if (seg * 8 < a.Dv) *reinterpret_cast<uint4*>(out + ((row0 + r) * a.Hq + hq) * a.Dv + seg * 8) = v;
+      }
+      __syncwarp();
     }
     if (a.lse && real)
       a.lse[(row0 + lane) * a.Hq + hq] = !ok ? NAN : l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;

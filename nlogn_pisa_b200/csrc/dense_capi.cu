@@ -97,8 +97,8 @@ int pisa_full_attn_fwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, 
                        int64_t k_st, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_st, int64_t v_sh,
                        const void* cu_seqlens_q, const void* cu_seqlens_k, int cu_bytes, int64_t sequences,
                        int64_t query_offset, int dtype, int64_t B, int64_t Tq, int64_t Hq, int64_t H, int64_t D,
-                       int64_t Dv, int64_t N, float scale, int causal, void* out, float* lse, void* workspace,
-                       int64_t workspace_bytes, pisa_stream_t stream) {
+                       int64_t Dv, int64_t N, float scale, int causal, void* out, void* out_low, float* lse,
+                       void* workspace, int64_t workspace_bytes, pisa_stream_t stream) {
   DenseAttnArgs a{};
   a.q = q; a.q_sb = q_sb; a.q_st = q_st; a.q_sh = q_sh;
   a.k = k; a.k_sb = k_sb; a.k_st = k_st; a.k_sh = k_sh;
@@ -111,6 +111,9 @@ int pisa_full_attn_fwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, 
   a.B = int(B); a.T = int(Tq); a.N = int(N); a.Hq = int(Hq); a.H = int(H); a.G = int(Hq / H);
   a.D = int(D); a.Dv = int(Dv);
   a.out = out; a.lse = lse;
+  a.out_low = dtype == PISA_F32 ? nullptr : out_low;
+  if (!rows16(out, dtype, 0, 0, 0) || !rows16(out_low, dtype, 0, 0, 0))
+    return fail(PISA_ERR_UNSUPPORTED, "out and out_low must be 16-byte aligned");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (workspace) {
     if (workspace_bytes < 256) return fail(PISA_ERR_INVALID, "workspace too small");
@@ -132,8 +135,8 @@ int64_t pisa_full_attn_bwd_workspace_bytes(int64_t B, int64_t Tq, int64_t Hq, in
 
 int pisa_full_attn_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb,
                        int64_t k_st, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_st, int64_t v_sh,
-                       const void* out, const void* dout, const float* lse, const void* cu_seqlens_q,
-                       const void* cu_seqlens_k, int cu_bytes, int64_t sequences, int64_t query_offset, int dtype,
+                       const void* out, const void* out_low, const void* dout, const float* lse,
+                       const void* cu_seqlens_q, const void* cu_seqlens_k, int cu_bytes, int64_t sequences, int64_t query_offset, int dtype,
                        int64_t B, int64_t Tq, int64_t Hq, int64_t H, int64_t D, int64_t Dv, int64_t N, float scale,
                        int causal, void* dq, void* dk, void* dv, void* workspace, int64_t workspace_bytes,
                        pisa_stream_t stream) {
@@ -145,12 +148,12 @@ int pisa_full_attn_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, 
   a.query_offset = query_offset; a.scale = scale; a.causal = causal ? 1 : 0;
   if (int rc = check_dense(a, dtype, B, Tq, Hq, H, D, Dv, N, sequences)) return rc;
   if (!out || !dout || !lse || !dq || !dk || !dv) return fail(PISA_ERR_INVALID, "out, dout, lse and the gradients are required");
-  if (!rows16(out, dtype, 0, 0, 0) || !rows16(dout, dtype, 0, 0, 0))
-    return fail(PISA_ERR_UNSUPPORTED, "out and dout must be 16-byte aligned");
+  if (!rows16(out, dtype, 0, 0, 0) || !rows16(dout, dtype, 0, 0, 0) || !rows16(out_low, dtype, 0, 0, 0))
+    return fail(PISA_ERR_UNSUPPORTED, "out, out_low and dout must be 16-byte aligned");
   a.sequences = int(sequences);
   a.B = int(B); a.T = int(Tq); a.N = int(N); a.Hq = int(Hq); a.H = int(H); a.G = int(Hq / H);
   a.D = int(D); a.Dv = int(Dv);
-  a.o = out; a.dout = dout; a.lse_in = lse; a.dq = dq; a.dk = dk; a.dv = dv;
+  a.o = out; a.o_low = dtype == PISA_F32 ? nullptr : out_low; a.dout = dout; a.lse_in = lse; a.dq = dq; a.dk = dk; a.dv = dv;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return fail(PISA_ERR_INVALID, "workspace must be 16-byte aligned");
   if (!workspace ||

@@ -57,11 +57,13 @@ def _packing(cu_q, cu_k):
     return _lib.ptr(cu_q), _lib.ptr(cu_k), cu_q.element_size(), cu_q.numel() - 1
 
 
-def _forward(q, k, v, cu_q, cu_k, offset, scale, causal, want_lse):
+def _forward(q, k, v, cu_q, cu_k, offset, scale, causal, want_lse, want_low=False):
     batch, tokens, q_heads, dim = q.shape
     heads, length, dim_v = k.shape[2], k.shape[1], v.shape[-1]
     out = torch.empty((batch, tokens, q_heads, dim_v), dtype=q.dtype, device=q.device)
     lse = torch.empty((batch, tokens, q_heads), dtype=torch.float32, device=q.device) if want_lse else None
+    # what rounding the output to 16 bits dropped, for the backward's row products
+    low = torch.empty_like(out) if want_low and q.dtype != torch.float32 else None
     library = _lib.lib()
     # the workspace holds only the status word: passed when it will be read
     workspace = None
@@ -73,13 +75,13 @@ def _forward(q, k, v, cu_q, cu_k, offset, scale, causal, want_lse):
         _lib.check(library.pisa_full_attn_fwd(
             _lib.ptr(q), *_strides(q), _lib.ptr(k), *_strides(k), _lib.ptr(v), *_strides(v), *_packing(cu_q, cu_k),
             offset, _lib.dtype_code(q), batch, tokens, q_heads, heads, dim, dim_v, length, scale, int(causal),
-            _lib.ptr(out), _lib.ptr(lse), _lib.ptr(workspace), 0 if workspace is None else workspace.numel(),
+            _lib.ptr(out), _lib.ptr(low), _lib.ptr(lse), _lib.ptr(workspace), 0 if workspace is None else workspace.numel(),
             _lib.stream_of(q.device)))
     _lib.check_workspace(workspace, q.device)
-    return out, lse
+    return out, lse, low
 
 
-def _backward(q, k, v, out, dout, lse, cu_q, cu_k, offset, scale, causal):
+def _backward(q, k, v, out, low, dout, lse, cu_q, cu_k, offset, scale, causal):
     batch, tokens, q_heads, dim = q.shape
     heads, length, dim_v = k.shape[2], k.shape[1], v.shape[-1]
     code = _lib.dtype_code(q)
@@ -93,7 +95,7 @@ def _backward(q, k, v, out, dout, lse, cu_q, cu_k, offset, scale, causal):
     with torch.cuda.device(q.device):
         _lib.check(library.pisa_full_attn_bwd(
             _lib.ptr(q), *_strides(q), _lib.ptr(k), *_strides(k), _lib.ptr(v), *_strides(v), _lib.ptr(out),
-            _lib.ptr(dout), _lib.ptr(lse), *_packing(cu_q, cu_k), offset, code, batch, tokens, q_heads, heads, dim,
+            _lib.ptr(low), _lib.ptr(dout), _lib.ptr(lse), *_packing(cu_q, cu_k), offset, code, batch, tokens, q_heads, heads, dim,
             dim_v, length, scale, int(causal), _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv), _lib.ptr(workspace), size,
             _lib.stream_of(q.device)))
     if _lib.status_checks():
@@ -104,8 +106,8 @@ def _backward(q, k, v, out, dout, lse, cu_q, cu_k, offset, scale, causal):
 class FullAttentionFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, offset, scale, causal):
-        out, lse = _forward(q, k, v, cu_q, cu_k, offset, scale, causal, True)
-        ctx.save_for_backward(q, k, v, out, lse, cu_q, cu_k)
+        out, lse, low = _forward(q, k, v, cu_q, cu_k, offset, scale, causal, True, True)
+        ctx.save_for_backward(q, k, v, out, low, lse, cu_q, cu_k)
         ctx.args = (offset, scale, causal)
         ctx.mark_non_differentiable(lse)
         return out, lse
@@ -113,9 +115,9 @@ class FullAttentionFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, _):
-        q, k, v, out, lse, cu_q, cu_k = ctx.saved_tensors
+        q, k, v, out, low, lse, cu_q, cu_k = ctx.saved_tensors
         dout = flat(dout)
-        dq, dk, dv = _backward(q, k, v, out, dout, lse, cu_q, cu_k, *ctx.args)
+        dq, dk, dv = _backward(q, k, v, out, low, dout, lse, cu_q, cu_k, *ctx.args)
         return dq, dk, dv, None, None, None, None, None
 
 
@@ -161,7 +163,7 @@ def full_attention(q, k, v, cu_seqlens=None, cu_seqlens_k=None, scale=None, quer
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
         out, lse = FullAttentionFunction.apply(q, k, v, cu_seqlens, cu_seqlens_k, offset, scale, bool(causal))
     else:
-        out, lse = _forward(q, k, v, cu_seqlens, cu_seqlens_k, offset, scale, causal, return_lse)
+        out, lse, _ = _forward(q, k, v, cu_seqlens, cu_seqlens_k, offset, scale, causal, return_lse)
     return (out, lse) if return_lse else out
 
 

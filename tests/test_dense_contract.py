@@ -25,7 +25,7 @@ def test_entry_checks_run_on_the_host():
     def full(B=1, T=4, Hq=4, H=2, D=64, Dv=64, N=4, scale=0.125, offset=0, dtype=_lib.BF16, align=256):
         p = align
         return lib.pisa_full_attn_fwd(p, 0, Hq * D, D, p, 0, H * D, D, p, 0, H * Dv, Dv, None, None, 0, 0, offset, dtype, B,
-                                      T, Hq, H, D, Dv, N, scale, 1, None, None, None, 0, None)
+                                      T, Hq, H, D, Dv, N, scale, 1, None, None, None, None, 0, None)
 
     for kw, word in (({"Hq": 3}, "whole number"), ({"D": 12}, "multiple of 8"), ({"Dv": 512}, "at most 256"),
                      ({"T": 0}, "nonempty"), ({"scale": 0.0}, "scale"), ({"scale": float("nan")}, "scale"),
@@ -36,7 +36,7 @@ def test_entry_checks_run_on_the_host():
         assert word in lib.pisa_last_error().decode(), (kw, lib.pisa_last_error())
     # a row of 12 bytes apart
     rc = lib.pisa_full_attn_fwd(256, 0, 250, 62, 256, 0, 128, 64, 256, 0, 128, 64, None, None, 0, 0, 0, _lib.BF16, 1, 4, 4,
-                                2, 64, 64, 4, 0.1, 1, 256, None, None, 0, None)
+                                2, 64, 64, 4, 0.1, 1, 256, None, None, None, 0, None)
     assert rc == _lib.ERR_UNSUPPORTED and "aligned" in lib.pisa_last_error().decode()
 
 
