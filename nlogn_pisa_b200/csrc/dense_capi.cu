@@ -60,13 +60,17 @@ struct PrefixPlan {
   int64_t prefix_splits, own_splits, ml_off, o_off, total;
 };
 
-// Splits of the keys: enough CTAs for two per SM, but at least 256 keys each.
-PrefixPlan plan_prefix(int64_t B, int64_t T, int64_t Hq, int64_t H, int64_t Dv, int64_t cap, int64_t P) {
+bool prefix_mma(int dtype, int64_t D, int64_t Dv) { return dtype != PISA_F32 && D <= 128 && Dv <= 128; }
+
+// Splits of the keys: enough CTAs for four (FMA form: two) per SM, but at
+// least 64 (256) keys each, the keys of one step of a CTA's four warps.
+PrefixPlan plan_prefix(int64_t B, int64_t T, int64_t Hq, int64_t H, int64_t D, int64_t Dv, int64_t cap, int64_t P, int dtype) {
   PrefixPlan p{};
-  const int64_t want = 2 * sm_count(), G = Hq / H;
+  const bool mma = prefix_mma(dtype, D, Dv);
+  const int64_t want = (mma ? 4 : 2) * sm_count(), least = mma ? 64 : 256, G = Hq / H;
   auto splits = [&](int64_t keys, int64_t rows, int64_t groups) {
     const int64_t items = groups * ((rows + 63) / 64);
-    return std::max<int64_t>(1, std::min((want + items - 1) / items, (keys + 255) / 256));
+    return std::max<int64_t>(1, std::min((want + items - 1) / items, (keys + least - 1) / least));
   };
   p.own_splits = splits(cap, T * G, B * H);
   p.prefix_splits = P > 0 ? splits(P, B * T * G, H) : 0;
@@ -171,7 +175,7 @@ int64_t pisa_prefix_attn_workspace_bytes(int64_t B, int64_t Tq, int64_t Hq, int6
   if (B <= 0 || Tq <= 0 || Hq <= 0 || H <= 0 || Hq % H || D <= 0 || Dv <= 0 || capacity <= 0 || prefix < 0 ||
       dtype < PISA_F32 || dtype > PISA_F16)
     return -1;
-  return plan_prefix(B, Tq, Hq, H, Dv, capacity, prefix).total;
+  return plan_prefix(B, Tq, Hq, H, D, Dv, capacity, prefix, dtype).total;
 }
 
 int pisa_prefix_attn(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb, int64_t k_st,
@@ -191,7 +195,7 @@ int pisa_prefix_attn(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, co
   if (!rows16(q, dtype, q_sb, q_st, q_sh) || !rows16(k, dtype, k_sb, k_st, k_sh) || !rows16(v, dtype, v_sb, v_st, v_sh) ||
       (prefix > 0 && (!rows16(prefix_k, dtype, 0, pk_st, pk_sh) || !rows16(prefix_v, dtype, 0, pv_st, pv_sh))))
     return fail(PISA_ERR_UNSUPPORTED, "q, k and v rows must be 16-byte aligned");
-  const PrefixPlan plan = plan_prefix(B, Tq, Hq, H, Dv, capacity, prefix);
+  const PrefixPlan plan = plan_prefix(B, Tq, Hq, H, D, Dv, capacity, prefix, dtype);
   if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return fail(PISA_ERR_INVALID, "workspace must be 16-byte aligned");
   if (!workspace || workspace_bytes < plan.total) return fail(PISA_ERR_INVALID, "workspace too small");
   char* ws = static_cast<char*>(workspace);
@@ -209,7 +213,7 @@ int pisa_prefix_attn(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, co
   a.part_ml = reinterpret_cast<float2*>(ws + plan.ml_off);
   a.part_o = reinterpret_cast<float*>(ws + plan.o_off);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (int rc = prefix_attn_simt(a, dtype, s)) return rc;
+  if (int rc = prefix_mma(dtype, D, Dv) ? prefix_attn_mma(a, dtype, s) : prefix_attn_simt(a, dtype, s)) return rc;
   return a.prefix_splits + a.own_splits > 1 ? prefix_combine(a, dtype, s) : PISA_OK;
 }
 

@@ -179,31 +179,43 @@ __global__ void __launch_bounds__(128) prefix_combine_kernel(const __grid_consta
     if (x.y != 0.f) top = fmaxf(top, x.x);
   }
   top = warp_max(top);
+  // slots without weight are left out, whatever their partial holds
   float total = 0.f;
-  for (int s = lane; s < slots; s += 32) {
-    const float2 x = ml[s];
-    if (x.y != 0.f) total += x.y * exp2f(x.x - top);
+  float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+  const float* po = a.part_o + row * slots * a.Dv;
+  for (int s0 = 0; s0 < slots; s0 += 32) {
+    const float2 x = s0 + lane < slots ? ml[s0 + lane] : make_float2(0.f, 0.f);
+    const float weight = x.y == 0.f ? 0.f : exp2f(x.x - top);   // of slot s0 + lane
+    total = fmaf(weight, x.y, total);
+    const uint32_t used = __ballot_sync(kFull, x.y != 0.f);
+#pragma unroll 8
+    for (int i = 0; i < min(32, slots - s0); ++i) {
+      const float w = __shfl_sync(kFull, weight, i);
+      if (!(used >> i & 1)) continue;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int d = lane * 4 + 128 * c;
+        if (d >= a.Dv) continue;
+        const float4 o = __ldcs(reinterpret_cast<const float4*>(po + int64_t(s0 + i) * a.Dv + d));
+        acc[c].x = fmaf(w, o.x, acc[c].x);
+        acc[c].y = fmaf(w, o.y, acc[c].y);
+        acc[c].z = fmaf(w, o.z, acc[c].z);
+        acc[c].w = fmaf(w, o.w, acc[c].w);
+      }
+    }
   }
   total = warp_sum(total);
   if (a.lse && lane == 0) a.lse[row] = total == 0.f ? -INFINITY : (top + log2f(total)) * kLn2;
   const float inv = total == 0.f ? 0.f : 1.f / total;
-  for (int d = lane * 4; d < a.Dv; d += 128) {
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < slots; ++s) {
-      const float2 x = ml[s];
-      if (x.y == 0.f) continue;
-      const float w = exp2f(x.x - top);
-      const float4 o = *reinterpret_cast<const float4*>(a.part_o + (row * slots + s) * a.Dv + d);
-      acc.x = fmaf(w, o.x, acc.x);
-      acc.y = fmaf(w, o.y, acc.y);
-      acc.z = fmaf(w, o.z, acc.z);
-      acc.w = fmaf(w, o.w, acc.w);
-    }
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int d = lane * 4 + 128 * c;
+    if (d >= a.Dv) continue;
     T* out = static_cast<T*>(a.out) + row * a.Dv + d;
-    out[0] = from_f32<T>(acc.x * inv);
-    out[1] = from_f32<T>(acc.y * inv);
-    out[2] = from_f32<T>(acc.z * inv);
-    out[3] = from_f32<T>(acc.w * inv);
+    out[0] = from_f32<T>(acc[c].x * inv);
+    out[1] = from_f32<T>(acc[c].y * inv);
+    out[2] = from_f32<T>(acc[c].z * inv);
+    out[3] = from_f32<T>(acc[c].w * inv);
   }
 }
 

@@ -45,6 +45,8 @@ __device__ __forceinline__ void split_range(int keys, int i, int n, int unit, in
 }
 
 int prefix_attn_simt(const PrefixArgs& a, int dtype, cudaStream_t stream);
+// 16-bit tensors of at most 128 dims
+int prefix_attn_mma(const PrefixArgs& a, int dtype, cudaStream_t stream);
 int prefix_combine(const PrefixArgs& a, int dtype, cudaStream_t stream);
 
 }  // namespace pisa
