@@ -431,7 +431,8 @@ PISA_API int64_t pisa_full_attn_bwd_workspace_bytes(int64_t B, int64_t Tq, int64
 /*
  * Decode attention of a step's Tq newest tokens of B sequences over a prefix
  * that all of them share and each one's own cache, one softmax over both.
- * q: [B,Tq,Hq,D]; k, v: own caches [B,capacity,H,D|Dv] (element strides) of
+ * q: [B,Tq,Hq,D] (element strides; q_sb = Tq * q_st when both B and Tq pass
+ * 1); k, v: own caches [B,capacity,H,D|Dv] (element strides) of
  * which the first lengths[b] keys are valid, this step's Tq included (device
  * integers of length_bytes 4 or 8, clamped to [0, capacity]); prefix_k,
  * prefix_v: [prefix,H,D|Dv] (element strides), or NULL with prefix 0.  Token t

@@ -32,7 +32,6 @@ namespace {
 
 constexpr int kMmaWarp = 8, kLoadWarp = 9;
 constexpr int kThreads = 320;
-constexpr float kRescale = 8.f;             // base-2 growth of a row maximum that moves it
 
 struct FwdTcArgs {
   CUtensorMap tm_q, tm_k, tm_v;             // boxes of 64 dims x 128 rows of one head
@@ -46,19 +45,6 @@ template <int DP> struct FwdTile {
   static constexpr int STAGES = DP == 128 ? 4 : 6;      // 64 dims: also keeps a second CTA off the SM's TMEM
   static constexpr int SMEM = (2 + STAGES) * BYTES + 1024;
 };
-
-// Largest of 64 values by four chains of three-input maxima.
-__device__ __forceinline__ float max_of(const float (&v)[64]) {
-  float m[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) m[i] = v[i];
-#pragma unroll
-  for (int i = 4; i < 60; i += 8) {
-#pragma unroll
-    for (int c = 0; c < 4; ++c) m[c] = tc::max3f(m[c], v[i + 2 * c], v[i + 2 * c + 1]);
-  }
-  return fmaxf(tc::max3f(m[0], v[60], v[61]), fmaxf(tc::max3f(m[1], v[62], v[63]), fmaxf(m[2], m[3])));
-}
 
 // Output row of query `i` summed over its visible keys alone, by one warp,
 // with the row's maximum m and weight sum l (base 2): acc[e] of column
@@ -235,63 +221,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
     for (int j = 0; j < tiles[i]; ++j) {
       if (!tc::mbar_wait(&s_full[i], j & 1)) { s_fail = 1; ok = false; break; }
       tc::fence_after_sync();
-      uint32_t s0[64], s1[64];
-      tc::tmem_ld64_nowait(ts, s0);
-      tc::tmem_ld64_nowait(ts + 64, s1);
-      tc::tmem_wait_ld2(s0, s1);
-      float x0[64], x1[64];
-#pragma unroll
-      for (int c = 0; c < 64; ++c) {
-        x0[c] = __uint_as_float(s0[c]);
-        x1[c] = __uint_as_float(s1[c]);
-      }
-      if (j >= full) {
-        const int lim = last - j * kRows;
-#pragma unroll
-        for (int c = 0; c < 64; ++c) {
-          if (c > lim) x0[c] = -INFINITY;
-          if (c + 64 > lim) x1[c] = -INFINITY;
-        }
-      }
-      const float top = fmaxf(max_of(x0), max_of(x1)) * sl;
-      if (j == 0) {
-        m = top;
-      } else if (__any_sync(kFull, top > m + kRescale)) {
-        const float to_m = fmaxf(m, top);
-        const float alpha = to_m == -INFINITY ? 1.f : tc::ex2f(m - to_m);
-        m = to_m;
-        l *= alpha;
-#pragma unroll
-        for (int c = 0; c < DP; c += 16) {
-          float o[16];
-          uint32_t r[16];
-          tc::tmem_ld16(to + c, o);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(o[e] * alpha);
-          tc::tmem_st16(to + c, r);
-        }
-      }
-      const float ref = m == -INFINITY ? 0.f : m;
-      const float2 k2 = make_float2(sl, sl), c2 = make_float2(-ref, -ref);
-      uint32_t w[32];
-      float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int c = 0; c < 64; c += 2) {
-        float2 p = tc::fma2(make_float2(x0[c], x0[c + 1]), k2, c2);
-        p = make_float2(tc::ex2f(p.x), tc::ex2f(p.y));
-        sum0 = tc::add2(sum0, p);
-        w[c / 2] = pack2<T>(p.x, p.y);
-      }
-      tmem_st32(ts, w);
-#pragma unroll
-      for (int c = 0; c < 64; c += 2) {
-        float2 p = tc::fma2(make_float2(x1[c], x1[c + 1]), k2, c2);
-        p = make_float2(tc::ex2f(p.x), tc::ex2f(p.y));
-        sum1 = tc::add2(sum1, p);
-        w[c / 2] = pack2<T>(p.x, p.y);
-      }
-      tmem_st32(ts + 32, w);
-      l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
+      softmax_tile<T, DP>(ts, to, sl, j == 0, j >= full ? last - j * kRows : kRows, m, l);
       tmem_wait_st();
       tc::fence_before_sync();
       __syncwarp();

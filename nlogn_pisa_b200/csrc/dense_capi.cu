@@ -57,24 +57,43 @@ int check_dense(const DenseAttnArgs& a, int dtype, int64_t B, int64_t Tq, int64_
 }
 
 struct PrefixPlan {
-  int64_t prefix_splits, own_splits, ml_off, o_off, total;
+  int64_t prefix_splits, own_splits, prefix_chunk, own_chunk, ml_off, o_off, total;
+  bool tiles;   // the prefix runs in 128-row tiles
 };
 
 bool prefix_mma(int dtype, int64_t D, int64_t Dv) { return dtype != PISA_F32 && D <= 128 && Dv <= 128; }
 
-// Splits of the keys: enough CTAs for four (FMA form: two) per SM, but at
-// least 64 (256) keys each, the keys of one step of a CTA's four warps.
+// Ranges of keys.  FMA form: two CTAs per SM, at least 256 keys each.  16-bit
+// forms: the prefix's tiles in one wave of CTAs; the streaming kernel in one
+// wave at least (of 64 keys or more), and ranges of about 512 keys where that
+// makes no more than eight per SM: sequences of different lengths then fill the
+// CTAs evenly (64 sequences of 1 to 2048 keys, 8 KV heads of 128: 55 us with
+// ranges of 256, 49 with 512, 51 with 1024 or 2048).
 PrefixPlan plan_prefix(int64_t B, int64_t T, int64_t Hq, int64_t H, int64_t D, int64_t Dv, int64_t cap, int64_t P, int dtype) {
   PrefixPlan p{};
   const bool mma = prefix_mma(dtype, D, Dv);
-  const int64_t want = (mma ? 4 : 2) * sm_count(), least = mma ? 64 : 256, G = Hq / H;
-  auto splits = [&](int64_t keys, int64_t rows, int64_t groups) {
-    const int64_t items = groups * ((rows + 63) / 64);
-    return std::max<int64_t>(1, std::min((want + items - 1) / items, (keys + least - 1) / least));
+  const int64_t sms = sm_count(), G = Hq / H, rows = B * T * Hq;
+  auto ranges = [](int64_t keys, int64_t count, int64_t least, int64_t* chunk) {
+    *chunk = std::max<int64_t>(1, ((keys + count - 1) / count + least - 1) / least) * least;
+    return std::max<int64_t>(1, (keys + *chunk - 1) / *chunk);
   };
-  p.own_splits = splits(cap, T * G, B * H);
-  p.prefix_splits = P > 0 ? splits(P, B * T * G, H) : 0;
-  const int64_t slots = p.own_splits + p.prefix_splits, rows = B * T * Hq;
+  if (mma) {
+    auto stream = [&](int64_t keys, int64_t items, int64_t* chunk) {
+      const int64_t most = std::min((keys + 511) / 512, (8 * sms + items - 1) / items);
+      return ranges(keys, std::max((sms + items - 1) / items, most), 64, chunk);
+    };
+    p.own_splits = stream(cap, B * H * ((T * G + 15) / 16), &p.own_chunk);
+    // more than 16 query rows per KV head: tiles of 128 rows, else the stream
+    p.tiles = P > 0 && B * T * G > 16 && G <= 128;
+    const int64_t tokens = p.tiles ? 128 / G : 1, tiles = (B * T + tokens - 1) / tokens;
+    if (p.tiles) p.prefix_splits = ranges(P, std::max<int64_t>(1, sms / (H * ((tiles + 1) / 2))), 128, &p.prefix_chunk);
+    else if (P > 0) p.prefix_splits = stream(P, H * ((B * T * G + 15) / 16), &p.prefix_chunk);
+  } else {
+    auto count = [&](int64_t items) { return (2 * sms + items - 1) / items; };
+    p.own_splits = ranges(cap, count(B * H * ((T * G + 63) / 64)), 256, &p.own_chunk);
+    p.prefix_splits = P > 0 ? ranges(P, count(H * ((B * T * G + 63) / 64)), 256, &p.prefix_chunk) : 0;
+  }
+  const int64_t slots = p.own_splits + p.prefix_splits;
   p.ml_off = 256;
   p.o_off = p.ml_off + (slots > 1 ? round256(rows * slots * 8) : 0);
   p.total = p.o_off + (slots > 1 ? rows * slots * Dv * 4 : 0);
@@ -190,13 +209,15 @@ int pisa_prefix_attn(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, co
   if (prefix > 0 && (!prefix_k || !prefix_v)) return fail(PISA_ERR_INVALID, "prefix keys and values are required");
   if (length_bytes != 4 && length_bytes != 8) return fail(PISA_ERR_INVALID, "lengths must be int32 or int64");
   constexpr int64_t most = (int64_t(1) << 31) - 4097;
-  if (capacity > most || prefix > most || B * H > 65535 || B * Tq * (Hq / H) > 65535 * 16 || B * Tq * Hq > most)
+  if (capacity > most || prefix > most || B > 65535 || Hq > 65535 || B * Tq * (Hq / H) > 65535 * 16 || B * Tq * Hq > most)
     return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
+  if (B > 1 && Tq > 1 && q_sb != Tq * q_st)
+    return fail(PISA_ERR_UNSUPPORTED, "the tokens of q must be a single stride apart over batch and tokens");
   if (!rows16(q, dtype, q_sb, q_st, q_sh) || !rows16(k, dtype, k_sb, k_st, k_sh) || !rows16(v, dtype, v_sb, v_st, v_sh) ||
       (prefix > 0 && (!rows16(prefix_k, dtype, 0, pk_st, pk_sh) || !rows16(prefix_v, dtype, 0, pv_st, pv_sh))))
     return fail(PISA_ERR_UNSUPPORTED, "q, k and v rows must be 16-byte aligned");
   const PrefixPlan plan = plan_prefix(B, Tq, Hq, H, D, Dv, capacity, prefix, dtype);
-  if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return fail(PISA_ERR_INVALID, "workspace must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(workspace) & 31u) != 0) return fail(PISA_ERR_INVALID, "workspace must be 32-byte aligned");
   if (!workspace || workspace_bytes < plan.total) return fail(PISA_ERR_INVALID, "workspace too small");
   char* ws = static_cast<char*>(workspace);
   PrefixArgs a{};
@@ -210,10 +231,17 @@ int pisa_prefix_attn(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, co
   a.cap = int(capacity); a.P = int(prefix);
   a.scale = scale; a.out = out; a.lse = lse;
   a.prefix_splits = int(plan.prefix_splits); a.own_splits = int(plan.own_splits);
+  a.prefix_chunk = int(plan.prefix_chunk); a.own_chunk = int(plan.own_chunk);
   a.part_ml = reinterpret_cast<float2*>(ws + plan.ml_off);
   a.part_o = reinterpret_cast<float*>(ws + plan.o_off);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (int rc = prefix_mma(dtype, D, Dv) ? prefix_attn_mma(a, dtype, s) : prefix_attn_simt(a, dtype, s)) return rc;
+  if (prefix_mma(dtype, D, Dv)) {
+    if (plan.tiles)
+      if (int rc = prefix_attn_tc(a, dtype, s)) return rc;
+    if (int rc = prefix_attn_mma(a, dtype, prefix > 0 && !plan.tiles, sm_count(), s)) return rc;
+  } else if (int rc = prefix_attn_simt(a, dtype, s)) {
+    return rc;
+  }
   return a.prefix_splits + a.own_splits > 1 ? prefix_combine(a, dtype, s) : PISA_OK;
 }
 

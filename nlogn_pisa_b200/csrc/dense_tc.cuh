@@ -102,4 +102,84 @@ __device__ __forceinline__ void store_lanes(uint32_t taddr, bool empty, float mu
   }
 }
 
+// Largest of 64 values by four chains of three-input maxima.
+__device__ __forceinline__ float max_of(const float (&v)[64]) {
+  float m[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m[i] = v[i];
+#pragma unroll
+  for (int i = 4; i < 60; i += 8) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) m[c] = tc::max3f(m[c], v[i + 2 * c], v[i + 2 * c + 1]);
+  }
+  return fmaxf(tc::max3f(m[0], v[60], v[61]), fmaxf(tc::max3f(m[1], v[62], v[63]), fmaxf(m[2], m[3])));
+}
+
+constexpr float kRescale = 8.f;   // base-2 growth of a row maximum that moves it
+
+// One tile of 128 scores of this thread's row (TMEM columns ts ..): updates the
+// row's maximum m and weight sum l (base-2 logits), rescales O (DP columns at
+// `to`) when the maximum moves, and leaves P, rounded to T, in the first 64
+// columns of the scores' place.  Keys past `lim` are hidden.  The caller waits
+// for the stores (tmem_wait_st) and hands P on.
+template <typename T, int DP>
+__device__ __forceinline__ void softmax_tile(uint32_t ts, uint32_t to, float sl, bool first, int lim, float& m, float& l) {
+  uint32_t s0[64], s1[64];
+  tc::tmem_ld64_nowait(ts, s0);
+  tc::tmem_ld64_nowait(ts + 64, s1);
+  tc::tmem_wait_ld2(s0, s1);
+  float x0[64], x1[64];
+#pragma unroll
+  for (int c = 0; c < 64; ++c) {
+    x0[c] = __uint_as_float(s0[c]);
+    x1[c] = __uint_as_float(s1[c]);
+  }
+  if (lim < kRows - 1) {
+#pragma unroll
+    for (int c = 0; c < 64; ++c) {
+      if (c > lim) x0[c] = -INFINITY;
+      if (c + 64 > lim) x1[c] = -INFINITY;
+    }
+  }
+  const float top = fmaxf(max_of(x0), max_of(x1)) * sl;
+  if (first) {
+    m = top;
+  } else if (__any_sync(kFull, top > m + kRescale)) {
+    const float next = fmaxf(m, top);
+    const float alpha = next == -INFINITY ? 1.f : tc::ex2f(m - next);
+    m = next;
+    l *= alpha;
+#pragma unroll
+    for (int c = 0; c < DP; c += 16) {
+      float o[16];
+      uint32_t r[16];
+      tc::tmem_ld16(to + c, o);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(o[e] * alpha);
+      tc::tmem_st16(to + c, r);
+    }
+  }
+  const float ref = m == -INFINITY ? 0.f : m;
+  const float2 k2 = make_float2(sl, sl), c2 = make_float2(-ref, -ref);
+  uint32_t w[32];
+  float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int c = 0; c < 64; c += 2) {
+    float2 p = tc::fma2(make_float2(x0[c], x0[c + 1]), k2, c2);
+    p = make_float2(tc::ex2f(p.x), tc::ex2f(p.y));
+    sum0 = tc::add2(sum0, p);
+    w[c / 2] = pack2<T>(p.x, p.y);
+  }
+  tmem_st32(ts, w);
+#pragma unroll
+  for (int c = 0; c < 64; c += 2) {
+    float2 p = tc::fma2(make_float2(x1[c], x1[c + 1]), k2, c2);
+    p = make_float2(tc::ex2f(p.x), tc::ex2f(p.y));
+    sum1 = tc::add2(sum1, p);
+    w[c / 2] = pack2<T>(p.x, p.y);
+  }
+  tmem_st32(ts + 32, w);
+  l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
+}
+
 }  // namespace pisa

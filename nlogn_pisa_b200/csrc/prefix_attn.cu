@@ -18,6 +18,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kKeys = 64;   // keys of one staged tile
+constexpr int kCombineWarps = 8;
 
 template <typename T, int DP, int LD>
 __device__ __forceinline__ void stage_row(float* dst, const T* src, bool real, int c, int D) {
@@ -40,11 +41,11 @@ __global__ void __launch_bounds__(kThreads) prefix_simt_kernel(const __grid_cons
   float* qs = smem;
   float* ks = qs + BR * LD;   // keys, then the values of the same tile
   float* ps = ks + kKeys * LD;
-  const int split = blockIdx.x, h = blockIdx.z % a.H, b = prefix ? 0 : blockIdx.z / a.H;
+  const int split = blockIdx.x / a.H, h = blockIdx.x % a.H, b = blockIdx.z;
   const int rows = (prefix ? a.B * a.T : a.T) * a.G, r0 = blockIdx.y * BR;
   const int length = prefix ? a.P : own_length(a, b);
   int begin, end;
-  split_range(length, split, prefix ? a.prefix_splits : a.own_splits, kKeys, begin, end);
+  split_range(length, split, prefix ? a.prefix_chunk : a.own_chunk, begin, end);
   const T* kp = prefix ? static_cast<const T*>(a.pk) + h * a.pk_sh : static_cast<const T*>(a.k) + b * a.k_sb + h * a.k_sh;
   const T* vp = prefix ? static_cast<const T*>(a.pv) + h * a.pv_sh : static_cast<const T*>(a.v) + b * a.v_sb + h * a.v_sh;
   const int64_t k_st = prefix ? a.pk_st : a.k_st, v_st = prefix ? a.pv_st : a.v_st;
@@ -166,15 +167,24 @@ __global__ void __launch_bounds__(kThreads) prefix_simt_kernel(const __grid_cons
   }
 }
 
-// Joins the slots of a row; one warp per row, 4 columns per lane and step.
+// Joins the slots of a row that were written: all prefix splits, and the own
+// splits that hold keys (one at least).  One CTA per row; its warps take the
+// slots in turn, a lane 4 columns (and 4 more past 128), and join through
+// shared memory: with a few hundred rows the work is a few loads deep, not a
+// chain of them.
 template <typename T>
-__global__ void __launch_bounds__(128) prefix_combine_kernel(const __grid_constant__ PrefixArgs a) {
-  const int64_t rows = int64_t(a.B) * a.T * a.Hq, row = blockIdx.x * int64_t(4) + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31, slots = a.prefix_splits + a.own_splits;
-  if (row >= rows) return;
+__global__ void prefix_combine_kernel(const __grid_constant__ PrefixArgs a) {
+  __shared__ float4 part[kCombineWarps][2][32];
+  const int64_t row = blockIdx.x;
+  const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+  const int slots = a.prefix_splits + a.own_splits;
+  const int ranges = (own_length(a, int(row / (int64_t(a.T) * a.Hq))) + a.own_chunk - 1) / a.own_chunk;
+  const int used = a.prefix_splits + max(1, ranges);
   const float2* ml = a.part_ml + row * slots;
+  const float* po = a.part_o + row * slots * a.Dv + lane * 4;
+  cudaGridDependencySynchronize();   // the partials are complete from here on
   float top = -INFINITY;
-  for (int s = lane; s < slots; s += 32) {
+  for (int s = lane; s < used; s += 32) {
     const float2 x = ml[s];
     if (x.y != 0.f) top = fmaxf(top, x.x);
   }
@@ -182,21 +192,19 @@ __global__ void __launch_bounds__(128) prefix_combine_kernel(const __grid_consta
   // slots without weight are left out, whatever their partial holds
   float total = 0.f;
   float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
-  const float* po = a.part_o + row * slots * a.Dv;
-  for (int s0 = 0; s0 < slots; s0 += 32) {
-    const float2 x = s0 + lane < slots ? ml[s0 + lane] : make_float2(0.f, 0.f);
+  for (int s0 = 0; s0 < used; s0 += 32) {
+    const float2 x = s0 + lane < used ? ml[s0 + lane] : make_float2(0.f, 0.f);
     const float weight = x.y == 0.f ? 0.f : exp2f(x.x - top);   // of slot s0 + lane
     total = fmaf(weight, x.y, total);
-    const uint32_t used = __ballot_sync(kFull, x.y != 0.f);
-#pragma unroll 8
-    for (int i = 0; i < min(32, slots - s0); ++i) {
+    const uint32_t heavy = __ballot_sync(kFull, x.y != 0.f);
+#pragma unroll 4
+    for (int i = warp; i < min(32, used - s0); i += warps) {
       const float w = __shfl_sync(kFull, weight, i);
-      if (!(used >> i & 1)) continue;
+      if (!(heavy >> i & 1)) continue;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const int d = lane * 4 + 128 * c;
-        if (d >= a.Dv) continue;
-        const float4 o = __ldcs(reinterpret_cast<const float4*>(po + int64_t(s0 + i) * a.Dv + d));
+        if (lane * 4 + 128 * c >= a.Dv) continue;
+        const float4 o = __ldcs(reinterpret_cast<const float4*>(po + int64_t(s0 + i) * a.Dv + 128 * c));
         acc[c].x = fmaf(w, o.x, acc[c].x);
         acc[c].y = fmaf(w, o.y, acc[c].y);
         acc[c].z = fmaf(w, o.z, acc[c].z);
@@ -205,17 +213,15 @@ __global__ void __launch_bounds__(128) prefix_combine_kernel(const __grid_consta
     }
   }
   total = warp_sum(total);
-  if (a.lse && lane == 0) a.lse[row] = total == 0.f ? -INFINITY : (top + log2f(total)) * kLn2;
+  if (a.lse && threadIdx.x == 0) a.lse[row] = total == 0.f ? -INFINITY : (top + log2f(total)) * kLn2;
+  part[warp][0][lane] = acc[0];
+  part[warp][1][lane] = acc[1];
+  __syncthreads();
   const float inv = total == 0.f ? 0.f : 1.f / total;
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    const int d = lane * 4 + 128 * c;
-    if (d >= a.Dv) continue;
-    T* out = static_cast<T*>(a.out) + row * a.Dv + d;
-    out[0] = from_f32<T>(acc[c].x * inv);
-    out[1] = from_f32<T>(acc[c].y * inv);
-    out[2] = from_f32<T>(acc[c].z * inv);
-    out[3] = from_f32<T>(acc[c].w * inv);
+  for (int d = threadIdx.x; d < a.Dv; d += blockDim.x) {
+    float v = 0.f;
+    for (int w = 0; w < warps; ++w) v += reinterpret_cast<const float*>(part[w])[d];
+    static_cast<T*>(a.out)[row * a.Dv + d] = from_f32<T>(v * inv);
   }
 }
 
@@ -226,8 +232,9 @@ int launch(const PrefixArgs& a, bool prefix, cudaStream_t s) {
   cudaError_t e = cudaFuncSetAttribute(prefix_simt_kernel<T, DP, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
   if (e != cudaSuccess) return fail_cuda(e, "prefix attention smem attribute");
   const int64_t rows = int64_t(prefix ? a.B : 1) * a.T * a.G;
-  const dim3 grid(unsigned(prefix ? a.prefix_splits : a.own_splits), unsigned((rows + BR - 1) / BR),
-                  unsigned((prefix ? 1 : a.B) * a.H));
+  // heads of a key range side by side: their rows share DRAM pages
+  const dim3 grid(unsigned((prefix ? a.prefix_splits : a.own_splits) * a.H), unsigned((rows + BR - 1) / BR),
+                  unsigned(prefix ? 1 : a.B));
   prefix_simt_kernel<T, DP, R><<<grid, kThreads, smem, s>>>(a, prefix);
   PISA_CHECK_LAUNCH();
   return PISA_OK;
@@ -253,10 +260,9 @@ int by_dim(const PrefixArgs& a, cudaStream_t s) {
 
 template <typename T>
 int combine(const PrefixArgs& a, cudaStream_t s) {
-  const int64_t rows = int64_t(a.B) * a.T * a.Hq;
-  prefix_combine_kernel<T><<<unsigned((rows + 3) / 4), 128, 0, s>>>(a);
-  PISA_CHECK_LAUNCH();
-  return PISA_OK;
+  const int slots = a.prefix_splits + a.own_splits;
+  const int warps = slots > 32 ? kCombineWarps : kCombineWarps / 2;
+  return launch_after(prefix_combine_kernel<T>, dim3(unsigned(int64_t(a.B) * a.T * a.Hq)), warps * 32, 0, a, s);
 }
 
 }  // namespace

@@ -1,24 +1,31 @@
-// Shared-prefix decode attention on mma.sync, for 16-bit tensors with heads of
-// at most 128 dims (formulas and partial results in prefix_attn.cu).
+// Shared-prefix decode attention for 16-bit tensors with heads of at most 128
+// dims and up to 16 query rows per KV head and pass (formulas and partial
+// results in prefix_attn.cu).
 //
-// A decode step reads every key and value once for a handful of query rows,
-// so it is bound by HBM; the kernel's task is to keep loads in flight.  A warp
-// takes 16 query rows (8 are enough up to G * T = 8) and 16 keys per step and
-// loads keys and values straight into the registers that the MMAs read:
-//  - a contraction may visit the dims in any order, so the B operand of
-//    S = Q K^T takes the 8 consecutive dims (16 bytes) that a thread loads of
-//    a key row as its operands of two steps; Q is loaded the same way;
-//  - the columns of O may stand in any order, so the B operand of O += P V
-//    takes 8 consecutive dims of four key rows, whose halves two byte
-//    permutations pair up.
-// There is no shared-memory staging and no barrier in the loop; the next
-// step's keys are requested when this step's scores are done, its values when
-// this step's products are.  Each warp keeps its own running maximum and sum;
-// the warps that share query rows join at the end.
+// A decode step reads every key and value once for a handful of query rows:
+// it is bound by HBM, and the kernel's task is an unbroken stream of loads.
+// One persistent CTA per SM walks work items (a range of keys of one KV head
+// for 8 or 16 query rows).  One warp issues TMA loads of 64-key tiles, keys
+// and values, into a ring that runs on across items (128 KB);
+// eight warps compute, four per tile, 16 keys each, on mma.sync: the query
+// rows are too few for a tensor-core tile of 128.
+//   S^T = K Q^T     keys along the MMA's 16 rows, query rows along its 8 columns
+//   O^T += V^T P^T  dims along the 16 rows; V^T by transposing ldmatrix
+// P^T leaves the first MMA key by thread group and enters the second query row
+// by thread group: an 8 x 8 transpose of the packed weights in registers.  A
+// warp's running maximum moves only when a score passes it by 2^8 (weights up
+// to 256 are as exact in 16-bit floating point), so the usual tile needs one
+// vote instead of a maximum over the threads.  The warps join through shared
+// memory at the end of an item.
+//
+// Items: the prefix's key ranges, then the own caches' ranges that hold keys,
+// counted on the device from the lengths (no CTA draws empty ranges).  Heads of
+// a range are neighbours, so their rows meet in the same DRAM pages.
 //
 // Hidden keys: scores are selected away, and value rows past the last key
-// that every row sees are zeroed in registers; the up to T - 1 newer keys
-// that only later tokens see are added row by row.
+// that every row sees are masked out of the operand registers (zero times an
+// infinite or NaN value is NaN); the up to T - 1 newer keys that only later
+// tokens see are added row by row.
 #include "dense_tc.cuh"
 #include "prefix_attn.cuh"
 
@@ -26,283 +33,428 @@ namespace pisa {
 
 namespace {
 
-constexpr int kWarps = 4, kThreads = kWarps * 32;
-constexpr int kStep = 16;                 // keys of a warp's step
+constexpr int kTile = 64;                        // keys of a ring stage
+constexpr int kComputeWarps = 8, kLoadWarp = 8, kThreads = (kComputeWarps + 1) * 32;
+constexpr int kTable = 1024;                     // entries of the table of own ranges
+
+struct StreamArgs {
+  CUtensorMap tm_k, tm_v, tm_pk, tm_pv;          // boxes of 64 dims x 64 keys of one head
+  PrefixArgs p;
+  int prefix_items;                              // key ranges x row blocks x heads of the prefix done here
+  int prefix_blocks, own_blocks;                 // row blocks of a KV head
+  int per_entry;                                 // sequences of a table entry
+  bool after_tiles;                              // follows the prefix's tile kernel, which it shares nothing with
+};
+
+template <int DP, int NR> struct Stream {
+  static constexpr int CH = DP / 64, BR = 8 * NR;
+  static constexpr int OPERAND = kTile * DP * 2, STAGE = 2 * OPERAND;
+  static constexpr int JOIN = kComputeWarps * BR * ((DP + 4) * 4 + 8);   // the warps' O, m and l
+  // an even number: a stage always belongs to the same four warps, which then
+  // wait for every phase of its barriers (parities cannot be taken for others)
+  static constexpr int STAGES = DP == 64 ? 8 : 4;
+  static_assert(STAGES % 2 == 0, "stages alternate between the two groups of warps");
+  static constexpr int SMEM = STAGES * STAGE + JOIN + 1024;
+};
 
 template <typename T>
-__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (std::is_same<T, __nv_bfloat16>::value)
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// 8 x 8 transpose of 16-bit elements: thread (g, t) gives row g, columns 2t
+// and 2t + 1, and takes rows 2t and 2t + 1 of column g.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
 
-__device__ __forceinline__ float quad_max(float v) {
-  v = fmaxf(v, __shfl_xor_sync(kFull, v, 1));
-  return fmaxf(v, __shfl_xor_sync(kFull, v, 2));
+// Over the eight thread groups g.
+__device__ __forceinline__ float groups_max(float v) {
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
+  return v;
 }
-__device__ __forceinline__ float quad_sum(float v) {
-  v += __shfl_xor_sync(kFull, v, 1);
-  return v + __shfl_xor_sync(kFull, v, 2);
+__device__ __forceinline__ float groups_sum(float v) {
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(kFull, v, o);
+  return v;
 }
 
-// Thread (g, t) = (lane / 4, lane % 4).  HALVES: 16-row fragments' halves in
-// use (1: rows 0-7 only).  row_warps: warps of the CTA with query rows of
-// their own; the other factor of kWarps splits the keys of a step.
-template <typename T, int DP, int HALVES>
-__global__ void __launch_bounds__(kThreads) prefix_mma_kernel(const __grid_constant__ PrefixArgs a, bool prefix, int row_warps) {
-  constexpr int KC = DP / 32, VC = DP / 64, NT = DP / 8;   // 16-byte loads of a key / value row per thread, O tiles
-  constexpr int BR = 8 * HALVES;
-  extern __shared__ __align__(16) float smem[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int split = blockIdx.x, h = blockIdx.z % a.H, b = prefix ? 0 : blockIdx.z / a.H;
-  const int rows = (prefix ? a.B * a.T : a.T) * a.G;
-  const int r0 = (int(blockIdx.y) * row_warps + warp % row_warps) * BR;
-  const int key_warps = kWarps / row_warps, key_warp = warp / row_warps;
-  const int length = prefix ? a.P : own_length(a, b);
-  int begin, end;
-  split_range(length, split, prefix ? a.prefix_splits : a.own_splits, kWarps * kStep, begin, end);
-  const int shared = prefix ? length : length - a.T + 1;   // keys before this one are seen by every row
-  const T* kp = prefix ? static_cast<const T*>(a.pk) + h * a.pk_sh : static_cast<const T*>(a.k) + b * a.k_sb + h * a.k_sh;
-  const T* vp = prefix ? static_cast<const T*>(a.pv) + h * a.pv_sh : static_cast<const T*>(a.v) + b * a.v_sb + h * a.v_sh;
-  const int64_t k_st = prefix ? a.pk_st : a.k_st, v_st = prefix ? a.pv_st : a.v_st;
+// Key ranges of sequence b's own cache: at least one, which may be empty.
+__device__ __forceinline__ int own_ranges(const PrefixArgs& a, int b) {
+  return max(1, (own_length(a, b) + a.own_chunk - 1) / a.own_chunk);
+}
 
-  uint4 q[HALVES][KC];
-  int last[HALVES];
-#pragma unroll
-  for (int i = 0; i < HALVES; ++i) {
-    const int row = r0 + g + 8 * i, tok = row / a.G, hq = h * a.G + row - tok * a.G;
-    const int qb = prefix ? tok / a.T : b, qt = prefix ? tok - qb * a.T : tok;
-    last[i] = row >= rows ? -1 : prefix ? length - 1 : length - a.T + tok;
-    const T* qp = static_cast<const T*>(a.q) + qb * a.q_sb + qt * a.q_st + hq * a.q_sh;
-#pragma unroll
-    for (int c = 0; c < KC; ++c)
-      q[i][c] = row < rows && 32 * c + 8 * t < a.D ? *reinterpret_cast<const uint4*>(qp + 32 * c + 8 * t) : make_uint4(0, 0, 0, 0);
-  }
-  const float sl = a.scale * kLog2e;
-  float o[NT][4], m[HALVES], l[HALVES];
-#pragma unroll
-  for (int i = 0; i < HALVES; ++i) {
-    m[i] = -INFINITY;
-    l[i] = 0.f;
-  }
-#pragma unroll
-  for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+struct Item {
+  bool prefix;
+  int b, h, block, split, length, begin, end;
+};
 
-  uint4 k[2][KC], v[4][VC];
-  // keys 8 i + g of the step at j; rows past the end repeat the last one (their scores are selected away)
-  auto load_k = [&](int j) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const T* p = kp + int64_t(min(j + 8 * i + g, end - 1)) * k_st + 8 * t;
-#pragma unroll
-      for (int c = 0; c < KC; ++c)
-        k[i][c] = 32 * c + 8 * t < a.D ? __ldg(reinterpret_cast<const uint4*>(p + 32 * c)) : make_uint4(0, 0, 0, 0);
+// Item `i` of the list; `table` holds the own ranges before each entry's sequences.
+__device__ __forceinline__ Item item_at(const StreamArgs& s, const int* table, int i) {
+  const PrefixArgs& a = s.p;
+  Item x;
+  x.prefix = i < s.prefix_items;
+  if (!x.prefix) i -= s.prefix_items;
+  const int blocks = x.prefix ? s.prefix_blocks : s.own_blocks;
+  x.h = i % a.H;
+  i /= a.H;
+  x.block = i % blocks;
+  i /= blocks;
+  x.b = 0;
+  if (!x.prefix) {
+    int lo = 0, hi = (a.B + s.per_entry - 1) / s.per_entry - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (table[mid] <= i) lo = mid;
+      else hi = mid - 1;
     }
-  };
-  // values of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9; zero from key min(end, shared) on
-  const int seen = min(end, shared);
-  auto load_v = [&](int j) {
+    i -= table[lo];
+    x.b = lo * s.per_entry;
+    for (int n; x.b + 1 < a.B && i >= (n = own_ranges(a, x.b)); ++x.b) i -= n;
+  }
+  x.split = i;
+  x.length = x.prefix ? a.P : own_length(a, x.b);
+  split_range(x.length, i, x.prefix ? a.prefix_chunk : a.own_chunk, x.begin, x.end);
+  return x;
+}
+
+template <typename T, int DP, int NR>
+__global__ void __launch_bounds__(kThreads, 1) prefix_stream_kernel(const __grid_constant__ StreamArgs args) {
+  using L = Stream<DP, NR>;
+  constexpr int MT = DP / 16, BR = L::BR;
+  const PrefixArgs& a = args.p;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t base = (tc::smem_u32(smem_raw) + 1023) & ~1023u;
+  float* so = reinterpret_cast<float*>(smem_raw + (base - tc::smem_u32(smem_raw)) + L::STAGES * L::STAGE);  // [warps][BR][DP + 4]
+  float2* sml = reinterpret_cast<float2*>(so + kComputeWarps * BR * (DP + 4));                              // [warps][BR]
+  __shared__ uint64_t full[L::STAGES], empty[L::STAGES];
+  __shared__ int table[kTable + 1];
+  __shared__ int s_fail;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  cudaTriggerProgrammaticLaunchCompletion();   // the joining launch may be scheduled
+
+  // own ranges before each table entry (an exclusive scan by one warp)
+  const int entries = (a.B + args.per_entry - 1) / args.per_entry;
+  if (warp == 0) {
+    int sum = 0;
+    for (int e0 = 0; e0 < entries; e0 += 32) {
+      const int e = e0 + lane;
+      int n = 0;
+      if (e < entries)
+        for (int b = e * args.per_entry; b < min(a.B, (e + 1) * args.per_entry); ++b) n += own_ranges(a, b);
+      int up = n;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int key = j + 2 * t + (i & 1) + 8 * (i >> 1);
-      const T* p = vp + int64_t(key) * v_st + 8 * g;
-#pragma unroll
-      for (int c = 0; c < VC; ++c)
-        v[i][c] = key < seen && 64 * c + 8 * g < a.Dv ? __ldg(reinterpret_cast<const uint4*>(p + 64 * c)) : make_uint4(0, 0, 0, 0);
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(kFull, up, o);
+        if (lane >= o) up += y;
+      }
+      if (e < entries) table[e] = sum + up - n;
+      sum += __shfl_sync(kFull, up, 31);
     }
-  };
-  const int stride = key_warps * kStep;
-  int j = begin + key_warp * kStep;
-  if (r0 < rows && j < end) {
-    load_k(j);
-    load_v(j);
-    for (; j < end; j += stride) {
-      float s[2][4];
+    if (lane == 0) table[entries] = sum;
+  } else if (tid == 32) {
+    for (int i = 0; i < L::STAGES; ++i) {
+      tc::mbar_init(&full[i], 1);
+      tc::mbar_init(&empty[i], 4);
+    }
+    s_fail = 0;
+    tc::fence_barrier_init();
+  }
+  __syncthreads();
+  const int items = args.prefix_items + table[entries] * args.own_blocks * a.H;
+
+  if (warp == kLoadWarp) {
+    if (lane == 0) {
+      int n = 0;   // tiles issued so far
+      bool ok = true;
+      for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
+        const Item x = item_at(args, table, i);
+        const CUtensorMap* mk = x.prefix ? &args.tm_pk : &args.tm_k;
+        const CUtensorMap* mv = x.prefix ? &args.tm_pv : &args.tm_v;
+        for (int j = x.begin; j < x.end; j += kTile, ++n) {
+          const int st = n % L::STAGES;
+          if (!tc::mbar_wait(&empty[st], ((n / L::STAGES) & 1) ^ 1)) { s_fail = 1; ok = false; break; }
+          tc::mbar_arrive_expect_tx(&full[st], L::STAGE);
+          const uint32_t k = base + st * L::STAGE, v = k + L::OPERAND;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
-#pragma unroll
-        for (int c = 0; c < KC; ++c) {
-          const uint4 lo = q[0][c], hi = HALVES == 2 ? q[HALVES - 1][c] : make_uint4(0, 0, 0, 0);
-          mma16816<T>(s[i], lo.x, hi.x, lo.y, hi.y, k[i][c].x, k[i][c].y);
-          mma16816<T>(s[i], lo.z, hi.z, lo.w, hi.w, k[i][c].z, k[i][c].w);
+          for (int c = 0; c < L::CH; ++c) {
+            tc::tma_load_4d(k + c * kTile * 128, mk, c * 64, x.h, j, x.b, &full[st]);
+            tc::tma_load_4d(v + c * kTile * 128, mv, c * 64, x.h, j, x.b, &full[st]);
+          }
         }
       }
-      if (j + stride < end) load_k(j + stride);
-      const bool partial = j + kStep > seen;    // keys past the end, or seen by some rows only
-      uint32_t p[2][HALVES];                    // P of key tiles 0 and 1 as A operands
-      float alpha[HALVES], pf[2][HALVES][2];
-      bool moved = false;
+      // after an expired wait: the copies in flight land before the CTA ends
+      if (!ok)
+        for (int x = max(0, n - L::STAGES); x < n; ++x) tc::mbar_wait(&full[x % L::STAGES], (x / L::STAGES) & 1);
+    }
+  } else {
+    const int g = lane >> 2, t = lane & 3, sub = warp & 3, side = warp >> 2;   // 16 keys of the CTA's even or odd tiles
+    const float sl = a.scale * kLog2e;
+    const int slots = a.prefix_splits + a.own_splits;
+    bool ok = true;
+    int n = 0;   // tiles of the items before
+    for (int i = blockIdx.x; i < items; i += gridDim.x) {
+      const Item x = item_at(args, table, i);
+      const int rows = (x.prefix ? a.B * a.T : a.T) * a.G, r0 = x.block * BR;
+      const int shared = x.prefix ? x.length : x.length - a.T + 1;   // keys before this one are seen by every row
+      const int seen = min(x.end, shared);
+      const T* vp = x.prefix ? static_cast<const T*>(a.pv) + x.h * a.pv_sh
+                             : static_cast<const T*>(a.v) + x.b * a.v_sb + x.h * a.v_sh;
+      const int64_t v_st = x.prefix ? a.pv_st : a.v_st;
+      // query row 8 r + g as the B operand; the rows whose scores this thread
+      // holds are 8 r + 2 t and 8 r + 2 t + 1
+      uint32_t q[NR][MT][2];
+      int last[NR][2];
+      float o[NR][MT][4], m[NR][2], l[NR][2];
 #pragma unroll
-      for (int i = 0; i < HALVES; ++i) {
-        float x[2][2];
+      for (int r = 0; r < NR; ++r) {
+        const int row = r0 + 8 * r + g, tok = row / a.G, hq = x.h * a.G + row - tok * a.G;
+        const int qb = x.prefix ? tok / a.T : x.b, qt = x.prefix ? tok - qb * a.T : tok;
+        const T* qp = static_cast<const T*>(a.q) + qb * a.q_sb + qt * a.q_st + hq * a.q_sh;
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
+        for (int s = 0; s < MT; ++s) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            x[n][e] = s[n][2 * i + e] * sl;
-            const int key = j + 8 * n + 2 * t + e;
-            if (partial && (key > last[i] || key >= end)) x[n][e] = -INFINITY;
+            const int d = 16 * s + 8 * e + 2 * t;
+            q[r][s][e] = row < rows && d < a.D ? *reinterpret_cast<const uint32_t*>(qp + d) : 0u;
           }
+          o[r][s][0] = o[r][s][1] = o[r][s][2] = o[r][s][3] = 0.f;
         }
-        const float top = quad_max(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1])));
-        const float to = fmaxf(m[i], top), ref = to == -INFINITY ? 0.f : to;
-        alpha[i] = m[i] == -INFINITY ? 0.f : tc::ex2f(m[i] - ref);
-        moved = moved || to > m[i];
-        m[i] = to;
-        float sum = 0.f;
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            pf[n][i][e] = tc::ex2f(x[n][e] - ref);
-            sum += pf[n][i][e];
-            const int key = j + 8 * n + 2 * t + e;
-            if (partial && key >= seen) x[n][e] = 0.f;      // added row by row below
-            else x[n][e] = pf[n][i][e];
-          }
-          p[n][i] = pack2<T>(x[n][0], x[n][1]);
-        }
-        l[i] = l[i] * alpha[i] + sum;    // this thread's share of the row's sum
-      }
-      if (__any_sync(kFull, moved)) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-          for (int i = 0; i < HALVES; ++i) {
-            o[n][2 * i] *= alpha[i];
-            o[n][2 * i + 1] *= alpha[i];
-          }
+        for (int e = 0; e < 2; ++e) {
+          const int mine = r0 + 8 * r + 2 * t + e;
+          last[r][e] = mine >= rows ? -1 : x.prefix ? x.length - 1 : x.length - a.T + mine / a.G;
+          m[r][e] = -INFINITY;
+          l[r][e] = 0.f;
         }
       }
+      const int tiles = (x.end - x.begin + kTile - 1) / kTile;
+      for (int u = (n ^ side) & 1; u < tiles && ok; u += 2) {   // tiles n + u of this side's parity
+        const int st = (n + u) % L::STAGES;
+        if (!tc::mbar_wait(&full[st], ((n + u) / L::STAGES) & 1)) { s_fail = 1; ok = false; break; }
+        const uint32_t kt = base + st * L::STAGE + sub * 16 * 128, vt = kt + L::OPERAND;
+        const int j = x.begin + u * kTile + sub * 16;      // first key of this warp
+        if (j < x.end) {
+          float s[NR][4];
 #pragma unroll
-      for (int c = 0; c < VC; ++c) {
-        const uint32_t* v0 = &v[0][c].x;
-        const uint32_t* v1 = &v[1][c].x;
-        const uint32_t* v2 = &v[2][c].x;
-        const uint32_t* v3 = &v[3][c].x;
+          for (int r = 0; r < NR; ++r) s[r][0] = s[r][1] = s[r][2] = s[r][3] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {   // O tile 8 c + e: dims 64 c + 8 g + e
-          const uint32_t sel = e & 1 ? 0x7632u : 0x5410u;
-          mma16816<T>(o[8 * c + e], p[0][0], HALVES == 2 ? p[0][HALVES - 1] : 0u, p[1][0], HALVES == 2 ? p[1][HALVES - 1] : 0u,
-                      __byte_perm(v0[e / 2], v1[e / 2], sel), __byte_perm(v2[e / 2], v3[e / 2], sel));
-        }
-      }
-      if (j + stride < end) load_v(j + stride);
-      if (partial) {
-        for (int key = max(j, shared); key < min(j + kStep, end); ++key) {
-          const int x = key - j, src = (lane & ~3) | ((x & 7) >> 1);
+          for (int c = 0; c < MT; ++c) {
+            const int row = lane & 15, seg = (c & 3) * 2 + (lane >> 4);
+            uint32_t k[4];
+            ldmatrix4(k, kt + (c >> 2) * kTile * 128 + row * 128 + ((seg ^ (row & 7)) << 4));
 #pragma unroll
-          for (int i = 0; i < HALVES; ++i) {
-            const float w0 = x < 8 ? pf[0][i][0] : pf[1][i][0], w1 = x < 8 ? pf[0][i][1] : pf[1][i][1];
-            const float w = __shfl_sync(kFull, x & 1 ? w1 : w0, src);
-            if (key > last[i]) continue;
-            // O tile n, columns 2 t and 2 t + 1: dims 64 c + 16 t + e and 8 more
+            for (int r = 0; r < NR; ++r) mma16816<T>(s[r], k, q[r][c][0], q[r][c][1]);
+          }
+          const bool partial = j + 16 > seen;              // keys past the end, or seen by some rows only
+          bool grown = false;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              const int d = 64 * (n / 8) + 16 * t + (n & 7);
-              if (d < a.Dv) o[n][2 * i] = fmaf(w, to_f32<T>(vp[int64_t(key) * v_st + d]), o[n][2 * i]);
-              if (d + 8 < a.Dv) o[n][2 * i + 1] = fmaf(w, to_f32<T>(vp[int64_t(key) * v_st + d + 8]), o[n][2 * i + 1]);
+          for (int r = 0; r < NR; ++r) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {                  // key g (e < 2) or g + 8 of row 8 r + 2 t + (e & 1)
+              s[r][e] *= sl;
+              const int key = j + g + 8 * (e >> 1);
+              if (partial && (key > last[r][e & 1] || key >= x.end)) s[r][e] = -INFINITY;
+              grown = grown || s[r][e] > m[r][e & 1] + 8.f;
+            }
+          }
+          if (__any_sync(kFull, grown)) {
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float to = fmaxf(m[r][e], groups_max(fmaxf(s[r][e], s[r][2 + e])));
+                const float alpha = m[r][e] == -INFINITY ? 0.f : tc::ex2f(m[r][e] - to);
+                m[r][e] = to;
+                l[r][e] *= alpha;
+#pragma unroll
+                for (int c = 0; c < MT; ++c) {
+                  o[r][c][e] *= alpha;
+                  o[r][c][2 + e] *= alpha;
+                }
+              }
+            }
+          }
+          uint32_t p[NR][2];                               // P^T of keys 0-7 and 8-15 as B operands
+#pragma unroll
+          for (int r = 0; r < NR; ++r) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float ref = m[r][e & 1] == -INFINITY ? 0.f : m[r][e & 1];
+              s[r][e] = tc::ex2f(s[r][e] - ref);
+            }
+            l[r][0] += s[r][0] + s[r][2];                  // this thread's share of the rows' sums
+            l[r][1] += s[r][1] + s[r][3];
+            // weights of keys that only some rows see join row by row below
+            p[r][0] = transpose8(!partial || j + g < seen ? pack2<T>(s[r][0], s[r][1]) : 0u);
+            p[r][1] = transpose8(!partial || j + 8 + g < seen ? pack2<T>(s[r][2], s[r][3]) : 0u);
+          }
+          // operand registers hold keys 2 t and 2 t + 1 (and 8 more) as a pair
+          const int k0 = j + 2 * t;
+          const uint32_t low = (k0 < seen ? 0xffffu : 0u) | (k0 + 1 < seen ? 0xffff0000u : 0u);
+          const uint32_t high = (k0 + 8 < seen ? 0xffffu : 0u) | (k0 + 9 < seen ? 0xffff0000u : 0u);
+#pragma unroll
+          for (int c = 0; c < MT; ++c) {                   // dims 16 c + g and 16 c + 8 + g
+            const int row = (lane & 7) + (lane >> 4) * 8, seg = (c & 3) * 2 + ((lane >> 3) & 1);
+            uint32_t v[4];
+            ldmatrix4_trans(v, vt + (c >> 2) * kTile * 128 + row * 128 + ((seg ^ (row & 7)) << 4));
+            if (partial) {
+              v[0] &= low;
+              v[1] &= low;
+              v[2] &= high;
+              v[3] &= high;
+            }
+#pragma unroll
+            for (int r = 0; r < NR; ++r) mma16816<T>(o[r][c], v, p[r][0], p[r][1]);
+          }
+          if (partial) {
+            for (int key = max(j, shared); key < min(j + 16, x.end); ++key) {
+              const int y = key - j, src = (y & 7) * 4 + t;
+#pragma unroll
+              for (int r = 0; r < NR; ++r) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const float w0 = __shfl_sync(kFull, s[r][e], src), w1 = __shfl_sync(kFull, s[r][2 + e], src);
+                  if (key > last[r][e]) continue;
+                  const float w = y < 8 ? w0 : w1;
+#pragma unroll
+                  for (int c = 0; c < MT; ++c) {
+                    const int d = 16 * c + g;
+                    if (d < a.Dv) o[r][c][e] = fmaf(w, to_f32<T>(vp[int64_t(key) * v_st + d]), o[r][c][e]);
+                    if (d + 8 < a.Dv) o[r][c][2 + e] = fmaf(w, to_f32<T>(vp[int64_t(key) * v_st + d + 8]), o[r][c][2 + e]);
+                  }
+                }
+              }
             }
           }
         }
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&empty[st]);
       }
-    }
-  }
-  // Join the warps that share query rows: (m, l) per row and O through shared memory.
-  float* so = smem;                                        // [kWarps][BR][DP + 4]
-  float2* sml = reinterpret_cast<float2*>(so + kWarps * BR * (DP + 4));   // [kWarps][BR]
+      n += tiles;
+      // Join: (m, l) per row and O of the eight warps through shared memory.
 #pragma unroll
-  for (int i = 0; i < HALVES; ++i) {
-    const int row = g + 8 * i;
-    const float sum = quad_sum(l[i]);
-    if (t == 0) sml[warp * BR + row] = make_float2(m[i], sum);
+      for (int r = 0; r < NR; ++r) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int d = 64 * (n / 8) + 16 * t + (n & 7);
-      so[(warp * BR + row) * (DP + 4) + d] = o[n][2 * i];
-      so[(warp * BR + row) * (DP + 4) + d + 8] = o[n][2 * i + 1];
+        for (int e = 0; e < 2; ++e) {
+          const int at = warp * BR + 8 * r + 2 * t + e;
+          const float sum = groups_sum(l[r][e]);
+          if (g == 0) sml[at] = make_float2(m[r][e], ok ? sum : NAN);
+#pragma unroll
+          for (int c = 0; c < MT; ++c) {
+            so[at * (DP + 4) + 16 * c + g] = o[r][c][e];
+            so[at * (DP + 4) + 16 * c + 8 + g] = o[r][c][2 + e];
+          }
+        }
+      }
+      tc::named_sync(1, kComputeWarps * 32);
+      const int slot = x.prefix ? x.split : a.prefix_splits + x.split;
+      for (int y = tid; y < BR * (DP / 4); y += kComputeWarps * 32) {
+        const int d = y % (DP / 4) * 4, r = y / (DP / 4), row = r0 + r;
+        if (row >= rows || d >= a.Dv) continue;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kComputeWarps; ++w) top = fmaxf(top, sml[w * BR + r].x);
+        const float ref = top == -INFINITY ? 0.f : top;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kComputeWarps; ++w) {
+          const float2 ml = sml[w * BR + r];
+          if (ml.y == 0.f) continue;                       // no keys, or only weightless ones
+          const float f = tc::ex2f(ml.x - ref);
+          const float4 z = *reinterpret_cast<const float4*>(so + (w * BR + r) * (DP + 4) + d);
+          sum = fmaf(f, ml.y, sum);
+          acc.x = fmaf(f, z.x, acc.x);
+          acc.y = fmaf(f, z.y, acc.y);
+          acc.z = fmaf(f, z.z, acc.z);
+          acc.w = fmaf(f, z.w, acc.w);
+        }
+        const int tok = row / a.G, hq = x.h * a.G + row - tok * a.G;
+        const int64_t at = (int64_t(x.b) * a.T + tok) * a.Hq + hq;   // in the prefix tok counts b * T + t
+        if (slots == 1) {
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at * a.Dv + d) =
+              make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+          if (d == 0 && a.lse) a.lse[at] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+        } else {
+          *reinterpret_cast<float4*>(a.part_o + (at * slots + slot) * a.Dv + d) = acc;
+          if (d == 0) a.part_ml[at * slots + slot] = make_float2(top, sum);
+        }
+      }
+      tc::named_sync(1, kComputeWarps * 32);
     }
   }
   __syncthreads();
-  const int slots = a.prefix_splits + a.own_splits, slot = prefix ? split : a.prefix_splits + split;
-  for (int x = threadIdx.x; x < row_warps * BR * (DP / 4); x += kThreads) {
-    const int d = x % (DP / 4) * 4, r = x / (DP / 4) % BR, rw = x / (DP / 4) / BR;
-    const int row = (int(blockIdx.y) * row_warps + rw) * BR + r;
-    if (row >= rows || d >= a.Dv) continue;
-    float top = -INFINITY;
-    for (int w = 0; w < key_warps; ++w) top = fmaxf(top, sml[(w * row_warps + rw) * BR + r].x);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f;
-    for (int w = 0; w < key_warps; ++w) {
-      const int at = (w * row_warps + rw) * BR + r;
-      const float2 y = sml[at];
-      if (y.y == 0.f) continue;            // no keys, or only weightless ones
-      const float f = tc::ex2f(y.x - ref);
-      const float4 z = *reinterpret_cast<const float4*>(so + at * (DP + 4) + d);
-      sum = fmaf(f, y.y, sum);
-      acc.x = fmaf(f, z.x, acc.x);
-      acc.y = fmaf(f, z.y, acc.y);
-      acc.z = fmaf(f, z.z, acc.z);
-      acc.w = fmaf(f, z.w, acc.w);
-    }
-    const int tok = row / a.G, hq = h * a.G + row - tok * a.G;
-    const int64_t at = (int64_t(b) * a.T + tok) * a.Hq + hq;   // in the prefix tok counts b * T + t
-    if (slots == 1) {
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      const uint2 w = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
-      *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at * a.Dv + d) = w;
-      if (d == 0 && a.lse) a.lse[at] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
-    } else {
-      *reinterpret_cast<float4*>(a.part_o + (at * slots + slot) * a.Dv + d) = acc;
-      if (d == 0) a.part_ml[at * slots + slot] = make_float2(top, sum);
-    }
-  }
+  if (tid == 0 && s_fail && a.status) atomicExch(a.status, PISA_ERR_TIMEOUT);
+  // scheduled while the prefix's tiles drain, whose partials the joining launch
+  // reads too: this kernel ends after that one
+  cudaGridDependencySynchronize();
 }
 
-template <typename T, int DP, int HALVES>
-int launch(const PrefixArgs& a, bool prefix, cudaStream_t s) {
-  constexpr int BR = 8 * HALVES;
-  const int64_t rows = int64_t(prefix ? a.B : 1) * a.T * a.G, blocks = (rows + BR - 1) / BR;
-  const int row_warps = blocks >= 4 ? 4 : blocks >= 2 ? 2 : 1;
-  constexpr int smem = kWarps * BR * ((DP + 4) * 4 + 8);
-  static_assert(smem <= 48 * 1024, "fits the default shared memory");
-  const dim3 grid(unsigned(prefix ? a.prefix_splits : a.own_splits), unsigned((blocks + row_warps - 1) / row_warps),
-                  unsigned((prefix ? 1 : a.B) * a.H));
-  prefix_mma_kernel<T, DP, HALVES><<<grid, kThreads, smem, s>>>(a, prefix, row_warps);
+template <typename T, int DP, int NR>
+int launch(const StreamArgs& s, int sms, cudaStream_t stream) {
+  using L = Stream<DP, NR>;
+  const PrefixArgs& a = s.p;
+  cudaError_t e = cudaFuncSetAttribute(prefix_stream_kernel<T, DP, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+  if (e != cudaSuccess) return fail_cuda(e, "prefix attention smem attribute");
+  const int64_t most = s.prefix_items + int64_t(a.B) * a.own_splits * s.own_blocks * a.H;
+  const dim3 grid(unsigned(min64(sms, most)));
+  if (s.after_tiles) return launch_after(prefix_stream_kernel<T, DP, NR>, grid, kThreads, L::SMEM, s, stream);
+  prefix_stream_kernel<T, DP, NR><<<grid, kThreads, L::SMEM, stream>>>(s);
   PISA_CHECK_LAUNCH();
   return PISA_OK;
 }
 
 template <typename T, int DP>
-int segment(const PrefixArgs& a, bool prefix, cudaStream_t s) {
-  // rows 8-15 of the fragments are left out when no KV head has them: half the
-  // accumulator registers, so more warps and more loads in flight
-  return int64_t(prefix ? a.B : 1) * a.T * a.G <= 8 ? launch<T, DP, 1>(a, prefix, s) : launch<T, DP, 2>(a, prefix, s);
-}
-
-template <typename T, int DP>
-int segments(const PrefixArgs& a, cudaStream_t s) {
-  int rc = PISA_OK;
-  if (a.prefix_splits) rc = segment<T, DP>(a, true, s);
-  if (rc == PISA_OK && a.own_splits) rc = segment<T, DP>(a, false, s);
-  return rc;
-}
-
-template <typename T>
-int by_dim(const PrefixArgs& a, cudaStream_t s) {
-  return a.D <= 64 && a.Dv <= 64 ? segments<T, 64>(a, s) : segments<T, 128>(a, s);
+int by_rows(StreamArgs s, bool prefix, int sms, cudaStream_t stream) {
+  const PrefixArgs& a = s.p;
+  const int64_t own_rows = int64_t(a.T) * a.G, prefix_rows = a.B * own_rows;
+  // 8 rows per pass when no KV head has more: half the registers and join
+  // buffers, one stage more; 16 otherwise: half the passes over the keys
+  const int br = (prefix ? prefix_rows : own_rows) <= 8 ? 8 : 16;
+  s.own_blocks = int((own_rows + br - 1) / br);
+  s.prefix_blocks = int((prefix_rows + br - 1) / br);
+  const int64_t items = int64_t(prefix ? a.prefix_splits : 0) * s.prefix_blocks * a.H;
+  if (items + int64_t(a.B) * a.own_splits * s.own_blocks * a.H >= (int64_t(1) << 31))
+    return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
+  s.prefix_items = int(items);
+  s.per_entry = (a.B + kTable - 1) / kTable;
+  return br == 8 ? launch<T, DP, 1>(s, sms, stream) : launch<T, DP, 2>(s, sms, stream);
 }
 
 }  // namespace
 
-int prefix_attn_mma(const PrefixArgs& a, int dtype, cudaStream_t stream) {
-  return dtype == PISA_BF16 ? by_dim<__nv_bfloat16>(a, stream) : by_dim<__half>(a, stream);
+int prefix_attn_mma(const PrefixArgs& a, int dtype, bool prefix, int sms, cudaStream_t stream) {
+  StreamArgs s{};
+  s.p = a;
+  s.after_tiles = a.prefix_splits > 0 && !prefix;
+  int rc = dense_tensor_map(&s.tm_k, a.k, dtype, a.B, a.cap, a.H, a.D, a.k_sb, a.k_st, a.k_sh, kTile);
+  if (rc == PISA_OK) rc = dense_tensor_map(&s.tm_v, a.v, dtype, a.B, a.cap, a.H, a.Dv, a.v_sb, a.v_st, a.v_sh, kTile);
+  if (rc == PISA_OK && prefix) rc = dense_tensor_map(&s.tm_pk, a.pk, dtype, 1, a.P, a.H, a.D, 0, a.pk_st, a.pk_sh, kTile);
+  if (rc == PISA_OK && prefix) rc = dense_tensor_map(&s.tm_pv, a.pv, dtype, 1, a.P, a.H, a.Dv, 0, a.pv_st, a.pv_sh, kTile);
+  if (rc) return rc;
+  const bool narrow = a.D <= 64 && a.Dv <= 64;
+  if (dtype == PISA_BF16)
+    return narrow ? by_rows<__nv_bfloat16, 64>(s, prefix, sms, stream) : by_rows<__nv_bfloat16, 128>(s, prefix, sms, stream);
+  return narrow ? by_rows<__half, 64>(s, prefix, sms, stream) : by_rows<__half, 128>(s, prefix, sms, stream);
 }
 
 }  // namespace pisa

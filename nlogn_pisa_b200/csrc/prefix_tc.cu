@@ -1,0 +1,276 @@
+// The shared prefix of decode attention on the tensor cores, for batches with
+// many query rows per KV head (formulas and partial results in
+// prefix_attn.cu; the pipeline is that of dense_attn_tc.cu).
+//
+// The prefix is the same for every sequence, so the query rows of the whole
+// batch (token by token, the G heads of a KV head side by side) form ordinary
+// tiles of up to 128 rows, and its keys and values are read once for 256 of
+// them.  One CTA takes a range of keys of one KV head.  With two row tiles or
+// more, its two tiles share the stream of keys; with one, both halves hold the
+// same rows and take every other key tile, so that the tensor core still
+// works for one half while the other half's weights are computed, and their
+// results join in shared memory.  Ranges are sized for one wave of CTAs.
+#include "dense_tc.cuh"
+#include "prefix_attn.cuh"
+
+namespace pisa {
+
+namespace {
+
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kThreads = 320;
+
+struct PrefixTcArgs {
+  CUtensorMap tm_q;                  // [B * T tokens, Hq, D], box of 64 dims x G heads x tokens of a tile
+  CUtensorMap tm_k, tm_v;            // prefix, boxes of 64 dims x 128 keys of one head
+  PrefixArgs p;
+  int tokens, tiles;                 // tokens of a row tile, row tiles
+  int bf16;
+};
+
+template <int DP> struct PrefixTile {
+  static constexpr int CH = DP / 64, BYTES = kRows * DP * 2;
+  static constexpr int STAGES = DP == 128 ? 4 : 6;      // 64 dims: also keeps a second CTA off the SM's TMEM
+  static constexpr int SMEM = (2 + STAGES) * BYTES + 1024;
+  static_assert(STAGES * BYTES >= kRows * (DP + 4) * 4, "half 1's output fits the ring");
+};
+
+__device__ __forceinline__ void st_global32(float* p, const float* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+               :: "l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_constant__ PrefixTcArgs args) {
+  using L = PrefixTile<DP>;
+  const PrefixArgs& a = args.p;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t base = (tc::smem_u32(smem_raw) + 1023) & ~1023u;
+  const uint32_t q_addr = base, kv_addr = base + 2 * L::BYTES;
+  float* join = reinterpret_cast<float*>(smem_raw + (kv_addr - tc::smem_u32(smem_raw)));   // [128][DP + 4], after the ring's use
+  __shared__ uint64_t q_full[2], kv_full[L::STAGES], kv_empty[L::STAGES], s_full[2], p_full[2], o_done[2], drained;
+  __shared__ float2 join_ml[kRows];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int s_fail;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  cudaTriggerProgrammaticLaunchCompletion();   // the own caches' kernel may be scheduled
+  const int h = blockIdx.x % a.H, split = blockIdx.x / a.H;
+  const bool dual = args.tiles == 1;            // one row tile: the halves take every other key tile
+  int begin, end;
+  split_range(a.P, split, a.prefix_chunk, begin, end);
+  const int keys = (end - begin + kRows - 1) / kRows;      // key tiles, at least one
+  const int row_tile[2] = {dual ? 0 : int(blockIdx.y) * 2, dual ? 0 : int(blockIdx.y) * 2 + 1};
+  const int steps[2] = {dual ? (keys + 1) / 2 : keys, dual ? keys / 2 : row_tile[1] < args.tiles ? keys : 0};
+  const int most = max(steps[0], steps[1]);
+  // ring position of the keys of half i's step s (its values: one more)
+  auto position = [&](int i, int s) { return dual ? 2 * (2 * s + i) : 2 * s; };
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&q_full[i], 1);
+      tc::mbar_init(&s_full[i], 1);
+      tc::mbar_init(&p_full[i], 4);
+      tc::mbar_init(&o_done[i], 1);
+    }
+    for (int i = 0; i < L::STAGES; ++i) {
+      tc::mbar_init(&kv_full[i], 1);
+      tc::mbar_init(&kv_empty[i], 1);
+    }
+    tc::mbar_init(&drained, 1);
+    s_fail = 0;
+    tc::fence_barrier_init();
+  }
+  if (warp == kMmaWarp) tc::tmem_alloc(&tmem_slot, 512);
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  const uint32_t tS[2] = {tmem, tmem + 128}, tO[2] = {tmem + 256, tmem + 256 + DP};
+
+  if (warp == kLoadWarp) {
+    if (lane == 0) {
+      const uint32_t q_bytes = uint32_t(args.tokens) * a.G * 128 * L::CH;
+      for (int i = 0; i < 2; ++i) {
+        if (!steps[i]) continue;
+        tc::mbar_arrive_expect_tx(&q_full[i], q_bytes);
+        for (int c = 0; c < L::CH; ++c)
+          tc::tma_load_4d(q_addr + i * L::BYTES + c * kRows * 128, &args.tm_q, c * 64, h * a.G, row_tile[i] * args.tokens, 0,
+                          &q_full[i]);
+      }
+      for (int n = 0; n < 2 * keys; ++n) {   // K0 V0 K1 V1 ...
+        const int st = n % L::STAGES;
+        if (!tc::mbar_wait(&kv_empty[st], ((n / L::STAGES) & 1) ^ 1)) {
+          s_fail = 1;
+          // the copies in flight land before the CTA ends
+          for (int x = max(0, n - L::STAGES); x < n; ++x) tc::mbar_wait(&kv_full[x % L::STAGES], (x / L::STAGES) & 1);
+          break;
+        }
+        tc::mbar_arrive_expect_tx(&kv_full[st], L::BYTES);
+        const CUtensorMap* map = n & 1 ? &args.tm_v : &args.tm_k;
+        for (int c = 0; c < L::CH; ++c)
+          tc::tma_load_4d(kv_addr + st * L::BYTES + c * kRows * 128, map, c * 64, h, begin + (n >> 1) * kRows, 0, &kv_full[st]);
+      }
+    }
+    __syncwarp();
+  } else if (warp == kMmaWarp) {
+    if (lane == 0) {
+      const uint32_t id_s = tc::idesc_f16(kRows, kRows, args.bf16), id_o = tc::idesc_f16(kRows, DP, args.bf16, 1);
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, int phase) {
+        if (ok && !tc::mbar_wait(bar, phase & 1)) { s_fail = 1; ok = false; }
+      };
+      // a stage that no later tile takes is not handed back: nothing may arrive after the CTA's end
+      auto hand_back = [&](int pos) {
+        if (pos + L::STAGES < 2 * keys) tc::mma_commit(&kv_empty[pos % L::STAGES]);
+      };
+      for (int s = 0; s <= most && ok; ++s) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (s >= 1 && s <= steps[i]) {        // O += P V of step s - 1
+            const int pos = position(i, s - 1) + 1;
+            wait(&kv_full[pos % L::STAGES], pos / L::STAGES);
+            wait(&p_full[i], s - 1);
+            if (!ok) break;
+            tc::fence_after_sync();
+            const uint32_t v = kv_addr + (pos % L::STAGES) * L::BYTES;
+#pragma unroll
+            for (int x = 0; x < kRows / 16; ++x)
+              tc::mma_f16_ts(tO[i], tS[i] + x * 8, tc::desc_make(v + x * 16 * 128, kRows * 128, 1024, 2), id_o, s > 1 || x > 0);
+            if (s == steps[i]) tc::mma_commit(&o_done[i]);
+            if (dual || i == (steps[1] ? 1 : 0)) hand_back(pos);
+          }
+          if (s < steps[i]) {                   // S = Q K^T of step s
+            const int pos = position(i, s);
+            if (s == 0) wait(&q_full[i], 0);
+            wait(&kv_full[pos % L::STAGES], pos / L::STAGES);
+            if (!ok) break;
+            tc::fence_after_sync();
+            const uint32_t k = kv_addr + (pos % L::STAGES) * L::BYTES, q = q_addr + i * L::BYTES;
+#pragma unroll
+            for (int x = 0; x < DP / 16; ++x) {
+              const uint32_t off = (x >> 2) * kRows * 128 + (x & 3) * 32;
+              tc::mma_f16(tS[i], tc::desc_sw128(q + off), tc::desc_sw128(k + off), id_s, x > 0);
+            }
+            tc::mma_commit(&s_full[i]);
+            if (dual || i == (steps[1] ? 1 : 0)) hand_back(pos);
+          }
+        }
+      }
+      if (!ok) {
+        tc::mma_commit(&drained);
+        tc::mbar_wait(&drained, 0);
+      }
+    }
+    __syncwarp();
+  } else {
+    const int i = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t lanes = uint32_t(quarter * 32) << 16;
+    const uint32_t ts = tS[i] + lanes, to = tO[i] + lanes;
+    const float sl = a.scale * kLog2e;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int s = 0; s < steps[i]; ++s) {
+      if (!tc::mbar_wait(&s_full[i], s & 1)) { s_fail = 1; ok = false; break; }
+      tc::fence_after_sync();
+      const int first = begin + (dual ? 2 * s + i : s) * kRows;
+      softmax_tile<T, DP>(ts, to, sl, s == 0, end - 1 - first, m, l);
+      tmem_wait_st();
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&p_full[i]);
+    }
+    if (steps[i] && ok && !tc::mbar_wait(&o_done[i], 0)) { s_fail = 1; ok = false; }
+    tc::fence_after_sync();
+    if (!ok) l = NAN;
+    // half 1's result joins half 0's when they hold the same rows
+    float mul = 1.f, mul1 = 0.f;
+    if (dual) {
+      if (i == 1) {
+        // the ring is free once half 0's last product is done, too
+        if (ok && !tc::mbar_wait(&o_done[0], 0)) { s_fail = 1; l = NAN; }
+        if (steps[1]) {
+#pragma unroll
+          for (int c = 0; c < DP; c += 32) {
+            float o[32];
+            tc::tmem_ld32(to + c, o);
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<float4*>(join + row * (DP + 4) + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
+        }
+        join_ml[row] = make_float2(m, l);
+      }
+      tc::named_sync(1, 256);
+      if (i == 0) {
+        const float2 x = join_ml[row];
+        const float top = fmaxf(m, x.x), ref = top == -INFINITY ? 0.f : top;
+        mul = m == -INFINITY ? 0.f : tc::ex2f(m - ref);
+        mul1 = x.y == 0.f ? 0.f : tc::ex2f(x.x - ref);
+        l = l * mul + (x.y == 0.f ? 0.f : x.y * mul1);
+        m = top;
+      }
+    }
+    const int tok = row_tile[i] * args.tokens + row / a.G, hq = h * a.G + row % a.G;
+    const bool real = steps[i] && !(dual && i == 1) && row < args.tokens * a.G && tok < a.B * a.T;
+    const int slots = a.prefix_splits + a.own_splits;
+    const int64_t at = (int64_t(tok) * a.Hq + hq) * slots + split;
+    if (steps[i] && !(dual && i == 1)) {
+#pragma unroll
+      for (int c = 0; c < DP; c += 32) {
+        float o[32];
+        tc::tmem_ld32(to + c, o);
+        if (dual) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            const float4 x = mul1 == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                         : *reinterpret_cast<const float4*>(join + row * (DP + 4) + c + e);
+            o[e] = o[e] * mul + x.x * mul1;
+            o[e + 1] = o[e + 1] * mul + x.y * mul1;
+            o[e + 2] = o[e + 2] * mul + x.z * mul1;
+            o[e + 3] = o[e + 3] * mul + x.w * mul1;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 32; e += 8)
+          if (real && c + e < a.Dv) st_global32(a.part_o + at * a.Dv + c + e, o + e);
+      }
+      if (real) a.part_ml[at] = make_float2(m, l);
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  if (tid == 0 && s_fail && a.status) atomicExch(a.status, PISA_ERR_TIMEOUT);
+  if (warp == kMmaWarp) tc::tmem_free(tmem, 512);
+}
+
+template <typename T, int DP>
+int launch(const PrefixTcArgs& a, cudaStream_t s) {
+  using L = PrefixTile<DP>;
+  cudaError_t e = cudaFuncSetAttribute(prefix_tc_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+  if (e != cudaSuccess) return fail_cuda(e, "prefix attention smem attribute");
+  prefix_tc_kernel<T, DP><<<dim3(unsigned(a.p.prefix_splits * a.p.H), unsigned((a.tiles + 1) / 2)), kThreads, L::SMEM, s>>>(a);
+  PISA_CHECK_LAUNCH();
+  return PISA_OK;
+}
+
+}  // namespace
+
+int prefix_attn_tc(const PrefixArgs& p, int dtype, cudaStream_t stream) {
+  PrefixTcArgs a{};
+  a.p = p;
+  a.bf16 = dtype == PISA_BF16;
+  a.tokens = kRows / p.G;
+  const int64_t tokens = int64_t(p.B) * p.T;
+  a.tiles = int((tokens + a.tokens - 1) / a.tokens);
+  int64_t st = p.T == 1 ? p.q_sb : p.q_st;
+  int64_t sh = p.Hq == 1 ? p.D : p.q_sh;
+  if (tokens == 1) st = p.Hq * sh;
+  int rc = make_tensor_map(&a.tm_q, p.q, dtype, 1, tokens, p.Hq, p.D, 0, st, sh, uint32_t(p.G), uint32_t(a.tokens));
+  if (rc == PISA_OK) rc = dense_tensor_map(&a.tm_k, p.pk, dtype, 1, p.P, p.H, p.D, 0, p.pk_st, p.pk_sh, kRows);
+  if (rc == PISA_OK) rc = dense_tensor_map(&a.tm_v, p.pv, dtype, 1, p.P, p.H, p.Dv, 0, p.pv_st, p.pv_sh, kRows);
+  if (rc) return rc;
+  const bool narrow = p.D <= 64 && p.Dv <= 64;
+  if (dtype == PISA_BF16) return narrow ? launch<__nv_bfloat16, 64>(a, stream) : launch<__nv_bfloat16, 128>(a, stream);
+  return narrow ? launch<__half, 64>(a, stream) : launch<__half, 128>(a, stream);
+}
+
+}  // namespace pisa

@@ -195,6 +195,8 @@ def prefix_attention(q, k, v, lengths, prefix_k=None, prefix_v=None, scale=None,
     code = _lib.dtype_code(q)
     scale = k.shape[-1] ** -0.5 if scale is None else float(scale)
     q, k, v, lengths = aligned_rows(q), aligned_rows(k), aligned_rows(v), lengths.contiguous()
+    if q.shape[0] > 1 and q.shape[1] > 1 and q.stride(0) != q.shape[1] * q.stride(1):
+        q = q.contiguous()
     if prefix:
         prefix_k, prefix_v = (aligned_rows(t[None])[0] for t in (prefix_k, prefix_v))
     batch, tokens, q_heads, dim = q.shape
