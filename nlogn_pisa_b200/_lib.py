@@ -149,6 +149,26 @@ def stream_of(device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+# the current stream as an integer, without building a Stream object per call
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def launch(fn, device_index, *args):
+    """``fn(*args, stream)`` on a device's current stream; raises for a bad status.
+
+    Pointers are plain integers (0 or None for NULL).  The device guard is
+    entered only when another device is current."""
+    stream = _raw_stream(device_index)
+    if torch.cuda.current_device() == device_index:
+        status = fn(*args, stream)
+    else:
+        with torch.cuda.device(device_index):
+            status = fn(*args, stream)
+    if status != OK:
+        check(status)
+
+
 def dtype_code(t):
     try:
         return DTYPES[t.dtype]

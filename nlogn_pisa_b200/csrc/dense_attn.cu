@@ -392,12 +392,11 @@ __global__ void __launch_bounds__(kThreads) dense_dkv_kernel(const __grid_consta
   store_rows<T, R, DP>(static_cast<T*>(a.dv) + row0 * a.Dv, int64_t(a.H) * a.Dv, valid, a.Dv, ty, tx, dv, one);
 }
 
-template <typename K>
-int launch(K kernel, int64_t blocks, size_t smem, const DenseAttnArgs& a, cudaStream_t s) {
+template <auto Kernel>
+int launch(int64_t blocks, size_t smem, const DenseAttnArgs& a, cudaStream_t s) {
   if (blocks >= (int64_t(1) << 31)) return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
-  if (e != cudaSuccess) return fail_cuda(e, "dense attention smem attribute");
-  kernel<<<unsigned(blocks), kThreads, smem, s>>>(a);
+  if (int rc = allow_smem<Kernel>(int(smem), "dense attention smem attribute")) return rc;
+  Kernel<<<unsigned(blocks), kThreads, smem, s>>>(a);
   PISA_CHECK_LAUNCH();
   return PISA_OK;
 }
@@ -406,7 +405,7 @@ template <typename T, int DP>
 int fwd_t(const DenseAttnArgs& a, cudaStream_t s) {
   using L = Tile<DP>;
   const int64_t slots = seq_slots(a.cu_q, a.B, a.T, a.sequences, L::BT);
-  return launch(dense_fwd_kernel<T, DP>, slots * a.Hq, sizeof(float) * L::BT * (3 * L::LD + L::LP), a, s);
+  return launch<dense_fwd_kernel<T, DP>>(slots * a.Hq, sizeof(float) * L::BT * (3 * L::LD + L::LP), a, s);
 }
 
 template <typename T, int DP>
@@ -418,10 +417,10 @@ int bwd_t(const DenseAttnArgs& a, cudaStream_t s) {
                                                                  static_cast<const T*>(a.o), static_cast<const T*>(a.o_low),
                                                                  a.delta, rows, a.Dv);
   PISA_CHECK_LAUNCH();
-  int rc = launch(dense_dq_kernel<T, DP>, seq_slots(a.cu_q, a.B, a.T, a.sequences, L::BT) * a.Hq,
+  int rc = launch<dense_dq_kernel<T, DP>>(seq_slots(a.cu_q, a.B, a.T, a.sequences, L::BT) * a.Hq,
                   sizeof(float) * L::BT * (4 * L::LD + L::LP), a, s);
   if (rc) return rc;
-  return launch(dense_dkv_kernel<T, DP>, seq_slots(a.cu_q, a.B, a.N, a.sequences, L::BT) * a.H,
+  return launch<dense_dkv_kernel<T, DP>>(seq_slots(a.cu_q, a.B, a.N, a.sequences, L::BT) * a.H,
                 sizeof(float) * L::BT * (4 * L::LD + 2 * L::LP), a, s);
 }
 

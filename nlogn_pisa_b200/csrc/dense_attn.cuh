@@ -2,6 +2,8 @@
 // and the mapping from a grid slot to a tile of one sequence.
 #pragma once
 
+#include <atomic>
+
 #include "internal.h"
 
 namespace pisa {
@@ -40,6 +42,30 @@ struct DenseAttnArgs {
   void* dk;
   void* dv;
 };
+
+// Multiprocessors of the current device, asked once per device.
+inline int sm_count() {
+  static std::atomic<int> known[64];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+  if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+// Lets a kernel use `smem` bytes of dynamic shared memory, once per device.
+template <auto Kernel>
+int allow_smem(int smem, const char* where) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1)) return PISA_OK;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return fail_cuda(e, where);
+  if (dev < 64) done.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
+  return PISA_OK;
+}
 
 // Tile `tile` of one sequence.  Queries q_begin .. q_begin + q_len and keys
 // k_begin .. k_begin + k_len of batch row b; query i sits at position

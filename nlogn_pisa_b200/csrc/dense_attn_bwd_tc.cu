@@ -528,12 +528,11 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
   if (warp == kMmaWarp) tc::tmem_free(tmem, 512);
 }
 
-template <typename K>
-int launch(K kernel, int64_t blocks, int smem, const BwdTcArgs& a, cudaStream_t s) {
+template <auto Kernel>
+int launch(int64_t blocks, int smem, const BwdTcArgs& a, cudaStream_t s) {
   if (blocks >= (int64_t(1) << 31)) return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return fail_cuda(e, "dense attention smem attribute");
-  kernel<<<unsigned(blocks), kThreads, smem, s>>>(a);
+  if (int rc = allow_smem<Kernel>(smem, "dense attention smem attribute")) return rc;
+  Kernel<<<unsigned(blocks), kThreads, smem, s>>>(a);
   PISA_CHECK_LAUNCH();
   return PISA_OK;
 }
@@ -543,8 +542,8 @@ int bwd_t(const BwdTcArgs& a, cudaStream_t s) {
   const DenseAttnArgs& d = a.d;
   dense_stats_kernel<T><<<dim3(unsigned(a.q_slots), kRows / 16), 256, 0, s>>>(a);
   PISA_CHECK_LAUNCH();
-  int rc = launch(dense_dkv_tc_kernel<T, DP>, seq_slots(d.cu_q, d.B, d.N, d.sequences, kRows) * d.H, BwdTile<DP>::SMEM, a, s);
-  return rc ? rc : launch(dense_dq_tc_kernel<T, DP>, a.q_slots * d.Hq, BwdTile<DP>::SMEM, a, s);
+  int rc = launch<dense_dkv_tc_kernel<T, DP>>(seq_slots(d.cu_q, d.B, d.N, d.sequences, kRows) * d.H, BwdTile<DP>::SMEM, a, s);
+  return rc ? rc : launch<dense_dq_tc_kernel<T, DP>>(a.q_slots * d.Hq, BwdTile<DP>::SMEM, a, s);
 }
 
 }  // namespace

@@ -306,8 +306,7 @@ int fwd_t(const FwdTcArgs& a, cudaStream_t s) {
   using L = FwdTile<DP>;
   const int64_t blocks = seq_slots(a.d.cu_q, a.d.B, a.d.T, a.d.sequences, 2 * kRows) * a.d.Hq;
   if (blocks >= (int64_t(1) << 31)) return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
-  cudaError_t e = cudaFuncSetAttribute(dense_fwd_tc_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
-  if (e != cudaSuccess) return fail_cuda(e, "dense attention smem attribute");
+  if (int rc = allow_smem<dense_fwd_tc_kernel<T, DP>>(L::SMEM, "dense attention smem attribute")) return rc;
   dense_fwd_tc_kernel<T, DP><<<unsigned(blocks), kThreads, L::SMEM, s>>>(a);
   PISA_CHECK_LAUNCH();
   return PISA_OK;

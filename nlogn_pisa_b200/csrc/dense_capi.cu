@@ -12,14 +12,6 @@ namespace {
 
 int64_t round256(int64_t x) { return (x + 255) / 256 * 256; }
 
-int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0)
-    return 148;
-  return n;
-}
-
 bool rows16(const void* p, int dtype, int64_t sb, int64_t st, int64_t sh) {
   const int64_t v = dtype == PISA_F32 ? 4 : 8;
   return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && sb % v == 0 && st % v == 0 && sh % v == 0;

@@ -19,7 +19,7 @@
 // Lanes keep their columns over all rows they visit, so dw accumulates in
 // registers; each CTA stores one partial row and a second launch adds the
 // partials in a fixed order (no atomics: results do not vary from run to run).
-#include "internal.h"
+#include "dense_attn.cuh"
 
 namespace pisa {
 
@@ -240,13 +240,7 @@ __global__ void __launch_bounds__(128) norm_weight_kernel(const float* __restric
   else static_cast<T*>(out)[d] = from_f32<T>(v);
 }
 
-int max_ctas() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0)
-    n = 148;
-  return n * 4;
-}
+int max_ctas() { return sm_count() * 4; }
 
 template <typename T, int V>
 int launch(NormArgs a, bool bwd, cudaStream_t s) {

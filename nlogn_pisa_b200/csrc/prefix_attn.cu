@@ -229,8 +229,7 @@ template <typename T, int DP, int R>
 int launch(const PrefixArgs& a, bool prefix, cudaStream_t s) {
   constexpr int BR = 16 * R;
   const size_t smem = sizeof(float) * (BR * (DP + 4) + kKeys * (DP + 4) + BR * (kKeys + 1));
-  cudaError_t e = cudaFuncSetAttribute(prefix_simt_kernel<T, DP, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
-  if (e != cudaSuccess) return fail_cuda(e, "prefix attention smem attribute");
+  if (int rc = allow_smem<prefix_simt_kernel<T, DP, R>>(int(smem), "prefix attention smem attribute")) return rc;
   const int64_t rows = int64_t(prefix ? a.B : 1) * a.T * a.G;
   // heads of a key range side by side: their rows share DRAM pages
   const dim3 grid(unsigned((prefix ? a.prefix_splits : a.own_splits) * a.H), unsigned((rows + BR - 1) / BR),

@@ -413,8 +413,7 @@ template <typename T, int DP, int NR>
 int launch(const StreamArgs& s, int sms, cudaStream_t stream) {
   using L = Stream<DP, NR>;
   const PrefixArgs& a = s.p;
-  cudaError_t e = cudaFuncSetAttribute(prefix_stream_kernel<T, DP, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
-  if (e != cudaSuccess) return fail_cuda(e, "prefix attention smem attribute");
+  if (int rc = allow_smem<prefix_stream_kernel<T, DP, NR>>(L::SMEM, "prefix attention smem attribute")) return rc;
   const int64_t most = s.prefix_items + int64_t(a.B) * a.own_splits * s.own_blocks * a.H;
   const dim3 grid(unsigned(min64(sms, most)));
   if (s.after_tiles) return launch_after(prefix_stream_kernel<T, DP, NR>, grid, kThreads, L::SMEM, s, stream);

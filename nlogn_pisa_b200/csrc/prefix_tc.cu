@@ -245,8 +245,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
 template <typename T, int DP>
 int launch(const PrefixTcArgs& a, cudaStream_t s) {
   using L = PrefixTile<DP>;
-  cudaError_t e = cudaFuncSetAttribute(prefix_tc_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
-  if (e != cudaSuccess) return fail_cuda(e, "prefix attention smem attribute");
+  if (int rc = allow_smem<prefix_tc_kernel<T, DP>>(L::SMEM, "prefix attention smem attribute")) return rc;
   prefix_tc_kernel<T, DP><<<dim3(unsigned(a.p.prefix_splits * a.p.H), unsigned((a.tiles + 1) / 2)), kThreads, L::SMEM, s>>>(a);
   PISA_CHECK_LAUNCH();
   return PISA_OK;

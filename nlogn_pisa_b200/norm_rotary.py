@@ -13,25 +13,24 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .dense import aligned_rows, flat
+from .dense import aligned_rows, flat, view
 from .validation import require_cuda
 
 
 def _operands(q, k, q_weight, k_weight, frequency, positions, position_offset):
-    """The leading arguments of both entry points after the tensors."""
-    return (_lib.ptr(q_weight), _lib.ptr(k_weight), _lib.dtype_code(q_weight), _lib.ptr(frequency), _lib.ptr(positions),
-            0 if positions is None or positions.shape[0] == 1 else positions.stride(0), position_offset,
-            _lib.dtype_code(q), *q.shape[:3], k.shape[2], q.shape[3])
+    """The arguments that both entry points take after the gradients, from the weights on."""
+    batch, tokens, q_heads, dim = q.shape
+    at, at_sb = (None, 0) if positions is None else (positions.data_ptr(),
+                                                     0 if positions.shape[0] == 1 else positions.stride(0))
+    return (q_weight.data_ptr(), k_weight.data_ptr(), _lib.DTYPES[q_weight.dtype], frequency.data_ptr(), at, at_sb,
+            position_offset, _lib.DTYPES[q.dtype], batch, tokens, q_heads, k.shape[2], dim)
 
 
 def _forward(q, k, q_weight, k_weight, frequency, positions, position_offset, eps):
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    with torch.cuda.device(q.device):
-        _lib.check(_lib.lib().pisa_qk_norm_rotary(
-            _lib.ptr(q), *q.stride()[:3], _lib.ptr(k), *k.stride()[:3],
-            *_operands(q, k, q_weight, k_weight, frequency, positions, position_offset), eps, _lib.ptr(q_out),
-            _lib.ptr(k_out), _lib.stream_of(q.device)))
+    q_out, k_out = q.new_empty(q.shape), k.new_empty(k.shape)
+    _lib.launch(_lib.lib().pisa_qk_norm_rotary, q.get_device(), *view(q), *view(k),
+                *_operands(q, k, q_weight, k_weight, frequency, positions, position_offset), eps, q_out.data_ptr(),
+                k_out.data_ptr())
     return q_out, k_out
 
 
@@ -48,18 +47,15 @@ class QkNormRotaryFunction(torch.autograd.Function):
         q, k, q_weight, k_weight, frequency, positions = ctx.saved_tensors
         position_offset, eps = ctx.args
         dq_out, dk_out = flat(dq_out), flat(dk_out)
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
         dq_weight, dk_weight = torch.empty_like(q_weight), torch.empty_like(k_weight)
         library = _lib.lib()
-        with torch.cuda.device(q.device):
+        with torch.cuda.device(q.device):   # the size depends on the device's multiprocessors
             size = library.pisa_qk_norm_rotary_bwd_workspace_bytes(q.shape[0], q.shape[1], q.shape[3])
             workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
-            _lib.check(library.pisa_qk_norm_rotary_bwd(
-                _lib.ptr(q), *q.stride()[:3], _lib.ptr(k), *k.stride()[:3], _lib.ptr(dq_out), _lib.ptr(dk_out),
-                *_operands(q, k, q_weight, k_weight, frequency, positions, position_offset), eps, _lib.ptr(dq),
-                _lib.ptr(dk), _lib.ptr(dq_weight), _lib.ptr(dk_weight), _lib.ptr(workspace), size,
-                _lib.stream_of(q.device)))
+            _lib.launch(library.pisa_qk_norm_rotary_bwd, q.get_device(), *view(q), *view(k), dq_out.data_ptr(),
+                        dk_out.data_ptr(), *_operands(q, k, q_weight, k_weight, frequency, positions, position_offset), eps,
+                        dq.data_ptr(), dk.data_ptr(), dq_weight.data_ptr(), dk_weight.data_ptr(), workspace.data_ptr(), size)
         return dq, dk, dq_weight, dk_weight, None, None, None, None
 
 
@@ -72,26 +68,27 @@ def qk_norm_rotary(q, k, q_weight, k_weight, frequency, positions=None, position
     ``mixer.rotary_frequencies``; a zero leaves its pair unrotated);
     ``positions``: [1|B, T] integers, or None for ``position_offset`` + token.
     """
-    if q.ndim != 4 or k.ndim != 4:
+    if q.dim() != 4 or k.dim() != 4:
         raise ValueError("q and k must have shape [batch, tokens, heads, head_dim]")
-    if q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
+    a, b = q.shape, k.shape
+    if a[:2] != b[:2] or a[3] != b[3]:
         raise ValueError("q and k must share batch, tokens and head dimension")
-    if min(*q.shape, *k.shape) <= 0:
+    if 0 in a or 0 in b:
         raise ValueError("nonempty tensors are required")
-    if q.device != k.device or q.dtype != k.dtype or not q.is_floating_point():
+    if q.dtype != k.dtype or q.device != k.device or not q.is_floating_point():
         raise ValueError("q and k must share a floating dtype and device")
-    dim = q.shape[3]
+    dim = a[3]
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w.shape != (dim,) or w.dtype not in (torch.float32, q.dtype) or w.device != q.device:
+        if w.dim() != 1 or w.shape[0] != dim or w.dtype not in (torch.float32, q.dtype) or w.device != q.device:
             raise ValueError(f"{name} must have head_dim elements in fp32 or q's dtype on q's device")
     if q_weight.dtype != k_weight.dtype:
         raise ValueError("q_weight and k_weight must share a dtype")
-    if frequency.shape != (dim // 2,) or dim % 2:
+    if frequency.dim() != 1 or 2 * frequency.shape[0] != dim:
         raise ValueError("frequency must have head_dim / 2 elements")
-    if positions is not None and (positions.ndim != 2 or positions.shape[0] not in (1, q.shape[0])
-                                  or positions.shape[1] != q.shape[1] or positions.is_floating_point()):
+    if positions is not None and (positions.dim() != 2 or positions.shape[0] not in (1, a[0])
+                                  or positions.shape[1] != a[1] or positions.is_floating_point()):
         raise ValueError("positions must be integers of shape [1 or B, T]")
-    require_cuda(q, k, q_weight, k_weight)
+    require_cuda(q)
     _lib.dtype_code(q)
     frequency = frequency.to(device=q.device, dtype=torch.float32).contiguous()
     if positions is not None:
@@ -99,6 +96,6 @@ def qk_norm_rotary(q, k, q_weight, k_weight, frequency, positions=None, position
     q, k = aligned_rows(q), aligned_rows(k)
     q_weight, k_weight = q_weight.contiguous(), k_weight.contiguous()
     args = (q, k, q_weight, k_weight, frequency, positions, int(position_offset), float(eps))
-    if torch.is_grad_enabled() and any(t.requires_grad for t in args[:4]):
+    if any(t.requires_grad for t in args[:4]) and torch.is_grad_enabled():
         return QkNormRotaryFunction.apply(*args)
     return _forward(*args)
