@@ -59,6 +59,40 @@ def test_many_tokens(cuda_device, dtype):
     compare(*inputs(gen, 3, 4001, 4, 2, 64, dtype, F32))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("batch,tokens,heads,kv_heads,dim", [(3, 4001, 4, 2, 64), (1, 1000, 32, 8, 128), (7, 333, 5, 1, 80),
+                                                             (1, 5, 3, 3, 40)])
+def test_nothing_is_written_past_the_rows(cuda_device, dtype, batch, tokens, heads, kv_heads, dim):
+    """Both entry points on slices of larger buffers: the rows after the last stay as they were."""
+    from nlogn_pisa_b200 import _lib
+
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    rows, spare = batch * tokens, 512
+    lib, stream = _lib.lib(), torch.cuda.current_stream().cuda_stream
+    frequency, weight = torch.rand(dim // 2, device="cuda"), torch.ones(dim, device="cuda")
+
+    def buffers():
+        return [torch.full((rows + 2 * spare, h, dim), 7.0, dtype=dtype, device="cuda") for h in (heads, kv_heads)]
+
+    def at(t):
+        return t[spare:].data_ptr()
+
+    x, g, y, dx = ([normal(gen, rows + 2 * spare, h, dim, dtype=dtype) for h in (heads, kv_heads)], buffers(), buffers(), buffers())
+    common = (weight.data_ptr(), weight.data_ptr(), _lib.F32, frequency.data_ptr(), None, 0, 0, _lib.DTYPES[dtype], batch,
+              tokens, heads, kv_heads, dim, EPS)
+    views = [v for t, h in zip(x, (heads, kv_heads)) for v in (at(t), tokens * h * dim, h * dim, dim)]
+    _lib.check(lib.pisa_qk_norm_rotary(*views, *common, at(y[0]), at(y[1]), stream))
+    dw = torch.zeros(2, dim, device="cuda")
+    size = lib.pisa_qk_norm_rotary_bwd_workspace_bytes(batch, tokens, dim)
+    workspace = torch.full((size + 4096,), 85, dtype=torch.uint8, device="cuda")
+    _lib.check(lib.pisa_qk_norm_rotary_bwd(*views, at(g[0]), at(g[1]), *common, at(dx[0]), at(dx[1]), dw[0].data_ptr(),
+                                           dw[1].data_ptr(), workspace.data_ptr(), size, stream))
+    for t in (*y, *dx):
+        assert bool((t[:spare] == 7).all()) and bool((t[spare + rows:] == 7).all())
+        assert bool((t[spare:spare + rows] != 7).any(-1).all())
+    assert bool((workspace[size:] == 85).all())
+
+
 def test_layouts(cuda_device):
     gen = torch.Generator(device="cuda").manual_seed(2)
     q, k, qw, kw, frequency = inputs(gen, 2, 50, 4, 2, 64, BF16, BF16)
