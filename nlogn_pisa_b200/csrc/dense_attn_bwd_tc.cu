@@ -102,26 +102,6 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, 
   for (int c = 0; c < DP / 64; ++c) tc::tma_load_4d(dst + c * kRows * 128, map, c * 64, head, row, b, bar);
 }
 
-// D (+)= A B^T over DP dims, both operands K-major in shared memory.
-template <int DP>
-__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
-#pragma unroll
-  for (int s = 0; s < DP / 16; ++s) {
-    const uint32_t off = (s >> 2) * kRows * 128 + (s & 3) * 32;
-    tc::mma_f16(d, tc::desc_sw128(a + off), tc::desc_sw128(b + off), idesc, s > 0);
-  }
-}
-
-// D (+)= A B over the first `steps` * 16 rows of B; A in TMEM as two halves of
-// 64 columns each (32 registers of pairs, 64 columns apart), B MN-major.
-__device__ __forceinline__ void mma_cols(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int steps, bool accumulate) {
-#pragma unroll
-  for (int s = 0; s < kRows / 16; ++s)
-    if (s < steps)
-      tc::mma_f16_ts(d, a + (s >> 2) * 64 + (s & 3) * 8, tc::desc_make(b + s * 16 * 128, kRows * 128, 1024, 2), idesc,
-                     accumulate || s > 0);
-}
-
 struct Wait {
   int* fail;
   bool ok = true;
@@ -247,13 +227,13 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
         const int steps = ragged(n) ? (tail + 15) / 16 : kRows / 16;
         if (!wait(&p_full, n)) break;
         tc::fence_after_sync();
-        mma_cols(tV, tS, tile(2 * n + 1), id_o, steps, n > 0);
+        mma_cols(tV, tS, 64, tile(2 * n + 1), id_o, steps, n > 0);
         // a slot that no later tile takes is not handed back: nothing may arrive after the CTA's end
         if (2 * n + 1 + L::RING < 2 * total) tc::mma_commit(&empty[(2 * n + 1) % L::RING]);
         if (n + 1 < total) scores(n + 1);
         if (!wait(&ds_full, n)) break;
         tc::fence_after_sync();
-        mma_cols(tK, tP, tile(2 * n), id_o, steps, n > 0);
+        mma_cols(tK, tP, 64, tile(2 * n), id_o, steps, n > 0);
         if (2 * n + L::RING < 2 * total) tc::mma_commit(&empty[(2 * n) % L::RING]);
         if (n + 1 < total) grads(n + 1);
       }
@@ -451,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
         if (!wait(&ds_full, n)) break;
         tc::fence_after_sync();
         const int steps = n + 1 == total ? (tail + 15) / 16 : kRows / 16;
-        mma_cols(tQ, n & 1 ? tS[1] : tS[0], tile(2 * n), id_o, steps, n > 0);
+        mma_cols(tQ, n & 1 ? tS[1] : tS[0], 64, tile(2 * n), id_o, steps, n > 0);
         // a slot that no later tile takes is not handed back: nothing may arrive after the CTA's end
         if (2 * n + L::RING < 2 * total) tc::mma_commit(&empty[(2 * n) % L::RING]);
       }

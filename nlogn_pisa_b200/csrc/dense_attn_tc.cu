@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
   __shared__ uint64_t q_full[2], kv_full[L::STAGES], kv_empty[L::STAGES], s_full[2], p_full[2], o_done[2], drained;
   __shared__ uint32_t tmem_slot;
   __shared__ int s_fail;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
   // the last query tiles, which see the most keys, first; heads of a tile side by side
   const int index = int(gridDim.x) - 1 - int(blockIdx.x);
   const int slot = index / a.Hq, hq = index - slot * a.Hq;
@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  const uint32_t tmem = tmem_slot;
+  const uint32_t tmem = __shfl_sync(kFull, tmem_slot, 0);
   // TMEM columns: S/P of the two tiles, then their O
   const uint32_t tS[2] = {tmem, tmem + 128}, tO[2] = {tmem + 256, tmem + 256 + DP};
 
@@ -160,51 +160,49 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
-    if (lane == 0) {
-      const uint32_t id_s = tc::idesc_f16(kRows, kRows, args.bf16), id_o = tc::idesc_f16(kRows, DP, args.bf16, 1);
-      bool ok = true;
-      auto wait = [&](uint64_t* bar, int phase) {
-        if (ok && !tc::mbar_wait(bar, phase & 1)) { s_fail = 1; ok = false; }
-      };
-      for (int j = 0; j <= most && ok; ++j) {
-        const int nk = 2 * j, nv = 2 * j - 1;   // ring positions of K_j and V_{j-1}
+    const bool leader = elect_one();
+    const uint32_t id_s = tc::idesc_f16(kRows, kRows, args.bf16), id_o = tc::idesc_f16(kRows, DP, args.bf16, 1);
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, int phase) {
+      if (ok && !tc::mbar_wait(bar, phase & 1)) { s_fail = 1; ok = false; }
+      ok = __all_sync(kFull, ok);
+    };
+    for (int j = 0; j <= most && ok; ++j) {
+      const int nk = 2 * j, nv = 2 * j - 1;   // ring positions of K_j and V_{j-1}
+      const int sk = nk % L::STAGES, sv = (nv + L::STAGES) % L::STAGES;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (j >= 1 && j <= tiles[i]) {        // O += P V of key tile j - 1
-            wait(&kv_full[nv % L::STAGES], nv / L::STAGES);
-            wait(&p_full[i], j - 1);
-            if (!ok) break;
-            tc::fence_after_sync();
-            const uint32_t v = kv_addr + (nv % L::STAGES) * L::BYTES;
-#pragma unroll
-            for (int s = 0; s < kRows / 16; ++s)
-              tc::mma_f16_ts(tO[i], tS[i] + s * 8, tc::desc_make(v + s * 16 * 128, kRows * 128, 1024, 2), id_o,
-                             j > 1 || s > 0);
+      for (int i = 0; i < 2; ++i) {
+        if (j >= 1 && j <= tiles[i]) {        // O += P V of key tile j - 1
+          wait(&kv_full[sv], nv / L::STAGES);
+          wait(&p_full[i], j - 1);
+          if (!ok) break;
+          tc::fence_after_sync();
+          if (leader) {
+            mma_cols(tO[i], tS[i], 32, kv_addr + sv * L::BYTES, id_o, kRows / 16, j > 1);
             if (j == tiles[i]) tc::mma_commit(&o_done[i]);
           }
-          if (j < tiles[i]) {                   // S = Q K^T of key tile j
-            if (j == 0) wait(&q_full[i], 0);
-            wait(&kv_full[nk % L::STAGES], nk / L::STAGES);
-            if (!ok) break;
-            tc::fence_after_sync();
-            const uint32_t k = kv_addr + (nk % L::STAGES) * L::BYTES, q = q_addr + i * L::BYTES;
-#pragma unroll
-            for (int s = 0; s < DP / 16; ++s) {
-              const uint32_t off = (s >> 2) * kRows * 128 + (s & 3) * 32;
-              tc::mma_f16(tS[i], tc::desc_sw128(q + off), tc::desc_sw128(k + off), id_s, s > 0);
-            }
+        }
+        if (j < tiles[i]) {                   // S = Q K^T of key tile j
+          if (j == 0) wait(&q_full[i], 0);
+          wait(&kv_full[sk], nk / L::STAGES);
+          if (!ok) break;
+          tc::fence_after_sync();
+          if (leader) {
+            mma_rows<DP>(tS[i], q_addr + i * L::BYTES, kv_addr + sk * L::BYTES, id_s);
             tc::mma_commit(&s_full[i]);
           }
         }
-        if (!ok) break;
-        // a stage that no later tile takes is not handed back: nothing may arrive after the CTA's end
-        if (j >= 1 && nv + L::STAGES < 2 * most) tc::mma_commit(&kv_empty[nv % L::STAGES]);
-        if (j < most && nk + L::STAGES < 2 * most) tc::mma_commit(&kv_empty[nk % L::STAGES]);
       }
-      if (!ok) {
-        tc::mma_commit(&drained);
-        tc::mbar_wait(&drained, 0);
+      if (!ok) break;
+      // a stage that no later tile takes is not handed back: nothing may arrive after the CTA's end
+      if (leader) {
+        if (j >= 1 && nv + L::STAGES < 2 * most) tc::mma_commit(&kv_empty[sv]);
+        if (j < most && nk + L::STAGES < 2 * most) tc::mma_commit(&kv_empty[sk]);
       }
+    }
+    if (!ok && leader) {
+      tc::mma_commit(&drained);
+      tc::mbar_wait(&drained, 0);
     }
     __syncwarp();
   } else {

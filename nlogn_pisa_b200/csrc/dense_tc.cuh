@@ -43,6 +43,57 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
   return v;
 }
 
+// True in one lane of a converged warp.  The MMA warps run their control flow
+// and waits as a whole and issue under this predicate: values then stay in the
+// uniform registers that MMA operands come from.  (With one lane running the
+// role alone, an MMA took about 110 cycles to issue.)
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+// Shared-memory operand descriptors as (low word: address and leading offset,
+// high word: the rest); steps along K only change the low word.
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t lbo) { return ((addr & 0x3FFFFu) >> 4) | ((lbo >> 4) << 16); }
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);   // 8-row groups 1024 B apart, version 1, 128-byte swizzle
+
+// D[tmem] (+)= A[smem] * B[smem]
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_low, uint32_t b_low, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}"
+      :: "r"(d), "r"(a_low), "r"(b_low), "r"(idesc), "r"(uint32_t(accumulate)), "r"(kDescHigh) : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem]
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_low, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tmov.b64 b, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}"
+      :: "r"(d), "r"(a), "r"(b_low), "r"(idesc), "r"(uint32_t(accumulate)), "r"(kDescHigh) : "memory");
+}
+
+// D = A B^T over DP dims of two K-major tiles of 128 rows in shared memory.
+template <int DP>
+__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+  const uint32_t al = desc_low(a, 16), bl = desc_low(b, 16);
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) {
+    const uint32_t off = (s >> 2) * (kRows * 128 / 16) + (s & 3) * 2;
+    mma_ss(d, al + off, bl + off, idesc, s > 0);
+  }
+}
+
+// D (+)= A B over the first `steps` * 16 rows of the MN-major tile B; A in TMEM,
+// 8 columns per step, the second four steps `gap` columns after the first.
+__device__ __forceinline__ void mma_cols(uint32_t d, uint32_t a, uint32_t gap, uint32_t b, uint32_t idesc, int steps,
+                                         bool accumulate) {
+  const uint32_t bl = desc_low(b, kRows * 128);
+#pragma unroll
+  for (int s = 0; s < kRows / 16; ++s)
+    if (s < steps) mma_ts(d, a + (s >> 2) * gap + (s & 3) * 8, bl + s * (16 * 128 / 16), idesc, accumulate || s > 0);
+}
+
 // (a * b) on two lanes at once
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   float2 d;
