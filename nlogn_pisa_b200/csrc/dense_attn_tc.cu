@@ -165,37 +165,33 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
     bool ok = true;
     auto wait = [&](uint64_t* bar, int phase) {
       if (ok && !tc::mbar_wait(bar, phase & 1)) { s_fail = 1; ok = false; }
-      ok = __all_sync(kFull, ok);
     };
-    for (int j = 0; j <= most && ok; ++j) {
+    for (int j = 0; j <= most && __all_sync(kFull, ok); ++j) {
       const int nk = 2 * j, nv = 2 * j - 1;   // ring positions of K_j and V_{j-1}
       const int sk = nk % L::STAGES, sv = (nv + L::STAGES) % L::STAGES;
+      if (j >= 1) wait(&kv_full[sv], nv / L::STAGES);
+      if (j < most) wait(&kv_full[sk], nk / L::STAGES);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         if (j >= 1 && j <= tiles[i]) {        // O += P V of key tile j - 1
-          wait(&kv_full[sv], nv / L::STAGES);
           wait(&p_full[i], j - 1);
-          if (!ok) break;
           tc::fence_after_sync();
-          if (leader) {
+          if (leader && ok) {
             mma_cols(tO[i], tS[i], 32, kv_addr + sv * L::BYTES, id_o, kRows / 16, j > 1);
             if (j == tiles[i]) tc::mma_commit(&o_done[i]);
           }
         }
         if (j < tiles[i]) {                   // S = Q K^T of key tile j
           if (j == 0) wait(&q_full[i], 0);
-          wait(&kv_full[sk], nk / L::STAGES);
-          if (!ok) break;
           tc::fence_after_sync();
-          if (leader) {
+          if (leader && ok) {
             mma_rows<DP>(tS[i], q_addr + i * L::BYTES, kv_addr + sk * L::BYTES, id_s);
             tc::mma_commit(&s_full[i]);
           }
         }
       }
-      if (!ok) break;
       // a stage that no later tile takes is not handed back: nothing may arrive after the CTA's end
-      if (leader) {
+      if (leader && ok) {
         if (j >= 1 && nv + L::STAGES < 2 * most) tc::mma_commit(&kv_empty[sv]);
         if (j < most && nk + L::STAGES < 2 * most) tc::mma_commit(&kv_empty[sk]);
       }
