@@ -42,8 +42,10 @@ struct FwdTcArgs {
 template <int DP> struct FwdTile {
   static constexpr int CH = DP / 64;                    // 64-dim chunks
   static constexpr int BYTES = kRows * DP * 2;          // one operand tile
-  static constexpr int STAGES = DP == 128 ? 4 : 6;      // 64 dims: also keeps a second CTA off the SM's TMEM
-  static constexpr int SMEM = (2 + STAGES) * BYTES + 1024;
+  // ring stages of the values of one key tile and the keys of the next; three
+  // of 64 dims also keep a second CTA off the SM's TMEM
+  static constexpr int STAGES = DP == 128 ? 2 : 3;
+  static constexpr int SMEM = (2 + 2 * STAGES) * BYTES + 1024;
 };
 
 // Output row of query `i` summed over its visible keys alone, by one warp,
@@ -131,7 +133,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
   tc::fence_after_sync();
   const uint32_t tmem = __shfl_sync(kFull, tmem_slot, 0);
   // TMEM columns: S/P of the two tiles, then their O
-  const uint32_t tS[2] = {tmem, tmem + 128}, tO[2] = {tmem + 256, tmem + 256 + DP};
+  const uint32_t tS = tmem, tO = tmem + 256;
 
   if (warp == kLoadWarp) {
     if (lane == 0) {
@@ -143,19 +145,24 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
           tc::tma_load_4d(q_addr + i * L::BYTES + c * kRows * 128, &args.tm_q, c * 64, hq, t.q_begin + q0 + i * kRows, t.b,
                           &q_full[i]);
       }
-      for (int n = 0; n < 2 * most; ++n) {   // K0 V0 K1 V1 ...
-        const int st = n % L::STAGES;
-        if (!tc::mbar_wait(&kv_empty[st], ((n / L::STAGES) & 1) ^ 1)) {
+      for (int j = 0; j <= most; ++j) {   // V_{j-1} and K_j
+        const int st = j % L::STAGES;
+        if (most == 0) break;
+        if (!tc::mbar_wait(&kv_empty[st], ((j / L::STAGES) & 1) ^ 1)) {
           s_fail = 1;
           // the copies in flight land before the CTA ends
-          for (int x = max(0, n - L::STAGES); x < n; ++x) tc::mbar_wait(&kv_full[x % L::STAGES], (x / L::STAGES) & 1);
+          for (int x = max(0, j - L::STAGES); x < j; ++x) tc::mbar_wait(&kv_full[x % L::STAGES], (x / L::STAGES) & 1);
           break;
         }
-        tc::mbar_arrive_expect_tx(&kv_full[st], L::BYTES);
-        const CUtensorMap* map = n & 1 ? &args.tm_v : &args.tm_k;
-        for (int c = 0; c < L::CH; ++c)
-          tc::tma_load_4d(kv_addr + st * L::BYTES + c * kRows * 128, map, c * 64, h, t.k_begin + (n >> 1) * kRows, t.b,
-                          &kv_full[st]);
+        const uint32_t v = kv_addr + st * 2 * L::BYTES, k = v + L::BYTES;
+        tc::mbar_arrive_expect_tx(&kv_full[st], (int(j > 0) + int(j < most)) * L::BYTES);
+#pragma unroll 1
+        for (int c = 0; c < L::CH; ++c) {
+          if (j < most)
+            tc::tma_load_4d(k + c * kRows * 128, &args.tm_k, c * 64, h, t.k_begin + j * kRows, t.b, &kv_full[st]);
+          if (j > 0)
+            tc::tma_load_4d(v + c * kRows * 128, &args.tm_v, c * 64, h, t.k_begin + (j - 1) * kRows, t.b, &kv_full[st]);
+        }
       }
     }
     __syncwarp();
@@ -166,35 +173,31 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
     auto wait = [&](uint64_t* bar, int phase) {
       if (ok && !tc::mbar_wait(bar, phase & 1)) { s_fail = 1; ok = false; }
     };
-    for (int j = 0; j <= most && __all_sync(kFull, ok); ++j) {
-      const int nk = 2 * j, nv = 2 * j - 1;   // ring positions of K_j and V_{j-1}
-      const int sk = nk % L::STAGES, sv = (nv + L::STAGES) % L::STAGES;
-      if (j >= 1) wait(&kv_full[sv], nv / L::STAGES);
-      if (j < most) wait(&kv_full[sk], nk / L::STAGES);
-#pragma unroll
+    if (tiles[0]) wait(&q_full[0], 0);
+    if (tiles[1]) wait(&q_full[1], 0);
+    for (int j = 0; j <= most && most > 0 && __all_sync(kFull, ok); ++j) {
+      const int st = j % L::STAGES;
+      const uint32_t v = kv_addr + st * 2 * L::BYTES, k = v + L::BYTES;
+      wait(&kv_full[st], j / L::STAGES);      // V_{j-1} and K_j
+#pragma unroll 1
       for (int i = 0; i < 2; ++i) {
-        if (j >= 1 && j <= tiles[i]) {        // O += P V of key tile j - 1
-          wait(&p_full[i], j - 1);
-          tc::fence_after_sync();
-          if (leader && ok) {
-            mma_cols(tO[i], tS[i], 32, kv_addr + sv * L::BYTES, id_o, kRows / 16, j > 1);
-            if (j == tiles[i]) tc::mma_commit(&o_done[i]);
+        const int own = i ? tiles[1] : tiles[0];
+        if (j >= 1 && j <= own) wait(&p_full[i], j - 1);
+        tc::fence_after_sync();
+        if (leader && ok) {
+          if (j >= 1 && j <= own) {           // O += P V of key tile j - 1
+            mma_cols(tO + i * DP, tS + i * 128, 32, v, id_o, kRows / 16, j > 1);
+            if (j == own) tc::mma_commit(&o_done[i]);
           }
-        }
-        if (j < tiles[i]) {                   // S = Q K^T of key tile j
-          if (j == 0) wait(&q_full[i], 0);
-          tc::fence_after_sync();
-          if (leader && ok) {
-            mma_rows<DP>(tS[i], q_addr + i * L::BYTES, kv_addr + sk * L::BYTES, id_s);
+          if (j < own) {                      // S = Q K^T of key tile j
+            mma_rows<DP>(tS + i * 128, q_addr + i * L::BYTES, k, id_s);
             tc::mma_commit(&s_full[i]);
           }
         }
+        __syncwarp();
       }
       // a stage that no later tile takes is not handed back: nothing may arrive after the CTA's end
-      if (leader && ok) {
-        if (j >= 1 && nv + L::STAGES < 2 * most) tc::mma_commit(&kv_empty[sv]);
-        if (j < most && nk + L::STAGES < 2 * most) tc::mma_commit(&kv_empty[sk]);
-      }
+      if (leader && ok && j + L::STAGES <= most) tc::mma_commit(&kv_empty[st]);
     }
     if (!ok && leader) {
       tc::mma_commit(&drained);
@@ -205,7 +208,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
     const int i = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const int qi = q0 + i * kRows + row;             // query of this thread
     const uint32_t lane_base = uint32_t(quarter * 32) << 16;
-    const uint32_t ts = tS[i] + lane_base, to = tO[i] + lane_base;
+    const uint32_t ts = tS + i * 128 + lane_base, to = tO + i * DP + lane_base;
     const bool real = qi < t.q_len;
     const int last = real ? last_visible(a, t, qi) : -1;
     const float sl = a.scale * kLog2e;

@@ -74,13 +74,18 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_low, u
 }
 
 // D = A B^T over DP dims of two K-major tiles of 128 rows in shared memory.
+// (Loops over 64-dim chunks stay rolled here and below: the softmax warps sweep
+// the instruction caches, and every line of the MMA warp's code is fetched
+// again each step.)
 template <int DP>
 __device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
-  const uint32_t al = desc_low(a, 16), bl = desc_low(b, 16);
+  uint32_t al = desc_low(a, 16), bl = desc_low(b, 16);
+#pragma unroll 1
+  for (int c = 0; c < DP / 64; ++c) {
 #pragma unroll
-  for (int s = 0; s < DP / 16; ++s) {
-    const uint32_t off = (s >> 2) * (kRows * 128 / 16) + (s & 3) * 2;
-    mma_ss(d, al + off, bl + off, idesc, s > 0);
+    for (int s = 0; s < 4; ++s) mma_ss(d, al + s * 2, bl + s * 2, idesc, c + s > 0);
+    al += kRows * 128 / 16;
+    bl += kRows * 128 / 16;
   }
 }
 
@@ -88,10 +93,15 @@ __device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a, uint32_t b, uin
 // 8 columns per step, the second four steps `gap` columns after the first.
 __device__ __forceinline__ void mma_cols(uint32_t d, uint32_t a, uint32_t gap, uint32_t b, uint32_t idesc, int steps,
                                          bool accumulate) {
-  const uint32_t bl = desc_low(b, kRows * 128);
+  uint32_t bl = desc_low(b, kRows * 128);
+#pragma unroll 1
+  for (int c = 0; c < 2; ++c) {
 #pragma unroll
-  for (int s = 0; s < kRows / 16; ++s)
-    if (s < steps) mma_ts(d, a + (s >> 2) * gap + (s & 3) * 8, bl + s * (16 * 128 / 16), idesc, accumulate || s > 0);
+    for (int s = 0; s < 4; ++s)
+      if (4 * c + s < steps) mma_ts(d, a + s * 8, bl + s * (16 * 128 / 16), idesc, accumulate || c + s > 0);
+    a += gap;
+    bl += 4 * (16 * 128 / 16);
+  }
 }
 
 // (a * b) on two lanes at once
