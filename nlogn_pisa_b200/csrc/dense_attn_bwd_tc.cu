@@ -105,10 +105,12 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, 
 struct Wait {
   int* fail;
   bool ok = true;
-  __device__ __forceinline__ bool operator()(uint64_t* bar, int phase) {
-    if (ok && !tc::mbar_wait(bar, phase & 1)) { *fail = 1; ok = false; }
+  __device__ __forceinline__ bool operator()(uint64_t* bar, int phase) {   // one thread
+    if (ok && !wait_phase(bar, phase, fail)) ok = false;
     return ok;
   }
+  // a warp with collective work: it goes on after an expired wait
+  __device__ __forceinline__ void warp(uint64_t* bar, int phase) { ok = wait_phase(bar, phase, fail) && ok; }
 };
 
 // Launch 2.
@@ -159,7 +161,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
   // ring position 2n holds its Q (and statistics), 2n + 1 its dO
   // after an expired wait: the copies in flight land before the CTA ends
   auto drain = [&](int issued) {
-    for (int pos = max(0, issued - L::RING); pos < issued; ++pos) tc::mbar_wait(&full[pos % L::RING], (pos / L::RING) & 1);
+    for (int pos = max(0, issued - L::RING); pos < issued; ++pos) wait_phase(&full[pos % L::RING], pos / L::RING, &s_fail);
   };
   auto ragged = [&](int n) { return tail < kRows && (n + 1) % per_head == 0; };
 
@@ -191,15 +193,15 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
   } else if (warp == kTrimWarp) {
     if (tail < kRows && total > 0) {
       uint32_t uses = 0;   // parity of the ragged tiles that each ring slot has held
-      for (int n = per_head - 1; n < total && wait.ok; n += per_head) {
+      for (int n = per_head - 1; n < total; n += per_head) {
         for (int pos = 2 * n; pos < 2 * n + 2; ++pos) {
           const int st = pos % L::RING;
-          if (!wait(&raw[st], uses >> st)) break;
+          wait.warp(&raw[st], uses >> st);
           uses ^= 1u << st;
           zero_rows<DP>(ring + st * L::BYTES, tail, (tail + 15) & ~15, lane);
           tc::fence_async_smem();
           __syncwarp();
-          if (lane == 0) tc::mbar_arrive(&full[st]);
+          if (lane == 0 && wait.ok) tc::mbar_arrive(&full[st]);
         }
       }
     }
@@ -238,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
         if (n + 1 < total) grads(n + 1);
       }
       tc::mma_commit(&done);
-      if (!wait.ok) tc::mbar_wait(&done, 0);
+      if (!wait.ok) wait_phase(&done, 0, &s_fail);
     }
     __syncwarp();
   } else {
@@ -250,7 +252,8 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
     int qt = first_tile;
     for (int n = 0; n < total; ++n) {
       const int st = (2 * n) % L::RING;
-      if (!wait(&full[st], (2 * n) / L::RING) || !wait(&s_full, n)) break;
+      wait.warp(&full[st], (2 * n) / L::RING);
+      wait.warp(&s_full, n);
       tc::fence_after_sync();
       const float4* nlse = reinterpret_cast<const float4*>(stat_smem + (st / 2) * 256 + side * 64);
       const float4* ndel = nlse + kRows / 4;
@@ -281,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
       tc::fence_before_sync();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&p_full);
-      if (!wait(&dp_full, n)) break;
+      wait.warp(&dp_full, n);
       tc::fence_after_sync();
       float dp[64];
       tc::tmem_ld64(tp, dp);
@@ -306,7 +309,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
       if (lane == 0) tc::mbar_arrive(&ds_full);
       if (++qt == end_tile) qt = first_tile;
     }
-    if (total > 0) wait(&done, 0);
+    if (total > 0) wait.warp(&done, 0);
     tc::fence_after_sync();
     // warps of side 0 store dV, of side 1 dK, staged in the V and K tiles
     const int rows = min(32, t.k_len - (j0 + quarter * 32));
@@ -387,18 +390,17 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
       }
       if (!wait.ok)   // the copies in flight land before the CTA ends
         for (int pos = max(0, issued - L::RING); pos < issued; ++pos)
-          tc::mbar_wait(&full[pos % L::RING], (pos / L::RING) & 1);
+          wait_phase(&full[pos % L::RING], pos / L::RING, &s_fail);
     }
     __syncwarp();
   } else if (warp == kTrimWarp) {
     if (total > 0 && tail < kRows) {
       const int st = (2 * total - 2) % L::RING;
-      if (wait(&raw, 0)) {
-        zero_rows<DP>(ring + st * L::BYTES, tail, (tail + 15) & ~15, lane);
-        tc::fence_async_smem();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&full[st]);
-      }
+      wait.warp(&raw, 0);
+      zero_rows<DP>(ring + st * L::BYTES, tail, (tail + 15) & ~15, lane);
+      tc::fence_async_smem();
+      __syncwarp();
+      if (lane == 0 && wait.ok) tc::mbar_arrive(&full[st]);
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
@@ -436,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
         if (2 * n + L::RING < 2 * total) tc::mma_commit(&empty[(2 * n) % L::RING]);
       }
       tc::mma_commit(&done);
-      if (!wait.ok) tc::mbar_wait(&done, 0);
+      if (!wait.ok) wait_phase(&done, 0, &s_fail);
     }
     __syncwarp();
   } else {
@@ -455,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
     const int whole = (last_visible(a, t, q0) + 1) / kRows;   // key tiles that every row sees whole
     for (int n = 0; n < total; ++n) {
       const uint32_t ts = (n & 1 ? tS[1] : tS[0]) + lanes + side * 64;
-      if (!wait(&s_full[n & 1], n >> 1)) break;
+      wait.warp(&s_full[n & 1], n >> 1);
       tc::fence_after_sync();
       float p[64], dp[64];
       tc::tmem_ld64(ts, p);
@@ -465,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
         p[c] = tc::ex2f(u.x);
         p[c + 1] = tc::ex2f(u.y);
       }
-      if (!wait(&dp_full, n)) break;
+      wait.warp(&dp_full, n);
       tc::fence_after_sync();
       tc::tmem_ld64(tP + lanes + side * 64, dp);
       tc::fence_before_sync();
@@ -492,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&ds_full);
     }
-    if (total > 0) wait(&done, 0);
+    if (total > 0) wait.warp(&done, 0);
     tc::fence_after_sync();
     // each side stores half of the columns, staged in the Q tile (its last reader is done)
     const int rows = min(32, valid - quarter * 32);

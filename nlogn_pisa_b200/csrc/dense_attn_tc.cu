@@ -4,14 +4,16 @@
 // One CTA holds two tiles of 128 consecutive queries of one head and walks
 // the keys of their sequence in tiles of 128:
 //   MMA 1  S = Q K^T   (M = 128 queries, N = 128 keys)  -> TMEM
-//   softmax in registers, a thread per query row (no shuffles); P rounded to
-//          the input type overwrites S in TMEM
+//   softmax in registers, two threads per query row, 64 keys each (no
+//          shuffles); P rounded to the input type overwrites S in TMEM
 //   MMA 2  O += P V    (A = P from TMEM, B = V with keys along K) -> TMEM
-// The two query tiles take turns: while four warps turn tile 0's scores into
-// weights, the tensor core works for tile 1.  Warps 0-3 and 4-7 are the two
-// tiles' softmax warps, warp 8 issues the MMAs, warp 9 the TMA loads (a ring
-// of key and value tiles).  TMEM: S/P of both tiles and O of both fill 512
-// columns at 128 dims.
+// The two query tiles take turns: while eight warps turn tile 0's scores into
+// weights, the tensor core works for tile 1.  A tile's step is a chain (S,
+// softmax, P V), so its length decides: two threads per row halve the softmax
+// part and give every scheduler four warps to hide its latencies with.  Warps
+// 0-7 and 8-15 are the two tiles' softmax warps, warp 16 issues the MMAs, warp
+// 17 the TMA loads (a ring of value and key tiles).  TMEM: S/P of both tiles
+// and O of both fill 512 columns at 128 dims.
 //
 // The running maximum only moves when a row's new maximum passes the one in
 // use by 2^8: weights up to 256 are as exact in 16-bit floating point as
@@ -30,8 +32,8 @@ namespace pisa {
 
 namespace {
 
-constexpr int kMmaWarp = 8, kLoadWarp = 9;
-constexpr int kThreads = 320;
+constexpr int kMmaWarp = 16, kLoadWarp = 17;
+constexpr int kThreads = 576;
 
 struct FwdTcArgs {
   CUtensorMap tm_q, tm_k, tm_v;             // boxes of 64 dims x 128 rows of one head
@@ -95,6 +97,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
   const uint32_t base = (tc::smem_u32(smem_raw) + 1023) & ~1023u;
   const uint32_t q_addr = base, kv_addr = base + 2 * L::BYTES;
   __shared__ uint64_t q_full[2], kv_full[L::STAGES], kv_empty[L::STAGES], s_full[2], p_full[2], o_done[2], drained;
+  __shared__ float s_other[2][2][kRows];      // the halves' maxima, at the end their sums
   __shared__ uint32_t tmem_slot;
   __shared__ int s_fail;
   const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
@@ -116,7 +119,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&q_full[i], 1);
       tc::mbar_init(&s_full[i], 1);
-      tc::mbar_init(&p_full[i], 4);
+      tc::mbar_init(&p_full[i], 8);
       tc::mbar_init(&o_done[i], 1);
     }
     for (int i = 0; i < L::STAGES; ++i) {
@@ -148,10 +151,9 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
       for (int j = 0; j <= most; ++j) {   // V_{j-1} and K_j
         const int st = j % L::STAGES;
         if (most == 0) break;
-        if (!tc::mbar_wait(&kv_empty[st], ((j / L::STAGES) & 1) ^ 1)) {
-          s_fail = 1;
+        if (!wait_phase(&kv_empty[st], (j / L::STAGES) + 1, &s_fail)) {
           // the copies in flight land before the CTA ends
-          for (int x = max(0, j - L::STAGES); x < j; ++x) tc::mbar_wait(&kv_full[x % L::STAGES], (x / L::STAGES) & 1);
+          for (int x = max(0, j - L::STAGES); x < j; ++x) wait_phase(&kv_full[x % L::STAGES], x / L::STAGES, &s_fail);
           break;
         }
         const uint32_t v = kv_addr + st * 2 * L::BYTES, k = v + L::BYTES;
@@ -171,7 +173,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
     const uint32_t id_s = tc::idesc_f16(kRows, kRows, args.bf16), id_o = tc::idesc_f16(kRows, DP, args.bf16, 1);
     bool ok = true;
     auto wait = [&](uint64_t* bar, int phase) {
-      if (ok && !tc::mbar_wait(bar, phase & 1)) { s_fail = 1; ok = false; }
+      if (ok && !wait_phase(bar, phase, &s_fail)) ok = false;
     };
     if (tiles[0]) wait(&q_full[0], 0);
     if (tiles[1]) wait(&q_full[1], 0);
@@ -186,7 +188,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
         tc::fence_after_sync();
         if (leader && ok) {
           if (j >= 1 && j <= own) {           // O += P V of key tile j - 1
-            mma_cols(tO + i * DP, tS + i * 128, 32, v, id_o, kRows / 16, j > 1);
+            mma_cols(tO + i * DP, tS + i * 128, 64, v, id_o, kRows / 16, j > 1);
             if (j == own) tc::mma_commit(&o_done[i]);
           }
           if (j < own) {                      // S = Q K^T of key tile j
@@ -201,62 +203,68 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
     }
     if (!ok && leader) {
       tc::mma_commit(&drained);
-      tc::mbar_wait(&drained, 0);
+      wait_phase(&drained, 0, &s_fail);
     }
     __syncwarp();
   } else {
-    const int i = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    const int i = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3, row = quarter * 32 + lane;
     const int qi = q0 + i * kRows + row;             // query of this thread
-    const uint32_t lane_base = uint32_t(quarter * 32) << 16;
-    const uint32_t ts = tS + i * 128 + lane_base, to = tO + i * DP + lane_base;
+    const uint32_t lanes = uint32_t(quarter * 32) << 16;
+    const uint32_t ts = tS + i * 128 + half * 64 + lanes, to = tO + i * DP + half * (DP / 2) + lanes;
     const bool real = qi < t.q_len;
-    const int last = real ? last_visible(a, t, qi) : -1;
+    const int last = (real ? last_visible(a, t, qi) : -1) - half * 64;
     const float sl = a.scale * kLog2e;
-    float m = -INFINITY, l = 0.f;                    // base-2 logits
+    float m = -INFINITY, l = 0.f;                    // base-2 logits; l: of this half's keys
     bool ok = true;
+    const int own = i ? tiles[1] : tiles[0];
     const int full = (last_visible(a, t, q0 + i * kRows) + 1) / kRows;   // key tiles that every row sees whole
-    for (int j = 0; j < tiles[i]; ++j) {
-      if (!tc::mbar_wait(&s_full[i], j & 1)) { s_fail = 1; ok = false; break; }
+    for (int j = 0; j < own; ++j) {
+      ok = wait_phase(&s_full[i], j, &s_fail) && ok;
       tc::fence_after_sync();
-      softmax_tile<T, DP>(ts, to, sl, j == 0, j >= full ? last - j * kRows : kRows, m, l);
+      softmax_half<T, DP>(ts, to, sl, j == 0, j >= full ? last - j * kRows : kRows, 1 + i, s_other[i], half, row, m, l);
       tmem_wait_st();
       tc::fence_before_sync();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&p_full[i]);
     }
-    // O / l through this warp's rows of the query tile's shared memory (its
-    // last reader was the tile's last S, complete before o_done): whole rows
-    // to global memory
-    const bool any = tiles[i] > 0;
-    if (any && ok && !tc::mbar_wait(&o_done[i], 0)) { s_fail = 1; ok = false; }
-    tc::fence_after_sync();
+    // O / l: each half stores its columns, through its share of the query
+    // tile's shared memory (the tile's last S is complete before o_done)
+    const bool any = own > 0;
+    if (any) {
+      ok = wait_phase(&o_done[i], 0, &s_fail) && ok;
+      tc::fence_after_sync();
+      s_other[i][half][row] = l;
+      tc::named_sync(1 + i, 256);
+      l += s_other[i][half ^ 1][row];
+    }
     const float inv = !ok ? NAN : l == 0.f ? 0.f : 1.f / l;
-    constexpr int SEG = DP / 8;                      // 16-byte segments of a row
-    const uint32_t stage = q_addr + i * L::BYTES + quarter * 32 * DP * 2;
+    constexpr int W = DP / 2, SEG = W / 8;           // columns of a half, their 16-byte segments
+    const uint32_t stage = q_addr + i * L::BYTES + (half * 4 + quarter) * 32 * W * 2;
     const int64_t row0 = int64_t(t.b) * a.T + t.q_begin + q0 + i * kRows + quarter * 32;
     const int rows = min(32, t.q_len - (q0 + i * kRows + quarter * 32));
     // pass 0 stores the rounded output, pass 1 what the rounding dropped
+#pragma unroll 1
     for (int pass = 0; pass < (a.out_low ? 2 : 1); ++pass) {
       bool wild = false;
-#pragma unroll
-      for (int c = 0; c < DP; c += 32) {
-        float o[32];
-        if (any && ok) {
-          tc::tmem_ld32(to + c, o);
+#pragma unroll 1
+      for (int c = 0; c < W; c += 16) {
+        float o[16];
+        if (any) {
+          tc::tmem_ld16(to + c, o);
         } else {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0.f;
+          for (int e = 0; e < 16; ++e) o[e] = 0.f;
         }
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
+        for (int e = 0; e < 16; ++e) {
           wild = wild || isnan(o[e]);
           o[e] = l == 0.f && ok ? 0.f : o[e] * inv;
           if (pass) o[e] -= to_f32<T>(from_f32<T>(o[e]));
         }
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
+        for (int s = 0; s < 2; ++s) {
           const int seg = c / 8 + s;
-          st_shared16(stage + (lane * SEG + (seg ^ (lane & 7))) * 16, pack2<T>(o[8 * s], o[8 * s + 1]),
+          st_shared16(stage + (lane * SEG + (seg ^ (lane & (SEG - 1)))) * 16, pack2<T>(o[8 * s], o[8 * s + 1]),
                       pack2<T>(o[8 * s + 2], o[8 * s + 3]), pack2<T>(o[8 * s + 4], o[8 * s + 5]),
                       pack2<T>(o[8 * s + 6], o[8 * s + 7]));
         }
@@ -271,24 +279,25 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
                          acc);
 #pragma unroll
         for (int e = 0; e < DP / 32; ++e) {
-          const int d = lane + 32 * e;
+          const int d = lane + 32 * e - half * W;
           T v = from_f32<T>(acc[e]);
           if (pass) v = from_f32<T>(acc[e] - to_f32<T>(v));
-          asm volatile("st.shared.b16 [%0], %1;"
-                       :: "r"(stage + (r * SEG + ((d >> 3) ^ (r & 7))) * 16 + (d & 7) * 2),
-                          "h"(*reinterpret_cast<const uint16_t*>(&v)) : "memory");
+          if (d >= 0 && d < W)
+            asm volatile("st.shared.b16 [%0], %1;"
+                         :: "r"(stage + (r * SEG + ((d >> 3) ^ (r & (SEG - 1)))) * 16 + (d & 7) * 2),
+                            "h"(*reinterpret_cast<const uint16_t*>(&v)) : "memory");
         }
         __syncwarp();
       }
-      T* out = static_cast<T*>(pass ? a.out_low : a.out);
+      T* out = static_cast<T*>(pass ? a.out_low : a.out) + half * W;
       for (int f = lane; f < rows * SEG; f += 32) {
         const int r = f / SEG, seg = f % SEG;
-        const uint4 v = ld_shared16(stage + (r * SEG + (seg ^ (r & 7))) * 16);
-        if (seg * 8 < a.Dv) *reinterpret_cast<uint4*>(out + ((row0 + r) * a.Hq + hq) * a.Dv + seg * 8) = v;
+        const uint4 v = ld_shared16(stage + (r * SEG + (seg ^ (r & (SEG - 1)))) * 16);
+        if (half * W + seg * 8 < a.Dv) *reinterpret_cast<uint4*>(out + ((row0 + r) * a.Hq + hq) * a.Dv + seg * 8) = v;
       }
       __syncwarp();
     }
-    if (a.lse && real)
+    if (a.lse && real && half == 0)
       a.lse[(row0 + lane) * a.Hq + hq] = !ok ? NAN : l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
   }
   tc::fence_before_sync();

@@ -32,6 +32,13 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
          "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+      :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+         "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t x0, uint32_t x1, uint32_t x2, uint32_t x3) {
@@ -41,6 +48,33 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
   return v;
+}
+
+// Waits for the phase with parity `phase & 1` of `bar`, half a second at most
+// (tries that suspend a microsecond each).  An expired wait sets *fail and
+// returns false, as does a wait of a CTA whose *fail is set.  Warps with
+// collective work do not leave their loops on a false result, which their
+// lanes need not share: they go on, store NaN, and each further wait is short.
+static __device__ __noinline__ bool wait_long(uint32_t addr, uint32_t parity, int* fail) {
+#pragma unroll 1
+  for (uint32_t i = 0; i < (1u << 19); ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done) : "r"(addr), "r"(parity) : "memory");
+    if (done) return true;
+    if ((i & 255) == 255 && *static_cast<volatile int*>(fail)) return false;
+  }
+  *static_cast<volatile int*>(fail) = 1;
+  return false;
+}
+__device__ __forceinline__ bool wait_phase(uint64_t* bar, int phase, int* fail) {
+  const uint32_t addr = tc::smem_u32(bar), parity = uint32_t(phase & 1);
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done) : "r"(addr), "r"(parity) : "memory");
+  return done ? true : wait_long(addr, parity, fail);
 }
 
 // True in one lane of a converged warp.  The MMA warps run their control flow
@@ -240,6 +274,73 @@ __device__ __forceinline__ void softmax_tile(uint32_t ts, uint32_t to, float sl,
     w[c / 2] = pack2<T>(p.x, p.y);
   }
   tmem_st32(ts + 32, w);
+  l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
+}
+
+// OR of `mine` over `count` threads that meet at hardware barrier `id`.
+__device__ __forceinline__ bool any_of(int id, int count, bool mine) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %1, 0;\n\tbar.red.or.pred p, %2, %3, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r) : "r"(uint32_t(mine)), "r"(id), "r"(count) : "memory");
+  return r != 0;
+}
+
+// Half a tile's scores (64 keys) of this thread's row; another warp of the same
+// quarter holds the row's other half.  As softmax_tile, with the halves'
+// maxima exchanged through `other` (128 rows x 2) only when one of the tile's
+// 256 threads needs a new maximum.  `ts`: TMEM of the half's scores, whose
+// first 32 columns receive P; `to`: the half of O's columns that this thread
+// rescales.  Keys past `lim` (of the half) are hidden.
+template <typename T, int DP>
+__device__ __forceinline__ void softmax_half(uint32_t ts, uint32_t to, float sl, bool first, int lim, int barrier,
+                                             float (*other)[kRows], int half, int row, float& m, float& l) {
+  float x[64];
+  tc::tmem_ld64(ts, x);
+  if (lim < 63) {
+#pragma unroll
+    for (int c = 0; c < 64; ++c)
+      if (c > lim) x[c] = -INFINITY;
+  }
+  const float top = max_of(x) * sl;
+  if (any_of(barrier, 256, first || top > m + kRescale)) {
+    other[half][row] = top;
+    tc::named_sync(barrier, 256);
+    const float next = fmaxf(m, fmaxf(top, other[half ^ 1][row]));
+    const float alpha = next == -INFINITY ? 1.f : tc::ex2f(m - next);
+    m = next;
+    if (!first) {
+      l *= alpha;
+#pragma unroll 1
+      for (int c = 0; c < DP / 2; c += 16) {
+        float o[16];
+        uint32_t r[16];
+        tc::tmem_ld16(to + c, o);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(o[e] * alpha);
+        tc::tmem_st16(to + c, r);
+      }
+    }
+  }
+  const float ref = m == -INFINITY ? 0.f : m;
+  const float2 k2 = make_float2(sl, sl), c2 = make_float2(-ref, -ref);
+  float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t w[16];
+#pragma unroll
+    for (int c = 0; c < 32; c += 4) {
+      float2 p = tc::fma2(make_float2(x[32 * h + c], x[32 * h + c + 1]), k2, c2);
+      float2 q = tc::fma2(make_float2(x[32 * h + c + 2], x[32 * h + c + 3]), k2, c2);
+      p = make_float2(tc::ex2f(p.x), tc::ex2f(p.y));
+      q = make_float2(tc::ex2f(q.x), tc::ex2f(q.y));
+      sum0 = tc::add2(sum0, p);
+      sum1 = tc::add2(sum1, q);
+      w[c / 2] = pack2<T>(p.x, p.y);
+      w[c / 2 + 1] = pack2<T>(q.x, q.y);
+    }
+    tmem_st16(ts + 16 * h, w);
+  }
   l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
 }
 

@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_stream_kernel(const __grid
         const CUtensorMap* mv = x.prefix ? &args.tm_pv : &args.tm_v;
         for (int j = x.begin; j < x.end; j += kTile, ++n) {
           const int st = n % L::STAGES;
-          if (!tc::mbar_wait(&empty[st], ((n / L::STAGES) & 1) ^ 1)) { s_fail = 1; ok = false; break; }
+          if (!wait_phase(&empty[st], (n / L::STAGES) + 1, &s_fail)) { ok = false; break; }
           tc::mbar_arrive_expect_tx(&full[st], L::STAGE);
           const uint32_t k = base + st * L::STAGE, v = k + L::OPERAND;
 #pragma unroll
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_stream_kernel(const __grid
       }
       // after an expired wait: the copies in flight land before the CTA ends
       if (!ok)
-        for (int x = max(0, n - L::STAGES); x < n; ++x) tc::mbar_wait(&full[x % L::STAGES], (x / L::STAGES) & 1);
+        for (int x = max(0, n - L::STAGES); x < n; ++x) wait_phase(&full[x % L::STAGES], x / L::STAGES, &s_fail);
     }
   } else {
     const int g = lane >> 2, t = lane & 3, sub = warp & 3, side = warp >> 2;   // 16 keys of the CTA's even or odd tiles
@@ -246,9 +246,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_stream_kernel(const __grid
         }
       }
       const int tiles = (x.end - x.begin + kTile - 1) / kTile;
-      for (int u = (n ^ side) & 1; u < tiles && ok; u += 2) {   // tiles n + u of this side's parity
+      for (int u = (n ^ side) & 1; u < tiles; u += 2) {   // tiles n + u of this side's parity
         const int st = (n + u) % L::STAGES;
-        if (!tc::mbar_wait(&full[st], ((n + u) / L::STAGES) & 1)) { s_fail = 1; ok = false; break; }
+        ok = wait_phase(&full[st], (n + u) / L::STAGES, &s_fail) && ok;
         const uint32_t kt = base + st * L::STAGE + sub * 16 * 128, vt = kt + L::OPERAND;
         const int j = x.begin + u * kTile + sub * 16;      // first key of this warp
         if (j < x.end) {
@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_stream_kernel(const __grid
           }
         }
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&empty[st]);
+        if (lane == 0 && ok) tc::mbar_arrive(&empty[st]);
       }
       n += tiles;
       // Join: (m, l) per row and O of the eight warps through shared memory.
@@ -355,8 +355,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_stream_kernel(const __grid
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int at = warp * BR + 8 * r + 2 * t + e;
-          const float sum = groups_sum(l[r][e]);
-          if (g == 0) sml[at] = make_float2(m[r][e], ok ? sum : NAN);
+          const float sum = groups_sum(ok ? l[r][e] : NAN);
+          if (g == 0) sml[at] = make_float2(m[r][e], sum);
 #pragma unroll
           for (int c = 0; c < MT; ++c) {
             so[at * (DP + 4) + 16 * c + g] = o[r][c][e];

@@ -97,10 +97,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
       }
       for (int n = 0; n < 2 * keys; ++n) {   // K0 V0 K1 V1 ...
         const int st = n % L::STAGES;
-        if (!tc::mbar_wait(&kv_empty[st], ((n / L::STAGES) & 1) ^ 1)) {
-          s_fail = 1;
+        if (!wait_phase(&kv_empty[st], (n / L::STAGES) + 1, &s_fail)) {
           // the copies in flight land before the CTA ends
-          for (int x = max(0, n - L::STAGES); x < n; ++x) tc::mbar_wait(&kv_full[x % L::STAGES], (x / L::STAGES) & 1);
+          for (int x = max(0, n - L::STAGES); x < n; ++x) wait_phase(&kv_full[x % L::STAGES], x / L::STAGES, &s_fail);
           break;
         }
         tc::mbar_arrive_expect_tx(&kv_full[st], L::BYTES);
@@ -115,7 +114,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
       const uint32_t id_s = tc::idesc_f16(kRows, kRows, args.bf16), id_o = tc::idesc_f16(kRows, DP, args.bf16, 1);
       bool ok = true;
       auto wait = [&](uint64_t* bar, int phase) {
-        if (ok && !tc::mbar_wait(bar, phase & 1)) { s_fail = 1; ok = false; }
+        if (ok && !wait_phase(bar, phase, &s_fail)) ok = false;
       };
       // a stage that no later tile takes is not handed back: nothing may arrive after the CTA's end
       auto hand_back = [&](int pos) {
@@ -156,7 +155,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
       }
       if (!ok) {
         tc::mma_commit(&drained);
-        tc::mbar_wait(&drained, 0);
+        wait_phase(&drained, 0, &s_fail);
       }
     }
     __syncwarp();
@@ -168,7 +167,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int s = 0; s < steps[i]; ++s) {
-      if (!tc::mbar_wait(&s_full[i], s & 1)) { s_fail = 1; ok = false; break; }
+      ok = wait_phase(&s_full[i], s, &s_fail) && ok;
       tc::fence_after_sync();
       const int first = begin + (dual ? 2 * s + i : s) * kRows;
       softmax_tile<T, DP>(ts, to, sl, s == 0, end - 1 - first, m, l);
@@ -177,7 +176,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&p_full[i]);
     }
-    if (steps[i] && ok && !tc::mbar_wait(&o_done[i], 0)) { s_fail = 1; ok = false; }
+    if (steps[i]) ok = wait_phase(&o_done[i], 0, &s_fail) && ok;
     tc::fence_after_sync();
     if (!ok) l = NAN;
     // half 1's result joins half 0's when they hold the same rows
@@ -185,7 +184,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
     if (dual) {
       if (i == 1) {
         // the ring is free once half 0's last product is done, too
-        if (ok && !tc::mbar_wait(&o_done[0], 0)) { s_fail = 1; l = NAN; }
+        if (!wait_phase(&o_done[0], 0, &s_fail)) l = NAN;
         if (steps[1]) {
 #pragma unroll
           for (int c = 0; c < DP; c += 32) {
