@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
   __shared__ uint64_t kv_full, full[L::RING], raw[L::RING], empty[L::RING], s_full, p_full, dp_full, ds_full, done;
   __shared__ uint32_t tmem_slot;
   __shared__ int s_fail;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
   const int slot = int(blockIdx.x) / a.H, h = int(blockIdx.x) - slot * a.H;   // early keys, seen by most queries, first
   const SeqTile t = seq_tile(a, slot, kRows, true);
   const int j0 = t.tile * kRows;
@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  const uint32_t tmem = tmem_slot;
+  const uint32_t tmem = __shfl_sync(kFull, tmem_slot, 0);
   const uint32_t tS = tmem, tP = tmem + 128, tV = tmem + 256, tK = tmem + 256 + DP;
   Wait wait{&s_fail};
   // tile n: query head h*G + n / per_head, query tile first_tile + n % per_head;
@@ -207,40 +207,69 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
-    if (lane == 0 && total > 0) {
+    if (total > 0) {
+      const bool leader = elect_one();
       const uint32_t id_s = tc::idesc_f16(kRows, kRows, args.bf16), id_o = tc::idesc_f16(kRows, DP, args.bf16, 1);
-      auto tile = [&](int pos) { return ring + (pos % L::RING) * L::BYTES; };
-      auto scores = [&](int n) {
-        if (!wait(&full[(2 * n) % L::RING], (2 * n) / L::RING)) return;
-        tc::fence_after_sync();
-        mma_rows<DP>(tS, k_addr, tile(2 * n), id_s);
+      wait.warp(&kv_full, 0);
+      // per query tile n: S(n) and dP(n) are issued one round ahead of the
+      // products that use them, each after the last use of its TMEM columns
+      int pos = 0, st = 0;                      // ring position 2 n and its slot
+      uint32_t phase = 0;                       // the slot's phase
+      wait.warp(&full[0], 0);
+      tc::fence_after_sync();
+      if (leader) {
+        mma_rows<DP>(tS, k_addr, ring, id_s);
         tc::mma_commit(&s_full);
-      };
-      auto grads = [&](int n) {
-        if (!wait(&full[(2 * n + 1) % L::RING], (2 * n + 1) / L::RING)) return;
-        tc::fence_after_sync();
-        mma_rows<DP>(tP, v_addr, tile(2 * n + 1), id_s);
-        tc::mma_commit(&dp_full);
-      };
-      wait(&kv_full, 0);
-      if (wait.ok) scores(0);
-      if (wait.ok) grads(0);
-      for (int n = 0; n < total && wait.ok; ++n) {
-        const int steps = ragged(n) ? (tail + 15) / 16 : kRows / 16;
-        if (!wait(&p_full, n)) break;
-        tc::fence_after_sync();
-        mma_cols(tV, tS, 64, tile(2 * n + 1), id_o, steps, n > 0);
-        // a slot that no later tile takes is not handed back: nothing may arrive after the CTA's end
-        if (2 * n + 1 + L::RING < 2 * total) tc::mma_commit(&empty[(2 * n + 1) % L::RING]);
-        if (n + 1 < total) scores(n + 1);
-        if (!wait(&ds_full, n)) break;
-        tc::fence_after_sync();
-        mma_cols(tK, tP, 64, tile(2 * n), id_o, steps, n > 0);
-        if (2 * n + L::RING < 2 * total) tc::mma_commit(&empty[(2 * n) % L::RING]);
-        if (n + 1 < total) grads(n + 1);
       }
-      tc::mma_commit(&done);
-      if (!wait.ok) wait_phase(&done, 0, &s_fail);
+      wait.warp(&full[1], 0);
+      tc::fence_after_sync();
+      if (leader) {
+        mma_rows<DP>(tP, v_addr, ring + L::BYTES, id_s);
+        tc::mma_commit(&dp_full);
+      }
+      int left = per_head;                      // tiles to the head's last one
+      for (int n = 0; n < total && __all_sync(kFull, wait.ok); ++n) {
+        const bool rag = tail < kRows && left == 1;
+        left = left == 1 ? per_head : left - 1;
+        const int steps = rag ? (tail + 15) / 16 : kRows / 16;
+        const uint32_t q = ring + st * L::BYTES;
+        const int next = st + 2 == L::RING ? 0 : st + 2;
+        const uint32_t next_phase = next ? phase : phase ^ 1;
+        wait.warp(&p_full, n);
+        tc::fence_after_sync();
+        // a slot that no later tile takes is not handed back: nothing may arrive after the CTA's end
+        if (leader) {
+          mma_cols(tV, tS, 64, q + L::BYTES, id_o, steps, n > 0);
+          if (pos + 1 + L::RING < 2 * total) tc::mma_commit(&empty[st + 1]);
+        }
+        if (n + 1 < total) {
+          wait.warp(&full[next], int(next_phase));
+          tc::fence_after_sync();
+          if (leader) {
+            mma_rows<DP>(tS, k_addr, ring + next * L::BYTES, id_s);
+            tc::mma_commit(&s_full);
+          }
+        }
+        wait.warp(&ds_full, n);
+        tc::fence_after_sync();
+        if (leader) {
+          mma_cols(tK, tP, 64, q, id_o, steps, n > 0);
+          if (pos + L::RING < 2 * total) tc::mma_commit(&empty[st]);
+        }
+        if (n + 1 < total) {
+          wait.warp(&full[next + 1], int(next_phase));
+          tc::fence_after_sync();
+          if (leader) {
+            mma_rows<DP>(tP, v_addr, ring + (next + 1) * L::BYTES, id_s);
+            tc::mma_commit(&dp_full);
+          }
+        }
+        pos += 2;
+        st = next;
+        phase = next_phase;
+      }
+      if (leader) tc::mma_commit(&done);
+      if (!__all_sync(kFull, wait.ok)) wait_phase(&done, 0, &s_fail);
     }
     __syncwarp();
   } else {
@@ -340,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
   __shared__ uint64_t q_full, full[L::RING], raw, empty[L::RING], s_full[2], dp_full, dp_free, ds_full, done;
   __shared__ uint32_t tmem_slot;
   __shared__ int s_fail;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
   const int index = int(gridDim.x) - 1 - int(blockIdx.x);   // late queries, which see the most keys, first
   const int slot = index / a.Hq, hq = index - slot * a.Hq, h = hq / a.G;
   const SeqTile t = seq_tile(a, slot, kRows, false);
@@ -369,8 +398,8 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  const uint32_t tmem = tmem_slot;
-  const uint32_t tS[2] = {tmem, tmem + 128}, tP = tmem + 256, tQ = tmem + 384;   // dS overwrites its S
+  const uint32_t tmem = __shfl_sync(kFull, tmem_slot, 0);
+  const uint32_t tS = tmem, tP = tmem + 256, tQ = tmem + 384;   // two S, whose dS overwrites it; dP; dQ
   Wait wait{&s_fail};
 
   if (warp == kLoadWarp) {
@@ -404,41 +433,56 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
-    if (lane == 0 && total > 0) {
+    if (total > 0) {
+      const bool leader = elect_one();
       const uint32_t id_s = tc::idesc_f16(kRows, kRows, args.bf16), id_o = tc::idesc_f16(kRows, DP, args.bf16, 1);
-      auto tile = [&](int pos) { return ring + (pos % L::RING) * L::BYTES; };
-      auto scores = [&](int n) {
-        if (!wait(&full[(2 * n) % L::RING], (2 * n) / L::RING)) return;
-        tc::fence_after_sync();
-        mma_rows<DP>(n & 1 ? tS[1] : tS[0], q_addr, tile(2 * n), id_s);
-        tc::mma_commit(&s_full[n & 1]);
-      };
-      auto grads = [&](int n) {
-        if (!wait(&full[(2 * n + 1) % L::RING], (2 * n + 1) / L::RING)) return;
-        tc::fence_after_sync();
-        mma_rows<DP>(tP, o_addr, tile(2 * n + 1), id_s);
-        tc::mma_commit(&dp_full);
-        if (2 * n + 1 + L::RING < 2 * total) tc::mma_commit(&empty[(2 * n + 1) % L::RING]);
-      };
-      wait(&q_full, 0);
-      if (wait.ok) scores(0);
-      if (wait.ok) grads(0);
-      for (int n = 0; n < total && wait.ok; ++n) {
-        if (n + 1 < total) {
-          scores(n + 1);                      // its buffer held dS(n - 1), whose product was issued before
-          if (!wait(&dp_free, n)) break;      // dP(n) is in registers
-          tc::fence_after_sync();
-          grads(n + 1);
-        }
-        if (!wait(&ds_full, n)) break;
-        tc::fence_after_sync();
-        const int steps = n + 1 == total ? (tail + 15) / 16 : kRows / 16;
-        mma_cols(tQ, n & 1 ? tS[1] : tS[0], 64, tile(2 * n), id_o, steps, n > 0);
-        // a slot that no later tile takes is not handed back: nothing may arrive after the CTA's end
-        if (2 * n + L::RING < 2 * total) tc::mma_commit(&empty[(2 * n) % L::RING]);
+      wait.warp(&q_full, 0);
+      int st = 0;                               // slot of K(n); V(n) is in the next one
+      uint32_t phase = 0;
+      wait.warp(&full[0], 0);
+      tc::fence_after_sync();
+      if (leader) {
+        mma_rows<DP>(tS, q_addr, ring, id_s);
+        tc::mma_commit(&s_full[0]);
       }
-      tc::mma_commit(&done);
-      if (!wait.ok) wait_phase(&done, 0, &s_fail);
+      wait.warp(&full[1], 0);
+      tc::fence_after_sync();
+      // a slot that no later tile takes is not handed back: nothing may arrive after the CTA's end
+      if (leader) {
+        mma_rows<DP>(tP, o_addr, ring + L::BYTES, id_s);
+        tc::mma_commit(&dp_full);
+        if (1 + L::RING < 2 * total) tc::mma_commit(&empty[1]);
+      }
+      for (int n = 0; n < total && __all_sync(kFull, wait.ok); ++n) {
+        const int next = st + 2 == L::RING ? 0 : st + 2;
+        const uint32_t next_phase = next ? phase : phase ^ 1;
+        if (n + 1 < total) {
+          wait.warp(&full[next], int(next_phase));
+          tc::fence_after_sync();
+          if (leader) {                         // its buffer held dS(n - 1), whose product was issued before
+            mma_rows<DP>(tS + ((n + 1) & 1) * 128, q_addr, ring + next * L::BYTES, id_s);
+            tc::mma_commit(&s_full[(n + 1) & 1]);
+          }
+          wait.warp(&dp_free, n);               // dP(n) is in registers
+          wait.warp(&full[next + 1], int(next_phase));
+          tc::fence_after_sync();
+          if (leader) {
+            mma_rows<DP>(tP, o_addr, ring + (next + 1) * L::BYTES, id_s);
+            tc::mma_commit(&dp_full);
+            if (2 * n + 3 + L::RING < 2 * total) tc::mma_commit(&empty[next + 1]);
+          }
+        }
+        wait.warp(&ds_full, n);
+        tc::fence_after_sync();
+        if (leader) {
+          mma_cols(tQ, tS + (n & 1) * 128, 64, ring + st * L::BYTES, id_o, n + 1 == total ? (tail + 15) / 16 : kRows / 16, n > 0);
+          if (2 * n + L::RING < 2 * total) tc::mma_commit(&empty[st]);
+        }
+        st = next;
+        phase = next_phase;
+      }
+      if (leader) tc::mma_commit(&done);
+      if (!__all_sync(kFull, wait.ok)) wait_phase(&done, 0, &s_fail);
     }
     __syncwarp();
   } else {
@@ -456,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
     const float2 nlse2 = make_float2(nlse, nlse), ndel2 = make_float2(ndel, ndel);
     const int whole = (last_visible(a, t, q0) + 1) / kRows;   // key tiles that every row sees whole
     for (int n = 0; n < total; ++n) {
-      const uint32_t ts = (n & 1 ? tS[1] : tS[0]) + lanes + side * 64;
+      const uint32_t ts = tS + (n & 1) * 128 + lanes + side * 64;
       wait.warp(&s_full[n & 1], n >> 1);
       tc::fence_after_sync();
       float p[64], dp[64];
