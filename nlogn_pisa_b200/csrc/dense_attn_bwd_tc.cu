@@ -33,6 +33,12 @@ namespace {
 
 constexpr int kMmaWarp = 8, kLoadWarp = 9, kTrimWarp = 10;
 constexpr int kThreads = 352;
+// Pairs of every eight whose exponential is a polynomial.  The softmax warps of
+// a CTA do the same phase at the same time, so the special-function unit bounds
+// one phase and idles in the other.  Training block, four sequences of 4096, 16
+// heads of 64: dK/dV 374 us with 0, 368 with 2, 363 with 3, 367 with 4; dQ 260
+// with 0, 251 with 2, 254 with 3, 261 with 4.
+constexpr int kPolyKv = 3, kPolyQ = 2;
 
 struct BwdTcArgs {
   CUtensorMap tm_q, tm_k, tm_v, tm_do;   // boxes of 64 dims x 128 rows of one head
@@ -54,43 +60,59 @@ __device__ __forceinline__ float* stat_tile(const BwdTcArgs& a, int hq, int64_t 
   return a.stats + (hq * a.q_slots + slot) * 2 * kRows;
 }
 
-// Launch 1: 16 queries x all heads per CTA, half a warp per row.
-template <typename T>
+// Launch 1: kStatTokens queries x all heads per CTA, DP/8 lanes per row, each
+// with U rows requested at a time (bound by HBM: reads dout, out and out_low).
+constexpr int kStatTokens = 8;
+
+template <typename T, int DP>
 __global__ void __launch_bounds__(256) dense_stats_kernel(const __grid_constant__ BwdTcArgs args) {
+  constexpr int LANES = DP / 8, PER = 256 / LANES, U = 4;   // rows of the CTA at a time
   const DenseAttnArgs& a = args.d;
   const int slot = blockIdx.x;
   const SeqTile t = seq_tile(a, slot, kRows, false);
   const int q0 = t.tile * kRows;
   if (q0 >= t.q_len) return;
-  const int half = threadIdx.x >> 4, lane = threadIdx.x & 15;
+  const int lane = threadIdx.x % LANES, d = lane * 8, token0 = blockIdx.y * kStatTokens;
   const T* out = static_cast<const T*>(a.o);
+  const T* low = static_cast<const T*>(a.o_low);
   const T* dout = static_cast<const T*>(a.dout);
-  for (int x = half; x < 16 * a.Hq; x += 16) {
-    const int r = blockIdx.y * 16 + x / a.Hq, hq = x % a.Hq;
-    const bool real = q0 + r < t.q_len;
-    float dot = 0.f, lse = -INFINITY;
-    if (real) {
-      const int64_t row = (int64_t(t.b) * a.T + t.q_begin + q0 + r) * a.Hq + hq;
-      lse = a.lse_in[row];
-      for (int d = lane * 8; d < a.Dv; d += 128) {
-        float u[8], v[8];
-        load_vec<T>(out + row * a.Dv + d, u);
-        load_vec<T>(dout + row * a.Dv + d, v);
+  const int64_t first = (int64_t(t.b) * a.T + t.q_begin + q0 + token0) * a.Hq;   // row of the CTA's first
+  const int rows = kStatTokens * a.Hq, real = (t.q_len - q0 - token0) * a.Hq;     // consecutive in memory
+  for (int x0 = threadIdx.x / LANES; x0 < rows; x0 += U * PER) {
+    uint4 u[U], v[U], w[U];
+    float lse[U];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) dot = fmaf(u[e], v[e], dot);
-        if (a.o_low) {
-          load_vec<T>(static_cast<const T*>(a.o_low) + row * a.Dv + d, u);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) dot = fmaf(u[e], v[e], dot);
+    for (int i = 0; i < U; ++i) {
+      const int x = x0 + i * PER;
+      u[i] = v[i] = w[i] = make_uint4(0, 0, 0, 0);
+      lse[i] = -INFINITY;
+      if (x < rows && x < real) {
+        lse[i] = a.lse_in[first + x];
+        if (d < a.Dv) {
+          const int64_t at = (first + x) * a.Dv + d;
+          u[i] = __ldg(reinterpret_cast<const uint4*>(dout + at));
+          v[i] = __ldg(reinterpret_cast<const uint4*>(out + at));
+          if (low) w[i] = __ldg(reinterpret_cast<const uint4*>(low + at));
         }
       }
     }
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) dot += __shfl_xor_sync(kFull, dot, o);
-    if (lane == 0) {
-      float* st = stat_tile(args, hq, slot);
-      st[r] = lse == -INFINITY ? -INFINITY : -lse * kLog2e;
-      st[kRows + r] = -dot * a.scale;
+    for (int i = 0; i < U; ++i) {
+      const int x = x0 + i * PER;
+      const T* ue = reinterpret_cast<const T*>(&u[i]);
+      const T* ve = reinterpret_cast<const T*>(&v[i]);
+      const T* we = reinterpret_cast<const T*>(&w[i]);
+      float dot = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) dot = fmaf(to_f32<T>(ue[e]), to_f32<T>(ve[e]) + to_f32<T>(we[e]), dot);
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(kFull, dot, o);
+      if (lane == 0 && x < rows) {
+        const int token = x / a.Hq;
+        float* st = stat_tile(args, x - token * a.Hq, slot) + token0 + token;
+        st[0] = lse[i] == -INFINITY ? -INFINITY : -lse[i] * kLog2e;
+        st[kRows] = -dot * a.scale;
+      }
     }
   }
 }
@@ -292,14 +314,15 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
 #pragma unroll
       for (int c = 0; c < 64; c += 4) {
         const float4 x = nlse[c / 4];
-        const float2 u = tc::fma2(make_float2(p[c], p[c + 1]), sl2, make_float2(x.x, x.y));
-        const float2 v = tc::fma2(make_float2(p[c + 2], p[c + 3]), sl2, make_float2(x.z, x.w));
-        p[c] = tc::ex2f(u.x);
-        p[c + 1] = tc::ex2f(u.y);
-        p[c + 2] = tc::ex2f(v.x);
-        p[c + 3] = tc::ex2f(v.y);
+        const float2 u = ex2_mixed(tc::fma2(make_float2(p[c], p[c + 1]), sl2, make_float2(x.x, x.y)), c / 2, kPolyKv);
+        const float2 v = ex2_mixed(tc::fma2(make_float2(p[c + 2], p[c + 3]), sl2, make_float2(x.z, x.w)), c / 2 + 1, kPolyKv);
+        p[c] = u.x;
+        p[c + 1] = u.y;
+        p[c + 2] = v.x;
+        p[c + 3] = v.y;
       }
-      if (qt * kRows < whole || ragged(n)) {
+      const bool edge = qt * kRows < whole || ragged(n);
+      if (edge) {
         // queries before column `low` do not see the key, those from `high` on are not the sequence's
         const int low = first - qt * kRows - side * 64, high = t.q_len - qt * kRows - side * 64;
 #pragma unroll
@@ -328,9 +351,13 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
         dp[c + 2] = v.x;
         dp[c + 3] = v.y;
       }
-      // without weight no gradient, whatever dP holds there
+      if (edge) {   // without weight no gradient, whatever dP holds there
 #pragma unroll
-      for (int c = 0; c < 64; c += 2) w[c / 2] = pack2<T>(p[c] == 0.f ? 0.f : dp[c], p[c + 1] == 0.f ? 0.f : dp[c + 1]);
+        for (int c = 0; c < 64; ++c)
+          if (p[c] == 0.f) dp[c] = 0.f;
+      }
+#pragma unroll
+      for (int c = 0; c < 64; c += 2) w[c / 2] = pack2<T>(dp[c], dp[c + 1]);
       tmem_st32(tp, w);
       tmem_wait_st();
       tc::fence_before_sync();
@@ -507,9 +534,9 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
       tc::tmem_ld64(ts, p);
 #pragma unroll
       for (int c = 0; c < 64; c += 2) {
-        const float2 u = tc::fma2(make_float2(p[c], p[c + 1]), sl2, nlse2);
-        p[c] = tc::ex2f(u.x);
-        p[c + 1] = tc::ex2f(u.y);
+        const float2 u = ex2_mixed(tc::fma2(make_float2(p[c], p[c + 1]), sl2, nlse2), c / 2, kPolyQ);
+        p[c] = u.x;
+        p[c + 1] = u.y;
       }
       wait.warp(&dp_full, n);
       tc::fence_after_sync();
@@ -566,7 +593,7 @@ int launch(int64_t blocks, int smem, const BwdTcArgs& a, cudaStream_t s) {
 template <typename T, int DP>
 int bwd_t(const BwdTcArgs& a, cudaStream_t s) {
   const DenseAttnArgs& d = a.d;
-  dense_stats_kernel<T><<<dim3(unsigned(a.q_slots), kRows / 16), 256, 0, s>>>(a);
+  dense_stats_kernel<T, DP><<<dim3(unsigned(a.q_slots), kRows / kStatTokens), 256, 0, s>>>(a);
   PISA_CHECK_LAUNCH();
   int rc = launch<dense_dkv_tc_kernel<T, DP>>(seq_slots(d.cu_q, d.B, d.N, d.sequences, kRows) * d.H, BwdTile<DP>::SMEM, a, s);
   return rc ? rc : launch<dense_dq_tc_kernel<T, DP>>(a.q_slots * d.Hq, BwdTile<DP>::SMEM, a, s);

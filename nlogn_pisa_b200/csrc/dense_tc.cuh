@@ -210,6 +210,38 @@ __device__ __forceinline__ float max_of(const float (&v)[64]) {
   return fmaxf(tc::max3f(m[0], v[60], v[61]), fmaxf(tc::max3f(m[1], v[62], v[63]), fmaxf(m[2], m[3])));
 }
 
+// Largest of two values, NaN if one is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// 2^x of a pair on the FMA and integer pipes, beside the special-function
+// unit: x = j + f with |f| <= 1/2 by adding and taking away 1.5 * 2^23 + 127
+// (the sum's low bits then are the exponent field of 2^j), 2^f by a polynomial
+// of degree 4 fitted for least relative error on that range (iteratively
+// reweighted least squares), 2.7e-6, against 2^-9 and 2^-12 of the rounding to
+// bf16 or fp16 that follows.  For x <= 100; below -126 it stays at 2^-126, so
+// hidden elements are set to zero afterwards.
+__device__ __forceinline__ float2 ex2_pair(float2 x) {
+  const float2 magic = make_float2(12583039.f, 12583039.f), minus = make_float2(-12583039.f, -12583039.f);
+  x = make_float2(max_nan(x.x, -126.f), max_nan(x.y, -126.f));
+  const float2 t = tc::add2(x, magic);
+  const float2 f = tc::fma2(tc::add2(t, minus), make_float2(-1.f, -1.f), x);
+  float2 p = tc::fma2(make_float2(0.009570105f, 0.009570105f), f, make_float2(0.05591787f, 0.05591787f));
+  p = tc::fma2(p, f, make_float2(0.24024744f, 0.24024744f));
+  p = tc::fma2(p, f, make_float2(0.6931218f, 0.6931218f));
+  p = tc::fma2(p, f, make_float2(0.9999993f, 0.9999993f));
+  return mul2(p, make_float2(__uint_as_float(__float_as_uint(t.x) << 23), __uint_as_float(__float_as_uint(t.y) << 23)));
+}
+
+// 2^x of pair number `i`: `poly` pairs of every eight by polynomial, spread out.
+__device__ __forceinline__ float2 ex2_mixed(float2 x, int i, int poly) {
+  const bool by_poly = (i % 8 + 1) * poly / 8 > (i % 8) * poly / 8;
+  return by_poly ? ex2_pair(x) : make_float2(tc::ex2f(x.x), tc::ex2f(x.y));
+}
+
 constexpr float kRescale = 8.f;   // base-2 growth of a row maximum that moves it
 
 // One tile of 128 scores of this thread's row (TMEM columns ts ..): updates the
