@@ -7,8 +7,9 @@ selection and attention over the selected blocks (select_blocks /
 sparse_attention), the output projection, and the decode cache (PyramidCache
 for keys, TensorCache for values) with the same dictionary layout.  The
 config is duck-typed: any object with the PisaConfig field names
-(xmixers/xmixers/pisa_config.py:8-46) works.  Only the PISA selection methods
-(pisa, pisa1, pisa2) are served; full attention and NSA are other layers.
+(xmixers/xmixers/pisa_config.py:8-46) works.  PyramidSparseAttention serves the
+PISA selection methods (pisa, pisa1, pisa2), FullAttention the layers between
+them that see every key (attention_method "full"); NSA is another layer.
 """
 
 from __future__ import annotations
@@ -19,6 +20,8 @@ from torch import nn
 from . import _lib
 from .attention import sparse_attention
 from .cache import PyramidCache, TensorCache
+from .dense import full_attention, prefix_attention
+from .norm_rotary import qk_norm_rotary
 from .selection import select_blocks
 
 
@@ -135,6 +138,95 @@ class PyramidSparseAttention(nn.Module):
                                 leaf_tile=cfg.leaf_tile, routing_schedule=schedule, branching=self.branching)
         output = sparse_attention(q, k, v, indices, block_size=cfg.block_size, cu_seqlens=cu_seqlens,
                                   query_offset=offset)
+        if past_key_values is not None and use_cache:
+            while len(past_key_values) <= self.layer_idx:
+                past_key_values.append(None)
+            past_key_values[self.layer_idx] = next_cache
+            next_cache = past_key_values
+        return self.o_proj(output.reshape(batch, length, -1)), next_cache
+
+
+class FullAttention(nn.Module):
+    """Full-attention token mixer: projections, per-head norms of q and k with the
+    rotation (qk_norm_rotary), attention over all keys, output projection.
+
+    Training and prompts run full_attention (batches, or packed documents under
+    ``cu_seqlens``).  With a cache, up to ``DECODE_TOKENS`` new tokens per
+    sequence run prefix_attention over the cache, longer continuations
+    full_attention again.  ``share_prefix`` turns the cache of one prompt into
+    the start of a batch of answers to it, without copying its keys.
+    """
+
+    DECODE_TOKENS = 16
+
+    def __init__(self, config, layer_idx=0):
+        super().__init__()
+        if config.attention_method != "full":
+            raise ValueError(f"attention_method {config.attention_method!r} is not full attention")
+        self.config = config
+        self.layer_idx = layer_idx
+        q_width = config.num_attention_heads * config.head_dim
+        kv_width = config.num_key_value_heads * config.head_dim
+        self.q_proj = nn.Linear(config.hidden_size, q_width, bias=config.bias)
+        self.k_proj = nn.Linear(config.hidden_size, kv_width, bias=config.bias)
+        self.v_proj = nn.Linear(config.hidden_size, kv_width, bias=config.bias)
+        self.o_proj = nn.Linear(q_width, config.hidden_size, bias=config.bias)
+        self.q_norm = nn.Parameter(torch.ones(config.head_dim))
+        self.k_norm = nn.Parameter(torch.ones(config.head_dim))
+        self.eps = getattr(config, "rms_norm_eps", 1e-6)
+        self.register_buffer("theta", rotary_frequencies(config.head_dim, config.rope_theta, config.rope_fraction),
+                             persistent=False)
+
+    @staticmethod
+    def share_prefix(cache):
+        """A cache whose prompt (batch 1) is shared by the sequences that follow."""
+        if cache["k"].shape[0] != 1 or cache.get("prefix_k") is not None:
+            raise ValueError("a shared prefix is the cache of a single prompt")
+        return {"prefix_k": cache["k"][0], "prefix_v": cache["v"][0], "key_storage": None, "value_storage": None}
+
+    def forward(self, x, cu_seqlens=None, cache=None, use_cache=False, attention_mask=None, past_key_values=None, **kwargs):
+        if attention_mask is not None and not bool(attention_mask.all()):
+            raise ValueError("Remove evaluation padding before native attention")
+        if past_key_values is not None:
+            cache = past_key_values[self.layer_idx] if len(past_key_values) > self.layer_idx else None
+        if cache is not None and cu_seqlens is not None:
+            raise ValueError("packed documents start without a cache")
+        cfg = self.config
+        batch, length, _ = x.shape
+        q = self.q_proj(x).view(batch, length, cfg.num_attention_heads, cfg.head_dim)
+        k = self.k_proj(x).view(batch, length, cfg.num_key_value_heads, cfg.head_dim)
+        v = self.v_proj(x).view(batch, length, cfg.num_key_value_heads, cfg.head_dim)
+        prefix_k = prefix_v = None
+        past = shared = 0
+        if cache is not None:
+            prefix_k, prefix_v = cache.get("prefix_k"), cache.get("prefix_v")
+            shared = 0 if prefix_k is None else prefix_k.shape[0]
+            past = 0 if cache["key_storage"] is None else cache["key_storage"].length
+        positions = None
+        if cu_seqlens is not None and cfg.rope_position_mode == "document":
+            positions = token_positions(length, x.device, cu_seqlens)
+        q, k = qk_norm_rotary(q, k, self.q_norm.to(q.dtype), self.k_norm.to(q.dtype), self.theta, positions=positions,
+                              position_offset=shared + past, eps=self.eps)
+        keys, values = k, v
+        next_cache = None
+        if use_cache or cache is not None:
+            if cache is None or cache["key_storage"] is None:
+                stores = TensorCache.from_tensor(k.detach()), TensorCache.from_tensor(v.detach())
+            elif use_cache:
+                stores = cache["key_storage"].append(k.detach()), cache["value_storage"].append(v.detach())
+            else:   # a look ahead: the cache stays as it is
+                stores = (TensorCache.from_tensor(cache["key_storage"].tensor).append(k.detach()),
+                          TensorCache.from_tensor(cache["value_storage"].tensor).append(v.detach()))
+            if use_cache:
+                next_cache = {"k": stores[0].tensor, "v": stores[1].tensor, "key_storage": stores[0],
+                              "value_storage": stores[1], "prefix_k": prefix_k, "prefix_v": prefix_v}
+        if cache is not None and (shared or length <= self.DECODE_TOKENS):
+            lengths = torch.full((batch,), past + length, dtype=torch.int32, device=x.device)
+            output = prefix_attention(q, stores[0].buffer, stores[1].buffer, lengths, prefix_k=prefix_k, prefix_v=prefix_v)
+        else:
+            if cache is not None:
+                keys, values = stores[0].tensor, stores[1].tensor
+            output = full_attention(q, keys, values, cu_seqlens=cu_seqlens)
         if past_key_values is not None and use_cache:
             while len(past_key_values) <= self.layer_idx:
                 past_key_values.append(None)

@@ -1,9 +1,9 @@
-"""A LLaMA-style decoder block around the PISA token mixer, for training runs.
+"""A LLaMA-style decoder block around the PISA or the full-attention token mixer, for training runs.
 
 The block of the reference's xmixers LLaMA models
 (xmixers/xmixers/models/transformer/llama/modeling_llama.py): pre-norm
-RMSNorm -> PyramidSparseAttention -> residual, RMSNorm -> SwiGLU FFN ->
-residual.  Norms, projections and the FFN are ordinary torch operations (GEMMs
+RMSNorm -> PyramidSparseAttention (FullAttention with attention_method
+"full") -> residual, RMSNorm -> SwiGLU FFN -> residual.  Norms, projections and the FFN are ordinary torch operations (GEMMs
 on cuBLAS); the selection and the attention forward/backward run in this
 library.  Used by the benchmark's training configuration (one block,
 data-parallel over the GPUs of a node).
@@ -17,7 +17,7 @@ import torch
 from torch import nn
 import torch.nn.functional as F
 
-from .mixer import PyramidSparseAttention
+from .mixer import FullAttention, PyramidSparseAttention
 
 
 @dataclass
@@ -76,7 +76,7 @@ class DecoderBlock(nn.Module):
         super().__init__()
         self.embed = nn.Embedding(cfg.vocab_size, cfg.hidden_size)
         self.norm1 = RMSNorm(cfg.hidden_size, cfg.rms_norm_eps)
-        self.attn = PyramidSparseAttention(cfg)
+        self.attn = (FullAttention if cfg.attention_method == "full" else PyramidSparseAttention)(cfg)
         self.norm2 = RMSNorm(cfg.hidden_size, cfg.rms_norm_eps)
         self.ffn = SwiGLU(cfg.hidden_size, cfg.intermediate_size, cfg.bias)
         self.norm_out = RMSNorm(cfg.hidden_size, cfg.rms_norm_eps)
@@ -84,9 +84,9 @@ class DecoderBlock(nn.Module):
             if isinstance(m, (nn.Linear, nn.Embedding)):
                 nn.init.normal_(m.weight, std=cfg.init_std)
 
-    def forward(self, tokens):
+    def forward(self, tokens, cu_seqlens=None):
         x = self.embed(tokens)
-        a, _ = self.attn(self.norm1(x))
+        a, _ = self.attn(self.norm1(x), cu_seqlens=cu_seqlens)
         x = x + a
         x = x + self.ffn(self.norm2(x))
         return self.norm_out(x)
