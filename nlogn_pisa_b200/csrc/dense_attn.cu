@@ -19,6 +19,7 @@
 // products with hidden keys are skipped, not multiplied by zero, so
 // infinities and NaN in hidden places reach nothing.
 #include "dense_attn.cuh"
+#include "tc.cuh"
 
 namespace pisa {
 
@@ -43,9 +44,14 @@ __device__ __forceinline__ void stage(float* dst, const T* src, int64_t stride, 
   }
 }
 
-// acc[i][j] += a row (ty*R + i) . b row (tx + 16 j)
+// acc[i][j] += a row (ty*R + i) . b row (tx + 16 j), pairs of dims at a time
 template <int R, int DP, int LD>
 __device__ __forceinline__ void rows_dot(const float* a, const float* b, int ty, int tx, float (&acc)[R][R]) {
+  float2 sum[R][R];
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int j = 0; j < R; ++j) sum[i][j] = make_float2(0.f, 0.f);
 #pragma unroll 4
   for (int d = 0; d < DP; d += 4) {
     float4 x[R], y[R];
@@ -57,34 +63,54 @@ __device__ __forceinline__ void rows_dot(const float* a, const float* b, int ty,
     for (int i = 0; i < R; ++i) {
 #pragma unroll
       for (int j = 0; j < R; ++j) {
-        acc[i][j] = fmaf(x[i].x, y[j].x, acc[i][j]);
-        acc[i][j] = fmaf(x[i].y, y[j].y, acc[i][j]);
-        acc[i][j] = fmaf(x[i].z, y[j].z, acc[i][j]);
-        acc[i][j] = fmaf(x[i].w, y[j].w, acc[i][j]);
+        sum[i][j] = tc::fma2(make_float2(x[i].x, x[i].y), make_float2(y[j].x, y[j].y), sum[i][j]);
+        sum[i][j] = tc::fma2(make_float2(x[i].z, x[i].w), make_float2(y[j].z, y[j].w), sum[i][j]);
       }
     }
   }
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int j = 0; j < R; ++j) acc[i][j] += sum[i][j].x + sum[i][j].y;
 }
 
 // acc[i][c] += sum_j w[ty*R + i][j] x[j][columns of tx]; a weight outside
 // [lo[i], hi[i]] is skipped when `partial`.  Columns of tx: 4 from tx*4 + 64 c.
+// Four keys per step: a row of weights is one 16-byte load.  Rows of w past
+// `count` (to a multiple of four) are skipped as well.
 template <int R, int DP, int LD, int LP>
 __device__ __forceinline__ void rows_sum(const float* w, const float* x, int count, int ty, int tx, bool partial,
-                                         const int (&lo)[R], const int (&hi)[R], float (&acc)[R][DP / 16]) {
-  for (int j = 0; j < count; ++j) {
-    float p[R];
+                                         const int (&lo)[R], const int (&hi)[R], float2 (&acc)[R][DP / 32]) {
+  const int whole = partial ? 0 : count & ~3;
+#pragma unroll 2
+  for (int j = 0; j < whole; j += 4) {
+    float4 p[R];
 #pragma unroll
-    for (int i = 0; i < R; ++i) p[i] = w[(ty * R + i) * LP + j];
+    for (int i = 0; i < R; ++i) p[i] = *reinterpret_cast<const float4*>(w + (ty * R + i) * LP + j);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+#pragma unroll
+      for (int c = 0; c < DP / 64; ++c) {
+        const float4 y = *reinterpret_cast<const float4*>(x + (j + e) * LD + tx * 4 + 64 * c);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          const float v = e == 0 ? p[i].x : e == 1 ? p[i].y : e == 2 ? p[i].z : p[i].w;
+          acc[i][2 * c] = tc::fma2(make_float2(v, v), make_float2(y.x, y.y), acc[i][2 * c]);
+          acc[i][2 * c + 1] = tc::fma2(make_float2(v, v), make_float2(y.z, y.w), acc[i][2 * c + 1]);
+        }
+      }
+    }
+  }
+  for (int j = whole; j < count; ++j) {
 #pragma unroll
     for (int c = 0; c < DP / 64; ++c) {
       const float4 y = *reinterpret_cast<const float4*>(x + j * LD + tx * 4 + 64 * c);
 #pragma unroll
       for (int i = 0; i < R; ++i) {
         if (partial && (j < lo[i] || j > hi[i])) continue;
-        acc[i][4 * c + 0] = fmaf(p[i], y.x, acc[i][4 * c + 0]);
-        acc[i][4 * c + 1] = fmaf(p[i], y.y, acc[i][4 * c + 1]);
-        acc[i][4 * c + 2] = fmaf(p[i], y.z, acc[i][4 * c + 2]);
-        acc[i][4 * c + 3] = fmaf(p[i], y.w, acc[i][4 * c + 3]);
+        const float v = w[(ty * R + i) * LP + j];
+        acc[i][2 * c] = tc::fma2(make_float2(v, v), make_float2(y.x, y.y), acc[i][2 * c]);
+        acc[i][2 * c + 1] = tc::fma2(make_float2(v, v), make_float2(y.z, y.w), acc[i][2 * c + 1]);
       }
     }
   }
@@ -92,12 +118,12 @@ __device__ __forceinline__ void rows_sum(const float* w, const float* x, int cou
 
 template <int DP> struct Tile {
   static constexpr int R = DP <= 128 ? 4 : 2;   // 256 dims: tiles of 32 keep four of them in shared memory
-  static constexpr int BT = R * 16, LD = DP + 4, LP = BT + 1;
+  static constexpr int BT = R * 16, LD = DP + 4, LP = BT + 4;
 };
 
 template <typename T, int R, int DP>
 __device__ __forceinline__ void store_rows(T* dst, int64_t stride, int valid, int D, int ty, int tx,
-                                           const float (&acc)[R][DP / 16], const float (&mul)[R]) {
+                                           const float2 (&acc)[R][DP / 32], const float (&mul)[R]) {
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int r = ty * R + i;
@@ -107,7 +133,8 @@ __device__ __forceinline__ void store_rows(T* dst, int64_t stride, int valid, in
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int d = tx * 4 + 64 * c + e;
-        if (d < D) dst[r * stride + d] = from_f32<T>(acc[i][4 * c + e] * mul[i]);
+        const float2 v = acc[i][2 * c + e / 2];
+        if (d < D) dst[r * stride + d] = from_f32<T>((e & 1 ? v.y : v.x) * mul[i]);
       }
     }
   }
@@ -135,7 +162,8 @@ __global__ void __launch_bounds__(kThreads) dense_fwd_kernel(const __grid_consta
   const T* vp = static_cast<const T*>(a.v) + t.b * a.v_sb + int64_t(t.k_begin) * a.v_st + h * a.v_sh;
   stage<T, DP, LD>(qs, qp, a.q_st, BT, valid, a.D);
   const float sl = a.scale * kLog2e;
-  float acc[R][DP / 16], m[R], l[R];
+  float2 acc[R][DP / 32];
+  float m[R], l[R];
   int last[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
@@ -143,7 +171,7 @@ __global__ void __launch_bounds__(kThreads) dense_fwd_kernel(const __grid_consta
     l[i] = 0.f;
     last[i] = last_visible(a, t, q0 + ty * R + i);
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) acc[i][c] = 0.f;
+    for (int c = 0; c < DP / 32; ++c) acc[i][c] = make_float2(0.f, 0.f);
   }
   const int end = last_visible(a, t, q0 + valid - 1) + 1, full = last_visible(a, t, q0) + 1;
   for (int j0 = 0; j0 < end; j0 += BT) {
@@ -182,7 +210,7 @@ __global__ void __launch_bounds__(kThreads) dense_fwd_kernel(const __grid_consta
       for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
       l[i] = l[i] * corr[i] + sum;
 #pragma unroll
-      for (int c = 0; c < DP / 16; ++c) acc[i][c] *= corr[i];
+      for (int c = 0; c < DP / 32; ++c) acc[i][c] = make_float2(acc[i][c].x * corr[i], acc[i][c].y * corr[i]);
     }
     __syncwarp();   // the rows of ps that a warp reads are its own
     rows_sum<R, DP, LD, LP>(ps, vs, min(nk, end - j0), ty, tx, j0 + BT > full, lo, hi, acc);
@@ -202,9 +230,9 @@ __global__ void __launch_bounds__(kThreads) dense_fwd_kernel(const __grid_consta
 #pragma unroll
     for (int i = 0; i < R; ++i) {
 #pragma unroll
-      for (int c = 0; c < DP / 16; ++c) {
-        const float v = acc[i][c] * inv[i];
-        acc[i][c] = v - to_f32<T>(from_f32<T>(v));
+      for (int c = 0; c < DP / 32; ++c) {
+        const float2 v = make_float2(acc[i][c].x * inv[i], acc[i][c].y * inv[i]);
+        acc[i][c] = make_float2(v.x - to_f32<T>(from_f32<T>(v.x)), v.y - to_f32<T>(from_f32<T>(v.y)));
       }
       inv[i] = 1.f;
     }
@@ -274,7 +302,8 @@ __global__ void __launch_bounds__(kThreads) dense_dq_kernel(const __grid_constan
                    a.q_st, BT, valid, a.D);
   stage<T, DP, LD>(os, static_cast<const T*>(a.dout) + row0 * a.Dv, int64_t(a.Hq) * a.Dv, BT, valid, a.Dv);
   const float sl = a.scale * kLog2e;
-  float acc[R][DP / 16], lse2[R], delta[R];
+  float2 acc[R][DP / 32];
+  float lse2[R], delta[R];
   int last[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
@@ -283,7 +312,7 @@ __global__ void __launch_bounds__(kThreads) dense_dq_kernel(const __grid_constan
     lse2[i] = r < valid ? lse_base2(a.lse_in[row0 + int64_t(r) * a.Hq]) : 0.f;
     delta[i] = r < valid ? a.delta[row0 + int64_t(r) * a.Hq] : 0.f;
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) acc[i][c] = 0.f;
+    for (int c = 0; c < DP / 32; ++c) acc[i][c] = make_float2(0.f, 0.f);
   }
   const int end = last_visible(a, t, q0 + valid - 1) + 1, full = last_visible(a, t, q0) + 1;
   for (int j0 = 0; j0 < end; j0 += BT) {
@@ -337,14 +366,14 @@ __global__ void __launch_bounds__(kThreads) dense_dkv_kernel(const __grid_consta
   stage<T, DP, LD>(vs, static_cast<const T*>(a.v) + t.b * a.v_sb + int64_t(t.k_begin + j0) * a.v_st + h * a.v_sh,
                    a.v_st, BT, valid, a.Dv);
   const float sl = a.scale * kLog2e;
-  float dk[R][DP / 16], dv[R][DP / 16];
+  float2 dk[R][DP / 32], dv[R][DP / 32];
   int first[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int r = ty * R + i;
     first[i] = r < valid ? first_seeing(a, t, j0 + r) : t.q_len;
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) dk[i][c] = dv[i][c] = 0.f;
+    for (int c = 0; c < DP / 32; ++c) dk[i][c] = dv[i][c] = make_float2(0.f, 0.f);
   }
   const int begin = first_seeing(a, t, j0) / BT * BT, full = first_seeing(a, t, j0 + valid - 1);
   for (int g = 0; g < a.G; ++g) {
