@@ -135,16 +135,15 @@ __device__ __forceinline__ SeqTile seq_tile(const DenseAttnArgs& a, int slot, in
   return t;
 }
 
-// Tile of rank `rank` when all sequences' tiles are ordered by the work they
-// stand for, largest first (one warp; packed sequences, at most kRanked of
-// them).  Blocks start in order of their index, so the long tiles start early
-// and the short ones fill the end.  A lane knows a few sequences; how many
-// tiles cost at least c is a sum of closed forms, and bisection finds the cost
-// of the rank: some 300 instructions and no table.  Packed prompts of 1 to 4099
-// tokens, 32 heads: 343 us in sequence order, 254 us in this one.
+// Tile of rank `rank` when all sequences' query tiles are ordered by the keys
+// they meet, most first (one warp; at most kRanked packed sequences).  CTAs
+// take ranks in turn: long tiles start early and short ones fill the end.  A
+// lane knows a few sequences; how many tiles cost at least c is a sum of closed
+// forms, and bisection finds the cost of the rank: some 300 instructions, no
+// table and no launch.  t.q_len == 0: past every tile.
 constexpr int kRanked = 128;
 
-__device__ __forceinline__ SeqTile seq_tile_ranked(const DenseAttnArgs& a, int rank, int rows, bool by_keys) {
+__device__ __forceinline__ SeqTile query_tile_ranked(const DenseAttnArgs& a, int rank, int rows) {
   constexpr int PER = kRanked / 32;
   const int lane = threadIdx.x & 31;
   // sequence lane + 32 i: its tiles, the cost of the largest, and x with x - c tiles of cost c or more
@@ -157,11 +156,11 @@ __device__ __forceinline__ SeqTile seq_tile_ranked(const DenseAttnArgs& a, int r
     if (s > a.sequences) continue;
     const int qb = seq_begin(a, a.cu_q, a.T, s), kb = seq_begin(a, a.cu_k, a.N, s);
     const int ql = seq_end(a, a.cu_q, a.T, s, qb) - qb, kl = seq_end(a, a.cu_k, a.N, s, kb) - kb;
-    tiles[i] = ((by_keys ? kl : ql) + rows - 1) / rows;
+    tiles[i] = (ql + rows - 1) / rows;
     if (s == a.sequences || ql == 0 || kl == 0) continue;      // rows that meet nothing cost nothing
-    const int q_tiles = (ql + rows - 1) / rows, ahead = max(0, kl - ql) / rows;
-    top[i] = by_keys ? q_tiles : a.causal ? ahead + tiles[i] : (kl + rows - 1) / rows;
-    x[i] = by_keys ? ahead + q_tiles + 1 : ahead + tiles[i] + 1;
+    const int ahead = max(0, kl - ql) / rows;
+    top[i] = a.causal ? ahead + tiles[i] : (kl + rows - 1) / rows;
+    x[i] = ahead + tiles[i] + 1;
     most = max(most, top[i]);
   }
   auto at_least = [&](int i, int c) {
@@ -176,7 +175,7 @@ __device__ __forceinline__ SeqTile seq_tile_ranked(const DenseAttnArgs& a, int r
   };
   int lo = 0, hi = int(__reduce_max_sync(kFull, unsigned(most)));
   SeqTile t{};
-  if (rank >= count(0)) return t;   // past every tile: no rows
+  if (rank >= count(0)) return t;
   while (lo < hi) {         // the largest cost that more than `rank` tiles reach
     const int mid = (lo + hi + 1) >> 1;
     if (count(mid) > rank) lo = mid;
@@ -193,14 +192,11 @@ __device__ __forceinline__ SeqTile seq_tile_ranked(const DenseAttnArgs& a, int r
       const int y = __shfl_up_sync(kFull, up, o);
       if (lane >= o) up += y;
     }
-    const bool mine = !found && left >= up - n && left < up;
-    // larger costs lie at later query tiles, and at earlier key tiles
-    const int first = by_keys ? at_least(i, lo + 1) : tiles[i] - at_least(i, lo);
-    const unsigned who = __ballot_sync(kFull, mine);
+    const unsigned who = __ballot_sync(kFull, !found && left >= up - n && left < up);
     if (who) {
       const int src = __ffs(who) - 1;
       seq = src + 32 * i;
-      tile = __shfl_sync(kFull, first + left - (up - n), src);
+      tile = __shfl_sync(kFull, tiles[i] - at_least(i, lo) + left - (up - n), src);   // larger costs lie at later tiles
       found = true;
     }
     left -= __shfl_sync(kFull, up, 31);
@@ -209,22 +205,10 @@ __device__ __forceinline__ SeqTile seq_tile_ranked(const DenseAttnArgs& a, int r
   t.q_begin = seq_begin(a, a.cu_q, a.T, seq);
   t.k_begin = seq_begin(a, a.cu_k, a.N, seq);
   t.q_len = seq_end(a, a.cu_q, a.T, seq, t.q_begin) - t.q_begin;
-  t.k_len = seq_end(a, a.cu_k, a.N, seq, t.k_begin) - t.k_begin;
+  t.k_len = seq >= a.sequences ? 0 : seq_end(a, a.cu_k, a.N, seq, t.k_begin) - t.k_begin;
   t.tile = tile;
-  if (seq >= a.sequences) {
-    if (by_keys) t.q_len = 0;
-    else t.k_len = 0;
-  }
   t.shift = int64_t(t.k_len) - t.q_len;
   return t;
-}
-
-// The tile of block `index` of `count`, heaviest first as far as the order is
-// known: equal sequences by their tile number, few packed ones by rank, many
-// in sequence order.  One warp.
-__device__ __forceinline__ SeqTile seq_tile_ordered(const DenseAttnArgs& a, int index, int count, int rows, bool by_keys) {
-  if (a.cu_q != nullptr && a.sequences < kRanked) return seq_tile_ranked(a, index, rows, by_keys);
-  return seq_tile(a, by_keys ? index : count - 1 - index, rows, by_keys);
 }
 
 // Slot of query tile `tile` (of `rows` queries) of t's sequence: the inverse of seq_tile.

@@ -12,8 +12,13 @@
 // softmax, P V), so its length decides: two threads per row halve the softmax
 // part and give every scheduler four warps to hide its latencies with.  Warps
 // 0-7 and 8-15 are the two tiles' softmax warps, warp 16 issues the MMAs, warp
-// 17 the TMA loads (a ring of value and key tiles).  TMEM: S/P of both tiles
-// and O of both fill 512 columns at 128 dims.
+// 17 the TMA loads (a ring of value and key tiles), warp 18 finds the next
+// item.  TMEM: S/P of both tiles and O of both fill 512 columns at 128 dims.
+//
+// One persistent CTA per SM takes items in turn, those that meet the most keys
+// first; the loads and first scores of an item overlap the output of the one
+// before.  (A CTA per item paid for its start, and packed sequences in their own
+// order ended in a few long tiles.)
 //
 // The running maximum only moves when a row's new maximum passes the one in
 // use by 2^8: weights up to 256 are as exact in 16-bit floating point as
@@ -32,12 +37,13 @@ namespace pisa {
 
 namespace {
 
-constexpr int kMmaWarp = 16, kLoadWarp = 17;
-constexpr int kThreads = 576;
+constexpr int kSoftWarps = 16, kMmaWarp = 16, kLoadWarp = 17, kPlanWarp = 18;
+constexpr int kThreads = 608;
 
 struct FwdTcArgs {
   CUtensorMap tm_q, tm_k, tm_v;             // boxes of 64 dims x 128 rows of one head
   DenseAttnArgs d;
+  int items;                                // slots of query tile pairs x heads
   int bf16;
 };
 
@@ -49,6 +55,18 @@ template <int DP> struct FwdTile {
   static constexpr int STAGES = DP == 128 ? 2 : 3;
   static constexpr int SMEM = (2 + 2 * STAGES) * BYTES + 1024;
 };
+
+// 16 columns (8 registers of pairs) to global memory; those past `left` are not there.
+template <typename T>
+__device__ __forceinline__ void store16(T* p, const uint32_t (&r)[8], int left) {
+  if (left >= 16 && (reinterpret_cast<uintptr_t>(p) & 31) == 0) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 :: "l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+  } else {
+    if (left > 0) *reinterpret_cast<uint4*>(p) = make_uint4(r[0], r[1], r[2], r[3]);
+    if (left > 8) *reinterpret_cast<uint4*>(p + 8) = make_uint4(r[4], r[5], r[6], r[7]);
+  }
+}
 
 // Output row of query `i` summed over its visible keys alone, by one warp,
 // with the row's maximum m and weight sum l (base 2): acc[e] of column
@@ -89,6 +107,14 @@ __device__ __noinline__ void row_again(const DenseAttnArgs& a, const SeqTile& t,
   for (int e = 0; e < DP / 32; ++e) acc[e] *= inv;
 }
 
+// One work item: the pair of query tiles of one head.  The scheduler warp hands
+// items out one ahead of their use.
+struct Work {
+  SeqTile t;
+  int hq;        // -1: no more work
+  int tiles[2];  // key tiles that each query tile visits
+};
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_constant__ FwdTcArgs args) {
   using L = FwdTile<DP>;
@@ -96,31 +122,23 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t base = (tc::smem_u32(smem_raw) + 1023) & ~1023u;
   const uint32_t q_addr = base, kv_addr = base + 2 * L::BYTES;
-  __shared__ uint64_t q_full[2], kv_full[L::STAGES], kv_empty[L::STAGES], s_full[2], p_full[2], o_done[2], drained;
+  __shared__ uint64_t w_full[2], w_empty[2], q_full[2], q_empty[2], kv_full[L::STAGES], kv_empty[L::STAGES];
+  __shared__ uint64_t s_full[2], p_full[2], o_done[2], o_free[2], drained;
   __shared__ float s_other[2][2][kRows];      // the halves' maxima, at the end their sums
+  __shared__ Work s_work[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int s_fail;
   const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
-  // the last query tiles, which see the most keys, first; heads of a tile side by side
-  const int index = int(gridDim.x) - 1 - int(blockIdx.x);
-  const int slot = index / a.Hq, hq = index - slot * a.Hq;
-  const SeqTile t = seq_tile(a, slot, 2 * kRows, false);
-  const int q0 = t.tile * 2 * kRows;
-  if (q0 >= t.q_len) return;
-  // key tiles that each query tile visits
-  int tiles[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int first = q0 + i * kRows, rows = min(kRows, t.q_len - first);
-    tiles[i] = rows > 0 ? (last_visible(a, t, first + rows - 1) + kRows) / kRows : 0;
-  }
-  const int most = max(tiles[0], tiles[1]);
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&w_full[i], 1);
+      tc::mbar_init(&w_empty[i], kSoftWarps + 2);
       tc::mbar_init(&q_full[i], 1);
+      tc::mbar_init(&q_empty[i], 1);
       tc::mbar_init(&s_full[i], 1);
-      tc::mbar_init(&p_full[i], 8);
+      tc::mbar_init(&p_full[i], kSoftWarps / 2);
       tc::mbar_init(&o_done[i], 1);
+      tc::mbar_init(&o_free[i], kSoftWarps / 2);
     }
     for (int i = 0; i < L::STAGES; ++i) {
       tc::mbar_init(&kv_full[i], 1);
@@ -137,168 +155,270 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
   const uint32_t tmem = __shfl_sync(kFull, tmem_slot, 0);
   // TMEM columns: S/P of the two tiles, then their O
   const uint32_t tS = tmem, tO = tmem + 256;
+  bool ok = true;
+  // the next item (every lane of the calling warp), handed back when read
+  auto take = [&](int n) {
+    ok = wait_phase(&w_full[n & 1], n >> 1, &s_fail) && ok;
+    Work w = s_work[n & 1];
+    __syncwarp();
+    if (lane == 0 && ok) tc::mbar_arrive(&w_empty[n & 1]);
+    if (!__all_sync(kFull, ok)) w.hq = -1;
+    return w;
+  };
 
-  if (warp == kLoadWarp) {
-    if (lane == 0) {
-      const int h = hq / a.G;
-      for (int i = 0; i < 2; ++i) {
-        if (!tiles[i]) continue;
-        tc::mbar_arrive_expect_tx(&q_full[i], L::BYTES);
-        for (int c = 0; c < L::CH; ++c)
-          tc::tma_load_4d(q_addr + i * L::BYTES + c * kRows * 128, &args.tm_q, c * 64, hq, t.q_begin + q0 + i * kRows, t.b,
-                          &q_full[i]);
-      }
-      for (int j = 0; j <= most; ++j) {   // V_{j-1} and K_j
-        const int st = j % L::STAGES;
-        if (most == 0) break;
-        if (!wait_phase(&kv_empty[st], (j / L::STAGES) + 1, &s_fail)) {
-          // the copies in flight land before the CTA ends
-          for (int x = max(0, j - L::STAGES); x < j; ++x) wait_phase(&kv_full[x % L::STAGES], x / L::STAGES, &s_fail);
-          break;
+  if (warp == kPlanWarp) {
+    const int slots = args.items / a.Hq;
+    const bool ranked = a.cu_q != nullptr && a.sequences < kRanked;
+    int n = 0;
+    for (int round = 0;; ++round) {
+      // items are in falling order of their work: every other round goes
+      // backwards, or the first CTA would draw the longest of every round
+      const int g = int(gridDim.x), c = int(blockIdx.x), r = round * g + (round & 1 ? g - 1 - c : c);
+      Work w;
+      w.hq = -1;
+      if (r < args.items) {
+        const int slot = r / a.Hq;             // heads of a tile side by side
+        w.hq = r - slot * a.Hq;
+        w.t = ranked ? query_tile_ranked(a, slot, 2 * kRows) : seq_tile(a, slots - 1 - slot, 2 * kRows, false);
+        const int q0 = w.t.tile * 2 * kRows;
+        if (q0 >= w.t.q_len) {
+          if (!ranked) continue;               // a slot without rows
+          w.hq = -1;                           // ranks end here
         }
-        const uint32_t v = kv_addr + st * 2 * L::BYTES, k = v + L::BYTES;
-        tc::mbar_arrive_expect_tx(&kv_full[st], (int(j > 0) + int(j < most)) * L::BYTES);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int first = q0 + i * kRows, rows = min(kRows, w.t.q_len - first);
+          w.tiles[i] = rows > 0 ? (last_visible(a, w.t, first + rows - 1) + kRows) / kRows : 0;
+        }
+      }
+      ok = wait_phase(&w_empty[n & 1], (n >> 1) + 1, &s_fail) && ok;
+      if (!__all_sync(kFull, ok)) w.hq = -1;
+      if (lane == 0) {
+        s_work[n & 1] = w;
+        tc::mbar_arrive(&w_full[n & 1]);
+      }
+      __syncwarp();
+      if (w.hq < 0) break;
+      ++n;
+    }
+  } else if (warp == kLoadWarp) {
+    int st = 0, uses[2] = {0, 0};              // ring slot; items that used each query tile
+    uint32_t phase = 0;
+    int loads = 0;
+    for (int n = 0;; ++n) {
+      const Work w = take(n);
+      if (w.hq < 0) break;
+      if (lane == 0) {
+        const int h = w.hq / a.G, most = max(w.tiles[0], w.tiles[1]);
 #pragma unroll 1
-        for (int c = 0; c < L::CH; ++c) {
-          if (j < most)
-            tc::tma_load_4d(k + c * kRows * 128, &args.tm_k, c * 64, h, t.k_begin + j * kRows, t.b, &kv_full[st]);
-          if (j > 0)
-            tc::tma_load_4d(v + c * kRows * 128, &args.tm_v, c * 64, h, t.k_begin + (j - 1) * kRows, t.b, &kv_full[st]);
+        for (int j = 0; j <= most && most > 0 && ok; ++j) {   // V_{j-1} and K_j; the queries before K_0
+          if (j == 0) {
+#pragma unroll 1
+            for (int i = 0; i < 2; ++i) {
+              if (!w.tiles[i]) continue;
+              ok = wait_phase(&q_empty[i], uses[i] + 1, &s_fail) && ok;
+              if (!ok) break;
+              ++uses[i];
+              tc::mbar_arrive_expect_tx(&q_full[i], L::BYTES);
+              for (int c = 0; c < L::CH; ++c)
+                tc::tma_load_4d(q_addr + i * L::BYTES + c * kRows * 128, &args.tm_q, c * 64, w.hq,
+                                w.t.q_begin + (w.t.tile * 2 + i) * kRows, w.t.b, &q_full[i]);
+            }
+          }
+          ok = ok && wait_phase(&kv_empty[st], int(phase) + 1, &s_fail);
+          if (!ok) break;
+          const uint32_t v = kv_addr + st * 2 * L::BYTES, k = v + L::BYTES;
+          tc::mbar_arrive_expect_tx(&kv_full[st], (int(j > 0) + int(j < most)) * L::BYTES);
+#pragma unroll 1
+          for (int c = 0; c < L::CH; ++c) {
+            if (j < most)
+              tc::tma_load_4d(k + c * kRows * 128, &args.tm_k, c * 64, h, w.t.k_begin + j * kRows, w.t.b, &kv_full[st]);
+            if (j > 0)
+              tc::tma_load_4d(v + c * kRows * 128, &args.tm_v, c * 64, h, w.t.k_begin + (j - 1) * kRows, w.t.b, &kv_full[st]);
+          }
+          ++loads;
+          if (++st == L::STAGES) {
+            st = 0;
+            phase ^= 1;
+          }
         }
       }
+      ok = __all_sync(kFull, ok);
+    }
+    if (lane == 0) {
+      // nothing may arrive after the CTA's end: every stage and query tile has
+      // been handed back (after an expired wait: the copies in flight have landed)
+      for (int x = max(0, loads - L::STAGES); x < loads; ++x)
+        wait_phase(ok ? &kv_empty[x % L::STAGES] : &kv_full[x % L::STAGES], x / L::STAGES, &s_fail);
+      for (int i = 0; i < 2; ++i)
+        if (uses[i]) wait_phase(ok ? &q_empty[i] : &q_full[i], uses[i] - 1, &s_fail);
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
     const bool leader = elect_one();
     const uint32_t id_s = tc::idesc_f16(kRows, kRows, args.bf16), id_o = tc::idesc_f16(kRows, DP, args.bf16, 1);
-    bool ok = true;
-    auto wait = [&](uint64_t* bar, int phase) {
-      if (ok && !wait_phase(bar, phase, &s_fail)) ok = false;
+    int st = 0;
+    uint32_t phase = 0, p_phase = 0;                          // bit i: of query tile i
+    int uses[2] = {0, 0};                                     // items that used each query tile
+    auto next_stage = [&]() {
+      if (leader && ok) tc::mma_commit(&kv_empty[st]);
+      if (++st == L::STAGES) {
+        st = 0;
+        phase ^= 1;
+      }
     };
-    if (tiles[0]) wait(&q_full[0], 0);
-    if (tiles[1]) wait(&q_full[1], 0);
-    for (int j = 0; j <= most && most > 0 && __all_sync(kFull, ok); ++j) {
-      const int st = j % L::STAGES;
-      const uint32_t v = kv_addr + st * 2 * L::BYTES, k = v + L::BYTES;
-      wait(&kv_full[st], j / L::STAGES);      // V_{j-1} and K_j
+    for (int n = 0;; ++n) {
+      const Work w = take(n);
+      if (w.hq < 0) break;
+      const int most = max(w.tiles[0], w.tiles[1]);
+      if (most == 0) continue;
+      ok = wait_phase(&kv_full[st], int(phase), &s_fail) && ok;   // K_0
 #pragma unroll 1
       for (int i = 0; i < 2; ++i) {
-        const int own = i ? tiles[1] : tiles[0];
-        if (j >= 1 && j <= own) wait(&p_full[i], j - 1);
+        const int own = i ? w.tiles[1] : w.tiles[0];
+        if (own == 0) continue;
+        ok = wait_phase(&q_full[i], i ? uses[1] : uses[0], &s_fail) && ok;
         tc::fence_after_sync();
         if (leader && ok) {
-          if (j >= 1 && j <= own) {           // O += P V of key tile j - 1
-            mma_cols(tO + i * DP, tS + i * 128, 64, v, id_o, kRows / 16, j > 1);
-            if (j == own) tc::mma_commit(&o_done[i]);
-          }
-          if (j < own) {                      // S = Q K^T of key tile j
-            mma_rows<DP>(tS + i * 128, q_addr + i * L::BYTES, k, id_s);
-            tc::mma_commit(&s_full[i]);
-          }
+          mma_rows<DP>(tS + i * 128, q_addr + i * L::BYTES, kv_addr + (2 * st + 1) * L::BYTES, id_s);
+          tc::mma_commit(&s_full[i]);
+          if (own == 1) tc::mma_commit(&q_empty[i]);
         }
         __syncwarp();
       }
-      // a stage that no later tile takes is not handed back: nothing may arrive after the CTA's end
-      if (leader && ok && j + L::STAGES <= most) tc::mma_commit(&kv_empty[st]);
+      next_stage();
+      // the tiles' O of the item before has been read out
+      for (int i = 0; i < 2; ++i) {
+        if (w.tiles[i] == 0) continue;
+        if (uses[i] > 0) ok = wait_phase(&o_free[i], uses[i] - 1, &s_fail) && ok;
+        ++uses[i];
+      }
+      for (int j = 1; j <= most && __all_sync(kFull, ok); ++j) {
+        const uint32_t v = kv_addr + st * 2 * L::BYTES, k = v + L::BYTES;
+        ok = wait_phase(&kv_full[st], int(phase), &s_fail) && ok;      // V_{j-1} and K_j
+#pragma unroll 1
+        for (int i = 0; i < 2; ++i) {
+          const int own = i ? w.tiles[1] : w.tiles[0];
+          if (j > own) continue;
+          ok = wait_phase(&p_full[i], int(p_phase >> i), &s_fail) && ok;
+          p_phase ^= 1u << i;
+          tc::fence_after_sync();
+          if (leader && ok) {
+            mma_cols(tO + i * DP, tS + i * 128, 64, v, id_o, kRows / 16, j > 1);   // O += P V of key tile j - 1
+            if (j < own) {                      // S = Q K^T of key tile j
+              mma_rows<DP>(tS + i * 128, q_addr + i * L::BYTES, k, id_s);
+              tc::mma_commit(&s_full[i]);
+              if (j + 1 == own) tc::mma_commit(&q_empty[i]);
+            } else {
+              tc::mma_commit(&o_done[i]);
+            }
+          }
+          __syncwarp();
+        }
+        next_stage();
+      }
     }
-    if (!ok && leader) {
-      tc::mma_commit(&drained);
+    if (!__all_sync(kFull, ok)) {
+      if (leader) tc::mma_commit(&drained);
       wait_phase(&drained, 0, &s_fail);
     }
     __syncwarp();
   } else {
     const int i = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3, row = quarter * 32 + lane;
-    const int qi = q0 + i * kRows + row;             // query of this thread
     const uint32_t lanes = uint32_t(quarter * 32) << 16;
-    const uint32_t ts = tS + i * 128 + half * 64 + lanes, to = tO + i * DP + half * (DP / 2) + lanes;
-    const bool real = qi < t.q_len;
-    const int last = (real ? last_visible(a, t, qi) : -1) - half * 64;
+    constexpr int W = DP / 2;                        // columns of a half
+    const uint32_t ts = tS + i * 128 + half * 64 + lanes, to = tO + i * DP + half * W + lanes;
     const float sl = a.scale * kLog2e;
-    float m = -INFINITY, l = 0.f;                    // base-2 logits; l: of this half's keys
-    bool ok = true;
-    const int own = i ? tiles[1] : tiles[0];
-    const int full = (last_visible(a, t, q0 + i * kRows) + 1) / kRows;   // key tiles that every row sees whole
-    for (int j = 0; j < own; ++j) {
-      ok = wait_phase(&s_full[i], j, &s_fail) && ok;
-      tc::fence_after_sync();
-      softmax_half<T, DP>(ts, to, sl, j == 0, j >= full ? last - j * kRows : kRows, 1 + i, s_other[i], half, row, m, l);
-      tmem_wait_st();
-      tc::fence_before_sync();
+    int step = 0, done = 0;                          // score tiles and items of this query tile so far
+    for (int n = 0;; ++n) {
+      // the item stays in shared memory while it is worked on: registers are short
+      ok = wait_phase(&w_full[n & 1], n >> 1, &s_fail) && ok;
+      const Work& w = s_work[n & 1];
+      if (w.hq < 0 || !__all_sync(kFull, ok)) break;
+      int last, own, full;                           // full: key tiles that every row sees whole
+      {
+        const SeqTile t = w.t;
+        const int q0 = (t.tile * 2 + i) * kRows;
+        last = (q0 + row < t.q_len ? last_visible(a, t, q0 + row) : -1) - half * 64;
+        full = (last_visible(a, t, q0) + 1) / kRows;
+        own = w.tiles[i];
+      }
+      float m = -INFINITY, l = 0.f;                  // base-2 logits; l: of this half's keys
+      for (int j = 0; j < own; ++j, ++step) {
+        ok = wait_phase(&s_full[i], step, &s_fail) && ok;
+        tc::fence_after_sync();
+        softmax_half<T, DP>(ts, to, sl, j == 0, j >= full ? last - j * kRows : kRows, 1 + i, s_other[i], half, row, m, l);
+        tmem_wait_st();
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&p_full[i]);
+      }
+      if (own > 0) {
+        ok = wait_phase(&o_done[i], done++, &s_fail) && ok;
+        tc::fence_after_sync();
+        s_other[i][half][row] = l;
+        tc::named_sync(1 + i, 256);
+        l += s_other[i][half ^ 1][row];
+      }
+      const SeqTile t = w.t;
+      const int hq = w.hq, qi = (t.tile * 2 + i) * kRows + row;   // query of this thread
+      const bool real = qi < t.q_len;
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&p_full[i]);
-    }
-    // O / l: each half stores its columns, through its share of the query
-    // tile's shared memory (the tile's last S is complete before o_done)
-    const bool any = own > 0;
-    if (any) {
-      ok = wait_phase(&o_done[i], 0, &s_fail) && ok;
-      tc::fence_after_sync();
-      s_other[i][half][row] = l;
-      tc::named_sync(1 + i, 256);
-      l += s_other[i][half ^ 1][row];
-    }
-    const float inv = !ok ? NAN : l == 0.f ? 0.f : 1.f / l;
-    constexpr int W = DP / 2, SEG = W / 8;           // columns of a half, their 16-byte segments
-    const uint32_t stage = q_addr + i * L::BYTES + (half * 4 + quarter) * 32 * W * 2;
-    const int64_t row0 = int64_t(t.b) * a.T + t.q_begin + q0 + i * kRows + quarter * 32;
-    const int rows = min(32, t.q_len - (q0 + i * kRows + quarter * 32));
-    // pass 0 stores the rounded output, pass 1 what the rounding dropped
-#pragma unroll 1
-    for (int pass = 0; pass < (a.out_low ? 2 : 1); ++pass) {
+      if (lane == 0) tc::mbar_arrive(&w_empty[n & 1]);
+      // O / l, stored by each thread for its half of the row (128 or 64
+      // consecutive bytes); pass 1 stores what the rounding dropped
+      const float inv = !ok ? NAN : l == 0.f ? 0.f : 1.f / l;
+      const int64_t at = (int64_t(t.b) * a.T + t.q_begin + qi) * a.Hq + hq;
       bool wild = false;
 #pragma unroll 1
       for (int c = 0; c < W; c += 16) {
         float o[16];
-        if (any) {
+        if (own > 0) {
           tc::tmem_ld16(to + c, o);
         } else {
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[e] = 0.f;
         }
+        uint32_t r[8], d[8];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          wild = wild || isnan(o[e]);
-          o[e] = l == 0.f && ok ? 0.f : o[e] * inv;
-          if (pass) o[e] -= to_f32<T>(from_f32<T>(o[e]));
+        for (int e = 0; e < 16; e += 2) {
+          wild = wild || isnan(o[e]) || isnan(o[e + 1]);
+          const float x = l == 0.f && ok ? 0.f : o[e] * inv, y = l == 0.f && ok ? 0.f : o[e + 1] * inv;
+          r[e / 2] = pack2<T>(x, y);
+          d[e / 2] = pack2<T>(x - to_f32<T>(from_f32<T>(x)), y - to_f32<T>(from_f32<T>(y)));
         }
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const int seg = c / 8 + s;
-          st_shared16(stage + (lane * SEG + (seg ^ (lane & (SEG - 1)))) * 16, pack2<T>(o[8 * s], o[8 * s + 1]),
-                      pack2<T>(o[8 * s + 2], o[8 * s + 3]), pack2<T>(o[8 * s + 4], o[8 * s + 5]),
-                      pack2<T>(o[8 * s + 6], o[8 * s + 7]));
+        const int col = half * W + c;
+        if (real) {
+          store16<T>(static_cast<T*>(a.out) + at * a.Dv + col, r, a.Dv - col);
+          if (a.out_low) store16<T>(static_cast<T*>(a.out_low) + at * a.Dv + col, d, a.Dv - col);
         }
       }
-      __syncwarp();
+      if (own > 0) {
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&o_free[i]);
+      }
+      __syncwarp();   // the rows' own stores come first
       uint32_t again = __ballot_sync(kFull, ok && real && wild && l != 0.f && !isnan(l));
       while (again) {
         const int r = __ffs(again) - 1;
         again &= again - 1;
         float acc[DP / 32];
-        row_again<T, DP>(a, t, hq, q0 + i * kRows + quarter * 32 + r, __shfl_sync(kFull, m, r), __shfl_sync(kFull, l, r),
-                         acc);
+        row_again<T, DP>(a, t, hq, qi - lane + r, __shfl_sync(kFull, m, r), __shfl_sync(kFull, l, r), acc);
+        const int64_t row_at = __shfl_sync(kFull, at, r) * a.Dv;
 #pragma unroll
         for (int e = 0; e < DP / 32; ++e) {
-          const int d = lane + 32 * e - half * W;
-          T v = from_f32<T>(acc[e]);
-          if (pass) v = from_f32<T>(acc[e] - to_f32<T>(v));
-          if (d >= 0 && d < W)
-            asm volatile("st.shared.b16 [%0], %1;"
-                         :: "r"(stage + (r * SEG + ((d >> 3) ^ (r & (SEG - 1)))) * 16 + (d & 7) * 2),
-                            "h"(*reinterpret_cast<const uint16_t*>(&v)) : "memory");
+          const int d = lane + 32 * e;
+          const T v = from_f32<T>(acc[e]);
+          if (d >= half * W && d < half * W + W && d < a.Dv) {
+            static_cast<T*>(a.out)[row_at + d] = v;
+            if (a.out_low) static_cast<T*>(a.out_low)[row_at + d] = from_f32<T>(acc[e] - to_f32<T>(v));
+          }
         }
         __syncwarp();
       }
-      T* out = static_cast<T*>(pass ? a.out_low : a.out) + half * W;
-      for (int f = lane; f < rows * SEG; f += 32) {
-        const int r = f / SEG, seg = f % SEG;
-        const uint4 v = ld_shared16(stage + (r * SEG + (seg ^ (r & (SEG - 1)))) * 16);
-        if (half * W + seg * 8 < a.Dv) *reinterpret_cast<uint4*>(out + ((row0 + r) * a.Hq + hq) * a.Dv + seg * 8) = v;
-      }
-      __syncwarp();
+      if (a.lse && real && half == 0) a.lse[at] = !ok ? NAN : l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
     }
-    if (a.lse && real && half == 0)
-      a.lse[(row0 + lane) * a.Hq + hq] = !ok ? NAN : l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
   }
   tc::fence_before_sync();
   __syncthreads();
@@ -308,12 +428,13 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
 }
 
 template <typename T, int DP>
-int fwd_t(const FwdTcArgs& a, cudaStream_t s) {
+int fwd_t(FwdTcArgs a, cudaStream_t s) {
   using L = FwdTile<DP>;
-  const int64_t blocks = seq_slots(a.d.cu_q, a.d.B, a.d.T, a.d.sequences, 2 * kRows) * a.d.Hq;
-  if (blocks >= (int64_t(1) << 31)) return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
+  const int64_t items = seq_slots(a.d.cu_q, a.d.B, a.d.T, a.d.sequences, 2 * kRows) * a.d.Hq;
+  if (items >= (int64_t(1) << 30)) return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
+  a.items = int(items);
   if (int rc = allow_smem<dense_fwd_tc_kernel<T, DP>>(L::SMEM, "dense attention smem attribute")) return rc;
-  dense_fwd_tc_kernel<T, DP><<<unsigned(blocks), kThreads, L::SMEM, s>>>(a);
+  dense_fwd_tc_kernel<T, DP><<<unsigned(min64(items, sm_count())), kThreads, L::SMEM, s>>>(a);
   PISA_CHECK_LAUNCH();
   return PISA_OK;
 }
