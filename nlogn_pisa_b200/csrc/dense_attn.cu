@@ -245,7 +245,8 @@ __global__ void __launch_bounds__(kThreads) dense_fwd_kernel(const __grid_consta
 template <typename T>
 __global__ void __launch_bounds__(128) dense_delta_kernel(const T* __restrict__ dout, const T* __restrict__ out,
                                                           const T* __restrict__ low, float* __restrict__ delta,
-                                                          int64_t rows, int Dv) {
+                                                          int64_t rows, int Dv, int* status) {
+  if (blockIdx.x == 0 && threadIdx.x == 0) *status = PISA_OK;
   constexpr int VN = Vec<T>::N;
   const int64_t r = blockIdx.x * int64_t(4) + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
@@ -444,7 +445,7 @@ int bwd_t(const DenseAttnArgs& a, cudaStream_t s) {
   if ((rows + 3) / 4 >= (int64_t(1) << 31)) return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
   dense_delta_kernel<T><<<unsigned((rows + 3) / 4), 128, 0, s>>>(static_cast<const T*>(a.dout),
                                                                  static_cast<const T*>(a.o), static_cast<const T*>(a.o_low),
-                                                                 a.delta, rows, a.Dv);
+                                                                 a.delta, rows, a.Dv, a.status);
   PISA_CHECK_LAUNCH();
   int rc = launch<dense_dq_kernel<T, DP>>(seq_slots(a.cu_q, a.B, a.T, a.sequences, L::BT) * a.Hq,
                   sizeof(float) * L::BT * (4 * L::LD + L::LP), a, s);

@@ -135,15 +135,15 @@ __device__ __forceinline__ SeqTile seq_tile(const DenseAttnArgs& a, int slot, in
   return t;
 }
 
-// Tile of rank `rank` when all sequences' query tiles are ordered by the keys
-// they meet, most first (one warp; at most kRanked packed sequences).  CTAs
-// take ranks in turn: long tiles start early and short ones fill the end.  A
-// lane knows a few sequences; how many tiles cost at least c is a sum of closed
-// forms, and bisection finds the cost of the rank: some 300 instructions, no
-// table and no launch.  t.q_len == 0: past every tile.
+// Tile of rank `rank` when all sequences' query (or key) tiles are ordered by
+// the tiles they meet, most first (one warp; fewer than kRanked packed
+// sequences).  CTAs take ranks in turn: long tiles start early and short ones
+// fill the end.  A lane knows a few sequences; how many tiles cost at least c
+// is a sum of closed forms, and bisection finds the cost of the rank: some 300
+// instructions and no table.  No rows (q_len or k_len 0): past every tile.
 constexpr int kRanked = 128;
 
-__device__ __forceinline__ SeqTile query_tile_ranked(const DenseAttnArgs& a, int rank, int rows) {
+__device__ __forceinline__ SeqTile tile_ranked(const DenseAttnArgs& a, int rank, int rows, bool by_keys) {
   constexpr int PER = kRanked / 32;
   const int lane = threadIdx.x & 31;
   // sequence lane + 32 i: its tiles, the cost of the largest, and x with x - c tiles of cost c or more
@@ -156,11 +156,11 @@ __device__ __forceinline__ SeqTile query_tile_ranked(const DenseAttnArgs& a, int
     if (s > a.sequences) continue;
     const int qb = seq_begin(a, a.cu_q, a.T, s), kb = seq_begin(a, a.cu_k, a.N, s);
     const int ql = seq_end(a, a.cu_q, a.T, s, qb) - qb, kl = seq_end(a, a.cu_k, a.N, s, kb) - kb;
-    tiles[i] = (ql + rows - 1) / rows;
+    tiles[i] = ((by_keys ? kl : ql) + rows - 1) / rows;
     if (s == a.sequences || ql == 0 || kl == 0) continue;      // rows that meet nothing cost nothing
-    const int ahead = max(0, kl - ql) / rows;
-    top[i] = a.causal ? ahead + tiles[i] : (kl + rows - 1) / rows;
-    x[i] = ahead + tiles[i] + 1;
+    const int ahead = max(0, kl - ql) / rows, q_tiles = (ql + rows - 1) / rows;
+    top[i] = by_keys ? q_tiles : a.causal ? ahead + tiles[i] : (kl + rows - 1) / rows;
+    x[i] = ahead + q_tiles + 1;
     most = max(most, top[i]);
   }
   auto at_least = [&](int i, int c) {
@@ -196,7 +196,8 @@ __device__ __forceinline__ SeqTile query_tile_ranked(const DenseAttnArgs& a, int
     if (who) {
       const int src = __ffs(who) - 1;
       seq = src + 32 * i;
-      tile = __shfl_sync(kFull, tiles[i] - at_least(i, lo) + left - (up - n), src);   // larger costs lie at later tiles
+      // larger costs lie at later query tiles, and at earlier key tiles
+      tile = __shfl_sync(kFull, (by_keys ? at_least(i, lo + 1) : tiles[i] - at_least(i, lo)) + left - (up - n), src);
       found = true;
     }
     left -= __shfl_sync(kFull, up, 31);
@@ -205,7 +206,11 @@ __device__ __forceinline__ SeqTile query_tile_ranked(const DenseAttnArgs& a, int
   t.q_begin = seq_begin(a, a.cu_q, a.T, seq);
   t.k_begin = seq_begin(a, a.cu_k, a.N, seq);
   t.q_len = seq_end(a, a.cu_q, a.T, seq, t.q_begin) - t.q_begin;
-  t.k_len = seq >= a.sequences ? 0 : seq_end(a, a.cu_k, a.N, seq, t.k_begin) - t.k_begin;
+  t.k_len = seq_end(a, a.cu_k, a.N, seq, t.k_begin) - t.k_begin;
+  if (seq >= a.sequences) {
+    if (by_keys) t.q_len = 0;
+    else t.k_len = 0;
+  }
   t.tile = tile;
   t.shift = int64_t(t.k_len) - t.q_len;
   return t;
@@ -229,20 +234,30 @@ __device__ __forceinline__ int first_seeing(const DenseAttnArgs& a, const SeqTil
   return int(first < 0 ? 0 : first > t.q_len ? t.q_len : first);
 }
 
+// make_tensor_map from any host thread: the encoding wants a current context,
+// which a thread whose first CUDA call this is (autograd's, a server's) does
+// not have until a runtime call binds the device's.
+inline int thread_tensor_map(CUtensorMap* map, const void* base, int dtype, int64_t B, int64_t T, int64_t H, int64_t D,
+                             int64_t sb, int64_t st, int64_t sh, uint32_t box_h, uint32_t box_t) {
+  if (make_tensor_map(map, base, dtype, B, T, H, D, sb, st, sh, box_h, box_t) == PISA_OK) return PISA_OK;
+  if (cudaFree(nullptr) != cudaSuccess) return fail(PISA_ERR_CUDA, "no CUDA context");
+  return make_tensor_map(map, base, dtype, B, T, H, D, sb, st, sh, box_h, box_t);
+}
+
 // make_tensor_map with a box of `rows` tokens of one head; strides of
 // dimensions of one element, which may hold anything, are replaced.
 inline int dense_tensor_map(CUtensorMap* map, const void* base, int dtype, int64_t B, int64_t T, int64_t H, int64_t D,
                             int64_t sb, int64_t st, int64_t sh, uint32_t rows) {
   if (H == 1) sh = D;
   if (T == 1) st = H * sh;
-  return make_tensor_map(map, base, dtype, B, T, H, D, sb, st, sh, 1, rows);
+  return thread_tensor_map(map, base, dtype, B, T, H, D, sb, st, sh, 1, rows);
 }
 
 // 16-bit tensors of at most 128 dims: tensor-core kernels
 bool dense_attn_tc_eligible(const DenseAttnArgs& a, int dtype);
 int dense_attn_fwd_tc(const DenseAttnArgs& a, int dtype, cudaStream_t stream);
-// a.delta: dense_bwd_stat_floats(...) floats
-int64_t dense_bwd_stat_floats(bool packed, int64_t B, int64_t T, int64_t Hq, int64_t sequences);
+// a.delta: dense_bwd_workspace(...) bytes
+int64_t dense_bwd_workspace(bool packed, int64_t B, int64_t T, int64_t N, int64_t Hq, int64_t sequences);
 int dense_attn_bwd_tc(const DenseAttnArgs& a, int dtype, cudaStream_t stream);
 
 int dense_attn_fwd_simt(const DenseAttnArgs& a, int dtype, cudaStream_t stream);

@@ -5,7 +5,8 @@
 //    out, with the part of out that its rounding dropped: it would add half
 //    again to the rounding errors of dQ and dK), base 2, in tiles of 128 queries of one sequence and head.  Rows past
 //    a sequence's end and rows without keys get lse = +inf, so their weights
-//    are zero below.
+//    are zero below.  The same launch lists the tiles in falling order of their
+//    work for the next two.
 // 2. dK, dV: one CTA per 128 keys of a KV head, over the query tiles that see
 //    them, for each of the G query heads:
 //      MMA  S^T  = K Q^T       (M = 128 keys, N = 128 queries)  -> TMEM
@@ -44,7 +45,8 @@ struct BwdTcArgs {
   CUtensorMap tm_q, tm_k, tm_v, tm_do;   // boxes of 64 dims x 128 rows of one head
   DenseAttnArgs d;
   float* stats;                          // [Hq][q_slots][2][128]
-  int64_t q_slots;
+  SeqTile* order;                        // query tiles, then key tiles, in falling order of their work
+  int64_t q_slots, k_slots;
   int bf16;
 };
 
@@ -69,9 +71,21 @@ __global__ void __launch_bounds__(256) dense_stats_kernel(const __grid_constant_
   constexpr int LANES = DP / 8, PER = 256 / LANES, U = 4;   // rows of the CTA at a time
   const DenseAttnArgs& a = args.d;
   const int slot = blockIdx.x;
+  if (blockIdx.y == kRows / kStatTokens) {
+    // the order of the tiles in the launches that follow: eight ranks per CTA
+    if (slot == 0 && threadIdx.x == 0) *a.status = PISA_OK;
+    const int64_t r = slot * int64_t(8) + threadIdx.x / 32, all = args.q_slots + args.k_slots;
+    if (r >= all) return;
+    const bool by_keys = r >= args.q_slots;
+    const int rank = int(by_keys ? r - args.q_slots : r);
+    const SeqTile t = a.cu_q != nullptr && a.sequences < kRanked ? tile_ranked(a, rank, kRows, by_keys)
+                      : seq_tile(a, by_keys ? rank : int(args.q_slots) - 1 - rank, kRows, by_keys);
+    if (threadIdx.x % 32 == 0) args.order[r] = t;
+    return;
+  }
   const SeqTile t = seq_tile(a, slot, kRows, false);
   const int q0 = t.tile * kRows;
-  if (q0 >= t.q_len) return;
+  if (slot >= args.q_slots || q0 >= t.q_len) return;
   const int lane = threadIdx.x % LANES, d = lane * 8, token0 = blockIdx.y * kStatTokens;
   const T* out = static_cast<const T*>(a.o);
   const T* low = static_cast<const T*>(a.o_low);
@@ -149,8 +163,8 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
   __shared__ uint32_t tmem_slot;
   __shared__ int s_fail;
   const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
-  const int slot = int(blockIdx.x) / a.H, h = int(blockIdx.x) - slot * a.H;   // early keys, seen by most queries, first
-  const SeqTile t = seq_tile(a, slot, kRows, true);
+  const int rank = int(blockIdx.x) / a.H, h = int(blockIdx.x) - rank * a.H;
+  const SeqTile t = args.order[args.q_slots + rank];
   const int j0 = t.tile * kRows;
   if (j0 >= t.k_len) return;
   const int first_tile = first_seeing(a, t, j0) / kRows, end_tile = (t.q_len + kRows - 1) / kRows;
@@ -397,9 +411,8 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
   __shared__ uint32_t tmem_slot;
   __shared__ int s_fail;
   const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
-  const int index = int(gridDim.x) - 1 - int(blockIdx.x);   // late queries, which see the most keys, first
-  const int slot = index / a.Hq, hq = index - slot * a.Hq, h = hq / a.G;
-  const SeqTile t = seq_tile(a, slot, kRows, false);
+  const int rank = int(blockIdx.x) / a.Hq, hq = int(blockIdx.x) - rank * a.Hq, h = hq / a.G;
+  const SeqTile t = args.order[rank];
   const int q0 = t.tile * kRows;
   if (q0 >= t.q_len) return;
   const int valid = min(kRows, t.q_len - q0);
@@ -519,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
     float nlse = -INFINITY, ndel = 0.f;
     int last = -1;
     if (row < valid) {
-      const float* st = stat_tile(args, hq, slot);
+      const float* st = stat_tile(args, hq, query_slot(a, t, t.tile, kRows));
       nlse = st[row];
       ndel = st[kRows + row];
       last = last_visible(a, t, q0 + row);
@@ -593,16 +606,18 @@ int launch(int64_t blocks, int smem, const BwdTcArgs& a, cudaStream_t s) {
 template <typename T, int DP>
 int bwd_t(const BwdTcArgs& a, cudaStream_t s) {
   const DenseAttnArgs& d = a.d;
-  dense_stats_kernel<T, DP><<<dim3(unsigned(a.q_slots), kRows / kStatTokens), 256, 0, s>>>(a);
+  const int64_t wide = a.q_slots > (a.q_slots + a.k_slots + 7) / 8 ? a.q_slots : (a.q_slots + a.k_slots + 7) / 8;
+  dense_stats_kernel<T, DP><<<dim3(unsigned(wide), kRows / kStatTokens + 1), 256, 0, s>>>(a);
   PISA_CHECK_LAUNCH();
-  int rc = launch<dense_dkv_tc_kernel<T, DP>>(seq_slots(d.cu_q, d.B, d.N, d.sequences, kRows) * d.H, BwdTile<DP>::SMEM, a, s);
+  int rc = launch<dense_dkv_tc_kernel<T, DP>>(a.k_slots * d.H, BwdTile<DP>::SMEM, a, s);
   return rc ? rc : launch<dense_dq_tc_kernel<T, DP>>(a.q_slots * d.Hq, BwdTile<DP>::SMEM, a, s);
 }
 
 }  // namespace
 
-int64_t dense_bwd_stat_floats(bool packed, int64_t B, int64_t T, int64_t Hq, int64_t sequences) {
-  return seq_slots(packed, B, T, sequences, kRows) * Hq * 2 * kRows;
+int64_t dense_bwd_workspace(bool packed, int64_t B, int64_t T, int64_t N, int64_t Hq, int64_t sequences) {
+  const int64_t q = seq_slots(packed, B, T, sequences, kRows), k = seq_slots(packed, B, N, sequences, kRows);
+  return q * Hq * 2 * kRows * int64_t(sizeof(float)) + (q + k) * int64_t(sizeof(SeqTile));
 }
 
 int dense_attn_bwd_tc(const DenseAttnArgs& d, int dtype, cudaStream_t stream) {
@@ -611,7 +626,9 @@ int dense_attn_bwd_tc(const DenseAttnArgs& d, int dtype, cudaStream_t stream) {
   a.bf16 = dtype == PISA_BF16;
   a.stats = d.delta;
   a.q_slots = seq_slots(d.cu_q, d.B, d.T, d.sequences, kRows);
-  if (a.q_slots >= (int64_t(1) << 31)) return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
+  a.k_slots = seq_slots(d.cu_q, d.B, d.N, d.sequences, kRows);
+  a.order = reinterpret_cast<SeqTile*>(d.delta + a.q_slots * d.Hq * 2 * kRows);
+  if (a.q_slots + a.k_slots >= (int64_t(1) << 31)) return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
   int rc = dense_tensor_map(&a.tm_q, d.q, dtype, d.B, d.T, d.Hq, d.D, d.q_sb, d.q_st, d.q_sh, kRows);
   if (rc == PISA_OK) rc = dense_tensor_map(&a.tm_k, d.k, dtype, d.B, d.N, d.H, d.D, d.k_sb, d.k_st, d.k_sh, kRows);
   if (rc == PISA_OK) rc = dense_tensor_map(&a.tm_v, d.v, dtype, d.B, d.N, d.H, d.Dv, d.v_sb, d.v_st, d.v_sh, kRows);

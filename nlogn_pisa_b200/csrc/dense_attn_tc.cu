@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
       if (r < args.items) {
         const int slot = r / a.Hq;             // heads of a tile side by side
         w.hq = r - slot * a.Hq;
-        w.t = ranked ? query_tile_ranked(a, slot, 2 * kRows) : seq_tile(a, slots - 1 - slot, 2 * kRows, false);
+        w.t = ranked ? tile_ranked(a, slot, 2 * kRows, false) : seq_tile(a, slots - 1 - slot, 2 * kRows, false);
         const int q0 = w.t.tile * 2 * kRows;
         if (q0 >= w.t.q_len) {
           if (!ranked) continue;               // a slot without rows

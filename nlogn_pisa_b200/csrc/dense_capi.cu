@@ -145,7 +145,7 @@ int64_t pisa_full_attn_bwd_workspace_bytes(int64_t B, int64_t Tq, int64_t Hq, in
       dtype > PISA_F16)
     return -1;
   if (dtype == PISA_F32 || D > 128 || Dv > 128) return 256 + B * Tq * Hq * 4;
-  return 256 + 4 * dense_bwd_stat_floats(sequences > 0, B, Tq, Hq, sequences);
+  return 256 + dense_bwd_workspace(sequences > 0, B, Tq, N, Hq, sequences);
 }
 
 int pisa_full_attn_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb,
@@ -174,9 +174,7 @@ int pisa_full_attn_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, 
   if (!workspace ||
       workspace_bytes < pisa_full_attn_bwd_workspace_bytes(B, Tq, Hq, H, D, Dv, N, cu_seqlens_q ? sequences : 0, dtype))
     return fail(PISA_ERR_INVALID, "workspace too small");
-  cudaError_t e = cudaMemsetAsync(workspace, 0, 256, s);
-  if (e != cudaSuccess) return fail_cuda(e, "status clear");
-  a.status = static_cast<int*>(workspace);
+  a.status = static_cast<int*>(workspace);   // cleared by the first launch, which waits for nothing
   a.delta = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
   return dense_attn_tc_eligible(a, dtype) ? dense_attn_bwd_tc(a, dtype, s) : dense_attn_bwd_simt(a, dtype, s);
 }

@@ -262,7 +262,7 @@ int prefix_attn_tc(const PrefixArgs& p, int dtype, cudaStream_t stream) {
   int64_t st = p.T == 1 ? p.q_sb : p.q_st;
   int64_t sh = p.Hq == 1 ? p.D : p.q_sh;
   if (tokens == 1) st = p.Hq * sh;
-  int rc = make_tensor_map(&a.tm_q, p.q, dtype, 1, tokens, p.Hq, p.D, 0, st, sh, uint32_t(p.G), uint32_t(a.tokens));
+  int rc = thread_tensor_map(&a.tm_q, p.q, dtype, 1, tokens, p.Hq, p.D, 0, st, sh, uint32_t(p.G), uint32_t(a.tokens));
   if (rc == PISA_OK) rc = dense_tensor_map(&a.tm_k, p.pk, dtype, 1, p.P, p.H, p.D, 0, p.pk_st, p.pk_sh, kRows);
   if (rc == PISA_OK) rc = dense_tensor_map(&a.tm_v, p.pv, dtype, 1, p.P, p.H, p.Dv, 0, p.pv_st, p.pv_sh, kRows);
   if (rc) return rc;

@@ -123,11 +123,14 @@ class FullAttentionFunction(torch.autograd.Function):
         ctx.save_for_backward(q, k, v, out, low, lse, cu_q, cu_k)
         ctx.args = (offset, scale, causal)
         ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)   # no zeros for lse
         return out, lse
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, _):
+        if dout is None:
+            return (None,) * 8
         q, k, v, out, low, lse, cu_q, cu_k = ctx.saved_tensors
         dout = flat(dout)
         dq, dk, dv = _backward(q, k, v, out, low, dout, lse, cu_q, cu_k, *ctx.args)

@@ -257,6 +257,32 @@ def test_many_short_sequences(cuda_device):
     compare(q, k, v, normal(gen, 1, total, 2, 64), lengths)
 
 
+def test_first_call_of_a_thread(cuda_device):
+    """A host thread without any CUDA call before: forward, backward and decode."""
+    import threading
+
+    import nlogn_pisa_b200 as P
+
+    gen = torch.Generator(device="cuda").manual_seed(16)
+    q, k, v, dout = normal(gen, 1, 200, 4, 128), *(normal(gen, 1, 200, 2, 128) for _ in range(2)), normal(gen, 1, 200, 4, 128)
+    lengths = torch.tensor([200], dtype=torch.int32, device="cuda")
+    leaves = [x.requires_grad_(True) for x in (q, k, v)]
+    out = P.full_attention(*leaves)
+    want = (out.detach(), P.prefix_attention(q[:, :1], k, v, lengths, prefix_k=k[0], prefix_v=v[0]).clone(),
+            *torch.autograd.grad(out, leaves, dout))
+    torch.cuda.synchronize()
+    calls = [lambda: P.full_attention(q.detach(), k.detach(), v.detach()),
+             lambda: P.prefix_attention(q[:, :1], k, v, lengths, prefix_k=k[0], prefix_v=v[0])]
+    got = []
+    for call in calls:
+        worker = threading.Thread(target=lambda: got.append(call()))
+        worker.start()
+        worker.join()
+    assert len(got) == 2
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_refusals(cuda_device):
     import nlogn_pisa_b200 as P
 
