@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
   __shared__ float2 join_ml[kRows];
   __shared__ uint32_t tmem_slot;
   __shared__ int s_fail;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
   cudaTriggerProgrammaticLaunchCompletion();   // the own caches' kernel may be scheduled
   const int h = blockIdx.x % a.H, split = blockIdx.x / a.H;
   const bool dual = args.tiles == 1;            // one row tile: the halves take every other key tile
@@ -82,8 +82,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  const uint32_t tmem = tmem_slot;
-  const uint32_t tS[2] = {tmem, tmem + 128}, tO[2] = {tmem + 256, tmem + 256 + DP};
+  const uint32_t tmem = __shfl_sync(kFull, tmem_slot, 0);
+  const uint32_t tS = tmem, tO = tmem + 256;
 
   if (warp == kLoadWarp) {
     if (lane == 0) {
@@ -110,59 +110,50 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
-    if (lane == 0) {
-      const uint32_t id_s = tc::idesc_f16(kRows, kRows, args.bf16), id_o = tc::idesc_f16(kRows, DP, args.bf16, 1);
-      bool ok = true;
-      auto wait = [&](uint64_t* bar, int phase) {
-        if (ok && !wait_phase(bar, phase, &s_fail)) ok = false;
-      };
-      // a stage that no later tile takes is not handed back: nothing may arrive after the CTA's end
-      auto hand_back = [&](int pos) {
-        if (pos + L::STAGES < 2 * keys) tc::mma_commit(&kv_empty[pos % L::STAGES]);
-      };
-      for (int s = 0; s <= most && ok; ++s) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (s >= 1 && s <= steps[i]) {        // O += P V of step s - 1
-            const int pos = position(i, s - 1) + 1;
-            wait(&kv_full[pos % L::STAGES], pos / L::STAGES);
-            wait(&p_full[i], s - 1);
-            if (!ok) break;
-            tc::fence_after_sync();
-            const uint32_t v = kv_addr + (pos % L::STAGES) * L::BYTES;
-#pragma unroll
-            for (int x = 0; x < kRows / 16; ++x)
-              tc::mma_f16_ts(tO[i], tS[i] + x * 8, tc::desc_make(v + x * 16 * 128, kRows * 128, 1024, 2), id_o, s > 1 || x > 0);
-            if (s == steps[i]) tc::mma_commit(&o_done[i]);
-            if (dual || i == (steps[1] ? 1 : 0)) hand_back(pos);
-          }
-          if (s < steps[i]) {                   // S = Q K^T of step s
-            const int pos = position(i, s);
-            if (s == 0) wait(&q_full[i], 0);
-            wait(&kv_full[pos % L::STAGES], pos / L::STAGES);
-            if (!ok) break;
-            tc::fence_after_sync();
-            const uint32_t k = kv_addr + (pos % L::STAGES) * L::BYTES, q = q_addr + i * L::BYTES;
-#pragma unroll
-            for (int x = 0; x < DP / 16; ++x) {
-              const uint32_t off = (x >> 2) * kRows * 128 + (x & 3) * 32;
-              tc::mma_f16(tS[i], tc::desc_sw128(q + off), tc::desc_sw128(k + off), id_s, x > 0);
-            }
-            tc::mma_commit(&s_full[i]);
-            if (dual || i == (steps[1] ? 1 : 0)) hand_back(pos);
+    const bool leader = elect_one();
+    const uint32_t id_s = tc::idesc_f16(kRows, kRows, args.bf16), id_o = tc::idesc_f16(kRows, DP, args.bf16, 1);
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, int phase) { ok = wait_phase(bar, phase, &s_fail) && ok; };
+    const int last = steps[1] ? 1 : 0;            // the half that hands a shared stage back
+    for (int s = 0; s <= most && __all_sync(kFull, ok); ++s) {
+#pragma unroll 1
+      for (int i = 0; i < 2; ++i) {
+        const int own = i ? steps[1] : steps[0];
+        // a stage that no later tile takes is not handed back: nothing may arrive after the CTA's end
+        if (s >= 1 && s <= own) {                 // O += P V of step s - 1
+          const int pos = position(i, s - 1) + 1, st = pos % L::STAGES;
+          if (dual || i == 0) wait(&kv_full[st], pos / L::STAGES);
+          wait(&p_full[i], s - 1);
+          tc::fence_after_sync();
+          if (leader && ok) {
+            mma_cols(tO + i * DP, tS + i * 128, 32, kv_addr + st * L::BYTES, id_o, kRows / 16, s > 1);
+            if (s == own) tc::mma_commit(&o_done[i]);
+            if ((dual || i == last) && pos + L::STAGES < 2 * keys) tc::mma_commit(&kv_empty[st]);
           }
         }
+        if (s < own) {                            // S = Q K^T of step s
+          const int pos = position(i, s), st = pos % L::STAGES;
+          if (s == 0) wait(&q_full[i], 0);
+          if (dual || i == 0) wait(&kv_full[st], pos / L::STAGES);
+          tc::fence_after_sync();
+          if (leader && ok) {
+            mma_rows<DP>(tS + i * 128, q_addr + i * L::BYTES, kv_addr + st * L::BYTES, id_s);
+            tc::mma_commit(&s_full[i]);
+            if ((dual || i == last) && pos + L::STAGES < 2 * keys) tc::mma_commit(&kv_empty[st]);
+          }
+        }
+        __syncwarp();
       }
-      if (!ok) {
-        tc::mma_commit(&drained);
-        wait_phase(&drained, 0, &s_fail);
-      }
+    }
+    if (!__all_sync(kFull, ok)) {
+      if (leader) tc::mma_commit(&drained);
+      wait_phase(&drained, 0, &s_fail);
     }
     __syncwarp();
   } else {
     const int i = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lanes = uint32_t(quarter * 32) << 16;
-    const uint32_t ts = tS[i] + lanes, to = tO[i] + lanes;
+    const uint32_t ts = tS + i * 128 + lanes, to = tO + i * DP + lanes;
     const float sl = a.scale * kLog2e;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
