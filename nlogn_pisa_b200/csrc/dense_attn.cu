@@ -18,6 +18,8 @@
 // columns of each output.  Rows outside the sequence are staged as zeros and
 // products with hidden keys are skipped, not multiplied by zero, so
 // infinities and NaN in hidden places reach nothing.
+#include <type_traits>
+
 #include "dense_attn.cuh"
 #include "tc.cuh"
 
@@ -26,6 +28,7 @@ namespace pisa {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr size_t kOnePerSm = 116 * 1024;   // more than half an SM's shared memory
 
 // rows x DP tile of `src` (row stride `stride` elements) into fp32 shared
 // memory, zero past `valid` rows and past D columns
@@ -43,6 +46,44 @@ __device__ __forceinline__ void stage(float* dst, const T* src, int64_t stride, 
       *reinterpret_cast<float4*>(dst + r * LD + c + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
   }
 }
+
+// The same tile by asynchronous copies (fp32); the caller waits for the group.
+template <int DP, int LD>
+__device__ __forceinline__ void stage_async(float* dst, const float* src, int64_t stride, int rows, int valid, int D) {
+  constexpr int SEG = DP / 4;
+  for (int i = threadIdx.x; i < rows * SEG; i += kThreads) {
+    const int r = i / SEG, c = (i - r * SEG) * 4;
+    const bool real = r < valid && c < D;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                 :: "r"(tc::smem_u32(dst + r * LD + c)), "l"(real ? src + r * stride + c : src), "r"(real ? 16 : 0) : "memory");
+  }
+}
+
+// Two tiles that a loop consumes one after the other (keys and values, or
+// queries and dout).  fp32: the next pair is copied while this one is used, in
+// the second of two buffers; one CTA per SM then starts its tiles in falling
+// order of their work.  Otherwise: converted into the one buffer in between.
+template <typename T, int DP, bool FITS = true> struct Pair {
+  static constexpr bool async = std::is_same<T, float>::value, ahead = async && FITS;
+  static constexpr int LD = DP + 4, BUFFERS = ahead ? 2 : 1;
+
+  template <int BT>
+  __device__ __forceinline__ static void fetch(float* buffer, const T* a, int64_t a_st, int da, const T* b, int64_t b_st,
+                                               int db, int valid) {
+    if constexpr (async) {
+      stage_async<DP, LD>(buffer, a, a_st, BT, valid, da);
+      stage_async<DP, LD>(buffer + BT * LD, b, b_st, BT, valid, db);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    } else {
+      stage<T, DP, LD>(buffer, a, a_st, BT, valid, da);
+      stage<T, DP, LD>(buffer + BT * LD, b, b_st, BT, valid, db);
+    }
+  }
+  __device__ __forceinline__ static void arrived() {
+    if constexpr (async) asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+  }
+};
 
 // acc[i][j] += a row (ty*R + i) . b row (tx + 16 j), pairs of dims at a time
 template <int R, int DP, int LD>
@@ -145,10 +186,10 @@ __global__ void __launch_bounds__(kThreads) dense_fwd_kernel(const __grid_consta
   using S = Tile<DP>;
   constexpr int R = S::R, BT = S::BT, LD = S::LD, LP = S::LP;
   extern __shared__ __align__(16) float smem[];
+  using P = Pair<T, DP>;
   float* qs = smem;
-  float* ks = qs + BT * LD;
-  float* vs = ks + BT * LD;
-  float* ps = vs + BT * LD;
+  float* ps = qs + BT * LD;
+  float* ring = ps + BT * LP;
   // later query tiles, which see more keys, first
   const int index = int(gridDim.x) - 1 - int(blockIdx.x);
   const int slot = index / a.Hq, hq = index - slot * a.Hq, h = hq / a.G;
@@ -174,43 +215,62 @@ __global__ void __launch_bounds__(kThreads) dense_fwd_kernel(const __grid_consta
     for (int c = 0; c < DP / 32; ++c) acc[i][c] = make_float2(0.f, 0.f);
   }
   const int end = last_visible(a, t, q0 + valid - 1) + 1, full = last_visible(a, t, q0) + 1;
+  auto fetch = [&](int j0, int buffer) {
+    P::template fetch<BT>(ring + buffer * 2 * BT * LD, kp + int64_t(j0) * a.k_st, a.k_st, a.D, vp + int64_t(j0) * a.v_st,
+                          a.v_st, a.Dv, min(BT, t.k_len - j0));
+  };
+  if (P::ahead && end > 0) fetch(0, 0);
+  int buffer = 0;
   for (int j0 = 0; j0 < end; j0 += BT) {
-    __syncthreads();
     const int nk = min(BT, t.k_len - j0);
-    stage<T, DP, LD>(ks, kp + int64_t(j0) * a.k_st, a.k_st, BT, nk, a.D);
-    stage<T, DP, LD>(vs, vp + int64_t(j0) * a.v_st, a.v_st, BT, nk, a.Dv);
-    __syncthreads();
+    if (!P::ahead) {
+      __syncthreads();
+      fetch(j0, 0);
+    }
+    P::arrived();
+    if (P::ahead && j0 + BT < end) fetch(j0 + BT, buffer ^ 1);
+    const float* ks = ring + buffer * 2 * BT * LD;
+    const float* vs = ks + BT * LD;
+    if (P::ahead) buffer ^= 1;
     float s[R][R] = {};
     rows_dot<R, DP, LD>(qs, ks, ty, tx, s);
-    float corr[R];
     int lo[R], hi[R];
+    bool grown = false;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      float top = m[i];
       lo[i] = 0;
       hi[i] = last[i] - j0;
 #pragma unroll
       for (int j = 0; j < R; ++j) {
         s[i][j] = tx + 16 * j <= hi[i] ? s[i][j] * sl : -INFINITY;
-        top = fmaxf(top, s[i][j]);
+        grown = grown || s[i][j] > m[i];
       }
+    }
+    // the rows' maxima move in few tiles: one vote instead of the shuffles
+    if (__any_sync(kFull, grown)) {
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
-      const float base = top == -INFINITY ? 0.f : top;
-      corr[i] = exp2f(m[i] - base);
-      m[i] = top;
-      float sum = 0.f;
+      for (int i = 0; i < R; ++i) {
+        float top = m[i];
+#pragma unroll
+        for (int j = 0; j < R; ++j) top = fmaxf(top, s[i][j]);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
+        const float corr = top == -INFINITY ? 1.f : exp2f(m[i] - top);
+        m[i] = top;
+        l[i] *= corr;
+#pragma unroll
+        for (int c = 0; c < DP / 32; ++c) acc[i][c] = make_float2(acc[i][c].x * corr, acc[i][c].y * corr);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const float base = m[i] == -INFINITY ? 0.f : m[i];
 #pragma unroll
       for (int j = 0; j < R; ++j) {
         const float p = exp2f(s[i][j] - base);
         ps[(ty * R + i) * LP + tx + 16 * j] = p;
-        sum += p;
+        l[i] += p;                          // this thread's share of the row's sum
       }
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
-      l[i] = l[i] * corr[i] + sum;
-#pragma unroll
-      for (int c = 0; c < DP / 32; ++c) acc[i][c] = make_float2(acc[i][c].x * corr[i], acc[i][c].y * corr[i]);
     }
     __syncwarp();   // the rows of ps that a warp reads are its own
     rows_sum<R, DP, LD, LP>(ps, vs, min(nk, end - j0), ty, tx, j0 + BT > full, lo, hi, acc);
@@ -218,6 +278,8 @@ __global__ void __launch_bounds__(kThreads) dense_fwd_kernel(const __grid_consta
   float inv[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) l[i] += __shfl_xor_sync(kFull, l[i], o);
     inv[i] = l[i] == 0.f ? 0.f : 1.f / l[i];
     const int r = ty * R + i;
     if (a.lse && tx == 0 && r < valid)
@@ -285,10 +347,10 @@ __global__ void __launch_bounds__(kThreads) dense_dq_kernel(const __grid_constan
   constexpr int R = S::R, BT = S::BT, LD = S::LD, LP = S::LP;
   extern __shared__ __align__(16) float smem[];
   float* qs = smem;
+  using P = Pair<T, DP>;
   float* os = qs + BT * LD;
-  float* ks = os + BT * LD;
-  float* vs = ks + BT * LD;
-  float* ds = vs + BT * LD;
+  float* ds = os + BT * LD;
+  float* ring = ds + BT * LP;
   const int index = int(gridDim.x) - 1 - int(blockIdx.x);
   const int slot = index / a.Hq, hq = index - slot * a.Hq, h = hq / a.G;
   const SeqTile t = seq_tile(a, slot, BT, false);
@@ -316,12 +378,23 @@ __global__ void __launch_bounds__(kThreads) dense_dq_kernel(const __grid_constan
     for (int c = 0; c < DP / 32; ++c) acc[i][c] = make_float2(0.f, 0.f);
   }
   const int end = last_visible(a, t, q0 + valid - 1) + 1, full = last_visible(a, t, q0) + 1;
+  auto fetch = [&](int j0, int buffer) {
+    P::template fetch<BT>(ring + buffer * 2 * BT * LD, kp + int64_t(j0) * a.k_st, a.k_st, a.D, vp + int64_t(j0) * a.v_st,
+                          a.v_st, a.Dv, min(BT, t.k_len - j0));
+  };
+  if (P::ahead && end > 0) fetch(0, 0);
+  int buffer = 0;
   for (int j0 = 0; j0 < end; j0 += BT) {
-    __syncthreads();
     const int nk = min(BT, t.k_len - j0);
-    stage<T, DP, LD>(ks, kp + int64_t(j0) * a.k_st, a.k_st, BT, nk, a.D);
-    stage<T, DP, LD>(vs, vp + int64_t(j0) * a.v_st, a.v_st, BT, nk, a.Dv);
-    __syncthreads();
+    if (!P::ahead) {
+      __syncthreads();
+      fetch(j0, 0);
+    }
+    P::arrived();
+    if (P::ahead && j0 + BT < end) fetch(j0 + BT, buffer ^ 1);
+    const float* ks = ring + buffer * 2 * BT * LD;
+    const float* vs = ks + BT * LD;
+    if (P::ahead) buffer ^= 1;
     float s[R][R] = {}, dp[R][R] = {};
     rows_dot<R, DP, LD>(qs, ks, ty, tx, s);
     rows_dot<R, DP, LD>(os, vs, ty, tx, dp);
@@ -344,6 +417,9 @@ __global__ void __launch_bounds__(kThreads) dense_dq_kernel(const __grid_constan
   store_rows<T, R, DP>(static_cast<T*>(a.dq) + row0 * a.D, int64_t(a.Hq) * a.D, valid, a.D, ty, tx, acc, one);
 }
 
+// 128 dims: six operand tiles and the two of weights pass the shared memory
+template <typename T, int DP> using KvPair = Pair<T, DP, DP != 128>;
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads) dense_dkv_kernel(const __grid_constant__ DenseAttnArgs a) {
   using S = Tile<DP>;
@@ -351,11 +427,11 @@ __global__ void __launch_bounds__(kThreads) dense_dkv_kernel(const __grid_consta
   extern __shared__ __align__(16) float smem[];
   float* ks = smem;
   float* vs = ks + BT * LD;
-  float* qs = vs + BT * LD;
-  float* os = qs + BT * LD;
-  float* ps = os + BT * LD;      // P^T: key rows, query columns
+  using P = KvPair<T, DP>;
+  float* ps = vs + BT * LD;      // P^T: key rows, query columns
   float* ds = ps + BT * LP;      // dS^T
-  __shared__ float lse_s[64], delta_s[64];
+  float* ring = ds + BT * LP;
+  __shared__ float lse_s[2][64], delta_s[2][64];
   const int slot = int(blockIdx.x) / a.H, h = int(blockIdx.x) - slot * a.H;   // early keys, seen by most queries, first
   const SeqTile t = seq_tile(a, slot, BT, true);
   const int j0 = t.tile * BT;
@@ -377,21 +453,35 @@ __global__ void __launch_bounds__(kThreads) dense_dkv_kernel(const __grid_consta
     for (int c = 0; c < DP / 32; ++c) dk[i][c] = dv[i][c] = make_float2(0.f, 0.f);
   }
   const int begin = first_seeing(a, t, j0) / BT * BT, full = first_seeing(a, t, j0 + valid - 1);
+  auto fetch = [&](int g, int q0, int buffer) {
+    const int hq = h * a.G + g, nq = min(BT, t.q_len - q0);
+    const int64_t row0 = (int64_t(t.b) * a.T + t.q_begin + q0) * a.Hq + hq;
+    P::template fetch<BT>(ring + buffer * 2 * BT * LD,
+                          static_cast<const T*>(a.q) + t.b * a.q_sb + int64_t(t.q_begin + q0) * a.q_st + hq * a.q_sh, a.q_st,
+                          a.D, static_cast<const T*>(a.dout) + row0 * a.Dv, int64_t(a.Hq) * a.Dv, a.Dv, nq);
+    if (threadIdx.x < BT) {
+      const bool real = int(threadIdx.x) < nq;
+      lse_s[buffer][threadIdx.x] = real ? lse_base2(a.lse_in[row0 + int64_t(threadIdx.x) * a.Hq]) : 0.f;
+      delta_s[buffer][threadIdx.x] = real ? a.delta[row0 + int64_t(threadIdx.x) * a.Hq] : 0.f;
+    }
+  };
+  int buffer = 0;
+  if (P::ahead && begin < t.q_len) fetch(0, begin, 0);
   for (int g = 0; g < a.G; ++g) {
-    const int hq = h * a.G + g;
     for (int q0 = begin; q0 < t.q_len; q0 += BT) {
-      const int nq = min(BT, t.q_len - q0);
-      const int64_t row0 = (int64_t(t.b) * a.T + t.q_begin + q0) * a.Hq + hq;
-      __syncthreads();
-      stage<T, DP, LD>(qs, static_cast<const T*>(a.q) + t.b * a.q_sb + int64_t(t.q_begin + q0) * a.q_st + hq * a.q_sh,
-                       a.q_st, BT, nq, a.D);
-      stage<T, DP, LD>(os, static_cast<const T*>(a.dout) + row0 * a.Dv, int64_t(a.Hq) * a.Dv, BT, nq, a.Dv);
-      if (threadIdx.x < BT) {
-        const bool real = int(threadIdx.x) < nq;
-        lse_s[threadIdx.x] = real ? lse_base2(a.lse_in[row0 + int64_t(threadIdx.x) * a.Hq]) : 0.f;
-        delta_s[threadIdx.x] = real ? a.delta[row0 + int64_t(threadIdx.x) * a.Hq] : 0.f;
+      const int nq = min(BT, t.q_len - q0), now = buffer;
+      if (!P::ahead) {
+        __syncthreads();
+        fetch(g, q0, 0);
       }
-      __syncthreads();
+      P::arrived();
+      if (P::ahead) {
+        buffer ^= 1;
+        if (q0 + BT < t.q_len) fetch(g, q0 + BT, buffer);
+        else if (g + 1 < a.G) fetch(g + 1, begin, buffer);
+      }
+      const float* qs = ring + now * 2 * BT * LD;
+      const float* os = qs + BT * LD;
       float s[R][R] = {}, dp[R][R] = {};
       rows_dot<R, DP, LD>(ks, qs, ty, tx, s);
       rows_dot<R, DP, LD>(vs, os, ty, tx, dp);
@@ -403,7 +493,7 @@ __global__ void __launch_bounds__(kThreads) dense_dkv_kernel(const __grid_consta
 #pragma unroll
         for (int j = 0; j < R; ++j) {
           const int c = tx + 16 * j;
-          const float2 pg = prob_grad(s[i][j], dp[i][j], sl, lse_s[c], delta_s[c], a.scale, c >= lo[i] && c <= hi[i]);
+          const float2 pg = prob_grad(s[i][j], dp[i][j], sl, lse_s[now][c], delta_s[now][c], a.scale, c >= lo[i] && c <= hi[i]);
           ps[(ty * R + i) * LP + c] = pg.x;
           ds[(ty * R + i) * LP + c] = pg.y;
         }
@@ -435,7 +525,9 @@ template <typename T, int DP>
 int fwd_t(const DenseAttnArgs& a, cudaStream_t s) {
   using L = Tile<DP>;
   const int64_t slots = seq_slots(a.cu_q, a.B, a.T, a.sequences, L::BT);
-  return launch<dense_fwd_kernel<T, DP>>(slots * a.Hq, sizeof(float) * L::BT * (3 * L::LD + L::LP), a, s);
+  size_t smem = sizeof(float) * L::BT * ((1 + 2 * Pair<T, DP>::BUFFERS) * L::LD + L::LP);
+  if (Pair<T, DP>::ahead && smem < kOnePerSm) smem = kOnePerSm;
+  return launch<dense_fwd_kernel<T, DP>>(slots * a.Hq, smem, a, s);
 }
 
 template <typename T, int DP>
@@ -448,10 +540,10 @@ int bwd_t(const DenseAttnArgs& a, cudaStream_t s) {
                                                                  a.delta, rows, a.Dv, a.status);
   PISA_CHECK_LAUNCH();
   int rc = launch<dense_dq_kernel<T, DP>>(seq_slots(a.cu_q, a.B, a.T, a.sequences, L::BT) * a.Hq,
-                  sizeof(float) * L::BT * (4 * L::LD + L::LP), a, s);
+                  sizeof(float) * L::BT * ((2 + 2 * Pair<T, DP>::BUFFERS) * L::LD + L::LP), a, s);
   if (rc) return rc;
   return launch<dense_dkv_kernel<T, DP>>(seq_slots(a.cu_q, a.B, a.N, a.sequences, L::BT) * a.H,
-                sizeof(float) * L::BT * (4 * L::LD + 2 * L::LP), a, s);
+                sizeof(float) * L::BT * ((2 + 2 * KvPair<T, DP>::BUFFERS) * L::LD + 2 * L::LP), a, s);
 }
 
 template <typename T>

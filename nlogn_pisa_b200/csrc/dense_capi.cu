@@ -75,6 +75,7 @@ PrefixPlan plan_prefix(int64_t B, int64_t T, int64_t Hq, int64_t H, int64_t D, i
       return ranges(keys, std::max((sms + items - 1) / items, most), 64, chunk);
     };
     p.own_splits = stream(cap, B * H * ((T * G + 15) / 16), &p.own_chunk);
+    if (P == 0 && cap <= 512) p.own_splits = ranges(cap, 1, 64, &p.own_chunk);   // short caches: nothing to join
     // more than 16 query rows per KV head: tiles of 128 rows, else the stream
     p.tiles = P > 0 && B * T * G > 16 && G <= 128;
     const int64_t tokens = p.tiles ? 128 / G : 1, tiles = (B * T + tokens - 1) / tokens;
