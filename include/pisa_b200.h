@@ -439,7 +439,8 @@ PISA_API int64_t pisa_full_attn_bwd_workspace_bytes(int64_t B, int64_t Tq, int64
  * sees the whole prefix and own keys 0 .. lengths[b] - Tq + t.
  * out: [B,Tq,Hq,Dv] contiguous; lse: [B,Tq,Hq] fp32 or NULL; without a
  * visible key 0 / -inf.  scale > 0; D, Dv multiples of 8, at most 256.
- * workspace: pisa_prefix_attn_workspace_bytes(...) bytes.
+ * workspace: pisa_prefix_attn_workspace_bytes(...) bytes, 32-byte aligned,
+ * status word first; rows of an expired wait are NaN.
  */
 PISA_API int pisa_prefix_attn(const void *q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void *k, int64_t k_sb,
                               int64_t k_st, int64_t k_sh, const void *v, int64_t v_sb, int64_t v_st, int64_t v_sh,
@@ -456,8 +457,9 @@ PISA_API int64_t pisa_prefix_attn_workspace_bytes(int64_t B, int64_t Tq, int64_t
  * Every kernel that waits on another part of the GPU waits a bounded number
  * of tries.  A wait that expires records PISA_ERR_TIMEOUT in the 4-byte
  * status word at byte offset 0 of the call's workspace (pisa_select_blocks,
- * pisa_leaf_scores, and pisa_sparse_attn_fwd when it takes the tensor-core
- * path); the entry point clears that word on `stream` before its kernels run.
+ * pisa_leaf_scores, pisa_full_attn_fwd and _bwd, pisa_prefix_attn, and
+ * pisa_sparse_attn_fwd when it takes the tensor-core path); the call clears that
+ * word on `stream` before any of its waits can expire.
  *
  * pisa_workspace_status copies the word back and synchronises `stream`:
  * PISA_OK, or PISA_ERR_TIMEOUT (the call's outputs are not valid). */

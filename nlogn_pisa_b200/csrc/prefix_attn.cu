@@ -38,6 +38,7 @@ template <typename T, int DP, int R>
 __global__ void __launch_bounds__(kThreads) prefix_simt_kernel(const __grid_constant__ PrefixArgs a, bool prefix) {
   constexpr int BR = 16 * R, LD = DP + 4, LP = kKeys + 1, VN = Vec<T>::N, SEG = DP / VN;
   extern __shared__ __align__(16) float smem[];
+  if (blockIdx.x + blockIdx.y + blockIdx.z + threadIdx.x == 0) *a.status = PISA_OK;
   float* qs = smem;
   float* ks = qs + BR * LD;   // keys, then the values of the same tile
   float* ps = ks + kKeys * LD;

@@ -28,7 +28,7 @@ struct PrefixArgs {
   int prefix_splits, own_splits, prefix_chunk, own_chunk;
   float* part_o;                 // [rows][slots][Dv], sum_j 2^(s_j - m) v_j
   float2* part_ml;               // [rows][slots], (m, l) with base-2 logits
-  int* status;
+  int* status;                   // device status word, cleared by block 0 of the first launch
 };
 
 __device__ __forceinline__ int own_length(const PrefixArgs& a, int b) {

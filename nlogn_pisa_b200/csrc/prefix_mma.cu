@@ -149,6 +149,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_stream_kernel(const __grid
   __shared__ int s_fail;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   cudaTriggerProgrammaticLaunchCompletion();   // the joining launch may be scheduled
+  // half a second before any wait can expire
+  if (!args.after_tiles && blockIdx.x + tid == 0) *a.status = PISA_OK;
 
   // own ranges before each table entry (an exclusive scan by one warp)
   const int entries = (a.B + args.per_entry - 1) / args.per_entry;
@@ -403,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_stream_kernel(const __grid
     }
   }
   __syncthreads();
-  if (tid == 0 && s_fail && a.status) atomicExch(a.status, PISA_ERR_TIMEOUT);
+  if (tid == 0 && s_fail) atomicExch(a.status, PISA_ERR_TIMEOUT);
   // scheduled while the prefix's tiles drain, whose partials the joining launch
   // reads too: this kernel ends after that one
   cudaGridDependencySynchronize();

@@ -53,6 +53,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
   __shared__ int s_fail;
   const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
   cudaTriggerProgrammaticLaunchCompletion();   // the own caches' kernel may be scheduled
+  // half a second before any wait can expire
+  if (blockIdx.x + blockIdx.y + tid == 0) *a.status = PISA_OK;
   const int h = blockIdx.x % a.H, split = blockIdx.x / a.H;
   const bool dual = args.tiles == 1;            // one row tile: the halves take every other key tile
   int begin, end;
@@ -228,7 +230,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  if (tid == 0 && s_fail && a.status) atomicExch(a.status, PISA_ERR_TIMEOUT);
+  if (tid == 0 && s_fail) atomicExch(a.status, PISA_ERR_TIMEOUT);
   if (warp == kMmaWarp) tc::tmem_free(tmem, 512);
 }
 

@@ -177,6 +177,21 @@ class FullAttention(nn.Module):
         self.register_buffer("theta", rotary_frequencies(config.head_dim, config.rope_theta, config.rope_fraction),
                              persistent=False)
 
+    def _apply(self, fn, recurse=True):
+        """Frequencies stay fp32 when the layer is cast to another type."""
+        super()._apply(fn, recurse)
+        cfg = self.config
+        self.theta = rotary_frequencies(cfg.head_dim, cfg.rope_theta, cfg.rope_fraction).to(self.theta.device)
+        return self
+
+    @staticmethod
+    def _document_positions(length, cu_seqlens, device):
+        """token_positions of packed documents, without reading their lengths on the host."""
+        at = torch.arange(length, device=device)
+        cu = cu_seqlens.to(device=device, dtype=torch.int64)
+        document = torch.searchsorted(cu[1:], at, right=True).clamp_(max=cu.shape[0] - 1)
+        return (at - cu[document])[None]
+
     @staticmethod
     def share_prefix(cache):
         """A cache whose prompt (batch 1) is shared by the sequences that follow."""
@@ -204,7 +219,7 @@ class FullAttention(nn.Module):
             past = 0 if cache["key_storage"] is None else cache["key_storage"].length
         positions = None
         if cu_seqlens is not None and cfg.rope_position_mode == "document":
-            positions = token_positions(length, x.device, cu_seqlens)
+            positions = self._document_positions(length, cu_seqlens, x.device)
         q, k = qk_norm_rotary(q, k, self.q_norm.to(q.dtype), self.k_norm.to(q.dtype), self.theta, positions=positions,
                               position_offset=shared + past, eps=self.eps)
         keys, values = k, v

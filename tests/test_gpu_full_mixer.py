@@ -162,3 +162,30 @@ def test_refusals(cuda_device):
         mixer(x, attention_mask=torch.tensor([[True, False]]))
     with pytest.raises(ValueError, match="full attention"):
         make(torch.bfloat16, attention_method="pisa")
+
+
+def test_status_checks_pass_on_the_dense_operators(cuda_device):
+    """With checks on, every call reads its status word back: set, and clean."""
+    import nlogn_pisa_b200 as P
+
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    junk = torch.full((1 << 24,), 255, dtype=torch.uint8, device="cuda")   # what the workspaces' memory held before
+    del junk
+    P.set_status_checks(True)
+    try:
+        for dtype, dim in ((torch.bfloat16, 128), (torch.float32, 64), (torch.float16, 64), (torch.bfloat16, 256)):
+            q, k, v = (torch.randn(2, 300, h, dim, generator=gen, device="cuda").to(dtype).requires_grad_(True) for h in (4, 2, 2))
+            P.full_attention(q, k, v).sum().backward()
+            n = torch.tensor([300, 7], device="cuda")
+            for rows, prefix in ((1, None), (3, None), (1, k[0]), (40, k[0])):
+                P.prefix_attention(q[:, :rows], k, v, n, prefix_k=prefix, prefix_v=prefix)
+    finally:
+        P.set_status_checks(False)
+
+
+def test_frequencies_stay_fp32(cuda_device):
+    from nlogn_pisa_b200.mixer import rotary_frequencies
+
+    mixer = make(torch.bfloat16)
+    assert mixer.theta.dtype == torch.float32
+    assert torch.equal(mixer.theta.cpu(), rotary_frequencies(64, 10000.0, 0.5))
