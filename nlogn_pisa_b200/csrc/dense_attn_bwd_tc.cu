@@ -56,6 +56,7 @@ template <int DP> struct BwdTile {
   // for three pairs, which also keeps a second CTA off the SM's TMEM
   static constexpr int RING = DP == 128 ? 4 : 6;
   static constexpr int SMEM = (2 + RING) * BYTES + RING / 2 * 1024 + 1024;
+  static constexpr int DQ_SMEM = (3 + RING) * BYTES + 1024;   // with the output's staging
 };
 
 __device__ __forceinline__ float* stat_tile(const BwdTcArgs& a, int hq, int64_t slot) {
@@ -399,38 +400,64 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
   if (warp == kMmaWarp) tc::tmem_free(tmem, 512);
 }
 
-// Launch 3.
+// Launch 3: a persistent CTA per SM.  Items (query tile, head) are taken in
+// falling order of their work, every other round backwards; the next item's
+// loads and first scores overlap the output of the one before.  All phases and
+// ring positions run on across items.
+struct DqItem {
+  SeqTile t;
+  int hq, valid, total, tail;   // hq < 0: no item; real rows; key tiles, and the real rows of the last
+};
+
+__device__ __forceinline__ DqItem dq_item(const BwdTcArgs& args, int& round) {
+  const DenseAttnArgs& a = args.d;
+  const int64_t items = args.q_slots * a.Hq;
+  const int g = int(gridDim.x), c = int(blockIdx.x);
+  DqItem w;
+  w.hq = -1;
+  for (;; ++round) {
+    const int64_t at = int64_t(round) * g + (round & 1 ? g - 1 - c : c);
+    if (at >= items) return w;
+    const int slot = int(at / a.Hq);
+    w.t = args.order[slot];
+    w.valid = min(kRows, w.t.q_len - w.t.tile * kRows);
+    if (w.valid <= 0) continue;   // a slot without rows
+    w.hq = int(at - int64_t(slot) * a.Hq);
+    const int keys = last_visible(a, w.t, w.t.tile * kRows + w.valid - 1) + 1;
+    w.total = (keys + kRows - 1) / kRows;
+    w.tail = min(kRows, w.t.k_len - (w.total - 1) * kRows);
+    ++round;
+    return w;
+  }
+}
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_constant__ BwdTcArgs args) {
   using L = BwdTile<DP>;
   const DenseAttnArgs& a = args.d;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t base = (tc::smem_u32(smem_raw) + 1023) & ~1023u;
-  const uint32_t q_addr = base, o_addr = base + L::BYTES, ring = base + 2 * L::BYTES;
-  __shared__ uint64_t q_full, full[L::RING], raw, empty[L::RING], s_full[2], dp_full, dp_free, ds_full, done;
+  const uint32_t q_addr = base, o_addr = base + L::BYTES, out_addr = base + 2 * L::BYTES, ring = base + 3 * L::BYTES;
+  __shared__ uint64_t q_full, q_empty, full[L::RING], raw[L::RING], empty[L::RING];
+  __shared__ uint64_t s_full[2], dp_full, dp_free, ds_full, done, drained;
   __shared__ uint32_t tmem_slot;
   __shared__ int s_fail;
   const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
-  const int rank = int(blockIdx.x) / a.Hq, hq = int(blockIdx.x) - rank * a.Hq, h = hq / a.G;
-  const SeqTile t = args.order[rank];
-  const int q0 = t.tile * kRows;
-  if (q0 >= t.q_len) return;
-  const int valid = min(kRows, t.q_len - q0);
-  const int keys = last_visible(a, t, q0 + valid - 1) + 1, total = (keys + kRows - 1) / kRows;
-  const int tail = min(kRows, t.k_len - (total - 1) * kRows);   // real rows of the last key tile
   if (tid == 0) {
     tc::mbar_init(&q_full, 1);
+    tc::mbar_init(&q_empty, 1);
     for (int i = 0; i < L::RING; ++i) {
       tc::mbar_init(&full[i], 1);
+      tc::mbar_init(&raw[i], 1);
       tc::mbar_init(&empty[i], 1);
     }
-    tc::mbar_init(&raw, 1);
     tc::mbar_init(&s_full[0], 1);
     tc::mbar_init(&s_full[1], 1);
     tc::mbar_init(&dp_full, 1);
     tc::mbar_init(&dp_free, 8);
     tc::mbar_init(&ds_full, 8);
     tc::mbar_init(&done, 1);
+    tc::mbar_init(&drained, 1);
     s_fail = 0;
     tc::fence_barrier_init();
   }
@@ -441,151 +468,189 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
   const uint32_t tmem = __shfl_sync(kFull, tmem_slot, 0);
   const uint32_t tS = tmem, tP = tmem + 256, tQ = tmem + 384;   // two S, whose dS overwrites it; dP; dQ
   Wait wait{&s_fail};
+  int round = 0;
 
   if (warp == kLoadWarp) {
-    if (lane == 0 && total > 0) {
-      tc::mbar_arrive_expect_tx(&q_full, 2 * L::BYTES);
-      load_tile<DP>(q_addr, &args.tm_q, hq, t.q_begin + q0, t.b, &q_full);
-      load_tile<DP>(o_addr, &args.tm_do, hq, t.q_begin + q0, t.b, &q_full);
-      int issued = 0;
-      for (int pos = 0; pos < 2 * total; ++pos) {   // K0 V0 K1 V1 ...
-        const int st = pos % L::RING;
-        if (!wait(&empty[st], (pos / L::RING) + 1)) break;
-        // keys of a ragged last tile pass through the trimming warp
-        uint64_t* bar = pos == 2 * total - 2 && tail < kRows ? &raw : &full[st];
-        tc::mbar_arrive_expect_tx(bar, L::BYTES);
-        load_tile<DP>(ring + st * L::BYTES, pos & 1 ? &args.tm_v : &args.tm_k, h, t.k_begin + (pos >> 1) * kRows, t.b, bar);
-        issued = pos + 1;
+    if (lane == 0) {
+      int pos = 0, used = 0;                    // ring position; items with keys so far
+      while (wait.ok) {
+        const DqItem w = dq_item(args, round);
+        if (w.hq < 0) break;
+        if (w.total <= 0) continue;
+        const int h = w.hq / a.G;
+        if (!wait(&q_empty, used + 1)) break;
+        tc::mbar_arrive_expect_tx(&q_full, 2 * L::BYTES);
+        load_tile<DP>(q_addr, &args.tm_q, w.hq, w.t.q_begin + w.t.tile * kRows, w.t.b, &q_full);
+        load_tile<DP>(o_addr, &args.tm_do, w.hq, w.t.q_begin + w.t.tile * kRows, w.t.b, &q_full);
+        ++used;
+        for (int x = 0; x < 2 * w.total; ++x, ++pos) {   // K0 V0 K1 V1 ...
+          const int st = pos % L::RING;
+          if (!wait(&empty[st], (pos / L::RING) + 1)) break;
+          // keys of a ragged last tile pass through the trimming warp
+          uint64_t* bar = x == 2 * w.total - 2 && w.tail < kRows ? &raw[st] : &full[st];
+          tc::mbar_arrive_expect_tx(bar, L::BYTES);
+          load_tile<DP>(ring + st * L::BYTES, x & 1 ? &args.tm_v : &args.tm_k, h, w.t.k_begin + (x >> 1) * kRows, w.t.b, bar);
+        }
       }
-      if (!wait.ok)   // the copies in flight land before the CTA ends
-        for (int pos = max(0, issued - L::RING); pos < issued; ++pos)
-          wait_phase(&full[pos % L::RING], pos / L::RING, &s_fail);
+      if (!wait.ok) {   // the copies in flight land before the CTA ends
+        if (used) wait_phase(&q_full, used - 1, &s_fail);
+        for (int x = max(0, pos - L::RING); x < pos; ++x) wait_phase(&full[x % L::RING], x / L::RING, &s_fail);
+      }
     }
     __syncwarp();
   } else if (warp == kTrimWarp) {
-    if (total > 0 && tail < kRows) {
-      const int st = (2 * total - 2) % L::RING;
-      wait.warp(&raw, 0);
-      zero_rows<DP>(ring + st * L::BYTES, tail, (tail + 15) & ~15, lane);
+    int pos = 0;
+    uint32_t uses = 0;                          // parity of the ragged tiles that each ring slot has held
+    for (;;) {
+      const DqItem w = dq_item(args, round);
+      if (w.hq < 0 || !__all_sync(kFull, wait.ok)) break;
+      if (w.total <= 0) continue;
+      pos += 2 * w.total;
+      if (w.tail >= kRows) continue;
+      const int st = (pos - 2) % L::RING;
+      wait.warp(&raw[st], uses >> st);
+      uses ^= 1u << st;
+      zero_rows<DP>(ring + st * L::BYTES, w.tail, (w.tail + 15) & ~15, lane);
       tc::fence_async_smem();
       __syncwarp();
       if (lane == 0 && wait.ok) tc::mbar_arrive(&full[st]);
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
-    if (total > 0) {
-      const bool leader = elect_one();
-      const uint32_t id_s = tc::idesc_f16(kRows, kRows, args.bf16), id_o = tc::idesc_f16(kRows, DP, args.bf16, 1);
-      wait.warp(&q_full, 0);
-      int st = 0;                               // slot of K(n); V(n) is in the next one
-      uint32_t phase = 0;
-      wait.warp(&full[0], 0);
-      tc::fence_after_sync();
-      if (leader) {
-        mma_rows<DP>(tS, q_addr, ring, id_s);
-        tc::mma_commit(&s_full[0]);
+    const bool leader = elect_one();
+    const uint32_t id_s = tc::idesc_f16(kRows, kRows, args.bf16), id_o = tc::idesc_f16(kRows, DP, args.bf16, 1);
+    int st = 0, tile = 0, used = 0;             // slot of a tile's K (its V is in the next one); tiles and items so far
+    uint32_t phase = 0;
+    DqItem w = dq_item(args, round);
+    while (w.hq >= 0 && __all_sync(kFull, wait.ok)) {
+      const int total = w.total, steps = (w.tail + 15) / 16;
+      if (total > 0) {
+        wait.warp(&q_full, used);
+        wait.warp(&full[st], int(phase));
+        tc::fence_after_sync();
+        if (leader) {                           // the buffers' last readers: products and warps waited for before
+          mma_rows<DP>(tS + (tile & 1) * 128, q_addr, ring + st * L::BYTES, id_s);
+          tc::mma_commit(&s_full[tile & 1]);
+        }
+        wait.warp(&full[st + 1], int(phase));
+        tc::fence_after_sync();
+        if (leader) {
+          mma_rows<DP>(tP, o_addr, ring + (st + 1) * L::BYTES, id_s);
+          tc::mma_commit(&dp_full);
+          tc::mma_commit(&empty[st + 1]);
+          if (total == 1) tc::mma_commit(&q_empty);
+        }
+        ++used;
       }
-      wait.warp(&full[1], 0);
-      tc::fence_after_sync();
-      // a slot that no later tile takes is not handed back: nothing may arrive after the CTA's end
-      if (leader) {
-        mma_rows<DP>(tP, o_addr, ring + L::BYTES, id_s);
-        tc::mma_commit(&dp_full);
-        if (1 + L::RING < 2 * total) tc::mma_commit(&empty[1]);
-      }
-      for (int n = 0; n < total && __all_sync(kFull, wait.ok); ++n) {
+      w = dq_item(args, round);
+      for (int n = 0; n < total && __all_sync(kFull, wait.ok); ++n, ++tile) {
         const int next = st + 2 == L::RING ? 0 : st + 2;
         const uint32_t next_phase = next ? phase : phase ^ 1;
         if (n + 1 < total) {
           wait.warp(&full[next], int(next_phase));
           tc::fence_after_sync();
-          if (leader) {                         // its buffer held dS(n - 1), whose product was issued before
-            mma_rows<DP>(tS + ((n + 1) & 1) * 128, q_addr, ring + next * L::BYTES, id_s);
-            tc::mma_commit(&s_full[(n + 1) & 1]);
+          if (leader) {                         // its buffer held dS of the tile before, whose product was issued
+            mma_rows<DP>(tS + ((tile + 1) & 1) * 128, q_addr, ring + next * L::BYTES, id_s);
+            tc::mma_commit(&s_full[(tile + 1) & 1]);
           }
-          wait.warp(&dp_free, n);               // dP(n) is in registers
+          wait.warp(&dp_free, tile);            // dP is in registers
           wait.warp(&full[next + 1], int(next_phase));
           tc::fence_after_sync();
           if (leader) {
             mma_rows<DP>(tP, o_addr, ring + (next + 1) * L::BYTES, id_s);
             tc::mma_commit(&dp_full);
-            if (2 * n + 3 + L::RING < 2 * total) tc::mma_commit(&empty[next + 1]);
+            tc::mma_commit(&empty[next + 1]);
+            if (n + 2 == total) tc::mma_commit(&q_empty);
           }
         }
-        wait.warp(&ds_full, n);
+        wait.warp(&ds_full, tile);              // and the dQ of the item before has been read
         tc::fence_after_sync();
         if (leader) {
-          mma_cols(tQ, tS + (n & 1) * 128, 64, ring + st * L::BYTES, id_o, n + 1 == total ? (tail + 15) / 16 : kRows / 16, n > 0);
-          if (2 * n + L::RING < 2 * total) tc::mma_commit(&empty[st]);
+          mma_cols(tQ, tS + (tile & 1) * 128, 64, ring + st * L::BYTES, id_o, n + 1 == total ? steps : kRows / 16, n > 0);
+          tc::mma_commit(&empty[st]);
+          if (n + 1 == total) tc::mma_commit(&done);
         }
         st = next;
         phase = next_phase;
       }
-      if (leader) tc::mma_commit(&done);
-      if (!__all_sync(kFull, wait.ok)) wait_phase(&done, 0, &s_fail);
     }
+    if (leader) tc::mma_commit(&drained);
+    wait_phase(&drained, 0, &s_fail);
     __syncwarp();
   } else {
     const int side = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;   // query row, keys 64*side ..
     const uint32_t lanes = uint32_t(quarter * 32) << 16;
     const float2 sl2 = make_float2(a.scale * kLog2e, a.scale * kLog2e), sc2 = make_float2(a.scale, a.scale);
+    int tile = 0, used = 0;
     float nlse = -INFINITY, ndel = 0.f;
-    int last = -1;
-    if (row < valid) {
-      const float* st = stat_tile(args, hq, query_slot(a, t, t.tile, kRows));
-      nlse = st[row];
-      ndel = st[kRows + row];
-      last = last_visible(a, t, q0 + row);
-    }
-    const float2 nlse2 = make_float2(nlse, nlse), ndel2 = make_float2(ndel, ndel);
-    const int whole = (last_visible(a, t, q0) + 1) / kRows;   // key tiles that every row sees whole
-    for (int n = 0; n < total; ++n) {
-      const uint32_t ts = tS + (n & 1) * 128 + lanes + side * 64;
-      wait.warp(&s_full[n & 1], n >> 1);
+    auto statistics = [&](const DqItem& w) {
+      nlse = -INFINITY;
+      ndel = 0.f;
+      if (w.hq >= 0 && row < w.valid) {
+        const float* st = stat_tile(args, w.hq, query_slot(a, w.t, w.t.tile, kRows));
+        nlse = st[row];
+        ndel = st[kRows + row];
+      }
+    };
+    DqItem w = dq_item(args, round);
+    statistics(w);
+    while (w.hq >= 0 && __all_sync(kFull, wait.ok)) {
+      const int q0 = w.t.tile * kRows;
+      const float2 nlse2 = make_float2(nlse, nlse), ndel2 = make_float2(ndel, ndel);
+      const int last = row < w.valid ? last_visible(a, w.t, q0 + row) : -1;
+      const int whole = (last_visible(a, w.t, q0) + 1) / kRows;   // key tiles that every row sees whole
+      for (int n = 0; n < w.total; ++n, ++tile) {
+        const uint32_t ts = tS + (tile & 1) * 128 + lanes + side * 64;
+        wait.warp(&s_full[tile & 1], tile >> 1);
+        tc::fence_after_sync();
+        float p[64], dp[64];
+        tc::tmem_ld64(ts, p);
+#pragma unroll
+        for (int c = 0; c < 64; c += 2) {
+          const float2 u = ex2_mixed(tc::fma2(make_float2(p[c], p[c + 1]), sl2, nlse2), c / 2, kPolyQ);
+          p[c] = u.x;
+          p[c + 1] = u.y;
+        }
+        wait.warp(&dp_full, tile);
+        tc::fence_after_sync();
+        tc::tmem_ld64(tP + lanes + side * 64, dp);
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&dp_free);
+        uint32_t x[32];
+        const int lim = last - n * kRows - side * 64;
+#pragma unroll
+        for (int c = 0; c < 64; c += 2) {
+          const float2 u = mul2(tc::fma2(make_float2(dp[c], dp[c + 1]), sc2, ndel2), make_float2(p[c], p[c + 1]));
+          dp[c] = u.x;
+          dp[c + 1] = u.y;
+        }
+        if (n >= whole) {
+#pragma unroll
+          for (int c = 0; c < 64; ++c)
+            if (c > lim) dp[c] = 0.f;
+        }
+#pragma unroll
+        for (int c = 0; c < 64; c += 2) x[c / 2] = pack2<T>(dp[c], dp[c + 1]);
+        tmem_st32(ts, x);
+        tmem_wait_st();
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&ds_full);
+      }
+      const DqItem next = dq_item(args, round);
+      statistics(next);
+      if (w.total > 0) wait.warp(&done, used++);
       tc::fence_after_sync();
-      float p[64], dp[64];
-      tc::tmem_ld64(ts, p);
-#pragma unroll
-      for (int c = 0; c < 64; c += 2) {
-        const float2 u = ex2_mixed(tc::fma2(make_float2(p[c], p[c + 1]), sl2, nlse2), c / 2, kPolyQ);
-        p[c] = u.x;
-        p[c + 1] = u.y;
-      }
-      wait.warp(&dp_full, n);
-      tc::fence_after_sync();
-      tc::tmem_ld64(tP + lanes + side * 64, dp);
-      tc::fence_before_sync();
+      // each side stores half of the columns
+      const int rows = min(32, w.valid - quarter * 32);
+      const int64_t at = (int64_t(w.t.b) * a.T + w.t.q_begin + q0 + quarter * 32) * a.Hq + w.hq;
+      store_lanes<T, DP / 2>(tQ + lanes + side * (DP / 2), w.total <= 0, wait.ok ? 1.f : NAN, out_addr + warp * 32 * DP,
+                             static_cast<T*>(a.dq) + at * a.D + side * (DP / 2), int64_t(a.Hq) * a.D, rows,
+                             a.D - side * (DP / 2), lane);
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&dp_free);
-      uint32_t w[32];
-      const int lim = last - n * kRows - side * 64;
-#pragma unroll
-      for (int c = 0; c < 64; c += 2) {
-        const float2 u = mul2(tc::fma2(make_float2(dp[c], dp[c + 1]), sc2, ndel2), make_float2(p[c], p[c + 1]));
-        dp[c] = u.x;
-        dp[c + 1] = u.y;
-      }
-      if (n >= whole) {
-#pragma unroll
-        for (int c = 0; c < 64; ++c)
-          if (c > lim) dp[c] = 0.f;
-      }
-#pragma unroll
-      for (int c = 0; c < 64; c += 2) w[c / 2] = pack2<T>(dp[c], dp[c + 1]);
-      tmem_st32(ts, w);
-      tmem_wait_st();
-      tc::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&ds_full);
+      w = next;
     }
-    if (total > 0) wait.warp(&done, 0);
-    tc::fence_after_sync();
-    // each side stores half of the columns, staged in the Q tile (its last reader is done)
-    const int rows = min(32, valid - quarter * 32);
-    const int64_t at = (int64_t(t.b) * a.T + t.q_begin + q0 + quarter * 32) * a.Hq + hq;
-    store_lanes<T, DP / 2>(tQ + lanes + side * (DP / 2), total == 0, wait.ok ? 1.f : NAN, q_addr + warp * 32 * DP,
-                           static_cast<T*>(a.dq) + at * a.D + side * (DP / 2), int64_t(a.Hq) * a.D, rows,
-                           a.D - side * (DP / 2), lane);
   }
   tc::fence_before_sync();
   __syncthreads();
@@ -610,7 +675,8 @@ int bwd_t(const BwdTcArgs& a, cudaStream_t s) {
   dense_stats_kernel<T, DP><<<dim3(unsigned(wide), kRows / kStatTokens + 1), 256, 0, s>>>(a);
   PISA_CHECK_LAUNCH();
   int rc = launch<dense_dkv_tc_kernel<T, DP>>(a.k_slots * d.H, BwdTile<DP>::SMEM, a, s);
-  return rc ? rc : launch<dense_dq_tc_kernel<T, DP>>(a.q_slots * d.Hq, BwdTile<DP>::SMEM, a, s);
+  if (rc) return rc;
+  return launch<dense_dq_tc_kernel<T, DP>>(min64(a.q_slots * d.Hq, sm_count()), BwdTile<DP>::DQ_SMEM, a, s);
 }
 
 }  // namespace
