@@ -46,6 +46,7 @@ struct BwdTcArgs {
   DenseAttnArgs d;
   float* stats;                          // [Hq][q_slots][2][128]
   SeqTile* order;                        // query tiles, then key tiles, in falling order of their work
+  int* counters;                         // items of launches 2 and 3 drawn past each CTA's first
   int64_t q_slots, k_slots;
   int bf16;
 };
@@ -55,8 +56,9 @@ template <int DP> struct BwdTile {
   // ring of operand tiles (Q dO Q dO ... or K V K V ...): 64 dims leave room
   // for three pairs, which also keeps a second CTA off the SM's TMEM
   static constexpr int RING = DP == 128 ? 4 : 6;
-  static constexpr int SMEM = (2 + RING) * BYTES + RING / 2 * 1024 + 1024;
-  static constexpr int DQ_SMEM = (3 + RING) * BYTES + 1024;   // with the output's staging
+  // with statistics and the outputs' staging
+  static constexpr int DKV_SMEM = (2 + RING) * BYTES + RING / 2 * 1024 + 8 * 32 * 64 + 1024;
+  static constexpr int DQ_SMEM = (3 + RING) * BYTES + 1024;
 };
 
 __device__ __forceinline__ float* stat_tile(const BwdTcArgs& a, int hq, int64_t slot) {
@@ -74,7 +76,10 @@ __global__ void __launch_bounds__(256) dense_stats_kernel(const __grid_constant_
   const int slot = blockIdx.x;
   if (blockIdx.y == kRows / kStatTokens) {
     // the order of the tiles in the launches that follow: eight ranks per CTA
-    if (slot == 0 && threadIdx.x == 0) *a.status = PISA_OK;
+    if (slot == 0 && threadIdx.x == 0) {
+      *a.status = PISA_OK;
+      args.counters[0] = args.counters[1] = 0;
+    }
     const int64_t r = slot * int64_t(8) + threadIdx.x / 32, all = args.q_slots + args.k_slots;
     if (r >= all) return;
     const bool by_keys = r >= args.q_slots;
@@ -150,7 +155,75 @@ struct Wait {
   __device__ __forceinline__ void warp(uint64_t* bar, int phase) { ok = wait_phase(bar, phase, fail) && ok; }
 };
 
-// Launch 2.
+// Launches 2 and 3 run one persistent CTA per SM.  Items come from a counter in
+// falling order of their work: the loading thread draws the next one when it
+// has issued the last load of the current one, so that the next item's loads
+// and first scores overlap the outputs before them.  (A CTA per item paid 7000
+// cycles for its start and end; a fixed share per CTA left packed documents
+// with four heads to a group 17 % above the mean.)  Which CTA takes an item
+// changes nothing in its result.  All phases and ring positions run on across
+// items.
+template <typename Item> struct Queue {
+  uint64_t full[2], empty[2];
+  Item item[2];
+  __device__ __forceinline__ void init() {
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&full[i], 1);
+      tc::mbar_init(&empty[i], 10);   // MMA, trimming and eight softmax warps
+    }
+  }
+  __device__ __forceinline__ void put(int n, const Item& w, Wait& wait) {   // one thread
+    if (!wait(&empty[n & 1], (n >> 1) + 1)) return;
+    item[n & 1] = w;
+    tc::mbar_arrive(&full[n & 1]);
+  }
+  // item n (every lane of the calling warp), handed back when read
+  __device__ __forceinline__ Item take(int n, Wait& wait, int lane) {
+    wait.warp(&full[n & 1], n >> 1);
+    Item w = item[n & 1];
+    __syncwarp();
+    if (lane == 0 && wait.ok) tc::mbar_arrive(&empty[n & 1]);
+    if (!__all_sync(kFull, wait.ok)) w.head = -1;
+    return w;
+  }
+};
+
+// Draws positions of the list until `visit` accepts one; false at its end.
+template <typename F> __device__ __forceinline__ bool draw(int n, int items, int* counter, F visit) {
+  for (bool first = n == 0;; first = false) {
+    const int at = first ? int(blockIdx.x) : int(gridDim.x) + atomicAdd(counter, 1);
+    if (at >= items) return false;
+    if (visit(at)) return true;
+  }
+}
+
+// Launch 2.  An item: key tile, KV head.
+struct DkvItem {
+  SeqTile t;
+  int head;                           // < 0: no item
+  int first_tile, end_tile;           // query tiles that see a key of the tile
+  int per_head, total, tail;          // their number, with all heads of the group; real rows of the last one
+};
+
+__device__ __forceinline__ DkvItem dkv_item(const BwdTcArgs& args, int n) {
+  const DenseAttnArgs& a = args.d;
+  DkvItem w;
+  const bool found = draw(n, int(args.k_slots * a.H), args.counters, [&](int at) {
+    const int slot = at / a.H, j0 = (w.t = args.order[args.q_slots + slot]).tile * kRows;
+    if (j0 >= w.t.k_len) return false;   // a slot without rows
+    w.head = at - slot * a.H;
+    const int first = first_seeing(a, w.t, j0);
+    w.first_tile = first / kRows;
+    w.end_tile = (w.t.q_len + kRows - 1) / kRows;
+    w.per_head = first < w.t.q_len ? w.end_tile - w.first_tile : 0;
+    w.total = w.per_head * a.G;
+    w.tail = w.t.q_len - (w.end_tile - 1) * kRows;
+    return true;
+  });
+  if (!found) w.head = -1;
+  return w;
+}
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_constant__ BwdTcArgs args) {
   using L = BwdTile<DP>;
@@ -158,22 +231,17 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t base = (tc::smem_u32(smem_raw) + 1023) & ~1023u;
   const uint32_t k_addr = base, v_addr = base + L::BYTES, ring = base + 2 * L::BYTES;
-  const uint32_t stat_addr = ring + L::RING * L::BYTES;
+  const uint32_t stat_addr = ring + L::RING * L::BYTES, out_addr = stat_addr + L::RING / 2 * 1024;
   const float* stat_smem = reinterpret_cast<const float*>(smem_raw + (stat_addr - tc::smem_u32(smem_raw)));
-  __shared__ uint64_t kv_full, full[L::RING], raw[L::RING], empty[L::RING], s_full, p_full, dp_full, ds_full, done;
+  __shared__ uint64_t kv_full, kv_empty, full[L::RING], raw[L::RING], empty[L::RING];
+  __shared__ uint64_t s_full, p_full, dp_full, ds_full, done, drained;
+  __shared__ Queue<DkvItem> queue;
   __shared__ uint32_t tmem_slot;
   __shared__ int s_fail;
   const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
-  const int rank = int(blockIdx.x) / a.H, h = int(blockIdx.x) - rank * a.H;
-  const SeqTile t = args.order[args.q_slots + rank];
-  const int j0 = t.tile * kRows;
-  if (j0 >= t.k_len) return;
-  const int first_tile = first_seeing(a, t, j0) / kRows, end_tile = (t.q_len + kRows - 1) / kRows;
-  const int per_head = first_seeing(a, t, j0) < t.q_len ? end_tile - first_tile : 0;
-  const int total = per_head * a.G;
-  const int tail = t.q_len - (end_tile - 1) * kRows;   // real rows of the last query tile
   if (tid == 0) {
     tc::mbar_init(&kv_full, 1);
+    tc::mbar_init(&kv_empty, 1);
     for (int i = 0; i < L::RING; ++i) {
       tc::mbar_init(&full[i], 1);
       tc::mbar_init(&raw[i], 1);
@@ -184,6 +252,8 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
     tc::mbar_init(&dp_full, 1);
     tc::mbar_init(&ds_full, 8);
     tc::mbar_init(&done, 1);
+    tc::mbar_init(&drained, 1);
+    queue.init();
     s_fail = 0;
     tc::fence_barrier_init();
   }
@@ -194,90 +264,108 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
   const uint32_t tmem = __shfl_sync(kFull, tmem_slot, 0);
   const uint32_t tS = tmem, tP = tmem + 128, tV = tmem + 256, tK = tmem + 256 + DP;
   Wait wait{&s_fail};
-  // tile n: query head h*G + n / per_head, query tile first_tile + n % per_head;
-  // ring position 2n holds its Q (and statistics), 2n + 1 its dO
-  // after an expired wait: the copies in flight land before the CTA ends
-  auto drain = [&](int issued) {
-    for (int pos = max(0, issued - L::RING); pos < issued; ++pos) wait_phase(&full[pos % L::RING], pos / L::RING, &s_fail);
-  };
-  auto ragged = [&](int n) { return tail < kRows && (n + 1) % per_head == 0; };
+  // tile n of an item: query head h*G + n / per_head, query tile first_tile +
+  // n % per_head; one ring position holds its Q (and statistics), the next its dO
 
   if (warp == kLoadWarp) {
-    if (lane == 0 && total > 0) {
-      tc::mbar_arrive_expect_tx(&kv_full, 2 * L::BYTES);
-      load_tile<DP>(k_addr, &args.tm_k, h, t.k_begin + j0, t.b, &kv_full);
-      load_tile<DP>(v_addr, &args.tm_v, h, t.k_begin + j0, t.b, &kv_full);
-      int g = 0, qt = first_tile, issued = 0;
-      for (int n = 0; n < total; ++n) {
-        const bool rag = ragged(n);
-        const int row = t.q_begin + qt * kRows, hq = h * a.G + g;
+    if (lane == 0) {
+      int pos = 0, used = 0;          // ring position; items with queries so far
+      for (int n = 0; wait.ok; ++n) {
+        const DkvItem w = dkv_item(args, n);
+        queue.put(n, w, wait);
+        if (w.head < 0) break;
+        if (w.total == 0) continue;
+        if (!wait(&kv_empty, used + 1)) break;
+        tc::mbar_arrive_expect_tx(&kv_full, 2 * L::BYTES);
+        load_tile<DP>(k_addr, &args.tm_k, w.head, w.t.k_begin + w.t.tile * kRows, w.t.b, &kv_full);
+        load_tile<DP>(v_addr, &args.tm_v, w.head, w.t.k_begin + w.t.tile * kRows, w.t.b, &kv_full);
+        ++used;
+        int g = 0, qt = w.first_tile;
+        for (int i = 0; i < w.total && wait.ok; ++i) {
+          const bool ragged = w.tail < kRows && qt + 1 == w.end_tile;
+          const int row = w.t.q_begin + qt * kRows, hq = w.head * a.G + g;
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int pos = 2 * n + x, st = pos % L::RING;
-          if (!wait(&empty[st], (pos / L::RING) + 1)) break;
-          uint64_t* bar = rag ? &raw[st] : &full[st];
-          tc::mbar_arrive_expect_tx(bar, L::BYTES + (x == 0 ? 1024 : 0));
-          load_tile<DP>(ring + st * L::BYTES, x == 0 ? &args.tm_q : &args.tm_do, hq, row, t.b, bar);
-          issued = pos + 1;
-          if (x == 0) bulk_load(stat_addr + (st / 2) * 1024, stat_tile(args, hq, query_slot(a, t, qt, kRows)), 1024, bar);
+          for (int x = 0; x < 2; ++x, ++pos) {
+            const int st = pos % L::RING;
+            if (!wait(&empty[st], (pos / L::RING) + 1)) break;
+            uint64_t* bar = ragged ? &raw[st] : &full[st];   // rows of a ragged tile pass through the trimming warp
+            tc::mbar_arrive_expect_tx(bar, L::BYTES + (x == 0 ? 1024 : 0));
+            load_tile<DP>(ring + st * L::BYTES, x == 0 ? &args.tm_q : &args.tm_do, hq, row, w.t.b, bar);
+            if (x == 0)
+              bulk_load(stat_addr + (st / 2) * 1024, stat_tile(args, hq, query_slot(a, w.t, qt, kRows)), 1024, bar);
+          }
+          if (++qt == w.end_tile) { qt = w.first_tile; ++g; }
         }
-        if (!wait.ok) break;
-        if (++qt == end_tile) { qt = first_tile; ++g; }
       }
-      if (!wait.ok) drain(issued);
+      if (!wait.ok) {                 // the copies in flight land before the CTA ends
+        if (used) wait_phase(&kv_full, used - 1, &s_fail);
+        for (int x = max(0, pos - L::RING); x < pos; ++x) wait_phase(&full[x % L::RING], x / L::RING, &s_fail);
+      }
     }
     __syncwarp();
   } else if (warp == kTrimWarp) {
-    if (tail < kRows && total > 0) {
-      uint32_t uses = 0;   // parity of the ragged tiles that each ring slot has held
-      for (int n = per_head - 1; n < total; n += per_head) {
-        for (int pos = 2 * n; pos < 2 * n + 2; ++pos) {
-          const int st = pos % L::RING;
-          wait.warp(&raw[st], uses >> st);
-          uses ^= 1u << st;
-          zero_rows<DP>(ring + st * L::BYTES, tail, (tail + 15) & ~15, lane);
-          tc::fence_async_smem();
-          __syncwarp();
-          if (lane == 0 && wait.ok) tc::mbar_arrive(&full[st]);
+    int start = 0;                    // the item's first ring position
+    uint32_t uses = 0;                // parity of the ragged tiles that each ring slot has held
+    for (int i = 0;; ++i) {
+      const DkvItem w = queue.take(i, wait, lane);
+      if (w.head < 0) break;
+      if (w.total > 0 && w.tail < kRows) {
+        for (int n = w.per_head - 1; n < w.total; n += w.per_head) {
+          for (int x = 0; x < 2; ++x) {
+            const int st = (start + 2 * n + x) % L::RING;
+            wait.warp(&raw[st], uses >> st);
+            uses ^= 1u << st;
+            zero_rows<DP>(ring + st * L::BYTES, w.tail, (w.tail + 15) & ~15, lane);
+            tc::fence_async_smem();
+            __syncwarp();
+            if (lane == 0 && wait.ok) tc::mbar_arrive(&full[st]);
+          }
         }
       }
+      start += 2 * w.total;
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
-    if (total > 0) {
-      const bool leader = elect_one();
-      const uint32_t id_s = tc::idesc_f16(kRows, kRows, args.bf16), id_o = tc::idesc_f16(kRows, DP, args.bf16, 1);
-      wait.warp(&kv_full, 0);
-      // per query tile n: S(n) and dP(n) are issued one round ahead of the
-      // products that use them, each after the last use of its TMEM columns
-      int pos = 0, st = 0;                      // ring position 2 n and its slot
-      uint32_t phase = 0;                       // the slot's phase
-      wait.warp(&full[0], 0);
-      tc::fence_after_sync();
-      if (leader) {
-        mma_rows<DP>(tS, k_addr, ring, id_s);
-        tc::mma_commit(&s_full);
+    const bool leader = elect_one();
+    const uint32_t id_s = tc::idesc_f16(kRows, kRows, args.bf16), id_o = tc::idesc_f16(kRows, DP, args.bf16, 1);
+    int st = 0, tile = 0, used = 0;   // slot of a tile's Q (its dO is in the next one); tiles and items so far
+    uint32_t phase = 0;               // the slot's phase
+    for (int i = 0;; ++i) {
+      const DkvItem w = queue.take(i, wait, lane);
+      if (w.head < 0) break;
+      const int total = w.total, per_head = w.per_head, tail = w.tail;
+      // per query tile: S and dP are issued one round ahead of the products
+      // that use them, each after the last use of its TMEM columns
+      if (total > 0) {
+        wait.warp(&kv_full, used);
+        wait.warp(&full[st], int(phase));
+        tc::fence_after_sync();
+        if (leader) {
+          mma_rows<DP>(tS, k_addr, ring + st * L::BYTES, id_s);
+          tc::mma_commit(&s_full);
+        }
+        wait.warp(&full[st + 1], int(phase));
+        tc::fence_after_sync();
+        if (leader) {
+          mma_rows<DP>(tP, v_addr, ring + (st + 1) * L::BYTES, id_s);
+          tc::mma_commit(&dp_full);
+          if (total == 1) tc::mma_commit(&kv_empty);
+        }
+        ++used;
       }
-      wait.warp(&full[1], 0);
-      tc::fence_after_sync();
-      if (leader) {
-        mma_rows<DP>(tP, v_addr, ring + L::BYTES, id_s);
-        tc::mma_commit(&dp_full);
-      }
-      int left = per_head;                      // tiles to the head's last one
-      for (int n = 0; n < total && __all_sync(kFull, wait.ok); ++n) {
+      int left = per_head;            // tiles to the head's last one
+      for (int n = 0; n < total && __all_sync(kFull, wait.ok); ++n, ++tile) {
         const bool rag = tail < kRows && left == 1;
         left = left == 1 ? per_head : left - 1;
         const int steps = rag ? (tail + 15) / 16 : kRows / 16;
         const uint32_t q = ring + st * L::BYTES;
         const int next = st + 2 == L::RING ? 0 : st + 2;
         const uint32_t next_phase = next ? phase : phase ^ 1;
-        wait.warp(&p_full, n);
+        wait.warp(&p_full, tile);     // and the outputs of the item before have been read
         tc::fence_after_sync();
-        // a slot that no later tile takes is not handed back: nothing may arrive after the CTA's end
         if (leader) {
           mma_cols(tV, tS, 64, q + L::BYTES, id_o, steps, n > 0);
-          if (pos + 1 + L::RING < 2 * total) tc::mma_commit(&empty[st + 1]);
+          tc::mma_commit(&empty[st + 1]);
         }
         if (n + 1 < total) {
           wait.warp(&full[next], int(next_phase));
@@ -287,11 +375,12 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
             tc::mma_commit(&s_full);
           }
         }
-        wait.warp(&ds_full, n);
+        wait.warp(&ds_full, tile);
         tc::fence_after_sync();
         if (leader) {
           mma_cols(tK, tP, 64, q, id_o, steps, n > 0);
-          if (pos + L::RING < 2 * total) tc::mma_commit(&empty[st]);
+          tc::mma_commit(&empty[st]);
+          if (n + 1 == total) tc::mma_commit(&done);
         }
         if (n + 1 < total) {
           wait.warp(&full[next + 1], int(next_phase));
@@ -299,99 +388,106 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
           if (leader) {
             mma_rows<DP>(tP, v_addr, ring + (next + 1) * L::BYTES, id_s);
             tc::mma_commit(&dp_full);
+            if (n + 2 == total) tc::mma_commit(&kv_empty);
           }
         }
-        pos += 2;
         st = next;
         phase = next_phase;
       }
-      if (leader) tc::mma_commit(&done);
-      if (!__all_sync(kFull, wait.ok)) wait_phase(&done, 0, &s_fail);
     }
+    if (leader) tc::mma_commit(&drained);
+    wait_phase(&drained, 0, &s_fail);
     __syncwarp();
   } else {
     const int side = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;   // key row, queries 64*side ..
     const uint32_t lanes = uint32_t(quarter * 32) << 16;
     const uint32_t ts = tS + lanes + side * 64, tp = tP + lanes + side * 64;
     const float2 sl2 = make_float2(a.scale * kLog2e, a.scale * kLog2e), sc2 = make_float2(a.scale, a.scale);
-    const int first = first_seeing(a, t, j0 + row), whole = first_seeing(a, t, j0 + kRows - 1);
-    int qt = first_tile;
-    for (int n = 0; n < total; ++n) {
-      const int st = (2 * n) % L::RING;
-      wait.warp(&full[st], (2 * n) / L::RING);
-      wait.warp(&s_full, n);
+    int tile = 0, used = 0, item = 0;
+    DkvItem w = queue.take(item, wait, lane);
+    while (w.head >= 0) {
+      const int j0 = w.t.tile * kRows;
+      const int first = first_seeing(a, w.t, j0 + row), whole = first_seeing(a, w.t, j0 + kRows - 1);
+      int qt = w.first_tile;
+      for (int n = 0; n < w.total; ++n, ++tile) {
+        const int st = (2 * tile) % L::RING;
+        wait.warp(&full[st], (2 * tile) / L::RING);
+        wait.warp(&s_full, tile);
+        tc::fence_after_sync();
+        const float4* nlse = reinterpret_cast<const float4*>(stat_smem + (st / 2) * 256 + side * 64);
+        const float4* ndel = nlse + kRows / 4;
+        float p[64];
+        uint32_t x16[32];
+        tc::tmem_ld64(ts, p);
+#pragma unroll
+        for (int c = 0; c < 64; c += 4) {
+          const float4 x = nlse[c / 4];
+          const float2 u = ex2_mixed(tc::fma2(make_float2(p[c], p[c + 1]), sl2, make_float2(x.x, x.y)), c / 2, kPolyKv);
+          const float2 v = ex2_mixed(tc::fma2(make_float2(p[c + 2], p[c + 3]), sl2, make_float2(x.z, x.w)), c / 2 + 1, kPolyKv);
+          p[c] = u.x;
+          p[c + 1] = u.y;
+          p[c + 2] = v.x;
+          p[c + 3] = v.y;
+        }
+        const bool edge = qt * kRows < whole || (w.tail < kRows && qt + 1 == w.end_tile);
+        if (edge) {
+          // queries before column `low` do not see the key, those from `high` on are not the sequence's
+          const int low = first - qt * kRows - side * 64, high = w.t.q_len - qt * kRows - side * 64;
+#pragma unroll
+          for (int c = 0; c < 64; ++c)
+            if (c < low || c >= high) p[c] = 0.f;
+        }
+#pragma unroll
+        for (int c = 0; c < 64; c += 2) x16[c / 2] = pack2<T>(p[c], p[c + 1]);
+        tmem_st32(ts, x16);
+        tmem_wait_st();
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&p_full);
+        wait.warp(&dp_full, tile);
+        tc::fence_after_sync();
+        float dp[64];
+        tc::tmem_ld64(tp, dp);
+#pragma unroll
+        for (int c = 0; c < 64; c += 4) {
+          const float4 x = ndel[c / 4];
+          const float2 u = mul2(tc::fma2(make_float2(dp[c], dp[c + 1]), sc2, make_float2(x.x, x.y)), make_float2(p[c], p[c + 1]));
+          const float2 v =
+              mul2(tc::fma2(make_float2(dp[c + 2], dp[c + 3]), sc2, make_float2(x.z, x.w)), make_float2(p[c + 2], p[c + 3]));
+          dp[c] = u.x;
+          dp[c + 1] = u.y;
+          dp[c + 2] = v.x;
+          dp[c + 3] = v.y;
+        }
+        if (edge) {   // without weight no gradient, whatever dP holds there
+#pragma unroll
+          for (int c = 0; c < 64; ++c)
+            if (p[c] == 0.f) dp[c] = 0.f;
+        }
+#pragma unroll
+        for (int c = 0; c < 64; c += 2) x16[c / 2] = pack2<T>(dp[c], dp[c + 1]);
+        tmem_st32(tp, x16);
+        tmem_wait_st();
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&ds_full);
+        if (++qt == w.end_tile) qt = w.first_tile;
+      }
+      const DkvItem next = queue.take(++item, wait, lane);
+      if (w.total > 0) wait.warp(&done, used++);
       tc::fence_after_sync();
-      const float4* nlse = reinterpret_cast<const float4*>(stat_smem + (st / 2) * 256 + side * 64);
-      const float4* ndel = nlse + kRows / 4;
-      float p[64];
-      uint32_t w[32];
-      tc::tmem_ld64(ts, p);
-#pragma unroll
-      for (int c = 0; c < 64; c += 4) {
-        const float4 x = nlse[c / 4];
-        const float2 u = ex2_mixed(tc::fma2(make_float2(p[c], p[c + 1]), sl2, make_float2(x.x, x.y)), c / 2, kPolyKv);
-        const float2 v = ex2_mixed(tc::fma2(make_float2(p[c + 2], p[c + 3]), sl2, make_float2(x.z, x.w)), c / 2 + 1, kPolyKv);
-        p[c] = u.x;
-        p[c + 1] = u.y;
-        p[c + 2] = v.x;
-        p[c + 3] = v.y;
+      // warps of side 0 store dV, of side 1 dK, 32 columns at a time
+      const int rows = min(32, w.t.k_len - (j0 + quarter * 32)), cols = side ? a.D : a.Dv;
+      const int64_t at = (int64_t(w.t.b) * a.N + w.t.k_begin + j0 + quarter * 32) * a.H + w.head;
+      T* to = static_cast<T*>(side ? a.dk : a.dv) + at * cols;
+#pragma unroll 1
+      for (int c = 0; c < DP; c += 32) {
+        store_lanes<T, 32>((side ? tK : tV) + lanes + c, w.total == 0, wait.ok ? 1.f : NAN, out_addr + warp * 32 * 64, to + c,
+                           int64_t(a.H) * cols, rows, cols - c, lane);
+        __syncwarp();
       }
-      const bool edge = qt * kRows < whole || ragged(n);
-      if (edge) {
-        // queries before column `low` do not see the key, those from `high` on are not the sequence's
-        const int low = first - qt * kRows - side * 64, high = t.q_len - qt * kRows - side * 64;
-#pragma unroll
-        for (int c = 0; c < 64; ++c)
-          if (c < low || c >= high) p[c] = 0.f;
-      }
-#pragma unroll
-      for (int c = 0; c < 64; c += 2) w[c / 2] = pack2<T>(p[c], p[c + 1]);
-      tmem_st32(ts, w);
-      tmem_wait_st();
-      tc::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&p_full);
-      wait.warp(&dp_full, n);
-      tc::fence_after_sync();
-      float dp[64];
-      tc::tmem_ld64(tp, dp);
-#pragma unroll
-      for (int c = 0; c < 64; c += 4) {
-        const float4 x = ndel[c / 4];
-        const float2 u = mul2(tc::fma2(make_float2(dp[c], dp[c + 1]), sc2, make_float2(x.x, x.y)), make_float2(p[c], p[c + 1]));
-        const float2 v =
-            mul2(tc::fma2(make_float2(dp[c + 2], dp[c + 3]), sc2, make_float2(x.z, x.w)), make_float2(p[c + 2], p[c + 3]));
-        dp[c] = u.x;
-        dp[c + 1] = u.y;
-        dp[c + 2] = v.x;
-        dp[c + 3] = v.y;
-      }
-      if (edge) {   // without weight no gradient, whatever dP holds there
-#pragma unroll
-        for (int c = 0; c < 64; ++c)
-          if (p[c] == 0.f) dp[c] = 0.f;
-      }
-#pragma unroll
-      for (int c = 0; c < 64; c += 2) w[c / 2] = pack2<T>(dp[c], dp[c + 1]);
-      tmem_st32(tp, w);
-      tmem_wait_st();
-      tc::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&ds_full);
-      if (++qt == end_tile) qt = first_tile;
+      w = next;
     }
-    if (total > 0) wait.warp(&done, 0);
-    tc::fence_after_sync();
-    // warps of side 0 store dV, of side 1 dK, staged in the V and K tiles
-    const int rows = min(32, t.k_len - (j0 + quarter * 32));
-    const int64_t at = (int64_t(t.b) * a.N + t.k_begin + j0 + quarter * 32) * a.H + h;
-    const float mul = wait.ok ? 1.f : NAN;
-    if (side == 0)
-      store_lanes<T, DP>(tV + lanes, total == 0, mul, v_addr + quarter * 32 * DP * 2, static_cast<T*>(a.dv) + at * a.Dv,
-                         int64_t(a.H) * a.Dv, rows, a.Dv, lane);
-    else
-      store_lanes<T, DP>(tK + lanes, total == 0, mul, k_addr + quarter * 32 * DP * 2, static_cast<T*>(a.dk) + at * a.D,
-                         int64_t(a.H) * a.D, rows, a.D, lane);
   }
   tc::fence_before_sync();
   __syncthreads();
@@ -400,35 +496,29 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
   if (warp == kMmaWarp) tc::tmem_free(tmem, 512);
 }
 
-// Launch 3: a persistent CTA per SM.  Items (query tile, head) are taken in
-// falling order of their work, every other round backwards; the next item's
-// loads and first scores overlap the output of the one before.  All phases and
-// ring positions run on across items.
+// Launch 3.  An item: query tile, query head.
 struct DqItem {
   SeqTile t;
-  int hq, valid, total, tail;   // hq < 0: no item; real rows; key tiles, and the real rows of the last
+  int head;                           // < 0: no item
+  int valid, total, tail;             // real rows; key tiles, and the real rows of the last one
 };
 
-__device__ __forceinline__ DqItem dq_item(const BwdTcArgs& args, int& round) {
+__device__ __forceinline__ DqItem dq_item(const BwdTcArgs& args, int n) {
   const DenseAttnArgs& a = args.d;
-  const int64_t items = args.q_slots * a.Hq;
-  const int g = int(gridDim.x), c = int(blockIdx.x);
   DqItem w;
-  w.hq = -1;
-  for (;; ++round) {
-    const int64_t at = int64_t(round) * g + (round & 1 ? g - 1 - c : c);
-    if (at >= items) return w;
-    const int slot = int(at / a.Hq);
+  const bool found = draw(n, int(args.q_slots * a.Hq), args.counters + 1, [&](int at) {
+    const int slot = at / a.Hq;
     w.t = args.order[slot];
     w.valid = min(kRows, w.t.q_len - w.t.tile * kRows);
-    if (w.valid <= 0) continue;   // a slot without rows
-    w.hq = int(at - int64_t(slot) * a.Hq);
+    if (w.valid <= 0) return false;      // a slot without rows
+    w.head = at - slot * a.Hq;
     const int keys = last_visible(a, w.t, w.t.tile * kRows + w.valid - 1) + 1;
     w.total = (keys + kRows - 1) / kRows;
     w.tail = min(kRows, w.t.k_len - (w.total - 1) * kRows);
-    ++round;
-    return w;
-  }
+    return true;
+  });
+  if (!found) w.head = -1;
+  return w;
 }
 
 template <typename T, int DP>
@@ -440,6 +530,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
   const uint32_t q_addr = base, o_addr = base + L::BYTES, out_addr = base + 2 * L::BYTES, ring = base + 3 * L::BYTES;
   __shared__ uint64_t q_full, q_empty, full[L::RING], raw[L::RING], empty[L::RING];
   __shared__ uint64_t s_full[2], dp_full, dp_free, ds_full, done, drained;
+  __shared__ Queue<DqItem> queue;
   __shared__ uint32_t tmem_slot;
   __shared__ int s_fail;
   const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
@@ -458,6 +549,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
     tc::mbar_init(&ds_full, 8);
     tc::mbar_init(&done, 1);
     tc::mbar_init(&drained, 1);
+    queue.init();
     s_fail = 0;
     tc::fence_barrier_init();
   }
@@ -468,20 +560,20 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
   const uint32_t tmem = __shfl_sync(kFull, tmem_slot, 0);
   const uint32_t tS = tmem, tP = tmem + 256, tQ = tmem + 384;   // two S, whose dS overwrites it; dP; dQ
   Wait wait{&s_fail};
-  int round = 0;
 
   if (warp == kLoadWarp) {
     if (lane == 0) {
       int pos = 0, used = 0;                    // ring position; items with keys so far
-      while (wait.ok) {
-        const DqItem w = dq_item(args, round);
-        if (w.hq < 0) break;
+      for (int n = 0; wait.ok; ++n) {
+        const DqItem w = dq_item(args, n);
+        queue.put(n, w, wait);
+        if (w.head < 0) break;
         if (w.total <= 0) continue;
-        const int h = w.hq / a.G;
+        const int h = w.head / a.G;
         if (!wait(&q_empty, used + 1)) break;
         tc::mbar_arrive_expect_tx(&q_full, 2 * L::BYTES);
-        load_tile<DP>(q_addr, &args.tm_q, w.hq, w.t.q_begin + w.t.tile * kRows, w.t.b, &q_full);
-        load_tile<DP>(o_addr, &args.tm_do, w.hq, w.t.q_begin + w.t.tile * kRows, w.t.b, &q_full);
+        load_tile<DP>(q_addr, &args.tm_q, w.head, w.t.q_begin + w.t.tile * kRows, w.t.b, &q_full);
+        load_tile<DP>(o_addr, &args.tm_do, w.head, w.t.q_begin + w.t.tile * kRows, w.t.b, &q_full);
         ++used;
         for (int x = 0; x < 2 * w.total; ++x, ++pos) {   // K0 V0 K1 V1 ...
           const int st = pos % L::RING;
@@ -501,9 +593,9 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
   } else if (warp == kTrimWarp) {
     int pos = 0;
     uint32_t uses = 0;                          // parity of the ragged tiles that each ring slot has held
-    for (;;) {
-      const DqItem w = dq_item(args, round);
-      if (w.hq < 0 || !__all_sync(kFull, wait.ok)) break;
+    for (int i = 0;; ++i) {
+      const DqItem w = queue.take(i, wait, lane);
+      if (w.head < 0) break;
       if (w.total <= 0) continue;
       pos += 2 * w.total;
       if (w.tail >= kRows) continue;
@@ -521,8 +613,9 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
     const uint32_t id_s = tc::idesc_f16(kRows, kRows, args.bf16), id_o = tc::idesc_f16(kRows, DP, args.bf16, 1);
     int st = 0, tile = 0, used = 0;             // slot of a tile's K (its V is in the next one); tiles and items so far
     uint32_t phase = 0;
-    DqItem w = dq_item(args, round);
-    while (w.hq >= 0 && __all_sync(kFull, wait.ok)) {
+    for (int i = 0;; ++i) {
+      const DqItem w = queue.take(i, wait, lane);
+      if (w.head < 0) break;
       const int total = w.total, steps = (w.tail + 15) / 16;
       if (total > 0) {
         wait.warp(&q_full, used);
@@ -542,7 +635,6 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
         }
         ++used;
       }
-      w = dq_item(args, round);
       for (int n = 0; n < total && __all_sync(kFull, wait.ok); ++n, ++tile) {
         const int next = st + 2 == L::RING ? 0 : st + 2;
         const uint32_t next_phase = next ? phase : phase ^ 1;
@@ -581,20 +673,20 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
     const int side = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;   // query row, keys 64*side ..
     const uint32_t lanes = uint32_t(quarter * 32) << 16;
     const float2 sl2 = make_float2(a.scale * kLog2e, a.scale * kLog2e), sc2 = make_float2(a.scale, a.scale);
-    int tile = 0, used = 0;
+    int tile = 0, used = 0, item = 0;
     float nlse = -INFINITY, ndel = 0.f;
     auto statistics = [&](const DqItem& w) {
       nlse = -INFINITY;
       ndel = 0.f;
-      if (w.hq >= 0 && row < w.valid) {
-        const float* st = stat_tile(args, w.hq, query_slot(a, w.t, w.t.tile, kRows));
+      if (w.head >= 0 && row < w.valid) {
+        const float* st = stat_tile(args, w.head, query_slot(a, w.t, w.t.tile, kRows));
         nlse = st[row];
         ndel = st[kRows + row];
       }
     };
-    DqItem w = dq_item(args, round);
+    DqItem w = queue.take(item, wait, lane);
     statistics(w);
-    while (w.hq >= 0 && __all_sync(kFull, wait.ok)) {
+    while (w.head >= 0) {
       const int q0 = w.t.tile * kRows;
       const float2 nlse2 = make_float2(nlse, nlse), ndel2 = make_float2(ndel, ndel);
       const int last = row < w.valid ? last_visible(a, w.t, q0 + row) : -1;
@@ -638,13 +730,13 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&ds_full);
       }
-      const DqItem next = dq_item(args, round);
+      const DqItem next = queue.take(++item, wait, lane);
       statistics(next);
       if (w.total > 0) wait.warp(&done, used++);
       tc::fence_after_sync();
       // each side stores half of the columns
       const int rows = min(32, w.valid - quarter * 32);
-      const int64_t at = (int64_t(w.t.b) * a.T + w.t.q_begin + q0 + quarter * 32) * a.Hq + w.hq;
+      const int64_t at = (int64_t(w.t.b) * a.T + w.t.q_begin + q0 + quarter * 32) * a.Hq + w.head;
       store_lanes<T, DP / 2>(tQ + lanes + side * (DP / 2), w.total <= 0, wait.ok ? 1.f : NAN, out_addr + warp * 32 * DP,
                              static_cast<T*>(a.dq) + at * a.D + side * (DP / 2), int64_t(a.Hq) * a.D, rows,
                              a.D - side * (DP / 2), lane);
@@ -661,7 +753,6 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
 
 template <auto Kernel>
 int launch(int64_t blocks, int smem, const BwdTcArgs& a, cudaStream_t s) {
-  if (blocks >= (int64_t(1) << 31)) return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
   if (int rc = allow_smem<Kernel>(smem, "dense attention smem attribute")) return rc;
   Kernel<<<unsigned(blocks), kThreads, smem, s>>>(a);
   PISA_CHECK_LAUNCH();
@@ -674,7 +765,7 @@ int bwd_t(const BwdTcArgs& a, cudaStream_t s) {
   const int64_t wide = a.q_slots > (a.q_slots + a.k_slots + 7) / 8 ? a.q_slots : (a.q_slots + a.k_slots + 7) / 8;
   dense_stats_kernel<T, DP><<<dim3(unsigned(wide), kRows / kStatTokens + 1), 256, 0, s>>>(a);
   PISA_CHECK_LAUNCH();
-  int rc = launch<dense_dkv_tc_kernel<T, DP>>(a.k_slots * d.H, BwdTile<DP>::SMEM, a, s);
+  int rc = launch<dense_dkv_tc_kernel<T, DP>>(min64(a.k_slots * d.H, sm_count()), BwdTile<DP>::DKV_SMEM, a, s);
   if (rc) return rc;
   return launch<dense_dq_tc_kernel<T, DP>>(min64(a.q_slots * d.Hq, sm_count()), BwdTile<DP>::DQ_SMEM, a, s);
 }
@@ -683,7 +774,8 @@ int bwd_t(const BwdTcArgs& a, cudaStream_t s) {
 
 int64_t dense_bwd_workspace(bool packed, int64_t B, int64_t T, int64_t N, int64_t Hq, int64_t sequences) {
   const int64_t q = seq_slots(packed, B, T, sequences, kRows), k = seq_slots(packed, B, N, sequences, kRows);
-  return q * Hq * 2 * kRows * int64_t(sizeof(float)) + (q + k) * int64_t(sizeof(SeqTile));
+  return q * Hq * 2 * kRows * int64_t(sizeof(float)) + (q + k) * int64_t(sizeof(SeqTile)) +
+         2 * int64_t(sizeof(int));
 }
 
 int dense_attn_bwd_tc(const DenseAttnArgs& d, int dtype, cudaStream_t stream) {
@@ -694,7 +786,8 @@ int dense_attn_bwd_tc(const DenseAttnArgs& d, int dtype, cudaStream_t stream) {
   a.q_slots = seq_slots(d.cu_q, d.B, d.T, d.sequences, kRows);
   a.k_slots = seq_slots(d.cu_q, d.B, d.N, d.sequences, kRows);
   a.order = reinterpret_cast<SeqTile*>(d.delta + a.q_slots * d.Hq * 2 * kRows);
-  if (a.q_slots + a.k_slots >= (int64_t(1) << 31)) return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
+  a.counters = reinterpret_cast<int*>(a.order + a.q_slots + a.k_slots);
+  if (a.q_slots * d.Hq >= (int64_t(1) << 31) - 4096 || a.k_slots * d.H >= (int64_t(1) << 31) - 4096) return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
   int rc = dense_tensor_map(&a.tm_q, d.q, dtype, d.B, d.T, d.Hq, d.D, d.q_sb, d.q_st, d.q_sh, kRows);
   if (rc == PISA_OK) rc = dense_tensor_map(&a.tm_k, d.k, dtype, d.B, d.N, d.H, d.D, d.k_sb, d.k_st, d.k_sh, kRows);
   if (rc == PISA_OK) rc = dense_tensor_map(&a.tm_v, d.v, dtype, d.B, d.N, d.H, d.Dv, d.v_sb, d.v_st, d.v_sh, kRows);
