@@ -37,14 +37,18 @@ constexpr int kThreads = 352;
 // Pairs of every eight whose exponential is a polynomial.  The softmax warps of
 // a CTA do the same phase at the same time, so the special-function unit bounds
 // one phase and idles in the other.  Training block, four sequences of 4096, 16
-// heads of 64: dK/dV 374 us with 0, 368 with 2, 363 with 3, 367 with 4; dQ 260
-// with 0, 251 with 2, 254 with 3, 261 with 4.
+// heads of 64: dK/dV 353 us with 0, 345 with 1, 346 with 2, 340 with 3, 348 with
+// 4; dQ 235, 231, 226, 232 and 238.
 constexpr int kPolyKv = 3, kPolyQ = 2;
+
+// Statistics of a query tile: -lse (base 2) and -scale * delta of its rows in
+// fp32, then 16 bytes per row for the products of launch 2 (see mma_stat).
+constexpr int kStat = 2 * kRows + kRows * 4, kStatBytes = kRows * 16;
 
 struct BwdTcArgs {
   CUtensorMap tm_q, tm_k, tm_v, tm_do;   // boxes of 64 dims x 128 rows of one head
   DenseAttnArgs d;
-  float* stats;                          // [Hq][q_slots][2][128]
+  float* stats;                          // [Hq][q_slots][kStat]
   SeqTile* order;                        // query tiles, then key tiles, in falling order of their work
   int* counters;                         // items of launches 2 and 3 drawn past each CTA's first
   int64_t q_slots, k_slots;
@@ -57,12 +61,43 @@ template <int DP> struct BwdTile {
   // for three pairs, which also keeps a second CTA off the SM's TMEM
   static constexpr int RING = DP == 128 ? 4 : 6;
   // with statistics and the outputs' staging
-  static constexpr int DKV_SMEM = (2 + RING) * BYTES + RING / 2 * 1024 + 8 * 32 * 64 + 1024;
+  static constexpr int DKV_SMEM = (2 + RING) * BYTES + (RING / 2 + 3) * kStatBytes + 8 * 32 * 64 + 1024;
   static constexpr int DQ_SMEM = (3 + RING) * BYTES + 1024;
 };
 
 __device__ __forceinline__ float* stat_tile(const BwdTcArgs& a, int hq, int64_t slot) {
-  return a.stats + (hq * a.q_slots + slot) * 2 * kRows;
+  return a.stats + (hq * a.q_slots + slot) * kStat;
+}
+
+// Factor of the scores in base 2, never quite zero (launch 2 divides by it).
+__device__ __forceinline__ float base2_scale(const DenseAttnArgs& a) {
+  const float sl = a.scale * kLog2e;
+  return fabsf(sl) < 1e-30f ? copysignf(1e-30f, sl) : sl;
+}
+
+// x = three bf16 values, to 24 bits
+__device__ __forceinline__ uint2 three_parts(float x) {
+  const __nv_bfloat16 hi = __float2bfloat16_rn(x);
+  const float rest = x - __bfloat162float(hi);
+  const __nv_bfloat16 mid = __float2bfloat16_rn(rest);
+  const __nv_bfloat16 lo = __float2bfloat16_rn(rest - __bfloat162float(mid));
+  return make_uint2(__bfloat16_as_ushort(hi) | uint32_t(__bfloat16_as_ushort(mid)) << 16, __bfloat16_as_ushort(lo));
+}
+
+// D += the row statistic of column j in every lane: one more step of the
+// product, whose A rows hold ones at the statistic's three parts and zeros
+// elsewhere and whose B rows are the tile's 16 bytes (the second 16 bytes of
+// both are `zeros`, the leading offset away).  The steps before had operands of
+// the input type; this one's are bf16 for either, as fp16 lacks the range.
+// Bound by shared-memory reads otherwise: a thread per key row needs the
+// statistics of all 64 columns, 512 cycles per tile and statistic.
+__device__ __forceinline__ void mma_stat(uint32_t d, uint32_t a, uint32_t b, uint32_t zeros) {
+  constexpr uint32_t kPlainHigh = (128u >> 4) | (1u << 14);   // 8-row groups 128 B apart, version 1, no swizzle
+  asm volatile(
+      "{\n\t.reg .b64 a, b;\n\t.reg .pred p;\n\tmov.b64 a, {%1, %4};\n\tmov.b64 b, {%2, %4};\n\tsetp.eq.u32 p, 0, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}"
+      :: "r"(d), "r"(desc_low(a, zeros - a)), "r"(desc_low(b, zeros - b)), "r"(tc::idesc_f16(kRows, kRows, 1)), "r"(kPlainHigh)
+      : "memory");
 }
 
 // Launch 1: kStatTokens queries x all heads per CTA, DP/8 lanes per row, each
@@ -129,9 +164,14 @@ __global__ void __launch_bounds__(256) dense_stats_kernel(const __grid_constant_
       for (int o = LANES / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(kFull, dot, o);
       if (lane == 0 && x < rows) {
         const int token = x / a.Hq;
-        float* st = stat_tile(args, x - token * a.Hq, slot) + token0 + token;
-        st[0] = lse[i] == -INFINITY ? -INFINITY : -lse[i] * kLog2e;
-        st[kRows] = -dot * a.scale;
+        float* tile = stat_tile(args, x - token * a.Hq, slot);
+        const int row = token0 + token;
+        const float nlse = -lse[i] * kLog2e, sl = base2_scale(a);
+        const bool dead = lse[i] == -INFINITY;
+        tile[row] = dead ? -INFINITY : nlse;
+        tile[kRows + row] = -dot * a.scale;
+        const uint2 m = three_parts(dead ? copysignf(0x1p127f, -sl) : nlse / sl), d3 = three_parts(-dot);
+        reinterpret_cast<uint4*>(tile + 2 * kRows)[row] = make_uint4(m.x, m.y, d3.x, d3.y);
       }
     }
   }
@@ -231,8 +271,9 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t base = (tc::smem_u32(smem_raw) + 1023) & ~1023u;
   const uint32_t k_addr = base, v_addr = base + L::BYTES, ring = base + 2 * L::BYTES;
-  const uint32_t stat_addr = ring + L::RING * L::BYTES, out_addr = stat_addr + L::RING / 2 * 1024;
-  const float* stat_smem = reinterpret_cast<const float*>(smem_raw + (stat_addr - tc::smem_u32(smem_raw)));
+  // statistics, the rows that pick each of them, zeros
+  const uint32_t stat_addr = ring + L::RING * L::BYTES, pick_lse = stat_addr + L::RING / 2 * kStatBytes;
+  const uint32_t pick_delta = pick_lse + kStatBytes, zeros = pick_delta + kStatBytes, out_addr = zeros + kStatBytes;
   __shared__ uint64_t kv_full, kv_empty, full[L::RING], raw[L::RING], empty[L::RING];
   __shared__ uint64_t s_full, p_full, dp_full, ds_full, done, drained;
   __shared__ Queue<DkvItem> queue;
@@ -256,6 +297,13 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
     queue.init();
     s_fail = 0;
     tc::fence_barrier_init();
+  }
+  if (warp < 4) {
+    constexpr uint32_t kOne = 0x3F80;   // 1 in bf16
+    st_shared16(pick_lse + tid * 16, kOne | kOne << 16, kOne, 0, 0);
+    st_shared16(pick_delta + tid * 16, 0, 0, kOne | kOne << 16, kOne);
+    st_shared16(zeros + tid * 16, 0, 0, 0, 0);
+    tc::fence_async_smem();
   }
   if (warp == kMmaWarp) tc::tmem_alloc(&tmem_slot, 512);
   tc::fence_before_sync();
@@ -289,10 +337,11 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
             const int st = pos % L::RING;
             if (!wait(&empty[st], (pos / L::RING) + 1)) break;
             uint64_t* bar = ragged ? &raw[st] : &full[st];   // rows of a ragged tile pass through the trimming warp
-            tc::mbar_arrive_expect_tx(bar, L::BYTES + (x == 0 ? 1024 : 0));
+            tc::mbar_arrive_expect_tx(bar, L::BYTES + (x == 0 ? kStatBytes : 0));
             load_tile<DP>(ring + st * L::BYTES, x == 0 ? &args.tm_q : &args.tm_do, hq, row, w.t.b, bar);
             if (x == 0)
-              bulk_load(stat_addr + (st / 2) * 1024, stat_tile(args, hq, query_slot(a, w.t, qt, kRows)), 1024, bar);
+              bulk_load(stat_addr + (st / 2) * kStatBytes, stat_tile(args, hq, query_slot(a, w.t, qt, kRows)) + 2 * kRows,
+                        kStatBytes, bar);
           }
           if (++qt == w.end_tile) { qt = w.first_tile; ++g; }
         }
@@ -342,12 +391,14 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
         tc::fence_after_sync();
         if (leader) {
           mma_rows<DP>(tS, k_addr, ring + st * L::BYTES, id_s);
+          mma_stat(tS, pick_lse, stat_addr + (st >> 1) * kStatBytes, zeros);
           tc::mma_commit(&s_full);
         }
         wait.warp(&full[st + 1], int(phase));
         tc::fence_after_sync();
         if (leader) {
           mma_rows<DP>(tP, v_addr, ring + (st + 1) * L::BYTES, id_s);
+          mma_stat(tP, pick_delta, stat_addr + (st >> 1) * kStatBytes, zeros);
           tc::mma_commit(&dp_full);
           if (total == 1) tc::mma_commit(&kv_empty);
         }
@@ -372,6 +423,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
           tc::fence_after_sync();
           if (leader) {
             mma_rows<DP>(tS, k_addr, ring + next * L::BYTES, id_s);
+            mma_stat(tS, pick_lse, stat_addr + (next >> 1) * kStatBytes, zeros);
             tc::mma_commit(&s_full);
           }
         }
@@ -387,6 +439,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
           tc::fence_after_sync();
           if (leader) {
             mma_rows<DP>(tP, v_addr, ring + (next + 1) * L::BYTES, id_s);
+            mma_stat(tP, pick_delta, stat_addr + (next >> 1) * kStatBytes, zeros);
             tc::mma_commit(&dp_full);
             if (n + 2 == total) tc::mma_commit(&kv_empty);
           }
@@ -402,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
     const int side = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;   // key row, queries 64*side ..
     const uint32_t lanes = uint32_t(quarter * 32) << 16;
     const uint32_t ts = tS + lanes + side * 64, tp = tP + lanes + side * 64;
-    const float2 sl2 = make_float2(a.scale * kLog2e, a.scale * kLog2e), sc2 = make_float2(a.scale, a.scale);
+    const float2 sl2 = make_float2(base2_scale(a), base2_scale(a)), sc2 = make_float2(a.scale, a.scale);
     int tile = 0, used = 0, item = 0;
     DkvItem w = queue.take(item, wait, lane);
     while (w.head >= 0) {
@@ -410,24 +463,16 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
       const int first = first_seeing(a, w.t, j0 + row), whole = first_seeing(a, w.t, j0 + kRows - 1);
       int qt = w.first_tile;
       for (int n = 0; n < w.total; ++n, ++tile) {
-        const int st = (2 * tile) % L::RING;
-        wait.warp(&full[st], (2 * tile) / L::RING);
         wait.warp(&s_full, tile);
         tc::fence_after_sync();
-        const float4* nlse = reinterpret_cast<const float4*>(stat_smem + (st / 2) * 256 + side * 64);
-        const float4* ndel = nlse + kRows / 4;
         float p[64];
         uint32_t x16[32];
         tc::tmem_ld64(ts, p);
 #pragma unroll
-        for (int c = 0; c < 64; c += 4) {
-          const float4 x = nlse[c / 4];
-          const float2 u = ex2_mixed(tc::fma2(make_float2(p[c], p[c + 1]), sl2, make_float2(x.x, x.y)), c / 2, kPolyKv);
-          const float2 v = ex2_mixed(tc::fma2(make_float2(p[c + 2], p[c + 3]), sl2, make_float2(x.z, x.w)), c / 2 + 1, kPolyKv);
+        for (int c = 0; c < 64; c += 2) {
+          const float2 u = ex2_mixed(mul2(make_float2(p[c], p[c + 1]), sl2), c / 2, kPolyKv);
           p[c] = u.x;
           p[c + 1] = u.y;
-          p[c + 2] = v.x;
-          p[c + 3] = v.y;
         }
         const bool edge = qt * kRows < whole || (w.tail < kRows && qt + 1 == w.end_tile);
         if (edge) {
@@ -449,15 +494,10 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
         float dp[64];
         tc::tmem_ld64(tp, dp);
 #pragma unroll
-        for (int c = 0; c < 64; c += 4) {
-          const float4 x = ndel[c / 4];
-          const float2 u = mul2(tc::fma2(make_float2(dp[c], dp[c + 1]), sc2, make_float2(x.x, x.y)), make_float2(p[c], p[c + 1]));
-          const float2 v =
-              mul2(tc::fma2(make_float2(dp[c + 2], dp[c + 3]), sc2, make_float2(x.z, x.w)), make_float2(p[c + 2], p[c + 3]));
+        for (int c = 0; c < 64; c += 2) {
+          const float2 u = mul2(mul2(make_float2(dp[c], dp[c + 1]), sc2), make_float2(p[c], p[c + 1]));
           dp[c] = u.x;
           dp[c + 1] = u.y;
-          dp[c + 2] = v.x;
-          dp[c + 3] = v.y;
         }
         if (edge) {   // without weight no gradient, whatever dP holds there
 #pragma unroll
@@ -774,7 +814,7 @@ int bwd_t(const BwdTcArgs& a, cudaStream_t s) {
 
 int64_t dense_bwd_workspace(bool packed, int64_t B, int64_t T, int64_t N, int64_t Hq, int64_t sequences) {
   const int64_t q = seq_slots(packed, B, T, sequences, kRows), k = seq_slots(packed, B, N, sequences, kRows);
-  return q * Hq * 2 * kRows * int64_t(sizeof(float)) + (q + k) * int64_t(sizeof(SeqTile)) +
+  return q * Hq * kStat * int64_t(sizeof(float)) + (q + k) * int64_t(sizeof(SeqTile)) +
          2 * int64_t(sizeof(int));
 }
 
@@ -785,7 +825,7 @@ int dense_attn_bwd_tc(const DenseAttnArgs& d, int dtype, cudaStream_t stream) {
   a.stats = d.delta;
   a.q_slots = seq_slots(d.cu_q, d.B, d.T, d.sequences, kRows);
   a.k_slots = seq_slots(d.cu_q, d.B, d.N, d.sequences, kRows);
-  a.order = reinterpret_cast<SeqTile*>(d.delta + a.q_slots * d.Hq * 2 * kRows);
+  a.order = reinterpret_cast<SeqTile*>(d.delta + a.q_slots * d.Hq * kStat);
   a.counters = reinterpret_cast<int*>(a.order + a.q_slots + a.k_slots);
   if (a.q_slots * d.Hq >= (int64_t(1) << 31) - 4096 || a.k_slots * d.H >= (int64_t(1) << 31) - 4096) return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
   int rc = dense_tensor_map(&a.tm_q, d.q, dtype, d.B, d.T, d.Hq, d.D, d.q_sb, d.q_st, d.q_sh, kRows);
