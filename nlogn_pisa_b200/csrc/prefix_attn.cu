@@ -9,7 +9,8 @@
 // w = 2^(m - max m).  The prefix is one key range for the query rows of the
 // whole batch, so its keys and values are read once for all of them; own
 // caches are read once each.  This file holds the form on the FMA pipes (fp32
-// tensors and heads wider than 128) and the joining launch.
+// tensors and heads wider than 128) and the joining launch.  Both are bound by
+// HBM; the join's reads (L2 mostly) and its start overlap the launch before it.
 #include "prefix_attn.cuh"
 
 namespace pisa {

@@ -10,6 +10,11 @@
 // same rows and take every other key tile, so that the tensor core still
 // works for one half while the other half's weights are computed, and their
 // results join in shared memory.  Ranges are sized for one wave of CTAs.
+//
+// Measured: 64 tokens of 32 query heads over 8192 shared keys (8 heads of 128):
+// 18 us for 8.6 GFLOP and 34 MB; 16 tokens over 65536: 48 us for 268 MB, 5.5
+// TB/s.  The streaming kernel reads a shared prefix once per 16 query rows: 195
+// us for the first of these, which is why more than 16 rows come here.
 #include "dense_tc.cuh"
 #include "prefix_attn.cuh"
 

@@ -85,6 +85,15 @@ def test_large_and_small_logits(cuda_device, dtype, sizes):
     compare((q.float() * sizes).to(dtype), k, v, normal(gen, 1, 400, 4, 64, dtype=dtype))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("scale", [1e-4, 1e-33])
+def test_small_scales(cuda_device, dtype, scale):
+    """Weights near equal; the kernels may divide statistics by the scale."""
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    q, k, v = normal(gen, 1, 300, 4, 64, dtype=dtype), *(normal(gen, 1, 300, 2, 64, dtype=dtype) for _ in range(2))
+    compare(q, k, v, normal(gen, 1, 300, 4, 64, dtype=dtype), [200, 0, 100], [300, 0, 0], scale=scale)
+
+
 def test_rising_logits(cuda_device):
     """The running maximum grows with every tile of keys."""
     gen = torch.Generator(device="cuda").manual_seed(7)
