@@ -224,6 +224,11 @@ int pisa_prefix_attn(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, co
   a.prefix_splits = int(plan.prefix_splits); a.own_splits = int(plan.own_splits);
   a.prefix_chunk = int(plan.prefix_chunk); a.own_chunk = int(plan.own_chunk);
   a.status = reinterpret_cast<int*>(ws);
+  a.sms = sm_count();
+  if (plan.tiles) {
+    const int64_t tokens = 128 / a.G, tiles = (B * Tq + tokens - 1) / tokens;
+    a.tile_ctas = int(H * ((tiles + 1) / 2));
+  }
   a.part_ml = reinterpret_cast<float2*>(ws + plan.ml_off);
   a.part_o = reinterpret_cast<float*>(ws + plan.o_off);
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -181,13 +181,15 @@ __global__ void prefix_combine_kernel(const __grid_constant__ PrefixArgs a) {
   const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5, lane = threadIdx.x & 31;
   const int slots = a.prefix_splits + a.own_splits;
   const int ranges = (own_length(a, int(row / (int64_t(a.T) * a.Hq))) + a.own_chunk - 1) / a.own_chunk;
-  const int used = a.prefix_splits + max(1, ranges);
   const float2* ml = a.part_ml + row * slots;
   const float* po = a.part_o + row * slots * a.Dv + lane * 4;
   cudaGridDependencySynchronize();   // the partials are complete from here on
+  // slots: the prefix's ranges, then, from prefix_splits on, the own cache's
+  const int shared = a.tile_ctas ? a.status[1] : a.prefix_splits, used = shared + max(1, ranges);
+  auto place = [&](int s) { return s < shared ? s : s - shared + a.prefix_splits; };
   float top = -INFINITY;
   for (int s = lane; s < used; s += 32) {
-    const float2 x = ml[s];
+    const float2 x = ml[place(s)];
     if (x.y != 0.f) top = fmaxf(top, x.x);
   }
   top = warp_max(top);
@@ -195,7 +197,7 @@ __global__ void prefix_combine_kernel(const __grid_constant__ PrefixArgs a) {
   float total = 0.f;
   float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
   for (int s0 = 0; s0 < used; s0 += 32) {
-    const float2 x = s0 + lane < used ? ml[s0 + lane] : make_float2(0.f, 0.f);
+    const float2 x = s0 + lane < used ? ml[place(s0 + lane)] : make_float2(0.f, 0.f);
     const float weight = x.y == 0.f ? 0.f : exp2f(x.x - top);   // of slot s0 + lane
     total = fmaf(weight, x.y, total);
     const uint32_t heavy = __ballot_sync(kFull, x.y != 0.f);
@@ -206,7 +208,7 @@ __global__ void prefix_combine_kernel(const __grid_constant__ PrefixArgs a) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         if (lane * 4 + 128 * c >= a.Dv) continue;
-        const float4 o = __ldcs(reinterpret_cast<const float4*>(po + int64_t(s0 + i) * a.Dv + 128 * c));
+        const float4 o = __ldcs(reinterpret_cast<const float4*>(po + int64_t(place(s0 + i)) * a.Dv + 128 * c));
         acc[c].x = fmaf(w, o.x, acc[c].x);
         acc[c].y = fmaf(w, o.y, acc[c].y);
         acc[c].z = fmaf(w, o.z, acc[c].z);

@@ -29,6 +29,10 @@ struct PrefixArgs {
   float* part_o;                 // [rows][slots][Dv], sum_j 2^(s_j - m) v_j
   float2* part_ml;               // [rows][slots], (m, l) with base-2 logits
   int* status;                   // device status word, cleared by block 0 of the first launch
+  // prefix in 128-row tiles: CTAs of one key range (0: another form, whose
+  // ranges are prefix_splits), multiprocessors; the number of ranges that the
+  // tiles' kernel settled on follows the status word
+  int tile_ctas, sms;
 };
 
 __device__ __forceinline__ int own_length(const PrefixArgs& a, int b) {
@@ -43,6 +47,40 @@ __device__ __forceinline__ int own_length(const PrefixArgs& a, int b) {
 __device__ __forceinline__ void split_range(int keys, int i, int chunk, int& begin, int& end) {
   begin = int(min64(keys, int64_t(i) * chunk));
   end = int(min64(keys, int64_t(i) * chunk + chunk));
+}
+
+// Key ranges of a prefix in 128-row tiles, at most prefix_splits, from the own
+// caches' total length.  Both kernels read at the same rate per multiprocessor,
+// so the prefix takes as many of them as make both end together, and the own
+// caches the rest from the start.  Times in 128-key tiles of a head; a range
+// starts and stores its rows in about 5.  (64 sequences of 1 to 2048 keys over
+// 8192 shared ones, 8 heads of 128: 66 us for the step, 76 with one wave of
+// prefix tiles before the own caches.)
+struct PrefixShare {
+  int ranges, chunk, own_ctas;   // own_ctas: CTAs that read the own caches
+};
+
+__device__ __forceinline__ PrefixShare prefix_share(const PrefixArgs& a, int64_t own_keys) {
+  const float own = float(own_keys) / 128.f * a.H * ((a.T * a.G + 15) / 16), prefix = float(a.P) / 128.f;
+  PrefixShare best{a.prefix_splits, 0, a.sms};
+  float least = prefix / a.prefix_splits + 5.f + own / a.sms;   // one after the other
+  // prefix / r + 5 = own / (sms - r * tile_ctas), solved for r
+  const float c = float(a.tile_ctas), b = 5.f * a.sms - c * prefix - own, root = sqrtf(b * b + 20.f * c * prefix * a.sms);
+  const int at = int(b > 0.f ? (b + root) / (10.f * c) : 2.f * prefix * a.sms / (root - b));
+  for (int i = 0; i < 2; ++i) {
+    const int r = min(max(at + i, 1), a.prefix_splits);
+    const int rest = a.sms - r * a.tile_ctas;
+    if (rest < 1) break;
+    const float time = fmaxf(prefix / r + 5.f, own / rest);
+    if (time < least) {
+      least = time;
+      best.ranges = r;
+      best.own_ctas = rest;
+    }
+  }
+  best.chunk = ((a.P + best.ranges - 1) / best.ranges + 127) / 128 * 128;
+  best.ranges = (a.P + best.chunk - 1) / best.chunk;
+  return best;
 }
 
 // Launches a kernel that may be scheduled while the stream's previous kernel

@@ -28,9 +28,10 @@
 // tokens see are added row by row.
 //
 // Measured: 64 sequences over caches of 1 to 2048 keys (8 heads of 128, 240 MB)
-// beside a shared prefix of 8192: 76 us for the whole step, of which the caches
-// stream at 4.9 TB/s; 16 sequences of 5 to 4096 keys beside 65536 shared ones:
-// 91 us.  One sequence of 700 keys: 4.4 us and 3.9 us for the join.
+// beside a shared prefix of 8192: 57 us on the SMs that the prefix leaves, 66 us
+// for the whole step; 16 sequences of 5 to 4096 keys beside 65536 shared ones: 73
+// and 90 us (5.7 TB/s for both kernels together).  The caches alone stream at 4.9
+// TB/s.  One sequence of 700 keys: 4.4 us and 3.9 us for the join.
 #include "dense_tc.cuh"
 #include "prefix_attn.cuh"
 
@@ -151,6 +152,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_stream_kernel(const __grid
   float2* sml = reinterpret_cast<float2*>(so + kComputeWarps * BR * (DP + 4));                              // [warps][BR]
   __shared__ uint64_t full[L::STAGES], empty[L::STAGES];
   __shared__ int table[kTable + 1];
+  __shared__ int ctas;                         // that take items: the others find the prefix's tiles on their SM
   __shared__ int s_fail;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   cudaTriggerProgrammaticLaunchCompletion();   // the joining launch may be scheduled
@@ -161,11 +163,15 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_stream_kernel(const __grid
   const int entries = (a.B + args.per_entry - 1) / args.per_entry;
   if (warp == 0) {
     int sum = 0;
+    int64_t keys = 0;
     for (int e0 = 0; e0 < entries; e0 += 32) {
       const int e = e0 + lane;
       int n = 0;
       if (e < entries)
-        for (int b = e * args.per_entry; b < min(a.B, (e + 1) * args.per_entry); ++b) n += own_ranges(a, b);
+        for (int b = e * args.per_entry; b < min(a.B, (e + 1) * args.per_entry); ++b) {
+          n += own_ranges(a, b);
+          keys += own_length(a, b);
+        }
       int up = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -175,7 +181,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_stream_kernel(const __grid
       if (e < entries) table[e] = sum + up - n;
       sum += __shfl_sync(kFull, up, 31);
     }
-    if (lane == 0) table[entries] = sum;
+    for (int o = 16; o > 0; o >>= 1) keys += __shfl_xor_sync(kFull, keys, o);
+    if (lane == 0) {
+      table[entries] = sum;
+      ctas = args.after_tiles ? min(int(gridDim.x), prefix_share(a, keys).own_ctas) : int(gridDim.x);
+    }
   } else if (tid == 32) {
     for (int i = 0; i < L::STAGES; ++i) {
       tc::mbar_init(&full[i], 1);
@@ -185,13 +195,13 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_stream_kernel(const __grid
     tc::fence_barrier_init();
   }
   __syncthreads();
-  const int items = args.prefix_items + table[entries] * args.own_blocks * a.H;
+  const int items = int(blockIdx.x) < ctas ? args.prefix_items + table[entries] * args.own_blocks * a.H : 0;
 
   if (warp == kLoadWarp) {
     if (lane == 0) {
       int n = 0;   // tiles issued so far
       bool ok = true;
-      for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
+      for (int i = blockIdx.x; i < items && ok; i += ctas) {
         const Item x = item_at(args, table, i);
         const CUtensorMap* mk = x.prefix ? &args.tm_pk : &args.tm_k;
         const CUtensorMap* mv = x.prefix ? &args.tm_pv : &args.tm_v;
@@ -217,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_stream_kernel(const __grid
     const int slots = a.prefix_splits + a.own_splits;
     bool ok = true;
     int n = 0;   // tiles of the items before
-    for (int i = blockIdx.x; i < items; i += gridDim.x) {
+    for (int i = blockIdx.x; i < items; i += ctas) {
       const Item x = item_at(args, table, i);
       const int rows = (x.prefix ? a.B * a.T : a.T) * a.G, r0 = x.block * BR;
       const int shared = x.prefix ? x.length : x.length - a.T + 1;   // keys before this one are seen by every row

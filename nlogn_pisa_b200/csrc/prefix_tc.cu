@@ -9,11 +9,13 @@
 // more, its two tiles share the stream of keys; with one, both halves hold the
 // same rows and take every other key tile, so that the tensor core still
 // works for one half while the other half's weights are computed, and their
-// results join in shared memory.  Ranges are sized for one wave of CTAs.
+// results join in shared memory.  The number of ranges follows from the own
+// caches' lengths (prefix_share): CTAs without a range leave at once.
 //
 // Measured: 64 tokens of 32 query heads over 8192 shared keys (8 heads of 128):
-// 18 us for 8.6 GFLOP and 34 MB; 16 tokens over 65536: 48 us for 268 MB, 5.5
-// TB/s.  The streaming kernel reads a shared prefix once per 16 query rows: 195
+// 18 us with all SMs for 8.6 GFLOP and 34 MB, 53 us on the few that end with the
+// own caches' stream; 16 tokens over 65536: 48 us for 268 MB (5.5 TB/s) with all,
+// 70 us beside the stream.  The streaming kernel reads a shared prefix once per 16 query rows: 195
 // us for the first of these, which is why more than 16 rows come here.
 #include "dense_tc.cuh"
 #include "prefix_attn.cuh"
@@ -54,6 +56,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
   float* join = reinterpret_cast<float*>(smem_raw + (kv_addr - tc::smem_u32(smem_raw)));   // [128][DP + 4], after the ring's use
   __shared__ uint64_t q_full[2], kv_full[L::STAGES], kv_empty[L::STAGES], s_full[2], p_full[2], o_done[2], drained;
   __shared__ float2 join_ml[kRows];
+  __shared__ int64_t s_own[kThreads / 32];
   __shared__ uint32_t tmem_slot;
   __shared__ int s_fail;
   const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
@@ -61,9 +64,19 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
   // half a second before any wait can expire
   if (blockIdx.x + blockIdx.y + tid == 0) *a.status = PISA_OK;
   const int h = blockIdx.x % a.H, split = blockIdx.x / a.H;
+  int64_t own = 0;
+  for (int b0 = 0; b0 < a.B; b0 += kThreads) own += b0 + tid < a.B ? own_length(a, b0 + tid) : 0;
+  for (int o = 16; o > 0; o >>= 1) own += __shfl_xor_sync(kFull, own, o);
+  if (lane == 0) s_own[warp] = own;
+  __syncthreads();
+  own = 0;
+  for (int w = 0; w < kThreads / 32; ++w) own += s_own[w];
+  const PrefixShare share = prefix_share(a, own);
+  if (blockIdx.x + blockIdx.y + tid == 0) a.status[1] = share.ranges;
+  if (split >= share.ranges) return;
   const bool dual = args.tiles == 1;            // one row tile: the halves take every other key tile
   int begin, end;
-  split_range(a.P, split, a.prefix_chunk, begin, end);
+  split_range(a.P, split, share.chunk, begin, end);
   const int keys = (end - begin + kRows - 1) / kRows;      // key tiles, at least one
   const int row_tile[2] = {dual ? 0 : int(blockIdx.y) * 2, dual ? 0 : int(blockIdx.y) * 2 + 1};
   const int steps[2] = {dual ? (keys + 1) / 2 : keys, dual ? keys / 2 : row_tile[1] < args.tiles ? keys : 0};

@@ -62,6 +62,19 @@ def test_shared_prefix(cuda_device, dtype, heads, kv_heads, dim, batch, new, pre
     compare(q, k, v, lengths, pk, pv)
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 8, 64), (8, 1, 128), (160, 160, 64)])
+@pytest.mark.parametrize("prefix,capacity,lengths", [(129, 3000, [3000] * 17), (6000, 300, [0] * 20), (6000, 300, [1] * 300),
+                                                     (2500, 2500, [2500, 0, 1] * 8)])
+def test_prefix_and_caches_share_the_device(cuda_device, heads, kv_heads, dim, prefix, capacity, lengths):
+    """From all the work in the caches to all of it in the prefix, whose key ranges follow from the lengths."""
+    gen = torch.Generator(device="cuda").manual_seed(prefix + heads)
+    if heads * len(lengths) > 3000:
+        lengths = lengths[:18]
+    batch = len(lengths)
+    q, k, v = normal(gen, batch, 1, heads, dim), *(normal(gen, batch, capacity, kv_heads, dim) for _ in range(2))
+    compare(q, k, v, lengths, *(normal(gen, prefix, kv_heads, dim) for _ in range(2)))
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_lengths_are_clamped_and_empty_rows_are_zero(cuda_device, dtype):
     gen = torch.Generator(device="cuda").manual_seed(3)
