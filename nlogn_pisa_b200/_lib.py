@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+from functools import lru_cache
 from pathlib import Path
 
 import torch
@@ -152,6 +153,13 @@ def stream_of(device):
 # the current stream as an integer, without building a Stream object per call
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+@lru_cache(maxsize=4096)
+def workspace_bytes(name, device_index, *shape):
+    """Size of a call's workspace, a function of shapes and the device's multiprocessors."""
+    with torch.cuda.device(device_index):
+        return getattr(lib(), name)(*shape)
 
 
 def launch(fn, device_index, *args):

@@ -9,8 +9,6 @@ that all sequences share, through pisa_prefix_attn.
 
 from __future__ import annotations
 
-from contextlib import nullcontext
-
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -105,8 +103,9 @@ def _backward(q, k, v, out, low, dout, lse, cu_q, cu_k, offset, scale, causal):
     _, length, heads, dim_v = v.shape
     library, code, packing = _lib.lib(), _lib.DTYPES[q.dtype], _packing(cu_q, cu_k)
     dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
-    size = library.pisa_full_attn_bwd_workspace_bytes(batch, tokens, q_heads, heads, dim, dim_v, length, packing[3], code)
-    workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+    size = _lib.workspace_bytes("pisa_full_attn_bwd_workspace_bytes", q.get_device(), batch, tokens, q_heads, heads, dim,
+                                dim_v, length, packing[3], code)
+    workspace = q.new_empty(size, dtype=torch.uint8)
     _lib.launch(library.pisa_full_attn_bwd, q.get_device(), *view(q), *view(k), *view(v), out.data_ptr(),
                 None if low is None else low.data_ptr(), dout.data_ptr(), lse.data_ptr(), *packing, offset, code, batch,
                 tokens, q_heads, heads, dim, dim_v, length, scale, int(causal), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
@@ -202,7 +201,7 @@ def prefix_attention(q, k, v, lengths, prefix_k=None, prefix_v=None, scale=None,
         raise ValueError("prefix_k and prefix_v come together")
     scale = dim ** -0.5 if scale is None else float(scale)
     lengths = lengths.contiguous()
-    q, k, v = aligned_rows(q.detach()), aligned_rows(k.detach()), aligned_rows(v.detach())
+    q, k, v = aligned_rows(q), aligned_rows(k), aligned_rows(v)   # read through their pointers: no graph follows
     if batch > 1 and tokens > 1 and q.stride(0) != tokens * q.stride(1):
         q = q.contiguous()
     prefix, shared = 0, (None, 0, 0, None, 0, 0)
@@ -216,16 +215,15 @@ def prefix_attention(q, k, v, lengths, prefix_k=None, prefix_v=None, scale=None,
             shared = (prefix_k.data_ptr(), *prefix_k.stride()[:2], prefix_v.data_ptr(), *prefix_v.stride()[:2])
     out = q.new_empty((batch, tokens, q_heads, dim_v))
     lse = q.new_empty((batch, tokens, q_heads), dtype=torch.float32) if return_lse else None
-    library, code = _lib.lib(), _lib.DTYPES[q.dtype]
-    # the key ranges, and so the size, are planned for the current device
-    with torch.cuda.device(device) if torch.cuda.current_device() != device else nullcontext():
-        size = library.pisa_prefix_attn_workspace_bytes(batch, tokens, q_heads, heads, dim, dim_v, capacity, prefix, code)
-        if size < 0:
-            raise ValueError("shapes outside the envelope of prefix_attention")
-        workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
-        _lib.launch(library.pisa_prefix_attn, device, *view(q), *view(k), *view(v), lengths.data_ptr(),
-                    lengths.element_size(), *shared, code, batch, tokens, q_heads, heads, dim, dim_v, capacity, prefix, scale,
-                    out.data_ptr(), None if lse is None else lse.data_ptr(), workspace.data_ptr(), size)
+    code = _lib.DTYPES[q.dtype]
+    size = _lib.workspace_bytes("pisa_prefix_attn_workspace_bytes", device, batch, tokens, q_heads, heads, dim, dim_v,
+                                capacity, prefix, code)
+    if size < 0:
+        raise ValueError("shapes outside the envelope of prefix_attention")
+    workspace = q.new_empty(size, dtype=torch.uint8)
+    _lib.launch(_lib.lib().pisa_prefix_attn, device, *view(q), *view(k), *view(v), lengths.data_ptr(),
+                lengths.element_size(), *shared, code, batch, tokens, q_heads, heads, dim, dim_v, capacity, prefix, scale,
+                out.data_ptr(), None if lse is None else lse.data_ptr(), workspace.data_ptr(), size)
     if _lib.status_checks():
         _lib.check_workspace(workspace, q.device)
     return (out, lse) if return_lse else out

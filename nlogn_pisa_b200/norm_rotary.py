@@ -49,13 +49,12 @@ class QkNormRotaryFunction(torch.autograd.Function):
         dq_out, dk_out = flat(dq_out), flat(dk_out)
         dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
         dq_weight, dk_weight = torch.empty_like(q_weight), torch.empty_like(k_weight)
-        library = _lib.lib()
-        with torch.cuda.device(q.device):   # the size depends on the device's multiprocessors
-            size = library.pisa_qk_norm_rotary_bwd_workspace_bytes(q.shape[0], q.shape[1], q.shape[3])
-            workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
-            _lib.launch(library.pisa_qk_norm_rotary_bwd, q.get_device(), *view(q), *view(k), dq_out.data_ptr(),
-                        dk_out.data_ptr(), *_operands(q, k, q_weight, k_weight, frequency, positions, position_offset), eps,
-                        dq.data_ptr(), dk.data_ptr(), dq_weight.data_ptr(), dk_weight.data_ptr(), workspace.data_ptr(), size)
+        size = _lib.workspace_bytes("pisa_qk_norm_rotary_bwd_workspace_bytes", q.get_device(), q.shape[0], q.shape[1],
+                                    q.shape[3])
+        workspace = q.new_empty(size, dtype=torch.uint8)
+        _lib.launch(_lib.lib().pisa_qk_norm_rotary_bwd, q.get_device(), *view(q), *view(k), dq_out.data_ptr(),
+                    dk_out.data_ptr(), *_operands(q, k, q_weight, k_weight, frequency, positions, position_offset), eps,
+                    dq.data_ptr(), dk.data_ptr(), dq_weight.data_ptr(), dk_weight.data_ptr(), workspace.data_ptr(), size)
         return dq, dk, dq_weight, dk_weight, None, None, None, None
 
 
@@ -75,11 +74,11 @@ def qk_norm_rotary(q, k, q_weight, k_weight, frequency, positions=None, position
         raise ValueError("q and k must share batch, tokens and head dimension")
     if 0 in a or 0 in b:
         raise ValueError("nonempty tensors are required")
-    if q.dtype != k.dtype or q.device != k.device or not q.is_floating_point():
+    if q.dtype != k.dtype or q.get_device() != k.get_device() or not q.is_floating_point():
         raise ValueError("q and k must share a floating dtype and device")
     dim = a[3]
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w.dim() != 1 or w.shape[0] != dim or w.dtype not in (torch.float32, q.dtype) or w.device != q.device:
+        if w.dim() != 1 or w.shape[0] != dim or w.dtype not in (torch.float32, q.dtype) or w.get_device() != q.get_device():
             raise ValueError(f"{name} must have head_dim elements in fp32 or q's dtype on q's device")
     if q_weight.dtype != k_weight.dtype:
         raise ValueError("q_weight and k_weight must share a dtype")
@@ -90,12 +89,16 @@ def qk_norm_rotary(q, k, q_weight, k_weight, frequency, positions=None, position
         raise ValueError("positions must be integers of shape [1 or B, T]")
     require_cuda(q)
     _lib.dtype_code(q)
-    frequency = frequency.to(device=q.device, dtype=torch.float32).contiguous()
+    if frequency.dtype != torch.float32 or frequency.get_device() != q.get_device():
+        frequency = frequency.to(device=q.device, dtype=torch.float32)
+    frequency = frequency.contiguous()
     if positions is not None:
-        positions = positions.to(device=q.device, dtype=torch.int64).contiguous()
+        if positions.dtype != torch.int64 or positions.get_device() != q.get_device():
+            positions = positions.to(device=q.device, dtype=torch.int64)
+        positions = positions.contiguous()
     q, k = aligned_rows(q), aligned_rows(k)
     q_weight, k_weight = q_weight.contiguous(), k_weight.contiguous()
     args = (q, k, q_weight, k_weight, frequency, positions, int(position_offset), float(eps))
-    if any(t.requires_grad for t in args[:4]) and torch.is_grad_enabled():
+    if (q.requires_grad or k.requires_grad or q_weight.requires_grad or k_weight.requires_grad) and torch.is_grad_enabled():
         return QkNormRotaryFunction.apply(*args)
     return _forward(*args)
