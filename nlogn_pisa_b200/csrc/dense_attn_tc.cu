@@ -28,9 +28,11 @@
 // fp32.
 //
 // Hidden keys of a tile weigh zero, but zero times an infinite or NaN value
-// is NaN.  A row whose output holds NaN although its weights do not is
-// therefore summed again over its visible keys alone (row_again); rows past
-// the sequence's end need nothing (they are not stored).
+// is NaN.  Only the last key tiles of an item (at most three) hide keys from
+// any of its rows.  Their values pass through warp 18, which zeroes rows that
+// are not finite before the products read them and lists those that some row
+// of the item may see; the rows that do add them again in fp32 when they are
+// stored.  That is at most 256 keys per row, whatever the length.
 //
 // Measured: one prompt of 16384, 32 query and 8 key heads of 128: 1685 us, 1305
 // TFLOP/s; a training block of four sequences of 4096, 16 heads of 64: 204 us,
@@ -48,6 +50,7 @@ namespace {
 
 constexpr int kSoftWarps = 16, kMmaWarp = 16, kLoadWarp = 17, kPlanWarp = 18;
 constexpr int kThreads = 608;
+constexpr int kListWords = 3 * kRows / 32;   // the key tiles of an item that hide keys: three at most
 
 struct FwdTcArgs {
   CUtensorMap tm_q, tm_k, tm_v;             // boxes of 64 dims x 128 rows of one head
@@ -77,43 +80,40 @@ __device__ __forceinline__ void store16(T* p, const uint32_t (&r)[8], int left) 
   }
 }
 
-// Output row of query `i` summed over its visible keys alone, by one warp,
-// with the row's maximum m and weight sum l (base 2): acc[e] of column
-// lane + 32 e.  Stops once every column is NaN.
-template <typename T, int DP>
-__device__ __noinline__ void row_again(const DenseAttnArgs& a, const SeqTile& t, int hq, int i, float m, float l,
-                                       float (&acc)[DP / 32]) {
-  const int lane = threadIdx.x & 31, h = hq / a.G;
+// Adds the listed values to 16 columns (from `col`) of this thread's row: those
+// of query `i`, with the row's maximum m (base 2), over the listed keys that it
+// sees.  Bit b of list[w] is key first + 32 w + b.
+template <typename T>
+__device__ __noinline__ void add_listed(const DenseAttnArgs& a, const SeqTile& t, int hq, int i, float m, const uint32_t* list,
+                                        int first, int col, float (&o)[16]) {
+  const int h = hq / a.G, last = last_visible(a, t, i);
   const T* qp = static_cast<const T*>(a.q) + t.b * a.q_sb + int64_t(t.q_begin + i) * a.q_st + hq * a.q_sh;
   const T* kp = static_cast<const T*>(a.k) + t.b * a.k_sb + int64_t(t.k_begin) * a.k_st + h * a.k_sh;
   const T* vp = static_cast<const T*>(a.v) + t.b * a.v_sb + int64_t(t.k_begin) * a.v_st + h * a.v_sh;
   const float sl = a.scale * kLog2e;
-  float q[DP / 32];
+  for (int w = 0; w < kListWords; ++w) {
+    for (uint32_t left = list[w]; left; left &= left - 1) {
+      const int j = first + 32 * w + __ffs(left) - 1;
+      if (j > last) continue;
+      float s = 0.f;
+      for (int d = 0; d < a.D; d += 8) {
+        float x[8], y[8];
+        load_vec<T>(qp + d, x);
+        load_vec<T>(kp + j * a.k_st + d, y);
 #pragma unroll
-  for (int e = 0; e < DP / 32; ++e) {
-    q[e] = lane + 32 * e < a.D ? to_f32<T>(qp[lane + 32 * e]) : 0.f;
-    acc[e] = 0.f;
-  }
-  const int last = last_visible(a, t, i);
-  for (int j = 0; j <= last; ++j) {
-    float s = 0.f;
+        for (int e = 0; e < 8; ++e) s = fmaf(x[e], y[e], s);
+      }
+      const float p = exp2f(fmaf(s, sl, -m));
 #pragma unroll
-    for (int e = 0; e < DP / 32; ++e)
-      if (lane + 32 * e < a.D) s = fmaf(q[e], to_f32<T>(kp[j * a.k_st + lane + 32 * e]), s);
-    const float p = exp2f(fmaf(warp_sum(s), sl, -m));
-    bool all = true;
+      for (int c = 0; c < 16; c += 8) {
+        if (col + c >= a.Dv) continue;
+        float v[8];
+        load_vec<T>(vp + j * a.v_st + col + c, v);
 #pragma unroll
-    for (int e = 0; e < DP / 32; ++e) {
-      if (lane + 32 * e < a.Dv) {
-        acc[e] = fmaf(p, to_f32<T>(vp[j * a.v_st + lane + 32 * e]), acc[e]);
-        all = all && isnan(acc[e]);
+        for (int e = 0; e < 8; ++e) o[c + e] = fmaf(p, v[e], o[c + e]);
       }
     }
-    if (__all_sync(kFull, all)) break;
   }
-  const float inv = 1.f / l;
-#pragma unroll
-  for (int e = 0; e < DP / 32; ++e) acc[e] *= inv;
 }
 
 // One work item: the pair of query tiles of one head.  The scheduler warp hands
@@ -122,7 +122,56 @@ struct Work {
   SeqTile t;
   int hq;        // -1: no more work
   int tiles[2];  // key tiles that each query tile visits
+  int seen[2];   // keys that every row of each query tile sees
+  __device__ __forceinline__ int most() const { return max(tiles[0], tiles[1]); }
+  // keys that every row of the query tiles that visit key tile j sees
+  __device__ __forceinline__ int seen_by_all(int j) const { return tiles[0] > j ? seen[0] : seen[1]; }
+  __device__ __forceinline__ bool hides(int j) const { return seen_by_all(j) < (j + 1) * kRows; }
+  // the first key tile that hides keys; those from `most` on are not visited
+  __device__ __forceinline__ int first_hiding() const { return seen_by_all(0) / kRows; }
 };
+
+// Does one of the 16-byte words of 16-bit elements hold an infinity or a NaN?
+// Zero times such an element is NaN and stays in the sum.
+template <typename T> struct Wild {
+  using T2 = std::conditional_t<std::is_same<T, __nv_bfloat16>::value, __nv_bfloat162, __half2>;
+  T2 sum;
+  __device__ __forceinline__ Wild() { *reinterpret_cast<uint32_t*>(&sum) = 0; }
+  __device__ __forceinline__ void add(const uint4& v) {
+    T2 zero;
+    *reinterpret_cast<uint32_t*>(&zero) = 0;
+    const T2* x = reinterpret_cast<const T2*>(&v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum = __hfma2(x[e], zero, sum);
+  }
+  __device__ __forceinline__ bool any() const { return isnan(to_f32<T>(sum.x)) || isnan(to_f32<T>(sum.y)); }
+};
+
+// Rows [first, 128) of a value tile ([DP/64][128 rows][128 B]) that hold an
+// infinity or a NaN become zeros; those before `real` are marked in list
+// (128 bits).  One warp; true if a row was changed.
+template <typename T, int DP>
+__device__ __forceinline__ bool silence(uint32_t tile, int first, int real, uint32_t* list, int lane) {
+  Wild<T> wild;
+#pragma unroll 1
+  for (int c = 0; c < DP / 64; ++c) {
+#pragma unroll 8
+    for (int r = first & ~3; r < kRows; r += 4)
+      wild.add(ld_shared16(tile + c * kRows * 128 + (r + lane / 8) * 128 + lane % 8 * 16));
+  }
+  if (!__any_sync(kFull, wild.any())) return false;
+  bool changed = false;
+  for (int r = first; r < kRows; ++r) {
+    const uint32_t at = tile + lane / 8 * kRows * 128 + r * 128 + lane % 8 * 16;
+    Wild<T> row;
+    if (lane < DP / 8) row.add(ld_shared16(at));
+    if (!__any_sync(kFull, row.any())) continue;
+    if (lane < DP / 8) st_shared16(at, 0, 0, 0, 0);
+    if (lane == 0 && r < real) list[r / 32] |= 1u << (r % 32);
+    changed = true;
+  }
+  return changed;
+}
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_constant__ FwdTcArgs args) {
@@ -132,8 +181,11 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
   const uint32_t base = (tc::smem_u32(smem_raw) + 1023) & ~1023u;
   const uint32_t q_addr = base, kv_addr = base + 2 * L::BYTES;
   __shared__ uint64_t w_full[2], w_empty[2], q_full[2], q_empty[2], kv_full[L::STAGES], kv_empty[L::STAGES];
+  __shared__ uint64_t kv_raw[L::STAGES], checked[2];   // values that hide keys, before their check; an item's checks
   __shared__ uint64_t s_full[2], p_full[2], o_done[2], o_free[2], drained;
   __shared__ float s_other[2][2][kRows];      // the halves' maxima, at the end their sums
+  __shared__ uint32_t s_list[2][kListWords];  // an item's keys with values that are not finite, from its first hiding tile on
+  __shared__ int s_listed[2];
   __shared__ Work s_work[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int s_fail;
@@ -148,9 +200,11 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
       tc::mbar_init(&p_full[i], kSoftWarps / 2);
       tc::mbar_init(&o_done[i], 1);
       tc::mbar_init(&o_free[i], kSoftWarps / 2);
+      tc::mbar_init(&checked[i], 1);
     }
     for (int i = 0; i < L::STAGES; ++i) {
       tc::mbar_init(&kv_full[i], 1);
+      tc::mbar_init(&kv_raw[i], 1);
       tc::mbar_init(&kv_empty[i], 1);
     }
     tc::mbar_init(&drained, 1);
@@ -178,7 +232,36 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
   if (warp == kPlanWarp) {
     const int slots = args.items / a.Hq;
     const bool ranked = a.cu_q != nullptr && a.sequences < kRanked;
-    int n = 0;
+    int n = 0, loads = 0;                      // items; ring positions of the items that were checked
+    uint32_t uses = 0;                         // parity of the unchecked loads that each ring slot has held
+    Work before;                               // the item before
+    before.hq = -1;
+    // the values of item n's tiles that hide keys
+    auto check = [&](const Work& w, int slot) {
+      if (lane < kListWords) s_list[slot][lane] = 0;
+      __syncwarp();
+      bool listed = false;
+      const int from = w.first_hiding(), most = w.most();
+      for (int j = from; j < most; ++j) {
+        if (!w.hides(j)) continue;
+        const int st = (loads + j + 1) % L::STAGES;
+        ok = wait_phase(&kv_raw[st], int(uses >> st), &s_fail) && ok;
+        uses ^= 1u << st;
+        if (!__all_sync(kFull, ok)) return;
+        if (silence<T, DP>(kv_addr + st * 2 * L::BYTES, max(0, w.seen_by_all(j) - j * kRows), w.t.k_len - j * kRows,
+                           s_list[slot] + (j - from) * (kRows / 32), lane)) {
+          listed = true;
+          tc::fence_async_smem();
+        }
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&kv_full[st]);
+      }
+      if (most > 0) loads += most + 1;
+      if (lane == 0) {
+        s_listed[slot] = listed;
+        tc::mbar_arrive(&checked[slot]);
+      }
+    };
     for (int round = 0;; ++round) {
       // items are in falling order of their work: every other round goes
       // backwards, or the first CTA would draw the longest of every round
@@ -198,6 +281,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
         for (int i = 0; i < 2; ++i) {
           const int first = q0 + i * kRows, rows = min(kRows, w.t.q_len - first);
           w.tiles[i] = rows > 0 ? (last_visible(a, w.t, first + rows - 1) + kRows) / kRows : 0;
+          w.seen[i] = last_visible(a, w.t, first) + 1;
         }
       }
       ok = wait_phase(&w_empty[n & 1], (n >> 1) + 1, &s_fail) && ok;
@@ -207,18 +291,21 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
         tc::mbar_arrive(&w_full[n & 1]);
       }
       __syncwarp();
+      // the next item is known by now: its loads follow those that wait here
+      if (before.hq >= 0 && __all_sync(kFull, ok)) check(before, (n & 1) ^ 1);
       if (w.hq < 0) break;
+      before = w;
       ++n;
     }
   } else if (warp == kLoadWarp) {
     int st = 0, uses[2] = {0, 0};              // ring slot; items that used each query tile
-    uint32_t phase = 0;
+    uint32_t phase = 0, raw = 0, raws = 0;     // bit st: the last load of slot st is unchecked; parity of those
     int loads = 0;
     for (int n = 0;; ++n) {
       const Work w = take(n);
       if (w.hq < 0) break;
       if (lane == 0) {
-        const int h = w.hq / a.G, most = max(w.tiles[0], w.tiles[1]);
+        const int h = w.hq / a.G, most = w.most();
 #pragma unroll 1
         for (int j = 0; j <= most && most > 0 && ok; ++j) {   // V_{j-1} and K_j; the queries before K_0
           if (j == 0) {
@@ -237,13 +324,15 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
           ok = ok && wait_phase(&kv_empty[st], int(phase) + 1, &s_fail);
           if (!ok) break;
           const uint32_t v = kv_addr + st * 2 * L::BYTES, k = v + L::BYTES;
-          tc::mbar_arrive_expect_tx(&kv_full[st], (int(j > 0) + int(j < most)) * L::BYTES);
+          const bool unchecked = j > 0 && w.hides(j - 1);
+          uint64_t* bar = unchecked ? &kv_raw[st] : &kv_full[st];
+          raw = (raw & ~(1u << st)) | uint32_t(unchecked) << st;
+          raws ^= uint32_t(unchecked) << st;
+          tc::mbar_arrive_expect_tx(bar, (int(j > 0) + int(j < most)) * L::BYTES);
 #pragma unroll 1
           for (int c = 0; c < L::CH; ++c) {
-            if (j < most)
-              tc::tma_load_4d(k + c * kRows * 128, &args.tm_k, c * 64, h, w.t.k_begin + j * kRows, w.t.b, &kv_full[st]);
-            if (j > 0)
-              tc::tma_load_4d(v + c * kRows * 128, &args.tm_v, c * 64, h, w.t.k_begin + (j - 1) * kRows, w.t.b, &kv_full[st]);
+            if (j < most) tc::tma_load_4d(k + c * kRows * 128, &args.tm_k, c * 64, h, w.t.k_begin + j * kRows, w.t.b, bar);
+            if (j > 0) tc::tma_load_4d(v + c * kRows * 128, &args.tm_v, c * 64, h, w.t.k_begin + (j - 1) * kRows, w.t.b, bar);
           }
           ++loads;
           if (++st == L::STAGES) {
@@ -257,8 +346,11 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
     if (lane == 0) {
       // nothing may arrive after the CTA's end: every stage and query tile has
       // been handed back (after an expired wait: the copies in flight have landed)
-      for (int x = max(0, loads - L::STAGES); x < loads; ++x)
-        wait_phase(ok ? &kv_empty[x % L::STAGES] : &kv_full[x % L::STAGES], x / L::STAGES, &s_fail);
+      for (int x = max(0, loads - L::STAGES); x < loads; ++x) {
+        const int y = x % L::STAGES;
+        if (!ok && (raw >> y & 1)) wait_phase(&kv_raw[y], int(raws >> y & 1) + 1, &s_fail);
+        else wait_phase(ok ? &kv_empty[y] : &kv_full[y], x / L::STAGES, &s_fail);
+      }
       for (int i = 0; i < 2; ++i)
         if (uses[i]) wait_phase(ok ? &q_empty[i] : &q_full[i], uses[i] - 1, &s_fail);
     }
@@ -279,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
     for (int n = 0;; ++n) {
       const Work w = take(n);
       if (w.hq < 0) break;
-      const int most = max(w.tiles[0], w.tiles[1]);
+      const int most = w.most();
       if (most == 0) continue;
       ok = wait_phase(&kv_full[st], int(phase), &s_fail) && ok;   // K_0
 #pragma unroll 1
@@ -369,16 +461,18 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
         tc::named_sync(1 + i, 256);
         l += s_other[i][half ^ 1][row];
       }
+      ok = wait_phase(&checked[n & 1], n >> 1, &s_fail) && ok;
+      const bool listed = s_listed[n & 1];
       const SeqTile t = w.t;
       const int hq = w.hq, qi = (t.tile * 2 + i) * kRows + row;   // query of this thread
+      const int list_first = listed ? w.first_hiding() * kRows : 0;
       const bool real = qi < t.q_len;
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&w_empty[n & 1]);
+      if (lane == 0 && !listed) tc::mbar_arrive(&w_empty[n & 1]);   // a list is handed back after its use
       // O / l, stored by each thread for its half of the row (128 or 64
       // consecutive bytes); pass 1 stores what the rounding dropped
       const float inv = !ok ? NAN : l == 0.f ? 0.f : 1.f / l;
       const int64_t at = (int64_t(t.b) * a.T + t.q_begin + qi) * a.Hq + hq;
-      bool wild = false;
 #pragma unroll 1
       for (int c = 0; c < W; c += 16) {
         float o[16];
@@ -388,10 +482,18 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[e] = 0.f;
         }
+        if (listed && real && l != 0.f) {
+          float x[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[e] = o[e];
+          add_listed<T>(a, t, hq, qi, m, s_list[n & 1], list_first, half * W + c, x);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[e] = x[e];
+        }
+        __syncwarp();
         uint32_t r[8], d[8];
 #pragma unroll
         for (int e = 0; e < 16; e += 2) {
-          wild = wild || isnan(o[e]) || isnan(o[e + 1]);
           const float x = l == 0.f && ok ? 0.f : o[e] * inv, y = l == 0.f && ok ? 0.f : o[e + 1] * inv;
           r[e / 2] = pack2<T>(x, y);
           d[e / 2] = pack2<T>(x - to_f32<T>(from_f32<T>(x)), y - to_f32<T>(from_f32<T>(y)));
@@ -407,24 +509,9 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&o_free[i]);
       }
-      __syncwarp();   // the rows' own stores come first
-      uint32_t again = __ballot_sync(kFull, ok && real && wild && l != 0.f && !isnan(l));
-      while (again) {
-        const int r = __ffs(again) - 1;
-        again &= again - 1;
-        float acc[DP / 32];
-        row_again<T, DP>(a, t, hq, qi - lane + r, __shfl_sync(kFull, m, r), __shfl_sync(kFull, l, r), acc);
-        const int64_t row_at = __shfl_sync(kFull, at, r) * a.Dv;
-#pragma unroll
-        for (int e = 0; e < DP / 32; ++e) {
-          const int d = lane + 32 * e;
-          const T v = from_f32<T>(acc[e]);
-          if (d >= half * W && d < half * W + W && d < a.Dv) {
-            static_cast<T*>(a.out)[row_at + d] = v;
-            if (a.out_low) static_cast<T*>(a.out_low)[row_at + d] = from_f32<T>(acc[e] - to_f32<T>(v));
-          }
-        }
+      if (listed) {
         __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&w_empty[n & 1]);
       }
       if (a.lse && real && half == 0) a.lse[at] = !ok ? NAN : l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
     }
