@@ -257,7 +257,7 @@ inline int dense_tensor_map(CUtensorMap* map, const void* base, int dtype, int64
 bool dense_attn_tc_eligible(const DenseAttnArgs& a, int dtype);
 int dense_attn_fwd_tc(const DenseAttnArgs& a, int dtype, cudaStream_t stream);
 // a.delta: dense_bwd_workspace(...) bytes
-int64_t dense_bwd_workspace(bool packed, int64_t B, int64_t T, int64_t N, int64_t Hq, int64_t sequences);
+int64_t dense_bwd_workspace(bool packed, int dtype, int64_t B, int64_t T, int64_t N, int64_t Hq, int64_t H, int64_t sequences);
 int dense_attn_bwd_tc(const DenseAttnArgs& a, int dtype, cudaStream_t stream);
 
 int dense_attn_fwd_simt(const DenseAttnArgs& a, int dtype, cudaStream_t stream);

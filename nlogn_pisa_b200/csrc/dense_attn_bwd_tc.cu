@@ -1,7 +1,7 @@
 // Dense attention backward on the tensor cores: 16-bit tensors, heads of at
 // most 128 dims (formulas in dense_attn.cu).  Three launches:
 //
-// 1. Row statistics: -lse and -scale * delta of every query (delta = dout .
+// 1. Row statistics: -lse and -scale * delta (fp16: -delta) of every query (delta = dout .
 //    out, with the part of out that its rounding dropped: it would add half
 //    again to the rounding errors of dQ and dK), base 2, in tiles of 128
 //    queries of one sequence and head.  Rows past a sequence's end and rows
@@ -21,7 +21,14 @@
 // Recomputing S and dP in launch 3 costs two more products than one kernel
 // that adds dQ tiles into memory, but every sum stays in TMEM: no atomics, no
 // fp32 copy of dQ, and results do not vary from run to run.  P and dS are
-// rounded to the input type because the MMAs take their operands so.
+// rounded to the input type because the MMAs take their operands so.  In fp16 dS
+// leaves the scale to the stores and carries a power of two instead, one per
+// sequence and KV head, that brings the largest possible dS just under the
+// type's range (launch 0 finds the largest finite |dout| and |v|; |dP - delta|
+// is at most twice their product times the dims).  Otherwise dS, about scale |dout|
+// / keys, falls below fp16's normal range: with dout of 1e-3, 2048 keys and 64
+// dims dQ and dK had an error of 0.0066 of their norm, now 0.00034 (a
+// once-rounded result: 0.00027).  bf16 has fp32's range and keeps the scale in dS.
 //
 // Rows of the last, ragged tile of a sequence belong to other sequences: the
 // products that sum over them take only the 16-row steps that hold real rows,
@@ -52,7 +59,7 @@ constexpr int kThreads = 352;
 // 4; dQ 235, 231, 226, 232 and 238.
 constexpr int kPolyKv = 3, kPolyQ = 2;
 
-// Statistics of a query tile: -lse (base 2) and -scale * delta of its rows in
+// Statistics of a query tile: -lse (base 2) and -scale * delta (fp16: -delta) of its rows in
 // fp32, then 16 bytes per row for the products of launch 2 (see mma_stat).
 constexpr int kStat = 2 * kRows + kRows * 4, kStatBytes = kRows * 16;
 
@@ -62,6 +69,7 @@ struct BwdTcArgs {
   float* stats;                          // [Hq][q_slots][kStat]
   SeqTile* order;                        // query tiles, then key tiles, in falling order of their work
   int* counters;                         // items of launches 2 and 3 drawn past each CTA's first
+  uint32_t* range;                       // fp16: bits of the largest |dout| and |v| by sequence and KV head
   int64_t q_slots, k_slots;
   int bf16;
 };
@@ -83,6 +91,51 @@ __device__ __forceinline__ float* stat_tile(const BwdTcArgs& a, int hq, int64_t 
 // Factor of the scores in base 2, never quite zero (the statistics are divided by it).
 __device__ __forceinline__ float base2_scale(const DenseAttnArgs& a) {
   return fmaxf(a.scale * kLog2e, 1e-30f);
+}
+
+template <typename T> constexpr bool kHalf = std::is_same<T, __half>::value;
+
+// Launch 0 (fp16): a CTA per query tile (dout) or key tile (v) and KV head.
+// Elements that are not finite are left out: they reach their own rows anyway.
+__global__ void __launch_bounds__(128) dense_range_kernel(const __grid_constant__ BwdTcArgs args) {
+  const DenseAttnArgs& a = args.d;
+  const bool keys = int64_t(blockIdx.x) >= args.q_slots;
+  const int h = blockIdx.y;
+  const SeqTile t = seq_tile(a, int(keys ? blockIdx.x - args.q_slots : blockIdx.x), kRows, keys);
+  const int first = t.tile * kRows, rows = min(kRows, (keys ? t.k_len : t.q_len) - first);
+  const int words = (keys ? 1 : a.G) * a.Dv / 8;       // of a row, side by side
+  const int64_t stride = keys ? a.v_st : int64_t(a.Hq) * a.Dv;
+  const __half* at = keys ? static_cast<const __half*>(a.v) + t.b * a.v_sb + int64_t(t.k_begin + first) * a.v_st + h * a.v_sh
+                          : static_cast<const __half*>(a.dout) +
+                                ((int64_t(t.b) * a.T + t.q_begin + first) * a.Hq + int64_t(h) * a.G) * a.Dv;
+  uint32_t most = 0;                                   // of the low and the high halves
+  for (int i = threadIdx.x; i < rows * words; i += 128) {
+    const int r = i / words;
+    const uint4 x = __ldg(reinterpret_cast<const uint4*>(at + r * stride + (i - r * words) * 8));
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t size = w[e] & 0x7fff7fffu;
+      most = __vmaxu2(most, size & ~__vcmpgeu2(size, 0x7c007c00u));
+    }
+  }
+  most = __reduce_max_sync(kFull, max(most & 0xffffu, most >> 16));
+  if (threadIdx.x % 32 == 0 && most) atomicMax(args.range + (int64_t(t.seq) * a.H + h) * 2 + int(keys), most);
+}
+
+// The factor of dS in the type's range: 2^15 over the next power of two above its bound.
+template <typename T>
+__device__ __forceinline__ float grad_factor(const BwdTcArgs& args, int seq, int h) {
+  if constexpr (!kHalf<T>) return args.d.scale;
+  const uint32_t* at = args.range + (int64_t(seq) * args.d.H + h) * 2;
+  const float bound = 2.f * float(args.d.Dv) * __half2float(__ushort_as_half(uint16_t(at[0]))) *
+                      __half2float(__ushort_as_half(uint16_t(at[1])));
+  return bound == 0.f ? 1.f : __uint_as_float((127u + 15u + 126u - (__float_as_uint(bound) >> 23)) << 23);
+}
+// What dS with that factor still lacks, at the stores of dQ and dK.
+template <typename T>
+__device__ __forceinline__ float grad_rest(const BwdTcArgs& args, float factor) {
+  return kHalf<T> ? args.d.scale / factor : 1.f;
 }
 
 // x = three bf16 values, to 24 bits
@@ -179,7 +232,7 @@ __global__ void __launch_bounds__(256) dense_stats_kernel(const __grid_constant_
         const float nlse = -lse[i] * kLog2e, sl = base2_scale(a);
         const bool dead = lse[i] == -INFINITY;
         tile[row] = dead ? -INFINITY : nlse;
-        tile[kRows + row] = -dot * a.scale;
+        tile[kRows + row] = kHalf<T> ? -dot : -dot * a.scale;
         const uint2 m = three_parts(dead ? -0x1p127f : nlse / sl), d3 = three_parts(-dot);
         reinterpret_cast<uint4*>(tile + 2 * kRows)[row] = make_uint4(m.x, m.y, d3.x, d3.y);
       }
@@ -253,9 +306,10 @@ struct DkvItem {
   int head;                           // < 0: no item
   int first_tile, end_tile;           // query tiles that see a key of the tile
   int per_head, total, tail;          // their number, with all heads of the group; real rows of the last one
+  float factor;                       // of dS
 };
 
-__device__ __forceinline__ DkvItem dkv_item(const BwdTcArgs& args, int n) {
+template <typename T> __device__ __forceinline__ DkvItem dkv_item(const BwdTcArgs& args, int n) {
   const DenseAttnArgs& a = args.d;
   DkvItem w;
   const bool found = draw(n, int(args.k_slots * a.H), args.counters, [&](int at) {
@@ -268,6 +322,7 @@ __device__ __forceinline__ DkvItem dkv_item(const BwdTcArgs& args, int n) {
     w.per_head = first < w.t.q_len ? w.end_tile - w.first_tile : 0;
     w.total = w.per_head * a.G;
     w.tail = w.t.q_len - (w.end_tile - 1) * kRows;
+    w.factor = grad_factor<T>(args, w.t.seq, w.head);
     return true;
   });
   if (!found) w.head = -1;
@@ -329,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
     if (lane == 0) {
       int pos = 0, used = 0;          // ring position; items with queries so far
       for (int n = 0; wait.ok; ++n) {
-        const DkvItem w = dkv_item(args, n);
+        const DkvItem w = dkv_item<T>(args, n);
         queue.put(n, w, wait);
         if (w.head < 0) break;
         if (w.total == 0) continue;
@@ -465,11 +520,12 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
     const int side = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;   // key row, queries 64*side ..
     const uint32_t lanes = uint32_t(quarter * 32) << 16;
     const uint32_t ts = tS + lanes + side * 64, tp = tP + lanes + side * 64;
-    const float2 sl2 = make_float2(base2_scale(a), base2_scale(a)), sc2 = make_float2(a.scale, a.scale);
+    const float2 sl2 = make_float2(base2_scale(a), base2_scale(a));
     int tile = 0, used = 0, item = 0;
     DkvItem w = queue.take(item, wait, lane);
     while (w.head >= 0) {
       const int j0 = w.t.tile * kRows;
+      const float2 sc2 = make_float2(w.factor, w.factor);
       const int first = first_seeing(a, w.t, j0 + row), whole = first_seeing(a, w.t, j0 + kRows - 1);
       int qt = w.first_tile;
       for (int n = 0; n < w.total; ++n, ++tile) {
@@ -530,9 +586,10 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
       const int rows = min(32, w.t.k_len - (j0 + quarter * 32)), cols = side ? a.D : a.Dv;
       const int64_t at = (int64_t(w.t.b) * a.N + w.t.k_begin + j0 + quarter * 32) * a.H + w.head;
       T* to = static_cast<T*>(side ? a.dk : a.dv) + at * cols;
+      const float rest = !wait.ok ? NAN : side ? grad_rest<T>(args, w.factor) : 1.f;
 #pragma unroll 1
       for (int c = 0; c < DP; c += 32) {
-        store_lanes<T, 32>((side ? tK : tV) + lanes + c, w.total == 0, wait.ok ? 1.f : NAN, out_addr + warp * 32 * 64, to + c,
+        store_lanes<T, 32>((side ? tK : tV) + lanes + c, w.total == 0, rest, out_addr + warp * 32 * 64, to + c,
                            int64_t(a.H) * cols, rows, cols - c, lane);
         __syncwarp();
       }
@@ -551,9 +608,10 @@ struct DqItem {
   SeqTile t;
   int head;                           // < 0: no item
   int valid, total, tail;             // real rows; key tiles, and the real rows of the last one
+  float factor;                       // of dS
 };
 
-__device__ __forceinline__ DqItem dq_item(const BwdTcArgs& args, int n) {
+template <typename T> __device__ __forceinline__ DqItem dq_item(const BwdTcArgs& args, int n) {
   const DenseAttnArgs& a = args.d;
   DqItem w;
   const bool found = draw(n, int(args.q_slots * a.Hq), args.counters + 1, [&](int at) {
@@ -565,6 +623,7 @@ __device__ __forceinline__ DqItem dq_item(const BwdTcArgs& args, int n) {
     const int keys = last_visible(a, w.t, w.t.tile * kRows + w.valid - 1) + 1;
     w.total = (keys + kRows - 1) / kRows;
     w.tail = min(kRows, w.t.k_len - (w.total - 1) * kRows);
+    w.factor = grad_factor<T>(args, w.t.seq, w.head / a.G);
     return true;
   });
   if (!found) w.head = -1;
@@ -615,7 +674,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
     if (lane == 0) {
       int pos = 0, used = 0;                    // ring position; items with keys so far
       for (int n = 0; wait.ok; ++n) {
-        const DqItem w = dq_item(args, n);
+        const DqItem w = dq_item<T>(args, n);
         queue.put(n, w, wait);
         if (w.head < 0) break;
         if (w.total <= 0) continue;
@@ -722,7 +781,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
   } else {
     const int side = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;   // query row, keys 64*side ..
     const uint32_t lanes = uint32_t(quarter * 32) << 16;
-    const float2 sl2 = make_float2(a.scale * kLog2e, a.scale * kLog2e), sc2 = make_float2(a.scale, a.scale);
+    const float2 sl2 = make_float2(a.scale * kLog2e, a.scale * kLog2e);
     int tile = 0, used = 0, item = 0;
     float nlse = -INFINITY, ndel = 0.f;
     auto statistics = [&](const DqItem& w) {
@@ -731,14 +790,14 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
       if (w.head >= 0 && row < w.valid) {
         const float* st = stat_tile(args, w.head, query_slot(a, w.t, w.t.tile, kRows));
         nlse = st[row];
-        ndel = st[kRows + row];
+        ndel = kHalf<T> ? st[kRows + row] * w.factor : st[kRows + row];
       }
     };
     DqItem w = queue.take(item, wait, lane);
     statistics(w);
     while (w.head >= 0) {
       const int q0 = w.t.tile * kRows;
-      const float2 nlse2 = make_float2(nlse, nlse), ndel2 = make_float2(ndel, ndel);
+      const float2 nlse2 = make_float2(nlse, nlse), ndel2 = make_float2(ndel, ndel), sc2 = make_float2(w.factor, w.factor);
       const int last = row < w.valid ? last_visible(a, w.t, q0 + row) : -1;
       const int whole = (last_visible(a, w.t, q0) + 1) / kRows;   // key tiles that every row sees whole
       for (int n = 0; n < w.total; ++n, ++tile) {
@@ -787,7 +846,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
       // each side stores half of the columns
       const int rows = min(32, w.valid - quarter * 32);
       const int64_t at = (int64_t(w.t.b) * a.T + w.t.q_begin + q0 + quarter * 32) * a.Hq + w.head;
-      store_lanes<T, DP / 2>(tQ + lanes + side * (DP / 2), w.total <= 0, wait.ok ? 1.f : NAN, out_addr + warp * 32 * DP,
+      store_lanes<T, DP / 2>(tQ + lanes + side * (DP / 2), w.total <= 0, wait.ok ? grad_rest<T>(args, w.factor) : NAN, out_addr + warp * 32 * DP,
                              static_cast<T*>(a.dq) + at * a.D + side * (DP / 2), int64_t(a.Hq) * a.D, rows,
                              a.D - side * (DP / 2), lane);
       __syncwarp();
@@ -822,10 +881,15 @@ int bwd_t(const BwdTcArgs& a, cudaStream_t s) {
 
 }  // namespace
 
-int64_t dense_bwd_workspace(bool packed, int64_t B, int64_t T, int64_t N, int64_t Hq, int64_t sequences) {
+namespace {
+// Entries of `range`: two per sequence (and one for the rows past the last) and KV head.
+int64_t range_entries(bool packed, int64_t B, int64_t H, int64_t sequences) { return 2 * H * (packed ? sequences + 1 : B); }
+}  // namespace
+
+int64_t dense_bwd_workspace(bool packed, int dtype, int64_t B, int64_t T, int64_t N, int64_t Hq, int64_t H, int64_t sequences) {
   const int64_t q = seq_slots(packed, B, T, sequences, kRows), k = seq_slots(packed, B, N, sequences, kRows);
   return q * Hq * kStat * int64_t(sizeof(float)) + (q + k) * int64_t(sizeof(SeqTile)) +
-         2 * int64_t(sizeof(int));
+         (2 + (dtype == PISA_F16 ? range_entries(packed, B, H, sequences) : 0)) * int64_t(sizeof(int));
 }
 
 int dense_attn_bwd_tc(const DenseAttnArgs& d, int dtype, cudaStream_t stream) {
@@ -838,6 +902,13 @@ int dense_attn_bwd_tc(const DenseAttnArgs& d, int dtype, cudaStream_t stream) {
   a.order = reinterpret_cast<SeqTile*>(d.delta + a.q_slots * d.Hq * kStat);
   a.counters = reinterpret_cast<int*>(a.order + a.q_slots + a.k_slots);
   if (a.q_slots * d.Hq >= (int64_t(1) << 31) - 4096 || a.k_slots * d.H >= (int64_t(1) << 31) - 4096) return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
+  if (dtype == PISA_F16) {
+    a.range = reinterpret_cast<uint32_t*>(a.counters + 2);
+    const cudaError_t e = cudaMemsetAsync(a.range, 0, range_entries(d.cu_q, d.B, d.H, d.sequences) * sizeof(int), stream);
+    if (e != cudaSuccess) return fail_cuda(e, "range clear");
+    dense_range_kernel<<<dim3(unsigned(a.q_slots + a.k_slots), unsigned(d.H)), 128, 0, stream>>>(a);
+    PISA_CHECK_LAUNCH();
+  }
   int rc = dense_tensor_map(&a.tm_q, d.q, dtype, d.B, d.T, d.Hq, d.D, d.q_sb, d.q_st, d.q_sh, kRows);
   if (rc == PISA_OK) rc = dense_tensor_map(&a.tm_k, d.k, dtype, d.B, d.N, d.H, d.D, d.k_sb, d.k_st, d.k_sh, kRows);
   if (rc == PISA_OK) rc = dense_tensor_map(&a.tm_v, d.v, dtype, d.B, d.N, d.H, d.Dv, d.v_sb, d.v_st, d.v_sh, kRows);

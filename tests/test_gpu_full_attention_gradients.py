@@ -1,0 +1,89 @@
+"""Gradients of full_attention over the types' ranges, by the norm of their error.
+
+The element bounds of dense_reference allow each of many roundings its worst
+case; here the error's norm is held to what random roundings of the same size
+give, so a gradient that lost its bits (or is zero) fails.
+"""
+
+import pytest
+import torch
+
+import dense_reference as R
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def normal(gen, *shape, dtype=BF16, size=1.0):
+    return (size * torch.randn(shape, generator=gen, device="cuda")).to(dtype)
+
+
+def cumulative(lengths):
+    return torch.tensor([0, *torch.tensor(lengths).cumsum(0).tolist()], dtype=torch.int32, device="cuda")
+
+
+def room(value, dtype):
+    """Norm of the error that a result may have: the rounding of the result
+    itself, once more the size of that for each of its two 16-bit operands, and
+    sums in fp32 (a random walk of a few hundred roundings)."""
+    once = float((value.to(dtype).double() - value).norm())
+    unit = 64 * R.EPS if dtype == F32 else R.UNIT[dtype]
+    return 2 * once + unit * float(value.norm())
+
+
+def compare(q, k, v, dout, lengths, scale=None, names=("dq", "dk", "dv")):
+    import nlogn_pisa_b200 as P
+
+    leaves = [x.detach().requires_grad_(True) for x in (q, k, v)]
+    out = P.full_attention(*leaves, cu_seqlens=cumulative(lengths), scale=scale)
+    grads = dict(zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, dout)))
+    value, _ = R.attention(q, k, v, queries=lengths, scale=scale, dout=dout)
+    begin = 0
+    for n in lengths:       # sequence by sequence: one may be far smaller than another
+        for name in names:
+            got, want = (x[0, begin:begin + n].double() for x in (grads[name], value[name]))
+            assert torch.isfinite(want.to(q.dtype)).all() and float(want.to(q.dtype).abs().max()) > 0
+            off = float((got - want).norm())
+            assert off <= room(want, q.dtype), (name, n, off / float(want.norm()), room(want, q.dtype) / float(want.norm()))
+        begin += n
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 4, 64), (4, 2, 128), (4, 1, 80), (2, 1, 160)])
+@pytest.mark.parametrize("size,v_size", [(1.0, 1.0), (1e-2, 1.0), (1e-3, 1.0), (1e-4, 1.0), (1e-2, 1e-2), (300.0, 20.0), (0.01, 1000.0)])
+def test_sizes(cuda_device, dtype, heads, kv_heads, dim, size, v_size):
+    """dout of a mean over many tokens, of a scaled loss, and values of other sizes."""
+    gen = torch.Generator(device="cuda").manual_seed(dim)
+    lengths = [1100, 333]
+    q, k = normal(gen, 1, 1433, heads, dim, dtype=dtype), normal(gen, 1, 1433, kv_heads, dim, dtype=dtype)
+    v, dout = normal(gen, 1, 1433, kv_heads, dim, dtype=dtype, size=v_size), normal(gen, 1, 1433, heads, dim, dtype=dtype, size=size)
+    compare(q, k, v, dout, lengths)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_sequences_of_different_sizes(cuda_device, dtype, dim):
+    """A packed sequence whose gradient is 10^5 times another's takes no bits from it; nor does another head's."""
+    gen = torch.Generator(device="cuda").manual_seed(dim + 1)
+    lengths = [700, 500]
+    q, k, v, dout = normal(gen, 1, 1200, 4, dim, dtype=dtype), *(normal(gen, 1, 1200, 2, dim, dtype=dtype) for _ in range(2)), \
+        normal(gen, 1, 1200, 4, dim, dtype=dtype)
+    loud = dout.clone()
+    loud[:, :700] *= 100
+    loud[:, 700:] *= 1e-3
+    compare(q, k, v, loud, lengths)
+    import nlogn_pisa_b200 as P
+
+    def grads(g):
+        leaves = [x.detach().requires_grad_(True) for x in (q, k, v)]
+        return torch.autograd.grad(P.full_attention(*leaves, cu_seqlens=cumulative(lengths)), leaves, g)
+
+    quiet = dout.clone()
+    quiet[:, 700:] *= 1e-3
+    for x, y in zip(grads(loud), grads(quiet)):
+        assert torch.equal(x[:, 700:], y[:, 700:])
+    tall = dout.clone()
+    tall[:, :, 2:] *= 100        # the query heads of the second KV head
+    for (x, y), n in zip(zip(grads(tall), grads(dout)), (2, 1, 1)):
+        assert torch.equal(x[:, :, :n], y[:, :, :n])
