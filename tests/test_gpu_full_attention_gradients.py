@@ -87,3 +87,40 @@ def test_sequences_of_different_sizes(cuda_device, dtype, dim):
     tall[:, :, 2:] *= 100        # the query heads of the second KV head
     for (x, y), n in zip(zip(grads(tall), grads(dout)), (2, 1, 1)):
         assert torch.equal(x[:, :, :n], y[:, :, :n])
+
+
+@pytest.mark.parametrize("dtype,scale,size", [(F32, 1e-4, 1.0), (F32, 1e-33, 1.0), (BF16, 1e-4, 1.0), (BF16, 1e-33, 1.0),
+                                              (F16, 1e-4, 1.0), (F16, 1e-4, 100.0), (F16, 1e-6, 1000.0), (F32, 3.0, 1.0),
+                                              (BF16, 3.0, 1.0), (F16, 3.0, 1.0)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_scales(cuda_device, dtype, scale, size, dim):
+    gen = torch.Generator(device="cuda").manual_seed(dim + 2)
+    q, k, v = normal(gen, 1, 520, 4, dim, dtype=dtype, size=0.2 if scale > 1 else 1.0), *(normal(gen, 1, 520, 2, dim, dtype=dtype) for _ in range(2))
+    compare(q, k, v, normal(gen, 1, 520, 4, dim, dtype=dtype, size=size), [300, 220], scale=scale)
+
+
+def test_against_differences(cuda_device):
+    """Differences of the fp32 forward along each operand's own gradient: zero, flipped or missing ones fail."""
+    import nlogn_pisa_b200 as P
+
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    lengths = [37, 70]
+    x = {n: normal(gen, 1, 107, h, 64, dtype=F32) for n, h in (("q", 4), ("k", 2), ("v", 2))}
+    w = normal(gen, 1, 107, 4, 64, dtype=F32)
+    leaves = [t.clone().requires_grad_(True) for t in x.values()]
+    grads = torch.autograd.grad(P.full_attention(*leaves, cu_seqlens=cumulative(lengths)), leaves, w)
+    value, _ = R.attention(*x.values(), queries=lengths, dout=w)
+    step = 2.0 ** -4
+    for name, grad in zip(x, grads):
+        way = value["d" + name] / value["d" + name].abs().max()
+        ends = [{**x, name: (x[name].double() + sign * step * way).float()} for sign in (1, -1)]
+        moved = (ends[0][name].double() - ends[1][name].double())        # what the rounded ends are apart
+        got = [float((P.full_attention(*e.values(), cu_seqlens=cumulative(lengths)).double() * w.double()).sum()) for e in ends]
+        exact = [float((R.attention(*e.values(), queries=lengths)[0]["out"] * w.double()).sum()) for e in ends]
+        along = float((grad.double() * moved).sum())
+        true = float((value["d" + name] * moved).sum())
+        # rounding of the two forwards (sixteen units per output, random signs), and the curvature that 64 bits show
+        slack = 2 * 16 * R.EPS * float(w.norm()) + abs(exact[0] - exact[1] - true)
+        assert slack <= 0.1 * abs(true)
+        assert abs(got[0] - got[1] - along) <= slack + 64 * R.EPS * abs(true)
+        assert abs(along - true) <= 64 * R.EPS * abs(true)
