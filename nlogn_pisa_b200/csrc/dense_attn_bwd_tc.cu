@@ -28,7 +28,9 @@
 // is at most twice their product times the dims).  Otherwise dS, about scale |dout|
 // / keys, falls below fp16's normal range: with dout of 1e-3, 2048 keys and 64
 // dims dQ and dK had an error of 0.0066 of their norm, now 0.00034 (a
-// once-rounded result: 0.00027).  bf16 has fp32's range and keeps the scale in dS.
+// once-rounded result: 0.00027).  P, about 1 / keys, is taken times 2^15 in launch
+// 2 for the same reason (262144 keys: error of dV 0.0044, now below 0.0009).
+// bf16 has fp32's range and keeps the scale in dS and P as it is.
 //
 // Rows of the last, ragged tile of a sequence belong to other sequences: the
 // products that sum over them take only the 16-row steps that hold real rows,
@@ -94,6 +96,8 @@ __device__ __forceinline__ float base2_scale(const DenseAttnArgs& a) {
 }
 
 template <typename T> constexpr bool kHalf = std::is_same<T, __half>::value;
+// P of launch 2 carries 2^kWeightShift: its largest, 2^15, is within fp16's range.
+template <typename T> constexpr int kWeightShift = kHalf<T> ? 15 : 0;
 
 // Launch 0 (fp16): a CTA per query tile (dout) or key tile (v) and KV head.
 // Elements that are not finite are left out: they reach their own rows anyway.
@@ -233,7 +237,7 @@ __global__ void __launch_bounds__(256) dense_stats_kernel(const __grid_constant_
         const bool dead = lse[i] == -INFINITY;
         tile[row] = dead ? -INFINITY : nlse;
         tile[kRows + row] = kHalf<T> ? -dot : -dot * a.scale;
-        const uint2 m = three_parts(dead ? -0x1p127f : nlse / sl), d3 = three_parts(-dot);
+        const uint2 m = three_parts(dead ? -0x1p127f : (nlse + float(kWeightShift<T>)) / sl), d3 = three_parts(-dot);
         reinterpret_cast<uint4*>(tile + 2 * kRows)[row] = make_uint4(m.x, m.y, d3.x, d3.y);
       }
     }
@@ -525,7 +529,8 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
     DkvItem w = queue.take(item, wait, lane);
     while (w.head >= 0) {
       const int j0 = w.t.tile * kRows;
-      const float2 sc2 = make_float2(w.factor, w.factor);
+      const float factor = kHalf<T> ? w.factor / float(1 << kWeightShift<T>) : w.factor;
+      const float2 sc2 = make_float2(factor, factor);
       const int first = first_seeing(a, w.t, j0 + row), whole = first_seeing(a, w.t, j0 + kRows - 1);
       int qt = w.first_tile;
       for (int n = 0; n < w.total; ++n, ++tile) {
@@ -586,7 +591,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
       const int rows = min(32, w.t.k_len - (j0 + quarter * 32)), cols = side ? a.D : a.Dv;
       const int64_t at = (int64_t(w.t.b) * a.N + w.t.k_begin + j0 + quarter * 32) * a.H + w.head;
       T* to = static_cast<T*>(side ? a.dk : a.dv) + at * cols;
-      const float rest = !wait.ok ? NAN : side ? grad_rest<T>(args, w.factor) : 1.f;
+      const float rest = !wait.ok ? NAN : side ? grad_rest<T>(args, w.factor) : 1.f / float(1 << kWeightShift<T>);
 #pragma unroll 1
       for (int c = 0; c < DP; c += 32) {
         store_lanes<T, 32>((side ? tK : tV) + lanes + c, w.total == 0, rest, out_addr + warp * 32 * 64, to + c,

@@ -89,6 +89,22 @@ def test_sequences_of_different_sizes(cuda_device, dtype, dim):
         assert torch.equal(x[:, :, :n], y[:, :, :n])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_small_weights(cuda_device, dtype):
+    """Weights near 1 / keys over many keys: dv keeps their bits."""
+    import nlogn_pisa_b200 as P
+
+    gen = torch.Generator(device="cuda").manual_seed(21)
+    keys, rows = 262144, 128
+    q, k = normal(gen, 1, rows, 1, 64, dtype=dtype, size=0.3), normal(gen, 1, keys, 1, 64, dtype=dtype)
+    v, dout = normal(gen, 1, keys, 1, 64, dtype=dtype), normal(gen, 1, rows, 1, 64, dtype=dtype, size=100.0)
+    leaves = [x.requires_grad_(True) for x in (q, k, v)]
+    dv = torch.autograd.grad(P.full_attention(*leaves, causal=False), leaves, dout)[2]
+    weights = torch.softmax(q[0, :, 0].detach().double() @ k[0, :, 0].detach().double().T / 8, -1)
+    want = weights.T @ dout[0, :, 0].double()
+    assert float((dv[0, :, 0].double() - want).norm()) <= room(want, dtype)
+
+
 @pytest.mark.parametrize("dtype,scale,size", [(F32, 1e-4, 1.0), (F32, 1e-33, 1.0), (BF16, 1e-4, 1.0), (BF16, 1e-33, 1.0),
                                               (F16, 1e-4, 1.0), (F16, 1e-4, 100.0), (F16, 1e-6, 1000.0), (F32, 3.0, 1.0),
                                               (BF16, 3.0, 1.0), (F16, 3.0, 1.0)])
