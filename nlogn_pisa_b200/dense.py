@@ -10,6 +10,7 @@ that all sequences share, through pisa_prefix_attn.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -27,6 +28,26 @@ def aligned_rows(t):
         elif t.stride(-1) == 1 and all(s % per == 0 and (s > 0 or n == 1) for s, n in zip(t.stride()[:-1], t.shape)):
             return t
     return t.clone(memory_format=torch.contiguous_format)
+
+
+def differentiated(*tensors):
+    """Whether autograd has to see a call on these tensors: one requires grad, or
+    carries a tangent (forward mode, for which the operators' autograd functions raise)."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                return True
+    return carries_tangent(*tensors)
+
+
+def carries_tangent(*tensors):
+    # outside every dual level there are none: one attribute instead of a call per tensor
+    if getattr(forward_ad, "_current_level", 0) < 0:
+        return False
+    for t in tensors:
+        if forward_ad.unpack_dual(t).tangent is not None:
+            return True
+    return False
 
 
 def flat(t):
@@ -147,7 +168,8 @@ def full_attention(q, k, v, cu_seqlens=None, cu_seqlens_k=None, scale=None, quer
     of a continued prompt), and each sequence's queries are its last positions.
     Sequences may be empty.  Cumulative lengths on the GPU are read there: the
     call never waits for the device.  Queries without a visible key give 0.
-    ``return_lse`` adds the [B,Tq,Hq] log-sum-exp (not differentiable).
+    ``return_lse`` adds the [B,Tq,Hq] log-sum-exp (not differentiable).  The
+    gradient is reverse mode only: forward mode raises RuntimeError.
     """
     _validate(q, k, v)
     scale = k.shape[-1] ** -0.5 if scale is None else float(scale)
@@ -173,7 +195,7 @@ def full_attention(q, k, v, cu_seqlens=None, cu_seqlens_k=None, scale=None, quer
             raise ValueError("query_offset must be an integer; sequences at different positions are packed ones")
         _, offset = query_positions(q, k, query_offset)
     q, k, v = aligned_rows(q), aligned_rows(k), aligned_rows(v)
-    if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+    if differentiated(q, k, v):
         out, lse = FullAttentionFunction.apply(q, k, v, cu_seqlens, cu_seqlens_k, offset, scale, bool(causal))
     else:
         out, lse, _ = _forward(q, k, v, cu_seqlens, cu_seqlens_k, offset, scale, causal, return_lse)
@@ -188,9 +210,11 @@ def prefix_attention(q, k, v, lengths, prefix_k=None, prefix_v=None, scale=None,
     GPU, clamped to the capacity); prefix_k, prefix_v: [P,H,D|Dv], shared by
     all sequences and read once for the whole batch.  Token t sees the prefix
     and its own keys up to lengths - Tq + t; without any, it gives 0.  For
-    inference: no gradient is recorded.
+    inference: no gradient is recorded, and forward-mode tangents are refused.
     """
     _validate(q, k, v)
+    if carries_tangent(q, k, v):
+        raise ValueError("prefix_attention has no derivative")
     batch, tokens, q_heads, dim = q.shape
     _, capacity, heads, dim_v = v.shape
     device = q.get_device()
@@ -206,6 +230,8 @@ def prefix_attention(q, k, v, lengths, prefix_k=None, prefix_v=None, scale=None,
         q = q.contiguous()
     prefix, shared = 0, (None, 0, 0, None, 0, 0)
     if prefix_k is not None:
+        if carries_tangent(prefix_k, prefix_v):
+            raise ValueError("prefix_attention has no derivative")
         if (prefix_k.dim() != 3 or prefix_k.shape[1:] != k.shape[2:] or prefix_v.shape != (*prefix_k.shape[:2], dim_v)
                 or any(t.dtype != q.dtype or t.device != q.device for t in (prefix_k, prefix_v))):
             raise ValueError("prefix_k and prefix_v must have shape [P,H,D] with the caches' heads, dims, dtype and device")

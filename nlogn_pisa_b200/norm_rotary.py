@@ -13,7 +13,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .dense import aligned_rows, flat, view
+from .dense import aligned_rows, differentiated, flat, view
 from .validation import require_cuda
 
 
@@ -66,6 +66,7 @@ def qk_norm_rotary(q, k, q_weight, k_weight, frequency, positions=None, position
     ``k_weight``: [D], both in fp32 or both in q's dtype; ``frequency``: [D/2] (as
     ``mixer.rotary_frequencies``; a zero leaves its pair unrotated);
     ``positions``: [1|B, T] integers, or None for ``position_offset`` + token.
+    The gradient is reverse mode only: forward mode raises RuntimeError.
     """
     if q.dim() != 4 or k.dim() != 4:
         raise ValueError("q and k must have shape [batch, tokens, heads, head_dim]")
@@ -99,6 +100,6 @@ def qk_norm_rotary(q, k, q_weight, k_weight, frequency, positions=None, position
     q, k = aligned_rows(q), aligned_rows(k)
     q_weight, k_weight = q_weight.contiguous(), k_weight.contiguous()
     args = (q, k, q_weight, k_weight, frequency, positions, int(position_offset), float(eps))
-    if (q.requires_grad or k.requires_grad or q_weight.requires_grad or k_weight.requires_grad) and torch.is_grad_enabled():
+    if differentiated(q, k, q_weight, k_weight):
         return QkNormRotaryFunction.apply(*args)
     return _forward(*args)
