@@ -4,7 +4,8 @@
 all keys of its sequence, for batches and for packed sequences, through
 pisa_full_attn_fwd / pisa_full_attn_bwd.  ``prefix_attention`` is its serving
 form for a step's newest tokens, over each sequence's own cache and a prefix
-that all sequences share, through pisa_prefix_attn.
+that all sequences share, through pisa_prefix_attn; ``continued_attention`` is
+the form for many new tokens per sequence over such a prefix.
 """
 
 from __future__ import annotations
@@ -209,7 +210,9 @@ def prefix_attention(q, k, v, lengths, prefix_k=None, prefix_v=None, scale=None,
     ``lengths`` [B] valid keys each (this step's included; integers on the
     GPU, clamped to the capacity); prefix_k, prefix_v: [P,H,D|Dv], shared by
     all sequences and read once for the whole batch.  Token t sees the prefix
-    and its own keys up to lengths - Tq + t; without any, it gives 0.  For
+    and its own keys up to lengths - Tq + t; without any, it gives 0.  Made
+    for a few tokens per sequence: own caches are read once per 16 query rows of
+    a KV head, and B * Tq * Hq / H may not pass 1048560.  For
     inference: no gradient is recorded, and forward-mode tangents are refused.
     """
     _validate(q, k, v)
@@ -253,3 +256,41 @@ def prefix_attention(q, k, v, lengths, prefix_k=None, prefix_v=None, scale=None,
     if _lib.status_checks():
         _lib.check_workspace(workspace, q.device)
     return (out, lse) if return_lse else out
+
+
+# elements of an output that are joined at a time: half a gigabyte of fp32
+JOIN_ELEMENTS = 1 << 27
+
+
+def continued_attention(q, k, v, prefix_k, prefix_v):
+    """Attention of many new tokens q [B,T,Hq,D] of every sequence, the last
+    ones of its own k, v [B,N,H,D|Dv], over a prefix [P,H,D|Dv] that all share
+    and their own keys -> [B,T,Hq,Dv].
+
+    prefix_attention's result for prompts after a shared prefix, on
+    full_attention's tiles: the queries of the whole batch against the prefix
+    as one sequence, each sequence against its own keys, joined by their
+    log-sum-exp in fp32 (with what rounding dropped from either part).  No
+    gradient is recorded.
+    """
+    _validate(q, k, v)
+    _, offset = query_positions(q, k)
+    batch, tokens, heads, dim = q.shape
+    scale, q = dim ** -0.5, aligned_rows(q)
+    own = _forward(q, aligned_rows(k), aligned_rows(v), None, None, offset, scale, True, True, True)
+    rows = aligned_rows(q.reshape(1, batch * tokens, heads, dim))
+    shared = _forward(rows, aligned_rows(prefix_k[None]), aligned_rows(prefix_v[None]), None, None, 0, scale, False, True, True)
+    shared = [None if t is None else t.view(batch, tokens, *t.shape[2:]) for t in shared]
+    out, step = own[0], max(1, JOIN_ELEMENTS // own[0][0].numel())
+    for b in range(0, batch, step):
+        at = slice(b, b + step)
+        top = torch.maximum(own[1][at], shared[1][at])
+        weights = [(part[1][at] - top).exp_()[..., None] for part in (own, shared)]
+        total = torch.zeros_like(out[at], dtype=torch.float32)
+        for (value, _, low), weight in zip((own, shared), weights):
+            exact = value[at].float()
+            if low is not None:
+                exact += low[at]
+            total += exact.mul_(weight)
+        out[at] = total.div_(weights[0] + weights[1])
+    return out

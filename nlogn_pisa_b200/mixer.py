@@ -20,7 +20,7 @@ from torch import nn
 from . import _lib
 from .attention import sparse_attention
 from .cache import PyramidCache, TensorCache
-from .dense import full_attention, prefix_attention
+from .dense import continued_attention, full_attention, prefix_attention
 from .norm_rotary import qk_norm_rotary
 from .selection import select_blocks
 
@@ -153,7 +153,8 @@ class FullAttention(nn.Module):
     Training and prompts run full_attention (batches, or packed documents under
     ``cu_seqlens``).  With a cache, up to ``DECODE_TOKENS`` new tokens per
     sequence run prefix_attention over the cache, longer continuations
-    full_attention again.  ``share_prefix`` turns the cache of one prompt into
+    full_attention again (continued_attention over a shared prefix).
+    ``share_prefix`` turns the cache of one prompt into
     the start of a batch of answers to it, without copying its keys.
     """
 
@@ -235,9 +236,11 @@ class FullAttention(nn.Module):
             if use_cache:
                 next_cache = {"k": stores[0].tensor, "v": stores[1].tensor, "key_storage": stores[0],
                               "value_storage": stores[1], "prefix_k": prefix_k, "prefix_v": prefix_v}
-        if cache is not None and (shared or length <= self.DECODE_TOKENS):
+        if cache is not None and length <= self.DECODE_TOKENS:
             lengths = torch.full((batch,), past + length, dtype=torch.int32, device=x.device)
             output = prefix_attention(q, stores[0].buffer, stores[1].buffer, lengths, prefix_k=prefix_k, prefix_v=prefix_v)
+        elif shared:
+            output = continued_attention(q, stores[0].tensor, stores[1].tensor, prefix_k, prefix_v)
         else:
             if cache is not None:
                 keys, values = stores[0].tensor, stores[1].tensor
