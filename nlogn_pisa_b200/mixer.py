@@ -16,11 +16,12 @@ from __future__ import annotations
 
 import torch
 from torch import nn
+from torch.autograd.function import once_differentiable
 
-from . import _lib
+from . import _lib, dense
 from .attention import sparse_attention
 from .cache import PyramidCache, TensorCache
-from .dense import continued_attention, full_attention, prefix_attention
+from .dense import full_attention
 from .norm_rotary import qk_norm_rotary
 from .selection import select_blocks
 
@@ -146,6 +147,45 @@ class PyramidSparseAttention(nn.Module):
         return self.o_proj(output.reshape(batch, length, -1)), next_cache
 
 
+def _attend_cache(q, stores, prefix, decode_tokens):
+    """Attention of the newest tokens over the caches that end with them, and a shared prompt."""
+    batch, tokens = q.shape[:2]
+    if tokens <= decode_tokens:
+        lengths = torch.full((batch,), stores[0].length, dtype=torch.int32, device=q.device)
+        return dense.prefix_attention(q, stores[0].buffer, stores[1].buffer, lengths, prefix_k=prefix[0], prefix_v=prefix[1])
+    keys, values = stores[0].tensor, stores[1].tensor
+    if prefix[0] is not None:
+        return dense.continued_attention(q, keys, values, *prefix)
+    return full_attention(q, keys, values)
+
+
+class _CachedAttention(torch.autograd.Function):
+    """_attend_cache with the gradient in the newest tokens' q, k and v; what was
+    cached before them is constant.  The backward recomputes over the cache:
+    caches only grow at their end, so the rows it keeps hold what they held."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, stores, prefix, decode_tokens):
+        ctx.save_for_backward(q)
+        ctx.cached = (stores[0].tensor, stores[1].tensor, *prefix)
+        return _attend_cache(q, stores, prefix, decode_tokens)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, = ctx.saved_tensors
+        keys, values, prefix_k, prefix_v = ctx.cached
+        tokens = q.shape[1]
+        if prefix_k is not None:
+            keys, values = (torch.cat((p[None].expand(x.shape[0], -1, -1, -1), x), 1)
+                            for p, x in ((prefix_k, keys), (prefix_v, values)))
+        with torch.enable_grad():
+            leaves = [x.detach().requires_grad_(True) for x in (q, keys, values)]
+            out = full_attention(*leaves)
+        dq, dk, dv = torch.autograd.grad(out, leaves, dout)
+        return dq, dk[:, -tokens:], dv[:, -tokens:], None, None, None
+
+
 class FullAttention(nn.Module):
     """Full-attention token mixer: projections, per-head norms of q and k with the
     rotation (qk_norm_rotary), attention over all keys, output projection.
@@ -154,8 +194,11 @@ class FullAttention(nn.Module):
     ``cu_seqlens``).  With a cache, up to ``DECODE_TOKENS`` new tokens per
     sequence run prefix_attention over the cache, longer continuations
     full_attention again (continued_attention over a shared prefix).
-    ``share_prefix`` turns the cache of one prompt into
-    the start of a batch of answers to it, without copying its keys.
+    ``share_prefix`` turns the cache of one prompt into the start of a batch of
+    answers to it, without copying its keys.
+    With a cache, gradients reach this call's tokens; what earlier calls cached
+    is constant.  A call with a cache and without ``use_cache`` (a look ahead)
+    copies the cache and leaves it as it is.
     """
 
     DECODE_TOKENS = 16
@@ -223,7 +266,6 @@ class FullAttention(nn.Module):
             positions = self._document_positions(length, cu_seqlens, x.device)
         q, k = qk_norm_rotary(q, k, self.q_norm.to(q.dtype), self.k_norm.to(q.dtype), self.theta, positions=positions,
                               position_offset=shared + past, eps=self.eps)
-        keys, values = k, v
         next_cache = None
         if use_cache or cache is not None:
             if cache is None or cache["key_storage"] is None:
@@ -236,15 +278,12 @@ class FullAttention(nn.Module):
             if use_cache:
                 next_cache = {"k": stores[0].tensor, "v": stores[1].tensor, "key_storage": stores[0],
                               "value_storage": stores[1], "prefix_k": prefix_k, "prefix_v": prefix_v}
-        if cache is not None and length <= self.DECODE_TOKENS:
-            lengths = torch.full((batch,), past + length, dtype=torch.int32, device=x.device)
-            output = prefix_attention(q, stores[0].buffer, stores[1].buffer, lengths, prefix_k=prefix_k, prefix_v=prefix_v)
-        elif shared:
-            output = continued_attention(q, stores[0].tensor, stores[1].tensor, prefix_k, prefix_v)
+        if cache is None:
+            output = full_attention(q, k, v, cu_seqlens=cu_seqlens)
+        elif dense.differentiated(q, k, v):
+            output = _CachedAttention.apply(q, k, v, stores, (prefix_k, prefix_v), self.DECODE_TOKENS)
         else:
-            if cache is not None:
-                keys, values = stores[0].tensor, stores[1].tensor
-            output = full_attention(q, keys, values, cu_seqlens=cu_seqlens)
+            output = _attend_cache(q, stores, (prefix_k, prefix_v), self.DECODE_TOKENS)
         if past_key_values is not None and use_cache:
             while len(past_key_values) <= self.layer_idx:
                 past_key_values.append(None)

@@ -1,4 +1,4 @@
-"""The full-attention token mixer with caches: long continuations over a shared prompt."""
+"""The full-attention token mixer with caches: long continuations over a shared prompt, gradients."""
 
 import pytest
 import torch
@@ -63,3 +63,68 @@ def test_continued_attention_is_prefix_attention(cuda_device, dtype):
         dense.JOIN_ELEMENTS = tight
     unit = {torch.float32: 64 * 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[dtype]
     assert float((got.double() - want.double()).norm()) <= 2 * unit * float(want.double().norm())
+
+
+def reference_step(mixer, params, history, x):
+    """One cached call in float64: ``history`` is every token before it, whose keys and values are constants."""
+    cfg, theta = mixer.config, mixer.theta.double()
+    group = cfg.num_attention_heads // cfg.num_key_value_heads
+
+    def heads(y, name, n):
+        return (y @ params[name + ".weight"].T).view(*y.shape[:2], n, cfg.head_dim)
+
+    def rotate(y, w, offset):
+        y = y / (y.square().mean(-1, keepdim=True) + mixer.eps).sqrt() * w
+        angle = ((torch.arange(y.shape[1], device=y.device) + offset).double()[:, None] * theta)[:, None]
+        a, b = y.chunk(2, -1)
+        return torch.cat((a * angle.cos() - b * angle.sin(), a * angle.sin() + b * angle.cos()), -1)
+
+    past, new = history.shape[1], x.shape[1]
+    q = rotate(heads(x, "q_proj", cfg.num_attention_heads), params["q_norm"], past)
+    k = rotate(heads(x, "k_proj", cfg.num_key_value_heads), params["k_norm"], past)
+    v = heads(x, "v_proj", cfg.num_key_value_heads)
+    old_k = rotate(heads(history, "k_proj", cfg.num_key_value_heads), params["k_norm"], 0).detach()
+    old_v = heads(history, "v_proj", cfg.num_key_value_heads).detach()
+    k, v = (torch.cat(pair, 1).repeat_interleave(group, 2) for pair in ((old_k, k), (old_v, v)))
+    s = torch.einsum("bqhd,bkhd->bhqk", q, k) * cfg.head_dim ** -0.5
+    hidden = torch.arange(past + new, device=x.device)[None] > past + torch.arange(new, device=x.device)[:, None]
+    p = torch.softmax(s.masked_fill(hidden, float("-inf")), -1)
+    return torch.einsum("bhqk,bkhd->bqhd", p, v).reshape(*x.shape[:2], -1) @ params["o_proj.weight"].T
+
+
+@pytest.mark.parametrize("shared", [False, True])
+@pytest.mark.parametrize("steps", [[1, 1], [5, 30], [30, 5], [16, 17]])
+@pytest.mark.parametrize("look", [False, True])
+def test_gradients_with_a_cache(cuda_device, shared, steps, look):
+    """The same gradient rule at every length: this call's tokens get theirs, cached ones are constant."""
+    from nlogn_pisa_b200.mixer import FullAttention
+
+    mixer = make(torch.float32)
+    batch, prompt = 3, 70
+    first = torch.randn(1 if shared else batch, prompt, 256, device="cuda")
+    x = torch.randn(batch, sum(steps), 256, device="cuda").requires_grad_(True)
+    w = torch.randn(batch, sum(steps), 256, device="cuda")
+    with torch.no_grad():
+        _, cache = mixer(first, use_cache=True)
+    if shared:
+        cache = FullAttention.share_prefix(cache)
+    params = {n: p.detach().double().requires_grad_(True) for n, p in mixer.named_parameters()}
+    x64 = x.detach().double().requires_grad_(True)
+    history = first.detach().double().expand(batch, -1, -1)
+    loss, want, begin = 0, 0, 0
+    for i, n in enumerate(steps):
+        at = slice(begin, begin + n)
+        if look and i + 1 == len(steps):
+            out, _ = mixer(x[:, at], cache=cache)
+        else:
+            out, cache = mixer(x[:, at], cache=cache, use_cache=True)
+        loss = loss + (out * w[:, at]).sum()
+        want = want + (reference_step(mixer, params, history, x64[:, at]) * w[:, at].double()).sum()
+        history = torch.cat((history, x64[:, at].detach()), 1)
+        begin += n
+    # the first step's graph is followed after the second step grew the cache in place
+    loss.backward()
+    want.backward()
+    near(x.grad, x64.grad, torch.float32)
+    for n, p in mixer.named_parameters():
+        near(p.grad, params[n].grad, torch.float32)
