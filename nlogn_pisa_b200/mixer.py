@@ -264,8 +264,10 @@ class FullAttention(nn.Module):
         positions = None
         if cu_seqlens is not None and cfg.rope_position_mode == "document":
             positions = self._document_positions(length, cu_seqlens, x.device)
-        q, k = qk_norm_rotary(q, k, self.q_norm.to(q.dtype), self.k_norm.to(q.dtype), self.theta, positions=positions,
-                              position_offset=shared + past, eps=self.eps)
+        weights = self.q_norm, self.k_norm
+        if any(w.dtype not in (torch.float32, q.dtype) for w in weights) or weights[0].dtype != weights[1].dtype:
+            weights = [w.float() for w in weights]   # fp32 weights keep their bits beside 16-bit activations
+        q, k = qk_norm_rotary(q, k, *weights, self.theta, positions=positions, position_offset=shared + past, eps=self.eps)
         next_cache = None
         if use_cache or cache is not None:
             if cache is None or cache["key_storage"] is None:

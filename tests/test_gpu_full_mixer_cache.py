@@ -128,3 +128,24 @@ def test_gradients_with_a_cache(cuda_device, shared, steps, look):
     near(x.grad, x64.grad, torch.float32)
     for n, p in mixer.named_parameters():
         near(p.grad, params[n].grad, torch.float32)
+
+
+@pytest.mark.parametrize("compute", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kept", [torch.float32, torch.bfloat16, torch.float16])
+def test_norm_weights_keep_their_bits(cuda_device, compute, kept):
+    """Under autocast the norms take the parameters themselves, not a rounded copy."""
+    import nlogn_pisa_b200 as P
+
+    mixer = make(torch.float32)
+    mixer.q_norm.data, mixer.k_norm.data = mixer.q_norm.data.to(kept), mixer.k_norm.data.to(kept)
+    x = torch.randn(2, 130, 256, device="cuda")
+    with torch.autocast("cuda", dtype=compute):
+        got, _ = mixer(x)
+        q, k, v = (getattr(mixer, n)(x).view(2, 130, h, 64) for n, h in (("q_proj", 8), ("k_proj", 2), ("v_proj", 2)))
+        assert q.dtype == compute
+        q, k = P.qk_norm_rotary(q, k, mixer.q_norm.float(), mixer.k_norm.float(), mixer.theta)
+        want = mixer.o_proj(P.full_attention(q, k, v).reshape(2, 130, -1))
+    assert torch.equal(got, want)
+    got.float().square().sum().backward()
+    assert mixer.q_norm.grad.dtype == kept and mixer.k_norm.grad.dtype == kept
+    assert torch.isfinite(mixer.q_norm.grad).all() and bool(mixer.q_norm.grad.any())
