@@ -349,7 +349,7 @@ PISA_API int pisa_rotary(const void *x, int64_t x_sb, int64_t x_st, int64_t x_sh
  * q: [B,T,Hq,D], k: [B,T,H,D] (element strides); weights: D elements each of
  * `weight_dtype` (PISA_F32 or `dtype`); frequency: D/2 fp32; positions as
  * pisa_rotary.  q_out [B,T,Hq,D] and k_out [B,T,H,D] are contiguous.
- * Constraints: D % 8 == 0, D <= 256.
+ * Constraints: D % 8 == 0, D <= 256; eps >= 0 and finite.
  */
 PISA_API int pisa_qk_norm_rotary(const void *q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void *k, int64_t k_sb,
                                  int64_t k_st, int64_t k_sh, const void *q_weight, const void *k_weight,

@@ -30,6 +30,8 @@
 // in flight per warp and CTAs per SM, forward of the first and forward and
 // backward of the second: U = 2 with 4 CTAs (forward) and 2 (backward) as kept;
 // U = 2 with 3: 130 us; U = 3 with 3: 122, 36 and 56 us; U = 4 with 3: 129 us.
+#include <cmath>
+
 #include "dense_tc.cuh"
 
 namespace pisa {
@@ -178,7 +180,8 @@ __device__ __forceinline__ void turn_rows(const NormArgs& a, const NormSide& s, 
       widen<T, V>(x[u][1], x1);
 #pragma unroll
       for (int i = 0; i < V / 2; ++i) sum = tc::fma2(x1[i], x1[i], tc::fma2(x0[i], x0[i], sum));
-      const float inv = rsqrtf(group_sum(sum.x + sum.y, lanes) * inv_d + a.eps);
+      const float size = group_sum(sum.x + sum.y, lanes) * inv_d + a.eps;
+      const float inv = live[u] ? rsqrtf(size) : 0.f;   // rows that are not there add nothing, also with eps 0
       const float2 inv2 = make_float2(inv, inv);
       const float4* cs = reinterpret_cast<const float4*>(table + token[u] * 2 * lanes * V) + (active ? c : 0);
       T* op = o_base + int64_t(token[u] * heads + head[u]) * a.D;
@@ -365,7 +368,8 @@ bool rows16(const void* p, int64_t es, int64_t sb, int64_t st, int64_t sh) {
 
 int check(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb, int64_t k_st,
           int64_t k_sh, const void* qw, const void* kw, const float* freq, int dtype, int w_dtype, int64_t B, int64_t T,
-          int64_t Hq, int64_t H, int64_t D) {
+          int64_t Hq, int64_t H, int64_t D, float eps) {
+  if (!(eps >= 0.f) || std::isinf(eps)) return fail(PISA_ERR_INVALID, "eps must be finite and not negative");
   if (dtype < PISA_F32 || dtype > PISA_F16) return fail(PISA_ERR_UNSUPPORTED, "the kernels support FP16, BF16 and FP32");
   if (w_dtype != dtype && w_dtype != PISA_F32) return fail(PISA_ERR_UNSUPPORTED, "norm weights must be FP32 or the tensors' type");
   if (B <= 0 || T <= 0 || Hq <= 0 || H <= 0 || D <= 0) return fail(PISA_ERR_INVALID, "nonempty tensors are required");
@@ -408,7 +412,7 @@ int pisa_qk_norm_rotary(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
                         int64_t position_offset, int dtype, int64_t B, int64_t T, int64_t Hq, int64_t H, int64_t D,
                         float eps, void* q_out, void* k_out, pisa_stream_t stream) {
   int rc = pisa::check(q, q_sb, q_st, q_sh, k, k_sb, k_st, k_sh, q_weight, k_weight, frequency, dtype, weight_dtype, B,
-                       T, Hq, H, D);
+                       T, Hq, H, D, eps);
   if (rc) return rc;
   if (!q_out || !k_out) return pisa::fail(PISA_ERR_INVALID, "q_out and k_out are required");
   pisa::NormArgs a = pisa::make_args(q, q_sb, q_st, q_sh, k, k_sb, k_st, k_sh, q_weight, k_weight,
@@ -431,7 +435,7 @@ int pisa_qk_norm_rotary_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q
                             int64_t H, int64_t D, float eps, void* dq, void* dk, void* dq_weight, void* dk_weight,
                             void* workspace, int64_t workspace_bytes, pisa_stream_t stream) {
   int rc = pisa::check(q, q_sb, q_st, q_sh, k, k_sb, k_st, k_sh, q_weight, k_weight, frequency, dtype, weight_dtype, B,
-                       T, Hq, H, D);
+                       T, Hq, H, D, eps);
   if (rc) return rc;
   if (!dq_out || !dk_out || !dq || !dk || !dq_weight || !dk_weight)
     return pisa::fail(PISA_ERR_INVALID, "the gradients are required");
