@@ -12,10 +12,14 @@ namespace {
 
 int64_t round256(int64_t x) { return (x + 255) / 256 * 256; }
 
-bool rows16(const void* p, int dtype, int64_t sb, int64_t st, int64_t sh) {
+// Rows of a [B, T, H, D] view start on 16 bytes; the stride of a dimension of
+// one element may hold anything.
+bool rows16(const void* p, int dtype, int64_t B, int64_t T, int64_t H, int64_t sb, int64_t st, int64_t sh) {
   const int64_t v = dtype == PISA_F32 ? 4 : 8;
-  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && sb % v == 0 && st % v == 0 && sh % v == 0;
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (B == 1 || sb % v == 0) && (T == 1 || st % v == 0) &&
+         (H == 1 || sh % v == 0);
 }
+bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 int check_common(int dtype, int64_t Hq, int64_t H, int64_t D, int64_t Dv, float scale) {
   if (dtype < PISA_F32 || dtype > PISA_F16) return fail(PISA_ERR_UNSUPPORTED, "the kernels support FP16, BF16 and FP32");
@@ -35,8 +39,8 @@ int check_dense(const DenseAttnArgs& a, int dtype, int64_t B, int64_t Tq, int64_
   if (Tq > most - 4096 || N > most - 4096 || B > most || Hq > 65535 || sequences > most / 2 || B * Tq * Hq > most * 4)
     return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
   if (!a.q || !a.k || !a.v) return fail(PISA_ERR_INVALID, "q, k and v are required");
-  if (!rows16(a.q, dtype, a.q_sb, a.q_st, a.q_sh) || !rows16(a.k, dtype, a.k_sb, a.k_st, a.k_sh) ||
-      !rows16(a.v, dtype, a.v_sb, a.v_st, a.v_sh))
+  if (!rows16(a.q, dtype, B, Tq, Hq, a.q_sb, a.q_st, a.q_sh) || !rows16(a.k, dtype, B, N, H, a.k_sb, a.k_st, a.k_sh) ||
+      !rows16(a.v, dtype, B, N, H, a.v_sb, a.v_st, a.v_sh))
     return fail(PISA_ERR_UNSUPPORTED, "q, k and v rows must be 16-byte aligned");
   if (a.cu_q || a.cu_k) {
     if (!a.cu_q || !a.cu_k || sequences < 1) return fail(PISA_ERR_INVALID, "cumulative lengths of queries and keys are required");
@@ -128,7 +132,7 @@ int pisa_full_attn_fwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, 
   a.D = int(D); a.Dv = int(Dv);
   a.out = out; a.lse = lse;
   a.out_low = dtype == PISA_F32 ? nullptr : out_low;
-  if (!rows16(out, dtype, 0, 0, 0) || !rows16(out_low, dtype, 0, 0, 0))
+  if (!on16(out) || !on16(out_low))
     return fail(PISA_ERR_UNSUPPORTED, "out and out_low must be 16-byte aligned");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (workspace) {
@@ -164,7 +168,7 @@ int pisa_full_attn_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, 
   a.query_offset = query_offset; a.scale = scale; a.causal = causal ? 1 : 0;
   if (int rc = check_dense(a, dtype, B, Tq, Hq, H, D, Dv, N, sequences)) return rc;
   if (!out || !dout || !lse || !dq || !dk || !dv) return fail(PISA_ERR_INVALID, "out, dout, lse and the gradients are required");
-  if (!rows16(out, dtype, 0, 0, 0) || !rows16(dout, dtype, 0, 0, 0) || !rows16(out_low, dtype, 0, 0, 0))
+  if (!on16(out) || !on16(dout) || !on16(out_low))
     return fail(PISA_ERR_UNSUPPORTED, "out, out_low and dout must be 16-byte aligned");
   a.sequences = int(sequences);
   a.B = int(B); a.T = int(Tq); a.N = int(N); a.Hq = int(Hq); a.H = int(H); a.G = int(Hq / H);
@@ -204,8 +208,10 @@ int pisa_prefix_attn(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, co
     return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
   if (B > 1 && Tq > 1 && q_sb != Tq * q_st)
     return fail(PISA_ERR_UNSUPPORTED, "the tokens of q must be a single stride apart over batch and tokens");
-  if (!rows16(q, dtype, q_sb, q_st, q_sh) || !rows16(k, dtype, k_sb, k_st, k_sh) || !rows16(v, dtype, v_sb, v_st, v_sh) ||
-      (prefix > 0 && (!rows16(prefix_k, dtype, 0, pk_st, pk_sh) || !rows16(prefix_v, dtype, 0, pv_st, pv_sh))))
+  if (!rows16(q, dtype, B, Tq, Hq, q_sb, q_st, q_sh) || !rows16(k, dtype, B, capacity, H, k_sb, k_st, k_sh) ||
+      !rows16(v, dtype, B, capacity, H, v_sb, v_st, v_sh) ||
+      (prefix > 0 && (!rows16(prefix_k, dtype, 1, prefix, H, 0, pk_st, pk_sh) ||
+                      !rows16(prefix_v, dtype, 1, prefix, H, 0, pv_st, pv_sh))))
     return fail(PISA_ERR_UNSUPPORTED, "q, k and v rows must be 16-byte aligned");
   const PrefixPlan plan = plan_prefix(B, Tq, Hq, H, D, Dv, capacity, prefix, dtype);
   if ((reinterpret_cast<uintptr_t>(workspace) & 31u) != 0) return fail(PISA_ERR_INVALID, "workspace must be 32-byte aligned");

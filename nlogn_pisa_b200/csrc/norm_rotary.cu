@@ -361,9 +361,11 @@ int dispatch(const NormArgs& a, int64_t B, int dtype, bool bwd, cudaStream_t s) 
   return a.half % 8 ? launch<__half, 4>(a, B, bwd, s) : launch<__half, 8>(a, B, bwd, s);
 }
 
-bool rows16(const void* p, int64_t es, int64_t sb, int64_t st, int64_t sh) {
+// The stride of a dimension of one element may hold anything.
+bool rows16(const void* p, int64_t es, int64_t B, int64_t T, int64_t H, int64_t sb, int64_t st, int64_t sh) {
   const int64_t v = 16 / es;
-  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && sb % v == 0 && st % v == 0 && sh % v == 0;
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (B == 1 || sb % v == 0) && (T == 1 || st % v == 0) &&
+         (H == 1 || sh % v == 0);
 }
 
 int check(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb, int64_t k_st,
@@ -376,11 +378,11 @@ int check(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k
   if (D % 8 || D > 256) return fail(PISA_ERR_UNSUPPORTED, "head_dim must be a multiple of 8 and at most 256");
   if (B * T >= (int64_t(1) << 30) || Hq + H >= (1 << 16)) return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
   constexpr int64_t wide = int64_t(1) << 31;
-  if (q_st >= wide || q_sh >= wide || k_st >= wide || k_sh >= wide)
+  if ((T > 1 && (q_st >= wide || k_st >= wide)) || (Hq > 1 && q_sh >= wide) || (H > 1 && k_sh >= wide))
     return fail(PISA_ERR_UNSUPPORTED, "token and head strides must be below 2^31 elements");
   if (!q || !k || !qw || !kw || !freq) return fail(PISA_ERR_INVALID, "q, k, the weights and frequency are required");
   const int64_t es = dtype == PISA_F32 ? 4 : 2;
-  if (!rows16(q, es, q_sb, q_st, q_sh) || !rows16(k, es, k_sb, k_st, k_sh))
+  if (!rows16(q, es, B, T, Hq, q_sb, q_st, q_sh) || !rows16(k, es, B, T, H, k_sb, k_st, k_sh))
     return fail(PISA_ERR_UNSUPPORTED, "q and k rows must be 16-byte aligned");
   return PISA_OK;
 }

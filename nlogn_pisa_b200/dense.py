@@ -26,7 +26,7 @@ def aligned_rows(t):
         if t.is_contiguous():
             if t.shape[-1] % per == 0:
                 return t
-        elif t.stride(-1) == 1 and all(s % per == 0 and (s > 0 or n == 1) for s, n in zip(t.stride()[:-1], t.shape)):
+        elif t.stride(-1) == 1 and all(n == 1 or (s > 0 and s % per == 0) for s, n in zip(t.stride()[:-1], t.shape)):
             return t
     return t.clone(memory_format=torch.contiguous_format)
 
