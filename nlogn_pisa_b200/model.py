@@ -3,9 +3,9 @@
 The block of the reference's xmixers LLaMA models
 (xmixers/xmixers/models/transformer/llama/modeling_llama.py): pre-norm
 RMSNorm -> PyramidSparseAttention (FullAttention with attention_method
-"full") -> residual, RMSNorm -> SwiGLU FFN -> residual.  Norms, projections and the FFN are ordinary torch operations (GEMMs
-on cuBLAS); the selection and the attention forward/backward run in this
-library.  Used by the benchmark's training configuration (one block,
+"full") -> residual, RMSNorm -> SwiGLU FFN -> residual.  Norms, projections and
+the FFN are ordinary torch operations (GEMMs on cuBLAS); the selection and the
+attention forward/backward run in this library.  Used by the benchmark's training configuration (one block,
 data-parallel over the GPUs of a node).
 """
 
@@ -86,7 +86,8 @@ class DecoderBlock(nn.Module):
 
     def forward(self, tokens, cu_seqlens=None):
         x = self.embed(tokens)
-        a, _ = self.attn(self.norm1(x), cu_seqlens=cu_seqlens)
+        # mixers that know no packed documents are called as before
+        a, _ = self.attn(self.norm1(x), **({} if cu_seqlens is None else {"cu_seqlens": cu_seqlens}))
         x = x + a
         x = x + self.ffn(self.norm2(x))
         return self.norm_out(x)
