@@ -477,6 +477,10 @@ PISA_API int pisa_wait_selftest(int arrive, int64_t max_tries, void *workspace, 
  * mufu[i] = ex2.approx.ftz.f32 of x[i]; device arrays of n floats. */
 PISA_API int pisa_ex2_selftest(const float *x, float *poly, float *mufu, int64_t n, pisa_stream_t stream);
 
+/* Accuracy check of the polynomial 2^x of the full-attention backward:
+ * y[i] = 2^x[i] for x <= 100 (2^-126 below -126, NaN for NaN); device arrays of n floats. */
+PISA_API int pisa_ex2_pair_selftest(const float *x, float *y, int64_t n, pisa_stream_t stream);
+
 /* ---- per-kernel device timing (profiling aid; the reference has no counterpart) ----
  * With timing on, the library records a pair of CUDA events on the launch
  * stream around every launch of the kernels below.  Reading returns the summed

@@ -77,6 +77,7 @@ SIGNATURES = {
     "pisa_workspace_status": (_I, [_P, _P]),
     "pisa_wait_selftest": (_I, [_I, _L, _P, _L, _P]),
     "pisa_ex2_selftest": (_I, [_P, _P, _P, _L, _P]),
+    "pisa_ex2_pair_selftest": (_I, [_P, _P, _L, _P]),
     "pisa_launch_count": (_L, []),
     "pisa_kernel_timing": (_I, [_I]),
     "pisa_kernel_time": (_I, [_I, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_int64)]),

@@ -10,8 +10,7 @@
 // pisa_workspace_status reads it back (one 4-byte copy and a stream
 // synchronisation); pisa_wait_selftest exercises the whole path with a wait
 // on a barrier that nothing ever arrives on.
-#include "internal.h"
-#include "tc.cuh"
+#include "dense_tc.cuh"
 
 namespace pisa {
 
@@ -51,6 +50,15 @@ __global__ void ex2_selftest_kernel(const float* x, float* poly, float* mufu, in
   }
 }
 
+// The polynomial 2^x of the dense attention backward (ex2_pair).
+__global__ void ex2_pair_selftest_kernel(const float* x, float* y, int64_t n) {
+  const int64_t i = (blockIdx.x * int64_t(blockDim.x) + threadIdx.x) * 2;
+  if (i >= n) return;
+  const float2 p = ex2_pair(make_float2(x[i], i + 1 < n ? x[i + 1] : 0.f));
+  y[i] = p.x;
+  if (i + 1 < n) y[i + 1] = p.y;
+}
+
 }  // namespace
 
 }  // namespace pisa
@@ -63,6 +71,15 @@ int pisa_ex2_selftest(const float* x, float* poly, float* mufu, int64_t n, pisa_
   const int64_t pairs = (n + 1) / 2;
   pisa::ex2_selftest_kernel<<<unsigned((pairs + 255) / 256), 256, 0, static_cast<cudaStream_t>(stream)>>>(
       x, poly, mufu, n);
+  PISA_CHECK_LAUNCH();
+  return PISA_OK;
+}
+
+int pisa_ex2_pair_selftest(const float* x, float* y, int64_t n, pisa_stream_t stream) {
+  if (n < 0 || (n > 0 && (!x || !y))) return pisa::fail(PISA_ERR_INVALID, "x and y are required");
+  if (n == 0) return PISA_OK;
+  const int64_t pairs = (n + 1) / 2;
+  pisa::ex2_pair_selftest_kernel<<<unsigned((pairs + 255) / 256), 256, 0, static_cast<cudaStream_t>(stream)>>>(x, y, n);
   PISA_CHECK_LAUNCH();
   return PISA_OK;
 }
