@@ -32,6 +32,7 @@ struct DenseAttnArgs {
   void* out_low;    // same shape: the part of the output that rounding dropped, or null
   float* lse;       // [B, T, Hq] or null
   int* status;      // device status word or null
+  uint32_t tries;   // of a wait (tensor-core forms), from wait_tries
   // backward
   const void* o;    // the forward's output, contiguous
   const void* o_low;  // its dropped part, or null
@@ -42,6 +43,12 @@ struct DenseAttnArgs {
   void* dk;
   void* dv;
 };
+
+// Tries of a wait, a microsecond each: half a second, and more where a wait may
+// last as long as an item of that many tiles (some wait for the whole item
+// before them; a tile takes 1 to 2 us).
+constexpr uint32_t kWaitTries = 1u << 19;
+inline uint32_t wait_tries(int64_t tiles) { return kWaitTries + uint32_t(tiles < (1 << 27) ? 8 * tiles : 1 << 30); }
 
 // Multiprocessors of the current device, asked once per device.
 inline int sm_count() {

@@ -252,14 +252,14 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, 
 }
 
 struct Wait {
-  int* fail;
+  WaitFlag* flag;
   bool ok = true;
   __device__ __forceinline__ bool operator()(uint64_t* bar, int phase) {   // one thread
-    if (ok && !wait_phase(bar, phase, fail)) ok = false;
+    if (ok && !wait_phase(bar, phase, flag)) ok = false;
     return ok;
   }
   // a warp with collective work: it goes on after an expired wait
-  __device__ __forceinline__ void warp(uint64_t* bar, int phase) { ok = wait_phase(bar, phase, fail) && ok; }
+  __device__ __forceinline__ void warp(uint64_t* bar, int phase) { ok = wait_phase(bar, phase, flag) && ok; }
 };
 
 // Launches 2 and 3 run one persistent CTA per SM.  Items come from a counter in
@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
   __shared__ uint64_t s_full, p_full, dp_full, ds_full, done, drained;
   __shared__ Queue<DkvItem> queue;
   __shared__ uint32_t tmem_slot;
-  __shared__ int s_fail;
+  __shared__ WaitFlag s_wait;
   const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
   if (tid == 0) {
     tc::mbar_init(&kv_full, 1);
@@ -364,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
     tc::mbar_init(&done, 1);
     tc::mbar_init(&drained, 1);
     queue.init();
-    s_fail = 0;
+    s_wait.init(a.tries);
     tc::fence_barrier_init();
   }
   if (warp < 4) {
@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
   tc::fence_after_sync();
   const uint32_t tmem = __shfl_sync(kFull, tmem_slot, 0);
   const uint32_t tS = tmem, tP = tmem + 128, tV = tmem + 256, tK = tmem + 256 + DP;
-  Wait wait{&s_fail};
+  Wait wait{&s_wait};
   // tile n of an item: query head h*G + n / per_head, query tile first_tile +
   // n % per_head; one ring position holds its Q (and statistics), the next its dO
 
@@ -416,8 +416,8 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
         }
       }
       if (!wait.ok) {                 // the copies in flight land before the CTA ends
-        if (used) wait_phase(&kv_full, used - 1, &s_fail);
-        for (int x = max(0, pos - L::RING); x < pos; ++x) wait_phase(&full[x % L::RING], x / L::RING, &s_fail);
+        if (used) wait_phase(&kv_full, used - 1, &s_wait);
+        for (int x = max(0, pos - L::RING); x < pos; ++x) wait_phase(&full[x % L::RING], x / L::RING, &s_wait);
       }
     }
     __syncwarp();
@@ -518,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
       }
     }
     if (leader) tc::mma_commit(&drained);
-    wait_phase(&drained, 0, &s_fail);
+    wait_phase(&drained, 0, &s_wait);
     __syncwarp();
   } else {
     const int side = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;   // key row, queries 64*side ..
@@ -604,7 +604,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  if (tid == 0 && s_fail && a.status) atomicExch(a.status, PISA_ERR_TIMEOUT);
+  if (tid == 0 && s_wait.expired && a.status) atomicExch(a.status, PISA_ERR_TIMEOUT);
   if (warp == kMmaWarp) tc::tmem_free(tmem, 512);
 }
 
@@ -646,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
   __shared__ uint64_t s_full[2], dp_full, dp_free, ds_full, done, drained;
   __shared__ Queue<DqItem> queue;
   __shared__ uint32_t tmem_slot;
-  __shared__ int s_fail;
+  __shared__ WaitFlag s_wait;
   const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
   if (tid == 0) {
     tc::mbar_init(&q_full, 1);
@@ -664,7 +664,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
     tc::mbar_init(&done, 1);
     tc::mbar_init(&drained, 1);
     queue.init();
-    s_fail = 0;
+    s_wait.init(a.tries);
     tc::fence_barrier_init();
   }
   if (warp == kMmaWarp) tc::tmem_alloc(&tmem_slot, 512);
@@ -673,7 +673,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
   tc::fence_after_sync();
   const uint32_t tmem = __shfl_sync(kFull, tmem_slot, 0);
   const uint32_t tS = tmem, tP = tmem + 256, tQ = tmem + 384;   // two S, whose dS overwrites it; dP; dQ
-  Wait wait{&s_fail};
+  Wait wait{&s_wait};
 
   if (warp == kLoadWarp) {
     if (lane == 0) {
@@ -699,8 +699,8 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
         }
       }
       if (!wait.ok) {   // the copies in flight land before the CTA ends
-        if (used) wait_phase(&q_full, used - 1, &s_fail);
-        for (int x = max(0, pos - L::RING); x < pos; ++x) wait_phase(&full[x % L::RING], x / L::RING, &s_fail);
+        if (used) wait_phase(&q_full, used - 1, &s_wait);
+        for (int x = max(0, pos - L::RING); x < pos; ++x) wait_phase(&full[x % L::RING], x / L::RING, &s_wait);
       }
     }
     __syncwarp();
@@ -781,7 +781,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
       }
     }
     if (leader) tc::mma_commit(&drained);
-    wait_phase(&drained, 0, &s_fail);
+    wait_phase(&drained, 0, &s_wait);
     __syncwarp();
   } else {
     const int side = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;   // query row, keys 64*side ..
@@ -861,7 +861,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  if (tid == 0 && s_fail && a.status) atomicExch(a.status, PISA_ERR_TIMEOUT);
+  if (tid == 0 && s_wait.expired && a.status) atomicExch(a.status, PISA_ERR_TIMEOUT);
   if (warp == kMmaWarp) tc::tmem_free(tmem, 512);
 }
 
@@ -900,6 +900,9 @@ int64_t dense_bwd_workspace(bool packed, int dtype, int64_t B, int64_t T, int64_
 int dense_attn_bwd_tc(const DenseAttnArgs& d, int dtype, cudaStream_t stream) {
   BwdTcArgs a{};
   a.d = d;
+  // an item of dK/dV visits the query tiles of a whole group, one of dQ the key tiles
+  const int64_t q_tiles = (int64_t(d.T) + kRows - 1) / kRows * d.G, k_tiles = (int64_t(d.N) + kRows - 1) / kRows;
+  a.d.tries = wait_tries(q_tiles > k_tiles ? q_tiles : k_tiles);
   a.bf16 = dtype == PISA_BF16;
   a.stats = d.delta;
   a.q_slots = seq_slots(d.cu_q, d.B, d.T, d.sequences, kRows);

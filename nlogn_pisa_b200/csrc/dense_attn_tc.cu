@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
   __shared__ int s_listed[2];
   __shared__ Work s_work[2];
   __shared__ uint32_t tmem_slot;
-  __shared__ int s_fail;
+  __shared__ WaitFlag s_wait;
   const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
       tc::mbar_init(&kv_empty[i], 1);
     }
     tc::mbar_init(&drained, 1);
-    s_fail = 0;
+    s_wait.init(a.tries);
     tc::fence_barrier_init();
   }
   if (warp == kMmaWarp) tc::tmem_alloc(&tmem_slot, 512);
@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
   bool ok = true;
   // the next item (every lane of the calling warp), handed back when read
   auto take = [&](int n) {
-    ok = wait_phase(&w_full[n & 1], n >> 1, &s_fail) && ok;
+    ok = wait_phase(&w_full[n & 1], n >> 1, &s_wait) && ok;
     Work w = s_work[n & 1];
     __syncwarp();
     if (lane == 0 && ok) tc::mbar_arrive(&w_empty[n & 1]);
@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
       for (int j = from; j < most; ++j) {
         if (!w.hides(j)) continue;
         const int st = (loads + j + 1) % L::STAGES;
-        ok = wait_phase(&kv_raw[st], int(uses >> st), &s_fail) && ok;
+        ok = wait_phase(&kv_raw[st], int(uses >> st), &s_wait) && ok;
         uses ^= 1u << st;
         if (!__all_sync(kFull, ok)) return;
         if (silence<T, DP>(kv_addr + st * 2 * L::BYTES, max(0, w.seen_by_all(j) - j * kRows), w.t.k_len - j * kRows,
@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
           w.seen[i] = last_visible(a, w.t, first) + 1;
         }
       }
-      ok = wait_phase(&w_empty[n & 1], (n >> 1) + 1, &s_fail) && ok;
+      ok = wait_phase(&w_empty[n & 1], (n >> 1) + 1, &s_wait) && ok;
       if (!__all_sync(kFull, ok)) w.hq = -1;
       if (lane == 0) {
         s_work[n & 1] = w;
@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
 #pragma unroll 1
             for (int i = 0; i < 2; ++i) {
               if (!w.tiles[i]) continue;
-              ok = wait_phase(&q_empty[i], uses[i] + 1, &s_fail) && ok;
+              ok = wait_phase(&q_empty[i], uses[i] + 1, &s_wait) && ok;
               if (!ok) break;
               ++uses[i];
               tc::mbar_arrive_expect_tx(&q_full[i], L::BYTES);
@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
                                 w.t.q_begin + (w.t.tile * 2 + i) * kRows, w.t.b, &q_full[i]);
             }
           }
-          ok = ok && wait_phase(&kv_empty[st], int(phase) + 1, &s_fail);
+          ok = ok && wait_phase(&kv_empty[st], int(phase) + 1, &s_wait);
           if (!ok) break;
           const uint32_t v = kv_addr + st * 2 * L::BYTES, k = v + L::BYTES;
           const bool unchecked = j > 0 && w.hides(j - 1);
@@ -348,11 +348,11 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
       // been handed back (after an expired wait: the copies in flight have landed)
       for (int x = max(0, loads - L::STAGES); x < loads; ++x) {
         const int y = x % L::STAGES;
-        if (!ok && (raw >> y & 1)) wait_phase(&kv_raw[y], int(raws >> y & 1) + 1, &s_fail);
-        else wait_phase(ok ? &kv_empty[y] : &kv_full[y], x / L::STAGES, &s_fail);
+        if (!ok && (raw >> y & 1)) wait_phase(&kv_raw[y], int(raws >> y & 1) + 1, &s_wait);
+        else wait_phase(ok ? &kv_empty[y] : &kv_full[y], x / L::STAGES, &s_wait);
       }
       for (int i = 0; i < 2; ++i)
-        if (uses[i]) wait_phase(ok ? &q_empty[i] : &q_full[i], uses[i] - 1, &s_fail);
+        if (uses[i]) wait_phase(ok ? &q_empty[i] : &q_full[i], uses[i] - 1, &s_wait);
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
@@ -373,12 +373,12 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
       if (w.hq < 0) break;
       const int most = w.most();
       if (most == 0) continue;
-      ok = wait_phase(&kv_full[st], int(phase), &s_fail) && ok;   // K_0
+      ok = wait_phase(&kv_full[st], int(phase), &s_wait) && ok;   // K_0
 #pragma unroll 1
       for (int i = 0; i < 2; ++i) {
         const int own = i ? w.tiles[1] : w.tiles[0];
         if (own == 0) continue;
-        ok = wait_phase(&q_full[i], i ? uses[1] : uses[0], &s_fail) && ok;
+        ok = wait_phase(&q_full[i], i ? uses[1] : uses[0], &s_wait) && ok;
         tc::fence_after_sync();
         if (leader && ok) {
           mma_rows<DP>(tS + i * 128, q_addr + i * L::BYTES, kv_addr + (2 * st + 1) * L::BYTES, id_s);
@@ -391,17 +391,17 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
       // the tiles' O of the item before has been read out
       for (int i = 0; i < 2; ++i) {
         if (w.tiles[i] == 0) continue;
-        if (uses[i] > 0) ok = wait_phase(&o_free[i], uses[i] - 1, &s_fail) && ok;
+        if (uses[i] > 0) ok = wait_phase(&o_free[i], uses[i] - 1, &s_wait) && ok;
         ++uses[i];
       }
       for (int j = 1; j <= most && __all_sync(kFull, ok); ++j) {
         const uint32_t v = kv_addr + st * 2 * L::BYTES, k = v + L::BYTES;
-        ok = wait_phase(&kv_full[st], int(phase), &s_fail) && ok;      // V_{j-1} and K_j
+        ok = wait_phase(&kv_full[st], int(phase), &s_wait) && ok;      // V_{j-1} and K_j
 #pragma unroll 1
         for (int i = 0; i < 2; ++i) {
           const int own = i ? w.tiles[1] : w.tiles[0];
           if (j > own) continue;
-          ok = wait_phase(&p_full[i], int(p_phase >> i), &s_fail) && ok;
+          ok = wait_phase(&p_full[i], int(p_phase >> i), &s_wait) && ok;
           p_phase ^= 1u << i;
           tc::fence_after_sync();
           if (leader && ok) {
@@ -421,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
     }
     if (!__all_sync(kFull, ok)) {
       if (leader) tc::mma_commit(&drained);
-      wait_phase(&drained, 0, &s_fail);
+      wait_phase(&drained, 0, &s_wait);
     }
     __syncwarp();
   } else {
@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
     int step = 0, done = 0;                          // score tiles and items of this query tile so far
     for (int n = 0;; ++n) {
       // the item stays in shared memory while it is worked on: registers are short
-      ok = wait_phase(&w_full[n & 1], n >> 1, &s_fail) && ok;
+      ok = wait_phase(&w_full[n & 1], n >> 1, &s_wait) && ok;
       const Work& w = s_work[n & 1];
       if (w.hq < 0 || !__all_sync(kFull, ok)) break;
       int last, own, full;                           // full: key tiles that every row sees whole
@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
       }
       float m = -INFINITY, l = 0.f;                  // base-2 logits; l: of this half's keys
       for (int j = 0; j < own; ++j, ++step) {
-        ok = wait_phase(&s_full[i], step, &s_fail) && ok;
+        ok = wait_phase(&s_full[i], step, &s_wait) && ok;
         tc::fence_after_sync();
         softmax_half<T, DP>(ts, to, sl, j == 0, j >= full ? last - j * kRows : kRows, 1 + i, s_other[i], half, row, m, l);
         tmem_wait_st();
@@ -455,13 +455,13 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
         if (lane == 0) tc::mbar_arrive(&p_full[i]);
       }
       if (own > 0) {
-        ok = wait_phase(&o_done[i], done++, &s_fail) && ok;
+        ok = wait_phase(&o_done[i], done++, &s_wait) && ok;
         tc::fence_after_sync();
         s_other[i][half][row] = l;
         tc::named_sync(1 + i, 256);
         l += s_other[i][half ^ 1][row];
       }
-      ok = wait_phase(&checked[n & 1], n >> 1, &s_fail) && ok;
+      ok = wait_phase(&checked[n & 1], n >> 1, &s_wait) && ok;
       const bool listed = s_listed[n & 1];
       const SeqTile t = w.t;
       const int hq = w.hq, qi = (t.tile * 2 + i) * kRows + row;   // query of this thread
@@ -519,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  if (tid == 0 && s_fail && a.status) atomicExch(a.status, PISA_ERR_TIMEOUT);
+  if (tid == 0 && s_wait.expired && a.status) atomicExch(a.status, PISA_ERR_TIMEOUT);
   if (warp == kMmaWarp) tc::tmem_free(tmem, 512);
 }
 
@@ -544,6 +544,7 @@ bool dense_attn_tc_eligible(const DenseAttnArgs& a, int dtype) {
 int dense_attn_fwd_tc(const DenseAttnArgs& d, int dtype, cudaStream_t stream) {
   FwdTcArgs a{};
   a.d = d;
+  a.d.tries = wait_tries((int64_t(d.N) + kRows - 1) / kRows);
   a.bf16 = dtype == PISA_BF16;
   int rc = dense_tensor_map(&a.tm_q, d.q, dtype, d.B, d.T, d.Hq, d.D, d.q_sb, d.q_st, d.q_sh, kRows);
   if (rc == PISA_OK) rc = dense_tensor_map(&a.tm_k, d.k, dtype, d.B, d.N, d.H, d.D, d.k_sb, d.k_st, d.k_sh, kRows);

@@ -50,31 +50,43 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
   return v;
 }
 
-// Waits for the phase with parity `phase & 1` of `bar`, half a second at most
-// (tries that suspend a microsecond each).  An expired wait sets *fail and
-// returns false, as does a wait of a CTA whose *fail is set.  Warps with
+// A CTA's waits: whether one of them has expired, and how many tries (of a
+// microsecond each) any of them makes.
+struct WaitFlag {
+  int expired;
+  uint32_t tries;
+  __device__ __forceinline__ void init(uint32_t most = kWaitTries) {
+    expired = 0;
+    tries = most;
+  }
+};
+
+// Waits for the phase with parity `phase & 1` of `bar`, flag->tries
+// microseconds at most (tries that suspend a microsecond each).  An expired wait
+// sets flag->expired and returns false, as does a wait of a CTA whose flag is set.  Warps with
 // collective work do not leave their loops on a false result, which their
 // lanes need not share: they go on, store NaN, and each further wait is short.
-static __device__ __noinline__ bool wait_long(uint32_t addr, uint32_t parity, int* fail) {
+static __device__ __noinline__ bool wait_long(uint32_t addr, uint32_t parity, WaitFlag* flag) {
+  const uint32_t tries = flag->tries;
 #pragma unroll 1
-  for (uint32_t i = 0; i < (1u << 19); ++i) {
+  for (uint32_t i = 0; i < tries; ++i) {
     uint32_t done;
     asm volatile(
         "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\tselp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(done) : "r"(addr), "r"(parity) : "memory");
     if (done) return true;
-    if ((i & 255) == 255 && *static_cast<volatile int*>(fail)) return false;
+    if ((i & 255) == 255 && *static_cast<volatile int*>(&flag->expired)) return false;
   }
-  *static_cast<volatile int*>(fail) = 1;
+  *static_cast<volatile int*>(&flag->expired) = 1;
   return false;
 }
-__device__ __forceinline__ bool wait_phase(uint64_t* bar, int phase, int* fail) {
+__device__ __forceinline__ bool wait_phase(uint64_t* bar, int phase, WaitFlag* flag) {
   const uint32_t addr = tc::smem_u32(bar), parity = uint32_t(phase & 1);
   uint32_t done;
   asm volatile(
       "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(done) : "r"(addr), "r"(parity) : "memory");
-  return done ? true : wait_long(addr, parity, fail);
+  return done ? true : wait_long(addr, parity, flag);
 }
 
 // True in one lane of a converged warp.  The MMA warps run their control flow

@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_stream_kernel(const __grid
   __shared__ uint64_t full[L::STAGES], empty[L::STAGES];
   __shared__ int table[kTable + 1];
   __shared__ int ctas;                         // that take items: the others find the prefix's tiles on their SM
-  __shared__ int s_fail;
+  __shared__ WaitFlag s_wait;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   cudaTriggerProgrammaticLaunchCompletion();   // the joining launch may be scheduled
   // half a second before any wait can expire
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_stream_kernel(const __grid
       tc::mbar_init(&full[i], 1);
       tc::mbar_init(&empty[i], 4);
     }
-    s_fail = 0;
+    s_wait.init();
     tc::fence_barrier_init();
   }
   __syncthreads();
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_stream_kernel(const __grid
         const CUtensorMap* mv = x.prefix ? &args.tm_pv : &args.tm_v;
         for (int j = x.begin; j < x.end; j += kTile, ++n) {
           const int st = n % L::STAGES;
-          if (!wait_phase(&empty[st], (n / L::STAGES) + 1, &s_fail)) { ok = false; break; }
+          if (!wait_phase(&empty[st], (n / L::STAGES) + 1, &s_wait)) { ok = false; break; }
           tc::mbar_arrive_expect_tx(&full[st], L::STAGE);
           const uint32_t k = base + st * L::STAGE, v = k + L::OPERAND;
 #pragma unroll
@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_stream_kernel(const __grid
       }
       // after an expired wait: the copies in flight land before the CTA ends
       if (!ok)
-        for (int x = max(0, n - L::STAGES); x < n; ++x) wait_phase(&full[x % L::STAGES], x / L::STAGES, &s_fail);
+        for (int x = max(0, n - L::STAGES); x < n; ++x) wait_phase(&full[x % L::STAGES], x / L::STAGES, &s_wait);
     }
   } else {
     const int g = lane >> 2, t = lane & 3, sub = warp & 3, side = warp >> 2;   // 16 keys of the CTA's even or odd tiles
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_stream_kernel(const __grid
       const int tiles = (x.end - x.begin + kTile - 1) / kTile;
       for (int u = (n ^ side) & 1; u < tiles; u += 2) {   // tiles n + u of this side's parity
         const int st = (n + u) % L::STAGES;
-        ok = wait_phase(&full[st], (n + u) / L::STAGES, &s_fail) && ok;
+        ok = wait_phase(&full[st], (n + u) / L::STAGES, &s_wait) && ok;
         const uint32_t kt = base + st * L::STAGE + sub * 16 * 128, vt = kt + L::OPERAND;
         const int j = x.begin + u * kTile + sub * 16;      // first key of this warp
         if (j < x.end) {
@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_stream_kernel(const __grid
     }
   }
   __syncthreads();
-  if (tid == 0 && s_fail) atomicExch(a.status, PISA_ERR_TIMEOUT);
+  if (tid == 0 && s_wait.expired) atomicExch(a.status, PISA_ERR_TIMEOUT);
   // scheduled while the prefix's tiles drain, whose partials the joining launch
   // reads too: this kernel ends after that one
   cudaGridDependencySynchronize();

@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
   __shared__ float2 join_ml[kRows];
   __shared__ int64_t s_own[kThreads / 32];
   __shared__ uint32_t tmem_slot;
-  __shared__ int s_fail;
+  __shared__ WaitFlag s_wait;
   const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
   cudaTriggerProgrammaticLaunchCompletion();   // the own caches' kernel may be scheduled
   // half a second before any wait can expire
@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
       tc::mbar_init(&kv_empty[i], 1);
     }
     tc::mbar_init(&drained, 1);
-    s_fail = 0;
+    s_wait.init();
     tc::fence_barrier_init();
   }
   if (warp == kMmaWarp) tc::tmem_alloc(&tmem_slot, 512);
@@ -117,9 +117,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
       }
       for (int n = 0; n < 2 * keys; ++n) {   // K0 V0 K1 V1 ...
         const int st = n % L::STAGES;
-        if (!wait_phase(&kv_empty[st], (n / L::STAGES) + 1, &s_fail)) {
+        if (!wait_phase(&kv_empty[st], (n / L::STAGES) + 1, &s_wait)) {
           // the copies in flight land before the CTA ends
-          for (int x = max(0, n - L::STAGES); x < n; ++x) wait_phase(&kv_full[x % L::STAGES], x / L::STAGES, &s_fail);
+          for (int x = max(0, n - L::STAGES); x < n; ++x) wait_phase(&kv_full[x % L::STAGES], x / L::STAGES, &s_wait);
           break;
         }
         tc::mbar_arrive_expect_tx(&kv_full[st], L::BYTES);
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
     const bool leader = elect_one();
     const uint32_t id_s = tc::idesc_f16(kRows, kRows, args.bf16), id_o = tc::idesc_f16(kRows, DP, args.bf16, 1);
     bool ok = true;
-    auto wait = [&](uint64_t* bar, int phase) { ok = wait_phase(bar, phase, &s_fail) && ok; };
+    auto wait = [&](uint64_t* bar, int phase) { ok = wait_phase(bar, phase, &s_wait) && ok; };
     const int last = steps[1] ? 1 : 0;            // the half that hands a shared stage back
     for (int s = 0; s <= most && __all_sync(kFull, ok); ++s) {
 #pragma unroll 1
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
     }
     if (!__all_sync(kFull, ok)) {
       if (leader) tc::mma_commit(&drained);
-      wait_phase(&drained, 0, &s_fail);
+      wait_phase(&drained, 0, &s_wait);
     }
     __syncwarp();
   } else {
@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int s = 0; s < steps[i]; ++s) {
-      ok = wait_phase(&s_full[i], s, &s_fail) && ok;
+      ok = wait_phase(&s_full[i], s, &s_wait) && ok;
       tc::fence_after_sync();
       const int first = begin + (dual ? 2 * s + i : s) * kRows;
       softmax_tile<T, DP>(ts, to, sl, s == 0, end - 1 - first, m, l);
@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&p_full[i]);
     }
-    if (steps[i]) ok = wait_phase(&o_done[i], 0, &s_fail) && ok;
+    if (steps[i]) ok = wait_phase(&o_done[i], 0, &s_wait) && ok;
     tc::fence_after_sync();
     if (!ok) l = NAN;
     // half 1's result joins half 0's when they hold the same rows
@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
     if (dual) {
       if (i == 1) {
         // the ring is free once half 0's last product is done, too
-        if (!wait_phase(&o_done[0], 0, &s_fail)) l = NAN;
+        if (!wait_phase(&o_done[0], 0, &s_wait)) l = NAN;
         if (steps[1]) {
 #pragma unroll
           for (int c = 0; c < DP; c += 32) {
@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  if (tid == 0 && s_fail) atomicExch(a.status, PISA_ERR_TIMEOUT);
+  if (tid == 0 && s_wait.expired) atomicExch(a.status, PISA_ERR_TIMEOUT);
   if (warp == kMmaWarp) tc::tmem_free(tmem, 512);
 }
 
