@@ -34,6 +34,11 @@
 // of the item may see; the rows that do add them again in fp32 when they are
 // stored.  That is at most 256 keys per row, whatever the length.
 //
+// The tensor core's fp32 accumulator truncates: over many keys of like weight
+// the output falls short, by about 1e-4 of itself at 65536 keys, 0.002 at a
+// million and 0.17 at 2^26.  Every 65536 keys O therefore moves from TMEM into fp32
+// workspace, summed there on the FMA pipes.
+//
 // Measured: one prompt of 16384, 32 query and 8 key heads of 128: 1685 us, 1305
 // TFLOP/s; a training block of four sequences of 4096, 16 heads of 64: 204 us,
 // 674 TFLOP/s.  A step of both tiles (128 keys) takes about 3170 cycles at 128
@@ -50,6 +55,7 @@ namespace {
 
 constexpr int kSoftWarps = 16, kMmaWarp = 16, kLoadWarp = 17, kPlanWarp = 18;
 constexpr int kThreads = 608;
+constexpr int kKeepTiles = 512;              // key tiles after which O leaves TMEM
 constexpr int kListWords = 3 * kRows / 32;   // the key tiles of an item that hide keys: three at most
 
 struct FwdTcArgs {
@@ -116,6 +122,29 @@ __device__ __noinline__ void add_listed(const DenseAttnArgs& a, const SeqTile& t
   }
 }
 
+// This thread's place in the workspace of outputs on their way: W columns and
+// the row's maximum (base 2) that they refer to.
+template <int W> __device__ __forceinline__ float* kept_at(const DenseAttnArgs& a, int i, int half, int row) {
+  return a.kept + (((int64_t(blockIdx.x) * 2 + i) * kRows + row) * 2 + half) * (W + 4);
+}
+__device__ __forceinline__ float kept_factor(const float* at, int w, float m) { return at[w] == m ? 1.f : exp2f(at[w] - m); }
+
+// Adds W columns of O (TMEM `to`) with row maximum m to the workspace and clears them; one warp.
+template <int W> __device__ __noinline__ void keep(uint32_t to, float* at, bool first, float m) {
+  const float f = first ? 0.f : kept_factor(at, W, m);
+#pragma unroll 1
+  for (int c = 0; c < W; c += 16) {
+    float o[16];
+    const uint32_t zero[16] = {};
+    tc::tmem_ld16(to + c, o);
+    tmem_st16(to + c, zero);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) at[c + e] = first ? o[e] : fmaf(at[c + e], f, o[e]);
+  }
+  at[W] = m;
+  tmem_wait_st();
+}
+
 // One work item: the pair of query tiles of one head.  The scheduler warp hands
 // items out one ahead of their use.
 struct Work {
@@ -173,7 +202,9 @@ __device__ __forceinline__ bool silence(uint32_t tile, int first, int real, uint
   return changed;
 }
 
-template <typename T, int DP>
+// KEEP: a sequence may pass 65536 keys (a kernel of its own: the code beside
+// the steps costs short sequences 3 %).
+template <typename T, int DP, bool KEEP>
 __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_constant__ FwdTcArgs args) {
   using L = FwdTile<DP>;
   const DenseAttnArgs& a = args.d;
@@ -448,6 +479,9 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
       for (int j = 0; j < own; ++j, ++step) {
         ok = wait_phase(&s_full[i], step, &s_wait) && ok;
         tc::fence_after_sync();
+        if constexpr (KEEP) {                        // with these scores, O of the tiles before is complete
+          if (j > 0 && j % kKeepTiles == 0) keep<W>(to, kept_at<W>(a, i, half, row), j == kKeepTiles, m);
+        }
         softmax_half<T, DP>(ts, to, sl, j == 0, j >= full ? last - j * kRows : kRows, 1 + i, s_other[i], half, row, m, l);
         tmem_wait_st();
         tc::fence_before_sync();
@@ -481,6 +515,14 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
         } else {
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[e] = 0.f;
+        }
+        if constexpr (KEEP) {
+          if (own > kKeepTiles) {
+            const float* at_kept = kept_at<W>(a, i, half, row);
+            const float f = kept_factor(at_kept, W, m);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = fmaf(at_kept[c + e], f, o[e]);
+          }
         }
         if (listed && real && l != 0.f) {
           float x[16];
@@ -523,19 +565,29 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
   if (warp == kMmaWarp) tc::tmem_free(tmem, 512);
 }
 
-template <typename T, int DP>
-int fwd_t(FwdTcArgs a, cudaStream_t s) {
+template <typename T, int DP, bool KEEP>
+int fwd_keep(FwdTcArgs a, cudaStream_t s) {
   using L = FwdTile<DP>;
   const int64_t items = seq_slots(a.d.cu_q, a.d.B, a.d.T, a.d.sequences, 2 * kRows) * a.d.Hq;
   if (items >= (int64_t(1) << 30)) return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
   a.items = int(items);
-  if (int rc = allow_smem<dense_fwd_tc_kernel<T, DP>>(L::SMEM, "dense attention smem attribute")) return rc;
-  dense_fwd_tc_kernel<T, DP><<<unsigned(min64(items, sm_count())), kThreads, L::SMEM, s>>>(a);
+  if (int rc = allow_smem<dense_fwd_tc_kernel<T, DP, KEEP>>(L::SMEM, "dense attention smem attribute")) return rc;
+  dense_fwd_tc_kernel<T, DP, KEEP><<<unsigned(min64(items, sm_count())), kThreads, L::SMEM, s>>>(a);
   PISA_CHECK_LAUNCH();
   return PISA_OK;
 }
 
+template <typename T, int DP>
+int fwd_t(const FwdTcArgs& a, cudaStream_t s) {
+  return a.d.kept ? fwd_keep<T, DP, true>(a, s) : fwd_keep<T, DP, false>(a, s);
+}
+
 }  // namespace
+
+int64_t dense_fwd_kept_bytes(int64_t N, int64_t D, int64_t Dv) {
+  if (N <= int64_t(kKeepTiles) * kRows) return 0;
+  return int64_t(sm_count()) * 2 * kRows * 2 * ((D <= 64 && Dv <= 64 ? 32 : 64) + 4) * int64_t(sizeof(float));
+}
 
 bool dense_attn_tc_eligible(const DenseAttnArgs& a, int dtype) {
   return dtype != PISA_F32 && a.D <= 128 && a.Dv <= 128;

@@ -106,16 +106,17 @@ def _forward(q, k, v, cu_q, cu_k, offset, scale, causal, want_lse, want_low=Fals
     # what rounding the output to 16 bits dropped, for the backward's row products
     low = torch.empty_like(out) if want_low and q.dtype != torch.float32 else None
     library, code, packing = _lib.lib(), _lib.DTYPES[q.dtype], _packing(cu_q, cu_k)
-    # the workspace holds only the status word: passed when it will be read
+    # up to 65536 keys the workspace holds only the status word: passed when it will be read
     workspace, size = None, 0
-    if _lib.status_checks():
-        size = library.pisa_full_attn_fwd_workspace_bytes(batch, tokens, q_heads, heads, dim, dim_v, length, packing[3], code)
+    if _lib.status_checks() or length > 65536:
+        size = _lib.workspace_bytes("pisa_full_attn_fwd_workspace_bytes", q.get_device(), batch, tokens, q_heads, heads, dim,
+                                    dim_v, length, packing[3], code)
         workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
     _lib.launch(library.pisa_full_attn_fwd, q.get_device(), *view(q), *view(k), *view(v), *packing, offset, code, batch,
                 tokens, q_heads, heads, dim, dim_v, length, scale, int(causal), out.data_ptr(),
                 None if low is None else low.data_ptr(), None if lse is None else lse.data_ptr(),
                 None if workspace is None else workspace.data_ptr(), size)
-    if workspace is not None:
+    if _lib.status_checks():
         _lib.check_workspace(workspace, q.device)
     return out, lse, low
 
