@@ -83,7 +83,8 @@ PrefixPlan plan_prefix(int64_t B, int64_t T, int64_t Hq, int64_t H, int64_t D, i
     // more than 16 query rows per KV head: tiles of 128 rows, else the stream
     p.tiles = P > 0 && B * T * G > 16 && G <= 128;
     const int64_t tokens = p.tiles ? 128 / G : 1, tiles = (B * T + tokens - 1) / tokens;
-    if (p.tiles) p.prefix_splits = ranges(P, std::max<int64_t>(1, sms / (H * ((tiles + 1) / 2))), 128, &p.prefix_chunk);
+    if (p.tiles)
+      p.prefix_splits = ranges(P, std::max<int64_t>(least_ranges(P), sms / (H * ((tiles + 1) / 2))), 128, &p.prefix_chunk);
     else if (P > 0) p.prefix_splits = stream(P, H * ((B * T * G + 15) / 16), &p.prefix_chunk);
   } else {
     auto count = [&](int64_t items) { return (2 * sms + items - 1) / items; };

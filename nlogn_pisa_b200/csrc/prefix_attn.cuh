@@ -35,6 +35,10 @@ struct PrefixArgs {
   int tile_ctas, sms;
 };
 
+// Key ranges that a prefix in 128-row tiles needs: the tensor core's accumulator
+// truncates, and passes 1e-4 of its sum over 65536 keys of like weight.
+__host__ __device__ __forceinline__ int least_ranges(int64_t keys) { return int((keys + 65535) / 65536); }
+
 __device__ __forceinline__ int own_length(const PrefixArgs& a, int b) {
   const int64_t n = a.len_bytes == 4 ? int64_t(static_cast<const int32_t*>(a.lengths)[b])
                                      : static_cast<const int64_t*>(a.lengths)[b];
@@ -68,7 +72,7 @@ __device__ __forceinline__ PrefixShare prefix_share(const PrefixArgs& a, int64_t
   const float c = float(a.tile_ctas), b = 5.f * a.sms - c * prefix - own, root = sqrtf(b * b + 20.f * c * prefix * a.sms);
   const int at = int(b > 0.f ? (b + root) / (10.f * c) : 2.f * prefix * a.sms / (root - b));
   for (int i = 0; i < 2; ++i) {
-    const int r = min(max(at + i, 1), a.prefix_splits);
+    const int r = min(max(at + i, least_ranges(a.P)), a.prefix_splits);
     const int rest = a.sms - r * a.tile_ctas;
     if (rest < 1) break;
     const float time = fmaxf(prefix / r + 5.f, own / rest);
