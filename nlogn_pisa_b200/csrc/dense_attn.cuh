@@ -264,7 +264,7 @@ inline int dense_tensor_map(CUtensorMap* map, const void* base, int dtype, int64
 // 16-bit tensors of at most 128 dims: tensor-core kernels
 bool dense_attn_tc_eligible(const DenseAttnArgs& a, int dtype);
 int dense_attn_fwd_tc(const DenseAttnArgs& a, int dtype, cudaStream_t stream);
-// workspace for outputs on their way over more than 65536 keys; 0 for fewer
+// workspace for outputs on their way over more than 8192 keys; 0 for fewer
 int64_t dense_fwd_kept_bytes(int64_t N, int64_t D, int64_t Dv);
 // a.delta: dense_bwd_workspace(...) bytes
 int64_t dense_bwd_workspace(bool packed, int dtype, int64_t B, int64_t T, int64_t N, int64_t Hq, int64_t H, int64_t sequences);

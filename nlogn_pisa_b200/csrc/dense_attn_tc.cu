@@ -35,9 +35,12 @@
 // stored.  That is at most 256 keys per row, whatever the length.
 //
 // The tensor core's fp32 accumulator truncates: over many keys of like weight
-// the output falls short, by about 1e-4 of itself at 65536 keys, 0.002 at a
+// the output falls short, by about 2e-4 of itself at 65536 keys, 0.002 at a
 // million and 0.17 at 2^26.  Every 65536 keys O therefore moves from TMEM into fp32
-// workspace, summed there on the FMA pipes.
+// workspace, summed there on the FMA pipes.  Where a backward follows it does so
+// every 8192 keys: delta inherits the loss, and dQ, a sum whose terms cancel,
+// multiplies it (65536 keys of like weight, k and v with a mean of half their
+// deviation: error of dQ 0.013 of its norm, now 0.002).
 //
 // Measured: one prompt of 16384, 32 query and 8 key heads of 128: 1685 us, 1305
 // TFLOP/s; a training block of four sequences of 4096, 16 heads of 64: 204 us,
@@ -55,13 +58,15 @@ namespace {
 
 constexpr int kSoftWarps = 16, kMmaWarp = 16, kLoadWarp = 17, kPlanWarp = 18;
 constexpr int kThreads = 608;
-constexpr int kKeepTiles = 512;              // key tiles after which O leaves TMEM
+// key tiles after which O leaves TMEM: in inference, and before a backward
+constexpr int kKeepTiles = 512, kKeepTilesTrain = 64;
 constexpr int kListWords = 3 * kRows / 32;   // the key tiles of an item that hide keys: three at most
 
 struct FwdTcArgs {
   CUtensorMap tm_q, tm_k, tm_v;             // boxes of 64 dims x 128 rows of one head
   DenseAttnArgs d;
   int items;                                // slots of query tile pairs x heads
+  int keep_tiles;
   int bf16;
 };
 
@@ -122,16 +127,22 @@ __device__ __noinline__ void add_listed(const DenseAttnArgs& a, const SeqTile& t
   }
 }
 
-// This thread's place in the workspace of outputs on their way: W columns and
-// the row's maximum (base 2) that they refer to.
-template <int W> __device__ __forceinline__ float* kept_at(const DenseAttnArgs& a, int i, int half, int row) {
-  return a.kept + (((int64_t(blockIdx.x) * 2 + i) * kRows + row) * 2 + half) * (W + 4);
+// Workspace of the outputs on their way, by CTA, query tile and half of the
+// columns: [W / 4][128 rows][4], then the row maxima (base 2) that they refer to.
+template <int W> __device__ __forceinline__ float* kept_at(const DenseAttnArgs& a, int i, int half) {
+  return a.kept + ((int64_t(blockIdx.x) * 2 + i) * 2 + half) * kRows * (W + 1);
 }
-__device__ __forceinline__ float kept_factor(const float* at, int w, float m) { return at[w] == m ? 1.f : exp2f(at[w] - m); }
+template <int W> __device__ __forceinline__ float kept_factor(const float* at, int row, float m) {
+  const float of = at[W * kRows + row];
+  return of == m ? 1.f : exp2f(of - m);
+}
+__device__ __forceinline__ float4* kept_columns(float* at, int row, int c) {
+  return reinterpret_cast<float4*>(at + c * kRows + row * 4);
+}
 
 // Adds W columns of O (TMEM `to`) with row maximum m to the workspace and clears them; one warp.
-template <int W> __device__ __noinline__ void keep(uint32_t to, float* at, bool first, float m) {
-  const float f = first ? 0.f : kept_factor(at, W, m);
+template <int W> __device__ __noinline__ void keep(uint32_t to, float* at, int row, bool first, float m) {
+  const float f = first ? 0.f : kept_factor<W>(at, row, m);
 #pragma unroll 1
   for (int c = 0; c < W; c += 16) {
     float o[16];
@@ -139,9 +150,13 @@ template <int W> __device__ __noinline__ void keep(uint32_t to, float* at, bool 
     tc::tmem_ld16(to + c, o);
     tmem_st16(to + c, zero);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) at[c + e] = first ? o[e] : fmaf(at[c + e], f, o[e]);
+    for (int e = 0; e < 16; e += 4) {
+      float4* x = kept_columns(at, row, c + e);
+      const float4 y = first ? make_float4(0.f, 0.f, 0.f, 0.f) : *x;
+      *x = make_float4(fmaf(y.x, f, o[e]), fmaf(y.y, f, o[e + 1]), fmaf(y.z, f, o[e + 2]), fmaf(y.w, f, o[e + 3]));
+    }
   }
-  at[W] = m;
+  at[W * kRows + row] = m;
   tmem_wait_st();
 }
 
@@ -202,8 +217,8 @@ __device__ __forceinline__ bool silence(uint32_t tile, int first, int real, uint
   return changed;
 }
 
-// KEEP: a sequence may pass 65536 keys (a kernel of its own: the code beside
-// the steps costs short sequences 3 %).
+// KEEP: a sequence may pass args.keep_tiles key tiles (a kernel of its own: the
+// code beside the steps costs short sequences 3 %).
 template <typename T, int DP, bool KEEP>
 __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_constant__ FwdTcArgs args) {
   using L = FwdTile<DP>;
@@ -480,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
         ok = wait_phase(&s_full[i], step, &s_wait) && ok;
         tc::fence_after_sync();
         if constexpr (KEEP) {                        // with these scores, O of the tiles before is complete
-          if (j > 0 && j % kKeepTiles == 0) keep<W>(to, kept_at<W>(a, i, half, row), j == kKeepTiles, m);
+          if (j > 0 && (j & (args.keep_tiles - 1)) == 0) keep<W>(to, kept_at<W>(a, i, half), row, j == args.keep_tiles, m);
         }
         softmax_half<T, DP>(ts, to, sl, j == 0, j >= full ? last - j * kRows : kRows, 1 + i, s_other[i], half, row, m, l);
         tmem_wait_st();
@@ -517,11 +532,17 @@ __global__ void __launch_bounds__(kThreads, 1) dense_fwd_tc_kernel(const __grid_
           for (int e = 0; e < 16; ++e) o[e] = 0.f;
         }
         if constexpr (KEEP) {
-          if (own > kKeepTiles) {
-            const float* at_kept = kept_at<W>(a, i, half, row);
-            const float f = kept_factor(at_kept, W, m);
+          if (own > args.keep_tiles) {
+            float* at_kept = kept_at<W>(a, i, half);
+            const float f = kept_factor<W>(at_kept, row, m);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = fmaf(at_kept[c + e], f, o[e]);
+            for (int e = 0; e < 16; e += 4) {
+              const float4 x = *kept_columns(at_kept, row, c + e);
+              o[e] = fmaf(x.x, f, o[e]);
+              o[e + 1] = fmaf(x.y, f, o[e + 1]);
+              o[e + 2] = fmaf(x.z, f, o[e + 2]);
+              o[e + 3] = fmaf(x.w, f, o[e + 3]);
+            }
           }
         }
         if (listed && real && l != 0.f) {
@@ -579,14 +600,14 @@ int fwd_keep(FwdTcArgs a, cudaStream_t s) {
 
 template <typename T, int DP>
 int fwd_t(const FwdTcArgs& a, cudaStream_t s) {
-  return a.d.kept ? fwd_keep<T, DP, true>(a, s) : fwd_keep<T, DP, false>(a, s);
+  return a.d.kept && a.d.N > a.keep_tiles * kRows ? fwd_keep<T, DP, true>(a, s) : fwd_keep<T, DP, false>(a, s);
 }
 
 }  // namespace
 
 int64_t dense_fwd_kept_bytes(int64_t N, int64_t D, int64_t Dv) {
-  if (N <= int64_t(kKeepTiles) * kRows) return 0;
-  return int64_t(sm_count()) * 2 * kRows * 2 * ((D <= 64 && Dv <= 64 ? 32 : 64) + 4) * int64_t(sizeof(float));
+  if (N <= int64_t(kKeepTilesTrain) * kRows) return 0;
+  return int64_t(sm_count()) * 2 * 2 * kRows * ((D <= 64 && Dv <= 64 ? 32 : 64) + 1) * int64_t(sizeof(float));
 }
 
 bool dense_attn_tc_eligible(const DenseAttnArgs& a, int dtype) {
@@ -598,6 +619,7 @@ int dense_attn_fwd_tc(const DenseAttnArgs& d, int dtype, cudaStream_t stream) {
   a.d = d;
   a.d.tries = wait_tries((int64_t(d.N) + kRows - 1) / kRows);
   a.bf16 = dtype == PISA_BF16;
+  a.keep_tiles = d.out_low ? kKeepTilesTrain : kKeepTiles;
   int rc = dense_tensor_map(&a.tm_q, d.q, dtype, d.B, d.T, d.Hq, d.D, d.q_sb, d.q_st, d.q_sh, kRows);
   if (rc == PISA_OK) rc = dense_tensor_map(&a.tm_k, d.k, dtype, d.B, d.N, d.H, d.D, d.k_sb, d.k_st, d.k_sh, kRows);
   if (rc == PISA_OK) rc = dense_tensor_map(&a.tm_v, d.v, dtype, d.B, d.N, d.H, d.Dv, d.v_sb, d.v_st, d.v_sh, kRows);

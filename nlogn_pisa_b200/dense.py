@@ -106,9 +106,9 @@ def _forward(q, k, v, cu_q, cu_k, offset, scale, causal, want_lse, want_low=Fals
     # what rounding the output to 16 bits dropped, for the backward's row products
     low = torch.empty_like(out) if want_low and q.dtype != torch.float32 else None
     library, code, packing = _lib.lib(), _lib.DTYPES[q.dtype], _packing(cu_q, cu_k)
-    # up to 65536 keys the workspace holds only the status word: passed when it will be read
+    # the workspace holds the status word, and over many keys the outputs on their way: passed when either is wanted
     workspace, size = None, 0
-    if _lib.status_checks() or length > 65536:
+    if _lib.status_checks() or length > (65536 if low is None else 8192):
         size = _lib.workspace_bytes("pisa_full_attn_fwd_workspace_bytes", q.get_device(), batch, tokens, q_heads, heads, dim,
                                     dim_v, length, packing[3], code)
         workspace = torch.empty(size, dtype=torch.uint8, device=q.device)

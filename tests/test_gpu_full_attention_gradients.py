@@ -140,3 +140,28 @@ def test_against_differences(cuda_device):
         assert slack <= 0.1 * abs(true)
         assert abs(got[0] - got[1] - along) <= slack + 64 * R.EPS * abs(true)
         assert abs(along - true) <= 64 * R.EPS * abs(true)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("keys,rows,dim", [(8192, 200, 64), (16384, 128, 128), (65536, 300, 64), (65536, 128, 128), (262144, 128, 64)])
+def test_cancelling_sums_over_many_keys(cuda_device, dtype, keys, rows, dim):
+    """dq of near-equal weights and k, v with a mean: an output that is off by e moves dq by e times delta and the mean key."""
+    import nlogn_pisa_b200 as P
+
+    gen = torch.Generator(device="cuda").manual_seed(keys + dim)
+    q = normal(gen, 1, rows, 2, dim, dtype=dtype, size=0.1)
+    k, v = ((0.5 + torch.randn(1, keys, 1, dim, generator=gen, device="cuda")).to(dtype) for _ in range(2))
+    dout = normal(gen, 1, rows, 2, dim, dtype=dtype, size=100.0)
+    leaves = [x.requires_grad_(True) for x in (q, k, v)]
+    dq = torch.autograd.grad(P.full_attention(*leaves, causal=False), leaves, dout)[0]
+    kd, vd, scale = k[0, :, 0].detach().double(), v[0, :, 0].detach().double(), dim ** -0.5
+    for h in range(2):
+        p = torch.softmax(q[0, :, h].detach().double() @ kd.T * scale, -1)
+        d = dout[0, :, h].double()
+        out = p @ vd
+        delta = (d * out).sum(-1, keepdim=True)
+        want = scale * (p * (d @ vd.T - delta)) @ kd
+        # outputs short by 2^-16 of themselves (sums of 8192 keys in a truncating accumulator of 24 bits)
+        off = 2.0 ** -16 * (2 * delta.abs() + (d * out).norm(dim=-1, keepdim=True))
+        slack = float((scale * off * (p @ kd).abs()).norm())
+        assert float((dq[0, :, h].double() - want).norm()) <= room(want, dtype) + slack
