@@ -32,7 +32,7 @@ struct DenseAttnArgs {
   void* out_low;    // same shape: the part of the output that rounding dropped, or null
   float* lse;       // [B, T, Hq] or null
   int* status;      // device status word or null
-  float* kept;      // tensor-core forward: dense_fwd_kept_bytes(...) of workspace, or null
+  float* kept;      // tensor-core forms: workspace of outputs on their way, or null
   uint32_t tries;   // of a wait (tensor-core forms), from wait_tries
   // backward
   const void* o;    // the forward's output, contiguous
@@ -267,7 +267,8 @@ int dense_attn_fwd_tc(const DenseAttnArgs& a, int dtype, cudaStream_t stream);
 // workspace for outputs on their way over more than 8192 keys; 0 for fewer
 int64_t dense_fwd_kept_bytes(int64_t N, int64_t D, int64_t Dv);
 // a.delta: dense_bwd_workspace(...) bytes
-int64_t dense_bwd_workspace(bool packed, int dtype, int64_t B, int64_t T, int64_t N, int64_t Hq, int64_t H, int64_t sequences);
+int64_t dense_bwd_workspace(bool packed, int dtype, int64_t B, int64_t T, int64_t N, int64_t Hq, int64_t H, int64_t D,
+                            int64_t Dv, int64_t sequences);
 int dense_attn_bwd_tc(const DenseAttnArgs& a, int dtype, cudaStream_t stream);
 
 int dense_attn_fwd_simt(const DenseAttnArgs& a, int dtype, cudaStream_t stream);

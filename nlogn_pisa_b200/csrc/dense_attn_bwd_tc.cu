@@ -37,6 +37,12 @@
 // and a warp zeroes the rest of the last step in shared memory first (a weight
 // of zero would not silence an infinite or NaN value).
 //
+// The tensor core's fp32 accumulator truncates, 2e-4 of a sum over 65536 rows of
+// one sign and with their number.  Items of more than 512 tiles therefore come in
+// parts: the sums of a part move from TMEM into fp32 workspace and the last part
+// stores them (1048576 query rows of a KV head: error of dV in fp16 0.003 of its
+// norm, now 0.0003).
+//
 // Measured: four sequences of 4096, 16 heads of 64: statistics 28 us, dK/dV 329
 // us (836 TFLOP/s), dQ 226 us (912); packed documents of 1 to 4096 tokens, 32
 // query and 8 key heads of 128: 54, 305 (1267) and 300 us (967).  At 64 dims the
@@ -60,6 +66,8 @@ constexpr int kThreads = 352;
 // heads of 64: dK/dV 353 us with 0, 345 with 1, 346 with 2, 340 with 3, 348 with
 // 4; dQ 235, 231, 226, 232 and 238.
 constexpr int kPolyKv = 3, kPolyQ = 2;
+
+constexpr int kPart = 512;               // tiles of an item's part
 
 // Statistics of a query tile: -lse (base 2) and -scale * delta (fp16: -delta) of its rows in
 // fp32, then 16 bytes per row for the products of launch 2 (see mma_stat).
@@ -93,6 +101,33 @@ __device__ __forceinline__ float* stat_tile(const BwdTcArgs& a, int hq, int64_t 
 // Factor of the scores in base 2, never quite zero (the statistics are divided by it).
 __device__ __forceinline__ float base2_scale(const DenseAttnArgs& a) {
   return fmaxf(a.scale * kLog2e, 1e-30f);
+}
+
+// This thread's place in the workspace of sums on their way: [columns / 4][128 rows][4] by CTA and side.
+template <int W> __device__ __forceinline__ float* kept_at(const DenseAttnArgs& a, int side, int row) {
+  return a.kept + (int64_t(blockIdx.x) * 2 + side) * kRows * W + row * 4;
+}
+// W columns of a part's sums (TMEM `from`): added to the workspace, and back into TMEM for the last part.  One warp.
+template <int W> __device__ __noinline__ void keep_part(uint32_t from, float* at, bool first, bool last) {
+#pragma unroll 1
+  for (int c = 0; c < W; c += 16) {
+    float o[16];
+    uint32_t r[16];
+    tc::tmem_ld16(from + c, o);
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      float4* x = reinterpret_cast<float4*>(at + (c + e) * kRows);
+      const float4 y = first ? make_float4(0.f, 0.f, 0.f, 0.f) : *x;
+      const float4 sum = make_float4(y.x + o[e], y.y + o[e + 1], y.z + o[e + 2], y.w + o[e + 3]);
+      if (!last) *x = sum;
+      r[e] = __float_as_uint(sum.x);
+      r[e + 1] = __float_as_uint(sum.y);
+      r[e + 2] = __float_as_uint(sum.z);
+      r[e + 3] = __float_as_uint(sum.w);
+    }
+    if (last) tmem_st16(from + c, r);
+  }
+  if (last) tmem_wait_st();
 }
 
 template <typename T> constexpr bool kHalf = std::is_same<T, __half>::value;
@@ -304,6 +339,19 @@ template <typename F> __device__ __forceinline__ bool draw(int n, int items, int
   }
 }
 
+// The next part of item w, of which `left` tiles are left (0: w is a new item).
+template <typename Item> __device__ __forceinline__ void next_part(Item& w, int& left) {
+  if (left == 0) {
+    left = w.head < 0 ? 0 : w.total;
+    w.part_from = 0;
+  } else {
+    w.part_from += w.total;
+  }
+  w.total = min(left, kPart);
+  left -= w.total;
+  w.part_last = left == 0;
+}
+
 // Launch 2.  An item: key tile, KV head.
 struct DkvItem {
   SeqTile t;
@@ -311,6 +359,10 @@ struct DkvItem {
   int first_tile, end_tile;           // query tiles that see a key of the tile
   int per_head, total, tail;          // their number, with all heads of the group; real rows of the last one
   float factor;                       // of dS
+  int part_from;                      // of a part: its first tile (`total` counts the part's)
+  bool part_last;                     // no part follows
+  template <bool PARTS> __device__ __forceinline__ int from() const { return PARTS ? part_from : 0; }
+  template <bool PARTS> __device__ __forceinline__ bool last() const { return !PARTS || part_last; }
 };
 
 template <typename T> __device__ __forceinline__ DkvItem dkv_item(const BwdTcArgs& args, int n) {
@@ -333,7 +385,8 @@ template <typename T> __device__ __forceinline__ DkvItem dkv_item(const BwdTcArg
   return w;
 }
 
-template <typename T, int DP>
+// PARTS: items may pass kPart tiles (kernels of their own: the others have no registers to spare).
+template <typename T, int DP, bool PARTS>
 __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_constant__ BwdTcArgs args) {
   using L = BwdTile<DP>;
   const DenseAttnArgs& a = args.d;
@@ -387,8 +440,11 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
   if (warp == kLoadWarp) {
     if (lane == 0) {
       int pos = 0, used = 0;          // ring position; items with queries so far
+      DkvItem w;
+      int left = 0, drawn = 0;        // tiles of the drawn item that no part took yet; items drawn
       for (int n = 0; wait.ok; ++n) {
-        const DkvItem w = dkv_item<T>(args, n);
+        if (!PARTS || left == 0) w = dkv_item<T>(args, drawn++);
+        if constexpr (PARTS) next_part(w, left);
         queue.put(n, w, wait);
         if (w.head < 0) break;
         if (w.total == 0) continue;
@@ -397,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
         load_tile<DP>(k_addr, &args.tm_k, w.head, w.t.k_begin + w.t.tile * kRows, w.t.b, &kv_full);
         load_tile<DP>(v_addr, &args.tm_v, w.head, w.t.k_begin + w.t.tile * kRows, w.t.b, &kv_full);
         ++used;
-        int g = 0, qt = w.first_tile;
+        int g = w.template from<PARTS>() / w.per_head, qt = w.first_tile + w.template from<PARTS>() % w.per_head;
         for (int i = 0; i < w.total && wait.ok; ++i) {
           const bool ragged = w.tail < kRows && qt + 1 == w.end_tile;
           const int row = w.t.q_begin + qt * kRows, hq = w.head * a.G + g;
@@ -428,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
       const DkvItem w = queue.take(i, wait, lane);
       if (w.head < 0) break;
       if (w.total > 0 && w.tail < kRows) {
-        for (int n = w.per_head - 1; n < w.total; n += w.per_head) {
+        for (int n = w.per_head - 1 - w.template from<PARTS>() % w.per_head; n < w.total; n += w.per_head) {
           for (int x = 0; x < 2; ++x) {
             const int st = (start + 2 * n + x) % L::RING;
             wait.warp(&raw[st], uses >> st);
@@ -473,7 +529,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
         }
         ++used;
       }
-      int left = per_head;            // tiles to the head's last one
+      int left = total > 0 ? per_head - w.template from<PARTS>() % per_head : 0;   // tiles to the head's last one
       for (int n = 0; n < total && __all_sync(kFull, wait.ok); ++n, ++tile) {
         const bool rag = tail < kRows && left == 1;
         left = left == 1 ? per_head : left - 1;
@@ -532,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
       const float factor = kHalf<T> ? w.factor / float(1 << kWeightShift<T>) : w.factor;
       const float2 sc2 = make_float2(factor, factor);
       const int first = first_seeing(a, w.t, j0 + row), whole = first_seeing(a, w.t, j0 + kRows - 1);
-      int qt = w.first_tile;
+      int qt = w.first_tile + (w.total > 0 ? w.template from<PARTS>() % w.per_head : 0);
       for (int n = 0; n < w.total; ++n, ++tile) {
         wait.warp(&s_full, tile);
         tc::fence_after_sync();
@@ -592,8 +648,12 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dkv_tc_kernel(const __grid_
       const int64_t at = (int64_t(w.t.b) * a.N + w.t.k_begin + j0 + quarter * 32) * a.H + w.head;
       T* to = static_cast<T*>(side ? a.dk : a.dv) + at * cols;
       const float rest = !wait.ok ? NAN : side ? grad_rest<T>(args, w.factor) : 1.f / float(1 << kWeightShift<T>);
+      if constexpr (PARTS) {
+        if (w.part_from > 0 || !w.part_last)
+          keep_part<DP>((side ? tK : tV) + lanes, kept_at<DP>(a, side, row), w.part_from == 0, w.part_last);
+      }
 #pragma unroll 1
-      for (int c = 0; c < DP; c += 32) {
+      for (int c = 0; c < DP && w.template last<PARTS>(); c += 32) {
         store_lanes<T, 32>((side ? tK : tV) + lanes + c, w.total == 0, rest, out_addr + warp * 32 * 64, to + c,
                            int64_t(a.H) * cols, rows, cols - c, lane);
         __syncwarp();
@@ -614,6 +674,10 @@ struct DqItem {
   int head;                           // < 0: no item
   int valid, total, tail;             // real rows; key tiles, and the real rows of the last one
   float factor;                       // of dS
+  int part_from;                      // of a part: its first key tile (`total` counts the part's)
+  bool part_last;                     // no part follows
+  template <bool PARTS> __device__ __forceinline__ int from() const { return PARTS ? part_from : 0; }
+  template <bool PARTS> __device__ __forceinline__ bool last() const { return !PARTS || part_last; }
 };
 
 template <typename T> __device__ __forceinline__ DqItem dq_item(const BwdTcArgs& args, int n) {
@@ -635,7 +699,7 @@ template <typename T> __device__ __forceinline__ DqItem dq_item(const BwdTcArgs&
   return w;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool PARTS>
 __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_constant__ BwdTcArgs args) {
   using L = BwdTile<DP>;
   const DenseAttnArgs& a = args.d;
@@ -678,8 +742,11 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
   if (warp == kLoadWarp) {
     if (lane == 0) {
       int pos = 0, used = 0;                    // ring position; items with keys so far
+      DqItem w;
+      int left = 0, drawn = 0;                  // tiles of the drawn item that no part took yet; items drawn
       for (int n = 0; wait.ok; ++n) {
-        const DqItem w = dq_item<T>(args, n);
+        if (!PARTS || left == 0) w = dq_item<T>(args, drawn++);
+        if constexpr (PARTS) next_part(w, left);
         queue.put(n, w, wait);
         if (w.head < 0) break;
         if (w.total <= 0) continue;
@@ -693,9 +760,9 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
           const int st = pos % L::RING;
           if (!wait(&empty[st], (pos / L::RING) + 1)) break;
           // keys of a ragged last tile pass through the trimming warp
-          uint64_t* bar = x == 2 * w.total - 2 && w.tail < kRows ? &raw[st] : &full[st];
+          uint64_t* bar = x == 2 * w.total - 2 && w.template last<PARTS>() && w.tail < kRows ? &raw[st] : &full[st];
           tc::mbar_arrive_expect_tx(bar, L::BYTES);
-          load_tile<DP>(ring + st * L::BYTES, x & 1 ? &args.tm_v : &args.tm_k, h, w.t.k_begin + (x >> 1) * kRows, w.t.b, bar);
+          load_tile<DP>(ring + st * L::BYTES, x & 1 ? &args.tm_v : &args.tm_k, h, w.t.k_begin + (w.template from<PARTS>() + (x >> 1)) * kRows, w.t.b, bar);
         }
       }
       if (!wait.ok) {   // the copies in flight land before the CTA ends
@@ -712,7 +779,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
       if (w.head < 0) break;
       if (w.total <= 0) continue;
       pos += 2 * w.total;
-      if (w.tail >= kRows) continue;
+      if (w.tail >= kRows || !w.template last<PARTS>()) continue;
       const int st = (pos - 2) % L::RING;
       wait.warp(&raw[st], uses >> st);
       uses ^= 1u << st;
@@ -730,7 +797,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
     for (int i = 0;; ++i) {
       const DqItem w = queue.take(i, wait, lane);
       if (w.head < 0) break;
-      const int total = w.total, steps = (w.tail + 15) / 16;
+      const int total = w.total, steps = w.template last<PARTS>() ? (w.tail + 15) / 16 : kRows / 16;
       if (total > 0) {
         wait.warp(&q_full, used);
         wait.warp(&full[st], int(phase));
@@ -824,14 +891,14 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&dp_free);
         uint32_t x[32];
-        const int lim = last - n * kRows - side * 64;
+        const int lim = last - (w.template from<PARTS>() + n) * kRows - side * 64;
 #pragma unroll
         for (int c = 0; c < 64; c += 2) {
           const float2 u = mul2(tc::fma2(make_float2(dp[c], dp[c + 1]), sc2, ndel2), make_float2(p[c], p[c + 1]));
           dp[c] = u.x;
           dp[c + 1] = u.y;
         }
-        if (n >= whole) {
+        if (w.template from<PARTS>() + n >= whole) {
 #pragma unroll
           for (int c = 0; c < 64; ++c)
             if (c > lim) dp[c] = 0.f;
@@ -851,9 +918,14 @@ __global__ void __launch_bounds__(kThreads, 1) dense_dq_tc_kernel(const __grid_c
       // each side stores half of the columns
       const int rows = min(32, w.valid - quarter * 32);
       const int64_t at = (int64_t(w.t.b) * a.T + w.t.q_begin + q0 + quarter * 32) * a.Hq + w.head;
-      store_lanes<T, DP / 2>(tQ + lanes + side * (DP / 2), w.total <= 0, wait.ok ? grad_rest<T>(args, w.factor) : NAN, out_addr + warp * 32 * DP,
-                             static_cast<T*>(a.dq) + at * a.D + side * (DP / 2), int64_t(a.Hq) * a.D, rows,
-                             a.D - side * (DP / 2), lane);
+      if constexpr (PARTS) {
+        if (w.part_from > 0 || !w.part_last)
+          keep_part<DP / 2>(tQ + lanes + side * (DP / 2), kept_at<DP / 2>(a, side, row), w.part_from == 0, w.part_last);
+      }
+      if (w.template last<PARTS>())
+        store_lanes<T, DP / 2>(tQ + lanes + side * (DP / 2), w.total <= 0, wait.ok ? grad_rest<T>(args, w.factor) : NAN,
+                               out_addr + warp * 32 * DP, static_cast<T*>(a.dq) + at * a.D + side * (DP / 2),
+                               int64_t(a.Hq) * a.D, rows, a.D - side * (DP / 2), lane);
       __syncwarp();
       w = next;
     }
@@ -879,9 +951,12 @@ int bwd_t(const BwdTcArgs& a, cudaStream_t s) {
   const int64_t wide = a.q_slots > (a.q_slots + a.k_slots + 7) / 8 ? a.q_slots : (a.q_slots + a.k_slots + 7) / 8;
   dense_stats_kernel<T, DP><<<dim3(unsigned(wide), kRows / kStatTokens + 1), 256, 0, s>>>(a);
   PISA_CHECK_LAUNCH();
-  int rc = launch<dense_dkv_tc_kernel<T, DP>>(min64(a.k_slots * d.H, sm_count()), BwdTile<DP>::DKV_SMEM, a, s);
+  const int64_t kv_ctas = min64(a.k_slots * d.H, sm_count()), q_ctas = min64(a.q_slots * d.Hq, sm_count());
+  int rc = d.kept ? launch<dense_dkv_tc_kernel<T, DP, true>>(kv_ctas, BwdTile<DP>::DKV_SMEM, a, s)
+                  : launch<dense_dkv_tc_kernel<T, DP, false>>(kv_ctas, BwdTile<DP>::DKV_SMEM, a, s);
   if (rc) return rc;
-  return launch<dense_dq_tc_kernel<T, DP>>(min64(a.q_slots * d.Hq, sm_count()), BwdTile<DP>::DQ_SMEM, a, s);
+  return d.kept ? launch<dense_dq_tc_kernel<T, DP, true>>(q_ctas, BwdTile<DP>::DQ_SMEM, a, s)
+                : launch<dense_dq_tc_kernel<T, DP, false>>(q_ctas, BwdTile<DP>::DQ_SMEM, a, s);
 }
 
 }  // namespace
@@ -889,12 +964,25 @@ int bwd_t(const BwdTcArgs& a, cudaStream_t s) {
 namespace {
 // Entries of `range`: two per sequence (and one for the rows past the last) and KV head.
 int64_t range_entries(bool packed, int64_t B, int64_t H, int64_t sequences) { return 2 * H * (packed ? sequences + 1 : B); }
+// Sums on their way, where an item may pass kPart tiles: its bytes, behind the rest.
+int64_t kept_bytes(int64_t T, int64_t N, int64_t G, int64_t D, int64_t Dv) {
+  const int64_t most = int64_t(kPart) * kRows;
+  if ((T + kRows) * G <= most && N <= most) return 0;
+  return int64_t(sm_count()) * 2 * kRows * (D <= 64 && Dv <= 64 ? 64 : 128) * int64_t(sizeof(float));
+}
+// Bytes of the statistics, the list of tiles, the counters and `range`; the sums
+// on their way begin there (on 16 bytes, as the workspace does).
+int64_t kept_offset(bool packed, int dtype, int64_t B, int64_t T, int64_t N, int64_t Hq, int64_t H, int64_t sequences) {
+  const int64_t q = seq_slots(packed, B, T, sequences, kRows), k = seq_slots(packed, B, N, sequences, kRows);
+  const int64_t words = 2 + (dtype == PISA_F16 ? range_entries(packed, B, H, sequences) : 0);
+  const int64_t bytes = q * Hq * kStat * int64_t(sizeof(float)) + (q + k) * int64_t(sizeof(SeqTile)) + words * int64_t(sizeof(int));
+  return (bytes + 15) / 16 * 16;
+}
 }  // namespace
 
-int64_t dense_bwd_workspace(bool packed, int dtype, int64_t B, int64_t T, int64_t N, int64_t Hq, int64_t H, int64_t sequences) {
-  const int64_t q = seq_slots(packed, B, T, sequences, kRows), k = seq_slots(packed, B, N, sequences, kRows);
-  return q * Hq * kStat * int64_t(sizeof(float)) + (q + k) * int64_t(sizeof(SeqTile)) +
-         (2 + (dtype == PISA_F16 ? range_entries(packed, B, H, sequences) : 0)) * int64_t(sizeof(int));
+int64_t dense_bwd_workspace(bool packed, int dtype, int64_t B, int64_t T, int64_t N, int64_t Hq, int64_t H, int64_t D,
+                            int64_t Dv, int64_t sequences) {
+  return kept_offset(packed, dtype, B, T, N, Hq, H, sequences) + kept_bytes(T, N, Hq / H, D, Dv);
 }
 
 int dense_attn_bwd_tc(const DenseAttnArgs& d, int dtype, cudaStream_t stream) {
@@ -910,6 +998,9 @@ int dense_attn_bwd_tc(const DenseAttnArgs& d, int dtype, cudaStream_t stream) {
   a.order = reinterpret_cast<SeqTile*>(d.delta + a.q_slots * d.Hq * kStat);
   a.counters = reinterpret_cast<int*>(a.order + a.q_slots + a.k_slots);
   if (a.q_slots * d.Hq >= (int64_t(1) << 31) - 4096 || a.k_slots * d.H >= (int64_t(1) << 31) - 4096) return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
+  if (kept_bytes(d.T, d.N, d.G, d.D, d.Dv))
+    a.d.kept = reinterpret_cast<float*>(reinterpret_cast<char*>(d.delta) +
+                                        kept_offset(d.cu_q, dtype, d.B, d.T, d.N, d.Hq, d.H, d.sequences));
   if (dtype == PISA_F16) {
     a.range = reinterpret_cast<uint32_t*>(a.counters + 2);
     const cudaError_t e = cudaMemsetAsync(a.range, 0, range_entries(d.cu_q, d.B, d.H, d.sequences) * sizeof(int), stream);

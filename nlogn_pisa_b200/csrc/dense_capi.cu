@@ -154,7 +154,7 @@ int64_t pisa_full_attn_bwd_workspace_bytes(int64_t B, int64_t Tq, int64_t Hq, in
       dtype > PISA_F16)
     return -1;
   if (dtype == PISA_F32 || D > 128 || Dv > 128) return 256 + B * Tq * Hq * 4;
-  return 256 + dense_bwd_workspace(sequences > 0, dtype, B, Tq, N, Hq, H, sequences);
+  return 256 + dense_bwd_workspace(sequences > 0, dtype, B, Tq, N, Hq, H, D, Dv, sequences);
 }
 
 int pisa_full_attn_bwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb,
