@@ -9,8 +9,11 @@
 // w = 2^(m - max m).  The prefix is one key range for the query rows of the
 // whole batch, so its keys and values are read once for all of them; own
 // caches are read once each.  This file holds the form on the FMA pipes (fp32
-// tensors and heads wider than 128) and the joining launch.  Both are bound by
-// HBM; the join's reads (L2 mostly) and its start overlap the launch before it.
+// tensors and heads wider than 128) and the joining launch.  The FMA form loads
+// a tile, waits and computes in turn, and its latencies bound it: in fp32 64
+// sequences of 1 to 2048 keys (8 heads of 128) take 458 us and the prefix of 8192
+// that they share 319 us, against 73 and 10 us for their bytes.  The join is bound by
+// its reads (L2 mostly), whose start overlaps the launch before it.
 #include "prefix_attn.cuh"
 
 namespace pisa {

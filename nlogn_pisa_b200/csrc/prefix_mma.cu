@@ -444,7 +444,7 @@ int by_rows(StreamArgs s, bool prefix, int sms, cudaStream_t stream) {
   const PrefixArgs& a = s.p;
   const int64_t own_rows = int64_t(a.T) * a.G, prefix_rows = a.B * own_rows;
   // 8 rows per pass when no KV head has more: half the registers and join
-  // buffers, one stage more; 16 otherwise: half the passes over the keys
+  // buffers; 16 otherwise: half the passes over the keys
   const int br = (prefix ? prefix_rows : own_rows) <= 8 ? 8 : 16;
   s.own_blocks = int((own_rows + br - 1) / br);
   s.prefix_blocks = int((prefix_rows + br - 1) / br);
