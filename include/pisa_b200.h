@@ -394,11 +394,11 @@ PISA_API int64_t pisa_qk_norm_rotary_bwd_workspace_bytes(int64_t B, int64_t T, i
  *   16-bit dtype lost, itself rounded, for the backward (fp32: not used).
  * scale > 0.  D, Dv multiples of 8, at most 256.
  * workspace: NULL, or pisa_full_attn_fwd_workspace_bytes(...) bytes (256 at
- *   least, 16-byte aligned) whose first 4 receive the device status word.  Over
- *   more than 65536 keys (8192 with out_low) the 16-bit kernels want all of it:
+ *   least) whose first 4 receive the device status word.  Over more than 65536
+ *   keys (8192 with out_low) the 16-bit kernels want all of it, 16-byte aligned:
  *   without, the tensor core's accumulator rounds towards zero on the way, and outputs
- *   fall short by 0.002 of themselves over a million keys of equal weight.  The outputs of a call with an
- *   expired wait are undefined.
+ *   fall short by 0.002 of themselves over a million keys of equal weight.  The
+ *   outputs of a call with an expired wait are undefined.
  */
 PISA_API int pisa_full_attn_fwd(const void *q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void *k, int64_t k_sb,
                                 int64_t k_st, int64_t k_sh, const void *v, int64_t v_sb, int64_t v_st, int64_t v_sh,

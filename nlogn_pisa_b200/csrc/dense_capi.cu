@@ -138,12 +138,11 @@ int pisa_full_attn_fwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, 
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (workspace) {
     if (workspace_bytes < 256) return fail(PISA_ERR_INVALID, "workspace too small");
-    if (!on16(workspace)) return fail(PISA_ERR_INVALID, "workspace must be 16-byte aligned");
     cudaError_t e = cudaMemsetAsync(workspace, 0, 256, s);
     if (e != cudaSuccess) return fail_cuda(e, "status clear");
     a.status = static_cast<int*>(workspace);
     const int64_t whole = pisa_full_attn_fwd_workspace_bytes(B, Tq, Hq, H, D, Dv, N, sequences, dtype);
-    if (whole > 256 && workspace_bytes >= whole) a.kept = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
+    if (whole > 256 && workspace_bytes >= whole && on16(workspace)) a.kept = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
   }
   return dense_attn_tc_eligible(a, dtype) ? dense_attn_fwd_tc(a, dtype, s) : dense_attn_fwd_simt(a, dtype, s);
 }
