@@ -456,12 +456,113 @@ PISA_API int pisa_prefix_attn(const void *q, int64_t q_sb, int64_t q_st, int64_t
 PISA_API int64_t pisa_prefix_attn_workspace_bytes(int64_t B, int64_t Tq, int64_t Hq, int64_t H, int64_t D, int64_t Dv,
                                                   int64_t capacity, int64_t prefix, int dtype);
 
+/*
+ * The norms after one branch of a decoder block and before the next, fused
+ * with the branch's gate and the residual scale.  Rows of D elements, `rows`
+ * of them (x_st, branch_st: element strides of the rows):
+ *   y = branch / sqrt(mean(branch^2) + eps) * post_weight  (NULL: y = branch)
+ *   h = residual_scale * x + branch_scale * gate * y       (gate NULL: 1)
+ *   n = h / sqrt(mean(h^2) + eps) * weight.
+ * branch NULL: h is x itself and is not written (gate and post_weight NULL).
+ * gate: with gate_rows 0 one row per row, in dtype; otherwise every gate_rows
+ *   consecutive rows (a divisor of `rows`) share a row, in FP32 or dtype
+ *   (gate_dtype); rows gate_st apart.
+ * post_weight, weight: [D] in FP32 or dtype.
+ * h, n: contiguous [rows, D] in dtype.  Instead of n, n_q (rows n_q_st bytes
+ *   apart, on 16 bytes) and n_scale [rows] receive its 8-bit form
+ *   (pisa_quantize_int8), rounded from the fp32 values.
+ * stats: [rows, 2] fp32 for the backward, or NULL.
+ * Rows need not be aligned; where all start on 16 bytes and D is a multiple of
+ * 8 the accesses are wide.  D at most 16384.
+ */
+PISA_API int pisa_residual_norm(const void *x, int64_t x_st, const void *branch, int64_t branch_st, const void *gate,
+                                int64_t gate_st, int64_t gate_rows, int gate_dtype, const void *post_weight,
+                                int post_dtype, const void *weight, int weight_dtype, int dtype, int64_t rows, int64_t D,
+                                float residual_scale, float branch_scale, float eps, void *h, void *n, int8_t *n_q,
+                                int64_t n_q_st, float *n_scale, float *stats, pisa_stream_t stream);
+
+/*
+ * Backward of pisa_residual_norm: dx, dbranch [rows, D] in dtype, dgate in the
+ * gate's type ([rows, D], or one contiguous row per gate row), dpost_weight and
+ * dweight [D] in the weights' types; all contiguous, every element written.
+ * dh (NULL: zero), dn: contiguous [rows, D]; the forward's operands, and stats
+ * as it wrote them.  Sums run in a fixed order.
+ * workspace: pisa_residual_norm_bwd_workspace_bytes(...) bytes (gate_rows: 0
+ * without a gate that rows share).
+ */
+PISA_API int pisa_residual_norm_bwd(const void *dh, const void *dn, const void *x, int64_t x_st, const void *branch,
+                                    int64_t branch_st, const void *gate, int64_t gate_st, int64_t gate_rows,
+                                    int gate_dtype, const void *post_weight, int post_dtype, const void *weight,
+                                    int weight_dtype, int dtype, int64_t rows, int64_t D, float residual_scale,
+                                    float branch_scale, const float *stats, void *dx, void *dbranch, void *dgate,
+                                    void *dpost_weight, void *dweight, void *workspace, int64_t workspace_bytes,
+                                    pisa_stream_t stream);
+
+PISA_API int64_t pisa_residual_norm_bwd_workspace_bytes(int64_t rows, int64_t D, int64_t gate_rows);
+
+/*
+ * The gated product of a feed-forward layer, out = gate * sigmoid(gate) * up,
+ * over `rows` rows of D elements (gate_st, up_st: element strides of the rows).
+ * out: contiguous [rows, D] in dtype.
+ * gate_q, up_q (both or neither; rows q_st bytes apart, on 16 bytes) and
+ *   gate_scale, up_scale [rows, ceil(D / 128)] receive gate and up in 8 bits
+ *   (pisa_quantize_int8, grouped) for the backward.
+ * out_q (rows out_q_st bytes apart, on 16 bytes) and out_scale [rows], instead
+ *   of out and the kept bytes: the product in 8 bits, rounded from its fp32
+ *   values; D at most 32768.
+ */
+PISA_API int pisa_swiglu(const void *gate, int64_t gate_st, const void *up, int64_t up_st, int dtype, int64_t rows,
+                         int64_t D, void *out, int8_t *gate_q, int8_t *up_q, int64_t q_st, float *gate_scale,
+                         float *up_scale, int8_t *out_q, int64_t out_q_st, float *out_scale, pisa_stream_t stream);
+
+/*
+ * Backward of pisa_swiglu: dgate, dup contiguous [rows, D] in dtype from dout
+ * (rows dout_st apart) and gate and up, or (gate_q not NULL) what their kept
+ * bytes stand for.  out: NULL, or receives the product again (contiguous).
+ */
+PISA_API int pisa_swiglu_bwd(const void *dout, int64_t dout_st, const void *gate, int64_t gate_st, const void *up,
+                             int64_t up_st, const int8_t *gate_q, const int8_t *up_q, int64_t q_st,
+                             const float *gate_scale, const float *up_scale, int dtype, int64_t rows, int64_t D,
+                             void *dgate, void *dup, void *out, pisa_stream_t stream);
+
+/*
+ * A tensor in 8 bits: q = round(x * (127 / m)) to the nearest (ties to even),
+ * scale = m / 127, m = max(largest |x|, 2^-100), each step one fp32 result,
+ * over every row (grouped 0; scale [rows]) or every 128 elements of a row
+ * (grouped 1; scale [rows, ceil(D / 128)]).  Values that hold an infinity or
+ * NaN become zeros under a scale of NaN.  x: rows x_st elements apart; q: rows
+ * q_st bytes apart, on 16 bytes; bytes between rows are not written.
+ */
+PISA_API int pisa_quantize_int8(const void *x, int64_t x_st, int dtype, int64_t rows, int64_t D, int grouped, int8_t *q,
+                                int64_t q_st, float *scale, pisa_stream_t stream);
+
+/* out[r, i] = q[r, i] * scale[r, i / 128], contiguous in dtype: the grouped form back. */
+PISA_API int pisa_restore_int8(const int8_t *q, int64_t q_st, const float *scale, int dtype, int64_t rows, int64_t D,
+                               void *out, pisa_stream_t stream);
+
+/*
+ * out[t, o] = x_scale[t] * weight_scale[o] * sum_k x[t, k] * weight[o, k] +
+ * bias[o] over signed bytes; the sums are exact.
+ * x: [T, K], weight: [O, K], rows x_st and weight_st bytes apart and on 16
+ * bytes (bytes past a row's K elements are not used); K below 131072.
+ * bias: [O] in FP32 or out_dtype, or NULL.  out: contiguous [T, O].
+ * workspace: NULL, or pisa_int8_linear_workspace_bytes(...) bytes whose first 4
+ *   receive the device status word; the outputs of a call with an expired wait
+ *   are undefined.
+ */
+PISA_API int pisa_int8_linear(const int8_t *x, int64_t x_st, const float *x_scale, const int8_t *weight,
+                              int64_t weight_st, const float *weight_scale, const void *bias, int bias_dtype,
+                              int out_dtype, int64_t T, int64_t K, int64_t O, void *out, void *workspace,
+                              int64_t workspace_bytes, pisa_stream_t stream);
+
+PISA_API int64_t pisa_int8_linear_workspace_bytes(int64_t T, int64_t K, int64_t O);
+
 /* ---- device status (no counterpart in the reference, whose Triton kernels never wait) ----
  * Every kernel that waits on another part of the GPU waits a bounded number
  * of tries.  A wait that expires records PISA_ERR_TIMEOUT in the 4-byte
  * status word at byte offset 0 of the call's workspace (pisa_select_blocks,
- * pisa_leaf_scores, pisa_full_attn_fwd and _bwd, pisa_prefix_attn, and
- * pisa_sparse_attn_fwd when it takes the tensor-core path); the call clears that
+ * pisa_leaf_scores, pisa_full_attn_fwd and _bwd, pisa_prefix_attn,
+ * pisa_int8_linear, and pisa_sparse_attn_fwd when it takes the tensor-core path); the call clears that
  * word on `stream` before any of its waits can expire.
  *
  * pisa_workspace_status copies the word back and synchronises `stream`:

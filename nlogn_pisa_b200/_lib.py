@@ -74,6 +74,17 @@ SIGNATURES = {
     "pisa_prefix_attn": (_I, [_P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _P, _I, _P, _L, _L, _P, _L, _L, _I, _L,
                               _L, _L, _L, _L, _L, _L, _L, _F, _P, _P, _P, _L, _P]),
     "pisa_prefix_attn_workspace_bytes": (_L, [_L, _L, _L, _L, _L, _L, _L, _L, _I]),
+    "pisa_residual_norm": (_I, [_P, _L, _P, _L, _P, _L, _L, _I, _P, _I, _P, _I, _I, _L, _L, _F, _F, _F, _P, _P, _P, _L, _P,
+                                _P, _P]),
+    "pisa_residual_norm_bwd": (_I, [_P, _P, _P, _L, _P, _L, _P, _L, _L, _I, _P, _I, _P, _I, _I, _L, _L, _F, _F, _P, _P, _P,
+                                    _P, _P, _P, _P, _L, _P]),
+    "pisa_residual_norm_bwd_workspace_bytes": (_L, [_L, _L, _L]),
+    "pisa_swiglu": (_I, [_P, _L, _P, _L, _I, _L, _L, _P, _P, _P, _L, _P, _P, _P, _L, _P, _P]),
+    "pisa_swiglu_bwd": (_I, [_P, _L, _P, _L, _P, _L, _P, _P, _L, _P, _P, _I, _L, _L, _P, _P, _P, _P]),
+    "pisa_quantize_int8": (_I, [_P, _L, _I, _L, _L, _I, _P, _L, _P, _P]),
+    "pisa_restore_int8": (_I, [_P, _L, _P, _I, _L, _L, _P, _P]),
+    "pisa_int8_linear": (_I, [_P, _L, _P, _P, _L, _P, _P, _I, _I, _L, _L, _L, _P, _P, _L, _P]),
+    "pisa_int8_linear_workspace_bytes": (_L, [_L, _L, _L]),
     "pisa_workspace_status": (_I, [_P, _P]),
     "pisa_wait_selftest": (_I, [_I, _L, _P, _L, _P]),
     "pisa_ex2_selftest": (_I, [_P, _P, _P, _L, _P]),

@@ -1,0 +1,326 @@
+// Products of 8-bit tensors with a scale per token and per output channel.
+//
+//   y[t, o] = ws[o] xs[t] sum_k w[o, k] x[t, k] + bias[o],
+// with int32 sums, which are exact for K < 2^17.
+//
+// tcgen05 tiles (kind::i8): 128 output channels are the rows of a tile and BN
+// tokens its columns, so a warp's lanes are 32 consecutive channels of every
+// token it stores and rows of any length leave without a detour.  K goes in
+// blocks of 128 bytes, a 128-byte-swizzled TMA box of each operand per stage.
+// Warp 0 loads, warp 1 issues the MMAs, warps 2 to 5 scale and store; two
+// accumulators in TMEM let a tile's stores run under the next tile's products.
+#include <cudaTypedefs.h>
+
+#include "dense_tc.cuh"
+
+namespace pisa {
+
+namespace {
+
+constexpr int kM = 128;          // output channels of a tile
+constexpr int kStepBytes = 128;  // bytes of K per stage
+constexpr int kThreads = 192;
+constexpr int kSmem = 220 * 1024;
+
+struct LinArgs {
+  CUtensorMap tm_w, tm_x;
+  const float* w_scale;
+  const float* x_scale;
+  const void* bias;     // or NULL
+  int bias_f32;
+  int T, O, steps;      // steps: K in blocks of 128 bytes
+  uint32_t tiles_o, tiles;
+  uint32_t tries;
+  void* out;
+  int* status;
+};
+
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint64_t* mbar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+      :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(tc::smem_u32(mbar)) : "memory");
+}
+
+// D[tmem] (+)= A[smem] * B[smem]^T of signed bytes, 32 of K.
+__device__ __forceinline__ void mma_i8(uint32_t d, uint32_t a_low, uint32_t b_low, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], a, b, %3, p;\n\t}"
+      :: "r"(d), "r"(a_low), "r"(b_low), "r"(idesc), "r"(uint32_t(accumulate)), "r"(kDescHigh) : "memory");
+}
+
+// Instruction descriptor of kind::i8: int32 sums of signed bytes, both operands K-major.
+__device__ __forceinline__ uint32_t idesc_i8(int M, int N) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(N >> 3) << 17) | (uint32_t(M >> 4) << 24);
+}
+
+template <int BN>
+struct Tile {
+  static constexpr int A_BYTES = kM * kStepBytes, B_BYTES = BN * kStepBytes, STAGE = A_BYTES + B_BYTES;
+  static constexpr int STAGES = (kSmem - 1024) / STAGE < 10 ? (kSmem - 1024) / STAGE : 10;
+  static constexpr int SMEM = STAGES * STAGE + 1024;
+  static constexpr int COLS = BN < 32 ? 32 : BN;             // TMEM columns of an accumulator
+};
+
+// 32 tokens of one channel per lane, stored token by token: 32 consecutive channels per warp.
+template <typename T>
+__device__ __forceinline__ void store_columns(const float (&v)[32], T* out, int64_t O, int t, int T_, int o, int O_, bool pairs) {
+  const int lane = threadIdx.x & 31;
+  if constexpr (sizeof(T) == 2) {
+    if (pairs) {
+      // neighbouring lanes swap, so that each holds both channels of a pair for every other token
+      const bool odd = lane & 1;
+      T* at = out + int64_t(t + odd) * O + (o & ~1);
+#pragma unroll
+      for (int j = 0; j < 32; j += 2) {
+        const float got = __shfl_xor_sync(kFull, odd ? v[j] : v[j + 1], 1);
+        if (t + j + odd < T_ && o < O_)
+          *reinterpret_cast<uint32_t*>(at + int64_t(j) * O) = odd ? pack2<T>(got, v[j + 1]) : pack2<T>(v[j], got);
+      }
+      return;
+    }
+  }
+  T* at = out + int64_t(t) * O + o;
+#pragma unroll
+  for (int j = 0; j < 32; ++j)
+    if (t + j < T_ && o < O_) at[int64_t(j) * O] = from_f32<T>(v[j]);
+}
+
+template <typename T, int BN>
+__global__ void __launch_bounds__(kThreads) int8_linear_kernel(const __grid_constant__ LinArgs a) {
+  using L = Tile<BN>;
+  extern __shared__ __align__(16) uint8_t raw[];
+  __shared__ uint64_t full[L::STAGES], empty[L::STAGES], acc_full[2], acc_empty[2], drained;
+  __shared__ uint32_t slot;
+  __shared__ WaitFlag wait;
+  __shared__ __align__(16) float s_xs[4][BN < 32 ? 32 : BN];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t base = (tc::smem_u32(raw) + 1023u) & ~1023u;
+  if (warp == 0 && lane == 0) {
+    for (int i = 0; i < L::STAGES; ++i) {
+      tc::mbar_init(&full[i], 1);
+      tc::mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&acc_full[i], 1);
+      tc::mbar_init(&acc_empty[i], 4);
+    }
+    tc::mbar_init(&drained, 1);
+    tc::fence_barrier_init();
+    wait.init(a.tries);
+  }
+  if (warp == 1) tc::tmem_alloc(&slot, 2 * L::COLS);
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = slot;
+  bool ok = true;
+  if (warp == 0) {
+    if (lane == 0) {
+      int st = 0, loads = 0;
+      uint32_t phase = 1;
+      for (uint32_t tile = blockIdx.x; tile < a.tiles && ok; tile += gridDim.x) {
+        const uint32_t tt = tile / a.tiles_o, to = tile - tt * a.tiles_o;
+        for (int k = 0; k < a.steps; ++k) {
+          if (!(ok = wait_phase(&empty[st], int(phase), &wait))) break;
+          const uint32_t at = base + st * L::STAGE;
+          tc::mbar_arrive_expect_tx(&full[st], L::STAGE);
+          tma_load_2d(at, &a.tm_w, k * kStepBytes, int(to) * kM, &full[st]);
+          tma_load_2d(at + L::A_BYTES, &a.tm_x, k * kStepBytes, int(tt) * BN, &full[st]);
+          ++loads;
+          if (++st == L::STAGES) {
+            st = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      // nothing may arrive after the CTA's end: the stages in use have been
+      // handed back (after an expired wait: their copies have landed)
+      for (int x = max(0, loads - L::STAGES); x < loads; ++x)
+        wait_phase(ok ? &empty[x % L::STAGES] : &full[x % L::STAGES], x / L::STAGES, &wait);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    const bool leader = elect_one();
+    const uint32_t idesc = idesc_i8(kM, BN);
+    int st = 0, n = 0;
+    uint32_t phase = 0;
+    for (uint32_t tile = blockIdx.x; tile < a.tiles && ok; tile += gridDim.x, ++n) {
+      const int buf = n & 1;
+      if (n >= 2) ok = wait_phase(&acc_empty[buf], (n >> 1) - 1, &wait);
+      tc::fence_after_sync();
+      const uint32_t d = tmem + buf * L::COLS;
+#pragma unroll 1
+      for (int k = 0; k < a.steps; ++k) {
+        ok = wait_phase(&full[st], int(phase), &wait) && ok;
+        if (!__all_sync(kFull, ok)) {
+          ok = false;
+          break;
+        }
+        tc::fence_after_sync();
+        if (leader) {
+          const uint32_t al = desc_low(base + st * L::STAGE, 16), bl = desc_low(base + st * L::STAGE + L::A_BYTES, 16);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mma_i8(d, al + 2 * i, bl + 2 * i, idesc, k > 0 || i > 0);
+          tc::mma_commit(&empty[st]);
+          if (k + 1 == a.steps) tc::mma_commit(&acc_full[buf]);
+        }
+        __syncwarp();
+        if (++st == L::STAGES) {
+          st = 0;
+          phase ^= 1;
+        }
+      }
+    }
+    if (!__all_sync(kFull, ok)) {
+      if (leader) tc::mma_commit(&drained);
+      wait_phase(&drained, 0, &wait);
+    }
+    __syncwarp();
+  } else {
+    const int quarter = warp & 3;                  // TMEM lanes that this warp may read
+    const uint32_t lanes = uint32_t(quarter * 32) << 16;
+    float* xs = s_xs[quarter];
+    const bool pairs = (a.O & 1) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 3u) == 0;
+    int n = 0;
+    for (uint32_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, ++n) {
+      const int buf = n & 1;
+      const uint32_t tt = tile / a.tiles_o, to = tile - tt * a.tiles_o;
+      const int t0 = int(tt) * BN, o = int(to) * kM + quarter * 32 + lane;
+      __syncwarp();
+      for (int i = lane; i < BN; i += 32) xs[i] = t0 + i < a.T ? a.x_scale[t0 + i] : 0.f;
+      const float ws = o < a.O ? a.w_scale[o] : 0.f;
+      float bias = 0.f;
+      if (a.bias && o < a.O) bias = a.bias_f32 ? static_cast<const float*>(a.bias)[o] : to_f32<T>(static_cast<const T*>(a.bias)[o]);
+      __syncwarp();
+      ok = wait_phase(&acc_full[buf], n >> 1, &wait) && ok;
+      if (!__all_sync(kFull, ok)) break;
+      tc::fence_after_sync();
+#pragma unroll 1
+      for (int c = 0; c < BN; c += 32) {
+        float v[32];
+        tc::tmem_ld32(tmem + buf * L::COLS + c + lanes, v);
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          const float4 s = *reinterpret_cast<const float4*>(xs + c + j);
+          v[j] = fmaf(float(__float_as_int(v[j])) * ws, s.x, bias);
+          v[j + 1] = fmaf(float(__float_as_int(v[j + 1])) * ws, s.y, bias);
+          v[j + 2] = fmaf(float(__float_as_int(v[j + 2])) * ws, s.z, bias);
+          v[j + 3] = fmaf(float(__float_as_int(v[j + 3])) * ws, s.w, bias);
+        }
+        // of a tile of 16 tokens, the other columns are not the product's: T ends before them
+        store_columns<T>(v, static_cast<T*>(a.out), a.O, t0 + c, BN < 32 ? min(a.T, t0 + BN) : a.T, o, a.O, pairs);
+      }
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&acc_empty[buf]);
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  if (threadIdx.x == 0 && wait.expired && a.status) atomicExch(a.status, PISA_ERR_TIMEOUT);
+  if (warp == 1) tc::tmem_free(tmem, 2 * L::COLS);
+}
+
+// 2-D map over rows of bytes: a box of 128 bytes of `box` rows, 128-byte
+// swizzle; bytes past a row's end and rows past the last read as zero.
+int byte_map(CUtensorMap* map, const void* base, int64_t rows, int64_t K, int64_t stride, uint32_t box) {
+  static PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  }();
+  if (!encode) return fail(PISA_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const cuuint64_t dims[2] = {cuuint64_t(K), cuuint64_t(rows)}, strides[1] = {cuuint64_t(stride)};
+  const cuuint32_t boxes[2] = {cuuint32_t(kStepBytes), box}, steps[2] = {1u, 1u};
+  for (int tries = 0; tries < 2; ++tries) {
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, boxes, steps,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r == CUDA_SUCCESS) return PISA_OK;
+    // a thread whose first CUDA call this is has no context until a runtime call binds the device's
+    if (cudaFree(nullptr) != cudaSuccess) return fail(PISA_ERR_CUDA, "no CUDA context");
+  }
+  return fail(PISA_ERR_UNSUPPORTED, "tensor map encoding rejected the operand layout");
+}
+
+struct Operands {
+  const void* x;
+  int64_t x_st;
+  const void* w;
+  int64_t w_st, K;
+};
+
+template <typename T, int BN>
+int launch(LinArgs a, const Operands& m, cudaStream_t s) {
+  using L = Tile<BN>;
+  int rc = byte_map(&a.tm_w, m.w, a.O, m.K, m.w_st, kM);
+  if (rc == PISA_OK) rc = byte_map(&a.tm_x, m.x, a.T, m.K, m.x_st, BN);
+  if (rc == PISA_OK) rc = allow_smem<int8_linear_kernel<T, BN>>(L::SMEM, "8-bit product smem attribute");
+  if (rc) return rc;
+  a.tiles_o = uint32_t((a.O + kM - 1) / kM);
+  const int64_t tiles = int64_t(a.tiles_o) * ((a.T + BN - 1) / BN);
+  if (tiles >= (int64_t(1) << 31)) return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
+  a.tiles = uint32_t(tiles);
+  int8_linear_kernel<T, BN><<<unsigned(min64(tiles, sm_count())), kThreads, L::SMEM, s>>>(a);
+  PISA_CHECK_LAUNCH();
+  return PISA_OK;
+}
+
+template <typename T>
+int dispatch(const LinArgs& a, const Operands& m, cudaStream_t s) {
+  if (a.T <= 16) return launch<T, 16>(a, m, s);
+  if (a.T <= 32) return launch<T, 32>(a, m, s);
+  if (a.T <= 64) return launch<T, 64>(a, m, s);
+  if (a.T <= 128) return launch<T, 128>(a, m, s);
+  return launch<T, 256>(a, m, s);
+}
+
+}  // namespace
+
+}  // namespace pisa
+
+extern "C" {
+
+int64_t pisa_int8_linear_workspace_bytes(int64_t T, int64_t K, int64_t O) {
+  return T <= 0 || K <= 0 || O <= 0 ? -1 : 256;
+}
+
+int pisa_int8_linear(const int8_t* x, int64_t x_st, const float* x_scale, const int8_t* weight, int64_t weight_st,
+                     const float* weight_scale, const void* bias, int bias_dtype, int out_dtype, int64_t T, int64_t K, int64_t O,
+                     void* out, void* workspace, int64_t workspace_bytes, pisa_stream_t stream) {
+  using namespace pisa;
+  if (out_dtype < PISA_F32 || out_dtype > PISA_F16) return fail(PISA_ERR_UNSUPPORTED, "the kernels support FP16, BF16 and FP32");
+  if (bias && bias_dtype != out_dtype && bias_dtype != PISA_F32)
+    return fail(PISA_ERR_UNSUPPORTED, "the bias must be FP32 or the output's type");
+  if (T <= 0 || K <= 0 || O <= 0) return fail(PISA_ERR_INVALID, "nonempty tensors are required");
+  if (K >= (int64_t(1) << 17)) return fail(PISA_ERR_UNSUPPORTED, "sums of 131072 or more products may not fit 32 bits");
+  if (T >= (int64_t(1) << 31) - 256 || O >= (int64_t(1) << 31) - 256) return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
+  if (!x || !x_scale || !weight || !weight_scale || !out) return fail(PISA_ERR_INVALID, "operands, scales and out are required");
+  if (T == 1) x_st = (K + 15) / 16 * 16;          // the stride of a single row may hold anything
+  if (O == 1) weight_st = (K + 15) / 16 * 16;
+  if ((reinterpret_cast<uintptr_t>(x) & 15u) || (reinterpret_cast<uintptr_t>(weight) & 15u) || x_st % 16 || weight_st % 16)
+    return fail(PISA_ERR_UNSUPPORTED, "8-bit rows must start on 16 bytes");
+  if (x_st < K || weight_st < K) return fail(PISA_ERR_UNSUPPORTED, "8-bit rows must not overlap");
+  if (workspace && workspace_bytes < 256) return fail(PISA_ERR_INVALID, "workspace too small");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  LinArgs a{};
+  a.w_scale = weight_scale; a.x_scale = x_scale; a.bias = bias; a.bias_f32 = bias_dtype == PISA_F32;
+  a.T = int(T); a.O = int(O); a.steps = int((K + kStepBytes - 1) / kStepBytes);
+  a.tries = wait_tries(a.steps);
+  a.out = out;
+  if (workspace) {
+    a.status = static_cast<int*>(workspace);
+    cudaError_t e = cudaMemsetAsync(workspace, 0, 256, s);
+    if (e != cudaSuccess) return fail_cuda(e, "status clear");
+  }
+  const Operands m{x, x_st, weight, weight_st, K};
+  if (out_dtype == PISA_F32) return dispatch<float>(a, m, s);
+  if (out_dtype == PISA_BF16) return dispatch<__nv_bfloat16>(a, m, s);
+  return dispatch<__half>(a, m, s);
+}
+
+}  // extern "C"

@@ -1,0 +1,219 @@
+// Tensors in 8 bits: a row, or every group of 128 elements of it, as signed
+// bytes with one fp32 scale (Scale8 in rows.cuh has the rounding).
+//
+// Rows serve 8-bit products (a scale per token or output channel), groups keep
+// activations for the backward.  Both are bound by HBM: 16-bit elements in, a
+// byte out (and back).
+#include "rows.cuh"
+
+namespace pisa {
+
+namespace {
+
+struct RowArgs {
+  const void* x;
+  int64_t x_st;
+  int64_t rows;
+  int64_t D;
+  uint32_t groups;
+  int8_t* q;
+  int64_t q_st;
+  float* scale;
+  void* out;
+};
+
+// A team holds the row.
+template <typename T, int TPR, int NV, bool A>
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) row_kernel(const __grid_constant__ RowArgs a) {
+  constexpr int TEAMS = TPR < 128 ? 128 / TPR : 1;
+  __shared__ float red[2 * (TPR / 32)];
+  int set = 0;
+  const int t = threadIdx.x % TPR, D = int(a.D);
+  const int64_t row = int64_t(blockIdx.x) * TEAMS + threadIdx.x / TPR;
+  if (row >= a.rows) return;                      // a whole warp
+  const T* xr = static_cast<const T*>(a.x) + row * a.x_st;
+  Raw8<T> x[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) x[j] = load_piece<T, TPR, A>(xr, j, t, D);
+  float top = 0.f;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    float f[8];
+    widen8<T>(x[j], f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max_nan(top, fabsf(f[e]));
+  }
+  top = team_reduce<TPR, true>(top, red, set);
+  const Scale8 s(top);
+  int8_t* qr = a.q + row * a.q_st;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    float f[8];
+    widen8<T>(x[j], f);
+    store_piece_s8<TPR, A>(qr, j, t, D, f, top < INFINITY, s.inv);
+  }
+  if (t == 0) a.scale[row] = s.scale;
+}
+
+// Rows too long for registers are read twice, in pieces of 8 times 512 elements.
+template <typename T, bool A>
+__global__ void __launch_bounds__(512) long_row_kernel(const __grid_constant__ RowArgs a) {
+  constexpr int TPR = 512, STEP = TPR * 8;
+  __shared__ float red[2 * (TPR / 32)];
+  int set = 0;
+  const int64_t row = blockIdx.x;
+  const T* xr = static_cast<const T*>(a.x) + row * a.x_st;
+  float top = 0.f;
+  for (int64_t at = 0; at < a.D; at += STEP) {
+    float f[8];
+    widen8<T>(load_piece<T, TPR, A>(xr + at, 0, threadIdx.x, int(min64(STEP, a.D - at))), f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max_nan(top, fabsf(f[e]));
+  }
+  top = team_reduce<TPR, true>(top, red, set);
+  const Scale8 s(top);
+  int8_t* qr = a.q + row * a.q_st;
+  for (int64_t at = 0; at < a.D; at += STEP) {
+    const int left = int(min64(STEP, a.D - at));
+    float f[8];
+    widen8<T>(load_piece<T, TPR, A>(xr + at, 0, threadIdx.x, left), f);
+    store_piece_s8<TPR, A>(qr + at, 0, threadIdx.x, left, f, top < INFINITY, s.inv);
+  }
+  if (threadIdx.x == 0) a.scale[row] = s.scale;
+}
+
+template <typename T, int TPR, int NV>
+int launch_row(const RowArgs& a, bool aligned, cudaStream_t s) {
+  constexpr int threads = TPR < 128 ? 128 : TPR, teams = threads / TPR;
+  const unsigned ctas = unsigned((a.rows + teams - 1) / teams);
+  if (aligned) row_kernel<T, TPR, NV, true><<<ctas, threads, 0, s>>>(a);
+  else row_kernel<T, TPR, NV, false><<<ctas, threads, 0, s>>>(a);
+  PISA_CHECK_LAUNCH();
+  return PISA_OK;
+}
+
+template <typename T>
+int rows8(const RowArgs& a, bool aligned, cudaStream_t s) {
+  if (a.D <= 256) return launch_row<T, 32, 1>(a, aligned, s);
+  if (a.D <= 1024) return launch_row<T, 32, 4>(a, aligned, s);
+  if (a.D <= 4096) return launch_row<T, 128, 4>(a, aligned, s);
+  if (a.D <= 16384) return launch_row<T, 512, 4>(a, aligned, s);
+  if (aligned) long_row_kernel<T, true><<<unsigned(a.rows), 512, 0, s>>>(a);
+  else long_row_kernel<T, false><<<unsigned(a.rows), 512, 0, s>>>(a);
+  PISA_CHECK_LAUNCH();
+  return PISA_OK;
+}
+
+constexpr int kThreads = 256;
+
+// Groups: sixteen threads each.
+template <typename T, bool A, bool BACK>
+__global__ void __launch_bounds__(kThreads) group_kernel(const __grid_constant__ RowArgs a) {
+  const int t = threadIdx.x & 15;
+  const int64_t item = int64_t(blockIdx.x) * (kThreads / 16) + (threadIdx.x >> 4);
+  const bool live = item < a.rows * a.groups;
+  const uint64_t at = live ? uint64_t(item) : 0;
+  const int64_t row = int64_t(at / a.groups), first = int64_t(at - uint64_t(row) * a.groups) * kGroup;
+  const int width = live ? int(min64(kGroup, a.D - first)) : 0;
+  int8_t* qr = a.q + row * a.q_st + first;
+  float f[8];
+  if constexpr (BACK) {
+    uint2 r = make_uint2(0, 0);
+    if constexpr (A) {
+      if (t * 8 < width) r = *reinterpret_cast<const uint2*>(qr + t * 8);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int c = column<16, A>(0, e, t);
+        const uint32_t b = c < width ? uint8_t(qr[c]) : 0;
+        if (e < 4) r.x |= b << (8 * e);
+        else r.y |= b << (8 * (e - 4));
+      }
+    }
+    const float scale = a.scale[at];
+    float lo[4], hi[4];
+    unpack_s8(r.x, lo);
+    unpack_s8(r.y, hi);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f[e] = lo[e] * scale;
+      f[4 + e] = hi[e] * scale;
+    }
+    store_piece<T, 16, A>(static_cast<T*>(a.out) + row * a.D + first, 0, t, width, f);
+  } else {
+    widen8<T>(load_piece<T, 16, A>(static_cast<const T*>(a.x) + row * a.x_st + first, 0, t, width), f);
+    float top = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max_nan(top, fabsf(f[e]));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(kFull, top, o));
+    const Scale8 s(top);
+    store_piece_s8<16, A>(qr, 0, t, width, f, top < INFINITY, s.inv);
+    if (live && t == 0) a.scale[at] = s.scale;
+  }
+}
+
+template <typename T, bool BACK>
+int groups8(const RowArgs& a, bool aligned, cudaStream_t s) {
+  const int64_t items = a.rows * a.groups, per = kThreads / 16;
+  const unsigned ctas = unsigned((items + per - 1) / per);
+  if (aligned) group_kernel<T, true, BACK><<<ctas, kThreads, 0, s>>>(a);
+  else group_kernel<T, false, BACK><<<ctas, kThreads, 0, s>>>(a);
+  PISA_CHECK_LAUNCH();
+  return PISA_OK;
+}
+
+int check(const void* x, const int8_t* q, int64_t q_st, const float* scale, int dtype, int64_t rows, int64_t D) {
+  if (dtype < PISA_F32 || dtype > PISA_F16) return fail(PISA_ERR_UNSUPPORTED, "the kernels support FP16, BF16 and FP32");
+  if (rows <= 0 || D <= 0) return fail(PISA_ERR_INVALID, "nonempty tensors are required");
+  if (rows >= (int64_t(1) << 31) || D >= (int64_t(1) << 31) || rows * ((D + kGroup - 1) / kGroup) >= (int64_t(1) << 34))
+    return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
+  if (!x || !q || !scale) return fail(PISA_ERR_INVALID, "the tensor, its bytes and scales are required");
+  if (!rows_on16(q, rows, q_st)) return fail(PISA_ERR_UNSUPPORTED, "8-bit rows must start on 16 bytes");
+  return PISA_OK;
+}
+
+RowArgs make_args(int64_t rows, int64_t D, int8_t* q, int64_t q_st, float* scale) {
+  RowArgs a{};
+  a.rows = rows; a.D = D; a.groups = uint32_t((D + kGroup - 1) / kGroup); a.q = q; a.q_st = q_st; a.scale = scale;
+  return a;
+}
+
+}  // namespace
+
+}  // namespace pisa
+
+extern "C" {
+
+int pisa_quantize_int8(const void* x, int64_t x_st, int dtype, int64_t rows, int64_t D, int grouped, int8_t* q, int64_t q_st,
+                       float* scale, pisa_stream_t stream) {
+  using namespace pisa;
+  if (int rc = check(x, q, q_st, scale, dtype, rows, D)) return rc;
+  RowArgs a = make_args(rows, D, q, q_st, scale);
+  a.x = x; a.x_st = x_st;
+  const bool aligned = D % 8 == 0 && rows_on16(x, rows, x_st * (dtype == PISA_F32 ? 4 : 2));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (grouped) {
+    if (dtype == PISA_F32) return groups8<float, false>(a, aligned, s);
+    if (dtype == PISA_BF16) return groups8<__nv_bfloat16, false>(a, aligned, s);
+    return groups8<__half, false>(a, aligned, s);
+  }
+  if (dtype == PISA_F32) return rows8<float>(a, aligned, s);
+  if (dtype == PISA_BF16) return rows8<__nv_bfloat16>(a, aligned, s);
+  return rows8<__half>(a, aligned, s);
+}
+
+int pisa_restore_int8(const int8_t* q, int64_t q_st, const float* scale, int dtype, int64_t rows, int64_t D, void* out,
+                      pisa_stream_t stream) {
+  using namespace pisa;
+  if (int rc = check(out, q, q_st, scale, dtype, rows, D)) return rc;
+  RowArgs a = make_args(rows, D, const_cast<int8_t*>(q), q_st, const_cast<float*>(scale));
+  a.out = out;
+  const bool aligned = D % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == PISA_F32) return groups8<float, true>(a, aligned, s);
+  if (dtype == PISA_BF16) return groups8<__nv_bfloat16, true>(a, aligned, s);
+  return groups8<__half, true>(a, aligned, s);
+}
+
+}  // extern "C"

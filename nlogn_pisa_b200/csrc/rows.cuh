@@ -1,0 +1,253 @@
+// Row-wise building blocks of the decoder block's operators: threads that share
+// a row, its sums and maxima, and the 8-bit form of a row or of a group of it.
+//
+// A team of TPR threads holds a row in registers, NV pieces of 8 elements per
+// thread.  Where every row starts on 16 bytes and its width is a multiple of 8
+// (A), piece j of thread t is 8 consecutive elements; otherwise its elements lie
+// TPR apart, so that a warp still touches consecutive ones.
+#pragma once
+
+#include <cmath>
+#include <type_traits>
+
+#include "dense_attn.cuh"
+#include "internal.h"
+
+namespace pisa {
+
+// Smallest magnitude that an 8-bit scale follows: below it 127 / max would overflow.
+constexpr float kTiny = 7.88860905221011805e-31f;   // 2^-100
+constexpr int kGroup = 128;                          // elements that share a scale of a kept activation
+
+// 8 elements as loaded.
+template <typename T> struct Raw8 { uint4 v[sizeof(T) / 2]; };
+
+template <typename T>
+__device__ __forceinline__ void widen8(const Raw8<T>& r, float (&f)[8]) {
+  if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      f[4 * i] = __uint_as_float(r.v[i].x);
+      f[4 * i + 1] = __uint_as_float(r.v[i].y);
+      f[4 * i + 2] = __uint_as_float(r.v[i].z);
+      f[4 * i + 3] = __uint_as_float(r.v[i].w);
+    }
+  } else {
+    const uint32_t w[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        f[2 * i] = __uint_as_float(w[i] << 16);
+        f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      } else {
+        const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        f[2 * i] = p.x;
+        f[2 * i + 1] = p.y;
+      }
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ Raw8<T> narrow8(const float (&f)[8]) {
+  Raw8<T> r;
+  if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      r.v[i] = make_uint4(__float_as_uint(f[4 * i]), __float_as_uint(f[4 * i + 1]), __float_as_uint(f[4 * i + 2]),
+                          __float_as_uint(f[4 * i + 3]));
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const __nv_bfloat162 p = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&p);
+      } else {
+        const __half2 p = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&p);
+      }
+    }
+    r.v[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  return r;
+}
+
+// Data that is read once: past L1.
+__device__ __forceinline__ uint4 load_stream(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+// Column of element e of piece j.
+template <int TPR, bool A>
+__device__ __forceinline__ int column(int j, int e, int t) {
+  return A ? (j * TPR + t) * 8 + e : (j * 8 + e) * TPR + t;
+}
+
+// Piece j of a row of D elements; elements past its end are zeros.
+template <typename T, int TPR, bool A>
+__device__ __forceinline__ Raw8<T> load_piece(const T* row, int j, int t, int D) {
+  Raw8<T> r;
+#pragma unroll
+  for (int i = 0; i < int(sizeof(T) / 2); ++i) r.v[i] = make_uint4(0, 0, 0, 0);
+  if constexpr (A) {
+    const int c = column<TPR, A>(j, 0, t);
+    if (c < D) {
+#pragma unroll
+      for (int i = 0; i < int(sizeof(T) / 2); ++i) r.v[i] = load_stream(reinterpret_cast<const uint4*>(row + c) + i);
+    }
+  } else {
+    uint32_t w[2 * sizeof(T)];
+#pragma unroll
+    for (int i = 0; i < int(2 * sizeof(T)); ++i) w[i] = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int c = column<TPR, A>(j, e, t);
+      if (c < D) {
+        if constexpr (sizeof(T) == 4) w[e] = reinterpret_cast<const uint32_t*>(row)[c];
+        else w[e / 2] |= uint32_t(reinterpret_cast<const uint16_t*>(row)[c]) << (e % 2 * 16);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < int(sizeof(T) / 2); ++i) r.v[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+  }
+  return r;
+}
+
+template <typename T, int TPR, bool A>
+__device__ __forceinline__ void store_piece(T* row, int j, int t, int D, const float (&f)[8]) {
+  if constexpr (A) {
+    const int c = column<TPR, A>(j, 0, t);
+    if (c < D) {
+      const Raw8<T> r = narrow8<T>(f);
+#pragma unroll
+      for (int i = 0; i < int(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(row + c)[i] = r.v[i];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int c = column<TPR, A>(j, e, t);
+      if (c < D) row[c] = from_f32<T>(f[e]);
+    }
+  }
+}
+
+// Piece j of a parameter row in fp32 or in the tensors' type (cached: many rows read it).
+template <typename T, int TPR, bool A>
+__device__ __forceinline__ void param_piece(const void* p, int f32, int j, int t, int D, float (&f)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = 0.f;
+  if constexpr (A) {
+    const int c = column<TPR, A>(j, 0, t);
+    if (c >= D) return;
+    if (f32) {
+      const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + c);
+      const float4 lo = __ldg(q), hi = __ldg(q + 1);
+      f[0] = lo.x; f[1] = lo.y; f[2] = lo.z; f[3] = lo.w;
+      f[4] = hi.x; f[5] = hi.y; f[6] = hi.z; f[7] = hi.w;
+    } else {
+      Raw8<T> r;
+#pragma unroll
+      for (int i = 0; i < int(sizeof(T) / 2); ++i)
+        r.v[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p) + c) + i);
+      widen8<T>(r, f);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int c = column<TPR, A>(j, e, t);
+      if (c < D) f[e] = f32 ? static_cast<const float*>(p)[c] : to_f32<T>(static_cast<const T*>(p)[c]);
+    }
+  }
+}
+
+// Larger of two, NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Sum (or maximum, NaN if any is) of a team's values, the same in all its
+// threads and in every run.  Teams of more than a warp are whole CTAs; `red`
+// holds two sets of TPR / 32 floats that calls use in turn (`set`), so that one
+// barrier per call is enough.
+template <int TPR, bool MAX>
+__device__ __forceinline__ float team_reduce(float v, float* red, int& set) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float w = __shfl_xor_sync(kFull, v, o);
+    v = MAX ? max_nan(v, w) : v + w;
+  }
+  if constexpr (TPR > 32) {
+    constexpr int W = TPR / 32;
+    float* at = red + set * W;
+    set ^= 1;
+    if ((threadIdx.x & 31) == 0) at[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = at[0];
+#pragma unroll
+    for (int i = 1; i < W; ++i) v = MAX ? max_nan(v, at[i]) : v + at[i];
+  }
+  return v;
+}
+
+// The 8-bit form of values whose largest magnitude is `top`: q = round(x * inv)
+// to the nearest (ties to even), x ~ q * scale, each step one fp32 result:
+//   m = max(top, 2^-100), inv = 127 / m, scale = m / 127.
+// Values that hold an infinity or NaN are zeros under a scale of NaN: they read
+// back as NaN.
+struct Scale8 {
+  float inv, scale;
+  __device__ __forceinline__ explicit Scale8(float top) {
+    const float m = fmaxf(top, kTiny);
+    const bool fine = top < INFINITY;
+    inv = fine ? __fdiv_rn(127.f, m) : 0.f;
+    scale = fine ? __fdiv_rn(m, 127.f) : __int_as_float(0x7fffffff);
+  }
+};
+
+// Four rounded values as bytes.  Adding 1.5 * 2^23 leaves the nearest integer
+// (ties to even, as the sum's rounding) in the low bits of the sum.
+__device__ __forceinline__ uint32_t pack_s8(float a, float b, float c, float d, float inv) {
+  const float magic = 12582912.f;
+  const uint32_t x = __float_as_uint(__fadd_rn(__fmul_rn(a, inv), magic)), y = __float_as_uint(__fadd_rn(__fmul_rn(b, inv), magic));
+  const uint32_t z = __float_as_uint(__fadd_rn(__fmul_rn(c, inv), magic)), w = __float_as_uint(__fadd_rn(__fmul_rn(d, inv), magic));
+  return __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
+}
+
+// Four bytes as floats.  A byte b in the low bits of 0x4B000000 | (b ^ 128) is
+// the float 2^23 + 128 + b.
+__device__ __forceinline__ void unpack_s8(uint32_t q, float (&f)[4]) {
+  const uint32_t u = q ^ 0x80808080u;
+  const float off = 8388736.f;
+  f[0] = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440)) - off;
+  f[1] = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7441)) - off;
+  f[2] = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7442)) - off;
+  f[3] = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7443)) - off;
+}
+
+template <int TPR, bool A>
+__device__ __forceinline__ void store_piece_s8(int8_t* row, int j, int t, int D, const float (&f)[8], bool fine, float inv) {
+  uint32_t lo = pack_s8(f[0], f[1], f[2], f[3], inv), hi = pack_s8(f[4], f[5], f[6], f[7], inv);
+  if (!fine) lo = hi = 0;
+  if constexpr (A) {
+    const int c = column<TPR, A>(j, 0, t);
+    if (c < D) *reinterpret_cast<uint2*>(row + c) = make_uint2(lo, hi);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int c = column<TPR, A>(j, e, t);
+      if (c < D) row[c] = int8_t((e < 4 ? lo >> (8 * e) : hi >> (8 * (e - 4))) & 255u);
+    }
+  }
+}
+
+// Host: whether a row view starts every row on 16 bytes (the stride of a single row may hold anything).
+inline bool rows_on16(const void* p, int64_t rows, int64_t stride_bytes) {
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (rows == 1 || stride_bytes % 16 == 0);
+}
+
+}  // namespace pisa

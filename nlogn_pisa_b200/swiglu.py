@@ -1,0 +1,152 @@
+"""The gated product of a feed-forward layer, with its inputs kept in 8 bits for the backward.
+
+``swiglu`` is silu(gate) * up; with ``checkpoint_bits=8`` what its backward needs
+is held as bytes with a scale per 128 elements instead of the 16-bit tensors
+(pisa_swiglu / pisa_swiglu_bwd).  ``swiglu_ffn`` is the whole layer, which keeps
+its input and the two products in that form only and rebuilds the gated
+product in its backward.
+"""
+
+from __future__ import annotations
+
+import torch
+import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .dense import carries_tangent, differentiated
+from .int8 import GROUP, byte_rows, checkpoint_int8, no_gradient, restore_int8, rows_of
+from .validation import require_cuda
+
+
+def _forward(gate, up, keep):
+    """The product, and gate and up in 8 bits: (values, scale) of each, as rows."""
+    rows = rows_of(gate), rows_of(up)
+    count, width = rows[0].shape
+    out, kept = gate.new_empty(gate.shape), (None,) * 4
+    pointers = (None, None, 0, None, None)
+    if keep:
+        values = [byte_rows(gate, (count, width)) for _ in range(2)]
+        scale = [gate.new_empty((count, -(-width // GROUP)), dtype=torch.float32) for _ in range(2)]
+        kept = (*values, *scale)
+        pointers = (values[0].data_ptr(), values[1].data_ptr(), -(-width // 16) * 16, scale[0].data_ptr(), scale[1].data_ptr())
+    _lib.launch(_lib.lib().pisa_swiglu, gate.get_device(), rows[0].data_ptr(), rows[0].stride(0), rows[1].data_ptr(),
+                rows[1].stride(0), _lib.DTYPES[gate.dtype], count, width, out.data_ptr(), *pointers, None, 0, None)
+    return out, kept
+
+
+def _backward(dout, gate, up, kept, want_out=False):
+    """(dgate, dup, and the product again or None) from gate and up, or from what was kept of them."""
+    rows = rows_of(dout)
+    count, width = rows.shape
+    dgate, dup = dout.new_empty(dout.shape), dout.new_empty(dout.shape)
+    out = dout.new_empty(dout.shape) if want_out else None
+    if kept is None:
+        gate, up = rows_of(gate), rows_of(up)
+        given = (gate.data_ptr(), gate.stride(0), up.data_ptr(), up.stride(0), None, None, 0, None, None)
+    else:
+        given = (None, 0, None, 0, kept[0].data_ptr(), kept[1].data_ptr(), -(-width // 16) * 16, kept[2].data_ptr(),
+                 kept[3].data_ptr())
+    _lib.launch(_lib.lib().pisa_swiglu_bwd, dout.get_device(), rows.data_ptr(), rows.stride(0), *given, _lib.DTYPES[dout.dtype],
+                count, width, dgate.data_ptr(), dup.data_ptr(), None if out is None else out.data_ptr())
+    return dgate, dup, out
+
+
+class SwigluFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, gate, up, keep):
+        out, kept = _forward(gate, up, keep)
+        ctx.keep = keep
+        ctx.save_for_backward(*(kept if keep else (gate, up)))
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        saved = ctx.saved_tensors
+        dgate, dup, _ = _backward(dout, None, None, saved) if ctx.keep else _backward(dout, *saved, None)
+        return dgate, dup, None
+
+
+def _check_bits(checkpoint_bits):
+    if checkpoint_bits not in (None, 8):
+        raise ValueError("checkpoint_bits must be None or 8")
+    return checkpoint_bits == 8
+
+
+def swiglu(gate, up, checkpoint_bits=None, quantize=False):
+    """silu(gate) * up of two tensors [..., D] of one shape.
+
+    Gradients reach both (reverse mode only).  ``checkpoint_bits=8``: the backward
+    reads gate and up in 8 bits (``checkpoint_int8``), half of what 16-bit copies
+    take; the product itself is exact.  ``quantize``: (values, scale), the product
+    in 8 bits as ``quantize_int8`` of its fp32 values, for ``int8_linear`` (D at
+    most 32768); for inference only.  gate and up may be halves of one tensor.
+    """
+    keep = _check_bits(checkpoint_bits)
+    if gate.dim() < 1 or gate.shape != up.shape or gate.dtype != up.dtype or not gate.is_floating_point():
+        raise ValueError("gate and up must share a shape and a floating dtype")
+    if 0 in gate.shape:
+        raise ValueError("nonempty tensors are required")
+    require_cuda(gate, up)
+    if gate.get_device() != up.get_device():
+        raise ValueError("gate and up must share a device")
+    code = _lib.dtype_code(gate)
+    if quantize:
+        no_gradient("quantize=True", gate, up)
+        rows = rows_of(gate), rows_of(up)
+        count, width = rows[0].shape
+        values, scale = byte_rows(gate, gate.shape), gate.new_empty(gate.shape[:-1], dtype=torch.float32)
+        _lib.launch(_lib.lib().pisa_swiglu, gate.get_device(), rows[0].data_ptr(), rows[0].stride(0), rows[1].data_ptr(),
+                    rows[1].stride(0), code, count, width, None, None, None, 0, None, None, values.data_ptr(),
+                    -(-width // 16) * 16, scale.data_ptr())
+        return values, scale
+    if differentiated(gate, up):
+        return SwigluFunction.apply(gate, up, keep)
+    return _forward(gate, up, False)[0]
+
+
+class SwigluFfnFunction(torch.autograd.Function):
+    """The layer's products are torch's; its backward starts from bytes."""
+
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, w_down, b_gate, b_up, b_down):
+        out, kept = _forward(F.linear(x, w_gate, b_gate), F.linear(x, w_up, b_up), True)
+        ctx.dtype = x.dtype
+        ctx.biases = tuple(b is not None for b in (b_gate, b_up, b_down))
+        ctx.save_for_backward(*checkpoint_int8(x), *kept, w_gate, w_up, w_down)
+        return F.linear(out, w_down, b_down)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x_values, x_scale, *kept, w_gate, w_up, w_down = ctx.saved_tensors
+        dgate, dup, out = _backward(dy @ w_down, None, None, kept, True)
+        rows = [t.reshape(-1, t.shape[-1]) for t in (dgate, dup, dy, out)]
+        x = restore_int8(x_values, x_scale, ctx.dtype).view(-1, x_values.shape[-1])
+        weights = rows[0].T @ x, rows[1].T @ x, rows[2].T @ rows[3]
+        biases = (t.sum(0) if has else None for t, has in zip(rows, ctx.biases))
+        return dgate @ w_gate + dup @ w_up, *weights, *biases
+
+
+def swiglu_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None):
+    """w_down(silu(w_gate(x)) * w_up(x)), its activations kept in 8 bits until the backward.
+
+    x [..., K]; weights as nn.Linear holds them ([O, K]), all in x's dtype.  Between
+    forward and backward x and the two inner products live as bytes with a scale
+    per 128 elements and the gated product is rebuilt from them, about a third of
+    what 16-bit copies take.  The forward's result does not depend on it.
+    Reverse mode only.
+    """
+    tensors = [t for t in (x, w_gate, w_up, w_down, b_gate, b_up, b_down) if t is not None]
+    if any(t.dtype != x.dtype for t in tensors) or not x.is_floating_point():
+        raise ValueError("x, weights and biases must share a floating dtype")
+    if x.dim() < 1 or 0 in x.shape:
+        raise ValueError("nonempty tensors are required")
+    require_cuda(*tensors)
+    _lib.dtype_code(x)
+    if carries_tangent(*tensors):
+        raise RuntimeError("swiglu_ffn has no forward-mode derivative")
+    if not differentiated(*tensors):
+        return F.linear(swiglu(F.linear(x, w_gate, b_gate), F.linear(x, w_up, b_up)), w_down, b_down)
+    return SwigluFfnFunction.apply(x, w_gate, w_up, w_down, b_gate, b_up, b_down)
