@@ -53,6 +53,9 @@ struct NormArgs {
   float* partial;         // [teams][sums][D]
   int sums, sum_post, sum_gate;   // rows of a partial: weight 0, then post and gate where they are summed
   uint32_t share_rows, share_teams;   // rows of a share (one gate row's, or all), teams of a share
+  uint32_t teams, cols;   // teams in all, CTAs of a gradient row
+  void* dw;
+  void* dpost;
 };
 
 template <typename T, int TPR, int NV, bool A>
@@ -149,64 +152,33 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm_fwd_kernel(const _
   }
 }
 
-// A team's running sums of one parameter's gradient: in registers, or (wide
-// rows) in shared memory, where each thread touches its own columns only.
-template <int TPR, int NV, bool SMEM>
+// A team's running sums of one parameter's gradient for wide rows: in shared
+// memory, where each thread touches its own columns only.
+template <int TPR, bool A>
 struct Sums {
-  float v[SMEM ? 1 : NV][8];
   float* at;
-  __device__ __forceinline__ void init(float* base, int D, int t) {
-    at = base;
-    if constexpr (SMEM) {
-      for (int c = t; c < D; c += TPR) base[c] = 0.f;
-      __syncthreads();
-    } else {
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[j][e] = 0.f;
-    }
-  }
-  template <bool A>
   __device__ __forceinline__ void add(int j, int t, int D, const float (&x)[8], const float (&y)[8]) {
-    if constexpr (SMEM) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int c = column<TPR, A>(j, e, t);
-        if (c < D) at[c] = fmaf(x[e], y[e], at[c]);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[j][e] = fmaf(x[e], y[e], v[j][e]);
+    for (int e = 0; e < 8; ++e) {
+      const int c = column<TPR, A>(j, e, t);
+      if (c < D) at[c] = fmaf(x[e], y[e], at[c]);
     }
-  }
-  template <bool A>
-  __device__ __forceinline__ void store(float* out, int t, int D) const {
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int c = column<TPR, A>(j, e, t);
-        if (c < D) out[c] = SMEM ? at[c] : v[SMEM ? 0 : j][e];
-      }
   }
 };
 
-template <typename T, int TPR, int NV, bool A, bool SMEM>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm_bwd_kernel(const __grid_constant__ NormArgs a) {
-  constexpr int TEAMS = TPR < 128 ? 128 / TPR : 1;
+// The backward for wider rows, a CTA each, their operands read as they are needed.
+template <typename T, int TPR, int NV, bool A>
+__global__ void __launch_bounds__(TPR) norm_bwd_kernel(const __grid_constant__ NormArgs a) {
   extern __shared__ float sums[];
   __shared__ float red[2 * (TPR / 32)];
   int set = 0;
-  const int t = threadIdx.x % TPR, D = a.D;
-  const uint32_t team = blockIdx.x * TEAMS + threadIdx.x / TPR;
+  const int t = threadIdx.x, D = a.D;
+  const uint32_t team = blockIdx.x;
   const uint32_t share = team / a.share_teams, first = team - share * a.share_teams;
   const int64_t begin = int64_t(share) * a.share_rows;
-  if (begin >= a.rows) return;                    // a whole warp
-  Sums<TPR, NV, SMEM> dw, dp, dg;
-  dw.init(sums, D, t);
-  if (!SMEM || a.sum_post) dp.init(sums + D, D, t);
-  if (!SMEM || a.sum_gate) dg.init(sums + a.sum_gate * int64_t(D), D, t);
+  Sums<TPR, A> dw{sums}, dp{sums + a.sum_post * D}, dg{sums + a.sum_gate * D};
+  for (int c = t; c < a.sums * D; c += TPR) sums[c] = 0.f;
+  __syncthreads();
   for (uint32_t i = first; i < a.share_rows; i += a.share_teams) {
     const int64_t row = begin + i;
     Raw8<T> x[NV], dn[NV], dh[NV], y[NV];
@@ -249,7 +221,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm_bwd_kernel(const _
       widen8<T>(dn[j], s[j]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[j][e] *= inv_h;
-      dw.template add<A>(j, t, D, s[j], v[j]);
+      dw.add(j, t, D, s[j], v[j]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         s[j][e] *= w[e];
@@ -291,7 +263,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm_bwd_kernel(const _
 #pragma unroll
         for (int e = 0; e < 8; ++e) u[e] = a.post ? v[j][e] * p[e] : v[j][e];
         if (a.sum_gate) {
-          dg.template add<A>(j, t, D, s[j], u);
+          dg.add(j, t, D, s[j], u);
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e) u[e] *= s[j][e];
@@ -301,7 +273,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm_bwd_kernel(const _
         for (int e = 0; e < 8; ++e) s[j][e] *= g[j][e];
       }
       if (a.post) {
-        dp.template add<A>(j, t, D, s[j], v[j]);
+        dp.add(j, t, D, s[j], v[j]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           s[j][e] *= p[e];
@@ -320,35 +292,175 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm_bwd_kernel(const _
 #pragma unroll
     for (int j = 0; j < NV; ++j) store_piece<T, TPR, A>(dyr, j, t, D, s[j]);
   }
+  __syncthreads();
   float* out = a.partial + int64_t(team) * a.sums * D;
-  dw.template store<A>(out, t, D);
-  if (a.sum_post) dp.template store<A>(out + a.sum_post * int64_t(D), t, D);
-  if (a.sum_gate) dg.template store<A>(out + a.sum_gate * int64_t(D), t, D);
+  for (int c = t; c < a.sums * D; c += TPR) out[c] = sums[c];
 }
 
-// One parameter's gradient from the teams' partials, added in a fixed order:
-// 32 columns per CTA, eight warps over the partials.  Output row r is the sum of
-// `count` partials from r * count; `cols` CTAs share a row.
+// The backward for rows that a team holds with 8 elements per thread.  A team
+// keeps the parameters and their running sums in registers, and the next row's
+// operands are on their way while it works on one.  One barrier per row: the
+// second norm's sum follows from three that need no other,
+//   mean(s p z) with s = b g t  is  S2 - mean(dn w v) / rms(h) S3,
+//   S2 = mean(q (dh + dn w / rms(h))), S3 = mean(q v), q = b g p z.
+template <typename T, int TPR, bool A>
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm_bwd_row_kernel(const __grid_constant__ NormArgs a) {
+  constexpr int TEAMS = TPR < 128 ? 128 / TPR : 1, W = TPR / 32;
+  __shared__ float red[2][3][W];
+  int set = 0;
+  const int t = threadIdx.x % TPR, D = a.D;
+  const uint32_t team = blockIdx.x * TEAMS + threadIdx.x / TPR;
+  const uint32_t share = team / a.share_teams, first = team - share * a.share_teams;
+  const int64_t begin = int64_t(share) * a.share_rows;
+  if (begin >= a.rows) return;                    // a whole warp
+  const bool token_gate = a.gate && !a.gate_rows;
+  const char* gr = static_cast<const char*>(a.gate);
+  float w[8], p[8], g[8], dw[8], dp[8], dg[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) dw[e] = dp[e] = dg[e] = 0.f, p[e] = g[e] = 1.f;
+  param_piece<T, TPR, A>(a.w, a.w_f32, 0, t, D, w);
+  if (a.post) param_piece<T, TPR, A>(a.post, a.post_f32, 0, t, D, p);
+  // the rows of a share have one gate row
+  if (gr && !token_gate)
+    param_piece<T, TPR, A>(gr + int64_t(uint32_t(begin) / a.gate_rows) * a.gate_st * (a.gate_f32 ? 4 : int(sizeof(T))), a.gate_f32, 0, t,
+                           D, g);
+  struct Row {
+    Raw8<T> x, y, dn, dh, g;
+    float inv_y, inv_h;
+  };
+  Row next;
+  auto fetch = [&](int64_t row) {
+    next.x = load_piece<T, TPR, A>(static_cast<const T*>(a.x) + row * a.x_st, 0, t, D);
+    next.dn = load_piece<T, TPR, A>(static_cast<const T*>(a.dn) + row * D, 0, t, D);
+    if (a.dh) next.dh = load_piece<T, TPR, A>(static_cast<const T*>(a.dh) + row * D, 0, t, D);
+    if (a.y) next.y = load_piece<T, TPR, A>(static_cast<const T*>(a.y) + row * a.y_st, 0, t, D);
+    if (token_gate) next.g = load_piece<T, TPR, A>(reinterpret_cast<const T*>(gr) + row * a.gate_st, 0, t, D);
+    next.inv_y = a.stats[2 * row];
+    next.inv_h = a.stats[2 * row + 1];
+  };
+  fetch(begin + first);
+  for (uint32_t i = first; i < a.share_rows; i += a.share_teams) {
+    const int64_t row = begin + i;
+    const Row r = next;
+    if (a.share_rows - i > a.share_teams) fetch(row + a.share_teams);
+    float z[8], v[8], s[8], d[8], sums[3] = {0.f, 0.f, 0.f};
+    widen8<T>(r.x, v);
+    widen8<T>(r.dn, s);
+    if (a.dh) {
+      widen8<T>(r.dh, d);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d[e] = 0.f;
+    }
+    if (token_gate) widen8<T>(r.g, g);
+    if (a.y) {
+      widen8<T>(r.y, z);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (a.post) z[e] *= r.inv_y;
+        v[e] = fmaf(a.b, g[e] * (z[e] * p[e]), a.a * v[e]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[e] *= r.inv_h;
+      dw[e] = fmaf(s[e], v[e], dw[e]);
+      s[e] *= w[e];
+      sums[0] = fmaf(s[e], v[e], sums[0]);
+      if (a.post) {
+        const float q = a.b * g[e] * (p[e] * z[e]);
+        sums[1] = fmaf(q, fmaf(r.inv_h, s[e], d[e]), sums[1]);
+        sums[2] = fmaf(q, v[e], sums[2]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      if (k && !a.post) break;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sums[k] += __shfl_xor_sync(kFull, sums[k], o);
+    }
+    if constexpr (W > 1) {
+      if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+        for (int k = 0; k < 3; ++k) red[set][k][threadIdx.x >> 5] = sums[k];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        if (k && !a.post) break;
+        sums[k] = red[set][k][0];
+#pragma unroll
+        for (int x = 1; x < W; ++x) sums[k] += red[set][k][x];
+      }
+      set ^= 1;
+    }
+    const float mean = sums[0] * a.inv_d, mean_y = fmaf(-mean * r.inv_h, sums[2], sums[1]) * a.inv_d;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      s[e] = fmaf(fmaf(-v[e], mean, s[e]), r.inv_h, d[e]);
+      d[e] = a.a * s[e];
+      s[e] *= a.b;
+    }
+    store_piece<T, TPR, A>(static_cast<T*>(a.dx) + row * D, 0, t, D, d);
+    if (!a.y) continue;
+    if (gr) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        d[e] = s[e] * (z[e] * p[e]);
+        dg[e] += d[e];
+        s[e] *= g[e];
+      }
+      if (token_gate) store_piece<T, TPR, A>(static_cast<T*>(a.dgate) + row * D, 0, t, D, d);
+    }
+    if (a.post) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        dp[e] = fmaf(s[e], z[e], dp[e]);
+        s[e] = fmaf(-z[e], mean_y, s[e] * p[e]) * r.inv_y;
+      }
+    }
+    store_piece<T, TPR, A>(static_cast<T*>(a.dy) + row * D, 0, t, D, s);
+  }
+  float* out = a.partial + int64_t(team) * a.sums * D;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int c = column<TPR, A>(0, e, t);
+    if (c < D) {
+      out[c] = dw[e];
+      if (a.sum_post) out[a.sum_post * int64_t(D) + c] = dp[e];
+      if (a.sum_gate) out[a.sum_gate * int64_t(D) + c] = dg[e];
+    }
+  }
+}
+
+// The parameters' gradients from the teams' partials, added in a fixed order:
+// 32 columns of one gradient row per CTA, a warp for every 32nd partial.  The
+// rows: dw and dp over all teams, then dg of every share over its own.
 template <typename T>
-__global__ void __launch_bounds__(256) norm_sum_kernel(const float* partial, int64_t stride, uint32_t count, int D, uint32_t cols,
-                                                       void* out, int f32) {
-  __shared__ float buf[8][32];
+__global__ void __launch_bounds__(1024) norm_sum_kernel(const __grid_constant__ NormArgs a) {
+  __shared__ float buf[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t r = blockIdx.x / cols;
-  const int c = (blockIdx.x - r * cols) * 32 + lane;
+  const uint32_t r = blockIdx.x / a.cols;
+  const int c = (blockIdx.x - r * a.cols) * 32 + lane;
+  const uint32_t whole = a.sum_post ? 2 : 1;      // rows that all teams share
+  const bool is_gate = r >= whole;
+  const uint32_t count = is_gate ? a.share_teams : a.teams;
+  const int64_t from = is_gate ? int64_t(r - whole) * a.share_teams : 0, stride = int64_t(a.sums) * a.D;
   float v = 0.f;
-  if (c < D) {
-    const float* at = partial + int64_t(r) * count * stride + c;
-#pragma unroll 4
-    for (uint32_t p = warp; p < count; p += 8) v += at[p * stride];
+  if (c < a.D) {
+    const float* at = a.partial + from * stride + (is_gate ? a.sum_gate : r ? a.sum_post : 0) * int64_t(a.D) + c;
+#pragma unroll 8
+    for (uint32_t p = warp; p < count; p += 32) v += at[p * stride];
   }
   buf[warp][lane] = v;
   __syncthreads();
-  if (warp || c >= D) return;
+  if (warp || c >= a.D) return;
+  v = 0.f;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) v += buf[i][lane];
-  const int64_t at = int64_t(r) * D + c;
-  if (f32) static_cast<float*>(out)[at] = v;
+  for (int i = 0; i < 32; ++i) v += buf[i][lane];
+  const int64_t at = (is_gate ? int64_t(r - whole) * a.D : 0) + c;
+  void* out = is_gate ? a.dgate : r ? a.dpost : a.dw;
+  if (is_gate ? a.gate_f32 : r ? a.post_f32 : a.w_f32) static_cast<float*>(out)[at] = v;
   else static_cast<T*>(out)[at] = from_f32<T>(v);
 }
 
@@ -396,44 +508,38 @@ Plan make_plan(int64_t rows, int64_t D, int64_t share_rows) {
   return p;
 }
 
-template <typename T, int TPR, int NV, bool SMEM>
-int launch_bwd(const NormArgs& a, const Plan& p, bool aligned, cudaStream_t s) {
+template <typename T, int TPR>
+int launch_bwd_row(const NormArgs& a, const Plan& p, bool aligned, cudaStream_t s) {
   constexpr int threads = TPR < 128 ? 128 : TPR;
-  const size_t smem = SMEM ? sizeof(float) * a.sums * a.D : 0;
-  auto kernel = aligned ? norm_bwd_kernel<T, TPR, NV, true, SMEM> : norm_bwd_kernel<T, TPR, NV, false, SMEM>;
-  if (SMEM) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
-    if (e != cudaSuccess) return fail_cuda(e, "norm shared memory");
-  }
-  kernel<<<unsigned(p.ctas), threads, smem, s>>>(a);
+  if (aligned) norm_bwd_row_kernel<T, TPR, true><<<unsigned(p.ctas), threads, 0, s>>>(a);
+  else norm_bwd_row_kernel<T, TPR, false><<<unsigned(p.ctas), threads, 0, s>>>(a);
+  PISA_CHECK_LAUNCH();
+  return PISA_OK;
+}
+
+template <typename T, int NV, bool A>
+int launch_bwd(const NormArgs& a, const Plan& p, cudaStream_t s) {
+  if (int rc = allow_smem<norm_bwd_kernel<T, 512, NV, A>>(int(sizeof(float)) * 3 * NV * 4096, "norm backward smem attribute")) return rc;
+  norm_bwd_kernel<T, 512, NV, A><<<unsigned(p.ctas), 512, sizeof(float) * a.sums * a.D, s>>>(a);
   PISA_CHECK_LAUNCH();
   return PISA_OK;
 }
 
 template <typename T>
-int bwd(const NormArgs& a, const Plan& p, bool aligned, void* dweight, void* dpost, cudaStream_t s) {
+int bwd(NormArgs a, const Plan& p, bool aligned, cudaStream_t s) {
   int rc;
-  if (a.D <= 256) rc = launch_bwd<T, 32, 1, false>(a, p, aligned, s);
-  else if (a.D <= 1024) rc = launch_bwd<T, 128, 1, false>(a, p, aligned, s);
-  else if (a.D <= 2048) rc = launch_bwd<T, 256, 1, false>(a, p, aligned, s);
-  else if (a.D <= 4096) rc = launch_bwd<T, 512, 1, false>(a, p, aligned, s);
-  else if (a.D <= 8192) rc = launch_bwd<T, 512, 2, true>(a, p, aligned, s);
-  else rc = launch_bwd<T, 512, 4, true>(a, p, aligned, s);
+  if (a.D <= 256) rc = launch_bwd_row<T, 32>(a, p, aligned, s);
+  else if (a.D <= 1024) rc = launch_bwd_row<T, 128>(a, p, aligned, s);
+  else if (a.D <= 2048) rc = launch_bwd_row<T, 256>(a, p, aligned, s);
+  else if (a.D <= 4096) rc = launch_bwd_row<T, 512>(a, p, aligned, s);
+  else if (a.D <= 8192) rc = aligned ? launch_bwd<T, 2, true>(a, p, s) : launch_bwd<T, 2, false>(a, p, s);
+  else rc = aligned ? launch_bwd<T, 4, true>(a, p, s) : launch_bwd<T, 4, false>(a, p, s);
   if (rc) return rc;
-  const int64_t stride = int64_t(a.sums) * a.D;
-  const unsigned cols = unsigned((a.D + 31) / 32);
-  norm_sum_kernel<T><<<cols, 256, 0, s>>>(a.partial, stride, uint32_t(p.teams), a.D, cols, dweight, a.w_f32);
+  a.teams = uint32_t(p.teams);
+  a.cols = uint32_t((a.D + 31) / 32);
+  const int64_t rows = 1 + (a.sum_post ? 1 : 0) + (a.sum_gate ? p.shares : 0);
+  norm_sum_kernel<T><<<unsigned(a.cols * rows), 1024, 0, s>>>(a);
   PISA_CHECK_LAUNCH();
-  if (a.sum_post) {
-    norm_sum_kernel<T><<<cols, 256, 0, s>>>(a.partial + a.sum_post * int64_t(a.D), stride, uint32_t(p.teams), a.D, cols,
-                                            dpost, a.post_f32);
-    PISA_CHECK_LAUNCH();
-  }
-  if (a.sum_gate) {
-    norm_sum_kernel<T><<<unsigned(cols * p.shares), 256, 0, s>>>(a.partial + a.sum_gate * int64_t(a.D), stride, p.share_teams,
-                                                                 a.D, cols, a.dgate, a.gate_f32);
-    PISA_CHECK_LAUNCH();
-  }
   return PISA_OK;
 }
 
@@ -454,7 +560,7 @@ int check(const void* x, int64_t x_st, const void* y, const void* gate, int64_t 
       return fail(PISA_ERR_UNSUPPORTED, "the gate must have the tensors' type, or FP32 where rows share it");
     if (gate_rows < 0 || gate_rows > rows || (gate_rows && rows % gate_rows))
       return fail(PISA_ERR_INVALID, "gate rows must divide the rows");
-    if (gate_rows && rows / gate_rows * ((D + 31) / 32) >= (int64_t(1) << 31))
+    if (gate_rows && (rows / gate_rows + 2) * ((D + 31) / 32) >= (int64_t(1) << 31))
       return fail(PISA_ERR_UNSUPPORTED, "too many gate rows");
   }
   return PISA_OK;
@@ -525,6 +631,7 @@ int pisa_residual_norm_bwd(const void* dh, const void* dn, const void* x, int64_
   a.stats = const_cast<float*>(stats);
   a.dh = dh; a.dn = dn; a.dx = dx; a.dy = dbranch; a.dgate = dgate;
   a.partial = static_cast<float*>(workspace);
+  a.dw = dweight; a.dpost = dpost_weight;
   a.sums = 1;
   if (post_weight) a.sum_post = a.sums++;
   if (shared) a.sum_gate = a.sums++;
@@ -535,9 +642,9 @@ int pisa_residual_norm_bwd(const void* dh, const void* dn, const void* x, int64_
                        param_on16(dn) && param_on16(dx) && param_on16(dbranch) && param_on16(dgate) && param_on16(weight) &&
                        param_on16(post_weight);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == PISA_F32) return bwd<float>(a, p, aligned, dweight, dpost_weight, s);
-  if (dtype == PISA_BF16) return bwd<__nv_bfloat16>(a, p, aligned, dweight, dpost_weight, s);
-  return bwd<__half>(a, p, aligned, dweight, dpost_weight, s);
+  if (dtype == PISA_F32) return bwd<float>(a, p, aligned, s);
+  if (dtype == PISA_BF16) return bwd<__nv_bfloat16>(a, p, aligned, s);
+  return bwd<__half>(a, p, aligned, s);
 }
 
 }  // extern "C"

@@ -21,33 +21,49 @@ MAX_INNER = 1 << 17     # sums of fewer products of bytes fit 32 bits
 
 
 def rows_of(t):
-    """``t`` as [rows, width] with contiguous rows, a view wherever its strides allow one."""
-    width = t.shape[-1]
-    if t.stride(-1) != 1 and width != 1:
-        t = t.contiguous()
-    try:
-        t = t.view(-1, width)
-    except RuntimeError:
-        t = t.reshape(-1, width)
-    return t if t.stride(-1) == 1 else t.contiguous()
+    """(tensor, stride): ``t``, or a copy where its strides need one, whose rows are contiguous and lie ``stride`` elements apart."""
+    shape = t.shape
+    width = shape[-1]
+    if t.is_contiguous():
+        return t, width
+    if t.stride(-1) == 1 or width == 1:
+        stride, count = 0, 1      # of the rows so far, from the last dimension on
+        for n, step in zip(reversed(shape[:-1]), reversed(t.stride()[:-1])):
+            if n == 1:
+                continue
+            if count == 1:
+                stride = step
+            elif step != stride * count:
+                return t.contiguous(), width
+            count *= n
+        return t, stride if count > 1 else width
+    return t.contiguous(), width
+
+
+def row_bytes(width):
+    """Bytes from one int8 row to the next, so that all start on 16."""
+    return (width + 15) // 16 * 16
 
 
 def byte_rows(like, shape):
     """An int8 tensor of ``shape`` whose rows start on 16 bytes."""
     width = shape[-1]
-    return like.new_empty((*shape[:-1], -(-width // 16) * 16), dtype=torch.int8)[..., :width]
+    step = row_bytes(width)
+    rows = like.new_empty((*shape[:-1], step), dtype=torch.int8)
+    return rows if step == width else rows[..., :width]
 
 
-def _aligned_bytes(t):
-    """int8 rows [rows, width] that start on 16 bytes: ``t`` or a copy."""
-    if t.data_ptr() % 16 == 0 and (t.shape[0] == 1 or (t.stride(0) % 16 == 0 and t.stride(0) >= t.shape[1])):
-        return t
-    return byte_rows(t, t.shape).copy_(t)
+def aligned_bytes(t):
+    """rows_of for int8 rows that have to start on 16 bytes and not overlap."""
+    t, stride = rows_of(t)
+    if t.data_ptr() % 16 == 0 and (t.numel() == t.shape[-1] or (stride % 16 == 0 and stride >= t.shape[-1])):
+        return t, stride
+    return byte_rows(t, t.shape).copy_(t), row_bytes(t.shape[-1])
 
 
 def no_gradient(name, *tensors):
     """Refuses a call whose result a gradient would have to pass."""
-    if differentiated(*[t for t in tensors if t is not None]):
+    if differentiated(*tensors):
         raise ValueError(f"{name} is for inference: it has no gradient")
 
 
@@ -61,12 +77,13 @@ def _floating(x, name):
 
 
 def _quantize(x, code, grouped):
-    rows = rows_of(x)
-    values = byte_rows(x, x.shape)
-    groups = (-(-x.shape[-1] // GROUP),) if grouped else ()
-    scale = x.new_empty((*x.shape[:-1], *groups), dtype=torch.float32)
-    _lib.launch(_lib.lib().pisa_quantize_int8, x.get_device(), rows.data_ptr(), rows.stride(0), code, rows.shape[0],
-                rows.shape[1], int(grouped), values.data_ptr(), -(-x.shape[-1] // 16) * 16, scale.data_ptr())
+    shape = x.shape
+    width = shape[-1]
+    rows, stride = rows_of(x)
+    values = byte_rows(x, shape)
+    scale = x.new_empty((*shape[:-1], -(-width // GROUP)) if grouped else shape[:-1], dtype=torch.float32)
+    _lib.launch(_lib.lib().pisa_quantize_int8, x.get_device(), rows.data_ptr(), stride, code, x.numel() // width, width,
+                int(grouped), values.data_ptr(), row_bytes(width), scale.data_ptr())
     return values, scale
 
 
@@ -106,9 +123,9 @@ def restore_int8(values, scale, dtype):
         raise ValueError("values and scale must share a device")
     out = values.new_empty(values.shape, dtype=dtype)
     code = _lib.dtype_code(out)
-    rows, scale = _aligned_bytes(rows_of(values)), scale.contiguous()
-    _lib.launch(_lib.lib().pisa_restore_int8, values.get_device(), rows.data_ptr(), rows.stride(0), scale.data_ptr(), code,
-                rows.shape[0], rows.shape[1], out.data_ptr())
+    (rows, stride), scale = aligned_bytes(values), scale.contiguous()
+    _lib.launch(_lib.lib().pisa_restore_int8, values.get_device(), rows.data_ptr(), stride, scale.data_ptr(), code,
+                values.numel() // values.shape[-1], values.shape[-1], out.data_ptr())
     return out
 
 
@@ -132,39 +149,42 @@ def int8_linear(x, weight, weight_scale, bias=None, x_scale=None, out_dtype=None
         raise ValueError("nonempty tensors are required")
     if inner >= MAX_INNER:
         raise ValueError("sums of 131072 or more products may not fit 32 bits")
-    device = x.get_device()
-    if weight_scale.dtype != torch.float32 or weight_scale.shape != (outer,):
+    shape, device, whole = x.shape[:-1], x.get_device(), x.dtype == torch.int8
+    if weight_scale.dtype != torch.float32 or weight_scale.dim() != 1 or weight_scale.shape[0] != outer:
         raise ValueError("weight_scale must be fp32 with one element per output channel")
-    if (x_scale is not None) != (x.dtype == torch.int8):
+    if (x_scale is not None) != whole:
         raise ValueError("int8 x comes with x_scale, floating x without")
-    if x_scale is not None and (x_scale.dtype != torch.float32 or x_scale.shape != x.shape[:-1]):
+    if whole and (x_scale.dtype != torch.float32 or x_scale.shape != shape):
         raise ValueError("x_scale must be fp32 with one element per row of x")
     if out_dtype is None:
-        out_dtype = torch.bfloat16 if x.dtype == torch.int8 else x.dtype
+        out_dtype = torch.bfloat16 if whole else x.dtype
     if out_dtype not in _lib.DTYPES:
         raise ValueError("the CUDA kernels support FP16, BF16 and FP32")
-    if bias is not None and (bias.shape != (outer,) or bias.dtype not in (torch.float32, out_dtype)):
+    if bias is not None and (bias.dim() != 1 or bias.shape[0] != outer or bias.dtype not in (torch.float32, out_dtype)):
         raise ValueError("bias must have one element per output channel in fp32 or the output's dtype")
-    tensors = [t for t in (x, weight, weight_scale, x_scale, bias) if t is not None]
-    require_cuda(*tensors)
-    if any(t.get_device() != device for t in tensors):
-        raise ValueError("x, weight, scales and bias must share a device")
-    no_gradient("int8_linear", x, weight_scale, x_scale, bias)
-    shape = x.shape[:-1]
-    if x_scale is None:
+    for t in (x, weight, weight_scale, x_scale, bias):
+        if t is not None and t.get_device() != device:
+            require_cuda(t, x)
+            raise ValueError("x, weight, scales and bias must share a device")
+    require_cuda(x)
+    no_gradient("int8_linear", x, weight_scale, *([x_scale] if whole else []), *([] if bias is None else [bias]))
+    if not whole:
         x, x_scale = _quantize(x, _floating(x, "x"), False)
-    rows, weight = _aligned_bytes(rows_of(x)), _aligned_bytes(weight if weight.stride(1) == 1 else weight.contiguous())
+    count = x.numel() // inner
+    (rows, x_stride), (weight, w_stride) = aligned_bytes(x), aligned_bytes(weight)
     x_scale, weight_scale = x_scale.contiguous(), weight_scale.contiguous()
-    bias = None if bias is None else bias.contiguous()
+    bias_args = (None, 0)
+    if bias is not None:
+        bias = bias.contiguous()
+        bias_args = bias.data_ptr(), _lib.DTYPES[bias.dtype]
     out = x_scale.new_empty((*shape, outer), dtype=out_dtype)
     workspace, size = None, 0
     if _lib.status_checks():
-        size = _lib.workspace_bytes("pisa_int8_linear_workspace_bytes", device, rows.shape[0], inner, outer)
+        size = _lib.workspace_bytes("pisa_int8_linear_workspace_bytes", device, count, inner, outer)
         workspace = torch.empty(size, dtype=torch.uint8, device=x.device)
-    _lib.launch(_lib.lib().pisa_int8_linear, device, rows.data_ptr(), rows.stride(0), x_scale.data_ptr(), weight.data_ptr(),
-                weight.stride(0), weight_scale.data_ptr(), None if bias is None else bias.data_ptr(),
-                0 if bias is None else _lib.DTYPES[bias.dtype], _lib.DTYPES[out_dtype], rows.shape[0], inner, outer,
-                out.data_ptr(), None if workspace is None else workspace.data_ptr(), size)
+    _lib.launch(_lib.lib().pisa_int8_linear, device, rows.data_ptr(), x_stride, x_scale.data_ptr(), weight.data_ptr(), w_stride,
+                weight_scale.data_ptr(), *bias_args, _lib.DTYPES[out_dtype], count, inner, outer, out.data_ptr(),
+                None if workspace is None else workspace.data_ptr(), size)
     if workspace is not None:
         _lib.check_workspace(workspace, x.device)
     return out

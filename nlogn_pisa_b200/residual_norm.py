@@ -16,33 +16,42 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .dense import differentiated, flat
-from .int8 import byte_rows, no_gradient, rows_of
+from .int8 import byte_rows, no_gradient, row_bytes, rows_of
 from .validation import require_cuda
 
 
-def _row_args(rows):
-    return (None, 0) if rows is None else (rows.data_ptr(), rows.stride(0))
-
-
-def _param_args(weight):
-    return (None, 0) if weight is None else (weight.data_ptr(), _lib.DTYPES[weight.dtype])
+def _operands(x, branch, gate, gate_rows, post_weight, weight, scales):
+    """The arguments that both entry points take for the forward's operands, and tensors to keep until the launch."""
+    width = x.shape[-1]
+    x, x_st = rows_of(x)
+    args, kept = [x.data_ptr(), x_st, None, 0, None, 0, gate_rows, 0, None, 0], [x]
+    if branch is not None:
+        branch, stride = rows_of(branch)
+        args[2:4] = branch.data_ptr(), stride
+        kept.append(branch)
+        if gate is not None:
+            gate, stride = rows_of(gate)
+            args[4:8] = gate.data_ptr(), stride, gate_rows, _lib.DTYPES[gate.dtype]
+            kept.append(gate)
+        if post_weight is not None:
+            args[8:] = post_weight.data_ptr(), _lib.DTYPES[post_weight.dtype]
+    return (*args, weight.data_ptr(), _lib.DTYPES[weight.dtype], _lib.DTYPES[x.dtype], x.numel() // width, width, *scales), kept
 
 
 def _forward(x, branch, gate, post_weight, weight, gate_rows, scales, eps, quantize, want_stats):
-    """x, branch, gate as rows; h, n (or its bytes and scales) and the row statistics, as rows."""
-    count, width = x.shape
-    h = None if branch is None else x.new_empty(count, width)
-    n = scale = stats = None
+    """h, n (or its bytes and scales) and the row statistics."""
+    operands, _kept = _operands(x, branch, gate, gate_rows, post_weight, weight, scales)
+    h = None if branch is None else x.new_empty(x.shape)
+    scale = stats = None
     if quantize:
-        n, scale = byte_rows(x, (count, width)), x.new_empty(count, dtype=torch.float32)
+        n, scale = byte_rows(x, x.shape), x.new_empty(x.shape[:-1], dtype=torch.float32)
+        out = None, n.data_ptr(), row_bytes(x.shape[-1]), scale.data_ptr()
     else:
-        n = x.new_empty(count, width)
+        n = x.new_empty(x.shape)
+        out = n.data_ptr(), None, 0, None
     if want_stats:
-        stats = x.new_empty((count, 2), dtype=torch.float32)
-    out = (None, n.data_ptr(), -(-width // 16) * 16, scale.data_ptr()) if quantize else (n.data_ptr(), None, 0, None)
-    _lib.launch(_lib.lib().pisa_residual_norm, x.get_device(), *_row_args(x), *_row_args(branch), *_row_args(gate), gate_rows,
-                0 if gate is None else _lib.DTYPES[gate.dtype], *_param_args(post_weight), *_param_args(weight),
-                _lib.DTYPES[x.dtype], count, width, *scales, eps, None if h is None else h.data_ptr(), *out,
+        stats = x.new_empty((*x.shape[:-1], 2), dtype=torch.float32)
+    _lib.launch(_lib.lib().pisa_residual_norm, x.get_device(), *operands, eps, None if h is None else h.data_ptr(), *out,
                 None if stats is None else stats.data_ptr())
     return h, n, scale, stats
 
@@ -50,16 +59,11 @@ def _forward(x, branch, gate, post_weight, weight, gate_rows, scales, eps, quant
 class ResidualNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, branch, gate, post_weight, weight, gate_rows, scales, eps):
-        rows = [None if t is None else rows_of(t) for t in (x, branch, gate)]
-        h, n, _, stats = _forward(*rows, post_weight, weight, gate_rows, scales, eps, False, True)
-        n = n.view(x.shape)
+        h, n, _, stats = _forward(x, branch, gate, post_weight, weight, gate_rows, scales, eps, False, True)
         ctx.args = gate_rows, scales
         ctx.set_materialize_grads(False)
-        if branch is None:
-            ctx.save_for_backward(x, None, None, None, weight, stats)
-            return n
         ctx.save_for_backward(x, branch, gate, post_weight, weight, stats)
-        return h.view(x.shape), n
+        return n if branch is None else (h, n)
 
     @staticmethod
     @once_differentiable
@@ -71,31 +75,33 @@ class ResidualNormFunction(torch.autograd.Function):
             return (None,) * 8
         dn = torch.zeros_like(x, memory_format=torch.contiguous_format) if dn is None else flat(dn)
         dh = None if dh is None else flat(dh)
-        rows, branch_rows, gate_view = (None if t is None else rows_of(t) for t in (x, branch, gate))
-        count, width = rows.shape
-        dx = x.new_empty(x.shape)
-        dbranch = None if branch is None else x.new_empty(x.shape)
-        dgate = None if gate is None else gate.new_empty(gate.shape)
-        dpost, dweight = (None if w is None else w.new_empty(w.shape) for w in (post_weight, weight))
-        size = _lib.workspace_bytes("pisa_residual_norm_bwd_workspace_bytes", x.get_device(), count, width,
+        operands, _kept = _operands(x, branch, gate, gate_rows, post_weight, weight, scales)
+        dx, dweight = x.new_empty(x.shape), torch.empty_like(weight)
+        dbranch = dgate = dpost = None
+        if branch is not None:
+            dbranch = x.new_empty(x.shape)
+            dgate = None if gate is None else gate.new_empty(gate.shape)
+            dpost = None if post_weight is None else torch.empty_like(post_weight)
+        width = x.shape[-1]
+        size = _lib.workspace_bytes("pisa_residual_norm_bwd_workspace_bytes", x.get_device(), x.numel() // width, width,
                                     0 if gate is None else gate_rows)
         workspace = x.new_empty(size, dtype=torch.uint8)
-        pointers = [None if t is None else t.data_ptr() for t in (dx, dbranch, dgate, dpost, dweight)]
         _lib.launch(_lib.lib().pisa_residual_norm_bwd, x.get_device(), None if dh is None else dh.data_ptr(), dn.data_ptr(),
-                    *_row_args(rows), *_row_args(branch_rows), *_row_args(gate_view), gate_rows,
-                    0 if gate is None else _lib.DTYPES[gate.dtype], *_param_args(post_weight), *_param_args(weight),
-                    _lib.DTYPES[x.dtype], count, width, *scales, stats.data_ptr(), *pointers, workspace.data_ptr(), size)
+                    *operands, stats.data_ptr(), dx.data_ptr(), *(None if t is None else t.data_ptr() for t in (dbranch, dgate, dpost)),
+                    dweight.data_ptr(), workspace.data_ptr(), size)
         return dx, dbranch, dgate, dpost, dweight, None, None, None
 
 
 def _gate_rows(gate, x):
     """How many rows share a row of the gate (0: a gate of x's own shape and dtype)."""
-    if gate.shape == x.shape and gate.dtype == x.dtype:
+    shape, of = x.shape, gate.shape
+    if of == shape and gate.dtype == x.dtype:
         return 0
-    if gate.numel() == x.shape[-1] and gate.shape[-1] == x.shape[-1]:
-        return x.numel() // x.shape[-1]
-    if gate.shape == (*x.shape[:-2], 1, x.shape[-1]):
-        return x.shape[-2]
+    if of and of[-1] == shape[-1]:
+        if gate.numel() == shape[-1]:
+            return x.numel() // shape[-1]
+        if of[-2] == 1 and of[:-2] == shape[:-2]:
+            return shape[-2]
     raise ValueError("gate must have shape [D], [..., 1, D] or x's shape (then in x's dtype)")
 
 
@@ -116,43 +122,48 @@ def residual_norm(x, branch, weight, post_weight=None, gate=None, residual_scale
     ``quantize``: (h, values, scale) with n in 8 bits, as ``quantize_int8`` of its
     fp32 values, for ``int8_linear``; for inference only.
     """
-    if x.dim() < 2 or 0 in x.shape:
+    shape, dtype, device = x.shape, x.dtype, x.get_device()
+    if len(shape) < 2 or 0 in shape:
         raise ValueError("x must have shape [..., tokens, D] and be nonempty")
-    width, device = x.shape[-1], x.get_device()
-    if not x.is_floating_point():
+    if not dtype.is_floating_point:
         raise ValueError("x must be floating")
+    tensors = [x, weight]
     if branch is None:
         if gate is not None or post_weight is not None or residual_scale != 1.0 or branch_scale != 1.0:
             raise ValueError("a gate, a post weight and scales belong to a branch")
-    elif branch.shape != x.shape or branch.dtype != x.dtype:
-        raise ValueError("branch must share x's shape and dtype")
-    for name, w in (("weight", weight), ("post_weight", post_weight)):
-        if w is not None and (w.shape != (width,) or w.dtype not in (torch.float32, x.dtype)):
-            raise ValueError(f"{name} must have D elements in fp32 or x's dtype")
+    else:
+        if branch.shape != shape or branch.dtype != dtype:
+            raise ValueError("branch must share x's shape and dtype")
+        tensors.append(branch)
+    if weight.dim() != 1 or weight.shape[0] != shape[-1] or weight.dtype not in (torch.float32, dtype):
+        raise ValueError("weight must have D elements in fp32 or x's dtype")
+    weight = weight.contiguous()
+    if post_weight is not None:
+        if post_weight.dim() != 1 or post_weight.shape[0] != shape[-1] or post_weight.dtype not in (torch.float32, dtype):
+            raise ValueError("post_weight must have D elements in fp32 or x's dtype")
+        post_weight = post_weight.contiguous()
+        tensors.append(post_weight)
     gate_rows = 0
     if gate is not None:
         gate_rows = _gate_rows(gate, x)
-        if gate.dtype not in (torch.float32, x.dtype):
+        if gate.dtype not in (torch.float32, dtype):
             raise ValueError("gate must be in fp32 or x's dtype")
-    tensors = [t for t in (x, branch, gate, post_weight, weight) if t is not None]
-    require_cuda(*tensors)
-    if any(t.get_device() != device for t in tensors):
-        raise ValueError("all tensors must share a device")
+        tensors.append(gate)
+    for t in tensors:
+        if t.get_device() != device:
+            require_cuda(*tensors)
+            raise ValueError("all tensors must share a device")
+    require_cuda(x)
     _lib.dtype_code(x)
     scales, eps = (float(residual_scale), float(branch_scale)), float(eps)
-    if not all(math.isfinite(s) for s in scales):
+    if not (math.isfinite(scales[0]) and math.isfinite(scales[1])):
         raise ValueError("scales must be finite")
-    weight = weight.contiguous()
-    post_weight = None if post_weight is None else post_weight.contiguous()
     if quantize:
         no_gradient("quantize=True", *tensors)
     elif differentiated(*tensors):
         if branch is None:
             return x, ResidualNormFunction.apply(x, None, None, None, weight, 0, scales, eps)
         return ResidualNormFunction.apply(x, branch, gate, post_weight, weight, gate_rows, scales, eps)
-    rows = [None if t is None else rows_of(t) for t in (x, branch, gate)]
-    h, n, scale, _ = _forward(*rows, post_weight, weight, gate_rows, scales, eps, quantize, False)
-    h = x if h is None else h.view(x.shape)
-    if quantize:
-        return h, n.view(x.shape), scale.view(x.shape[:-1])
-    return h, n.view(x.shape)
+    h, n, scale, _ = _forward(x, branch, gate, post_weight, weight, gate_rows, scales, eps, quantize, False)
+    h = x if branch is None else h
+    return (h, n, scale) if quantize else (h, n)

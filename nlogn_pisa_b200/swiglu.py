@@ -15,40 +15,45 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .dense import carries_tangent, differentiated
-from .int8 import GROUP, byte_rows, checkpoint_int8, no_gradient, restore_int8, rows_of
+from .int8 import GROUP, byte_rows, checkpoint_int8, no_gradient, restore_int8, row_bytes, rows_of
 from .validation import require_cuda
 
 
+def _kept_args(kept, count, width):
+    """Pointers into the buffer that holds gate and up in 8 bits: bytes of both, then scales of both."""
+    step, groups = row_bytes(width), (width + GROUP - 1) // GROUP
+    at = kept.data_ptr()
+    scales = at + 2 * count * step
+    return at, at + count * step, step, scales, scales + 4 * count * groups
+
+
 def _forward(gate, up, keep):
-    """The product, and gate and up in 8 bits: (values, scale) of each, as rows."""
-    rows = rows_of(gate), rows_of(up)
-    count, width = rows[0].shape
-    out, kept = gate.new_empty(gate.shape), (None,) * 4
-    pointers = (None, None, 0, None, None)
+    """The product, and the buffer that keeps gate and up in 8 bits, or None."""
+    width = gate.shape[-1]
+    (rows, g_st), (up_rows, u_st), count = rows_of(gate), rows_of(up), gate.numel() // width
+    out, kept, pointers = gate.new_empty(gate.shape), None, (None, None, 0, None, None)
     if keep:
-        values = [byte_rows(gate, (count, width)) for _ in range(2)]
-        scale = [gate.new_empty((count, -(-width // GROUP)), dtype=torch.float32) for _ in range(2)]
-        kept = (*values, *scale)
-        pointers = (values[0].data_ptr(), values[1].data_ptr(), -(-width // 16) * 16, scale[0].data_ptr(), scale[1].data_ptr())
-    _lib.launch(_lib.lib().pisa_swiglu, gate.get_device(), rows[0].data_ptr(), rows[0].stride(0), rows[1].data_ptr(),
-                rows[1].stride(0), _lib.DTYPES[gate.dtype], count, width, out.data_ptr(), *pointers, None, 0, None)
+        size = 2 * count * (row_bytes(width) + 4 * ((width + GROUP - 1) // GROUP))
+        kept = gate.new_empty(size, dtype=torch.int8)
+        pointers = _kept_args(kept, count, width)
+    _lib.launch(_lib.lib().pisa_swiglu, gate.get_device(), rows.data_ptr(), g_st, up_rows.data_ptr(), u_st,
+                _lib.DTYPES[gate.dtype], count, width, out.data_ptr(), *pointers, None, 0, None)
     return out, kept
 
 
 def _backward(dout, gate, up, kept, want_out=False):
     """(dgate, dup, and the product again or None) from gate and up, or from what was kept of them."""
-    rows = rows_of(dout)
-    count, width = rows.shape
+    width = dout.shape[-1]
+    (rows, stride), count = rows_of(dout), dout.numel() // width
     dgate, dup = dout.new_empty(dout.shape), dout.new_empty(dout.shape)
     out = dout.new_empty(dout.shape) if want_out else None
     if kept is None:
-        gate, up = rows_of(gate), rows_of(up)
-        given = (gate.data_ptr(), gate.stride(0), up.data_ptr(), up.stride(0), None, None, 0, None, None)
+        (gate, g_st), (up, u_st) = rows_of(gate), rows_of(up)
+        given = (gate.data_ptr(), g_st, up.data_ptr(), u_st, None, None, 0, None, None)
     else:
-        given = (None, 0, None, 0, kept[0].data_ptr(), kept[1].data_ptr(), -(-width // 16) * 16, kept[2].data_ptr(),
-                 kept[3].data_ptr())
-    _lib.launch(_lib.lib().pisa_swiglu_bwd, dout.get_device(), rows.data_ptr(), rows.stride(0), *given, _lib.DTYPES[dout.dtype],
-                count, width, dgate.data_ptr(), dup.data_ptr(), None if out is None else out.data_ptr())
+        given = (None, 0, None, 0, *_kept_args(kept, count, width))
+    _lib.launch(_lib.lib().pisa_swiglu_bwd, dout.get_device(), rows.data_ptr(), stride, *given, _lib.DTYPES[dout.dtype], count,
+                width, dgate.data_ptr(), dup.data_ptr(), None if out is None else out.data_ptr())
     return dgate, dup, out
 
 
@@ -56,15 +61,17 @@ class SwigluFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate, up, keep):
         out, kept = _forward(gate, up, keep)
-        ctx.keep = keep
-        ctx.save_for_backward(*(kept if keep else (gate, up)))
+        if keep:
+            ctx.save_for_backward(kept)
+        else:
+            ctx.save_for_backward(gate, up)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
         saved = ctx.saved_tensors
-        dgate, dup, _ = _backward(dout, None, None, saved) if ctx.keep else _backward(dout, *saved, None)
+        dgate, dup, _ = _backward(dout, None, None, *saved) if len(saved) == 1 else _backward(dout, *saved, None)
         return dgate, dup, None
 
 
@@ -94,12 +101,12 @@ def swiglu(gate, up, checkpoint_bits=None, quantize=False):
     code = _lib.dtype_code(gate)
     if quantize:
         no_gradient("quantize=True", gate, up)
-        rows = rows_of(gate), rows_of(up)
-        count, width = rows[0].shape
+        width = gate.shape[-1]
+        (rows, g_st), (up_rows, u_st) = rows_of(gate), rows_of(up)
         values, scale = byte_rows(gate, gate.shape), gate.new_empty(gate.shape[:-1], dtype=torch.float32)
-        _lib.launch(_lib.lib().pisa_swiglu, gate.get_device(), rows[0].data_ptr(), rows[0].stride(0), rows[1].data_ptr(),
-                    rows[1].stride(0), code, count, width, None, None, None, 0, None, None, values.data_ptr(),
-                    -(-width // 16) * 16, scale.data_ptr())
+        _lib.launch(_lib.lib().pisa_swiglu, gate.get_device(), rows.data_ptr(), g_st, up_rows.data_ptr(), u_st, code,
+                    gate.numel() // width, width, None, None, None, 0, None, None, values.data_ptr(), row_bytes(width),
+                    scale.data_ptr())
         return values, scale
     if differentiated(gate, up):
         return SwigluFunction.apply(gate, up, keep)
@@ -114,13 +121,13 @@ class SwigluFfnFunction(torch.autograd.Function):
         out, kept = _forward(F.linear(x, w_gate, b_gate), F.linear(x, w_up, b_up), True)
         ctx.dtype = x.dtype
         ctx.biases = tuple(b is not None for b in (b_gate, b_up, b_down))
-        ctx.save_for_backward(*checkpoint_int8(x), *kept, w_gate, w_up, w_down)
+        ctx.save_for_backward(*checkpoint_int8(x), kept, w_gate, w_up, w_down)
         return F.linear(out, w_down, b_down)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x_values, x_scale, *kept, w_gate, w_up, w_down = ctx.saved_tensors
+        x_values, x_scale, kept, w_gate, w_up, w_down = ctx.saved_tensors
         dgate, dup, out = _backward(dy @ w_down, None, None, kept, True)
         rows = [t.reshape(-1, t.shape[-1]) for t in (dgate, dup, dy, out)]
         x = restore_int8(x_values, x_scale, ctx.dtype).view(-1, x_values.shape[-1])

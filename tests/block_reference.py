@@ -70,6 +70,7 @@ def residual_norm(x, branch, weight, post=None, gate=None, a=1.0, b=1.0, eps=1e-
     s = dn * weight
     m = (s * v).mean(-1, keepdim=True)
     em = (s.abs() * ev + (ROW + 4 * EPS) * (s * v).abs()).mean(-1, keepdim=True)
+    first = m
     t = dh + (s - v * m) * inv
     et = inv * (ev * m.abs() + v.abs() * em + (einv + 8 * EPS) * (s.abs() + (v * m).abs())) + 2 * EPS * dh.abs()
     found["dx"] = (a * t, u * (a * t).abs() + abs(a) * et * 1.01 + EPS * (a * t).abs() + tiny)
@@ -90,7 +91,10 @@ def residual_norm(x, branch, weight, post=None, gate=None, a=1.0, b=1.0, eps=1e-
                                                          + (EPS * (rows + 64) + ROW) * (s * z).abs().sum(lead)) * 1.01)
             es, s = es * post.abs() + EPS * (s * post).abs(), s * post
             m = (s * z).mean(-1, keepdim=True)
-            em = (es * z.abs() + 2 * ROW * (s * z).abs()).mean(-1, keepdim=True)
+            # this row sum may be taken in the parts that make up s: their magnitudes, not the sum's, carry its rounding
+            parts = (abs(b) * (post * z).abs() * (1.0 if gate is None else gate.abs())
+                     * (dh.abs() + inv * ((dn * weight).abs() + (v * first).abs())))
+            em = (es * z.abs() + 2 * ROW * (s * z).abs() + ROW * parts).mean(-1, keepdim=True)
             es = inv_y * (es + z.abs() * em + (2 * ROW + 8 * EPS) * (s.abs() + (z * m).abs()))
             s = (s - z * m) * inv_y
         found["dbranch"] = (s, u * s.abs() + es * 1.01 + tiny)
