@@ -14,8 +14,9 @@ struct RowArgs {
   const void* x;
   int64_t x_st;
   int64_t rows;
+  uint32_t items;         // groups of all rows
   int64_t D;
-  uint32_t groups;
+  FastDiv groups;
   int8_t* q;
   int64_t q_st;
   float* scale;
@@ -110,35 +111,15 @@ constexpr int kThreads = 256;
 template <typename T, bool A, bool BACK>
 __global__ void __launch_bounds__(kThreads) group_kernel(const __grid_constant__ RowArgs a) {
   const int t = threadIdx.x & 15;
-  const int64_t item = int64_t(blockIdx.x) * (kThreads / 16) + (threadIdx.x >> 4);
-  const bool live = item < a.rows * a.groups;
-  const uint64_t at = live ? uint64_t(item) : 0;
-  const int64_t row = int64_t(at / a.groups), first = int64_t(at - uint64_t(row) * a.groups) * kGroup;
+  const uint32_t item = blockIdx.x * (kThreads / 16) + (threadIdx.x >> 4);
+  const bool live = item < a.items;
+  const uint32_t at = live ? item : 0;
+  const int64_t row = a.groups.div(at), first = int64_t(at - uint32_t(row) * a.groups.d) * kGroup;
   const int width = live ? int(min64(kGroup, a.D - first)) : 0;
   int8_t* qr = a.q + row * a.q_st + first;
   float f[8];
   if constexpr (BACK) {
-    uint2 r = make_uint2(0, 0);
-    if constexpr (A) {
-      if (t * 8 < width) r = *reinterpret_cast<const uint2*>(qr + t * 8);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int c = column<16, A>(0, e, t);
-        const uint32_t b = c < width ? uint8_t(qr[c]) : 0;
-        if (e < 4) r.x |= b << (8 * e);
-        else r.y |= b << (8 * (e - 4));
-      }
-    }
-    const float scale = a.scale[at];
-    float lo[4], hi[4];
-    unpack_s8(r.x, lo);
-    unpack_s8(r.y, hi);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      f[e] = lo[e] * scale;
-      f[4 + e] = hi[e] * scale;
-    }
+    widen8_s8(load_piece_s8<16, A>(qr, t, width), a.scale[at], f);
     store_piece<T, 16, A>(static_cast<T*>(a.out) + row * a.D + first, 0, t, width, f);
   } else {
     widen8<T>(load_piece<T, 16, A>(static_cast<const T*>(a.x) + row * a.x_st + first, 0, t, width), f);
@@ -155,7 +136,7 @@ __global__ void __launch_bounds__(kThreads) group_kernel(const __grid_constant__
 
 template <typename T, bool BACK>
 int groups8(const RowArgs& a, bool aligned, cudaStream_t s) {
-  const int64_t items = a.rows * a.groups, per = kThreads / 16;
+  const int64_t items = a.rows * a.groups.d, per = kThreads / 16;
   const unsigned ctas = unsigned((items + per - 1) / per);
   if (aligned) group_kernel<T, true, BACK><<<ctas, kThreads, 0, s>>>(a);
   else group_kernel<T, false, BACK><<<ctas, kThreads, 0, s>>>(a);
@@ -166,7 +147,7 @@ int groups8(const RowArgs& a, bool aligned, cudaStream_t s) {
 int check(const void* x, const int8_t* q, int64_t q_st, const float* scale, int dtype, int64_t rows, int64_t D) {
   if (dtype < PISA_F32 || dtype > PISA_F16) return fail(PISA_ERR_UNSUPPORTED, "the kernels support FP16, BF16 and FP32");
   if (rows <= 0 || D <= 0) return fail(PISA_ERR_INVALID, "nonempty tensors are required");
-  if (rows >= (int64_t(1) << 31) || D >= (int64_t(1) << 31) || rows * ((D + kGroup - 1) / kGroup) >= (int64_t(1) << 34))
+  if (rows >= (int64_t(1) << 31) || D >= (int64_t(1) << 31) || rows * ((D + kGroup - 1) / kGroup) >= (int64_t(1) << 31) - 256)
     return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
   if (!x || !q || !scale) return fail(PISA_ERR_INVALID, "the tensor, its bytes and scales are required");
   if (!rows_on16(q, rows, q_st)) return fail(PISA_ERR_UNSUPPORTED, "8-bit rows must start on 16 bytes");
@@ -175,7 +156,7 @@ int check(const void* x, const int8_t* q, int64_t q_st, const float* scale, int 
 
 RowArgs make_args(int64_t rows, int64_t D, int8_t* q, int64_t q_st, float* scale) {
   RowArgs a{};
-  a.rows = rows; a.D = D; a.groups = uint32_t((D + kGroup - 1) / kGroup); a.q = q; a.q_st = q_st; a.scale = scale;
+  a.rows = rows; a.D = D; a.groups = FastDiv::make(uint32_t((D + kGroup - 1) / kGroup)); a.items = uint32_t(rows) * a.groups.d; a.q = q; a.q_st = q_st; a.scale = scale;
   return a;
 }
 

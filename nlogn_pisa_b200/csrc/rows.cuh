@@ -245,6 +245,34 @@ __device__ __forceinline__ void store_piece_s8(int8_t* row, int j, int t, int D,
   }
 }
 
+// Piece 0 of kept bytes, zeros past their end, and as floats.
+template <int TPR, bool A>
+__device__ __forceinline__ uint2 load_piece_s8(const int8_t* row, int t, int D) {
+  uint2 r = make_uint2(0, 0);
+  if constexpr (A) {
+    if (t * 8 < D) asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(row + t * 8));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int c = column<TPR, A>(0, e, t);
+      const uint32_t b = c < D ? uint8_t(row[c]) : 0;
+      if (e < 4) r.x |= b << (8 * e);
+      else r.y |= b << (8 * (e - 4));
+    }
+  }
+  return r;
+}
+__device__ __forceinline__ void widen8_s8(const uint2& q, float scale, float (&f)[8]) {
+  float lo[4], hi[4];
+  unpack_s8(q.x, lo);
+  unpack_s8(q.y, hi);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    f[e] = lo[e] * scale;
+    f[4 + e] = hi[e] * scale;
+  }
+}
+
 // Host: whether a row view starts every row on 16 bytes (the stride of a single row may hold anything).
 inline bool rows_on16(const void* p, int64_t rows, int64_t stride_bytes) {
   return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (rows == 1 || stride_bytes % 16 == 0);

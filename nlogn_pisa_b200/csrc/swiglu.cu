@@ -26,8 +26,9 @@ struct GluArgs {
   const void* u;
   int64_t u_st;
   int64_t rows;
+  uint32_t items;         // groups of all rows
   int D;
-  uint32_t groups;        // groups of 128 of a row
+  FastDiv groups;         // groups of 128 of a row
   void* out;              // contiguous [rows, D]
   int8_t* g_q;            // kept bytes, rows q_st apart, and scales [rows, groups]
   int8_t* u_q;
@@ -45,10 +46,16 @@ struct GluArgs {
   float* a_scale;
 };
 
+__device__ __forceinline__ float fast_rcp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 template <typename T>
 __device__ __forceinline__ float sigmoid(float x) {
   if constexpr (std::is_same<T, float>::value) return 1.f / (1.f + expf(-x));
-  else return __fdividef(1.f, 1.f + __expf(-x));   // 0 where the sum passes 2^126
+  else return fast_rcp(1.f + __expf(-x));
 }
 
 // Maximum over the sixteen threads of a group, NaN if any is.
@@ -65,90 +72,100 @@ __device__ __forceinline__ float largest8(const float (&f)[8]) {
   return top;
 }
 
-// The eight kept values of a thread.  A group of a row is a row of 128 to its sixteen threads.
-template <bool A>
-__device__ __forceinline__ void load8(const int8_t* q, float scale, int t, int width, float (&f)[8]) {
-  uint2 r = make_uint2(0, 0);
-  if constexpr (A) {
-    if (t * 8 < width) asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(q + t * 8));
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int c = column<16, A>(0, e, t);
-      const uint32_t b = c < width ? uint8_t(q[c]) : 0;
-      if (e < 4) r.x |= b << (8 * e);
-      else r.y |= b << (8 * (e - 4));
-    }
-  }
-  float lo[4], hi[4];
-  unpack_s8(r.x, lo);
-  unpack_s8(r.y, hi);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    f[e] = lo[e] * scale;
-    f[4 + e] = hi[e] * scale;
-  }
-}
+constexpr int kGluThreads = 256, kGluTeams = kGluThreads / 16;
 
-constexpr int kGluThreads = 256;
+// Where group `u` of a team's U lies; a group past the last has no elements.
+template <int U>
+struct GluGroup {
+  uint32_t at;
+  int64_t row;
+  int first, width;
+  __device__ __forceinline__ GluGroup(const GluArgs& a, int u) {
+    const uint32_t item = (blockIdx.x * U + u) * kGluTeams + (threadIdx.x >> 4);
+    const bool live = item < a.items;
+    at = live ? item : 0;
+    row = a.groups.div(at);
+    first = int(at - uint32_t(row) * a.groups.d) * kGroup;
+    width = live ? min(kGroup, a.D - first) : 0;
+  }
+};
 
-// Sixteen threads per group of a row; whole warps run on (the maxima need them) with nothing to load or store.
-template <typename T, bool A, bool KEEP>
+// Sixteen threads per group; all of a thread's loads are under way before its first use.
+template <typename T, int U, bool A, bool KEEP>
 __global__ void __launch_bounds__(kGluThreads) glu_fwd_kernel(const __grid_constant__ GluArgs a) {
   const int t = threadIdx.x & 15;
-  const int64_t item = int64_t(blockIdx.x) * (kGluThreads / 16) + (threadIdx.x >> 4);
-  const bool live = item < a.rows * a.groups;
-  const uint64_t at = live ? uint64_t(item) : 0;
-  const int64_t row = int64_t(at / a.groups);
-  const int first = int(at - uint64_t(row) * a.groups) * kGroup;
-  const int width = live ? min(kGroup, a.D - first) : 0;
-  const Raw8<T> gr = load_piece<T, 16, A>(static_cast<const T*>(a.g) + row * a.g_st + first, 0, t, width);
-  const Raw8<T> ur = load_piece<T, 16, A>(static_cast<const T*>(a.u) + row * a.u_st + first, 0, t, width);
-  float g[8], u[8], o[8];
-  widen8<T>(gr, g);
-  widen8<T>(ur, u);
+  Raw8<T> gr[U], ur[U];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) o[e] = g[e] * sigmoid<T>(g[e]) * u[e];
-  store_piece<T, 16, A>(static_cast<T*>(a.out) + row * a.D + first, 0, t, width, o);
-  if constexpr (KEEP) {
-    const float top_g = group_max(largest8(g)), top_u = group_max(largest8(u));
-    const Scale8 sg(top_g), su(top_u);
-    store_piece_s8<16, A>(a.g_q + row * a.q_st + first, 0, t, width, g, top_g < INFINITY, sg.inv);
-    store_piece_s8<16, A>(a.u_q + row * a.q_st + first, 0, t, width, u, top_u < INFINITY, su.inv);
-    if (live && t == 0) {
-      a.g_scale[at] = sg.scale;
-      a.u_scale[at] = su.scale;
+  for (int i = 0; i < U; ++i) {
+    const GluGroup<U> n(a, i);
+    gr[i] = load_piece<T, 16, A>(static_cast<const T*>(a.g) + n.row * a.g_st + n.first, 0, t, n.width);
+    ur[i] = load_piece<T, 16, A>(static_cast<const T*>(a.u) + n.row * a.u_st + n.first, 0, t, n.width);
+  }
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const GluGroup<U> n(a, i);
+    float g[8], u[8], o[8];
+    widen8<T>(gr[i], g);
+    widen8<T>(ur[i], u);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = g[e] * sigmoid<T>(g[e]) * u[e];
+    store_piece<T, 16, A>(static_cast<T*>(a.out) + n.row * a.D + n.first, 0, t, n.width, o);
+    if constexpr (KEEP) {
+      const float top_g = group_max(largest8(g)), top_u = group_max(largest8(u));
+      // Scale8 of both: its four quotients are four lanes' (a quotient costs more than a shuffle)
+      const float m = fmaxf(t & 1 ? top_u : top_g, kTiny), r = __fdiv_rn(t & 2 ? m : 127.f, t & 2 ? 127.f : m);
+      const int team = threadIdx.x & 16;
+      const bool fine_g = top_g < INFINITY, fine_u = top_u < INFINITY;
+      store_piece_s8<16, A>(a.g_q + n.row * a.q_st + n.first, 0, t, n.width, g, fine_g, __shfl_sync(kFull, r, team));
+      store_piece_s8<16, A>(a.u_q + n.row * a.q_st + n.first, 0, t, n.width, u, fine_u, __shfl_sync(kFull, r, team + 1));
+      if (n.width && (t & ~1) == 2) (t & 1 ? a.u_scale : a.g_scale)[n.at] = (t & 1 ? fine_u : fine_g) ? r : __int_as_float(0x7fffffff);
     }
   }
 }
 
-template <typename T, bool A, bool KEPT>
+template <typename T, int U, bool A, bool KEPT>
 __global__ void __launch_bounds__(kGluThreads) glu_bwd_kernel(const __grid_constant__ GluArgs a) {
   const int t = threadIdx.x & 15;
-  const int64_t item = int64_t(blockIdx.x) * (kGluThreads / 16) + (threadIdx.x >> 4);
-  if (item >= a.rows * a.groups) return;
-  const int64_t row = int64_t(uint64_t(item) / a.groups);
-  const int first = int(item - row * a.groups) * kGroup, width = min(kGroup, a.D - first);
-  const Raw8<T> dr = load_piece<T, 16, A>(static_cast<const T*>(a.dout) + row * a.dout_st + first, 0, t, width);
-  float d[8], g[8], u[8], o[8];
-  if constexpr (KEPT) {
-    load8<A>(a.g_q + row * a.q_st + first, a.g_scale[item], t, width, g);
-    load8<A>(a.u_q + row * a.q_st + first, a.u_scale[item], t, width, u);
-  } else {
-    widen8<T>(load_piece<T, 16, A>(static_cast<const T*>(a.g) + row * a.g_st + first, 0, t, width), g);
-    widen8<T>(load_piece<T, 16, A>(static_cast<const T*>(a.u) + row * a.u_st + first, 0, t, width), u);
-  }
-  widen8<T>(dr, d);
+  Raw8<T> dr[U], gr[U], ur[U];
+  uint2 gq[U], uq[U];
+  float gs[U], us[U];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float s = sigmoid<T>(g[e]), y = g[e] * s;
-    if (a.out) o[e] = y * u[e];
-    u[e] = d[e] * u[e] * s * fmaf(g[e], 1.f - s, 1.f);
-    g[e] = d[e] * y;
+  for (int i = 0; i < U; ++i) {
+    const GluGroup<U> n(a, i);
+    dr[i] = load_piece<T, 16, A>(static_cast<const T*>(a.dout) + n.row * a.dout_st + n.first, 0, t, n.width);
+    if constexpr (KEPT) {
+      gq[i] = load_piece_s8<16, A>(a.g_q + n.row * a.q_st + n.first, t, n.width);
+      uq[i] = load_piece_s8<16, A>(a.u_q + n.row * a.q_st + n.first, t, n.width);
+      gs[i] = a.g_scale[n.at];
+      us[i] = a.u_scale[n.at];
+    } else {
+      gr[i] = load_piece<T, 16, A>(static_cast<const T*>(a.g) + n.row * a.g_st + n.first, 0, t, n.width);
+      ur[i] = load_piece<T, 16, A>(static_cast<const T*>(a.u) + n.row * a.u_st + n.first, 0, t, n.width);
+    }
   }
-  store_piece<T, 16, A>(static_cast<T*>(a.dg) + row * a.D + first, 0, t, width, u);
-  store_piece<T, 16, A>(static_cast<T*>(a.du) + row * a.D + first, 0, t, width, g);
-  if (a.out) store_piece<T, 16, A>(static_cast<T*>(a.out) + row * a.D + first, 0, t, width, o);
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const GluGroup<U> n(a, i);
+    float d[8], g[8], u[8], o[8];
+    if constexpr (KEPT) {
+      widen8_s8(gq[i], gs[i], g);
+      widen8_s8(uq[i], us[i], u);
+    } else {
+      widen8<T>(gr[i], g);
+      widen8<T>(ur[i], u);
+    }
+    widen8<T>(dr[i], d);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float s = sigmoid<T>(g[e]), y = g[e] * s;
+      if (a.out) o[e] = y * u[e];
+      u[e] = d[e] * u[e] * s * fmaf(g[e], 1.f - s, 1.f);
+      g[e] = d[e] * y;
+    }
+    store_piece<T, 16, A>(static_cast<T*>(a.dg) + n.row * a.D + n.first, 0, t, n.width, u);
+    store_piece<T, 16, A>(static_cast<T*>(a.du) + n.row * a.D + n.first, 0, t, n.width, g);
+    if (a.out) store_piece<T, 16, A>(static_cast<T*>(a.out) + n.row * a.D + n.first, 0, t, n.width, o);
+  }
 }
 
 // The product in 8 bits with one scale per row: a team holds the row.
@@ -203,41 +220,43 @@ int rows8(const GluArgs& a, bool aligned, cudaStream_t s) {
   return launch_row<T, 1024, 4>(a, aligned, s);
 }
 
-template <typename T>
-int fwd(const GluArgs& a, bool aligned, cudaStream_t s) {
-  if (a.a_q) return rows8<T>(a, aligned, s);
-  const int64_t items = a.rows * a.groups, per = kGluThreads / 16;
-  const unsigned ctas = unsigned((items + per - 1) / per);
-  if (a.g_q) {
-    if (aligned) glu_fwd_kernel<T, true, true><<<ctas, kGluThreads, 0, s>>>(a);
-    else glu_fwd_kernel<T, false, true><<<ctas, kGluThreads, 0, s>>>(a);
+template <typename T, int U, bool KEEP, bool BWD>
+int launch_groups(const GluArgs& a, bool aligned, cudaStream_t s) {
+  constexpr int64_t per = kGluTeams * U;
+  const unsigned ctas = unsigned((a.items + per - 1) / per);
+  if constexpr (BWD) {
+    if (aligned) glu_bwd_kernel<T, U, true, KEEP><<<ctas, kGluThreads, 0, s>>>(a);
+    else glu_bwd_kernel<T, U, false, KEEP><<<ctas, kGluThreads, 0, s>>>(a);
   } else {
-    if (aligned) glu_fwd_kernel<T, true, false><<<ctas, kGluThreads, 0, s>>>(a);
-    else glu_fwd_kernel<T, false, false><<<ctas, kGluThreads, 0, s>>>(a);
+    if (aligned) glu_fwd_kernel<T, U, true, KEEP><<<ctas, kGluThreads, 0, s>>>(a);
+    else glu_fwd_kernel<T, U, false, KEEP><<<ctas, kGluThreads, 0, s>>>(a);
   }
   PISA_CHECK_LAUNCH();
   return PISA_OK;
 }
 
+// Four groups per team where that still gives every SM four CTAs, else one.
+template <typename T, bool BWD>
+int groups(const GluArgs& a, bool aligned, cudaStream_t s) {
+  const bool many = a.items >= uint32_t(4 * kGluTeams * 4 * sm_count());
+  if (a.g_q) return many ? launch_groups<T, 4, true, BWD>(a, aligned, s) : launch_groups<T, 1, true, BWD>(a, aligned, s);
+  return many ? launch_groups<T, 4, false, BWD>(a, aligned, s) : launch_groups<T, 1, false, BWD>(a, aligned, s);
+}
+
+template <typename T>
+int fwd(const GluArgs& a, bool aligned, cudaStream_t s) {
+  return a.a_q ? rows8<T>(a, aligned, s) : groups<T, false>(a, aligned, s);
+}
+
 template <typename T>
 int bwd(const GluArgs& a, bool aligned, cudaStream_t s) {
-  const int64_t items = a.rows * a.groups, per = kGluThreads / 16;
-  const unsigned ctas = unsigned((items + per - 1) / per);
-  if (a.g_q) {
-    if (aligned) glu_bwd_kernel<T, true, true><<<ctas, kGluThreads, 0, s>>>(a);
-    else glu_bwd_kernel<T, false, true><<<ctas, kGluThreads, 0, s>>>(a);
-  } else {
-    if (aligned) glu_bwd_kernel<T, true, false><<<ctas, kGluThreads, 0, s>>>(a);
-    else glu_bwd_kernel<T, false, false><<<ctas, kGluThreads, 0, s>>>(a);
-  }
-  PISA_CHECK_LAUNCH();
-  return PISA_OK;
+  return groups<T, true>(a, aligned, s);
 }
 
 int check(int dtype, int64_t rows, int64_t D) {
   if (dtype < PISA_F32 || dtype > PISA_F16) return fail(PISA_ERR_UNSUPPORTED, "the kernels support FP16, BF16 and FP32");
   if (rows <= 0 || D <= 0) return fail(PISA_ERR_INVALID, "nonempty tensors are required");
-  if (rows >= (int64_t(1) << 31) || D >= (int64_t(1) << 30) || rows * ((D + kGroup - 1) / kGroup) >= (int64_t(1) << 34))
+  if (rows >= (int64_t(1) << 31) || D >= (int64_t(1) << 30) || rows * ((D + kGroup - 1) / kGroup) >= (int64_t(1) << 31) - 256)
     return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
   return PISA_OK;
 }
@@ -265,7 +284,7 @@ int pisa_swiglu(const void* gate, int64_t gate_st, const void* up, int64_t up_st
     return fail(PISA_ERR_UNSUPPORTED, "8-bit rows must start on 16 bytes");
   GluArgs a{};
   a.g = gate; a.g_st = gate_st; a.u = up; a.u_st = up_st; a.rows = rows; a.D = int(D);
-  a.groups = uint32_t((D + kGroup - 1) / kGroup);
+  a.groups = FastDiv::make(uint32_t((D + kGroup - 1) / kGroup)); a.items = uint32_t(rows) * a.groups.d;
   a.out = out; a.g_q = gate_q; a.u_q = up_q; a.q_st = q_st; a.g_scale = gate_scale; a.u_scale = up_scale;
   a.a_q = out_q; a.a_q_st = out_q_st; a.a_scale = out_scale;
   const int es = dtype == PISA_F32 ? 4 : 2;
@@ -288,7 +307,7 @@ int pisa_swiglu_bwd(const void* dout, int64_t dout_st, const void* gate, int64_t
     return fail(PISA_ERR_UNSUPPORTED, "8-bit rows must start on 16 bytes");
   GluArgs a{};
   a.g = gate; a.g_st = gate_st; a.u = up; a.u_st = up_st; a.rows = rows; a.D = int(D);
-  a.groups = uint32_t((D + kGroup - 1) / kGroup);
+  a.groups = FastDiv::make(uint32_t((D + kGroup - 1) / kGroup)); a.items = uint32_t(rows) * a.groups.d;
   a.out = out; a.g_q = const_cast<int8_t*>(gate_q); a.u_q = const_cast<int8_t*>(up_q); a.q_st = q_st;
   a.g_scale = const_cast<float*>(gate_scale); a.u_scale = const_cast<float*>(up_scale);
   a.dout = dout; a.dout_st = dout_st; a.dg = dgate; a.du = dup;

@@ -41,6 +41,15 @@ def test_matches(cuda_device, dtype, width, bits):
         compare(*(normal(gen, *shape, width, dtype=dtype, scale=s) for s in (3.0, 1.0, 1.0)), bits)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("bits", [None, 8])
+def test_many_groups(cuda_device, dtype, bits):
+    """Teams with several groups, the last ones without any; aligned rows and others."""
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    for rows, width in ((1733, 2816), (1733, 2817), (40003, 40)):
+        compare(*(normal(gen, rows, width, dtype=dtype) for _ in range(3)), bits)
+
+
 @pytest.mark.parametrize("bits", [None, 8])
 def test_layouts(cuda_device, bits):
     gen = torch.Generator(device="cuda").manual_seed(1)
