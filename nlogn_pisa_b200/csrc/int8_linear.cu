@@ -3,12 +3,17 @@
 //   y[t, o] = ws[o] xs[t] sum_k w[o, k] x[t, k] + bias[o],
 // with int32 sums, which are exact for K < 2^17.
 //
-// tcgen05 tiles (kind::i8): 128 output channels are the rows of a tile and BN
-// tokens its columns, so a warp's lanes are 32 consecutive channels of every
+// tcgen05 tiles (kind::i8): 128 output channels are the rows of a tile and up
+// to BN tokens its columns, so a warp's lanes are 32 consecutive channels of every
 // token it stores and rows of any length leave without a detour.  K goes in
 // blocks of 128 bytes, a 128-byte-swizzled TMA box of each operand per stage.
-// Warp 0 loads, warp 1 issues the MMAs, warps 2 to 5 scale and store; two
+// Warp 0 loads, warp 1 issues the MMAs, warps 2 to 9 scale and store; two
 // accumulators in TMEM let a tile's stores run under the next tile's products.
+//
+// Where the tiles are fewer than the SMs, a cluster of CTAs shares each: every
+// CTA sums a range of K, leaves its int32 sums in shared memory, and takes a
+// share of the tile's tokens, for which it adds all ranges' sums (integers: in
+// any order the same).
 #include <cudaTypedefs.h>
 
 #include "dense_tc.cuh"
@@ -19,7 +24,7 @@ namespace {
 
 constexpr int kM = 128;          // output channels of a tile
 constexpr int kStepBytes = 128;  // bytes of K per stage
-constexpr int kThreads = 192;
+constexpr int kThreads = 320;    // a warp of loads, one of products, eight of stores
 constexpr int kSmem = 220 * 1024;
 
 struct LinArgs {
@@ -29,7 +34,9 @@ struct LinArgs {
   const void* bias;     // or NULL
   int bias_f32;
   int T, O, steps;      // steps: K in blocks of 128 bytes
+  int bn;               // tokens of a tile, a multiple of 16
   uint32_t tiles_o, tiles;
+  uint32_t split;       // CTAs that share a tile
   uint32_t tries;
   void* out;
   int* status;
@@ -93,7 +100,7 @@ __global__ void __launch_bounds__(kThreads) int8_linear_kernel(const __grid_cons
   __shared__ uint64_t full[L::STAGES], empty[L::STAGES], acc_full[2], acc_empty[2], drained;
   __shared__ uint32_t slot;
   __shared__ WaitFlag wait;
-  __shared__ __align__(16) float s_xs[4][BN < 32 ? 32 : BN];
+  __shared__ __align__(16) float s_xs[8][BN < 32 ? 32 : BN];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = (tc::smem_u32(raw) + 1023u) & ~1023u;
   if (warp == 0 && lane == 0) {
@@ -103,7 +110,7 @@ __global__ void __launch_bounds__(kThreads) int8_linear_kernel(const __grid_cons
     }
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&acc_full[i], 1);
-      tc::mbar_init(&acc_empty[i], 4);
+      tc::mbar_init(&acc_empty[i], 8);
     }
     tc::mbar_init(&drained, 1);
     tc::fence_barrier_init();
@@ -114,6 +121,7 @@ __global__ void __launch_bounds__(kThreads) int8_linear_kernel(const __grid_cons
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = slot;
+  const uint32_t stage_bytes = uint32_t(L::A_BYTES + a.bn * kStepBytes);
   bool ok = true;
   if (warp == 0) {
     if (lane == 0) {
@@ -124,9 +132,9 @@ __global__ void __launch_bounds__(kThreads) int8_linear_kernel(const __grid_cons
         for (int k = 0; k < a.steps; ++k) {
           if (!(ok = wait_phase(&empty[st], int(phase), &wait))) break;
           const uint32_t at = base + st * L::STAGE;
-          tc::mbar_arrive_expect_tx(&full[st], L::STAGE);
+          tc::mbar_arrive_expect_tx(&full[st], stage_bytes);
           tma_load_2d(at, &a.tm_w, k * kStepBytes, int(to) * kM, &full[st]);
-          tma_load_2d(at + L::A_BYTES, &a.tm_x, k * kStepBytes, int(tt) * BN, &full[st]);
+          tma_load_2d(at + L::A_BYTES, &a.tm_x, k * kStepBytes, int(tt) * a.bn, &full[st]);
           ++loads;
           if (++st == L::STAGES) {
             st = 0;
@@ -142,7 +150,7 @@ __global__ void __launch_bounds__(kThreads) int8_linear_kernel(const __grid_cons
     __syncwarp();
   } else if (warp == 1) {
     const bool leader = elect_one();
-    const uint32_t idesc = idesc_i8(kM, BN);
+    const uint32_t idesc = idesc_i8(kM, a.bn);
     int st = 0, n = 0;
     uint32_t phase = 0;
     for (uint32_t tile = blockIdx.x; tile < a.tiles && ok; tile += gridDim.x, ++n) {
@@ -178,17 +186,18 @@ __global__ void __launch_bounds__(kThreads) int8_linear_kernel(const __grid_cons
     }
     __syncwarp();
   } else {
-    const int quarter = warp & 3;                  // TMEM lanes that this warp may read
+    // TMEM lanes that this warp may read; two warps share them, with every other 32 tokens each
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
     const uint32_t lanes = uint32_t(quarter * 32) << 16;
-    float* xs = s_xs[quarter];
+    float* xs = s_xs[warp - 2];
     const bool pairs = (a.O & 1) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 3u) == 0;
     int n = 0;
     for (uint32_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, ++n) {
       const int buf = n & 1;
       const uint32_t tt = tile / a.tiles_o, to = tile - tt * a.tiles_o;
-      const int t0 = int(tt) * BN, o = int(to) * kM + quarter * 32 + lane;
+      const int t0 = int(tt) * a.bn, t1 = min(a.T, t0 + a.bn), o = int(to) * kM + quarter * 32 + lane;
       __syncwarp();
-      for (int i = lane; i < BN; i += 32) xs[i] = t0 + i < a.T ? a.x_scale[t0 + i] : 0.f;
+      for (int i = half * 32 + lane; i < a.bn; i += 64) xs[i] = t0 + i < a.T ? a.x_scale[t0 + i] : 0.f;
       const float ws = o < a.O ? a.w_scale[o] : 0.f;
       float bias = 0.f;
       if (a.bias && o < a.O) bias = a.bias_f32 ? static_cast<const float*>(a.bias)[o] : to_f32<T>(static_cast<const T*>(a.bias)[o]);
@@ -197,7 +206,7 @@ __global__ void __launch_bounds__(kThreads) int8_linear_kernel(const __grid_cons
       if (!__all_sync(kFull, ok)) break;
       tc::fence_after_sync();
 #pragma unroll 1
-      for (int c = 0; c < BN; c += 32) {
+      for (int c = half * 32; c < a.bn; c += 64) {
         float v[32];
         tc::tmem_ld32(tmem + buf * L::COLS + c + lanes, v);
 #pragma unroll
@@ -208,8 +217,8 @@ __global__ void __launch_bounds__(kThreads) int8_linear_kernel(const __grid_cons
           v[j + 2] = fmaf(float(__float_as_int(v[j + 2])) * ws, s.z, bias);
           v[j + 3] = fmaf(float(__float_as_int(v[j + 3])) * ws, s.w, bias);
         }
-        // of a tile of 16 tokens, the other columns are not the product's: T ends before them
-        store_columns<T>(v, static_cast<T*>(a.out), a.O, t0 + c, BN < 32 ? min(a.T, t0 + BN) : a.T, o, a.O, pairs);
+        // columns past the tile's tokens are not the product's
+        store_columns<T>(v, static_cast<T*>(a.out), a.O, t0 + c, t1, o, a.O, pairs);
       }
       tc::fence_before_sync();
       __syncwarp();
@@ -221,6 +230,181 @@ __global__ void __launch_bounds__(kThreads) int8_linear_kernel(const __grid_cons
   tc::fence_after_sync();
   if (threadIdx.x == 0 && wait.expired && a.status) atomicExch(a.status, PISA_ERR_TIMEOUT);
   if (warp == 1) tc::tmem_free(tmem, 2 * L::COLS);
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ int4 load_peer(uint32_t addr, int rank) {
+  int4 v;
+  asm volatile("{\n\t.reg .b32 at;\n\tmapa.shared::cluster.u32 at, %4, %5;\n\tld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [at];\n\t}"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr), "r"(rank));
+  return v;
+}
+
+// A warp's tokens c, c + step, ... below c1 of a tile split over S ranges of K:
+// four channels per lane, the sums of several tokens on their way at a time.
+template <typename T, int S>
+__device__ __forceinline__ void join(const LinArgs& a, uint32_t base, int c, int c1, int step, int64_t t0, int o) {
+  constexpr int U = S == 8 ? 2 : 4;
+  const int lane = threadIdx.x & 31, left = a.O - o;
+  float ws[4], bias[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    ws[i] = i < left ? a.w_scale[o + i] : 0.f;
+    bias[i] = 0.f;
+    if (a.bias && i < left)
+      bias[i] = a.bias_f32 ? static_cast<const float*>(a.bias)[o + i] : to_f32<T>(static_cast<const T*>(a.bias)[o + i]);
+  }
+  const bool wide = left >= 4 && a.O % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out) & (4 * sizeof(T) - 1)) == 0;
+  for (; c < c1; c += U * step) {
+    int4 v[U][S];
+    float xs[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int at = min(c + u * step, c1 - 1);
+      xs[u] = a.x_scale[t0 + at];
+#pragma unroll
+      for (int r = 0; r < S; ++r) v[u][r] = load_peer(base + uint32_t(at * kM + lane * 4) * 4, r);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (c + u * step >= c1) break;
+      int4 sum = v[u][0];
+#pragma unroll
+      for (int r = 1; r < S; ++r) {
+        sum.x += v[u][r].x;
+        sum.y += v[u][r].y;
+        sum.z += v[u][r].z;
+        sum.w += v[u][r].w;
+      }
+      const float y[4] = {fmaf(float(sum.x) * ws[0], xs[u], bias[0]), fmaf(float(sum.y) * ws[1], xs[u], bias[1]),
+                          fmaf(float(sum.z) * ws[2], xs[u], bias[2]), fmaf(float(sum.w) * ws[3], xs[u], bias[3])};
+      T* out = static_cast<T*>(a.out) + (t0 + c + u * step) * a.O + o;
+      if (wide) {
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(out) = make_float4(y[0], y[1], y[2], y[3]);
+        else *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < left) out[i] = from_f32<T>(y[i]);
+      }
+    }
+  }
+}
+
+// One tile per cluster of a.split CTAs.
+template <typename T, int BN>
+__global__ void __launch_bounds__(kThreads) int8_linear_split_kernel(const __grid_constant__ LinArgs a) {
+  using L = Tile<BN>;
+  static_assert(BN * kM * 4 <= L::STAGES * L::STAGE, "the sums take the stages' place");
+  extern __shared__ __align__(16) uint8_t raw[];
+  __shared__ uint64_t full[L::STAGES], empty[L::STAGES], acc_full, drained;
+  __shared__ uint32_t slot;
+  __shared__ WaitFlag wait;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t base = (tc::smem_u32(raw) + 1023u) & ~1023u;
+  const uint32_t tile = blockIdx.x / a.split, rank = blockIdx.x - tile * a.split;   // rank: clusters are runs of a.split CTAs
+  const uint32_t tt = tile / a.tiles_o, to = tile - tt * a.tiles_o;
+  const int k0 = int(int64_t(a.steps) * rank / a.split), k1 = int(int64_t(a.steps) * (rank + 1) / a.split);
+  if (warp == 0 && lane == 0) {
+    for (int i = 0; i < L::STAGES; ++i) {
+      tc::mbar_init(&full[i], 1);
+      tc::mbar_init(&empty[i], 1);
+    }
+    tc::mbar_init(&acc_full, 1);
+    tc::mbar_init(&drained, 1);
+    tc::fence_barrier_init();
+    wait.init(a.tries);
+  }
+  if (warp == 1) tc::tmem_alloc(&slot, L::COLS);
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = slot;
+  const uint32_t stage_bytes = uint32_t(L::A_BYTES + a.bn * kStepBytes);
+  bool ok = true;
+  if (warp == 0) {
+    if (lane == 0) {
+      int st = 0, loads = 0;
+      uint32_t phase = 1;
+      for (int k = k0; k < k1; ++k) {
+        if (!(ok = wait_phase(&empty[st], int(phase), &wait))) break;
+        const uint32_t at = base + st * L::STAGE;
+        tc::mbar_arrive_expect_tx(&full[st], stage_bytes);
+        tma_load_2d(at, &a.tm_w, k * kStepBytes, int(to) * kM, &full[st]);
+        tma_load_2d(at + L::A_BYTES, &a.tm_x, k * kStepBytes, int(tt) * a.bn, &full[st]);
+        ++loads;
+        if (++st == L::STAGES) {
+          st = 0;
+          phase ^= 1;
+        }
+      }
+      for (int x = max(0, loads - L::STAGES); x < loads; ++x)
+        wait_phase(ok ? &empty[x % L::STAGES] : &full[x % L::STAGES], x / L::STAGES, &wait);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    const bool leader = elect_one();
+    const uint32_t idesc = idesc_i8(kM, a.bn);
+    int st = 0;
+    uint32_t phase = 0;
+#pragma unroll 1
+    for (int k = k0; k < k1; ++k) {
+      ok = wait_phase(&full[st], int(phase), &wait) && ok;
+      if (!__all_sync(kFull, ok)) {
+        ok = false;
+        break;
+      }
+      tc::fence_after_sync();
+      if (leader) {
+        const uint32_t al = desc_low(base + st * L::STAGE, 16), bl = desc_low(base + st * L::STAGE + L::A_BYTES, 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mma_i8(tmem, al + 2 * i, bl + 2 * i, idesc, k > k0 || i > 0);
+        tc::mma_commit(&empty[st]);
+        if (k + 1 == k1) tc::mma_commit(&acc_full);
+      }
+      __syncwarp();
+      if (++st == L::STAGES) {
+        st = 0;
+        phase ^= 1;
+      }
+    }
+    if (!__all_sync(kFull, ok)) {
+      if (leader) tc::mma_commit(&drained);
+      wait_phase(&drained, 0, &wait);
+    }
+    __syncwarp();
+  } else {
+    const int quarter = warp & 3;
+    const uint32_t mine = base + (quarter * 32 + lane) * 4;      // sums: [token][channel]
+    // the sums' products are done, so every stage has been read
+    ok = wait_phase(&acc_full, 0, &wait);
+    tc::fence_after_sync();
+    if (__all_sync(kFull, ok)) {
+#pragma unroll 1
+      for (int c = (warp - 2) >> 2 << 4; c < a.bn; c += 32) {
+        float v[16];
+        tc::tmem_ld16(tmem + c + (uint32_t(quarter * 32) << 16), v);
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          asm volatile("st.shared.f32 [%0], %1;" :: "r"(mine + uint32_t(c + j) * (kM * 4)), "f"(v[j]) : "memory");
+      }
+    }
+    __syncwarp();
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  if (threadIdx.x == 0 && wait.expired && a.status) atomicExch(a.status, PISA_ERR_TIMEOUT);
+  if (warp == 1) tc::tmem_free(tmem, L::COLS);
+  cluster_sync();
+  const int64_t t0 = int64_t(tt) * a.bn;
+  const int c0 = int(a.bn * rank / a.split), c1 = int(min64(a.bn * (rank + 1) / a.split, a.T - t0)), o = int(to) * kM + lane * 4;
+  if (a.split == 2) join<T, 2>(a, base, c0 + warp, c1, kThreads / 32, t0, o);
+  else if (a.split == 4) join<T, 4>(a, base, c0 + warp, c1, kThreads / 32, t0, o);
+  else join<T, 8>(a, base, c0 + warp, c1, kThreads / 32, t0, o);
+  cluster_sync();   // no CTA leaves while another reads its sums
 }
 
 // 2-D map over rows of bytes: a box of 128 bytes of `box` rows, 128-byte
@@ -254,29 +438,84 @@ struct Operands {
   int64_t w_st, K;
 };
 
+// Tokens of a tile of at most `most`: as many for each tile, in whole sixteens.
+int tile_tokens(int64_t T, int most) {
+  const int64_t tiles = (T + most - 1) / most;
+  return int(((T + tiles - 1) / tiles + 15) / 16 * 16);
+}
+
 template <typename T, int BN>
-int launch(LinArgs a, const Operands& m, cudaStream_t s) {
+int launch(LinArgs a, const Operands& m, int split, cudaStream_t s) {
   using L = Tile<BN>;
+  a.bn = tile_tokens(a.T, BN);
   int rc = byte_map(&a.tm_w, m.w, a.O, m.K, m.w_st, kM);
-  if (rc == PISA_OK) rc = byte_map(&a.tm_x, m.x, a.T, m.K, m.x_st, BN);
-  if (rc == PISA_OK) rc = allow_smem<int8_linear_kernel<T, BN>>(L::SMEM, "8-bit product smem attribute");
+  if (rc == PISA_OK) rc = byte_map(&a.tm_x, m.x, a.T, m.K, m.x_st, uint32_t(a.bn));
   if (rc) return rc;
   a.tiles_o = uint32_t((a.O + kM - 1) / kM);
-  const int64_t tiles = int64_t(a.tiles_o) * ((a.T + BN - 1) / BN);
+  const int64_t tiles = int64_t(a.tiles_o) * ((a.T + a.bn - 1) / a.bn);
   if (tiles >= (int64_t(1) << 31)) return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
   a.tiles = uint32_t(tiles);
-  int8_linear_kernel<T, BN><<<unsigned(min64(tiles, sm_count())), kThreads, L::SMEM, s>>>(a);
+  a.split = uint32_t(split);
+  if (split == 1) {
+    if ((rc = allow_smem<int8_linear_kernel<T, BN>>(L::SMEM, "8-bit product smem attribute"))) return rc;
+    int8_linear_kernel<T, BN><<<unsigned(min64(tiles, sm_count())), kThreads, L::SMEM, s>>>(a);
+    PISA_CHECK_LAUNCH();
+    return PISA_OK;
+  }
+  if ((rc = allow_smem<int8_linear_split_kernel<T, BN>>(L::SMEM, "8-bit product smem attribute"))) return rc;
+  cudaLaunchConfig_t config{};
+  cudaLaunchAttribute cluster;
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = unsigned(split);
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  config.gridDim = dim3(unsigned(tiles * split));
+  config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = L::SMEM;
+  config.stream = s;
+  config.attrs = &cluster;
+  config.numAttrs = 1;
+  if (cudaLaunchKernelEx(&config, int8_linear_split_kernel<T, BN>, a) != cudaSuccess) return fail_cuda(cudaGetLastError(), "8-bit product");
   PISA_CHECK_LAUNCH();
   return PISA_OK;
 }
 
+// Tokens of a tile (at most) and CTAs that share one.
+struct Shape {
+  int bn, split;
+};
+
+Shape choose(int64_t T, int64_t O, int64_t steps) {
+  const int64_t sms = sm_count(), tiles_o = (O + kM - 1) / kM;
+  Shape best{256, 1};
+  double least = 1e30;
+  for (int most = 16; most <= 256; most *= 2) {
+    const int bn = tile_tokens(T, most);
+    if (most > 16 && bn <= most / 2) break;
+    const int64_t tiles = tiles_o * ((T + bn - 1) / bn);
+    const double step = 0.22 + 0.00105 * bn, start = 4 + 0.01 * bn;
+    for (int split = 1; split <= 8; split *= 2) {
+      if (split > steps || (split > 1 && tiles * split > (split == 8 ? sms * 3 / 4 : sms))) break;
+      const int64_t waves = (tiles * split + sms - 1) / sms;
+      const double cost = start + waves * ((steps + split - 1) / split) * step + (split > 1 ? 1.5 + 0.01 * bn : 0);
+      if (cost < least) {
+        least = cost;
+        best = {most, split};
+      }
+    }
+  }
+  return best;
+}
+
 template <typename T>
 int dispatch(const LinArgs& a, const Operands& m, cudaStream_t s) {
-  if (a.T <= 16) return launch<T, 16>(a, m, s);
-  if (a.T <= 32) return launch<T, 32>(a, m, s);
-  if (a.T <= 64) return launch<T, 64>(a, m, s);
-  if (a.T <= 128) return launch<T, 128>(a, m, s);
-  return launch<T, 256>(a, m, s);
+  const Shape c = choose(a.T, a.O, a.steps);
+  switch (c.bn) {
+    case 16: return launch<T, 16>(a, m, c.split, s);
+    case 32: return launch<T, 32>(a, m, c.split, s);
+    case 64: return launch<T, 64>(a, m, c.split, s);
+    case 128: return launch<T, 128>(a, m, c.split, s);
+    default: return launch<T, 256>(a, m, c.split, s);
+  }
 }
 
 }  // namespace

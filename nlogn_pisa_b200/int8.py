@@ -40,6 +40,11 @@ def rows_of(t):
     return t.contiguous(), width
 
 
+def empty(t):
+    """A contiguous tensor like ``t`` (empty_like takes half the time of new_empty)."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def row_bytes(width):
     """Bytes from one int8 row to the next, so that all start on 16."""
     return (width + 15) // 16 * 16
@@ -49,8 +54,11 @@ def byte_rows(like, shape):
     """An int8 tensor of ``shape`` whose rows start on 16 bytes."""
     width = shape[-1]
     step = row_bytes(width)
-    rows = like.new_empty((*shape[:-1], step), dtype=torch.int8)
-    return rows if step == width else rows[..., :width]
+    if step == width:
+        if shape == like.shape and like.is_contiguous():
+            return torch.empty_like(like, dtype=torch.int8)
+        return like.new_empty(shape, dtype=torch.int8)
+    return like.new_empty((*shape[:-1], step), dtype=torch.int8)[..., :width]
 
 
 def aligned_bytes(t):

@@ -16,7 +16,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .dense import differentiated, flat
-from .int8 import byte_rows, no_gradient, row_bytes, rows_of
+from .int8 import byte_rows, empty, no_gradient, row_bytes, rows_of
 from .validation import require_cuda
 
 
@@ -41,13 +41,13 @@ def _operands(x, branch, gate, gate_rows, post_weight, weight, scales):
 def _forward(x, branch, gate, post_weight, weight, gate_rows, scales, eps, quantize, want_stats):
     """h, n (or its bytes and scales) and the row statistics."""
     operands, _kept = _operands(x, branch, gate, gate_rows, post_weight, weight, scales)
-    h = None if branch is None else x.new_empty(x.shape)
+    h = None if branch is None else empty(x)
     scale = stats = None
     if quantize:
         n, scale = byte_rows(x, x.shape), x.new_empty(x.shape[:-1], dtype=torch.float32)
         out = None, n.data_ptr(), row_bytes(x.shape[-1]), scale.data_ptr()
     else:
-        n = x.new_empty(x.shape)
+        n = empty(x)
         out = n.data_ptr(), None, 0, None
     if want_stats:
         stats = x.new_empty((*x.shape[:-1], 2), dtype=torch.float32)
@@ -76,11 +76,11 @@ class ResidualNormFunction(torch.autograd.Function):
         dn = torch.zeros_like(x, memory_format=torch.contiguous_format) if dn is None else flat(dn)
         dh = None if dh is None else flat(dh)
         operands, _kept = _operands(x, branch, gate, gate_rows, post_weight, weight, scales)
-        dx, dweight = x.new_empty(x.shape), torch.empty_like(weight)
+        dx, dweight = empty(x), torch.empty_like(weight)
         dbranch = dgate = dpost = None
         if branch is not None:
-            dbranch = x.new_empty(x.shape)
-            dgate = None if gate is None else gate.new_empty(gate.shape)
+            dbranch = empty(x)
+            dgate = None if gate is None else empty(gate)
             dpost = None if post_weight is None else torch.empty_like(post_weight)
         width = x.shape[-1]
         size = _lib.workspace_bytes("pisa_residual_norm_bwd_workspace_bytes", x.get_device(), x.numel() // width, width,

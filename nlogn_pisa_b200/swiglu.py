@@ -15,7 +15,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .dense import carries_tangent, differentiated
-from .int8 import GROUP, byte_rows, checkpoint_int8, no_gradient, restore_int8, row_bytes, rows_of
+from .int8 import GROUP, byte_rows, checkpoint_int8, empty, no_gradient, restore_int8, row_bytes, rows_of
 from .validation import require_cuda
 
 
@@ -31,7 +31,7 @@ def _forward(gate, up, keep):
     """The product, and the buffer that keeps gate and up in 8 bits, or None."""
     width = gate.shape[-1]
     (rows, g_st), (up_rows, u_st), count = rows_of(gate), rows_of(up), gate.numel() // width
-    out, kept, pointers = gate.new_empty(gate.shape), None, (None, None, 0, None, None)
+    out, kept, pointers = empty(gate), None, (None, None, 0, None, None)
     if keep:
         size = 2 * count * (row_bytes(width) + 4 * ((width + GROUP - 1) // GROUP))
         kept = gate.new_empty(size, dtype=torch.int8)
@@ -45,8 +45,7 @@ def _backward(dout, gate, up, kept, want_out=False):
     """(dgate, dup, and the product again or None) from gate and up, or from what was kept of them."""
     width = dout.shape[-1]
     (rows, stride), count = rows_of(dout), dout.numel() // width
-    dgate, dup = dout.new_empty(dout.shape), dout.new_empty(dout.shape)
-    out = dout.new_empty(dout.shape) if want_out else None
+    dgate, dup, out = empty(dout), empty(dout), empty(dout) if want_out else None
     if kept is None:
         (gate, g_st), (up, u_st) = rows_of(gate), rows_of(up)
         given = (gate.data_ptr(), g_st, up.data_ptr(), u_st, None, None, 0, None, None)
