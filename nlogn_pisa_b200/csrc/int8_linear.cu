@@ -69,28 +69,65 @@ struct Tile {
   static constexpr int COLS = BN < 32 ? 32 : BN;             // TMEM columns of an accumulator
 };
 
-// 32 tokens of one channel per lane, stored token by token: 32 consecutive channels per warp.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// 32 tokens of one channel per lane, stored token by token: 32 consecutive
+// channels per warp.  `whole`: all 32 tokens and channels exist (the warp takes
+// one path without a test per store; those cost half of its instructions).
 template <typename T>
-__device__ __forceinline__ void store_columns(const float (&v)[32], T* out, int64_t O, int t, int T_, int o, int O_, bool pairs) {
-  const int lane = threadIdx.x & 31;
+__device__ __forceinline__ void store_columns(const float (&v)[32], T* out, int64_t O, int t, int T_, int o, int O_, bool pairs,
+                                              bool whole) {
   if constexpr (sizeof(T) == 2) {
     if (pairs) {
       // neighbouring lanes swap, so that each holds both channels of a pair for every other token
-      const bool odd = lane & 1;
+      const bool odd = threadIdx.x & 1;
+      const uint32_t pick = odd ? 0x3276u : 0x5410u;
       T* at = out + int64_t(t + odd) * O + (o & ~1);
+      uint32_t r[16];
 #pragma unroll
-      for (int j = 0; j < 32; j += 2) {
-        const float got = __shfl_xor_sync(kFull, odd ? v[j] : v[j + 1], 1);
-        if (t + j + odd < T_ && o < O_)
-          *reinterpret_cast<uint32_t*>(at + int64_t(j) * O) = odd ? pack2<T>(got, v[j + 1]) : pack2<T>(v[j], got);
+      for (int j = 0; j < 16; ++j) {
+        const uint32_t own = pack2<T>(v[2 * j], v[2 * j + 1]);
+        r[j] = __byte_perm(own, __shfl_xor_sync(kFull, own, 1), pick);
+      }
+      if (whole) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j, at += 2 * O) *reinterpret_cast<uint32_t*>(at) = r[j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j, at += 2 * O)
+          if (t + 2 * j + odd < T_ && o < O_) *reinterpret_cast<uint32_t*>(at) = r[j];
       }
       return;
     }
   }
   T* at = out + int64_t(t) * O + o;
+  if (whole) {
 #pragma unroll
-  for (int j = 0; j < 32; ++j)
-    if (t + j < T_ && o < O_) at[int64_t(j) * O] = from_f32<T>(v[j]);
+    for (int j = 0; j < 32; ++j, at += O) *at = from_f32<T>(v[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j, at += O)
+      if (t + j < T_ && o < O_) *at = from_f32<T>(v[j]);
+  }
+}
+
+// 32 columns of a finished tile, scaled and stored for tokens t .. t1 - 1 (columns past the tile's tokens are not the product's).
+template <typename T>
+__device__ __forceinline__ void store_tile(const LinArgs& a, uint32_t tmem, const float* xs, float ws, float bias, int t, int t1, int o,
+                                           bool pairs) {
+  float v[32];
+  tc::tmem_ld32(tmem, v);
+#pragma unroll
+  for (int j = 0; j < 32; j += 4) {
+    const float4 s = *reinterpret_cast<const float4*>(xs + j);
+    v[j] = fmaf(float(__float_as_int(v[j])) * ws, s.x, bias);
+    v[j + 1] = fmaf(float(__float_as_int(v[j + 1])) * ws, s.y, bias);
+    v[j + 2] = fmaf(float(__float_as_int(v[j + 2])) * ws, s.z, bias);
+    v[j + 3] = fmaf(float(__float_as_int(v[j + 3])) * ws, s.w, bias);
+  }
+  const bool whole = t + 32 <= t1 && (o | 31) < a.O;
+  store_columns<T>(v, static_cast<T*>(a.out), a.O, t, t1, o, a.O, pairs, whole);
 }
 
 template <typename T, int BN>
@@ -206,20 +243,7 @@ __global__ void __launch_bounds__(kThreads) int8_linear_kernel(const __grid_cons
       if (!__all_sync(kFull, ok)) break;
       tc::fence_after_sync();
 #pragma unroll 1
-      for (int c = half * 32; c < a.bn; c += 64) {
-        float v[32];
-        tc::tmem_ld32(tmem + buf * L::COLS + c + lanes, v);
-#pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-          const float4 s = *reinterpret_cast<const float4*>(xs + c + j);
-          v[j] = fmaf(float(__float_as_int(v[j])) * ws, s.x, bias);
-          v[j + 1] = fmaf(float(__float_as_int(v[j + 1])) * ws, s.y, bias);
-          v[j + 2] = fmaf(float(__float_as_int(v[j + 2])) * ws, s.z, bias);
-          v[j + 3] = fmaf(float(__float_as_int(v[j + 3])) * ws, s.w, bias);
-        }
-        // columns past the tile's tokens are not the product's
-        store_columns<T>(v, static_cast<T*>(a.out), a.O, t0 + c, t1, o, a.O, pairs);
-      }
+      for (int c = half * 32; c < a.bn; c += 64) store_tile<T>(a, tmem + buf * L::COLS + c + lanes, xs + c, ws, bias, t0 + c, t1, o, pairs);
       tc::fence_before_sync();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&acc_empty[buf]);
@@ -232,9 +256,181 @@ __global__ void __launch_bounds__(kThreads) int8_linear_kernel(const __grid_cons
   if (warp == 1) tc::tmem_free(tmem, 2 * L::COLS);
 }
 
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+// ---------------------------------------------------------------------------
+// Tiles of 256 channels for pairs of CTAs: each loads its 128 channels and half
+// of the tokens, and one issues MMAs (cta_group::2) that read both shared
+// memories and sum each CTA's channels in its own TMEM.  A pair moves two thirds
+// of the bytes per product of two separate tiles of 128 x 256.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t leader_address(const void* p) {
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(tc::smem_u32(p)));
+  return at;
 }
+// Into this CTA's shared memory, counted on the leader's barrier.
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t mbar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+      :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(mbar) : "memory");
+}
+__device__ __forceinline__ void mma_i8_pair(uint32_t d, uint32_t a_low, uint32_t b_low, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], a, b, %3, p;\n\t}"
+      :: "r"(d), "r"(a_low), "r"(b_low), "r"(idesc), "r"(uint32_t(accumulate)), "r"(kDescHigh) : "memory");
+}
+// Arrive on `mbar` of both CTAs once the pair's MMAs so far have completed.
+__device__ __forceinline__ void commit_pair(uint64_t* mbar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+               :: "r"(tc::smem_u32(mbar)), "h"(uint16_t(3)) : "memory");
+}
+__device__ __forceinline__ void arrive_at(uint32_t mbar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" :: "r"(mbar) : "memory");
+}
+
+struct PairTile {
+  static constexpr int A_BYTES = kM * kStepBytes, B_BYTES = 128 * kStepBytes, STAGE = A_BYTES + B_BYTES;
+  static constexpr int STAGES = 6, SMEM = STAGES * STAGE + 1024, COLS = 256;
+};
+
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads) int8_linear_pair_kernel(const __grid_constant__ LinArgs a) {
+  using L = PairTile;
+  extern __shared__ __align__(16) uint8_t raw[];
+  // full and acc_empty are the leader's; the other CTA counts on them from afar
+  __shared__ uint64_t full[L::STAGES], empty[L::STAGES], acc_full[2], acc_empty[2], drained;
+  __shared__ uint32_t slot;
+  __shared__ WaitFlag wait;
+  __shared__ __align__(16) float s_xs[8][256];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t base = (tc::smem_u32(raw) + 1023u) & ~1023u;
+  const uint32_t rank = blockIdx.x & 1, pairs = gridDim.x >> 1, first = blockIdx.x >> 1;
+  if (warp == 0 && lane == 0) {
+    for (int i = 0; i < L::STAGES; ++i) {
+      tc::mbar_init(&full[i], 1);
+      tc::mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&acc_full[i], 1);
+      tc::mbar_init(&acc_empty[i], 16);
+    }
+    tc::mbar_init(&drained, 1);
+    tc::fence_barrier_init();
+    wait.init(a.tries);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(tc::smem_u32(&slot)), "r"(2 * L::COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  cluster_sync();
+  tc::fence_after_sync();
+  const uint32_t tmem = slot;
+  const int half_tokens = a.bn / 2;
+  bool ok = true;
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint32_t stage_bytes = uint32_t(2 * (L::A_BYTES + half_tokens * kStepBytes));   // of both CTAs
+      int st = 0, loads = 0;
+      uint32_t phase = 1;
+      for (uint32_t tile = first; tile < a.tiles && ok; tile += pairs) {
+        const uint32_t tt = tile / a.tiles_o, to = tile - tt * a.tiles_o;
+        const int o = int(to * 2 + rank) * kM, t = int(tt) * a.bn + int(rank) * half_tokens;
+        for (int k = 0; k < a.steps; ++k) {
+          if (!(ok = wait_phase(&empty[st], int(phase), &wait))) break;
+          const uint32_t at = base + st * L::STAGE, bar = leader_address(&full[st]);
+          if (rank == 0) tc::mbar_arrive_expect_tx(&full[st], stage_bytes);
+          tma_load_2d_pair(at, &a.tm_w, k * kStepBytes, o, bar);
+          tma_load_2d_pair(at + L::A_BYTES, &a.tm_x, k * kStepBytes, t, bar);
+          ++loads;
+          if (++st == L::STAGES) {
+            st = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      // Nothing may arrive after the pair's end, which both CTAs reach together:
+      // stages have been handed back to both; after an expired wait the leader
+      // sees both CTAs' copies land, or waits its limit out.
+      if (ok || rank == 0)
+        for (int x = max(0, loads - L::STAGES); x < loads; ++x)
+          wait_phase(ok ? &empty[x % L::STAGES] : &full[x % L::STAGES], x / L::STAGES, &wait);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (rank == 0) {
+      const bool leader = elect_one();
+      const uint32_t idesc = idesc_i8(2 * kM, a.bn);
+      int st = 0, n = 0;
+      uint32_t phase = 0;
+      for (uint32_t tile = first; tile < a.tiles && ok; tile += pairs, ++n) {
+        const int buf = n & 1;
+        if (n >= 2) ok = wait_phase(&acc_empty[buf], (n >> 1) - 1, &wait);
+        tc::fence_after_sync();
+        const uint32_t d = tmem + buf * L::COLS;
+#pragma unroll 1
+        for (int k = 0; k < a.steps; ++k) {
+          ok = wait_phase(&full[st], int(phase), &wait) && ok;
+          if (!__all_sync(kFull, ok)) {
+            ok = false;
+            break;
+          }
+          tc::fence_after_sync();
+          if (leader) {
+            const uint32_t al = desc_low(base + st * L::STAGE, 16), bl = desc_low(base + st * L::STAGE + L::A_BYTES, 16);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mma_i8_pair(d, al + 2 * i, bl + 2 * i, idesc, k > 0 || i > 0);
+            commit_pair(&empty[st]);
+            if (k + 1 == a.steps) commit_pair(&acc_full[buf]);
+          }
+          __syncwarp();
+          if (++st == L::STAGES) {
+            st = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      if (!__all_sync(kFull, ok)) {
+        if (leader) commit_pair(&drained);
+        wait_phase(&drained, 0, &wait);
+      }
+    }
+    __syncwarp();
+  } else {
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t lanes = uint32_t(quarter * 32) << 16;
+    float* xs = s_xs[warp - 2];
+    const bool pairwise = (a.O & 1) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 3u) == 0;
+    int n = 0;
+    for (uint32_t tile = first; tile < a.tiles; tile += pairs, ++n) {
+      const int buf = n & 1;
+      const uint32_t tt = tile / a.tiles_o, to = tile - tt * a.tiles_o;
+      const int t0 = int(tt) * a.bn, t1 = min(a.T, t0 + a.bn), o = int(to * 2 + rank) * kM + quarter * 32 + lane;
+      __syncwarp();
+      for (int i = half * 32 + lane; i < a.bn; i += 64) xs[i] = t0 + i < a.T ? a.x_scale[t0 + i] : 0.f;
+      const float ws = o < a.O ? a.w_scale[o] : 0.f;
+      float bias = 0.f;
+      if (a.bias && o < a.O) bias = a.bias_f32 ? static_cast<const float*>(a.bias)[o] : to_f32<T>(static_cast<const T*>(a.bias)[o]);
+      __syncwarp();
+      ok = wait_phase(&acc_full[buf], n >> 1, &wait) && ok;
+      if (!__all_sync(kFull, ok)) break;
+      tc::fence_after_sync();
+#pragma unroll 1
+      for (int c = half * 32; c < a.bn; c += 64) store_tile<T>(a, tmem + buf * L::COLS + c + lanes, xs + c, ws, bias, t0 + c, t1, o, pairwise);
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) arrive_at(leader_address(&acc_empty[buf]));
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  if (threadIdx.x == 0 && wait.expired && a.status) atomicExch(a.status, PISA_ERR_TIMEOUT);
+  cluster_sync();   // the other CTA's signals have arrived, its reads of this one's shared memory are done
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(2 * L::COLS) : "memory");
+}
+
 __device__ __forceinline__ int4 load_peer(uint32_t addr, int rank) {
   int4 v;
   asm volatile("{\n\t.reg .b32 at;\n\tmapa.shared::cluster.u32 at, %4, %5;\n\tld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [at];\n\t}"
@@ -479,36 +675,72 @@ int launch(LinArgs a, const Operands& m, int split, cudaStream_t s) {
   return PISA_OK;
 }
 
-// Tokens of a tile (at most) and CTAs that share one.
+template <typename T>
+int launch_pairs(LinArgs a, const Operands& m, cudaStream_t s) {
+  a.bn = (tile_tokens(a.T, 256) + 31) / 32 * 32;      // halves of whole sixteens
+  int rc = byte_map(&a.tm_w, m.w, a.O, m.K, m.w_st, kM);
+  if (rc == PISA_OK) rc = byte_map(&a.tm_x, m.x, a.T, m.K, m.x_st, uint32_t(a.bn / 2));
+  if (rc == PISA_OK) rc = allow_smem<int8_linear_pair_kernel<T>>(PairTile::SMEM, "8-bit product smem attribute");
+  if (rc) return rc;
+  a.tiles_o = uint32_t((a.O + 2 * kM - 1) / (2 * kM));
+  const int64_t tiles = int64_t(a.tiles_o) * ((a.T + a.bn - 1) / a.bn);
+  if (tiles >= (int64_t(1) << 31)) return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
+  a.tiles = uint32_t(tiles);
+  int8_linear_pair_kernel<T><<<unsigned(2 * min64(tiles, sm_count() / 2)), kThreads, PairTile::SMEM, s>>>(a);
+  PISA_CHECK_LAUNCH();
+  return PISA_OK;
+}
+
+// Tokens of a tile (at most), CTAs that share one, and whether pairs of CTAs take tiles of 256 channels (split 0).
 struct Shape {
   int bn, split;
 };
 
+// The form with the least estimated time.  The estimates, in microseconds, are
+// fits of measurements over tiles, splits and shapes (1 to 32768 tokens, K 16 to
+// 16384, 96 to 60000 channels): a step of 128 bytes of K takes 0.235 + 0.00065 per
+// token of the tile (16 tokens 0.245, 256 tokens 0.40), of a pair's tile 0.20 +
+// 0.0005 (256 tokens 0.33), and all tiles' operands no less than HBM takes for
+// them; storing a tile takes 0.75 + 0.0095 per token, a pair's 1 + 0.011, mostly under
+// the next tile's steps; a split costs 1.3 and 0.008 per token, and clusters of 8
+// fit on three quarters of the SMs.  Both sides of each choice: 16384 x 4096 x
+// 11264 takes 499 us in single tiles and 437 in pairs, 8192 x 1024 x 5632 takes 45.6
+// and 46.8; one token over 4096 x 4096 takes 11.6 us unsplit and 8.4 split by 4,
+// over 1024 x 5632 5.7 and 6.8 (split by 2); 5110 x 64 x 3392 takes 13.9 us in tiles
+// of 256 tokens and 34.1 of 32, 326 x 128 x 1088 takes 5.1 and 3.7.
 Shape choose(int64_t T, int64_t O, int64_t steps) {
-  const int64_t sms = sm_count(), tiles_o = (O + kM - 1) / kM;
+  const int64_t sms = sm_count();
+  const double memory = double(T + O) * double(steps * kStepBytes) / 6.5e6;
   Shape best{256, 1};
   double least = 1e30;
+  const auto consider = [&](int most, int split, int64_t ctas, int64_t room, double step, double store, double fixed) {
+    const int64_t waves = (ctas + room - 1) / room;
+    const double work = double((steps + (split > 1 ? split : 1) - 1) / (split > 1 ? split : 1)) * step;
+    const double all = double(waves) * (work > store ? work + 0.1 * store : store + 0.1 * work);
+    const double cost = fixed + store + (all > memory ? all : memory);
+    if (cost < least) {
+      least = cost;
+      best = {most, split};
+    }
+  };
   for (int most = 16; most <= 256; most *= 2) {
     const int bn = tile_tokens(T, most);
     if (most > 16 && bn <= most / 2) break;
-    const int64_t tiles = tiles_o * ((T + bn - 1) / bn);
-    const double step = 0.22 + 0.00105 * bn, start = 4 + 0.01 * bn;
+    const int64_t tiles = (O + kM - 1) / kM * ((T + bn - 1) / bn);
     for (int split = 1; split <= 8; split *= 2) {
       if (split > steps || (split > 1 && tiles * split > (split == 8 ? sms * 3 / 4 : sms))) break;
-      const int64_t waves = (tiles * split + sms - 1) / sms;
-      const double cost = start + waves * ((steps + split - 1) / split) * step + (split > 1 ? 1.5 + 0.01 * bn : 0);
-      if (cost < least) {
-        least = cost;
-        best = {most, split};
-      }
+      consider(most, split, tiles * split, sms, 0.235 + 0.00065 * bn, 0.75 + 0.0095 * bn, split > 1 ? 5.3 + 0.008 * bn : 4.0);
     }
   }
+  const int bn = (tile_tokens(T, 256) + 31) / 32 * 32;
+  consider(256, 0, (O + 2 * kM - 1) / (2 * kM) * ((T + bn - 1) / bn), sms / 2, 0.20 + 0.0005 * bn, 1.0 + 0.011 * bn, 4.5);
   return best;
 }
 
 template <typename T>
 int dispatch(const LinArgs& a, const Operands& m, cudaStream_t s) {
   const Shape c = choose(a.T, a.O, a.steps);
+  if (c.split == 0) return launch_pairs<T>(a, m, s);
   switch (c.bn) {
     case 16: return launch<T, 16>(a, m, c.split, s);
     case 32: return launch<T, 32>(a, m, c.split, s);

@@ -63,9 +63,12 @@ def test_long_sums_are_exact(cuda_device, tokens):
 
 
 def test_large(cuda_device):
-    """Many tiles per CTA, in both directions."""
+    """Many tiles per CTA, in both directions; long K, where pairs of CTAs share tiles."""
     gen = torch.Generator(device="cuda").manual_seed(1)
     compare(*case(gen, 4099, 640, 3000), dtype=BF16)
+    compare(*case(gen, 4099, 2820, 865), dtype=F16)
+    compare(*case(gen, 2500, 4096, 3001), scales(gen, 3001), F32)
+    compare(*case(gen, 700, 9000, 1030), dtype=BF16)
     compare(*case(gen, 9000, 200, 1100), scales(gen, 1100), F16)
     compare(*case(gen, 20, 300, 70000), dtype=F32)
 
