@@ -73,6 +73,35 @@ __device__ __forceinline__ Raw8<T> narrow8(const float (&f)[8]) {
   return r;
 }
 
+// Arithmetic on pairs: one instruction for two fp32 results.
+__device__ __forceinline__ float2 pair_fma(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rc, {%6, %7};\n\t"
+      "fma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 pair_mul(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmul.rn.f32x2 rd, ra, rb;\n\t"
+      "mov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 pair_add(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tadd.rn.f32x2 rd, ra, rb;\n\t"
+      "mov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 pair_at(const float (&f)[8], int i) { return make_float2(f[2 * i], f[2 * i + 1]); }
+__device__ __forceinline__ void set_pair(float (&f)[8], int i, float2 v) {
+  f[2 * i] = v.x;
+  f[2 * i + 1] = v.y;
+}
+
 // Data that is read once: past L1.
 __device__ __forceinline__ uint4 load_stream(const void* p) {
   uint4 v;
@@ -106,8 +135,12 @@ __device__ __forceinline__ Raw8<T> load_piece(const T* row, int j, int t, int D)
     for (int e = 0; e < 8; ++e) {
       const int c = column<TPR, A>(j, e, t);
       if (c < D) {
-        if constexpr (sizeof(T) == 4) w[e] = reinterpret_cast<const uint32_t*>(row)[c];
-        else w[e / 2] |= uint32_t(reinterpret_cast<const uint16_t*>(row)[c]) << (e % 2 * 16);
+        if constexpr (sizeof(T) == 4) asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(w[e]) : "l"(row + c));
+        else {
+          uint16_t h;
+          asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(h) : "l"(row + c));
+          w[e / 2] |= uint32_t(h) << (e % 2 * 16);
+        }
       }
     }
 #pragma unroll
@@ -177,7 +210,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 template <int TPR, bool MAX>
 __device__ __forceinline__ float team_reduce(float v, float* red, int& set) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
+  for (int o = TPR < 32 ? TPR / 2 : 16; o > 0; o >>= 1) {
     const float w = __shfl_xor_sync(kFull, v, o);
     v = MAX ? max_nan(v, w) : v + w;
   }

@@ -48,7 +48,7 @@ def compare(t, a=1.0, b=1.0, grads=None, seed=99):
         R.check("d" + k, got[k], *want["d" + k])
 
 
-WIDTHS = [1, 7, 8, 64, 255, 256, 257, 264, 512, 1000, 1024, 1025, 2048, 2056, 4096, 4097, 8192, 8200, 16383, 16384]
+WIDTHS = [1, 7, 8, 64, 72, 128, 136, 255, 256, 257, 264, 512, 1000, 1024, 1025, 2048, 2056, 4096, 4097, 8192, 8200, 16383, 16384]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
@@ -70,8 +70,8 @@ def test_gates(cuda_device, dtype, gate, post, batch, tokens):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("width", [64, 520, 1536, 2560])
-@pytest.mark.parametrize("gate", ["width", "sequence"])
+@pytest.mark.parametrize("width", [40, 61, 104, 200, 520, 1536, 2560, 4800])
+@pytest.mark.parametrize("gate", ["width", "sequence", "token"])
 def test_many_rows(cuda_device, dtype, width, gate):
     """More rows than teams: parameter gradients over many turns, shares of unequal teams."""
     gen = torch.Generator(device="cuda").manual_seed(1)
@@ -81,6 +81,8 @@ def test_many_rows(cuda_device, dtype, width, gate):
 def test_many_short_sequences(cuda_device):
     gen = torch.Generator(device="cuda").manual_seed(2)
     compare(inputs(gen, 3001, 2, 72, BF16, "sequence"))
+    compare(inputs(gen, 3001, 3, 24, BF16, "sequence", True, BF16))
+    compare(inputs(gen, 7, 5, 24, F32, "sequence", False))
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -136,7 +138,7 @@ def test_layouts(cuda_device):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("rows,width", [(1, 64), (37, 72), (700, 1000), (5, 1001), (3, 8200)])
+@pytest.mark.parametrize("rows,width", [(1, 64), (37, 72), (700, 1000), (5, 1001), (3, 8200), (5000, 48), (3000, 57), (900, 6001)])
 def test_nothing_is_written_past_the_rows(cuda_device, dtype, rows, width):
     """Both entry points on slices of larger buffers: what lies around the outputs stays as it was."""
     from nlogn_pisa_b200 import _lib
