@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) row_kernel(const __grid
   for (int j = 0; j < NV; ++j) {
     float f[8];
     widen8<T>(x[j], f);
-    store_piece_s8<TPR, A>(qr, j, t, D, f, top < INFINITY, s.inv);
+    store_piece_s8<T, TPR, A>(qr, j, t, D, f, top < INFINITY, s.inv);
   }
   if (t == 0) a.scale[row] = s.scale;
 }
@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(512) long_row_kernel(const __grid_constant__ R
     const int left = int(min64(STEP, a.D - at));
     float f[8];
     widen8<T>(load_piece<T, TPR, A>(xr + at, 0, threadIdx.x, left), f);
-    store_piece_s8<TPR, A>(qr + at, 0, threadIdx.x, left, f, top < INFINITY, s.inv);
+    store_piece_s8<T, TPR, A>(qr + at, 0, threadIdx.x, left, f, top < INFINITY, s.inv);
   }
   if (threadIdx.x == 0) a.scale[row] = s.scale;
 }
@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(kThreads) group_kernel(const __grid_constant__
   int8_t* qr = a.q + row * a.q_st + first;
   float f[8];
   if constexpr (BACK) {
-    widen8_s8(load_piece_s8<16, A>(qr, t, width), a.scale[at], f);
+    widen8_s8(load_piece_s8<T, 16, A>(qr, t, width), a.scale[at], f);
     store_piece<T, 16, A>(static_cast<T*>(a.out) + row * a.D + first, 0, t, width, f);
   } else {
     widen8<T>(load_piece<T, 16, A>(static_cast<const T*>(a.x) + row * a.x_st + first, 0, t, width), f);
@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(kThreads) group_kernel(const __grid_constant__
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(kFull, top, o));
     const Scale8 s(top);
-    store_piece_s8<16, A>(qr, 0, t, width, f, top < INFINITY, s.inv);
+    store_piece_s8<T, 16, A>(qr, 0, t, width, f, top < INFINITY, s.inv);
     if (live && t == 0) a.scale[at] = s.scale;
   }
 }

@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm_fwd_kernel(const _
     const Scale8 s(top);
     int8_t* qr = a.n_q + row * a.n_q_st;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) store_piece_s8<TPR, A>(qr, j, t, D, h[j], top < INFINITY, s.inv);
+    for (int j = 0; j < NV; ++j) store_piece_s8<T, TPR, A>(qr, j, t, D, h[j], top < INFINITY, s.inv);
     if (t == 0 && live) a.n_scale[row] = s.scale;
   } else {
     T* nr = static_cast<T*>(a.n) + row * a.D;
@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(128) norm_columns_kernel(const __grid_constant
   float* out = a.partial + int64_t(team) * a.sums * D + c0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const int c = column<TPR, A>(0, e, t);
+    const int c = column<T, TPR, A>(0, e, t);
     if (c < width) {
       out[c] = dw[e];
       if (a.sum_post) out[a.sum_post * int64_t(D) + c] = dp[e];
@@ -344,12 +344,14 @@ struct Ring {
   __device__ __forceinline__ uint32_t stats(int slot) const {
     return base + ROWS * tensors * PIECES * THREADS * 16 + (slot * THREADS + threadIdx.x) * 8;
   }
-  __device__ __forceinline__ void fill(int slot, int k, const T* row, int c, int D) const {
+  __device__ __forceinline__ void fill(int slot, int k, const T* row, int t, int D) const {
     // columns past the row's end are zeros: nothing is read
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i)
+    for (int i = 0; i < PIECES; ++i) {
+      const int c = column<T, TPR, true>(0, 4 * i, t);
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(at(slot, k) + i * THREADS * 16),
-                   "l"(row + (c < D ? c + i * (8 / PIECES) : 0)), "r"(c < D ? 16 : 0) : "memory");
+                   "l"(row + (c < D ? c : 0)), "r"(c < D ? 16 : 0) : "memory");
+    }
   }
   __device__ __forceinline__ Raw8<T> take(int slot, int k) const {
     Raw8<T> r;
@@ -399,12 +401,11 @@ norm_bwd_row_kernel(const __grid_constant__ NormArgs a) {
   const T* dhs = static_cast<const T*>(a.dh);
   auto fetch = [&](int64_t row, int slot) {
     if constexpr (A) {
-      const int c = column<TPR, true>(0, 0, t);
-      ring.fill(slot, 0, xs + row * a.x_st, c, D);
-      ring.fill(slot, 1, dns + row * D, c, D);
-      if (dhs) ring.fill(slot, 2, dhs + row * D, c, D);
-      if (ys) ring.fill(slot, 3, ys + row * a.y_st, c, D);
-      if (token_gate) ring.fill(slot, 4, gs + row * a.gate_st, c, D);
+      ring.fill(slot, 0, xs + row * a.x_st, t, D);
+      ring.fill(slot, 1, dns + row * D, t, D);
+      if (dhs) ring.fill(slot, 2, dhs + row * D, t, D);
+      if (ys) ring.fill(slot, 3, ys + row * a.y_st, t, D);
+      if (token_gate) ring.fill(slot, 4, gs + row * a.gate_st, t, D);
       asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" :: "r"(ring.stats(slot)), "l"(a.stats + 2 * row) : "memory");
     } else {
       next.x = load_piece<T, TPR, A>(xs + row * a.x_st, 0, t, D);
@@ -553,7 +554,7 @@ norm_bwd_row_kernel(const __grid_constant__ NormArgs a) {
     float* mine = buf + int(threadIdx.x / TPR) * a.sums * D;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int c = column<TPR, A>(0, e, t);
+      const int c = column<T, TPR, A>(0, e, t);
       if (c < D) {
         mine[c] = dw[e];
         if (a.sum_post) mine[a.sum_post * D + c] = dp[e];
@@ -573,7 +574,7 @@ norm_bwd_row_kernel(const __grid_constant__ NormArgs a) {
   float* out = a.partial + int64_t(team) * a.sums * D;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const int c = column<TPR, A>(0, e, t);
+    const int c = column<T, TPR, A>(0, e, t);
     if (c < D) {
       out[c] = dw[e];
       if (a.sum_post) out[a.sum_post * int64_t(D) + c] = dp[e];

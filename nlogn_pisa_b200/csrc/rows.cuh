@@ -3,7 +3,8 @@
 //
 // A team of TPR threads holds a row in registers, NV pieces of 8 elements per
 // thread.  Where every row starts on 16 bytes and its width is a multiple of 8
-// (A), piece j of thread t is 8 consecutive elements; otherwise its elements lie
+// (A), piece j of thread t is 8 consecutive elements, in fp32 two times 4 of them,
+// so that a warp's 16-byte accesses lie side by side; otherwise its elements lie
 // TPR apart, so that a warp still touches consecutive ones.
 #pragma once
 
@@ -110,9 +111,11 @@ __device__ __forceinline__ uint4 load_stream(const void* p) {
 }
 
 // Column of element e of piece j.
-template <int TPR, bool A>
+template <typename T, int TPR, bool A>
 __device__ __forceinline__ int column(int j, int e, int t) {
-  return A ? (j * TPR + t) * 8 + e : (j * 8 + e) * TPR + t;
+  if constexpr (!A) return (j * 8 + e) * TPR + t;
+  else if constexpr (sizeof(T) == 2) return (j * TPR + t) * 8 + e;
+  else return ((2 * j + e / 4) * TPR + t) * 4 + e % 4;
 }
 
 // Piece j of a row of D elements; elements past its end are zeros.
@@ -122,10 +125,10 @@ __device__ __forceinline__ Raw8<T> load_piece(const T* row, int j, int t, int D)
 #pragma unroll
   for (int i = 0; i < int(sizeof(T) / 2); ++i) r.v[i] = make_uint4(0, 0, 0, 0);
   if constexpr (A) {
-    const int c = column<TPR, A>(j, 0, t);
-    if (c < D) {
 #pragma unroll
-      for (int i = 0; i < int(sizeof(T) / 2); ++i) r.v[i] = load_stream(reinterpret_cast<const uint4*>(row + c) + i);
+    for (int i = 0; i < int(sizeof(T) / 2); ++i) {
+      const int c = column<T, TPR, A>(j, 4 * i, t);
+      if (c < D) r.v[i] = load_stream(row + c);
     }
   } else {
     uint32_t w[2 * sizeof(T)];
@@ -133,7 +136,7 @@ __device__ __forceinline__ Raw8<T> load_piece(const T* row, int j, int t, int D)
     for (int i = 0; i < int(2 * sizeof(T)); ++i) w[i] = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int c = column<TPR, A>(j, e, t);
+      const int c = column<T, TPR, A>(j, e, t);
       if (c < D) {
         if constexpr (sizeof(T) == 4) asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(w[e]) : "l"(row + c));
         else {
@@ -152,16 +155,16 @@ __device__ __forceinline__ Raw8<T> load_piece(const T* row, int j, int t, int D)
 template <typename T, int TPR, bool A>
 __device__ __forceinline__ void store_piece(T* row, int j, int t, int D, const float (&f)[8]) {
   if constexpr (A) {
-    const int c = column<TPR, A>(j, 0, t);
-    if (c < D) {
-      const Raw8<T> r = narrow8<T>(f);
+    const Raw8<T> r = narrow8<T>(f);
 #pragma unroll
-      for (int i = 0; i < int(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(row + c)[i] = r.v[i];
+    for (int i = 0; i < int(sizeof(T) / 2); ++i) {
+      const int c = column<T, TPR, A>(j, 4 * i, t);
+      if (c < D) *reinterpret_cast<uint4*>(row + c) = r.v[i];
     }
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int c = column<TPR, A>(j, e, t);
+      const int c = column<T, TPR, A>(j, e, t);
       if (c < D) row[c] = from_f32<T>(f[e]);
     }
   }
@@ -173,24 +176,25 @@ __device__ __forceinline__ void param_piece(const void* p, int f32, int j, int t
 #pragma unroll
   for (int e = 0; e < 8; ++e) f[e] = 0.f;
   if constexpr (A) {
-    const int c = column<TPR, A>(j, 0, t);
-    if (c >= D) return;
     if (f32) {
-      const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + c);
-      const float4 lo = __ldg(q), hi = __ldg(q + 1);
-      f[0] = lo.x; f[1] = lo.y; f[2] = lo.z; f[3] = lo.w;
-      f[4] = hi.x; f[5] = hi.y; f[6] = hi.z; f[7] = hi.w;
-    } else {
-      Raw8<T> r;
 #pragma unroll
-      for (int i = 0; i < int(sizeof(T) / 2); ++i)
-        r.v[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p) + c) + i);
+      for (int i = 0; i < 2; ++i) {
+        const int c = column<T, TPR, A>(j, 4 * i, t);
+        if (c >= D) continue;
+        const float4 q = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + c));
+        f[4 * i] = q.x; f[4 * i + 1] = q.y; f[4 * i + 2] = q.z; f[4 * i + 3] = q.w;
+      }
+    } else if constexpr (sizeof(T) == 2) {
+      const int c = column<T, TPR, A>(j, 0, t);
+      if (c >= D) return;
+      Raw8<T> r;
+      r.v[0] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p) + c));
       widen8<T>(r, f);
     }
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int c = column<TPR, A>(j, e, t);
+      const int c = column<T, TPR, A>(j, e, t);
       if (c < D) f[e] = f32 ? static_cast<const float*>(p)[c] : to_f32<T>(static_cast<const T*>(p)[c]);
     }
   }
@@ -262,32 +266,43 @@ __device__ __forceinline__ void unpack_s8(uint32_t q, float (&f)[4]) {
   f[3] = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7443)) - off;
 }
 
-template <int TPR, bool A>
+template <typename T, int TPR, bool A>
 __device__ __forceinline__ void store_piece_s8(int8_t* row, int j, int t, int D, const float (&f)[8], bool fine, float inv) {
   uint32_t lo = pack_s8(f[0], f[1], f[2], f[3], inv), hi = pack_s8(f[4], f[5], f[6], f[7], inv);
   if (!fine) lo = hi = 0;
   if constexpr (A) {
-    const int c = column<TPR, A>(j, 0, t);
-    if (c < D) *reinterpret_cast<uint2*>(row + c) = make_uint2(lo, hi);
+    const int c = column<T, TPR, A>(j, 0, t), c4 = column<T, TPR, A>(j, 4, t);
+    if constexpr (sizeof(T) == 2) {
+      if (c < D) *reinterpret_cast<uint2*>(row + c) = make_uint2(lo, hi);
+    } else {
+      if (c < D) *reinterpret_cast<uint32_t*>(row + c) = lo;
+      if (c4 < D) *reinterpret_cast<uint32_t*>(row + c4) = hi;
+    }
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int c = column<TPR, A>(j, e, t);
+      const int c = column<T, TPR, A>(j, e, t);
       if (c < D) row[c] = int8_t((e < 4 ? lo >> (8 * e) : hi >> (8 * (e - 4))) & 255u);
     }
   }
 }
 
 // Piece 0 of kept bytes, zeros past their end, and as floats.
-template <int TPR, bool A>
+template <typename T, int TPR, bool A>
 __device__ __forceinline__ uint2 load_piece_s8(const int8_t* row, int t, int D) {
   uint2 r = make_uint2(0, 0);
   if constexpr (A) {
-    if (t * 8 < D) asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(row + t * 8));
+    const int c = column<T, TPR, A>(0, 0, t), c4 = column<T, TPR, A>(0, 4, t);
+    if constexpr (sizeof(T) == 2) {
+      if (c < D) asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(row + c));
+    } else {
+      if (c < D) asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(r.x) : "l"(row + c));
+      if (c4 < D) asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(r.y) : "l"(row + c4));
+    }
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int c = column<TPR, A>(0, e, t);
+      const int c = column<T, TPR, A>(0, e, t);
       const uint32_t b = c < D ? uint8_t(row[c]) : 0;
       if (e < 4) r.x |= b << (8 * e);
       else r.y |= b << (8 * (e - 4));

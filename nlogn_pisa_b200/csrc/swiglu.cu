@@ -116,8 +116,8 @@ __global__ void __launch_bounds__(kGluThreads) glu_fwd_kernel(const __grid_const
       const float m = fmaxf(t & 1 ? top_u : top_g, kTiny), r = __fdiv_rn(t & 2 ? m : 127.f, t & 2 ? 127.f : m);
       const int team = threadIdx.x & 16;
       const bool fine_g = top_g < INFINITY, fine_u = top_u < INFINITY;
-      store_piece_s8<16, A>(a.g_q + n.row * a.q_st + n.first, 0, t, n.width, g, fine_g, __shfl_sync(kFull, r, team));
-      store_piece_s8<16, A>(a.u_q + n.row * a.q_st + n.first, 0, t, n.width, u, fine_u, __shfl_sync(kFull, r, team + 1));
+      store_piece_s8<T, 16, A>(a.g_q + n.row * a.q_st + n.first, 0, t, n.width, g, fine_g, __shfl_sync(kFull, r, team));
+      store_piece_s8<T, 16, A>(a.u_q + n.row * a.q_st + n.first, 0, t, n.width, u, fine_u, __shfl_sync(kFull, r, team + 1));
       if (n.width && (t & ~1) == 2) (t & 1 ? a.u_scale : a.g_scale)[n.at] = (t & 1 ? fine_u : fine_g) ? r : __int_as_float(0x7fffffff);
     }
   }
@@ -134,8 +134,8 @@ __global__ void __launch_bounds__(kGluThreads) glu_bwd_kernel(const __grid_const
     const GluGroup<U> n(a, i);
     dr[i] = load_piece<T, 16, A>(static_cast<const T*>(a.dout) + n.row * a.dout_st + n.first, 0, t, n.width);
     if constexpr (KEPT) {
-      gq[i] = load_piece_s8<16, A>(a.g_q + n.row * a.q_st + n.first, t, n.width);
-      uq[i] = load_piece_s8<16, A>(a.u_q + n.row * a.q_st + n.first, t, n.width);
+      gq[i] = load_piece_s8<T, 16, A>(a.g_q + n.row * a.q_st + n.first, t, n.width);
+      uq[i] = load_piece_s8<T, 16, A>(a.u_q + n.row * a.q_st + n.first, t, n.width);
       gs[i] = a.g_scale[n.at];
       us[i] = a.u_scale[n.at];
     } else {
@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) glu_row_kernel(const __
   const Scale8 s(top);
   int8_t* qr = a.a_q + row * a.a_q_st;
 #pragma unroll
-  for (int j = 0; j < NV; ++j) store_piece_s8<TPR, A>(qr, j, t, D, o[j], top < INFINITY, s.inv);
+  for (int j = 0; j < NV; ++j) store_piece_s8<T, TPR, A>(qr, j, t, D, o[j], top < INFINITY, s.inv);
   if (t == 0) a.a_scale[row] = s.scale;
 }
 
