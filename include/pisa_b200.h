@@ -40,6 +40,7 @@ extern "C" {
 #define PISA_F32 0
 #define PISA_BF16 1
 #define PISA_F16 2
+#define PISA_S8 3   /* signed bytes (pisa_int8_linear) */
 
 /* ---- scoring methods (pisa1 = first order, pisa2 = second order, pisa = LSE) ---- */
 #define PISA_METHOD_PISA1 0
@@ -543,19 +544,22 @@ PISA_API int pisa_restore_int8(const int8_t *q, int64_t q_st, const float *scale
 /*
  * out[t, o] = x_scale[t] * weight_scale[o] * sum_k x[t, k] * weight[o, k] +
  * bias[o] over signed bytes; the sums are exact.
- * x: [T, K], weight: [O, K], rows x_st and weight_st bytes apart and on 16
- * bytes (bytes past a row's K elements are not used); K below 131072.
+ * x: [T, K] in x_dtype, rows x_st elements apart.  PISA_S8: bytes with their
+ *   scales x_scale [T].  Otherwise the call rounds the rows into its workspace,
+ *   as pisa_quantize_int8 (x_scale is not used).
+ * weight: [O, K] bytes, rows weight_st apart.  8-bit rows start on 16 bytes
+ *   (bytes past a row's K elements are not used); K below 131072.
  * bias: [O] in FP32 or out_dtype, or NULL.  out: contiguous [T, O].
- * workspace: NULL, or pisa_int8_linear_workspace_bytes(...) bytes whose first 4
- *   receive the device status word; the outputs of a call with an expired wait
- *   are undefined.
+ * workspace: pisa_int8_linear_workspace_bytes(...) bytes on 16 bytes (NULL is
+ *   allowed with PISA_S8) whose first 4 receive the device status word; the
+ *   outputs of a call with an expired wait are undefined.
  */
-PISA_API int pisa_int8_linear(const int8_t *x, int64_t x_st, const float *x_scale, const int8_t *weight,
+PISA_API int pisa_int8_linear(const void *x, int64_t x_st, int x_dtype, const float *x_scale, const int8_t *weight,
                               int64_t weight_st, const float *weight_scale, const void *bias, int bias_dtype,
                               int out_dtype, int64_t T, int64_t K, int64_t O, void *out, void *workspace,
                               int64_t workspace_bytes, pisa_stream_t stream);
 
-PISA_API int64_t pisa_int8_linear_workspace_bytes(int64_t T, int64_t K, int64_t O);
+PISA_API int64_t pisa_int8_linear_workspace_bytes(int64_t T, int64_t K, int64_t O, int x_dtype);
 
 /* ---- device status (no counterpart in the reference, whose Triton kernels never wait) ----
  * Every kernel that waits on another part of the GPU waits a bounded number

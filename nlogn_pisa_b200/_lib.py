@@ -17,7 +17,7 @@ import torch
 LIB_PATH = Path(__file__).resolve().with_name("libpisa_b200.so")
 
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_CUDA, ERR_TIMEOUT = 0, 1, 2, 3, 4
-F32, BF16, F16 = 0, 1, 2
+F32, BF16, F16, S8 = 0, 1, 2, 3
 METHODS = {"pisa1": 0, "pisa2": 1, "pisa": 2}
 SCHEDULES = {"grouped": 0, "fused": 1}
 DTYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
@@ -83,8 +83,8 @@ SIGNATURES = {
     "pisa_swiglu_bwd": (_I, [_P, _L, _P, _L, _P, _L, _P, _P, _L, _P, _P, _I, _L, _L, _P, _P, _P, _P]),
     "pisa_quantize_int8": (_I, [_P, _L, _I, _L, _L, _I, _P, _L, _P, _P]),
     "pisa_restore_int8": (_I, [_P, _L, _P, _I, _L, _L, _P, _P]),
-    "pisa_int8_linear": (_I, [_P, _L, _P, _P, _L, _P, _P, _I, _I, _L, _L, _L, _P, _P, _L, _P]),
-    "pisa_int8_linear_workspace_bytes": (_L, [_L, _L, _L]),
+    "pisa_int8_linear": (_I, [_P, _L, _I, _P, _P, _L, _P, _P, _I, _I, _L, _L, _L, _P, _P, _L, _P]),
+    "pisa_int8_linear_workspace_bytes": (_L, [_L, _L, _L, _I]),
     "pisa_workspace_status": (_I, [_P, _P]),
     "pisa_wait_selftest": (_I, [_I, _L, _P, _L, _P]),
     "pisa_ex2_selftest": (_I, [_P, _P, _P, _L, _P]),

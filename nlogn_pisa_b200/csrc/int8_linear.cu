@@ -20,6 +20,10 @@
 
 namespace pisa {
 
+// pisa_quantize_int8 of rows, which clears a status word on its way (int8_rows.cu)
+int quantize_rows(const void* x, int64_t x_st, int dtype, int64_t rows, int64_t D, int8_t* q, int64_t q_st, float* scale, int* status,
+                  cudaStream_t s);
+
 namespace {
 
 constexpr int kM = 128;          // output channels of a tile
@@ -756,39 +760,56 @@ int dispatch(const LinArgs& a, const Operands& m, cudaStream_t s) {
 
 extern "C" {
 
-int64_t pisa_int8_linear_workspace_bytes(int64_t T, int64_t K, int64_t O) {
-  return T <= 0 || K <= 0 || O <= 0 ? -1 : 256;
+// workspace: status word, then (floating x) the tokens' scales and bytes
+int64_t pisa_int8_linear_workspace_bytes(int64_t T, int64_t K, int64_t O, int x_dtype) {
+  if (T <= 0 || K <= 0 || O <= 0 || x_dtype < PISA_F32 || x_dtype > PISA_S8) return -1;
+  return 256 + (x_dtype == PISA_S8 ? 0 : (T * 4 + 255) / 256 * 256 + T * ((K + 15) / 16 * 16));
 }
 
-int pisa_int8_linear(const int8_t* x, int64_t x_st, const float* x_scale, const int8_t* weight, int64_t weight_st,
+int pisa_int8_linear(const void* x, int64_t x_st, int x_dtype, const float* x_scale, const int8_t* weight, int64_t weight_st,
                      const float* weight_scale, const void* bias, int bias_dtype, int out_dtype, int64_t T, int64_t K, int64_t O,
                      void* out, void* workspace, int64_t workspace_bytes, pisa_stream_t stream) {
   using namespace pisa;
-  if (out_dtype < PISA_F32 || out_dtype > PISA_F16) return fail(PISA_ERR_UNSUPPORTED, "the kernels support FP16, BF16 and FP32");
+  const bool bytes = x_dtype == PISA_S8;
+  if (out_dtype < PISA_F32 || out_dtype > PISA_F16 || x_dtype < PISA_F32 || x_dtype > PISA_S8)
+    return fail(PISA_ERR_UNSUPPORTED, "the kernels support FP16, BF16 and FP32");
   if (bias && bias_dtype != out_dtype && bias_dtype != PISA_F32)
     return fail(PISA_ERR_UNSUPPORTED, "the bias must be FP32 or the output's type");
   if (T <= 0 || K <= 0 || O <= 0) return fail(PISA_ERR_INVALID, "nonempty tensors are required");
   if (K >= (int64_t(1) << 17)) return fail(PISA_ERR_UNSUPPORTED, "sums of 131072 or more products may not fit 32 bits");
   if (T >= (int64_t(1) << 31) - 256 || O >= (int64_t(1) << 31) - 256) return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
-  if (!x || !x_scale || !weight || !weight_scale || !out) return fail(PISA_ERR_INVALID, "operands, scales and out are required");
-  if (T == 1) x_st = (K + 15) / 16 * 16;          // the stride of a single row may hold anything
-  if (O == 1) weight_st = (K + 15) / 16 * 16;
-  if ((reinterpret_cast<uintptr_t>(x) & 15u) || (reinterpret_cast<uintptr_t>(weight) & 15u) || x_st % 16 || weight_st % 16)
+  if (!x || (bytes && !x_scale) || !weight || !weight_scale || !out)
+    return fail(PISA_ERR_INVALID, "operands, scales and out are required");
+  const int64_t row_bytes = (K + 15) / 16 * 16;
+  if (T == 1 && bytes) x_st = row_bytes;          // the stride of a single row may hold anything
+  if (O == 1) weight_st = row_bytes;
+  if ((bytes && ((reinterpret_cast<uintptr_t>(x) & 15u) || x_st % 16)) || (reinterpret_cast<uintptr_t>(weight) & 15u) || weight_st % 16)
     return fail(PISA_ERR_UNSUPPORTED, "8-bit rows must start on 16 bytes");
-  if (x_st < K || weight_st < K) return fail(PISA_ERR_UNSUPPORTED, "8-bit rows must not overlap");
-  if (workspace && workspace_bytes < 256) return fail(PISA_ERR_INVALID, "workspace too small");
+  if ((bytes && x_st < K) || weight_st < K) return fail(PISA_ERR_UNSUPPORTED, "8-bit rows must not overlap");
+  if (workspace ? workspace_bytes < pisa_int8_linear_workspace_bytes(T, K, O, x_dtype) : !bytes)
+    return fail(PISA_ERR_INVALID, "workspace too small");
+  if (!bytes && (reinterpret_cast<uintptr_t>(workspace) & 15u)) return fail(PISA_ERR_INVALID, "workspace must start on 16 bytes");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   LinArgs a{};
+  a.status = static_cast<int*>(workspace);
+  Operands m{x, x_st, weight, weight_st, K};
+  if (bytes) {
+    if (workspace) {
+      cudaError_t e = cudaMemsetAsync(workspace, 0, 256, s);
+      if (e != cudaSuccess) return fail_cuda(e, "status clear");
+    }
+  } else {
+    float* scale = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
+    int8_t* values = static_cast<int8_t*>(workspace) + 256 + (T * 4 + 255) / 256 * 256;
+    if (int rc = quantize_rows(x, x_st, x_dtype, T, K, values, row_bytes, scale, a.status, s)) return rc;
+    x_scale = scale;
+    m.x = values;
+    m.x_st = row_bytes;
+  }
   a.w_scale = weight_scale; a.x_scale = x_scale; a.bias = bias; a.bias_f32 = bias_dtype == PISA_F32;
   a.T = int(T); a.O = int(O); a.steps = int((K + kStepBytes - 1) / kStepBytes);
   a.tries = wait_tries(a.steps);
   a.out = out;
-  if (workspace) {
-    a.status = static_cast<int*>(workspace);
-    cudaError_t e = cudaMemsetAsync(workspace, 0, 256, s);
-    if (e != cudaSuccess) return fail_cuda(e, "status clear");
-  }
-  const Operands m{x, x_st, weight, weight_st, K};
   if (out_dtype == PISA_F32) return dispatch<float>(a, m, s);
   if (out_dtype == PISA_BF16) return dispatch<__nv_bfloat16>(a, m, s);
   return dispatch<__half>(a, m, s);

@@ -21,6 +21,7 @@ struct RowArgs {
   int64_t q_st;
   float* scale;
   void* out;
+  int* status;            // cleared on the way, or NULL
 };
 
 // A team holds the row.
@@ -31,6 +32,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) row_kernel(const __grid
   int set = 0;
   const int t = threadIdx.x % TPR, D = int(a.D);
   const int64_t row = int64_t(blockIdx.x) * TEAMS + threadIdx.x / TPR;
+  if (a.status && row == 0 && t == 0) *a.status = PISA_OK;
   if (row >= a.rows) return;                      // a whole warp
   const T* xr = static_cast<const T*>(a.x) + row * a.x_st;
   Raw8<T> x[NV];
@@ -63,6 +65,7 @@ __global__ void __launch_bounds__(512) long_row_kernel(const __grid_constant__ R
   __shared__ float red[2 * (TPR / 32)];
   int set = 0;
   const int64_t row = blockIdx.x;
+  if (a.status && row == 0 && threadIdx.x == 0) *a.status = PISA_OK;
   const T* xr = static_cast<const T*>(a.x) + row * a.x_st;
   float top = 0.f;
   for (int64_t at = 0; at < a.D; at += STEP) {
@@ -162,6 +165,17 @@ RowArgs make_args(int64_t rows, int64_t D, int8_t* q, int64_t q_st, float* scale
 
 }  // namespace
 
+int quantize_rows(const void* x, int64_t x_st, int dtype, int64_t rows, int64_t D, int8_t* q, int64_t q_st, float* scale, int* status,
+                  cudaStream_t s) {
+  if (int rc = check(x, q, q_st, scale, dtype, rows, D)) return rc;
+  RowArgs a = make_args(rows, D, q, q_st, scale);
+  a.x = x; a.x_st = x_st; a.status = status;
+  const bool aligned = D % 8 == 0 && rows_on16(x, rows, x_st * (dtype == PISA_F32 ? 4 : 2));
+  if (dtype == PISA_F32) return rows8<float>(a, aligned, s);
+  if (dtype == PISA_BF16) return rows8<__nv_bfloat16>(a, aligned, s);
+  return rows8<__half>(a, aligned, s);
+}
+
 }  // namespace pisa
 
 extern "C" {
@@ -169,19 +183,15 @@ extern "C" {
 int pisa_quantize_int8(const void* x, int64_t x_st, int dtype, int64_t rows, int64_t D, int grouped, int8_t* q, int64_t q_st,
                        float* scale, pisa_stream_t stream) {
   using namespace pisa;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (!grouped) return quantize_rows(x, x_st, dtype, rows, D, q, q_st, scale, nullptr, s);
   if (int rc = check(x, q, q_st, scale, dtype, rows, D)) return rc;
   RowArgs a = make_args(rows, D, q, q_st, scale);
   a.x = x; a.x_st = x_st;
   const bool aligned = D % 8 == 0 && rows_on16(x, rows, x_st * (dtype == PISA_F32 ? 4 : 2));
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (grouped) {
-    if (dtype == PISA_F32) return groups8<float, false>(a, aligned, s);
-    if (dtype == PISA_BF16) return groups8<__nv_bfloat16, false>(a, aligned, s);
-    return groups8<__half, false>(a, aligned, s);
-  }
-  if (dtype == PISA_F32) return rows8<float>(a, aligned, s);
-  if (dtype == PISA_BF16) return rows8<__nv_bfloat16>(a, aligned, s);
-  return rows8<__half>(a, aligned, s);
+  if (dtype == PISA_F32) return groups8<float, false>(a, aligned, s);
+  if (dtype == PISA_BF16) return groups8<__nv_bfloat16, false>(a, aligned, s);
+  return groups8<__half, false>(a, aligned, s);
 }
 
 int pisa_restore_int8(const int8_t* q, int64_t q_st, const float* scale, int dtype, int64_t rows, int64_t D, void* out,

@@ -176,24 +176,26 @@ def int8_linear(x, weight, weight_scale, bias=None, x_scale=None, out_dtype=None
             raise ValueError("x, weight, scales and bias must share a device")
     require_cuda(x)
     no_gradient("int8_linear", x, weight_scale, *([x_scale] if whole else []), *([] if bias is None else [bias]))
-    if not whole:
-        x, x_scale = _quantize(x, _floating(x, "x"), False)
     count = x.numel() // inner
-    (rows, x_stride), (weight, w_stride) = aligned_bytes(x), aligned_bytes(weight)
-    x_scale, weight_scale = x_scale.contiguous(), weight_scale.contiguous()
+    weight, w_stride = aligned_bytes(weight)
+    weight_scale = weight_scale.contiguous()
     bias_args = (None, 0)
     if bias is not None:
         bias = bias.contiguous()
         bias_args = bias.data_ptr(), _lib.DTYPES[bias.dtype]
-    out = x_scale.new_empty((*shape, outer), dtype=out_dtype)
     workspace, size = None, 0
+    if whole:
+        (rows, x_stride), x_scale, code = aligned_bytes(x), x_scale.contiguous(), _lib.S8
+    else:
+        (rows, x_stride), code = rows_of(x), _floating(x, "x")
+    if not whole or _lib.status_checks():
+        size = _lib.workspace_bytes("pisa_int8_linear_workspace_bytes", device, count, inner, outer, code)
+        workspace = weight.new_empty(size)
+    out = weight_scale.new_empty((*shape, outer), dtype=out_dtype)
+    _lib.launch(_lib.lib().pisa_int8_linear, device, rows.data_ptr(), x_stride, code, x_scale.data_ptr() if whole else None,
+                weight.data_ptr(), w_stride, weight_scale.data_ptr(), *bias_args, _lib.DTYPES[out_dtype], count, inner, outer,
+                out.data_ptr(), None if workspace is None else workspace.data_ptr(), size)
     if _lib.status_checks():
-        size = _lib.workspace_bytes("pisa_int8_linear_workspace_bytes", device, count, inner, outer)
-        workspace = torch.empty(size, dtype=torch.uint8, device=x.device)
-    _lib.launch(_lib.lib().pisa_int8_linear, device, rows.data_ptr(), x_stride, x_scale.data_ptr(), weight.data_ptr(), w_stride,
-                weight_scale.data_ptr(), *bias_args, _lib.DTYPES[out_dtype], count, inner, outer, out.data_ptr(),
-                None if workspace is None else workspace.data_ptr(), size)
-    if workspace is not None:
         _lib.check_workspace(workspace, x.device)
     return out
 

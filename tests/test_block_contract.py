@@ -94,12 +94,14 @@ def test_entry_checks_run_on_the_host():
     refused(lib.pisa_quantize_int8(256, 64, _lib.BF16, 4, 64, 0, 8, 64, 256, None), "16 bytes")
     refused(lib.pisa_restore_int8(256, 64, None, _lib.BF16, 4, 64, 256, None), "required")
 
-    def linear(T=4, K=64, O=8, x=256, x_st=64, w_st=64, out=_lib.BF16, size=0, workspace=None, bias=None, bias_dtype=0):
-        return lib.pisa_int8_linear(x, x_st, 256, 256, w_st, 256, bias, bias_dtype, out, T, K, O, 256, workspace, size, None)
+    def linear(T=4, K=64, O=8, x=256, x_st=64, x_dtype=_lib.S8, w_st=64, out=_lib.BF16, size=0, workspace=None, bias=None,
+               bias_dtype=0):
+        return lib.pisa_int8_linear(x, x_st, x_dtype, 256, 256, w_st, 256, bias, bias_dtype, out, T, K, O, 256, workspace, size, None)
 
     for kw, word in (({"T": 0}, "nonempty"), ({"K": 1 << 17}, "32 bits"), ({"O": 0}, "nonempty"), ({"x": 8}, "16 bytes"),
                      ({"x_st": 72}, "16 bytes"), ({"w_st": 48}, "overlap"), ({"out": 9}, "support"), ({"T": 1 << 31}, "too large"),
-                     ({"workspace": 256, "size": 16}, "workspace"), ({"bias": 256, "bias_dtype": _lib.F16}, "bias")):
+                     ({"workspace": 256, "size": 16}, "workspace"), ({"x_dtype": _lib.BF16}, "workspace"), ({"x_dtype": 4}, "support"),
+                     ({"x_dtype": _lib.BF16, "workspace": 8, "size": 4096}, "16 bytes"), ({"bias": 256, "bias_dtype": _lib.F16}, "bias")):
         refused(linear(**kw), word)
 
 
@@ -111,5 +113,6 @@ def test_workspace_sizes_are_pure_host_functions():
     assert lib.pisa_residual_norm_bwd_workspace_bytes(12, 64, 4) % (3 * 3 * 64 * 4) == 0
     assert lib.pisa_residual_norm_bwd_workspace_bytes(12, 64, 5) == -1
     assert lib.pisa_residual_norm_bwd_workspace_bytes(0, 64, 0) == -1
-    assert lib.pisa_int8_linear_workspace_bytes(4, 64, 8) >= 256
-    assert lib.pisa_int8_linear_workspace_bytes(4, 0, 8) == -1
+    assert lib.pisa_int8_linear_workspace_bytes(4, 64, 8, _lib.S8) == 256
+    assert lib.pisa_int8_linear_workspace_bytes(4, 65, 8, _lib.BF16) == 512 + 4 * 80
+    assert lib.pisa_int8_linear_workspace_bytes(4, 0, 8, _lib.S8) == -1

@@ -134,15 +134,26 @@ def test_nothing_is_written_past_the_rows(cuda_device, out, tokens, inner, outer
     spare = 4096
     got = torch.full((tokens * outer + 2 * spare,), 7.0, dtype=out, device="cuda")
     lib, stream = _lib.lib(), torch.cuda.current_stream().cuda_stream
-    size = lib.pisa_int8_linear_workspace_bytes(tokens, inner, outer)
+    size = lib.pisa_int8_linear_workspace_bytes(tokens, inner, outer, _lib.S8)
     workspace = torch.full((size + 4096,), 85, dtype=torch.uint8, device="cuda")
-    _lib.check(lib.pisa_int8_linear(x.data_ptr(), step, xs.data_ptr(), w.data_ptr(), step, ws.data_ptr(), None, 0, _lib.DTYPES[out],
+    _lib.check(lib.pisa_int8_linear(x.data_ptr(), step, _lib.S8, xs.data_ptr(), w.data_ptr(), step, ws.data_ptr(), None, 0, _lib.DTYPES[out],
                                     tokens, inner, outer, got.data_ptr() + spare * got.element_size(), workspace.data_ptr(), size,
                                     stream))
     assert bool((got[:spare] == 7).all()) and bool((got[-spare:] == 7).all())
     assert bool((workspace[size:] == 85).all())
     _lib.check_workspace(workspace, x.device)
     R.check("out", got[spare:-spare].view(tokens, outer), *R.int8_linear(x[:, :inner], xs, w[:, :inner], ws, None, out))
+    # floating tokens, rounded in the workspace
+    f = torch.randn(tokens, inner, generator=gen, device="cuda").to(BF16)
+    size = lib.pisa_int8_linear_workspace_bytes(tokens, inner, outer, _lib.BF16)
+    workspace = torch.full((size + 4096,), 85, dtype=torch.uint8, device="cuda")
+    got.fill_(7.0)
+    _lib.check(lib.pisa_int8_linear(f.data_ptr(), inner, _lib.BF16, None, w.data_ptr(), step, ws.data_ptr(), None, 0,
+                                    _lib.DTYPES[out], tokens, inner, outer, got.data_ptr() + spare * got.element_size(),
+                                    workspace.data_ptr(), size, stream))
+    assert bool((got[:spare] == 7).all()) and bool((got[-spare:] == 7).all()) and bool((workspace[size:] == 85).all())
+    _lib.check_workspace(workspace, x.device)
+    R.check("out", got[spare:-spare].view(tokens, outer), *R.int8_linear(*R.quantized(f.float()), w[:, :inner], ws, None, out))
 
 
 def test_repeats_and_status(cuda_device):
@@ -154,6 +165,7 @@ def test_repeats_and_status(cuda_device):
     P.set_status_checks(True)
     try:
         assert torch.equal(P.int8_linear(x, w, ws, x_scale=xs), first)
+        assert torch.equal(P.int8_linear(x.float(), w, ws), P.int8_linear(x.float(), w, ws))
     finally:
         P.set_status_checks(False)
 
