@@ -52,6 +52,10 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
       :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(tc::smem_u32(mbar)) : "memory");
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" :: "l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
+
 // D[tmem] (+)= A[smem] * B[smem]^T of signed bytes, 32 of K.
 __device__ __forceinline__ void mma_i8(uint32_t d, uint32_t a_low, uint32_t b_low, uint32_t idesc, bool accumulate) {
   asm volatile(
@@ -144,7 +148,15 @@ __global__ void __launch_bounds__(kThreads) int8_linear_kernel(const __grid_cons
   __shared__ __align__(16) float s_xs[8][BN < 32 ? 32 : BN];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = (tc::smem_u32(raw) + 1023u) & ~1023u;
+  auto load = [&](int st, int k, uint32_t tt, uint32_t to) {
+    const uint32_t at = base + st * L::STAGE;
+    tc::mbar_arrive_expect_tx(&full[st], uint32_t(L::A_BYTES + a.bn * kStepBytes));
+    tma_load_2d(at, &a.tm_w, k * kStepBytes, int(to) * kM, &full[st]);
+    tma_load_2d(at + L::A_BYTES, &a.tm_x, k * kStepBytes, int(tt) * a.bn, &full[st]);
+  };
   if (warp == 0 && lane == 0) {
+    prefetch_map(&a.tm_w);
+    prefetch_map(&a.tm_x);
     for (int i = 0; i < L::STAGES; ++i) {
       tc::mbar_init(&full[i], 1);
       tc::mbar_init(&empty[i], 1);
@@ -156,26 +168,25 @@ __global__ void __launch_bounds__(kThreads) int8_linear_kernel(const __grid_cons
     tc::mbar_init(&drained, 1);
     tc::fence_barrier_init();
     wait.init(a.tries);
+    // the first stages are on their way while the others get ready (the first tile of a CTA always exists)
+    const uint32_t tt = blockIdx.x / a.tiles_o, to = blockIdx.x - tt * a.tiles_o;
+    for (int k = 0; k < min(L::STAGES, a.steps); ++k) load(k, k, tt, to);
   }
   if (warp == 1) tc::tmem_alloc(&slot, 2 * L::COLS);
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = slot;
-  const uint32_t stage_bytes = uint32_t(L::A_BYTES + a.bn * kStepBytes);
   bool ok = true;
   if (warp == 0) {
     if (lane == 0) {
-      int st = 0, loads = 0;
-      uint32_t phase = 1;
-      for (uint32_t tile = blockIdx.x; tile < a.tiles && ok; tile += gridDim.x) {
+      int loads = min(L::STAGES, a.steps), st = loads % L::STAGES, k = loads;
+      uint32_t phase = loads == L::STAGES ? 0 : 1;
+      for (uint32_t tile = blockIdx.x; tile < a.tiles && ok; tile += gridDim.x, k = 0) {
         const uint32_t tt = tile / a.tiles_o, to = tile - tt * a.tiles_o;
-        for (int k = 0; k < a.steps; ++k) {
+        for (; k < a.steps; ++k) {
           if (!(ok = wait_phase(&empty[st], int(phase), &wait))) break;
-          const uint32_t at = base + st * L::STAGE;
-          tc::mbar_arrive_expect_tx(&full[st], stage_bytes);
-          tma_load_2d(at, &a.tm_w, k * kStepBytes, int(to) * kM, &full[st]);
-          tma_load_2d(at + L::A_BYTES, &a.tm_x, k * kStepBytes, int(tt) * a.bn, &full[st]);
+          load(st, k, tt, to);
           ++loads;
           if (++st == L::STAGES) {
             st = 0;
@@ -310,6 +321,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads) int8_linea
   const uint32_t base = (tc::smem_u32(raw) + 1023u) & ~1023u;
   const uint32_t rank = blockIdx.x & 1, pairs = gridDim.x >> 1, first = blockIdx.x >> 1;
   if (warp == 0 && lane == 0) {
+    prefetch_map(&a.tm_w);
+    prefetch_map(&a.tm_x);
     for (int i = 0; i < L::STAGES; ++i) {
       tc::mbar_init(&full[i], 1);
       tc::mbar_init(&empty[i], 1);
@@ -507,7 +520,16 @@ __global__ void __launch_bounds__(kThreads) int8_linear_split_kernel(const __gri
   const uint32_t tile = blockIdx.x / a.split, rank = blockIdx.x - tile * a.split;   // rank: clusters are runs of a.split CTAs
   const uint32_t tt = tile / a.tiles_o, to = tile - tt * a.tiles_o;
   const int k0 = int(int64_t(a.steps) * rank / a.split), k1 = int(int64_t(a.steps) * (rank + 1) / a.split);
+  auto load = [&](int st, int k) {
+    const uint32_t at = base + st * L::STAGE;
+    tc::mbar_arrive_expect_tx(&full[st], uint32_t(L::A_BYTES + a.bn * kStepBytes));
+    tma_load_2d(at, &a.tm_w, k * kStepBytes, int(to) * kM, &full[st]);
+    tma_load_2d(at + L::A_BYTES, &a.tm_x, k * kStepBytes, int(tt) * a.bn, &full[st]);
+  };
+  const int early = min(L::STAGES, k1 - k0);
   if (warp == 0 && lane == 0) {
+    prefetch_map(&a.tm_w);
+    prefetch_map(&a.tm_x);
     for (int i = 0; i < L::STAGES; ++i) {
       tc::mbar_init(&full[i], 1);
       tc::mbar_init(&empty[i], 1);
@@ -516,24 +538,21 @@ __global__ void __launch_bounds__(kThreads) int8_linear_split_kernel(const __gri
     tc::mbar_init(&drained, 1);
     tc::fence_barrier_init();
     wait.init(a.tries);
+    for (int i = 0; i < early; ++i) load(i, k0 + i);   // on their way while the others get ready
   }
   if (warp == 1) tc::tmem_alloc(&slot, L::COLS);
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = slot;
-  const uint32_t stage_bytes = uint32_t(L::A_BYTES + a.bn * kStepBytes);
   bool ok = true;
   if (warp == 0) {
     if (lane == 0) {
-      int st = 0, loads = 0;
-      uint32_t phase = 1;
-      for (int k = k0; k < k1; ++k) {
+      int loads = early, st = loads % L::STAGES;
+      uint32_t phase = loads == L::STAGES ? 0 : 1;
+      for (int k = k0 + early; k < k1; ++k) {
         if (!(ok = wait_phase(&empty[st], int(phase), &wait))) break;
-        const uint32_t at = base + st * L::STAGE;
-        tc::mbar_arrive_expect_tx(&full[st], stage_bytes);
-        tma_load_2d(at, &a.tm_w, k * kStepBytes, int(to) * kM, &full[st]);
-        tma_load_2d(at + L::A_BYTES, &a.tm_x, k * kStepBytes, int(tt) * a.bn, &full[st]);
+        load(st, k);
         ++loads;
         if (++st == L::STAGES) {
           st = 0;
