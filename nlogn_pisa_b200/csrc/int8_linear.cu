@@ -709,7 +709,7 @@ int launch_pairs(LinArgs a, const Operands& m, cudaStream_t s) {
   const int64_t tiles = int64_t(a.tiles_o) * ((a.T + a.bn - 1) / a.bn);
   if (tiles >= (int64_t(1) << 31)) return fail(PISA_ERR_UNSUPPORTED, "tensor too large");
   a.tiles = uint32_t(tiles);
-  int8_linear_pair_kernel<T><<<unsigned(2 * min64(tiles, sm_count() / 2)), kThreads, PairTile::SMEM, s>>>(a);
+  int8_linear_pair_kernel<T><<<unsigned(2 * min64(tiles, (sm_count() + 1) / 2)), kThreads, PairTile::SMEM, s>>>(a);
   PISA_CHECK_LAUNCH();
   return PISA_OK;
 }
@@ -756,7 +756,7 @@ Shape choose(int64_t T, int64_t O, int64_t steps) {
     }
   }
   const int bn = (tile_tokens(T, 256) + 31) / 32 * 32;
-  consider(256, 0, (O + 2 * kM - 1) / (2 * kM) * ((T + bn - 1) / bn), sms / 2, 0.20 + 0.0005 * bn, 1.0 + 0.011 * bn, 4.5);
+  consider(256, 0, (O + 2 * kM - 1) / (2 * kM) * ((T + bn - 1) / bn), (sms + 1) / 2, 0.20 + 0.0005 * bn, 1.0 + 0.011 * bn, 4.5);
   return best;
 }
 

@@ -116,23 +116,28 @@ class SwigluFfnFunction(torch.autograd.Function):
     """The layer's products are torch's; its backward starts from bytes."""
 
     @staticmethod
+    @torch.amp.custom_fwd(device_type="cuda")
     def forward(ctx, x, w_gate, w_up, w_down, b_gate, b_up, b_down):
         out, kept = _forward(F.linear(x, w_gate, b_gate), F.linear(x, w_up, b_up), True)
         ctx.dtype = x.dtype
-        ctx.biases = tuple(b is not None for b in (b_gate, b_up, b_down))
         ctx.save_for_backward(*checkpoint_int8(x), kept, w_gate, w_up, w_down)
         return F.linear(out, w_down, b_down)
 
     @staticmethod
+    @torch.amp.custom_bwd(device_type="cuda")
     @once_differentiable
     def backward(ctx, dy):
         x_values, x_scale, kept, w_gate, w_up, w_down = ctx.saved_tensors
-        dgate, dup, out = _backward(dy @ w_down, None, None, kept, True)
-        rows = [t.reshape(-1, t.shape[-1]) for t in (dgate, dup, dy, out)]
-        x = restore_int8(x_values, x_scale, ctx.dtype).view(-1, x_values.shape[-1])
-        weights = rows[0].T @ x, rows[1].T @ x, rows[2].T @ rows[3]
-        biases = (t.sum(0) if has else None for t, has in zip(rows, ctx.biases))
-        return dgate @ w_gate + dup @ w_up, *weights, *biases
+        need = ctx.needs_input_grad
+        dgate, dup, out = _backward(dy @ w_down, None, None, kept, need[3])
+        dx = dgate @ w_gate + dup @ w_up if need[0] else None
+        dgate, dup, dy = (t.reshape(-1, t.shape[-1]) for t in (dgate, dup, dy))
+        weights = [None, None, dy.T @ out.view(-1, out.shape[-1]) if need[3] else None]
+        if need[1] or need[2]:
+            x = restore_int8(x_values, x_scale, ctx.dtype).view(-1, x_values.shape[-1])
+            weights[:2] = (t.T @ x if needed else None for t, needed in ((dgate, need[1]), (dup, need[2])))
+        biases = (t.sum(0) if needed else None for t, needed in zip((dgate, dup, dy), need[4:]))
+        return dx, *weights, *biases
 
 
 def swiglu_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None):
@@ -142,7 +147,7 @@ def swiglu_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None):
     forward and backward x and the two inner products live as bytes with a scale
     per 128 elements and the gated product is rebuilt from them, about a third of
     what 16-bit copies take.  The forward's result does not depend on it.
-    Reverse mode only.
+    Under autocast the products run in its type.  Reverse mode only.
     """
     tensors = [t for t in (x, w_gate, w_up, w_down, b_gate, b_up, b_down) if t is not None]
     if any(t.dtype != x.dtype for t in tensors) or not x.is_floating_point():
