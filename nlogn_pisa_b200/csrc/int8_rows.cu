@@ -43,8 +43,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) row_kernel(const __grid
   for (int j = 0; j < NV; ++j) {
     float f[8];
     widen8<T>(x[j], f);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) top = max_nan(top, fabsf(f[e]));
+    top = max_nan(top, largest8<T>(x[j], f));
   }
   top = team_reduce<TPR, true>(top, red, set);
   const Scale8 s(top);
@@ -125,10 +124,9 @@ __global__ void __launch_bounds__(kThreads) group_kernel(const __grid_constant__
     widen8_s8(load_piece_s8<T, 16, A>(qr, t, width), a.scale[at], f);
     store_piece<T, 16, A>(static_cast<T*>(a.out) + row * a.D + first, 0, t, width, f);
   } else {
-    widen8<T>(load_piece<T, 16, A>(static_cast<const T*>(a.x) + row * a.x_st + first, 0, t, width), f);
-    float top = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) top = max_nan(top, fabsf(f[e]));
+    const Raw8<T> x = load_piece<T, 16, A>(static_cast<const T*>(a.x) + row * a.x_st + first, 0, t, width);
+    widen8<T>(x, f);
+    float top = largest8<T>(x, f);
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(kFull, top, o));
     const Scale8 s(top);

@@ -246,30 +246,46 @@ struct Scale8 {
   }
 };
 
-// Four rounded values as bytes.  Adding 1.5 * 2^23 leaves the nearest integer
-// (ties to even, as the sum's rounding) in the low bits of the sum.
-__device__ __forceinline__ uint32_t pack_s8(float a, float b, float c, float d, float inv) {
-  const float magic = 12582912.f;
-  const uint32_t x = __float_as_uint(__fadd_rn(__fmul_rn(a, inv), magic)), y = __float_as_uint(__fadd_rn(__fmul_rn(b, inv), magic));
-  const uint32_t z = __float_as_uint(__fadd_rn(__fmul_rn(c, inv), magic)), w = __float_as_uint(__fadd_rn(__fmul_rn(d, inv), magic));
-  return __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
+// Eight rounded values as bytes.  Adding 1.5 * 2^23 leaves the nearest integer
+// (ties to even, as the sum's rounding) in the low bits of the sum.  The product
+// is rounded before: as pairs the two steps became one multiply-add, whose single
+// rounding differs next to ties.
+__device__ __forceinline__ uint2 pack8_s8(const float (&f)[8], float inv) {
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(__fadd_rn(__fmul_rn(f[i], inv), 12582912.f));
+  return make_uint2(__byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410),
+                    __byte_perm(__byte_perm(w[4], w[5], 0x0040), __byte_perm(w[6], w[7], 0x0040), 0x5410));
 }
 
-// Four bytes as floats.  A byte b in the low bits of 0x4B000000 | (b ^ 128) is
-// the float 2^23 + 128 + b.
-__device__ __forceinline__ void unpack_s8(uint32_t q, float (&f)[4]) {
-  const uint32_t u = q ^ 0x80808080u;
-  const float off = 8388736.f;
-  f[0] = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440)) - off;
-  f[1] = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7441)) - off;
-  f[2] = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7442)) - off;
-  f[3] = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7443)) - off;
+// Largest magnitude of a thread's 8 values, NaN if any is: 16-bit values in
+// their packed form.
+template <typename T>
+__device__ __forceinline__ float largest8(const Raw8<T>& r, const float (&f)[8]) {
+  if constexpr (std::is_same<T, float>::value) {
+    float top = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max_nan(top, fabsf(f[e]));
+    return top;
+  } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const uint32_t w[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
+    __nv_bfloat162 m = __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[0]));
+#pragma unroll
+    for (int i = 1; i < 4; ++i) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[i])));
+    return max_nan(__low2float(m), __high2float(m));
+  } else {
+    const uint32_t w[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
+    __half2 m = __habs2(*reinterpret_cast<const __half2*>(&w[0]));
+#pragma unroll
+    for (int i = 1; i < 4; ++i) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __half2*>(&w[i])));
+    return max_nan(__low2float(m), __high2float(m));
+  }
 }
 
 template <typename T, int TPR, bool A>
 __device__ __forceinline__ void store_piece_s8(int8_t* row, int j, int t, int D, const float (&f)[8], bool fine, float inv) {
-  uint32_t lo = pack_s8(f[0], f[1], f[2], f[3], inv), hi = pack_s8(f[4], f[5], f[6], f[7], inv);
-  if (!fine) lo = hi = 0;
+  const uint2 bytes = pack8_s8(f, inv);
+  const uint32_t lo = fine ? bytes.x : 0, hi = fine ? bytes.y : 0;
   if constexpr (A) {
     const int c = column<T, TPR, A>(j, 0, t), c4 = column<T, TPR, A>(j, 4, t);
     if constexpr (sizeof(T) == 2) {
@@ -310,14 +326,14 @@ __device__ __forceinline__ uint2 load_piece_s8(const int8_t* row, int t, int D) 
   }
   return r;
 }
+// A byte b in the low bits of 0x4B000000 | (b ^ 128) is the float 2^23 + 128 + b.
 __device__ __forceinline__ void widen8_s8(const uint2& q, float scale, float (&f)[8]) {
-  float lo[4], hi[4];
-  unpack_s8(q.x, lo);
-  unpack_s8(q.y, hi);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    f[e] = lo[e] * scale;
-    f[4 + e] = hi[e] * scale;
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t u = (i < 2 ? q.x : q.y) ^ 0x80808080u;
+    const float2 x = make_float2(__uint_as_float(__byte_perm(u, 0x4B000000u, i % 2 ? 0x7442 : 0x7440)),
+                                 __uint_as_float(__byte_perm(u, 0x4B000000u, i % 2 ? 0x7443 : 0x7441)));
+    set_pair(f, i, pair_mul(pair_add(x, both(-8388736.f)), both(scale)));
   }
 }
 

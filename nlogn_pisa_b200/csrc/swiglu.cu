@@ -51,11 +51,22 @@ __device__ __forceinline__ float fast_rcp(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+__device__ __forceinline__ float fast_ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 
+// s(x) of a pair.
 template <typename T>
-__device__ __forceinline__ float sigmoid(float x) {
-  if constexpr (std::is_same<T, float>::value) return 1.f / (1.f + expf(-x));
-  else return fast_rcp(1.f + __expf(-x));
+__device__ __forceinline__ float2 sigmoid2(float2 x) {
+  if constexpr (std::is_same<T, float>::value) {
+    return make_float2(1.f / (1.f + expf(-x.x)), 1.f / (1.f + expf(-x.y)));
+  } else {
+    constexpr float kLog2e = 1.4426950408889634f;
+    const float2 y = pair_mul(x, both(-kLog2e)), z = pair_add(make_float2(fast_ex2(y.x), fast_ex2(y.y)), both(1.f));
+    return make_float2(fast_rcp(z.x), fast_rcp(z.y));
+  }
 }
 
 // Maximum over the sixteen threads of a group, NaN if any is.
@@ -63,13 +74,6 @@ __device__ __forceinline__ float group_max(float v) {
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(kFull, v, o));
   return v;
-}
-
-__device__ __forceinline__ float largest8(const float (&f)[8]) {
-  float top = 0.f;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) top = max_nan(top, fabsf(f[e]));
-  return top;
 }
 
 constexpr int kGluThreads = 256, kGluTeams = kGluThreads / 16;
@@ -108,10 +112,13 @@ __global__ void __launch_bounds__(kGluThreads) glu_fwd_kernel(const __grid_const
     widen8<T>(gr[i], g);
     widen8<T>(ur[i], u);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = g[e] * sigmoid<T>(g[e]) * u[e];
+    for (int k = 0; k < 4; ++k) {
+      const float2 x = pair_at(g, k);
+      set_pair(o, k, pair_mul(pair_mul(x, sigmoid2<T>(x)), pair_at(u, k)));
+    }
     store_piece<T, 16, A>(static_cast<T*>(a.out) + n.row * a.D + n.first, 0, t, n.width, o);
     if constexpr (KEEP) {
-      const float top_g = group_max(largest8(g)), top_u = group_max(largest8(u));
+      const float top_g = group_max(largest8<T>(gr[i], g)), top_u = group_max(largest8<T>(ur[i], u));
       // Scale8 of both: its four quotients are four lanes' (a quotient costs more than a shuffle)
       const float m = fmaxf(t & 1 ? top_u : top_g, kTiny), r = __fdiv_rn(t & 2 ? m : 127.f, t & 2 ? 127.f : m);
       const int team = threadIdx.x & 16;
@@ -156,11 +163,13 @@ __global__ void __launch_bounds__(kGluThreads) glu_bwd_kernel(const __grid_const
     }
     widen8<T>(dr[i], d);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float s = sigmoid<T>(g[e]), y = g[e] * s;
-      if (a.out) o[e] = y * u[e];
-      u[e] = d[e] * u[e] * s * fmaf(g[e], 1.f - s, 1.f);
-      g[e] = d[e] * y;
+    for (int k = 0; k < 4; ++k) {
+      const float2 x = pair_at(g, k), s = sigmoid2<T>(x), y = pair_mul(x, s), v = pair_at(u, k), e = pair_at(d, k);
+      if (a.out) set_pair(o, k, pair_mul(y, v));
+      // s (1 + x (1 - s)) with 1 - s as 1 + (-1) s
+      const float2 slope = pair_mul(s, pair_fma(x, pair_fma(s, both(-1.f), both(1.f)), both(1.f)));
+      set_pair(u, k, pair_mul(pair_mul(e, v), slope));
+      set_pair(g, k, pair_mul(e, y));
     }
     store_piece<T, 16, A>(static_cast<T*>(a.dg) + n.row * a.D + n.first, 0, t, n.width, u);
     store_piece<T, 16, A>(static_cast<T*>(a.du) + n.row * a.D + n.first, 0, t, n.width, g);
@@ -190,8 +199,12 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) glu_row_kernel(const __
     widen8<T>(g[j], f);
     widen8<T>(u[j], o[j]);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[j][e] *= f[e] * sigmoid<T>(f[e]);
-    top = max_nan(top, largest8(o[j]));
+    for (int k = 0; k < 4; ++k) {
+      const float2 x = pair_at(f, k);
+      set_pair(o[j], k, pair_mul(pair_mul(x, sigmoid2<T>(x)), pair_at(o[j], k)));
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max_nan(top, fabsf(o[j][e]));
   }
   top = team_reduce<TPR, true>(top, red, set);
   const Scale8 s(top);
