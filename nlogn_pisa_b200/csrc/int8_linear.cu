@@ -10,6 +10,12 @@
 // Warp 0 loads, warp 1 issues the MMAs, warps 2 to 9 scale and store; two
 // accumulators in TMEM let a tile's stores run under the next tile's products.
 //
+// Many tokens are bound by the tensor cores (and, back to back, by power), few by
+// HBM and the start of a launch: 16384 x 4096 x 11264 takes 437 to 449 us (3.4
+// PTOP/s, tensor pipe 86 % busy on a smaller case), 64 tokens over 4096 x 16384
+// 14.7 us (4.7 TB/s), one token over 1024 x 5632 5.4 us.  Tiles of short K are bound
+// by their stores: 30000 x 512 x 2000 49 us (65 with a test per store).
+//
 // Where the tiles are fewer than the SMs, a cluster of CTAs shares each: every
 // CTA sums a range of K, leaves its int32 sums in shared memory, and takes a
 // share of the tile's tokens, for which it adds all ranges' sums (integers: in
