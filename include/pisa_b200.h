@@ -551,8 +551,9 @@ PISA_API int pisa_restore_int8(const int8_t *q, int64_t q_st, const float *scale
  *   (bytes past a row's K elements are not used); K below 131072.
  * bias: [O] in FP32 or out_dtype, or NULL.  out: contiguous [T, O].
  * workspace: pisa_int8_linear_workspace_bytes(...) bytes on 16 bytes (NULL is
- *   allowed with PISA_S8) whose first 4 receive the device status word; the
- *   outputs of a call with an expired wait are undefined.
+ *   allowed where that is 256: with PISA_S8, and for a few floating tokens) whose
+ *   first 4 receive the device status word; the outputs of a call with an expired
+ *   wait are undefined.
  */
 PISA_API int pisa_int8_linear(const void *x, int64_t x_st, int x_dtype, const float *x_scale, const int8_t *weight,
                               int64_t weight_st, const float *weight_scale, const void *bias, int bias_dtype,

@@ -16,6 +16,10 @@
 // 14.7 us (4.7 TB/s), one token over 1024 x 5632 5.4 us.  Tiles of short K are bound
 // by their stores: 30000 x 512 x 2000 49 us (65 with a test per store).
 //
+// A few floating tokens are rounded by the storing warps of every CTA, which
+// keep their bytes in shared memory for all of its tiles, while the first weights
+// arrive: one launch instead of two.
+//
 // Where the tiles are fewer than the SMs, a cluster of CTAs shares each: every
 // CTA sums a range of K, leaves its int32 sums in shared memory, and takes a
 // share of the tile's tokens, for which it adds all ranges' sums (integers: in
@@ -23,6 +27,7 @@
 #include <cudaTypedefs.h>
 
 #include "dense_tc.cuh"
+#include "rows.cuh"
 
 namespace pisa {
 
@@ -50,6 +55,10 @@ struct LinArgs {
   uint32_t tries;
   void* out;
   int* status;
+  // floating tokens that the kernel rounds itself
+  const void* x;
+  int64_t x_st;
+  int x_dtype, x_wide, K;   // x_wide: rows start on 16 bytes and K is a multiple of 8
 };
 
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint64_t* mbar) {
@@ -75,13 +84,77 @@ __device__ __forceinline__ uint32_t idesc_i8(int M, int N) {
   return (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(N >> 3) << 17) | (uint32_t(M >> 4) << 24);
 }
 
-template <int BN>
+constexpr int kRoundTokens = 16, kRoundSteps = 48;   // tokens that a CTA rounds itself, steps of K that it holds of them
+
+// ROUND: stages hold weights only, the tokens' bytes lie behind them.
+template <int BN, bool ROUND = false>
 struct Tile {
-  static constexpr int A_BYTES = kM * kStepBytes, B_BYTES = BN * kStepBytes, STAGE = A_BYTES + B_BYTES;
-  static constexpr int STAGES = (kSmem - 1024) / STAGE < 10 ? (kSmem - 1024) / STAGE : 10;
-  static constexpr int SMEM = STAGES * STAGE + 1024;
+  static constexpr int A_BYTES = kM * kStepBytes, B_BYTES = BN * kStepBytes, STAGE = A_BYTES + (ROUND ? 0 : B_BYTES);
+  static constexpr int STAGES = ROUND ? 7 : (kSmem - 1024) / STAGE < 10 ? (kSmem - 1024) / STAGE : 10;
+  static constexpr int SMEM = STAGES * STAGE + (ROUND ? kRoundSteps * B_BYTES : 0) + 1024;
   static constexpr int COLS = BN < 32 ? 32 : BN;             // TMEM columns of an accumulator
 };
+
+// Elements c .. c + 7 of a token, zeros past its end.
+template <typename X>
+__device__ __forceinline__ void token_piece(const LinArgs& a, const X* row, int c, float (&f)[8]) {
+  if (a.x_wide && c < a.K) {
+    Raw8<X> r;
+#pragma unroll
+    for (int i = 0; i < int(sizeof(X) / 2); ++i) r.v[i] = __ldg(reinterpret_cast<const uint4*>(row + c) + i);
+    widen8<X>(r, f);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = c + e < a.K ? to_f32<X>(row[c + e]) : 0.f;
+  }
+}
+
+// The storing warps (256 threads, as many for each token) round the tokens as
+// pisa_quantize_int8 does; the bytes of steps k0 .. k1 - 1 go to 128-byte-swizzled
+// tiles of 16 rows from `at` on, scales to `scale`.  Rows past the last token are
+// not written: no one stores their products.
+template <typename X>
+__device__ __forceinline__ void round_tokens(const LinArgs& a, uint32_t at, int k0, int k1, float* scale, float* red) {
+  int lg = 0;
+  while ((1 << lg) < a.T) ++lg;
+  const int id = int(threadIdx.x) - 64, each = 256 >> lg, row = id / each, t = id % each;
+  const X* x = static_cast<const X*>(a.x) + int64_t(min(row, a.T - 1)) * a.x_st;
+  float top = 0.f;
+#pragma unroll 4
+  for (int p = t; p < a.steps * 16; p += each) {
+    float f[8];
+    token_piece<X>(a, x, p * 8, f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = larger(top, fabsf(f[e]));
+  }
+  for (int o = min(each, 32) / 2; o > 0; o >>= 1) top = larger(top, __shfl_xor_sync(kFull, top, o));
+  if (each > 32) {
+    if ((id & 31) == 0) red[id >> 5] = top;
+    tc::named_sync(1, 256);
+    for (int w = row * each >> 5; w < (row + 1) * each >> 5; ++w) top = larger(top, red[w]);
+  }
+  const Scale8 s(top);
+  if (t == 0) scale[row] = s.scale;
+  if (row < a.T) {
+#pragma unroll 4
+    for (int p = k0 * 16 + t; p < k1 * 16; p += each) {
+      float f[8];
+      token_piece<X>(a, x, p * 8, f);
+      uint2 q = pack8_s8(f, s.inv);
+      if (!(top < INFINITY)) q = make_uint2(0, 0);
+      const uint32_t to = at + uint32_t((p >> 4) - k0) * (kRoundTokens * kStepBytes) + tc::swizzle128(row, (p & 15) >> 1) + (p & 1) * 8;
+      asm volatile("st.shared.v2.u32 [%0], {%1,%2};" :: "r"(to), "r"(q.x), "r"(q.y) : "memory");
+    }
+  }
+  tc::fence_async_smem();
+}
+__device__ __forceinline__ void round_tokens(const LinArgs& a, uint32_t at, int k0, int k1, float* scale, float* red, uint64_t* ready) {
+  if (a.x_dtype == PISA_F32) round_tokens<float>(a, at, k0, k1, scale, red);
+  else if (a.x_dtype == PISA_BF16) round_tokens<__nv_bfloat16>(a, at, k0, k1, scale, red);
+  else round_tokens<__half>(a, at, k0, k1, scale, red);
+  tc::named_sync(1, 256);
+  if ((threadIdx.x & 31) == 0) tc::mbar_arrive(ready);
+}
 
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -144,25 +217,26 @@ __device__ __forceinline__ void store_tile(const LinArgs& a, uint32_t tmem, cons
   store_columns<T>(v, static_cast<T*>(a.out), a.O, t, t1, o, a.O, pairs, whole);
 }
 
-template <typename T, int BN>
+template <typename T, int BN, bool ROUND>
 __global__ void __launch_bounds__(kThreads) int8_linear_kernel(const __grid_constant__ LinArgs a) {
-  using L = Tile<BN>;
+  using L = Tile<BN, ROUND>;
   extern __shared__ __align__(16) uint8_t raw[];
-  __shared__ uint64_t full[L::STAGES], empty[L::STAGES], acc_full[2], acc_empty[2], drained;
+  __shared__ uint64_t full[L::STAGES], empty[L::STAGES], acc_full[2], acc_empty[2], drained, x_ready;
   __shared__ uint32_t slot;
   __shared__ WaitFlag wait;
   __shared__ __align__(16) float s_xs[8][BN < 32 ? 32 : BN];
+  __shared__ float s_scale[kRoundTokens], s_red[8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = (tc::smem_u32(raw) + 1023u) & ~1023u;
   auto load = [&](int st, int k, uint32_t tt, uint32_t to) {
     const uint32_t at = base + st * L::STAGE;
-    tc::mbar_arrive_expect_tx(&full[st], uint32_t(L::A_BYTES + a.bn * kStepBytes));
+    tc::mbar_arrive_expect_tx(&full[st], uint32_t(L::A_BYTES + (ROUND ? 0 : a.bn * kStepBytes)));
     tma_load_2d(at, &a.tm_w, k * kStepBytes, int(to) * kM, &full[st]);
-    tma_load_2d(at + L::A_BYTES, &a.tm_x, k * kStepBytes, int(tt) * a.bn, &full[st]);
+    if (!ROUND) tma_load_2d(at + L::A_BYTES, &a.tm_x, k * kStepBytes, int(tt) * a.bn, &full[st]);
   };
   if (warp == 0 && lane == 0) {
     prefetch_map(&a.tm_w);
-    prefetch_map(&a.tm_x);
+    if (!ROUND) prefetch_map(&a.tm_x);
     for (int i = 0; i < L::STAGES; ++i) {
       tc::mbar_init(&full[i], 1);
       tc::mbar_init(&empty[i], 1);
@@ -172,6 +246,7 @@ __global__ void __launch_bounds__(kThreads) int8_linear_kernel(const __grid_cons
       tc::mbar_init(&acc_empty[i], 8);
     }
     tc::mbar_init(&drained, 1);
+    tc::mbar_init(&x_ready, 8);
     tc::fence_barrier_init();
     wait.init(a.tries);
     // the first stages are on their way while the others get ready (the first tile of a CTA always exists)
@@ -182,7 +257,7 @@ __global__ void __launch_bounds__(kThreads) int8_linear_kernel(const __grid_cons
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  const uint32_t tmem = slot;
+  const uint32_t tmem = slot, x_at = base + L::STAGES * L::STAGE;
   bool ok = true;
   if (warp == 0) {
     if (lane == 0) {
@@ -211,6 +286,7 @@ __global__ void __launch_bounds__(kThreads) int8_linear_kernel(const __grid_cons
     const uint32_t idesc = idesc_i8(kM, a.bn);
     int st = 0, n = 0;
     uint32_t phase = 0;
+    if (ROUND) ok = wait_phase(&x_ready, 0, &wait);
     for (uint32_t tile = blockIdx.x; tile < a.tiles && ok; tile += gridDim.x, ++n) {
       const int buf = n & 1;
       if (n >= 2) ok = wait_phase(&acc_empty[buf], (n >> 1) - 1, &wait);
@@ -225,7 +301,7 @@ __global__ void __launch_bounds__(kThreads) int8_linear_kernel(const __grid_cons
         }
         tc::fence_after_sync();
         if (leader) {
-          const uint32_t al = desc_low(base + st * L::STAGE, 16), bl = desc_low(base + st * L::STAGE + L::A_BYTES, 16);
+          const uint32_t al = desc_low(base + st * L::STAGE, 16), bl = desc_low(ROUND ? x_at + k * L::B_BYTES : base + st * L::STAGE + L::A_BYTES, 16);
 #pragma unroll
           for (int i = 0; i < 4; ++i) mma_i8(d, al + 2 * i, bl + 2 * i, idesc, k > 0 || i > 0);
           tc::mma_commit(&empty[st]);
@@ -249,13 +325,14 @@ __global__ void __launch_bounds__(kThreads) int8_linear_kernel(const __grid_cons
     const uint32_t lanes = uint32_t(quarter * 32) << 16;
     float* xs = s_xs[warp - 2];
     const bool pairs = (a.O & 1) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 3u) == 0;
+    if (ROUND) round_tokens(a, x_at, 0, a.steps, s_scale, s_red, &x_ready);
     int n = 0;
     for (uint32_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, ++n) {
       const int buf = n & 1;
       const uint32_t tt = tile / a.tiles_o, to = tile - tt * a.tiles_o;
       const int t0 = int(tt) * a.bn, t1 = min(a.T, t0 + a.bn), o = int(to) * kM + quarter * 32 + lane;
       __syncwarp();
-      for (int i = half * 32 + lane; i < a.bn; i += 64) xs[i] = t0 + i < a.T ? a.x_scale[t0 + i] : 0.f;
+      for (int i = half * 32 + lane; i < a.bn; i += 64) xs[i] = t0 + i < a.T ? (ROUND ? s_scale[i] : a.x_scale[t0 + i]) : 0.f;
       const float ws = o < a.O ? a.w_scale[o] : 0.f;
       float bias = 0.f;
       if (a.bias && o < a.O) bias = a.bias_f32 ? static_cast<const float*>(a.bias)[o] : to_f32<T>(static_cast<const T*>(a.bias)[o]);
@@ -464,7 +541,7 @@ __device__ __forceinline__ int4 load_peer(uint32_t addr, int rank) {
 // A warp's tokens c, c + step, ... below c1 of a tile split over S ranges of K:
 // four channels per lane, the sums of several tokens on their way at a time.
 template <typename T, int S>
-__device__ __forceinline__ void join(const LinArgs& a, uint32_t base, int c, int c1, int step, int64_t t0, int o) {
+__device__ __forceinline__ void join(const LinArgs& a, const float* x_scale, uint32_t base, int c, int c1, int step, int64_t t0, int o) {
   constexpr int U = S == 8 ? 2 : 4;
   const int lane = threadIdx.x & 31, left = a.O - o;
   float ws[4], bias[4];
@@ -482,7 +559,7 @@ __device__ __forceinline__ void join(const LinArgs& a, uint32_t base, int c, int
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int at = min(c + u * step, c1 - 1);
-      xs[u] = a.x_scale[t0 + at];
+      xs[u] = x_scale[at];
 #pragma unroll
       for (int r = 0; r < S; ++r) v[u][r] = load_peer(base + uint32_t(at * kM + lane * 4) * 4, r);
     }
@@ -513,14 +590,15 @@ __device__ __forceinline__ void join(const LinArgs& a, uint32_t base, int c, int
 }
 
 // One tile per cluster of a.split CTAs.
-template <typename T, int BN>
+template <typename T, int BN, bool ROUND>
 __global__ void __launch_bounds__(kThreads) int8_linear_split_kernel(const __grid_constant__ LinArgs a) {
-  using L = Tile<BN>;
-  static_assert(BN * kM * 4 <= L::STAGES * L::STAGE, "the sums take the stages' place");
+  using L = Tile<BN, ROUND>;
+  static_assert(BN * kM * 4 <= L::STAGES * L::STAGE && (!ROUND || BN == kRoundTokens), "the sums take the stages' place");
   extern __shared__ __align__(16) uint8_t raw[];
-  __shared__ uint64_t full[L::STAGES], empty[L::STAGES], acc_full, drained;
+  __shared__ uint64_t full[L::STAGES], empty[L::STAGES], acc_full, drained, x_ready;
   __shared__ uint32_t slot;
   __shared__ WaitFlag wait;
+  __shared__ float s_scale[kRoundTokens], s_red[8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = (tc::smem_u32(raw) + 1023u) & ~1023u;
   const uint32_t tile = blockIdx.x / a.split, rank = blockIdx.x - tile * a.split;   // rank: clusters are runs of a.split CTAs
@@ -528,20 +606,21 @@ __global__ void __launch_bounds__(kThreads) int8_linear_split_kernel(const __gri
   const int k0 = int(int64_t(a.steps) * rank / a.split), k1 = int(int64_t(a.steps) * (rank + 1) / a.split);
   auto load = [&](int st, int k) {
     const uint32_t at = base + st * L::STAGE;
-    tc::mbar_arrive_expect_tx(&full[st], uint32_t(L::A_BYTES + a.bn * kStepBytes));
+    tc::mbar_arrive_expect_tx(&full[st], uint32_t(L::A_BYTES + (ROUND ? 0 : a.bn * kStepBytes)));
     tma_load_2d(at, &a.tm_w, k * kStepBytes, int(to) * kM, &full[st]);
-    tma_load_2d(at + L::A_BYTES, &a.tm_x, k * kStepBytes, int(tt) * a.bn, &full[st]);
+    if (!ROUND) tma_load_2d(at + L::A_BYTES, &a.tm_x, k * kStepBytes, int(tt) * a.bn, &full[st]);
   };
   const int early = min(L::STAGES, k1 - k0);
   if (warp == 0 && lane == 0) {
     prefetch_map(&a.tm_w);
-    prefetch_map(&a.tm_x);
+    if (!ROUND) prefetch_map(&a.tm_x);
     for (int i = 0; i < L::STAGES; ++i) {
       tc::mbar_init(&full[i], 1);
       tc::mbar_init(&empty[i], 1);
     }
     tc::mbar_init(&acc_full, 1);
     tc::mbar_init(&drained, 1);
+    tc::mbar_init(&x_ready, 8);
     tc::fence_barrier_init();
     wait.init(a.tries);
     for (int i = 0; i < early; ++i) load(i, k0 + i);   // on their way while the others get ready
@@ -550,7 +629,7 @@ __global__ void __launch_bounds__(kThreads) int8_linear_split_kernel(const __gri
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  const uint32_t tmem = slot;
+  const uint32_t tmem = slot, x_at = base + L::STAGES * L::STAGE;
   bool ok = true;
   if (warp == 0) {
     if (lane == 0) {
@@ -574,6 +653,7 @@ __global__ void __launch_bounds__(kThreads) int8_linear_split_kernel(const __gri
     const uint32_t idesc = idesc_i8(kM, a.bn);
     int st = 0;
     uint32_t phase = 0;
+    if (ROUND) ok = wait_phase(&x_ready, 0, &wait);
 #pragma unroll 1
     for (int k = k0; k < k1; ++k) {
       ok = wait_phase(&full[st], int(phase), &wait) && ok;
@@ -583,7 +663,7 @@ __global__ void __launch_bounds__(kThreads) int8_linear_split_kernel(const __gri
       }
       tc::fence_after_sync();
       if (leader) {
-        const uint32_t al = desc_low(base + st * L::STAGE, 16), bl = desc_low(base + st * L::STAGE + L::A_BYTES, 16);
+        const uint32_t al = desc_low(base + st * L::STAGE, 16), bl = desc_low(ROUND ? x_at + (k - k0) * L::B_BYTES : base + st * L::STAGE + L::A_BYTES, 16);
 #pragma unroll
         for (int i = 0; i < 4; ++i) mma_i8(tmem, al + 2 * i, bl + 2 * i, idesc, k > k0 || i > 0);
         tc::mma_commit(&empty[st]);
@@ -603,6 +683,7 @@ __global__ void __launch_bounds__(kThreads) int8_linear_split_kernel(const __gri
   } else {
     const int quarter = warp & 3;
     const uint32_t mine = base + (quarter * 32 + lane) * 4;      // sums: [token][channel]
+    if (ROUND) round_tokens(a, x_at, k0, k1, s_scale, s_red, &x_ready);
     // the sums' products are done, so every stage has been read
     ok = wait_phase(&acc_full, 0, &wait);
     tc::fence_after_sync();
@@ -626,9 +707,10 @@ __global__ void __launch_bounds__(kThreads) int8_linear_split_kernel(const __gri
   cluster_sync();
   const int64_t t0 = int64_t(tt) * a.bn;
   const int c0 = int(a.bn * rank / a.split), c1 = int(min64(a.bn * (rank + 1) / a.split, a.T - t0)), o = int(to) * kM + lane * 4;
-  if (a.split == 2) join<T, 2>(a, base, c0 + warp, c1, kThreads / 32, t0, o);
-  else if (a.split == 4) join<T, 4>(a, base, c0 + warp, c1, kThreads / 32, t0, o);
-  else join<T, 8>(a, base, c0 + warp, c1, kThreads / 32, t0, o);
+  const float* x_scale = ROUND ? s_scale : a.x_scale + t0;
+  if (a.split == 2) join<T, 2>(a, x_scale, base, c0 + warp, c1, kThreads / 32, t0, o);
+  else if (a.split == 4) join<T, 4>(a, x_scale, base, c0 + warp, c1, kThreads / 32, t0, o);
+  else join<T, 8>(a, x_scale, base, c0 + warp, c1, kThreads / 32, t0, o);
   cluster_sync();   // no CTA leaves while another reads its sums
 }
 
@@ -669,12 +751,12 @@ int tile_tokens(int64_t T, int most) {
   return int(((T + tiles - 1) / tiles + 15) / 16 * 16);
 }
 
-template <typename T, int BN>
+template <typename T, int BN, bool ROUND = false>
 int launch(LinArgs a, const Operands& m, int split, cudaStream_t s) {
-  using L = Tile<BN>;
+  using L = Tile<BN, ROUND>;
   a.bn = tile_tokens(a.T, BN);
   int rc = byte_map(&a.tm_w, m.w, a.O, m.K, m.w_st, kM);
-  if (rc == PISA_OK) rc = byte_map(&a.tm_x, m.x, a.T, m.K, m.x_st, uint32_t(a.bn));
+  if (!ROUND && rc == PISA_OK) rc = byte_map(&a.tm_x, m.x, a.T, m.K, m.x_st, uint32_t(a.bn));
   if (rc) return rc;
   a.tiles_o = uint32_t((a.O + kM - 1) / kM);
   const int64_t tiles = int64_t(a.tiles_o) * ((a.T + a.bn - 1) / a.bn);
@@ -682,12 +764,12 @@ int launch(LinArgs a, const Operands& m, int split, cudaStream_t s) {
   a.tiles = uint32_t(tiles);
   a.split = uint32_t(split);
   if (split == 1) {
-    if ((rc = allow_smem<int8_linear_kernel<T, BN>>(L::SMEM, "8-bit product smem attribute"))) return rc;
-    int8_linear_kernel<T, BN><<<unsigned(min64(tiles, sm_count())), kThreads, L::SMEM, s>>>(a);
+    if ((rc = allow_smem<int8_linear_kernel<T, BN, ROUND>>(L::SMEM, "8-bit product smem attribute"))) return rc;
+    int8_linear_kernel<T, BN, ROUND><<<unsigned(min64(tiles, sm_count())), kThreads, L::SMEM, s>>>(a);
     PISA_CHECK_LAUNCH();
     return PISA_OK;
   }
-  if ((rc = allow_smem<int8_linear_split_kernel<T, BN>>(L::SMEM, "8-bit product smem attribute"))) return rc;
+  if ((rc = allow_smem<int8_linear_split_kernel<T, BN, ROUND>>(L::SMEM, "8-bit product smem attribute"))) return rc;
   cudaLaunchConfig_t config{};
   cudaLaunchAttribute cluster;
   cluster.id = cudaLaunchAttributeClusterDimension;
@@ -699,7 +781,7 @@ int launch(LinArgs a, const Operands& m, int split, cudaStream_t s) {
   config.stream = s;
   config.attrs = &cluster;
   config.numAttrs = 1;
-  if (cudaLaunchKernelEx(&config, int8_linear_split_kernel<T, BN>, a) != cudaSuccess) return fail_cuda(cudaGetLastError(), "8-bit product");
+  if (cudaLaunchKernelEx(&config, int8_linear_split_kernel<T, BN, ROUND>, a) != cudaSuccess) return fail_cuda(cudaGetLastError(), "8-bit product");
   PISA_CHECK_LAUNCH();
   return PISA_OK;
 }
@@ -737,7 +819,7 @@ struct Shape {
 // and 46.8; one token over 4096 x 4096 takes 11.6 us unsplit and 8.4 split by 4,
 // over 1024 x 5632 5.7 and 6.8 (split by 2); 5110 x 64 x 3392 takes 13.9 us in tiles
 // of 256 tokens and 34.1 of 32, 326 x 128 x 1088 takes 5.1 and 3.7.
-Shape choose(int64_t T, int64_t O, int64_t steps) {
+Shape choose(int64_t T, int64_t O, int64_t steps, bool pairs = true) {
   const int64_t sms = sm_count();
   const double memory = double(T + O) * double(steps * kStepBytes) / 6.5e6;
   Shape best{256, 1};
@@ -762,12 +844,23 @@ Shape choose(int64_t T, int64_t O, int64_t steps) {
     }
   }
   const int bn = (tile_tokens(T, 256) + 31) / 32 * 32;
-  consider(256, 0, (O + 2 * kM - 1) / (2 * kM) * ((T + bn - 1) / bn), (sms + 1) / 2, 0.20 + 0.0005 * bn, 1.0 + 0.011 * bn, 4.5);
+  if (pairs) consider(256, 0, (O + 2 * kM - 1) / (2 * kM) * ((T + bn - 1) / bn), (sms + 1) / 2, 0.20 + 0.0005 * bn, 1.0 + 0.011 * bn, 4.5);
   return best;
+}
+
+// Whether the product's kernel rounds floating tokens itself, and its split: few
+// elements (every CTA reads them all: a rounding of their own takes 2 us and a
+// launch), and no more steps per CTA than its shared memory holds.
+int rounds_itself(int64_t T, int64_t K, int64_t O) {
+  if (T > kRoundTokens || T * K > 16384) return 0;
+  const int64_t steps = (K + kStepBytes - 1) / kStepBytes;
+  const Shape c = choose(T, O, steps, false);
+  return (steps + c.split - 1) / c.split <= kRoundSteps ? c.split : 0;
 }
 
 template <typename T>
 int dispatch(const LinArgs& a, const Operands& m, cudaStream_t s) {
+  if (a.x) return launch<T, kRoundTokens, true>(a, m, rounds_itself(a.T, a.K, a.O), s);
   const Shape c = choose(a.T, a.O, a.steps);
   if (c.split == 0) return launch_pairs<T>(a, m, s);
   switch (c.bn) {
@@ -785,10 +878,11 @@ int dispatch(const LinArgs& a, const Operands& m, cudaStream_t s) {
 
 extern "C" {
 
-// workspace: status word, then (floating x) the tokens' scales and bytes
+// workspace: status word, then (floating x, unless the product's kernel rounds it) the tokens' scales and bytes
 int64_t pisa_int8_linear_workspace_bytes(int64_t T, int64_t K, int64_t O, int x_dtype) {
   if (T <= 0 || K <= 0 || O <= 0 || x_dtype < PISA_F32 || x_dtype > PISA_S8) return -1;
-  return 256 + (x_dtype == PISA_S8 ? 0 : (T * 4 + 255) / 256 * 256 + T * ((K + 15) / 16 * 16));
+  if (x_dtype == PISA_S8 || pisa::rounds_itself(T, K, O)) return 256;
+  return 256 + (T * 4 + 255) / 256 * 256 + T * ((K + 15) / 16 * 16);
 }
 
 int pisa_int8_linear(const void* x, int64_t x_st, int x_dtype, const float* x_scale, const int8_t* weight, int64_t weight_st,
@@ -811,14 +905,19 @@ int pisa_int8_linear(const void* x, int64_t x_st, int x_dtype, const float* x_sc
   if ((bytes && ((reinterpret_cast<uintptr_t>(x) & 15u) || x_st % 16)) || (reinterpret_cast<uintptr_t>(weight) & 15u) || weight_st % 16)
     return fail(PISA_ERR_UNSUPPORTED, "8-bit rows must start on 16 bytes");
   if ((bytes && x_st < K) || weight_st < K) return fail(PISA_ERR_UNSUPPORTED, "8-bit rows must not overlap");
-  if (workspace ? workspace_bytes < pisa_int8_linear_workspace_bytes(T, K, O, x_dtype) : !bytes)
+  const bool own = !bytes && rounds_itself(T, K, O);   // no workspace but for the status word
+  if (workspace ? workspace_bytes < pisa_int8_linear_workspace_bytes(T, K, O, x_dtype) : !bytes && !own)
     return fail(PISA_ERR_INVALID, "workspace too small");
   if (!bytes && (reinterpret_cast<uintptr_t>(workspace) & 15u)) return fail(PISA_ERR_INVALID, "workspace must start on 16 bytes");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   LinArgs a{};
   a.status = static_cast<int*>(workspace);
   Operands m{x, x_st, weight, weight_st, K};
-  if (bytes) {
+  if (bytes || own) {
+    if (own) {
+      a.x = x; a.x_st = x_st; a.x_dtype = x_dtype; a.K = int(K);
+      a.x_wide = K % 8 == 0 && rows_on16(x, T, x_st * (x_dtype == PISA_F32 ? 4 : 2));
+    }
     if (workspace) {
       cudaError_t e = cudaMemsetAsync(workspace, 0, 256, s);
       if (e != cudaSuccess) return fail_cuda(e, "status clear");

@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) row_kernel(const __grid
   for (int j = 0; j < NV; ++j) {
     float f[8];
     widen8<T>(x[j], f);
-    top = max_nan(top, largest8<T>(x[j], f));
+    top = larger(top, largest8<T>(x[j], f));
   }
   top = team_reduce<TPR, true>(top, red, set);
   const Scale8 s(top);
@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(512) long_row_kernel(const __grid_constant__ R
     float f[8];
     widen8<T>(load_piece<T, TPR, A>(xr + at, 0, threadIdx.x, int(min64(STEP, a.D - at))), f);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) top = max_nan(top, fabsf(f[e]));
+    for (int e = 0; e < 8; ++e) top = larger(top, fabsf(f[e]));
   }
   top = team_reduce<TPR, true>(top, red, set);
   const Scale8 s(top);
@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(kThreads) group_kernel(const __grid_constant__
     widen8<T>(x, f);
     float top = largest8<T>(x, f);
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(kFull, top, o));
+    for (int o = 8; o > 0; o >>= 1) top = larger(top, __shfl_xor_sync(kFull, top, o));
     const Scale8 s(top);
     store_piece_s8<T, 16, A>(qr, 0, t, width, f, top < INFINITY, s.inv);
     if (live && t == 0) a.scale[at] = s.scale;

@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm_fwd_kernel(const _
     for (int k = 0; k < 4; ++k) set_pair(h[j], k, pair_mul(pair_mul(pair_at(h[j], k), both(inv_h)), pair_at(w, k)));
     if (a.n_q) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) top = max_nan(top, fabsf(h[j][e]));
+      for (int e = 0; e < 8; ++e) top = larger(top, fabsf(h[j][e]));
     }
   }
   if (a.n_q) {

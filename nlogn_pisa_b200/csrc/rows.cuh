@@ -201,7 +201,7 @@ __device__ __forceinline__ void param_piece(const void* p, int f32, int j, int t
 }
 
 // Larger of two, NaN if either is.
-__device__ __forceinline__ float max_nan(float a, float b) {
+__device__ __forceinline__ float larger(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
@@ -216,7 +216,7 @@ __device__ __forceinline__ float team_reduce(float v, float* red, int& set) {
 #pragma unroll
   for (int o = TPR < 32 ? TPR / 2 : 16; o > 0; o >>= 1) {
     const float w = __shfl_xor_sync(kFull, v, o);
-    v = MAX ? max_nan(v, w) : v + w;
+    v = MAX ? larger(v, w) : v + w;
   }
   if constexpr (TPR > 32) {
     constexpr int W = TPR / 32;
@@ -226,7 +226,7 @@ __device__ __forceinline__ float team_reduce(float v, float* red, int& set) {
     __syncthreads();
     v = at[0];
 #pragma unroll
-    for (int i = 1; i < W; ++i) v = MAX ? max_nan(v, at[i]) : v + at[i];
+    for (int i = 1; i < W; ++i) v = MAX ? larger(v, at[i]) : v + at[i];
   }
   return v;
 }
@@ -265,20 +265,20 @@ __device__ __forceinline__ float largest8(const Raw8<T>& r, const float (&f)[8])
   if constexpr (std::is_same<T, float>::value) {
     float top = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) top = max_nan(top, fabsf(f[e]));
+    for (int e = 0; e < 8; ++e) top = larger(top, fabsf(f[e]));
     return top;
   } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
     const uint32_t w[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
     __nv_bfloat162 m = __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[0]));
 #pragma unroll
     for (int i = 1; i < 4; ++i) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[i])));
-    return max_nan(__low2float(m), __high2float(m));
+    return larger(__low2float(m), __high2float(m));
   } else {
     const uint32_t w[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
     __half2 m = __habs2(*reinterpret_cast<const __half2*>(&w[0]));
 #pragma unroll
     for (int i = 1; i < 4; ++i) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __half2*>(&w[i])));
-    return max_nan(__low2float(m), __high2float(m));
+    return larger(__low2float(m), __high2float(m));
   }
 }
 

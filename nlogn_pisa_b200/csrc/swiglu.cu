@@ -76,7 +76,7 @@ __device__ __forceinline__ float2 sigmoid2(float2 x) {
 // Maximum over the sixteen threads of a group, NaN if any is.
 __device__ __forceinline__ float group_max(float v) {
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(kFull, v, o));
+  for (int o = 8; o > 0; o >>= 1) v = larger(v, __shfl_xor_sync(kFull, v, o));
   return v;
 }
 
@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) glu_row_kernel(const __
       set_pair(o[j], k, pair_mul(pair_mul(x, sigmoid2<T>(x)), pair_at(o[j], k)));
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) top = max_nan(top, fabsf(o[j][e]));
+    for (int e = 0; e < 8; ++e) top = larger(top, fabsf(o[j][e]));
   }
   top = team_reduce<TPR, true>(top, red, set);
   const Scale8 s(top);

@@ -190,7 +190,8 @@ def int8_linear(x, weight, weight_scale, bias=None, x_scale=None, out_dtype=None
         (rows, x_stride), code = rows_of(x), _floating(x, "x")
     if not whole or _lib.status_checks():
         size = _lib.workspace_bytes("pisa_int8_linear_workspace_bytes", device, count, inner, outer, code)
-        workspace = weight.new_empty(size)
+        if size > 256 or _lib.status_checks():   # more than the status word: rows rounded on their way
+            workspace = weight.new_empty(size)
     out = weight_scale.new_empty((*shape, outer), dtype=out_dtype)
     _lib.launch(_lib.lib().pisa_int8_linear, device, rows.data_ptr(), x_stride, code, x_scale.data_ptr() if whole else None,
                 weight.data_ptr(), w_stride, weight_scale.data_ptr(), *bias_args, _lib.DTYPES[out_dtype], count, inner, outer,

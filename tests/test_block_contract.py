@@ -100,7 +100,7 @@ def test_entry_checks_run_on_the_host():
 
     for kw, word in (({"T": 0}, "nonempty"), ({"K": 1 << 17}, "32 bits"), ({"O": 0}, "nonempty"), ({"x": 8}, "16 bytes"),
                      ({"x_st": 72}, "16 bytes"), ({"w_st": 48}, "overlap"), ({"out": 9}, "support"), ({"T": 1 << 31}, "too large"),
-                     ({"workspace": 256, "size": 16}, "workspace"), ({"x_dtype": _lib.BF16}, "workspace"), ({"x_dtype": 4}, "support"),
+                     ({"workspace": 256, "size": 16}, "workspace"), ({"x_dtype": _lib.BF16, "T": 17}, "workspace"), ({"x_dtype": 4}, "support"),
                      ({"x_dtype": _lib.BF16, "workspace": 8, "size": 4096}, "16 bytes"), ({"bias": 256, "bias_dtype": _lib.F16}, "bias")):
         refused(linear(**kw), word)
 
@@ -114,5 +114,7 @@ def test_workspace_sizes_are_pure_host_functions():
     assert lib.pisa_residual_norm_bwd_workspace_bytes(12, 64, 5) == -1
     assert lib.pisa_residual_norm_bwd_workspace_bytes(0, 64, 0) == -1
     assert lib.pisa_int8_linear_workspace_bytes(4, 64, 8, _lib.S8) == 256
-    assert lib.pisa_int8_linear_workspace_bytes(4, 65, 8, _lib.BF16) == 512 + 4 * 80
+    assert lib.pisa_int8_linear_workspace_bytes(4, 65, 8, _lib.BF16) == 256       # rounded by the product's kernel
+    assert lib.pisa_int8_linear_workspace_bytes(17, 65, 8, _lib.BF16) == 512 + 17 * 80
+    assert lib.pisa_int8_linear_workspace_bytes(1, 16385, 8, _lib.BF16) == 512 + 16400
     assert lib.pisa_int8_linear_workspace_bytes(4, 0, 8, _lib.S8) == -1

@@ -94,7 +94,8 @@ def test_layouts(cuda_device):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
-@pytest.mark.parametrize("tokens,inner", [(1, 64), (50, 1000), (300, 4099)])
+@pytest.mark.parametrize("tokens,inner", [(1, 64), (50, 1000), (300, 4099), (1, 1), (1, 5000), (1, 16384), (2, 8192), (3, 5461), (5, 777),
+                                          (7, 2048), (9, 1820), (16, 1024), (16, 1023), (15, 128), (17, 512), (4, 4100)])
 def test_floating_tokens_are_rounded_in_the_call(cuda_device, dtype, tokens, inner):
     import nlogn_pisa_b200 as P
 
@@ -105,20 +106,30 @@ def test_floating_tokens_are_rounded_in_the_call(cuda_device, dtype, tokens, inn
     out = P.int8_linear(x, w, ws)
     assert out.dtype == dtype
     R.check("out", out, *R.int8_linear(values, scale, w, ws, None, dtype))
+    # the same bytes as tokens rounded before, other layouts, many tiles
+    assert torch.equal(out, P.int8_linear(values, w, ws, x_scale=scale, out_dtype=dtype))
+    wide = torch.randn(tokens, inner + 9, generator=gen, device="cuda").to(dtype)
+    wide[:, 3:inner + 3] = x
+    assert torch.equal(out, P.int8_linear(wide[:, 3:inner + 3], w, ws))
+    w, ws = P.quantize_int8(torch.randn(20003, inner, generator=gen, device="cuda"))
+    bias = torch.randn(20003, generator=gen, device="cuda")
+    out = P.int8_linear(x, w, ws, bias=bias)
+    R.check("out", out, *R.int8_linear(values, scale, w, ws, bias, dtype))
 
 
 def test_wild_rows_keep_to_themselves(cuda_device):
     import nlogn_pisa_b200 as P
 
     gen = torch.Generator(device="cuda").manual_seed(3)
-    x = torch.randn(40, 256, generator=gen, device="cuda")
     w, ws = P.quantize_int8(torch.randn(100, 256, generator=gen, device="cuda"))
-    clean = P.int8_linear(x, w, ws)
-    x[7, 3], x[9, 100] = float("nan"), float("inf")
-    wild = P.int8_linear(x, w, ws)
-    keep = torch.ones(40, dtype=torch.bool, device="cuda")
-    keep[7] = keep[9] = False
-    assert torch.equal(clean[keep], wild[keep]) and bool(wild[~keep].isnan().all())
+    for tokens in (40, 11):
+        x = torch.randn(tokens, 256, generator=gen, device="cuda")
+        clean = P.int8_linear(x, w, ws)
+        x[7, 3], x[9, 100], x[4] = float("nan"), float("inf"), 0
+        wild = P.int8_linear(x, w, ws)
+        keep = torch.ones(tokens, dtype=torch.bool, device="cuda")
+        keep[[4, 7, 9]] = False
+        assert torch.equal(clean[keep], wild[keep]) and bool(wild[[7, 9]].isnan().all()) and bool((wild[4] == 0).all())
 
 
 @pytest.mark.parametrize("out", [F32, BF16])
