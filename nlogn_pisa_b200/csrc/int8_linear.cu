@@ -13,7 +13,7 @@
 // Many tokens are bound by the tensor cores (and, back to back, by power), few by
 // HBM and the start of a launch: 16384 x 4096 x 11264 takes 437 to 449 us (3.4
 // PTOP/s, tensor pipe 86 % busy on a smaller case), 64 tokens over 4096 x 16384
-// 14.7 us (4.7 TB/s), one token over 1024 x 5632 5.4 us.  Tiles of short K are bound
+// 14.7 us (4.7 TB/s), one token in bytes over 1024 x 5632 5.4 us.  Tiles of short K are bound
 // by their stores: 30000 x 512 x 2000 49 us (65 with a test per store).
 //
 // A few floating tokens are rounded by the storing warps of every CTA, which
@@ -95,17 +95,22 @@ struct Tile {
   static constexpr int COLS = BN < 32 ? 32 : BN;             // TMEM columns of an accumulator
 };
 
-// Elements c .. c + 7 of a token, zeros past its end.
-template <typename X>
-__device__ __forceinline__ void token_piece(const LinArgs& a, const X* row, int c, float (&f)[8]) {
-  if (a.x_wide && c < a.K) {
-    Raw8<X> r;
+// Pieces p, p + step, ... (U of 8 elements) of a token, zeros past its end.
+template <typename X, bool WIDE, int U>
+__device__ __forceinline__ void token_pieces(const X* row, int p, int step, int K, Raw8<X> (&r)[U]) {
 #pragma unroll
-    for (int i = 0; i < int(sizeof(X) / 2); ++i) r.v[i] = __ldg(reinterpret_cast<const uint4*>(row + c) + i);
-    widen8<X>(r, f);
-  } else {
+  for (int u = 0; u < U; ++u) {
+    const int c = (p + u * step) * 8;
+    if constexpr (WIDE) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = c + e < a.K ? to_f32<X>(row[c + e]) : 0.f;
+      for (int i = 0; i < int(sizeof(X) / 2); ++i)
+        r[u].v[i] = c < K ? __ldg(reinterpret_cast<const uint4*>(row + c) + i) : make_uint4(0, 0, 0, 0);
+    } else {
+      X e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = c + i < K ? row[c + i] : from_f32<X>(0.f);
+      r[u] = *reinterpret_cast<const Raw8<X>*>(e);
+    }
   }
 }
 
@@ -113,19 +118,23 @@ __device__ __forceinline__ void token_piece(const LinArgs& a, const X* row, int 
 // pisa_quantize_int8 does; the bytes of steps k0 .. k1 - 1 go to 128-byte-swizzled
 // tiles of 16 rows from `at` on, scales to `scale`.  Rows past the last token are
 // not written: no one stores their products.
-template <typename X>
+template <typename X, bool WIDE>
 __device__ __forceinline__ void round_tokens(const LinArgs& a, uint32_t at, int k0, int k1, float* scale, float* red) {
+  constexpr int U = 16 / int(sizeof(X));
   int lg = 0;
   while ((1 << lg) < a.T) ++lg;
   const int id = int(threadIdx.x) - 64, each = 256 >> lg, row = id / each, t = id % each;
   const X* x = static_cast<const X*>(a.x) + int64_t(min(row, a.T - 1)) * a.x_st;
   float top = 0.f;
-#pragma unroll 4
-  for (int p = t; p < a.steps * 16; p += each) {
-    float f[8];
-    token_piece<X>(a, x, p * 8, f);
+  for (int p = t; p * 8 < a.K; p += U * each) {
+    Raw8<X> r[U];
+    token_pieces<X, WIDE, U>(x, p, each, a.K, r);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) top = larger(top, fabsf(f[e]));
+    for (int u = 0; u < U; ++u) {
+      float f[8];
+      widen8<X>(r[u], f);
+      top = larger(top, largest8<X>(r[u], f));
+    }
   }
   for (int o = min(each, 32) / 2; o > 0; o >>= 1) top = larger(top, __shfl_xor_sync(kFull, top, o));
   if (each > 32) {
@@ -136,17 +145,28 @@ __device__ __forceinline__ void round_tokens(const LinArgs& a, uint32_t at, int 
   const Scale8 s(top);
   if (t == 0) scale[row] = s.scale;
   if (row < a.T) {
-#pragma unroll 4
-    for (int p = k0 * 16 + t; p < k1 * 16; p += each) {
-      float f[8];
-      token_piece<X>(a, x, p * 8, f);
-      uint2 q = pack8_s8(f, s.inv);
-      if (!(top < INFINITY)) q = make_uint2(0, 0);
-      const uint32_t to = at + uint32_t((p >> 4) - k0) * (kRoundTokens * kStepBytes) + tc::swizzle128(row, (p & 15) >> 1) + (p & 1) * 8;
-      asm volatile("st.shared.v2.u32 [%0], {%1,%2};" :: "r"(to), "r"(q.x), "r"(q.y) : "memory");
+    for (int p = k0 * 16 + t; p < k1 * 16; p += U * each) {
+      Raw8<X> r[U];
+      token_pieces<X, WIDE, U>(x, p, each, a.K, r);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int n = p + u * each;
+        if (n >= k1 * 16) break;
+        float f[8];
+        widen8<X>(r[u], f);
+        uint2 q = pack8_s8(f, s.inv);
+        if (!(top < INFINITY)) q = make_uint2(0, 0);
+        const uint32_t to = at + uint32_t((n >> 4) - k0) * (kRoundTokens * kStepBytes) + tc::swizzle128(row, (n & 15) >> 1) + (n & 1) * 8;
+        asm volatile("st.shared.v2.u32 [%0], {%1,%2};" :: "r"(to), "r"(q.x), "r"(q.y) : "memory");
+      }
     }
   }
   tc::fence_async_smem();
+}
+template <typename X>
+__device__ __forceinline__ void round_tokens(const LinArgs& a, uint32_t at, int k0, int k1, float* scale, float* red) {
+  if (a.x_wide) round_tokens<X, true>(a, at, k0, k1, scale, red);
+  else round_tokens<X, false>(a, at, k0, k1, scale, red);
 }
 __device__ __forceinline__ void round_tokens(const LinArgs& a, uint32_t at, int k0, int k1, float* scale, float* red, uint64_t* ready) {
   if (a.x_dtype == PISA_F32) round_tokens<float>(a, at, k0, k1, scale, red);
@@ -849,8 +869,10 @@ Shape choose(int64_t T, int64_t O, int64_t steps, bool pairs = true) {
 }
 
 // Whether the product's kernel rounds floating tokens itself, and its split: few
-// elements (every CTA reads them all: a rounding of their own takes 2 us and a
-// launch), and no more steps per CTA than its shared memory holds.
+// elements, since every CTA reads them all (one token 1024 -> 5632: 9.1 us, in two
+// launches 2.1 + 5.4 and the gap between them; 16 tokens 9.5 and 7.9; the host
+// spends 14 us on one and 21 on two), and no more steps per CTA than its shared
+// memory holds.
 int rounds_itself(int64_t T, int64_t K, int64_t O) {
   if (T > kRoundTokens || T * K > 16384) return 0;
   const int64_t steps = (K + kStepBytes - 1) / kStepBytes;
