@@ -22,8 +22,8 @@
 // 45 us with it.
 //
 // Measured, bf16: 32768 rows of 4096 forward 165 us (6.5 TB/s); 16384 rows of 1024,
-// norms on both sides and a gate: forward 27 us (5.0 TB/s), backward 45 and 5 for
-// the parameters (4.5 TB/s; issue slots 53 % busy, 16 warps per SM at 118
+// norms on both sides and a gate: forward 27 us (5.0 TB/s), backward 43 and 5 for
+// the parameters (4.6 TB/s; issue slots 53 % busy, 16 warps per SM at 118
 // registers; 5 or 6 CTAs per SM spill: 58 and 86 us).  8192 rows of 4096 backward
 // 100 us (one CTA of 512 threads per SM, which waits at its barrier).  Odd widths
 // read elements one by one: 8193 rows of 1001 fp16 with a gate per token 23 and 58
@@ -379,7 +379,7 @@ norm_bwd_row_kernel(const __grid_constant__ NormArgs a) {
   constexpr int TEAMS = TPR < 128 ? 128 / TPR : 1, W = TPR / 32;
   using R = Ring<T, TPR>;
   extern __shared__ __align__(16) uint8_t ring_bytes[];
-  __shared__ float red[2][3][W > 1 ? W : 1];
+  __shared__ __align__(16) float red[2][W > 1 ? 4 * W : 4];
   int set = 0;
   const int t = threadIdx.x % TPR, D = a.D;
   const uint32_t team = blockIdx.x * TEAMS + threadIdx.x / TPR;
@@ -505,26 +505,59 @@ norm_bwd_row_kernel(const __grid_constant__ NormArgs a) {
       set_pair(s, k, sw);
     }
     float sums[3] = {sum1.x + sum1.y, sum2.x + sum2.y, sum3.x + sum3.y};
-#pragma unroll
-    for (int k = 0; k < 3; ++k) {
-      if (k && !a.post) break;
-#pragma unroll
-      for (int o = TPR < 32 ? TPR / 2 : 16; o > 0; o >>= 1) sums[k] += __shfl_xor_sync(kFull, sums[k], o);
-    }
-    if constexpr (W > 1) {
-      if ((threadIdx.x & 31) == 0) {
-#pragma unroll
-        for (int k = 0; k < 3; ++k) red[set][k][threadIdx.x >> 5] = sums[k];
-      }
-      __syncthreads();
+    if constexpr (TPR < 32 || (TPR > 128 && sizeof(T) == 2)) {
 #pragma unroll
       for (int k = 0; k < 3; ++k) {
         if (k && !a.post) break;
-        sums[k] = red[set][k][0];
 #pragma unroll
-        for (int x = 1; x < W; ++x) sums[k] += red[set][k][x];
+        for (int o = TPR < 32 ? TPR / 2 : 16; o > 0; o >>= 1) sums[k] += __shfl_xor_sync(kFull, sums[k], o);
       }
-      set ^= 1;
+      if constexpr (W > 1) {
+        if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+          for (int k = 0; k < 3; ++k) red[set][k * W + (threadIdx.x >> 5)] = sums[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+          if (k && !a.post) break;
+          sums[k] = red[set][k * W];
+#pragma unroll
+          for (int x = 1; x < W; ++x) sums[k] += red[set][k * W + x];
+        }
+        set ^= 1;
+      }
+    } else {
+      // Three sums in six shuffles: halves of the warp carry different ones on (16384 x 1024 43 us, 45 with fifteen;
+      // 16-bit teams of 256 and 512 threads have no registers left for it: 54 and 112 us against 48 and 100).
+      const bool hi = threadIdx.x & 16, mid = threadIdx.x & 8;
+      float u = hi ? sums[1] : sums[0], v1 = hi ? sums[0] : sums[1];
+      u += __shfl_xor_sync(kFull, v1, 16);                                  // lanes 0-15: sum 0, 16-31: sum 1
+      const float third = sums[2] + __shfl_xor_sync(kFull, sums[2], 16);
+      float k = mid ? third : u;
+      k += __shfl_xor_sync(kFull, mid ? u : third, 8);                      // lanes 0-7: sum 0, 16-23: sum 1, 8-15 and 24-31: sum 2
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) k += __shfl_xor_sync(kFull, k, o);
+      if constexpr (W > 1) {
+        if ((threadIdx.x & 7) == 0 && (threadIdx.x & 24) != 24) red[set][4 * (threadIdx.x >> 5) + ((threadIdx.x & 8) ? 2 : (threadIdx.x & 16) >> 4)] = k;
+        __syncthreads();
+        float4 all = *reinterpret_cast<const float4*>(&red[set][0]);
+#pragma unroll
+        for (int x = 1; x < W; ++x) {
+          const float4 more = *reinterpret_cast<const float4*>(&red[set][4 * x]);
+          all.x += more.x;
+          all.y += more.y;
+          all.z += more.z;
+        }
+        sums[0] = all.x;
+        sums[1] = all.y;
+        sums[2] = all.z;
+        set ^= 1;
+      } else {
+        sums[0] = __shfl_sync(kFull, k, 0);
+        sums[1] = __shfl_sync(kFull, k, 16);
+        sums[2] = __shfl_sync(kFull, k, 8);
+      }
     }
     const float mean = sums[0] * a.inv_d, mean_y = fmaf(-mean * inv_h.x, sums[2], sums[1]) * a.inv_d;
     const int width = live ? D : 0;
