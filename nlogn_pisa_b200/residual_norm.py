@@ -113,7 +113,7 @@ def residual_norm(x, branch, weight, post_weight=None, gate=None, residual_scale
         h = residual_scale * x + branch_scale * gate * y         (gate None: 1)
         n = h / sqrt(mean(h^2) + eps) * weight
 
-    ``branch`` None: h is x, and only the norm is computed.  ``weight``,
+    The scales are numbers.  ``branch`` None: h is x, and only the norm is computed.  ``weight``,
     ``post_weight``: [D] in fp32 or x's dtype.  ``gate``: [D] or [..., 1, D] (one
     per sequence) in fp32 or x's dtype, or a tensor like x.  n is computed from h
     before its rounding.  D at most 16384.  Gradients reach every tensor, in
@@ -155,6 +155,8 @@ def residual_norm(x, branch, weight, post_weight=None, gate=None, residual_scale
             raise ValueError("all tensors must share a device")
     require_cuda(x)
     _lib.dtype_code(x)
+    if isinstance(residual_scale, torch.Tensor) or isinstance(branch_scale, torch.Tensor):
+        raise ValueError("scales are numbers: a learned one is a gate")
     scales, eps = (float(residual_scale), float(branch_scale)), float(eps)
     if not (math.isfinite(scales[0]) and math.isfinite(scales[1])):
         raise ValueError("scales must be finite")

@@ -305,6 +305,8 @@ def test_refusals(cuda_device):
         P.residual_norm(t["x"].double(), t["x"].double(), t["weight"].double())
     with pytest.raises(ValueError, match="scales"):
         call(t, float("nan"))
+    with pytest.raises(ValueError, match="numbers"):
+        call(t, 1.0, torch.ones((), device="cuda", requires_grad=True))
     with forward_ad.dual_level():
         dual = {**t, "branch": forward_ad.make_dual(t["branch"], torch.ones_like(t["branch"]))}
         with pytest.raises(RuntimeError, match="jvp"):
