@@ -44,6 +44,20 @@ def token_positions(length, device, cu_seqlens=None, offset=0):
     return positions
 
 
+def _projections(mixer, x):
+    """q [B,T,Hq,D], k and v [B,T,H,D] of a mixer: three products, or one whose
+    outputs lie side by side where the mixer has been given a ``qkv_proj``
+    (``model.int8_projections``)."""
+    cfg = mixer.config
+    heads = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.num_key_value_heads
+    joined = getattr(mixer, "qkv_proj", None)
+    if joined is None:
+        parts = mixer.q_proj(x), mixer.k_proj(x), mixer.v_proj(x)
+    else:
+        parts = joined(x).split([n * cfg.head_dim for n in heads], -1)
+    return [t.view(*x.shape[:2], n, cfg.head_dim) for t, n in zip(parts, heads)]
+
+
 def _rotary(x, frequency, positions):
     out = torch.empty_like(x)
     pos = positions.to(device=x.device, dtype=torch.int64).contiguous()
@@ -111,9 +125,7 @@ class PyramidSparseAttention(nn.Module):
             cache = past_key_values[self.layer_idx] if len(past_key_values) > self.layer_idx else None
         cfg = self.config
         batch, length, _ = x.shape
-        q = self.q_proj(x).view(batch, length, cfg.num_attention_heads, cfg.head_dim)
-        raw_k = self.k_proj(x).view(batch, length, cfg.num_key_value_heads, cfg.head_dim)
-        v = self.v_proj(x).view(batch, length, cfg.num_key_value_heads, cfg.head_dim)
+        q, raw_k, v = _projections(self, x)
         offset = 0 if cache is None else cache["k"].shape[1]
         boundaries = cu_seqlens if cfg.rope_position_mode == "document" else None
         positions = token_positions(length, x.device, boundaries, offset)
@@ -252,9 +264,7 @@ class FullAttention(nn.Module):
             raise ValueError("packed documents start without a cache")
         cfg = self.config
         batch, length, _ = x.shape
-        q = self.q_proj(x).view(batch, length, cfg.num_attention_heads, cfg.head_dim)
-        k = self.k_proj(x).view(batch, length, cfg.num_key_value_heads, cfg.head_dim)
-        v = self.v_proj(x).view(batch, length, cfg.num_key_value_heads, cfg.head_dim)
+        q, k, v = _projections(self, x)
         prefix_k = prefix_v = None
         past = shared = 0
         if cache is not None:

@@ -162,8 +162,11 @@ class Int8SwiGLU(nn.Module):
 
 
 def int8_projections(module):
-    """A copy of a token mixer with every nn.Linear in 8 bits."""
+    """A copy of a token mixer with its projections in 8 bits: q, k and v as one product, which rounds the tokens once."""
     module = copy.deepcopy(module)
+    if all(isinstance(getattr(module, n, None), nn.Linear) for n in ("q_proj", "k_proj", "v_proj")):
+        module.qkv_proj = Int8Linear.from_linear(module.q_proj, module.k_proj, module.v_proj)
+        del module.q_proj, module.k_proj, module.v_proj
     for name, child in list(module.named_children()):
         if isinstance(child, nn.Linear):
             setattr(module, name, Int8Linear.from_linear(child))

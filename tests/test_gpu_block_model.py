@@ -79,6 +79,7 @@ def test_checkpoints_leave_the_forward_alone(cuda_device):
 def test_int8_block_is_its_operators(cuda_device, method, options):
     """Each step against its own definition from the step before; the block is the steps, bit for bit."""
     import nlogn_pisa_b200 as P
+    from nlogn_pisa_b200 import mixer
     from nlogn_pisa_b200.model import DecoderBlock, Int8DecoderBlock
 
     torch.manual_seed(2)
@@ -91,11 +92,14 @@ def test_int8_block_is_its_operators(cuda_device, method, options):
     with torch.no_grad():
         x = block.embed(tokens)
         n = P.residual_norm(x, None, block.norm1.weight, eps=cfg.rms_norm_eps)[1]
-        q = served.attn.q_proj(n)
-        w, ws = R.quantized(block.attn.q_proj.weight.detach().float())
+        qkv = served.attn.qkv_proj(n)
+        projections = [getattr(block.attn, p) for p in ("q_proj", "k_proj", "v_proj")]
+        w, ws = R.quantized(torch.cat([p.weight for p in projections]).detach().float())
         values, scale = R.quantized(n.float())
-        bias = block.attn.q_proj.bias
-        R.check("q", q, *R.int8_linear(values, scale, w, ws, None if bias is None else bias.float(), BF16))
+        bias = None if projections[0].bias is None else torch.cat([p.bias for p in projections]).float()
+        R.check("qkv", qkv, *R.int8_linear(values, scale, w, ws, bias, BF16))
+        for part, p in zip(mixer._projections(served.attn, n), projections):
+            assert torch.equal(part.flatten(2), P.Int8Linear.from_linear(p)(n))
         a, _ = served.attn(n)
         join = block.join1
         kw = dict(post_weight=join.post_norm, gate=join.gate, branch_scale=cfg.branch_scale) if options else {}
