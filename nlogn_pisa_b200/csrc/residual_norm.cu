@@ -26,8 +26,8 @@
 // the parameters (4.6 TB/s; issue slots 53 % busy, 16 warps per SM at 118
 // registers; 5 or 6 CTAs per SM spill: 58 and 86 us).  8192 rows of 4096 backward
 // 100 us (one CTA of 512 threads per SM, which waits at its barrier).  Odd widths
-// read elements one by one: 8193 rows of 1001 fp16 with a gate per token 23 and 58
-// us (3.6 and 2.3 TB/s).
+// read elements one by one: 8193 rows of 1001 fp16 with a gate per token 25 and 54
+// us (3.2 and 2.4 TB/s).
 #include "rows.cuh"
 
 namespace pisa {

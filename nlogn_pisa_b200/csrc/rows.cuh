@@ -162,10 +162,16 @@ __device__ __forceinline__ void store_piece(T* row, int j, int t, int D, const f
       if (c < D) *reinterpret_cast<uint4*>(row + c) = r.v[i];
     }
   } else {
+    T* at = row + column<T, TPR, A>(j, 0, t);
+    const Raw8<T> r = narrow8<T>(f);
+    const T* e = reinterpret_cast<const T*>(&r);
+    if (TPR > 16 && (j + 1) * 8 * TPR <= D) {   // a whole piece for all threads: no test per element
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int c = column<T, TPR, A>(j, e, t);
-      if (c < D) row[c] = from_f32<T>(f[e]);
+      for (int i = 0; i < 8; ++i) at[i * TPR] = e[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (column<T, TPR, A>(j, i, t) < D) at[i * TPR] = e[i];
     }
   }
 }
@@ -192,10 +198,16 @@ __device__ __forceinline__ void param_piece(const void* p, int f32, int j, int t
       widen8<T>(r, f);
     }
   } else {
+    if (f32) {
+      const float* at = static_cast<const float*>(p) + column<T, TPR, A>(j, 0, t);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int c = column<T, TPR, A>(j, e, t);
-      if (c < D) f[e] = f32 ? static_cast<const float*>(p)[c] : to_f32<T>(static_cast<const T*>(p)[c]);
+      for (int e = 0; e < 8; ++e)
+        if (column<T, TPR, A>(j, e, t) < D) f[e] = __ldg(at + e * TPR);
+    } else {
+      const T* at = static_cast<const T*>(p) + column<T, TPR, A>(j, 0, t);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (column<T, TPR, A>(j, e, t) < D) f[e] = to_f32<T>(__ldg(at + e * TPR));
     }
   }
 }
@@ -295,10 +307,14 @@ __device__ __forceinline__ void store_piece_s8(int8_t* row, int j, int t, int D,
       if (c4 < D) *reinterpret_cast<uint32_t*>(row + c4) = hi;
     }
   } else {
+    int8_t* at = row + column<T, TPR, A>(j, 0, t);
+    if (TPR > 16 && (j + 1) * 8 * TPR <= D) {   // a whole piece for all threads: no test per element
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int c = column<T, TPR, A>(j, e, t);
-      if (c < D) row[c] = int8_t((e < 4 ? lo >> (8 * e) : hi >> (8 * (e - 4))) & 255u);
+      for (int e = 0; e < 8; ++e) at[e * TPR] = int8_t((e < 4 ? lo >> (8 * e) : hi >> (8 * (e - 4))) & 255u);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (column<T, TPR, A>(j, e, t) < D) at[e * TPR] = int8_t((e < 4 ? lo >> (8 * e) : hi >> (8 * (e - 4))) & 255u);
     }
   }
 }
@@ -316,13 +332,17 @@ __device__ __forceinline__ uint2 load_piece_s8(const int8_t* row, int t, int D) 
       if (c4 < D) asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(r.y) : "l"(row + c4));
     }
   } else {
+    const uint8_t* at = reinterpret_cast<const uint8_t*>(row) + column<T, TPR, A>(0, 0, t);
+    uint32_t b[8];
+    if (8 * TPR <= D) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int c = column<T, TPR, A>(0, e, t);
-      const uint32_t b = c < D ? uint8_t(row[c]) : 0;
-      if (e < 4) r.x |= b << (8 * e);
-      else r.y |= b << (8 * (e - 4));
+      for (int e = 0; e < 8; ++e) b[e] = __ldg(at + e * TPR);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) b[e] = column<T, TPR, A>(0, e, t) < D ? __ldg(at + e * TPR) : 0;
     }
+    r.x = b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24;
+    r.y = b[4] | b[5] << 8 | b[6] << 16 | b[7] << 24;
   }
   return r;
 }

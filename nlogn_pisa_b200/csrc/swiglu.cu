@@ -14,7 +14,8 @@
 // Close behind is instruction issue: with the group's index by 64-bit division,
 // single operations and a quotient per thread the two passes took 75 and 71 us
 // for 16384 x 2816 in bf16, now 58 and 59 (6.3 TB/s); 8191 x 11264 in fp16 takes
-// 112 and 113.  Teams with one group and few bytes in flight: 73 us, with two 68.
+// 112 and 113, and 16384 x 2817, whose rows are read element by element, 145 a
+// pass.  Teams with one group and few bytes in flight: 73 us, with two 68.
 // Arithmetic is fp32; exponentials and reciprocals are the fast forms for
 // 16-bit tensors (errors of a few 2^-22 before a rounding of 2^-9 or 2^-12) and
 // the exact ones for fp32.
