@@ -118,7 +118,11 @@ class SwigluFfnFunction(torch.autograd.Function):
     @staticmethod
     @torch.amp.custom_fwd(device_type="cuda")
     def forward(ctx, x, w_gate, w_up, w_down, b_gate, b_up, b_down):
-        out, kept = _forward(F.linear(x, w_gate, b_gate), F.linear(x, w_up, b_up), True)
+        gate, up = F.linear(x, w_gate, b_gate), F.linear(x, w_up, b_up)
+        if gate.shape != up.shape:
+            raise ValueError("the products of w_gate and w_up must share a shape")
+        out, kept = _forward(gate, up, True)
+        del gate, up
         ctx.dtype = x.dtype
         ctx.save_for_backward(*checkpoint_int8(x), kept, w_gate, w_up, w_down)
         return F.linear(out, w_down, b_down)
@@ -154,6 +158,13 @@ def swiglu_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None):
         raise ValueError("x, weights and biases must share a floating dtype")
     if x.dim() < 1 or 0 in x.shape:
         raise ValueError("nonempty tensors are required")
+    # the kernels read up's rows by gate's shape
+    if w_gate.dim() != 2 or w_gate.shape[1] != x.shape[-1] or w_up.shape != w_gate.shape:
+        raise ValueError("w_gate and w_up must share a shape [O, K], K that of x")
+    if w_down.dim() != 2 or w_down.shape[1] != w_gate.shape[0]:
+        raise ValueError("w_down must have shape [N, O], O that of w_gate")
+    if 0 in w_gate.shape:
+        raise ValueError("nonempty weights are required")
     require_cuda(*tensors)
     _lib.dtype_code(x)
     if carries_tangent(*tensors):

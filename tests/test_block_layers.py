@@ -1,0 +1,23 @@
+"""Layers around the decoder block's operators: what they refuse, keep and call (no GPU)."""
+
+import pytest
+import torch
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_ffn_refuses_weights_that_do_not_fit(grad):
+    """The gated product reads up's rows by gate's shape: a smaller up would be read past its end."""
+    import nlogn_pisa_b200 as P
+
+    def zeros(*shape):
+        return torch.zeros(*shape, requires_grad=grad)
+
+    x = zeros(3, 64)
+    for shapes, word in ((((16, 64), (8, 64), (64, 16)), "w_gate and w_up must share"),
+                         (((8, 64), (16, 64), (64, 8)), "w_gate and w_up must share"),
+                         (((8, 32), (8, 32), (64, 8)), "w_gate and w_up must share"),
+                         (((64,), (64,), (64, 8)), "w_gate and w_up must share"),
+                         (((8, 64), (8, 64), (64, 16)), "w_down must"), (((8, 64), (8, 64), (8,)), "w_down must"),
+                         (((0, 64), (0, 64), (64, 0)), "nonempty weights")):
+        with pytest.raises(ValueError, match=word):
+            P.swiglu_ffn(x, *(zeros(*s) for s in shapes))
