@@ -206,7 +206,7 @@ class Int8Linear(nn.Module):
 
     ``from_linear`` rounds the weight of an nn.Linear on the GPU.  The forward
     takes what ``int8_linear`` takes: floating tokens, or int8 ones and their
-    scales.
+    scales.  Like it, it refuses tokens that require a gradient.
     """
 
     def __init__(self, in_features, out_features, bias=True):
@@ -244,5 +244,5 @@ class Int8Linear(nn.Module):
         bias = self.bias
         if bias is not None and bias.dtype != torch.float32:
             bias = bias.float()
-        return int8_linear(x.detach(), self.weight[:, :self.in_features], self.weight_scale, bias=bias, x_scale=x_scale,
+        return int8_linear(x, self.weight[:, :self.in_features], self.weight_scale, bias=bias, x_scale=x_scale,
                            out_dtype=out_dtype)

@@ -2,6 +2,7 @@
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 pytestmark = pytest.mark.gpu
 
@@ -21,3 +22,47 @@ def test_ffn_refuses_weights_that_do_not_fit(cuda_device, autocast):
         y = P.swiglu_ffn(x, gate, gate, down)
     # 16 products of silu(64) * 64 = 4096: exact in every type
     assert bool((y == 65536).all())
+
+
+def config(**kw):
+    from nlogn_pisa_b200.model import BlockConfig
+
+    return BlockConfig(**{**dict(vocab_size=300, hidden_size=128, intermediate_size=352, num_attention_heads=4,
+                                 num_key_value_heads=2, head_dim=64, topk=8, block_size=16, branching=2, init_std=0.1), **kw})
+
+
+def test_int8_layers_refuse_tokens_with_gradients(cuda_device):
+    """In grad mode a gradient would be lost; without it, and under no_grad, the layers run."""
+    import nlogn_pisa_b200 as P
+    from nlogn_pisa_b200 import mixer
+    from nlogn_pisa_b200.model import Int8SwiGLU, SwiGLU, int8_projections
+
+    torch.manual_seed(1)
+    layers = [P.Int8Linear.from_linear(torch.nn.Linear(128, 48, device="cuda", dtype=BF16)),
+              Int8SwiGLU(SwiGLU(128, 352, True).to("cuda", BF16))]
+    for kind, method in ((mixer.FullAttention, "full"), (mixer.PyramidSparseAttention, "pisa2")):
+        attention = int8_projections(kind(config(attention_method=method)).to("cuda", BF16))
+        assert not any(p.requires_grad for p in attention.parameters())
+        layers.append(lambda x, attention=attention: attention(x)[0])
+    x = torch.randn(2, 40, 128, device="cuda", dtype=BF16)
+    for layer in layers:
+        leaf = x.clone().requires_grad_(True)
+        for tokens in (leaf, leaf * 1):
+            with pytest.raises(ValueError, match="inference"):
+                layer(tokens)
+        with torch.no_grad():
+            quiet = layer(leaf)
+        out = layer(x)
+        assert torch.equal(out, quiet) and not out.requires_grad
+    with forward_ad.dual_level():
+        with pytest.raises(ValueError, match="inference"):
+            layers[0](forward_ad.make_dual(x, torch.ones_like(x)))
+
+
+def test_int8_mixers_leave_the_original_trainable(cuda_device):
+    from nlogn_pisa_b200 import mixer
+    from nlogn_pisa_b200.model import int8_projections
+
+    attention = mixer.FullAttention(config(attention_method="full")).to("cuda", BF16)
+    int8_projections(attention)
+    assert all(p.requires_grad for p in attention.parameters()) and hasattr(attention, "q_proj")
