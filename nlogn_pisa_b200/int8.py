@@ -221,7 +221,9 @@ class Int8Linear(nn.Module):
         """Scales stay fp32 when the layer is cast to another type."""
         scale = self.weight_scale
         super()._apply(fn, recurse)
-        self.weight_scale = scale.to(self.weight.device)
+        if self.weight_scale.dtype != scale.dtype:
+            device = self.weight_scale.device
+            self.weight_scale = torch.empty_like(scale, device=device) if scale.is_meta else scale.to(device)
         return self
 
     @classmethod

@@ -34,3 +34,33 @@ def test_int8_layer_passes_its_tokens_on(monkeypatch):
     layer(x * 1)
     layer(x.detach())
     assert [t.requires_grad for t in seen] == [True, False]
+
+
+def test_int8_layer_is_built_without_memory_first():
+    """Under the meta device, then given memory, then loaded."""
+    from nlogn_pisa_b200 import int8
+
+    source = int8.Int8Linear(40, 6)
+    for t in source.state_dict().values():
+        t.copy_(torch.randint(-100, 100, t.shape))
+    for cast in (False, True):
+        with torch.device("meta"):
+            model = torch.nn.Sequential(int8.Int8Linear(40, 6))
+        model = (model.half() if cast else model).to_empty(device="cpu")
+        assert model[0].weight_scale.dtype == torch.float32 and not model[0].weight_scale.is_meta
+        model[0].load_state_dict(source.state_dict())
+        for name, t in source.state_dict().items():
+            assert torch.equal(model[0].state_dict()[name], t), name
+
+
+def test_int8_layer_moves_with_its_model():
+    from nlogn_pisa_b200 import int8
+
+    layer = int8.Int8Linear(40, 6)
+    layer.weight_scale.copy_(torch.rand(6))
+    scale = layer.weight_scale.clone()
+    for move in (lambda m: m.half(), lambda m: m.bfloat16(), lambda m: m.double(), lambda m: m.to(torch.float16), lambda m: m.float()):
+        move(layer)
+        assert layer.weight_scale.dtype == torch.float32 and torch.equal(layer.weight_scale, scale)
+        assert layer.weight.dtype == torch.int8
+    assert layer.to("meta").weight_scale.is_meta
