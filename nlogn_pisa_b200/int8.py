@@ -215,15 +215,16 @@ class Int8Linear(nn.Module):
         # rows of whole 16 bytes, as the products read them
         self.register_buffer("weight", torch.zeros(out_features, -(-in_features // 16) * 16, dtype=torch.int8))
         self.register_buffer("weight_scale", torch.zeros(out_features, dtype=torch.float32))
-        self.register_buffer("bias", torch.zeros(out_features) if bias else None)
+        self.register_buffer("bias", torch.zeros(out_features, dtype=torch.float32) if bias else None)
 
     def _apply(self, fn, recurse=True):
-        """Scales stay fp32 when the layer is cast to another type."""
-        scale = self.weight_scale
+        """Scales and bias stay fp32 when the layer is cast to another type."""
+        kept = {name: t for name, t in self._buffers.items() if t is not None and t.dtype == torch.float32}
         super()._apply(fn, recurse)
-        if self.weight_scale.dtype != scale.dtype:
-            device = self.weight_scale.device
-            self.weight_scale = torch.empty_like(scale, device=device) if scale.is_meta else scale.to(device)
+        for name, t in kept.items():
+            device = self._buffers[name].device
+            if self._buffers[name].dtype != torch.float32:
+                self._buffers[name] = torch.empty_like(t, device=device) if t.is_meta else t.to(device)
         return self
 
     @classmethod

@@ -64,3 +64,22 @@ def test_int8_layer_moves_with_its_model():
         assert layer.weight_scale.dtype == torch.float32 and torch.equal(layer.weight_scale, scale)
         assert layer.weight.dtype == torch.int8
     assert layer.to("meta").weight_scale.is_meta
+
+
+@pytest.mark.parametrize("cast", ["half", "bfloat16", "double"])
+def test_int8_layer_keeps_its_bias_in_fp32(cast):
+    """Values that 16 bits do not hold survive a cast, on their own and within a model."""
+    from nlogn_pisa_b200 import int8
+
+    layer = int8.Int8Linear(40, 6)
+    bias = torch.tensor([1 + 2.0 ** -20, -3e-9, 70000.5, 0.1, 1e30, 0.0])
+    layer.bias.copy_(bias)
+    getattr(torch.nn.Sequential(layer), cast)()
+    assert layer.bias.dtype == torch.float32 and torch.equal(layer.bias, bias)
+    assert getattr(int8.Int8Linear(40, 6, bias=False), cast)().bias is None
+    default = torch.get_default_dtype()
+    torch.set_default_dtype(torch.bfloat16)
+    try:
+        assert int8.Int8Linear(40, 6).bias.dtype == torch.float32
+    finally:
+        torch.set_default_dtype(default)

@@ -66,3 +66,17 @@ def test_int8_mixers_leave_the_original_trainable(cuda_device):
     attention = mixer.FullAttention(config(attention_method="full")).to("cuda", BF16)
     int8_projections(attention)
     assert all(p.requires_grad for p in attention.parameters()) and hasattr(attention, "q_proj")
+
+
+@pytest.mark.parametrize("cast", [F16, BF16])
+def test_int8_layer_cast_with_its_model(cuda_device, cast):
+    """A cast changes the tokens' type, not what the layer holds: the same product of the same tokens."""
+    import nlogn_pisa_b200 as P
+
+    torch.manual_seed(2)
+    linear = torch.nn.Linear(100, 30, device="cuda")
+    layer, other = P.Int8Linear.from_linear(linear), P.Int8Linear.from_linear(linear).to(cast)
+    x = torch.randn(5, 100, device="cuda").to(cast)
+    assert torch.equal(other.bias, linear.bias)
+    for out_dtype in (None, F32):
+        assert torch.equal(layer(x, out_dtype=out_dtype), other(x, out_dtype=out_dtype))
