@@ -83,3 +83,53 @@ def test_int8_layer_keeps_its_bias_in_fp32(cast):
         assert int8.Int8Linear(40, 6).bias.dtype == torch.float32
     finally:
         torch.set_default_dtype(default)
+
+
+class Adapted(torch.nn.Linear):
+    """A linear layer with a low-rank part beside its weight."""
+
+    def __init__(self, inner, outer):
+        super().__init__(inner, outer)
+        self.low, self.high = torch.nn.Linear(inner, 4, bias=False), torch.nn.Linear(4, outer, bias=False)
+
+    def forward(self, x):
+        return super().forward(x) + self.high(self.low(x))
+
+
+def watchers(module, seen):
+    """Ways to watch calls of a module, each with its undoing."""
+    own = module.forward
+    yield module.register_forward_hook(lambda *a: seen.append(1)).remove
+    yield module.register_forward_pre_hook(lambda *a: seen.append(1)).remove
+    module.forward = lambda *a, **kw: (seen.append(1), own(*a, **kw))[1]
+    yield lambda: module.__dict__.pop("forward")
+    yield torch.nn.modules.module.register_module_forward_hook(lambda m, *a: m is module and seen.append(1) or None).remove
+
+
+@pytest.mark.parametrize("name", ["gate", "up", "down"])
+def test_checkpointed_ffn_calls_its_layers(monkeypatch, name):
+    """Hooks and layers with a forward of their own are not passed by; plain layers run as one operator."""
+    from torch.nn import functional as F
+
+    from nlogn_pisa_b200 import model
+
+    whole = []
+    monkeypatch.setattr(model, "swiglu", lambda g, u, checkpoint_bits: F.silu(g) * u)
+    monkeypatch.setattr(model, "swiglu_ffn", lambda x, wg, wu, wd, bg, bu, bd: whole.append(1) or F.linear(
+        F.silu(F.linear(x, wg, bg)) * F.linear(x, wu, bu), wd, bd))
+    ffn, x = model.SwiGLU(8, 12, True, 8), torch.randn(3, 8)
+    plain = ffn(x)
+    assert whole == [1]
+    seen = []
+    for count, undo in enumerate(watchers(getattr(ffn, name), seen), 1):
+        assert torch.equal(ffn(x), plain) and len(seen) == count and len(whole) == count
+        undo()
+        assert torch.equal(ffn(x), plain) and len(seen) == count
+    layer = getattr(ffn, name)
+    setattr(ffn, name, Adapted(layer.in_features, layer.out_features))
+    whole.clear()
+    assert torch.equal(ffn(x), ffn.down(F.silu(ffn.gate(x)) * ffn.up(x))) and not whole
+    # a weight computed from others is still the layer's weight
+    setattr(ffn, name, torch.nn.utils.parametrizations.weight_norm(layer))
+    ffn(x).sum().backward()
+    assert whole and all(p.grad is not None for p in getattr(ffn, name).parameters())

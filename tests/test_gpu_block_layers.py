@@ -80,3 +80,40 @@ def test_int8_layer_cast_with_its_model(cuda_device, cast):
     assert torch.equal(other.bias, linear.bias)
     for out_dtype in (None, F32):
         assert torch.equal(layer(x, out_dtype=out_dtype), other(x, out_dtype=out_dtype))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_checkpointed_ffn_around_other_layers(cuda_device, dtype):
+    """With a hook or an adapter the layers are called: the same forward, and the gradients of the gated product's kept
+    inputs, for the adapter too."""
+    import nlogn_pisa_b200 as P
+    from nlogn_pisa_b200.model import SwiGLU
+
+    torch.manual_seed(3)
+    ffn = SwiGLU(96, 200, True, 8).to("cuda", dtype)
+    x = torch.randn(2, 9, 96, device="cuda", dtype=dtype, requires_grad=True)
+    plain, calls = ffn(x), []
+    hooks = [getattr(ffn, n).register_full_backward_hook(lambda *a: calls.append(1)) for n in ("gate", "up", "down")]
+    out = ffn(x)
+    assert torch.equal(out, plain)
+    out.sum().backward()
+    assert len(calls) == 3
+    for hook in hooks:
+        hook.remove()
+
+    class Adapter(torch.nn.Module):
+        def __init__(self, layer):
+            super().__init__()
+            self.layer, self.low = layer, torch.nn.Linear(layer.in_features, layer.out_features, False).to("cuda", dtype)
+
+        def forward(self, x):
+            return self.layer(x) + self.low(x)
+
+    for name in ("gate", "up", "down"):
+        setattr(ffn, name, Adapter(getattr(ffn, name)))
+    d = torch.randn_like(plain)
+    leaves = [x, *ffn.parameters()]
+    got, want = ffn(x), ffn.down(P.swiglu(ffn.gate(x), ffn.up(x), checkpoint_bits=8))
+    assert torch.equal(got, want)
+    for g, w in zip(*(torch.autograd.grad(y, leaves, d) for y in (got, want))):
+        assert torch.equal(g, w) and bool(g.any())
