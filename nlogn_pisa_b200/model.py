@@ -24,7 +24,7 @@ import torch
 from torch import nn
 import torch.nn.functional as F
 
-from .int8 import Int8Linear
+from .int8 import Int8Linear, quantize_int8
 from .mixer import FullAttention, PyramidSparseAttention
 from .residual_norm import residual_norm
 from .swiglu import swiglu, swiglu_ffn
@@ -105,26 +105,38 @@ class SwiGLU(nn.Module):
 
 
 class BranchJoin(nn.Module):
-    """What lies between a branch and the next norm: the branch's own norm and gate, and the scales."""
+    """What lies between a branch and the next norm: the branch's own norm and gate, and the scales.
+
+    The next norm is part of the operator where it is a plain RMSNorm; one of another kind, or with hooks, is called on
+    the residual stream."""
 
     def __init__(self, cfg: BlockConfig):
         super().__init__()
         self.post_norm = nn.Parameter(torch.ones(cfg.hidden_size)) if cfg.post_norm else None
         self.gate = nn.Parameter(torch.ones(cfg.hidden_size)) if cfg.branch_gate else None
         self.scales = cfg.residual_scale, cfg.branch_scale
+        self.eps = cfg.rms_norm_eps
 
     def forward(self, x, branch, norm, quantize=False):
         """residual_norm of the residual stream and the branch, with the next norm's weight."""
+        fused = bare(norm, RMSNorm)
         weights = [w if w is None or w.dtype in (torch.float32, x.dtype) else w.float()
-                   for w in (norm.weight, self.post_norm, self.gate)]
+                   for w in (norm.weight if fused else x.new_ones(x.shape[-1]), self.post_norm, self.gate)]
         if quantize:
             weights = [None if w is None else w.detach() for w in weights]
-        return residual_norm(x, branch.to(x.dtype), weights[0], post_weight=weights[1], gate=weights[2],
-                             residual_scale=self.scales[0], branch_scale=self.scales[1], eps=norm.eps, quantize=quantize)
+        results = residual_norm(x, branch.to(x.dtype), weights[0], post_weight=weights[1], gate=weights[2],
+                                residual_scale=self.scales[0], branch_scale=self.scales[1],
+                                eps=norm.eps if isinstance(norm, RMSNorm) else self.eps, quantize=quantize and fused)
+        if fused:
+            return results
+        h = results[0]
+        return (h, *quantize_int8(norm(h))) if quantize else (h, norm(h))
 
     @staticmethod
     def first(x, norm):
         """The norm before the first branch."""
+        if not bare(norm, RMSNorm):
+            return norm(x)
         weight = norm.weight if norm.weight.dtype in (torch.float32, x.dtype) else norm.weight.float()
         return residual_norm(x, None, weight, eps=norm.eps)[1]
 

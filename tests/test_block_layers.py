@@ -133,3 +133,54 @@ def test_checkpointed_ffn_calls_its_layers(monkeypatch, name):
     setattr(ffn, name, torch.nn.utils.parametrizations.weight_norm(layer))
     ffn(x).sum().backward()
     assert whole and all(p.grad is not None for p in getattr(ffn, name).parameters())
+
+
+@pytest.mark.parametrize("options", [{"fused_norms": True}, {"post_norm": True, "branch_gate": True, "branch_scale": 0.5}])
+@pytest.mark.parametrize("name", ["norm1", "norm2", "norm_out"])
+def test_fused_block_calls_its_norms(monkeypatch, name, options):
+    """A norm with hooks, or of another kind, is called; a plain RMSNorm is part of the operator."""
+    from nlogn_pisa_b200 import model
+
+    def rms(t, eps):
+        return t * torch.rsqrt(t.square().mean(-1, keepdim=True) + eps)
+
+    whole = []
+
+    def joined(x, branch, weight, post_weight=None, gate=None, residual_scale=1.0, branch_scale=1.0, eps=1e-6, quantize=False):
+        whole.append(weight)
+        if branch is not None:
+            branch = branch if post_weight is None else rms(branch, eps) * post_weight
+            x = residual_scale * x + branch_scale * (branch if gate is None else gate * branch)
+        return x, rms(x, eps) * weight
+
+    class Mix(torch.nn.Module):
+        def forward(self, x):
+            return x.cumsum(1), None
+
+    monkeypatch.setattr(model, "residual_norm", joined)
+    block = model.DecoderBlock(model.BlockConfig(vocab_size=30, hidden_size=16, intermediate_size=24, num_attention_heads=2,
+                                                 num_key_value_heads=2, head_dim=8, attention_method="full", **options))
+    block.attn = Mix()
+    tokens = torch.randint(0, 30, (2, 5))
+    plain, norm = block(tokens), getattr(block, name)
+    assert [w is n.weight for w, n in zip(whole, (block.norm1, block.norm2, block.norm_out))] == [True] * 3
+    seen = []
+    for count, undo in enumerate(watchers(norm, seen), 1):
+        # the same function in another order: some units of 2^-24 on values of order 1
+        assert torch.allclose(block(tokens), plain, rtol=0, atol=1e-4) and len(seen) == count
+        undo()
+        assert torch.equal(block(tokens), plain) and len(seen) == count
+    other = torch.nn.LayerNorm(16)
+    torch.nn.init.normal_(other.weight)
+    inputs = []
+    other.register_forward_hook(lambda m, args, out: inputs.append((args[0], out)))
+    setattr(block, name, other)
+    out = block(tokens)
+    (h, n), = inputs
+    assert not torch.equal(out, plain)
+    if name == "norm_out":
+        assert torch.equal(out, n)
+    if name == "norm1":
+        assert torch.equal(h, block.embed(tokens))
+    out.sum().backward()
+    assert other.weight.grad is not None and all(p.grad is not None for p in block.parameters())

@@ -117,3 +117,34 @@ def test_checkpointed_ffn_around_other_layers(cuda_device, dtype):
     assert torch.equal(got, want)
     for g, w in zip(*(torch.autograd.grad(y, leaves, d) for y in (got, want))):
         assert torch.equal(g, w) and bool(g.any())
+
+
+@pytest.mark.parametrize("options", [{"fused_norms": True}, {"post_norm": True, "branch_gate": True, "branch_scale": 0.5}])
+def test_fused_block_with_watched_norms(cuda_device, options):
+    """Hooks on the norms see their calls and change the outputs by a rounding of the residual stream at most."""
+    from nlogn_pisa_b200.model import DecoderBlock, Int8DecoderBlock
+
+    torch.manual_seed(4)
+    cfg = config(attention_method="full", **options)
+    block = DecoderBlock(cfg).cuda()
+    tokens = torch.randint(0, 300, (2, 30), device="cuda")
+    with torch.no_grad():
+        plain = block(tokens)
+    served = Int8DecoderBlock(block, cfg)
+    served_plain, _ = served(tokens)
+    seen = []
+    hooks = [n.register_forward_hook(lambda m, args, out: seen.append((m, out)))
+             for b in (block, served) for n in (b.norm1, b.norm2, b.norm_out)]
+    out = block(tokens)
+    # the bound of test_fused_norms_are_the_blocks: some hundred units of 2^-24 for each of about twelve operators
+    assert len(seen) in (3, 6) and float((out - plain).norm() / plain.norm()) < 7e-4
+    grads = torch.autograd.grad(out.square().sum(), list(block.parameters()))
+    assert all(bool(g.isfinite().all()) and bool(g.any()) for g in grads)
+    seen.clear()
+    hidden, _ = served(tokens)
+    # here an 8-bit step may move: one of 127 to a value, in few of many
+    assert len(seen) in (3, 6) and float((hidden - served_plain).norm() / served_plain.norm()) < 1 / 127
+    for hook in hooks:
+        hook.remove()
+    with torch.no_grad():
+        assert torch.equal(block(tokens), plain) and torch.equal(served(tokens)[0], served_plain)
