@@ -14,7 +14,7 @@ from torch import nn
 
 from . import _lib
 from .dense import carries_tangent, differentiated
-from .validation import require_cuda
+from .validation import bare, require_cuda
 
 GROUP = 128             # elements that share a scale of a kept activation
 MAX_INNER = 1 << 17     # sums of fewer products of bytes fit 32 bits
@@ -230,7 +230,11 @@ class Int8Linear(nn.Module):
     @classmethod
     @torch.no_grad()
     def from_linear(cls, *linears):
-        """The layer of one nn.Linear, or of several with the same input, their outputs side by side."""
+        """The layer of one nn.Linear, or of several with the same input, their outputs side by side.
+
+        It takes over weights and biases alone: layers with hooks or a forward of their own (adapters) are refused."""
+        if not all(bare(m, nn.Linear) for m in linears):
+            raise ValueError("only linear layers without hooks or a forward of their own have an 8-bit form")
         first = linears[0]
         bias = first.bias is not None
         if any(m.in_features != first.in_features or (m.bias is not None) != bias for m in linears):

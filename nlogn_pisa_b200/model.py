@@ -28,6 +28,7 @@ from .int8 import Int8Linear, quantize_int8
 from .mixer import FullAttention, PyramidSparseAttention
 from .residual_norm import residual_norm
 from .swiglu import swiglu, swiglu_ffn
+from .validation import bare
 
 
 @dataclass
@@ -62,12 +63,9 @@ class BlockConfig:
     checkpoint_bits: int | None = None  # 8: the FFN's activations in 8 bits until the backward
 
 
-def bare(module, kind):
-    """Whether calling ``module`` is ``kind``'s forward and nothing else (no hooks, no forward of its own), so that an
-    operator on its parameters may stand in for the call."""
-    hooks = module._forward_hooks, module._forward_pre_hooks, module._backward_hooks, module._backward_pre_hooks
-    return (type(module).forward is kind.forward and "forward" not in module.__dict__ and not any(hooks)
-            and not nn.modules.module._has_any_global_hook())
+def replaceable(module, kind):
+    """Whether an operator on the module's parameters may stand in for calling it: a bare ``kind``, and no hooks on all modules."""
+    return bare(module, kind) and not nn.modules.module._has_any_global_hook()
 
 
 class RMSNorm(nn.Module):
@@ -97,7 +95,7 @@ class SwiGLU(nn.Module):
 
     def forward(self, x):
         if self.checkpoint_bits == 8:
-            if not all(bare(m, nn.Linear) for m in (self.gate, self.up, self.down)):
+            if not all(replaceable(m, nn.Linear) for m in (self.gate, self.up, self.down)):
                 return self.down(swiglu(self.gate(x), self.up(x), checkpoint_bits=8))
             return swiglu_ffn(x, self.gate.weight, self.up.weight, self.down.weight, self.gate.bias, self.up.bias,
                               self.down.bias)
@@ -119,7 +117,7 @@ class BranchJoin(nn.Module):
 
     def forward(self, x, branch, norm, quantize=False):
         """residual_norm of the residual stream and the branch, with the next norm's weight."""
-        fused = bare(norm, RMSNorm)
+        fused = replaceable(norm, RMSNorm)
         weights = [w if w is None or w.dtype in (torch.float32, x.dtype) else w.float()
                    for w in (norm.weight if fused else x.new_ones(x.shape[-1]), self.post_norm, self.gate)]
         if quantize:
@@ -135,7 +133,7 @@ class BranchJoin(nn.Module):
     @staticmethod
     def first(x, norm):
         """The norm before the first branch."""
-        if not bare(norm, RMSNorm):
+        if not replaceable(norm, RMSNorm):
             return norm(x)
         weight = norm.weight if norm.weight.dtype in (torch.float32, x.dtype) else norm.weight.float()
         return residual_norm(x, None, weight, eps=norm.eps)[1]
@@ -178,6 +176,8 @@ class Int8SwiGLU(nn.Module):
 
     def __init__(self, ffn: SwiGLU):
         super().__init__()
+        if not bare(ffn, SwiGLU):
+            raise ValueError("only a SwiGLU without hooks or a forward of its own has an 8-bit form")
         self.gate_up = Int8Linear.from_linear(ffn.gate, ffn.up)
         self.down = Int8Linear.from_linear(ffn.down)
 

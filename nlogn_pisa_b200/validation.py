@@ -91,3 +91,9 @@ def require_cuda(*tensors):
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise ValueError("nlogn_pisa_b200 runs on CUDA tensors only; there is no CPU path")
+
+
+def bare(module, kind):
+    """Whether calling ``module`` runs ``kind``'s forward and nothing else: no hooks, no forward of its own."""
+    hooks = module._forward_hooks, module._forward_pre_hooks, module._backward_hooks, module._backward_pre_hooks
+    return type(module).forward is kind.forward and "forward" not in module.__dict__ and not any(hooks)

@@ -1,5 +1,7 @@
 """Layers around the decoder block's operators: what they refuse, keep and call (no GPU)."""
 
+import itertools
+
 import pytest
 import torch
 
@@ -184,3 +186,39 @@ def test_fused_block_calls_its_norms(monkeypatch, name, options):
         assert torch.equal(h, block.embed(tokens))
     out.sum().backward()
     assert other.weight.grad is not None and all(p.grad is not None for p in block.parameters())
+
+
+def test_int8_forms_refuse_what_they_would_drop(monkeypatch):
+    """An 8-bit layer takes over weights: adapters, hooks and other forwards would be lost without a word."""
+    from nlogn_pisa_b200 import int8, model
+
+    def rounded(w):
+        scale = w.abs().amax(-1) / 127
+        return (w / scale[:, None]).round().to(torch.int8), scale
+
+    class Other(model.SwiGLU):
+        def forward(self, x):
+            return self.down(self.gate(x).relu() * self.up(x))
+
+    monkeypatch.setattr(int8, "quantize_int8", rounded)
+    plain = torch.nn.Linear(32, 8)
+    assert int8.Int8Linear.from_linear(plain, torch.nn.Linear(32, 4)).out_features == 12
+    for undo in itertools.islice(watchers(plain, []), 3):
+        with pytest.raises(ValueError, match="hooks or a forward"):
+            int8.Int8Linear.from_linear(torch.nn.Linear(32, 4), plain)
+        undo()
+    # a weight computed from others is taken as it is
+    int8.Int8Linear.from_linear(torch.nn.utils.parametrizations.weight_norm(plain))
+    with pytest.raises(ValueError, match="hooks or a forward"):
+        int8.Int8Linear.from_linear(Adapted(32, 8))
+    model.Int8SwiGLU(model.SwiGLU(32, 48, True))
+    with pytest.raises(ValueError, match="SwiGLU"):
+        model.Int8SwiGLU(Other(32, 48, True))
+    ffn = model.SwiGLU(32, 48, True)
+    ffn.down = Adapted(48, 32)
+    with pytest.raises(ValueError, match="hooks or a forward"):
+        model.Int8SwiGLU(ffn)
+    mixer = torch.nn.Module()
+    mixer.o_proj = Adapted(32, 8)
+    with pytest.raises(ValueError, match="hooks or a forward"):
+        model.int8_projections(mixer)
