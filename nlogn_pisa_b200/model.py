@@ -187,10 +187,11 @@ class Int8SwiGLU(nn.Module):
 
 
 def int8_projections(module):
-    """A copy of a token mixer for inference with its projections in 8 bits: q, k and v as one product, which rounds the
-    tokens once.  Its parameters take no gradients, and tokens that require one are refused."""
+    """A copy of a token mixer for inference with its projections in 8 bits: q, k and v of this package's mixers as one
+    product, which rounds the tokens once.  Its parameters take no gradients, and tokens that require one are refused."""
     module = copy.deepcopy(module).requires_grad_(False)
-    if all(isinstance(getattr(module, n, None), nn.Linear) for n in ("q_proj", "k_proj", "v_proj")):
+    own = type(module).forward in (FullAttention.forward, PyramidSparseAttention.forward) and "forward" not in module.__dict__
+    if own and all(isinstance(getattr(module, n, None), nn.Linear) for n in ("q_proj", "k_proj", "v_proj")):
         module.qkv_proj = Int8Linear.from_linear(module.q_proj, module.k_proj, module.v_proj)
         del module.q_proj, module.k_proj, module.v_proj
     for name, child in list(module.named_children()):

@@ -222,3 +222,35 @@ def test_int8_forms_refuse_what_they_would_drop(monkeypatch):
     mixer.o_proj = Adapted(32, 8)
     with pytest.raises(ValueError, match="hooks or a forward"):
         model.int8_projections(mixer)
+
+
+def test_int8_copy_of_a_mixer_with_its_own_forward(monkeypatch):
+    """Only this package's mixers know the joined projection; others find theirs where they left them."""
+    from nlogn_pisa_b200 import int8, mixer, model
+
+    class Mix(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.q_proj, self.k_proj, self.v_proj, self.o_proj = (torch.nn.Linear(16, 16) for _ in range(4))
+
+        def forward(self, x):
+            return self.o_proj(self.q_proj(x) * self.k_proj(x) + self.v_proj(x)), None
+
+    class Masked(mixer.FullAttention):
+        def forward(self, x):
+            return self.o_proj(self.q_proj(x) * self.k_proj(x) + self.v_proj(x)), None
+
+    def rounded(w):
+        scale = w.abs().amax(-1) / 127
+        return (w / scale[:, None]).round().to(torch.int8), scale
+
+    monkeypatch.setattr(int8, "quantize_int8", rounded)
+    monkeypatch.setattr(int8, "int8_linear", lambda x, w, s, bias=None, **kw: x @ (w * s[:, None]).T + (0 if bias is None else bias))
+    cfg = model.BlockConfig(hidden_size=16, num_attention_heads=2, num_key_value_heads=2, head_dim=8, attention_method="full", bias=True)
+    x = torch.randn(2, 3, 16)
+    for own in (Mix(), Masked(cfg)):
+        copy = model.int8_projections(own)
+        assert all(isinstance(getattr(copy, n), int8.Int8Linear) for n in ("q_proj", "k_proj", "v_proj", "o_proj"))
+        assert torch.allclose(copy(x)[0], own(x)[0], atol=0.2)
+    joined = model.int8_projections(mixer.FullAttention(cfg))
+    assert joined.qkv_proj.out_features == 48 and not hasattr(joined, "q_proj")
