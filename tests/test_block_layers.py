@@ -254,3 +254,37 @@ def test_int8_copy_of_a_mixer_with_its_own_forward(monkeypatch):
         assert torch.allclose(copy(x)[0], own(x)[0], atol=0.2)
     joined = model.int8_projections(mixer.FullAttention(cfg))
     assert joined.qkv_proj.out_features == 48 and not hasattr(joined, "q_proj")
+
+
+def without_kernels(monkeypatch):
+    """Rounding and the products of 8-bit layers on the host."""
+    from nlogn_pisa_b200 import int8
+
+    def rounded(w):
+        scale = w.abs().amax(-1) / 127
+        return (w / scale[:, None]).round().to(torch.int8), scale
+
+    monkeypatch.setattr(int8, "quantize_int8", rounded)
+    monkeypatch.setattr(int8, "int8_linear", lambda x, w, s, bias=None, **kw: x @ (w * s[:, None]).T + (0 if bias is None else bias))
+
+
+@pytest.mark.parametrize("options", [{}, {"post_norm": True, "branch_gate": True, "branch_scale": 0.5}])
+def test_int8_block_is_a_copy(monkeypatch, options):
+    """Neither block follows the other's training or casts."""
+    from nlogn_pisa_b200 import model
+
+    without_kernels(monkeypatch)
+    cfg = model.BlockConfig(vocab_size=30, hidden_size=16, intermediate_size=24, num_attention_heads=2, num_key_value_heads=2,
+                            head_dim=8, attention_method="full", **options)
+    block = model.DecoderBlock(cfg)
+    served = model.Int8DecoderBlock(block, cfg)
+    before = {n: t.clone() for n, t in served.state_dict().items()}
+    with torch.no_grad():
+        for p in block.parameters():
+            p.add_(1)
+    assert all(torch.equal(t, before[n]) for n, t in served.state_dict().items())
+    assert not any(p.requires_grad for p in served.parameters()) and all(p.requires_grad for p in block.parameters())
+    served.half()
+    assert all(p.dtype == torch.float32 for p in block.parameters())
+    held = {t.untyped_storage().data_ptr() for t in block.state_dict().values()}
+    assert not held & {t.untyped_storage().data_ptr() for t in model.Int8DecoderBlock(block, cfg).state_dict().values()}
