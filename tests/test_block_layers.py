@@ -288,3 +288,31 @@ def test_int8_block_is_a_copy(monkeypatch, options):
     assert all(p.dtype == torch.float32 for p in block.parameters())
     held = {t.untyped_storage().data_ptr() for t in block.state_dict().values()}
     assert not held & {t.untyped_storage().data_ptr() for t in model.Int8DecoderBlock(block, cfg).state_dict().values()}
+
+
+@pytest.mark.parametrize("given", [{"post_norm": True}, {"branch_gate": True}, {"branch_scale": 0.5}, {"residual_scale": 2.0}, {}])
+def test_int8_block_joins_as_its_block_does(monkeypatch, given):
+    """A configuration that differs from the block's adds no norm, gate or scale to the served form, and takes none away."""
+    from dataclasses import replace
+
+    from nlogn_pisa_b200 import model
+
+    without_kernels(monkeypatch)
+    calls = []
+
+    def joined(x, branch, weight, **kw):
+        calls.append(kw)
+        return (x, x) if not kw.get("quantize") else (x, x, None)
+
+    monkeypatch.setattr(model, "residual_norm", joined)
+    base = model.BlockConfig(vocab_size=30, hidden_size=16, intermediate_size=24, num_attention_heads=2, num_key_value_heads=2,
+                             head_dim=8, attention_method="full")
+    for own, cfg in ((base, replace(base, **given)), (replace(base, **given), base)):
+        block = model.DecoderBlock(own)
+        served = model.Int8DecoderBlock(block, cfg)
+        x, a = torch.zeros(2, 3, 16), torch.zeros(2, 3, 16)
+        for join in (served.join1, served.join2):
+            calls.clear()
+            join(x, a, served.norm2)
+            assert (calls[0]["post_weight"] is not None, calls[0]["gate"] is not None) == (own.post_norm, own.branch_gate)
+            assert (calls[0]["residual_scale"], calls[0]["branch_scale"]) == (own.residual_scale, own.branch_scale)
