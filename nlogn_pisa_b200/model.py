@@ -18,7 +18,7 @@ projection in 8 bits.
 from __future__ import annotations
 
 import copy
-from dataclasses import dataclass, replace
+from dataclasses import dataclass
 
 import torch
 from torch import nn
@@ -206,15 +206,14 @@ class Int8DecoderBlock(nn.Module):
     Norms and residual sums run in residual_norm, which gives the FFN its tokens
     in 8 bits; the mixer's projections round theirs.  Returns the hidden states
     and the mixer's cache.  The block's parameters are copied: training or casting
-    it afterwards leaves this one as it is, and the other way round.  Post norms, gates and scales are the block's own,
-    whatever ``cfg`` says of them.
+    it afterwards leaves this one as it is, and the other way round.  Post norms, gates and scales are the block's own:
+    ``cfg`` is not read.
     """
 
-    def __init__(self, block: DecoderBlock, cfg: BlockConfig):
+    def __init__(self, block: DecoderBlock, cfg: BlockConfig | None = None):
         super().__init__()
         # a block without joins adds its branches as they are
-        plain = replace(cfg, post_norm=False, branch_gate=False, residual_scale=1.0, branch_scale=1.0)
-        join1, join2 = (j or BranchJoin(plain) for j in (block.join1, block.join2))
+        join1, join2 = (j or BranchJoin(BlockConfig()) for j in (block.join1, block.join2))
         self.embed, self.norm1, self.norm2, self.norm_out, self.join1, self.join2 = (
             copy.deepcopy(m).requires_grad_(False) for m in (block.embed, block.norm1, block.norm2, block.norm_out, join1, join2))
         self.attn = int8_projections(block.attn)

@@ -307,7 +307,7 @@ def test_int8_block_joins_as_its_block_does(monkeypatch, given):
     monkeypatch.setattr(model, "residual_norm", joined)
     base = model.BlockConfig(vocab_size=30, hidden_size=16, intermediate_size=24, num_attention_heads=2, num_key_value_heads=2,
                              head_dim=8, attention_method="full")
-    for own, cfg in ((base, replace(base, **given)), (replace(base, **given), base)):
+    for own, cfg in ((base, replace(base, **given)), (replace(base, **given), base), (replace(base, **given), None)):
         block = model.DecoderBlock(own)
         served = model.Int8DecoderBlock(block, cfg)
         x, a = torch.zeros(2, 3, 16), torch.zeros(2, 3, 16)
