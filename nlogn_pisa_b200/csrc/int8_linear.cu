@@ -869,10 +869,14 @@ Shape choose(int64_t T, int64_t O, int64_t steps, bool pairs = true) {
 }
 
 // Whether the product's kernel rounds floating tokens itself, and its split: few
-// elements, since every CTA reads them all (one token 1024 -> 5632: 9.1 us, in two
-// launches 2.1 + 5.4 and the gap between them; 16 tokens 9.5 and 7.9; the host
-// spends 14 us on one and 21 on two), and no more steps per CTA than its shared
-// memory holds.
+// elements, since every CTA reads them all, and no more steps per CTA than its
+// shared memory holds.  Replayed in a graph, weights from HBM and tokens as the
+// step before left them in L2, one launch takes less than rounding and product in
+// two: 1024 -> 5632 6.5 us against 7.5 for one token, 7.3 and 7.7 for 16, 4096 ->
+// 4096 9.6 and 10.7, 1024 -> 50257 14.0 and 15.4; of 33 sizes only 4 tokens of 4096 ->
+// 16384 lose (17.4 and 17.1).  The host spends 14 us on one launch and 21 on two.
+// Tokens that come from HBM too cost each CTA a wait of their own: 1024 -> 5632 9.7
+// us for one and 10.2 for 16, where the two kernels alone take 2.1 + 5.9.
 int rounds_itself(int64_t T, int64_t K, int64_t O) {
   if (T > kRoundTokens || T * K > 16384) return 0;
   const int64_t steps = (K + kStepBytes - 1) / kStepBytes;

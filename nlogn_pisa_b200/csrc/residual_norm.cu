@@ -23,11 +23,13 @@
 //
 // Measured, bf16: 32768 rows of 4096 forward 165 us (6.5 TB/s); 16384 rows of 1024,
 // norms on both sides and a gate: forward 27 us (5.0 TB/s), backward 43 and 5 for
-// the parameters (4.6 TB/s; issue slots 53 % busy, 16 warps per SM at 118
-// registers; 5 or 6 CTAs per SM spill: 58 and 86 us).  8192 rows of 4096 backward
-// 100 us (one CTA of 512 threads per SM, which waits at its barrier).  Odd widths
-// read elements one by one: 8193 rows of 1001 fp16 with a gate per token 25 and 54
-// us (3.2 and 2.4 TB/s).
+// the parameters (4.6 TB/s; issue slots 54 % busy, 16 warps per SM at 126
+// registers; 5 or 6 CTAs per SM spill: 58 and 86 us); the second norm alone (no
+// gate, no post weight) 19 and 37 us.  8192 rows of 4096 backward 100 us, the second
+// norm alone 76 (one CTA of 512 threads per SM, which waits at its barrier).  Odd
+// widths read elements one by one: 8193 rows of 1001 fp16 with a gate per token 25
+// and 54 us (3.2 and 2.4 TB/s).  Their backward in fp32 spills 104 to 152 bytes per
+// thread, that of aligned fp32 rows over 1024 elements 24, of 16-bit odd ones 8.
 #include "rows.cuh"
 
 namespace pisa {
@@ -171,7 +173,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) norm_fwd_kernel(const _
 // The backward for wider rows in two passes: the two means of every row, and
 // then columns, of which a thread keeps 8 over many rows without a barrier.  It
 // reads the operands twice; one pass with the parameters' sums in shared memory
-// took 275 us for 4096 rows of 8192 (bf16), these two take less than half.
+// took 275 us for 4096 rows of 8192 (bf16), these two take 64 and 82.
 // Means of a row: of dn w v, and of s p z (as in norm_bwd_row_kernel).
 constexpr int kWideThreads = 256, kSlab = 1024;   // columns of a CTA of the second pass
 

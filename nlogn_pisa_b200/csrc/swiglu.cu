@@ -14,11 +14,16 @@
 // Close behind is instruction issue: with the group's index by 64-bit division,
 // single operations and a quotient per thread the two passes took 75 and 71 us
 // for 16384 x 2816 in bf16, now 58 and 59 (6.3 TB/s); 8191 x 11264 in fp16 takes
-// 112 and 113, and 16384 x 2817, whose rows are read element by element, 145 a
-// pass.  Teams with one group and few bytes in flight: 73 us, with two 68.
-// Arithmetic is fp32; exponentials and reciprocals are the fast forms for
-// 16-bit tensors (errors of a few 2^-22 before a rounding of 2^-9 or 2^-12) and
-// the exact ones for fp32.
+// 112 and 113, and 16384 x 2817, whose rows are read element by element, 106 and
+// 148.  Teams with one group and few bytes in flight: 73 us, with two 68.  Without
+// kept bytes 16384 x 2816 takes 38 and 70 us in bf16, 86 and 140 in fp32; with them
+// 118 and 122 in fp32; as 8-bit rows 48 (bf16) and 79 (fp32).  fp32 rows of more than
+// 16384 spill 56 to 80 bytes per thread (4096 x 32768: 242 us, 5.0 TB/s).
+// Arithmetic is fp32; exponentials and reciprocals are the exact ones for fp32 and
+// the fast forms for 16-bit tensors.  There s(x) is off by about 2^-24 (8 + |x|) of
+// itself (the exponent's product is rounded), 5e-6 at x = -80, before a rounding of
+// 2^-9 or 2^-12; below x = -87.3, where s(x) is under the smallest normal number, it
+// is 0.
 #include "rows.cuh"
 
 namespace pisa {
