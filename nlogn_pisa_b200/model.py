@@ -63,9 +63,13 @@ class BlockConfig:
     checkpoint_bits: int | None = None  # 8: the FFN's activations in 8 bits until the backward
 
 
+# hooks that torch runs around every module's call
+_global_hooks = getattr(nn.modules.module, "_has_any_global_hook", None) or (lambda: False)
+
+
 def replaceable(module, kind):
     """Whether an operator on the module's parameters may stand in for calling it: a bare ``kind``, and no hooks on all modules."""
-    return bare(module, kind) and not nn.modules.module._has_any_global_hook()
+    return bare(module, kind) and not _global_hooks()
 
 
 class RMSNorm(nn.Module):

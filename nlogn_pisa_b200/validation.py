@@ -95,5 +95,6 @@ def require_cuda(*tensors):
 
 def bare(module, kind):
     """Whether calling ``module`` runs ``kind``'s forward and nothing else: no hooks, no forward of its own."""
-    hooks = module._forward_hooks, module._forward_pre_hooks, module._backward_hooks, module._backward_pre_hooks
-    return type(module).forward is kind.forward and "forward" not in module.__dict__ and not any(hooks)
+    if getattr(type(module), "forward", None) is not kind.forward or "forward" in module.__dict__:
+        return False
+    return not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks)

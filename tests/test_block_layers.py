@@ -87,6 +87,18 @@ def test_int8_layer_keeps_its_bias_in_fp32(cast):
         torch.set_default_dtype(default)
 
 
+def without_kernels(monkeypatch):
+    """Rounding and the products of 8-bit layers on the host."""
+    from nlogn_pisa_b200 import int8
+
+    def rounded(w):
+        scale = w.abs().amax(-1) / 127
+        return (w / scale[:, None]).round().to(torch.int8), scale
+
+    monkeypatch.setattr(int8, "quantize_int8", rounded)
+    monkeypatch.setattr(int8, "int8_linear", lambda x, w, s, bias=None, **kw: x @ (w * s[:, None]).T + (0 if bias is None else bias))
+
+
 class Adapted(torch.nn.Linear):
     """A linear layer with a low-rank part beside its weight."""
 
@@ -192,15 +204,11 @@ def test_int8_forms_refuse_what_they_would_drop(monkeypatch):
     """An 8-bit layer takes over weights: adapters, hooks and other forwards would be lost without a word."""
     from nlogn_pisa_b200 import int8, model
 
-    def rounded(w):
-        scale = w.abs().amax(-1) / 127
-        return (w / scale[:, None]).round().to(torch.int8), scale
-
     class Other(model.SwiGLU):
         def forward(self, x):
             return self.down(self.gate(x).relu() * self.up(x))
 
-    monkeypatch.setattr(int8, "quantize_int8", rounded)
+    without_kernels(monkeypatch)
     plain = torch.nn.Linear(32, 8)
     assert int8.Int8Linear.from_linear(plain, torch.nn.Linear(32, 4)).out_features == 12
     for undo in itertools.islice(watchers(plain, []), 3):
@@ -240,12 +248,7 @@ def test_int8_copy_of_a_mixer_with_its_own_forward(monkeypatch):
         def forward(self, x):
             return self.o_proj(self.q_proj(x) * self.k_proj(x) + self.v_proj(x)), None
 
-    def rounded(w):
-        scale = w.abs().amax(-1) / 127
-        return (w / scale[:, None]).round().to(torch.int8), scale
-
-    monkeypatch.setattr(int8, "quantize_int8", rounded)
-    monkeypatch.setattr(int8, "int8_linear", lambda x, w, s, bias=None, **kw: x @ (w * s[:, None]).T + (0 if bias is None else bias))
+    without_kernels(monkeypatch)
     cfg = model.BlockConfig(hidden_size=16, num_attention_heads=2, num_key_value_heads=2, head_dim=8, attention_method="full", bias=True)
     x = torch.randn(2, 3, 16)
     for own in (Mix(), Masked(cfg)):
@@ -254,18 +257,6 @@ def test_int8_copy_of_a_mixer_with_its_own_forward(monkeypatch):
         assert torch.allclose(copy(x)[0], own(x)[0], atol=0.2)
     joined = model.int8_projections(mixer.FullAttention(cfg))
     assert joined.qkv_proj.out_features == 48 and not hasattr(joined, "q_proj")
-
-
-def without_kernels(monkeypatch):
-    """Rounding and the products of 8-bit layers on the host."""
-    from nlogn_pisa_b200 import int8
-
-    def rounded(w):
-        scale = w.abs().amax(-1) / 127
-        return (w / scale[:, None]).round().to(torch.int8), scale
-
-    monkeypatch.setattr(int8, "quantize_int8", rounded)
-    monkeypatch.setattr(int8, "int8_linear", lambda x, w, s, bias=None, **kw: x @ (w * s[:, None]).T + (0 if bias is None else bias))
 
 
 @pytest.mark.parametrize("options", [{}, {"post_norm": True, "branch_gate": True, "branch_scale": 0.5}])
